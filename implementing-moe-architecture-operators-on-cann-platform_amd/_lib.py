@@ -16,8 +16,10 @@ STATUS_NAMES = {
     0: "MOE_OK", 1: "MOE_ERR_NULL", 2: "MOE_ERR_RANK", 3: "MOE_ERR_SHAPE", 4: "MOE_ERR_ARG",
     5: "MOE_ERR_WORKSPACE", 6: "MOE_ERR_UNSUPPORTED", 7: "MOE_ERR_HIP",
 }
+DT_FLOAT32 = 0
 DT_FLOAT16 = 1
 DT_INT32 = 3
+DT_BFLOAT16 = 27
 
 
 class MoeError(RuntimeError):
@@ -50,6 +52,7 @@ class CombinePlan(C.Structure):
 
 _I64 = C.c_int64
 _I32 = C.c_int32
+_F32 = C.c_float
 _P = C.c_void_p
 _I64P = C.POINTER(C.c_int64)
 
@@ -75,6 +78,16 @@ SIGNATURES = {
     "moe_combine_infer_dtype": (_I32, [C.POINTER(_I32)]),
     "moe_combine_plan_for": (_I32, [_I64, _I64, _I64, C.POINTER(CombinePlan)]),
     "moe_combine": (_I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "moe_routing_group_topk": (_I32, [_P, _I64, _I32, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32,
+                                      _F32, _P]),
+    "moe_routing_group_topk_grad": (_I32, [_P, _I32, _P, _I64, _I32, _P, _P, _I64, _I64, _I64, _I32, _I32, _F32, _P]),
+    "moe_combine_grad": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "moe_linear_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64, _I32]),
+    "moe_linear": (_I32, [_P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64, _I64, _I32, _I32, _I32,
+                          _P]),
+    "moe_linear_grad_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64, _I32]),
+    "moe_linear_grad": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64, _I64,
+                               _I32, _I32, _P]),
     "moe_trace_enable": (_I32, [_I32]),
     "moe_trace_collect": (_I32, []),
     "moe_trace_get": (_I32, [_I32, C.POINTER(C.c_char_p), _I64P, C.POINTER(C.c_double)]),

@@ -1,0 +1,94 @@
+// moe_combine_grad.hip -- MoeCombineGrad for gfx950: the gradients of y[t, :] = sum_k weights[t, k] expert_out[t, k, :].
+//
+//   grad_expert_out[t, k, :] = weights[t, k] * grad_y[t, :]
+//   grad_weights[t, k]       = sum_h grad_y[t, h] * expert_out[t, k, h]
+//
+// The forward is the reference's op_kernel/moe_combine.cpp:80-111; it has no gradient there.
+// Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 4 experts at
+// a time, loads their rows, adds to their dot products and writes their gradient rows. A wave has a token to itself, or
+// four waves share it; the dot products are added over the lanes and then over the waves in a fixed order.
+#include "moe_device.h"
+#include "moe_launch.h"
+
+namespace moe {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBatch = 4;  // experts in flight per thread
+
+template <int WAVES>  // waves of one token: 1 or 4
+__global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* __restrict__ grad_y,
+                                                                const uint16_t* __restrict__ expert_out,
+                                                                const uint16_t* __restrict__ weights,
+                                                                uint16_t* __restrict__ grad_eo,
+                                                                uint16_t* __restrict__ grad_w, int64_t T, int H, int K) {
+    __shared__ float part[4][kBatch];
+    const int wave = static_cast<int>(threadIdx.x) / kWave, lane = lane_id();
+    const int64_t t = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : static_cast<int64_t>(blockIdx.x);
+    if (t >= T) return;  // with four waves a token the whole workgroup
+    const uint16_t* dy = grad_y + t * H;
+    const int first = (WAVES == 1 ? lane : static_cast<int>(threadIdx.x)) * 8;
+    for (int k0 = 0; k0 < K; k0 += kBatch) {
+        float dot[kBatch] = {0.f, 0.f, 0.f, 0.f}, w[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) w[u] = k0 + u < K ? f16_bits_to_f32(weights[t * K + k0 + u]) : 0.0f;
+        for (int c = first; c < H; c += WAVES * kWave * 8) {
+            const f16x8 d = load_f16x8(dy + c);
+            f16x8 o[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+                if (k0 + u < K) o[u] = load_f16x8(expert_out + (t * K + k0 + u) * H + c);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (k0 + u < K) {
+                    f16x8 v;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float g = static_cast<float>(d[j]);
+                        dot[u] += g * static_cast<float>(o[u][j]);
+                        v[j] = static_cast<f16>(w[u] * g);
+                    }
+                    *reinterpret_cast<f16x8*>(grad_eo + (t * K + k0 + u) * H + c) = v;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int d = kWave / 2; d > 0; d >>= 1) dot[u] += __shfl_xor(dot[u], d, kWave);
+        if (WAVES == 1) {
+            if (lane < kBatch && k0 + lane < K) {
+                const float v = lane == 0 ? dot[0] : lane == 1 ? dot[1] : lane == 2 ? dot[2] : dot[3];
+                grad_w[t * K + k0 + lane] = f32_to_f16_bits(v);
+            }
+        } else {
+            if (lane == 0) {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) part[wave][u] = dot[u];
+            }
+            __syncthreads();
+            const int u = static_cast<int>(threadIdx.x);
+            if (u < kBatch && k0 + u < K)
+                grad_w[t * K + k0 + u] = f32_to_f16_bits(part[0][u] + part[1][u] + part[2][u] + part[3][u]);
+            __syncthreads();
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, const uint16_t* weights,
+                               uint16_t* grad_eo, uint16_t* grad_w, int64_t T, int H, int K, hipStream_t stream) {
+    TraceScope trace("moe_combine_grad", stream);
+    // a wave a token once that gives every SIMD two waves
+    if (T >= 2048)
+        combine_grad_kernel<1><<<static_cast<unsigned>((T + 3) / 4), kThreads, 0, stream>>>(
+            grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+    else
+        combine_grad_kernel<4><<<static_cast<unsigned>(T), kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo,
+                                                                                   grad_w, T, H, K);
+    return hipGetLastError();
+}
+
+}  // namespace moe

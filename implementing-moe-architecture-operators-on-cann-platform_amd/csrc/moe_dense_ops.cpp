@@ -1,0 +1,368 @@
+// moe_dense_ops.cpp -- host side of the operators around the routed experts (include/moe_ops.h): routing from logits,
+// the dense product with its epilogue, and the gradients of both and of the combine.
+//
+// As moe_ops.cpp: nothing here allocates device memory, and every check runs before the first launch.
+
+#include <hip/hip_runtime.h>
+
+#include "moe_gemm.h"
+#include "moe_host.h"
+#include "moe_launch.h"
+#include "moe_ops.h"
+
+using namespace moe::host;
+
+namespace {
+
+bool is_half(int32_t t) { return t == MOE_DT_FLOAT16 || t == MOE_DT_BFLOAT16; }
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// ------------------------------------------------------------------------------------------------
+// routing from logits
+// ------------------------------------------------------------------------------------------------
+
+moe_status check_group_routing(const char* op, int64_t T, int64_t E, int64_t K, int64_t ld, int32_t logits_type,
+                               int32_t weights_type, bool grad) {
+    if (T < 0 || E <= 0) return fail(MOE_ERR_ARG, "%s: sizes must be T >= 0, E > 0 (T=%lld E=%lld)", op, (long long)T,
+                                     (long long)E);
+    if (K < 1 || K > E) return fail(MOE_ERR_ARG, "%s: topK=%lld must be in [1, numExperts=%lld]", op, (long long)K,
+                                    (long long)E);
+    if (E > kMaxExperts)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: numExperts=%lld exceeds %lld", op, (long long)E, (long long)kMaxExperts);
+    if (T >= int64_t{1} << 27) return fail(MOE_ERR_UNSUPPORTED, "%s: T=%lld too large", op, (long long)T);
+    if (ld < E || ld > kInt32Max)
+        return fail(MOE_ERR_ARG, "%s: logits rows %lld elements apart hold %lld", op, (long long)ld, (long long)E);
+    if (logits_type != MOE_DT_FLOAT32 && !is_half(logits_type))
+        return fail(MOE_ERR_ARG, "%s: logits type %d (float32, float16 or bfloat16 expected)", op, logits_type);
+    if (weights_type != MOE_DT_FLOAT32 && weights_type != MOE_DT_FLOAT16 && !(grad && weights_type == MOE_DT_BFLOAT16))
+        return fail(MOE_ERR_ARG, "%s: weights type %d (float32 or float16%s expected)", op, weights_type,
+                    grad ? " or bfloat16" : "");
+    return ok();
+}
+
+moe_status check_scoring(const char* op, int32_t scoring, float scale) {
+    if (scoring != MOE_SCORE_SOFTMAX && scoring != MOE_SCORE_SIGMOID)
+        return fail(MOE_ERR_ARG, "%s: scoring %d", op, scoring);
+    if (!(scale - scale == 0.0f)) return fail(MOE_ERR_ARG, "%s: scale must be finite", op);
+    return ok();
+}
+
+// ------------------------------------------------------------------------------------------------
+// dense products
+// ------------------------------------------------------------------------------------------------
+
+constexpr int kMaxActivation = MOE_ACT_SWIGLU;
+constexpr int64_t kMaxTiles = int64_t{1} << 23;  // workgroups of a launch, far below HIP's 2^32 threads
+
+moe_status check_linear(const char* op, int64_t T, int64_t N, int64_t H, int32_t act, int32_t dtype) {
+    if (T < 0 || N <= 0 || H <= 0)
+        return fail(MOE_ERR_ARG, "%s: sizes must be T >= 0, N > 0, H > 0 (T=%lld N=%lld H=%lld)", op, (long long)T,
+                    (long long)N, (long long)H);
+    if (act < 0 || act > kMaxActivation) return fail(MOE_ERR_ARG, "%s: activation %d", op, act);
+    if (!is_half(dtype)) return fail(MOE_ERR_ARG, "%s: type %d (float16 or bfloat16 expected)", op, dtype);
+    if (N > kMaxDim || H > kMaxDim)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: N=%lld, H=%lld exceed %lld", op, (long long)N, (long long)H,
+                    (long long)kMaxDim);
+    // 128 x 128 tiles (64 columns of a SwiGLU) of the forward and of both gradients
+    if (T > kInt32Max || ((T + 127) / 128) * ((N > H ? N : H) / 64 + 1) >= kMaxTiles ||
+        (N / 64 + 1) * (H / 128 + 1) >= kMaxTiles)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: T=%lld N=%lld H=%lld too large", op, (long long)T, (long long)N,
+                    (long long)H);
+    return ok();
+}
+
+moe_status check_pitch(const char* op, const char* what, int64_t rows, int64_t width, int64_t ld) {
+    if (rows > 1 && ld < width)
+        return fail(MOE_ERR_ARG, "%s: %s rows overlap (%lld elements apart, %lld long)", op, what, (long long)ld,
+                    (long long)width);
+    if (ld > int64_t{1} << 40 || ld < 0) return fail(MOE_ERR_ARG, "%s: %s stride %lld", op, what, (long long)ld);
+    return ok();
+}
+
+// How one product runs
+struct ProductPlan {
+    int bm;
+    int splits;
+    int64_t split_k;
+    size_t partial_bytes;
+};
+
+// The product is split over k while its tiles leave workgroup slots of the GPU empty (two a CU), with at least four
+// stages a piece.
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k) {
+    ProductPlan p{};
+    p.bm = p_by_k || m > 32 ? 128 : 32;
+    const int64_t tiles = (m + p.bm - 1) / p.bm * ((n + (swiglu ? 63 : 127)) / (swiglu ? 64 : 128));
+    const int64_t stages = (k + 63) / 64;
+    int64_t splits = tiles > 0 ? 512 / tiles : 1;
+    if (splits > stages / 4) splits = stages / 4;
+    if (splits < 1) splits = 1;
+    const int64_t per = (stages + splits - 1) / splits;
+    p.split_k = per > 0 ? per * 64 : 64;
+    p.splits = per > 0 ? static_cast<int>((stages + per - 1) / per) : 1;
+    p.partial_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * m * moe::part_ld(static_cast<int>(n), swiglu) * 4 : 0;
+    return p;
+}
+
+// Whether an operand allows 16-byte copies: granules on 16 bytes in every row, tile offsets within 32 bits
+bool direct_operand(const void* p, int64_t ld) {
+    return aligned16(p) && ld % 8 == 0 && ld <= int64_t{1} << 22;
+}
+
+// p_padded: P's rows are zero from k up to the next multiple of 8
+hipError_t run_product(moe::GemmArgs g, const ProductPlan& plan, void* partial, bool p_by_k, bool q_by_k, bool bf16,
+                       hipStream_t stream, bool p_padded = false) {
+    const bool swiglu = g.act == moe::kActSwiglu;
+    const bool direct = direct_operand(g.p, g.ldp) && direct_operand(g.q, g.ldq) &&
+                        (g.k % 8 == 0 || (q_by_k && (p_by_k || p_padded))) && !(swiglu && q_by_k && g.n % 8 != 0);
+    g.partial = static_cast<float*>(partial);
+    g.splits = plan.splits;
+    g.split_k = static_cast<int>(plan.split_k);
+    hipError_t err = moe::launch_gemm_mid(g, p_by_k, q_by_k, bf16, direct, plan.bm, stream);
+    if (err == hipSuccess && plan.splits > 1) err = moe::launch_gemm_reduce(g, bf16, stream);
+    return err;
+}
+
+size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
+    return plan_product(T, N, H, act == MOE_ACT_SWIGLU, false).partial_bytes;
+}
+
+// Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | partial sums of a split product
+struct GradWorkspace {
+    int64_t Z, ldz;
+    size_t sums_at, partial_at, bytes;
+    ProductPlan x, w;
+};
+GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
+    GradWorkspace g{};
+    g.Z = act == MOE_ACT_SWIGLU ? 2 * N : N;
+    g.ldz = round_up(g.Z, 8);
+    g.x = plan_product(T, H, g.ldz, false, false);
+    g.w = plan_product(g.Z, H, T, false, true);
+    g.sums_at = round_up(T * g.ldz * 2, 256);
+    g.partial_at = g.sums_at + round_up(static_cast<int64_t>(moe::act_grad_row_blocks(T, static_cast<int>(g.Z))) * g.Z * 4, 256);
+    g.bytes = g.partial_at + (g.x.partial_bytes > g.w.partial_bytes ? g.x.partial_bytes : g.w.partial_bytes);
+    return g;
+}
+
+}  // namespace
+
+extern "C" {
+
+moe_status moe_routing_group_topk(const void* logits, int64_t logits_stride, int32_t logits_type, const float* bias,
+                                  int32_t* expert_ids, void* weights, int32_t weights_type, int64_t T, int64_t E,
+                                  int64_t K, int64_t groups, int64_t top_groups, int64_t group_top, int32_t scoring,
+                                  int32_t renormalize, float scale, void* stream) {
+    const char* op = "MoeRoutingGroupTopK";
+    moe_status st = check_group_routing(op, T, E, K, logits_stride, logits_type, weights_type, false);
+    if (st != MOE_OK) return st;
+    st = check_scoring(op, scoring, scale);
+    if (st != MOE_OK) return st;
+    if (groups < 1 || groups > E || E % groups != 0)
+        return fail(MOE_ERR_ARG, "%s: numGroups=%lld must divide numExperts=%lld", op, (long long)groups, (long long)E);
+    if (top_groups < 1 || top_groups > groups)
+        return fail(MOE_ERR_ARG, "%s: topGroups=%lld must be in [1, numGroups=%lld]", op, (long long)top_groups,
+                    (long long)groups);
+    if (group_top != 1 && group_top != 2)
+        return fail(MOE_ERR_ARG, "%s: groupTop=%lld must be 1 or 2", op, (long long)group_top);
+    if (K > top_groups * (E / groups))
+        return fail(MOE_ERR_ARG, "%s: topK=%lld exceeds the %lld experts of %lld groups", op, (long long)K,
+                    (long long)(top_groups * (E / groups)), (long long)top_groups);
+    if (T == 0) return ok();
+    if (!logits || !expert_ids || !weights) return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    moe::GroupRouting r{};
+    r.logits = logits;
+    r.ld = logits_stride;
+    r.logits_type = logits_type;
+    r.bias = bias;
+    r.T = T;
+    r.E = static_cast<int>(E);
+    r.K = static_cast<int>(K);
+    r.groups = static_cast<int>(groups);
+    r.top_groups = static_cast<int>(top_groups);
+    r.group_top = static_cast<int>(group_top);
+    r.sigmoid = scoring == MOE_SCORE_SIGMOID;
+    r.renormalize = renormalize != 0;
+    r.scale = scale;
+    r.weights_type = weights_type;
+    const hipError_t err = moe::launch_group_routing(r, expert_ids, weights, as_stream(stream));
+    if (err != hipSuccess) return hip_fail(err, "MoeRoutingGroupTopK launch");
+    return ok();
+}
+
+moe_status moe_routing_group_topk_grad(const void* grad_weights, int32_t weights_type, const void* logits,
+                                       int64_t logits_stride, int32_t logits_type, const int32_t* expert_ids,
+                                       void* grad_logits, int64_t T, int64_t E, int64_t K, int32_t scoring,
+                                       int32_t renormalize, float scale, void* stream) {
+    const char* op = "MoeRoutingGroupTopKGrad";
+    moe_status st = check_group_routing(op, T, E, K, logits_stride, logits_type, weights_type, true);
+    if (st != MOE_OK) return st;
+    st = check_scoring(op, scoring, scale);
+    if (st != MOE_OK) return st;
+    if (T == 0) return ok();
+    if (!grad_weights || !logits || !expert_ids || !grad_logits)
+        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    moe::GroupRouting r{};
+    r.logits = logits;
+    r.ld = logits_stride;
+    r.logits_type = logits_type;
+    r.T = T;
+    r.E = static_cast<int>(E);
+    r.K = static_cast<int>(K);
+    r.sigmoid = scoring == MOE_SCORE_SIGMOID;
+    r.renormalize = renormalize != 0;
+    r.scale = scale;
+    r.weights_type = weights_type;
+    const hipError_t err =
+        moe::launch_group_routing_grad(r, grad_weights, expert_ids, grad_logits, as_stream(stream));
+    if (err != hipSuccess) return hip_fail(err, "MoeRoutingGroupTopKGrad launch");
+    return ok();
+}
+
+moe_status moe_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, const uint16_t* weights,
+                            uint16_t* grad_expert_out, uint16_t* grad_weights, int64_t T, int64_t H, int64_t K,
+                            void* stream) {
+    const char* op = "MoeCombineGrad";
+    if (T < 0 || H <= 0 || K < 1)
+        return fail(MOE_ERR_ARG, "%s: sizes must be T >= 0, H > 0, K >= 1 (T=%lld H=%lld K=%lld)", op, (long long)T,
+                    (long long)H, (long long)K);
+    if (H % 8 != 0) return fail(MOE_ERR_UNSUPPORTED, "%s: hiddenSize=%lld must be a multiple of 8", op, (long long)H);
+    if (H > kMaxDim)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: hiddenSize=%lld exceeds %lld", op, (long long)H, (long long)kMaxDim);
+    if (product_exceeds(T, K, kInt32Max) || T >= int64_t{1} << 25)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: T=%lld K=%lld too large", op, (long long)T, (long long)K);
+    if (T == 0) return ok();
+    if (!grad_y || !expert_out || !weights || !grad_expert_out || !grad_weights)
+        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    if (!aligned16(grad_y) || !aligned16(expert_out) || !aligned16(grad_expert_out))
+        return fail(MOE_ERR_UNSUPPORTED, "%s: grad_y, expert_out and grad_expert_out must be 16-byte aligned", op);
+    const hipError_t err = moe::launch_combine_grad(grad_y, expert_out, weights, grad_expert_out, grad_weights, T,
+                                                    static_cast<int>(H), static_cast<int>(K), as_stream(stream));
+    if (err != hipSuccess) return hip_fail(err, "MoeCombineGrad launch");
+    return ok();
+}
+
+size_t moe_linear_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation) {
+    if (check_linear("MoeLinear", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
+    return linear_workspace(T, N, H, activation);
+}
+
+moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                      int32_t weight_transposed, const void* bias, const void* residual, void* y, void* pre,
+                      void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
+                      int32_t dtype, int32_t out_dtype, void* stream) {
+    const char* op = "MoeLinear";
+    moe_status st = check_linear(op, T, N, H, activation, dtype);
+    if (st != MOE_OK) return st;
+    if (out_dtype != dtype && out_dtype != MOE_DT_FLOAT32)
+        return fail(MOE_ERR_ARG, "%s: result type %d (the operands' or float32 expected)", op, out_dtype);
+    const int64_t Z = activation == MOE_ACT_SWIGLU ? 2 * N : N;
+    st = check_pitch(op, "x", T, H, x_stride);
+    if (st != MOE_OK) return st;
+    st = weight_transposed ? check_pitch(op, "weight", H, Z, weight_stride) : check_pitch(op, "weight", Z, H, weight_stride);
+    if (st != MOE_OK) return st;
+    if (T == 0) return ok();
+    if (!x || !weight || !y) return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    const ProductPlan plan = plan_product(T, N, H, activation == MOE_ACT_SWIGLU, false);
+    if (plan.partial_bytes > 0 && (!workspace || workspace_bytes < plan.partial_bytes))
+        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace,
+                    plan.partial_bytes);
+    if (plan.partial_bytes > 0 && !aligned16(workspace))
+        return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
+    moe::GemmArgs g{};
+    g.p = static_cast<const uint16_t*>(x);
+    g.q = static_cast<const uint16_t*>(weight);
+    g.ldp = x_stride;
+    g.ldq = weight_stride;
+    g.m = static_cast<int>(T);
+    g.n = static_cast<int>(N);
+    g.k = static_cast<int>(H);
+    g.out = y;
+    g.pre = static_cast<uint16_t*>(pre);
+    g.bias = static_cast<const uint16_t*>(bias);
+    g.residual = residual;
+    g.act = activation;
+    g.out_f32 = out_dtype == MOE_DT_FLOAT32;
+    const hipError_t err = run_product(g, plan, workspace, false, weight_transposed != 0, dtype == MOE_DT_BFLOAT16,
+                                       as_stream(stream));
+    if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
+    return ok();
+}
+
+size_t moe_linear_grad_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation) {
+    if (check_linear("MoeLinearGrad", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
+    return grad_workspace(T, N, H, activation).bytes;
+}
+
+moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
+                           const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
+                           void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                           int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, void* stream) {
+    const char* op = "MoeLinearGrad";
+    moe_status st = check_linear(op, T, N, H, activation, dtype);
+    if (st != MOE_OK) return st;
+    const GradWorkspace ws = grad_workspace(T, N, H, activation);
+    st = check_pitch(op, "grad_y", T, N, grad_y_stride);
+    if (st != MOE_OK) return st;
+    if (grad_weight) st = check_pitch(op, "x", T, H, x_stride);
+    if (st != MOE_OK) return st;
+    if (grad_x)
+        st = weight_transposed ? check_pitch(op, "weight", H, ws.Z, weight_stride)
+                               : check_pitch(op, "weight", ws.Z, H, weight_stride);
+    if (st != MOE_OK) return st;
+    if (!grad_x && !grad_weight && !grad_bias) return ok();
+    const bool act = activation != MOE_ACT_NONE;
+    if (T > 0 && (!grad_y || (act && !pre) || (grad_weight && !x) || (grad_x && !weight)))
+        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    if (T == 0 && !grad_weight && !grad_bias) return ok();
+    if (!workspace || workspace_bytes < ws.bytes)
+        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace,
+                    ws.bytes);
+    if (!aligned16(workspace)) return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
+    const hipStream_t s = as_stream(stream);
+    const bool bf16 = dtype == MOE_DT_BFLOAT16;
+    char* base = static_cast<char*>(workspace);
+    // without an activation dz is grad_y itself, where the products can read that in 16-byte copies
+    const bool as_is = !act && N % 8 == 0 && direct_operand(grad_y, grad_y_stride);
+    const bool need_dz = !as_is && (grad_x || grad_weight) && T > 0;
+    const uint16_t* dz = as_is ? static_cast<const uint16_t*>(grad_y) : reinterpret_cast<uint16_t*>(base);
+    const int64_t ldz = as_is ? grad_y_stride : ws.ldz;
+    hipError_t err = hipSuccess;
+    if (need_dz || grad_bias)
+        err = moe::launch_act_grad(static_cast<const uint16_t*>(grad_y), grad_y_stride,
+                                   act ? static_cast<const uint16_t*>(pre) : nullptr,
+                                   need_dz ? reinterpret_cast<uint16_t*>(base) : nullptr, ws.ldz,
+                                   reinterpret_cast<float*>(base + ws.sums_at), static_cast<uint16_t*>(grad_bias), T,
+                                   static_cast<int>(N), activation, bf16, s);
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad activation launch");
+    void* partial = base + ws.partial_at;
+    if (grad_x && T > 0) {
+        moe::GemmArgs g{};
+        g.p = dz;
+        g.ldp = ldz;
+        g.q = static_cast<const uint16_t*>(weight);
+        g.ldq = weight_stride;
+        g.m = static_cast<int>(T);
+        g.n = static_cast<int>(H);
+        g.k = static_cast<int>(ws.Z);
+        g.out = grad_x;
+        err = run_product(g, ws.x, partial, false, weight_transposed == 0, bf16, s, need_dz);
+        if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad grad_x launch");
+    }
+    if (grad_weight) {
+        moe::GemmArgs g{};
+        g.p = dz;
+        g.ldp = ldz;
+        g.q = static_cast<const uint16_t*>(x);
+        g.ldq = x_stride;
+        g.m = static_cast<int>(ws.Z);
+        g.n = static_cast<int>(H);
+        g.k = static_cast<int>(T);
+        g.out = grad_weight;
+        err = run_product(g, ws.w, partial, true, true, bf16, s);
+        if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad grad_weight launch");
+    }
+    return ok();
+}
+
+}  // extern "C"

@@ -167,6 +167,34 @@ int combine_grid(int64_t T, int64_t H);
 hipError_t launch_combine(const uint16_t* expert_out, const uint16_t* weights, uint16_t* y, int T, int H, int K,
                           hipStream_t stream);
 
+hipError_t launch_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, const uint16_t* weights,
+                               uint16_t* grad_eo, uint16_t* grad_w, int64_t T, int H, int K, hipStream_t stream);
+
+// ---- routing from logits: scores, balance bias, groups, top-K (moe_group_routing.hip) ----
+struct GroupRouting {
+    const void* logits;  // [T, E], rows ld elements apart
+    int64_t ld;
+    int32_t logits_type;  // moe_dtype
+    const float* bias;    // [E] or null
+    int64_t T;
+    int E, K, groups, top_groups, group_top;
+    bool sigmoid, renormalize;
+    float scale;
+    int32_t weights_type;  // moe_dtype
+};
+hipError_t launch_group_routing(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream);
+// grad_weights (weights_type) and ids [T, K] -> grad_logits [T, E] of logits_type, contiguous
+hipError_t launch_group_routing_grad(const GroupRouting& r, const void* grad_weights, const int32_t* ids,
+                                     void* grad_logits, hipStream_t stream);
+
+// ---- dense products (moe_linear*.hip) ----
+enum Activation { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActSwiglu = 5 };
+// dz = dy * act'(pre) with rows of ldz (zeros past Z); bias_grad (null: not wanted) = column sums through `part`
+// (act_grad_row_blocks(T, Z) * Z floats); dz null: the sums alone
+int act_grad_row_blocks(int64_t T, int Z);
+hipError_t launch_act_grad(const uint16_t* dy, int64_t ldy, const uint16_t* pre, uint16_t* dz, int64_t ldz, float* part,
+                           uint16_t* bias_grad, int64_t T, int N, int act, bool bf16, hipStream_t stream);
+
 // ---- synthetic inputs / calibration (moe_synth.hip) ----
 hipError_t launch_synth_normal_f16(uint16_t* out, uint64_t n, uint64_t seed, uint64_t stream_id, double sigma_a,
                                    double sigma_b, uint64_t period, uint64_t split, hipStream_t stream);

@@ -1,0 +1,313 @@
+// moe_linear.hip -- MoeLinear and MoeLinearGrad for gfx950: y = act(x W^T + b) + r and its gradients.
+//
+// No counterpart in the reference, whose products are the expert FFN's (op_kernel/moe_expert_ffn.cpp:265-394).
+// Every product here is C[m][n] = sum_k P[m][k] Q[n][k] with fp16 or bf16 operands and fp32 sums (MFMA):
+//   forward    P = x  (by rows), Q = W (by rows, or by k when W is a transposed view)
+//   grad_x     P = dz (by rows), Q = W read the other way round
+//   grad_W     P = dz (by k: its T rows are the reduction), Q = x (by k)
+#include "moe_gemm.h"
+
+namespace moe {
+
+namespace {
+
+constexpr int kBN = 128;      // Q rows of a tile (SwiGLU: 64 gate and the matching 64 up rows)
+constexpr int kBK = 64;       // k of a stage
+constexpr int kThreads = 256; // 4 waves
+constexpr int kXcds = 8;
+constexpr uint32_t kPastEnd = 0x80000000u;  // a buffer offset past every buffer: the load returns zeros
+
+// Stages in the LDS ring: two 64 KB workgroups a CU at 128 rows, two of 72 or 80 KB below
+constexpr int ring_stages(int bm) { return bm >= 128 ? 2 : bm == 64 ? 3 : 4; }
+constexpr int mid_lds_bytes(int bm) { return ring_stages(bm) * (bm + kBN) * kBK * 2; }
+
+// Where the 16 bytes that lane `lane` of copy instruction `i` writes to LDS come from. Direct-to-LDS copies write 64
+// consecutive 16-byte granules, so the layout's swizzle is in which granule each lane fetches.
+//   by rows: an LDS row is one operand row, 64 k = 8 granules; granule g of row r stands at g ^ ((r >> 1) & 7), so the
+//            16 rows one ds_read_b128 touches spread over all banks.
+//   by k:    an LDS row is one k, ROWS operand rows = ROWS / 8 granules; its 32-byte pairs stand at pair ^ f(k), f over
+//            (k & 3, k >> 3 & 1), so the 8 k that half a wave's ds_read_b64_tr_b16 touches spread over all banks.
+struct Granule {
+    int row;  // by rows: operand row of the tile; by k: k of the stage
+    int el;   // by rows: first k of the stage; by k: first operand row of the tile
+};
+template <bool BY_K, int ROWS>
+__device__ __forceinline__ Granule granule_of(int i, int lane) {
+    static_assert(!BY_K || ROWS == 128, "the swizzle by k permutes 8 pairs of granules");
+    if (!BY_K) {
+        const int r = i * 8 + lane / 8;
+        return Granule{r, ((lane % 8) ^ ((r >> 1) & 7)) * 8};
+    }
+    constexpr int kPer = ROWS / 8;  // granules per LDS row
+    const int k = i * (64 / kPer) + lane / kPer;
+    const int f = (k & 3) | (((k >> 3) & 1) << 2);
+    return Granule{k, ((lane % kPer) ^ (f << 1)) * 8};
+}
+
+// Fragment of 16 operand rows from r0 on and 32 k from 32 kk on: lane (row16, kg) gets 8 k of row r0 + row16.
+template <bool BY_K, int ROWS>
+__device__ __forceinline__ s16x8 read_fragment(const uint16_t* tile, int r0, int kk, int lane) {
+    const int kg = lane >> 4;
+    if (!BY_K) {
+        const int r = r0 + (lane & 15);
+        return *reinterpret_cast<const s16x8*>(tile + r * kBK + (((kk * 4 + kg) ^ ((r >> 1) & 7)) * 8));
+    }
+    s16x4 h[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int k = kk * 32 + kg * 8 + t * 4 + ((lane & 15) >> 2);
+        const int f = (k & 3) | (((k >> 3) & 1) << 2);
+        const int q = lane & 3;  // 4 rows = 8 bytes: granule r0 / 8 + q / 2, half q & 1
+        h[t] = lds_read_transposed(tile + k * ROWS + (((r0 / 8 + (q >> 1)) ^ (f << 1)) * 8) + (q & 1) * 4);
+    }
+    return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
+}
+
+// C[m][n] tile of BM x 128 (4 waves), one ring of direct-to-LDS stages, one barrier a stage.
+// DIRECT: both operands allow 16-byte copies (bases and row pitches 16-byte aligned, by rows k % 8 == 0). Otherwise the
+// elements are loaded one by one and written to the same layout.
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
+__global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
+    extern __shared__ __align__(16) uint16_t lds[];
+    constexpr int NS = ring_stages(BM);
+    constexpr int WM = BM >= 128 ? 2 : 1, WN = 4 / WM;  // waves along m and n
+    constexpr int FM = BM / WM / 16, FN = kBN / WN / 16;  // 16 x 16 blocks of a wave
+    constexpr int PC = BM / 32, QC = kBN / 32;  // copy instructions per wave and stage
+    constexpr int kSlot = (BM + kBN) * kBK;
+    const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int wm = wave / WN, wn = wave % WN;
+    const int row16 = lane & 15, kg = lane >> 4;
+
+    // Workgroups go round-robin over the XCDs; each XCD takes a contiguous run of the items (n-tile, split, m-tile), m
+    // fastest, so the m-tiles that read the same piece of Q share an L2.
+    const int per_xcd = static_cast<int>(gridDim.x) / kXcds;
+    const int item = (static_cast<int>(blockIdx.x) % kXcds) * per_xcd + static_cast<int>(blockIdx.x) / kXcds;
+    if (item >= mtiles * ntiles * g.splits) return;
+    const int mt = item % mtiles, sp = item / mtiles % g.splits, nt = item / mtiles / g.splits;
+    const int k0 = sp * g.split_k, k1 = min(g.k, k0 + g.split_k);
+    const int nst = max(1, (k1 - k0 + kBK - 1) / kBK);
+    const int m0 = mt * BM, n0 = nt * (SWIGLU ? kBN / 2 : kBN);
+
+    // Q row of tile row r. SwiGLU: a wave's rows are half gate, half up, of the same output columns.
+    auto q_col = [&](int r) {
+        if (!SWIGLU) return n0 + r;
+        constexpr int kHalf = kBN / WN / 2;
+        return n0 + r / (2 * kHalf) * kHalf + r % kHalf;
+    };
+    auto q_up = [&](int r) { return SWIGLU && (r / (kBN / WN / 2)) % 2 == 1; };
+
+    int prow[PC], pel[PC], qrow[QC], qel[QC];
+#pragma unroll
+    for (int c = 0; c < PC; ++c) {
+        const Granule a = granule_of<PK, BM>(wave * PC + c, lane);
+        prow[c] = a.row;
+        pel[c] = a.el;
+    }
+#pragma unroll
+    for (int c = 0; c < QC; ++c) {
+        const Granule a = granule_of<QK, kBN>(wave * QC + c, lane);
+        qrow[c] = a.row;
+        qel[c] = a.el;
+    }
+    // Copies stage s. Offsets are relative to (by rows) the tile's first row, (by k) the stage's first k, with 64-bit
+    // arithmetic in the base alone, so an operand may be larger than 4 GiB.
+    auto copy_stage = [&](int s) __attribute__((always_inline)) {
+        uint16_t* slot = lds + (s % NS) * kSlot;
+        const int kc = k0 + s * kBK;
+        if (DIRECT) {
+            const uint32_t ppitch = static_cast<uint32_t>(g.ldp) * 2;
+            const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<uint16_t*>(g.p + static_cast<int64_t>(PK ? kc : m0) * g.ldp), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+            for (int c = 0; c < PC; ++c) {
+                const int row = m0 + (PK ? pel[c] : prow[c]), k = kc + (PK ? prow[c] : pel[c]);
+                const uint32_t off = prow[c] * ppitch + (PK ? row : k) * 2u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    pr, (__attribute__((address_space(3))) void*)(slot + (wave * PC + c) * 512), 16,
+                    static_cast<int>(row < g.m && k < k1 ? off : kPastEnd), 0, 0, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < QC; ++c) {
+                // by rows a copy instruction covers 8 rows, all gate or all up: the base tells them apart, so that the
+                // offsets stay within the tile
+                const int tr = QK ? qel[c] : qrow[c];
+                const int col = q_col(tr), k = kc + (QK ? qrow[c] : qel[c]);
+                const int64_t first = QK ? kc : n0 + (q_up((wave * QC + c) * 8) ? static_cast<int64_t>(g.n) : 0);
+                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<uint16_t*>(g.q + first * g.ldq), 0, 0x7fffffff, 0x00020000);
+                const uint32_t pitch = static_cast<uint32_t>(g.ldq) * 2;
+                const uint32_t off = QK ? qrow[c] * pitch + (col + (q_up(tr) ? g.n : 0)) * 2u
+                                        : (col - n0) * pitch + k * 2u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    r, (__attribute__((address_space(3))) void*)(slot + BM * kBK + (wave * QC + c) * 512), 16,
+                    static_cast<int>(col < g.n && k < k1 ? off : kPastEnd), 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < PC; ++c) {
+                s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int row = m0 + (PK ? pel[c] + e : prow[c]), k = kc + (PK ? prow[c] : pel[c] + e);
+                    if (row < g.m && k < k1)
+                        v[e] = static_cast<short>(PK ? g.p[static_cast<int64_t>(k) * g.ldp + row]
+                                                     : g.p[static_cast<int64_t>(row) * g.ldp + k]);
+                }
+                *reinterpret_cast<s16x8*>(slot + (wave * PC + c) * 512 + lane * 8) = v;
+            }
+#pragma unroll
+            for (int c = 0; c < QC; ++c) {
+                s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int tr = QK ? qel[c] + e : qrow[c], col = q_col(tr);
+                    const int k = kc + (QK ? qrow[c] : qel[c] + e);
+                    const int64_t row = col + (q_up(tr) ? g.n : 0);
+                    if (col < g.n && k < k1)
+                        v[e] = static_cast<short>(QK ? g.q[static_cast<int64_t>(k) * g.ldq + row]
+                                                     : g.q[row * g.ldq + k]);
+                }
+                *reinterpret_cast<s16x8*>(slot + BM * kBK + (wave * QC + c) * 512 + lane * 8) = v;
+            }
+        }
+    };
+
+    f32x4 acc[FN][FM];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) copy_stage(s);  // stages past the last are all past k1: zeros, no traffic
+    for (int s = 0; s < nst; ++s) {
+        // this wave's reads of stage s - 1 are in registers and its copies of stage s have landed; after the barrier
+        // so have everyone's, and the slot of stage s - 1 may be filled again
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * (PC + QC)) & 0xf0ffu);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        __builtin_amdgcn_sched_barrier(0);
+        copy_stage(s + NS - 1);
+        const uint16_t* tp = lds + (s % NS) * kSlot;
+        const uint16_t* tq = tp + BM * kBK;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            s16x8 fp[FM], fq[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fp[i] = read_fragment<PK, BM>(tp, wm * (BM / WM) + i * 16, kk, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fq[j] = read_fragment<QK, kBN>(tq, wn * (kBN / WN) + j * 16, kk, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[j][i] = T::mfma(fq[j], fp[i], acc[j][i]);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the surplus copies have landed before the workgroup ends
+
+    // acc[j][i]: D[Q row 4 kg + r of block j][P row row16 of block i], 4 consecutive columns of one row
+    constexpr int FO = SWIGLU ? FN / 2 : FN;
+    const bool vec = vector_rows(g);
+    const int64_t pld = part_ld(g.n, SWIGLU), pcols = part_cols(g.n);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int row = m0 + wm * (BM / WM) + i * 16 + row16;
+        if (row >= g.m) continue;
+#pragma unroll
+        for (int j = 0; j < FO; ++j) {
+            const int col = n0 + wn * (FO * 16) + j * 16 + kg * 4;
+            if (g.splits > 1) {
+                if (col >= g.n) continue;
+                float* dst = g.partial + (static_cast<int64_t>(sp) * g.m + row) * pld + col;
+                *reinterpret_cast<f32x4*>(dst) = acc[j][i];
+                if (SWIGLU) *reinterpret_cast<f32x4*>(dst + pcols) = acc[j + FO][i];
+            } else {
+                store4<T, SWIGLU>(g, row, col, acc[j][i], SWIGLU ? acc[j + FO][i] : acc[j][i], vec);
+            }
+        }
+    }
+}
+
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
+hipError_t run_mid(const GemmArgs& g, hipStream_t stream) {
+    const int bn = SWIGLU ? kBN / 2 : kBN;
+    const int mtiles = (g.m + BM - 1) / BM, ntiles = (g.n + bn - 1) / bn;
+    const int64_t items = static_cast<int64_t>(mtiles) * ntiles * g.splits;
+    const int grid = static_cast<int>((items + kXcds - 1) / kXcds * kXcds);
+    auto fn = &gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT>;
+    const hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(fn), mid_lds_bytes(BM));
+    if (err != hipSuccess) return err;
+    TraceScope trace("moe_linear_gemm", stream);
+    fn<<<grid, kThreads, mid_lds_bytes(BM), stream>>>(g, mtiles, ntiles);
+    return hipGetLastError();
+}
+
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU>
+hipError_t run_mid_direct(const GemmArgs& g, bool direct, hipStream_t stream) {
+    return direct ? run_mid<T, PK, QK, BM, SWIGLU, true>(g, stream) : run_mid<T, PK, QK, BM, SWIGLU, false>(g, stream);
+}
+
+template <typename T>
+hipError_t run_mid_any(const GemmArgs& g, bool p_by_k, bool q_by_k, bool direct, int bm, hipStream_t stream) {
+    const bool swiglu = g.act == kActSwiglu;
+    if (p_by_k) return run_mid_direct<T, true, true, 128, false>(g, direct, stream);
+    if (bm == 128) {
+        if (q_by_k) return swiglu ? run_mid_direct<T, false, true, 128, true>(g, direct, stream)
+                                  : run_mid_direct<T, false, true, 128, false>(g, direct, stream);
+        return swiglu ? run_mid_direct<T, false, false, 128, true>(g, direct, stream)
+                      : run_mid_direct<T, false, false, 128, false>(g, direct, stream);
+    }
+    if (q_by_k) return swiglu ? run_mid_direct<T, false, true, 32, true>(g, direct, stream)
+                              : run_mid_direct<T, false, true, 32, false>(g, direct, stream);
+    return swiglu ? run_mid_direct<T, false, false, 32, true>(g, direct, stream)
+                  : run_mid_direct<T, false, false, 32, false>(g, direct, stream);
+}
+
+// Adds the splits' sums in order and applies the epilogue; a thread has 4 columns of a row.
+constexpr int kReduceThreads = 256;
+template <typename T, bool SWIGLU>
+__global__ __launch_bounds__(kReduceThreads) void gemm_reduce_kernel(GemmArgs g) {
+    const int64_t pcols = part_cols(g.n), pld = part_ld(g.n, SWIGLU), per_row = pcols / 4;
+    const int64_t idx = static_cast<int64_t>(blockIdx.x) * kReduceThreads + threadIdx.x;
+    if (idx >= per_row * g.m) return;
+    const int64_t row = idx / per_row;
+    const int col = static_cast<int>(idx % per_row) * 4;
+    const float* src = g.partial + row * pld + col;
+    const int64_t step = static_cast<int64_t>(g.m) * pld;
+    f32x4 z = *reinterpret_cast<const f32x4*>(src), u = {0.f, 0.f, 0.f, 0.f};
+    if (SWIGLU) u = *reinterpret_cast<const f32x4*>(src + pcols);
+#pragma unroll 4
+    for (int s = 1; s < g.splits; ++s) {
+        z += *reinterpret_cast<const f32x4*>(src + s * step);
+        if (SWIGLU) u += *reinterpret_cast<const f32x4*>(src + s * step + pcols);
+    }
+    store4<T, SWIGLU>(g, row, col, z, u, vector_rows(g));
+}
+
+}  // namespace
+
+hipError_t launch_gemm_mid(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, bool direct, int bm,
+                           hipStream_t stream) {
+    return bf16 ? run_mid_any<Bf16>(g, p_by_k, q_by_k, direct, bm, stream)
+                : run_mid_any<Half>(g, p_by_k, q_by_k, direct, bm, stream);
+}
+
+hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream) {
+    const bool swiglu = g.act == kActSwiglu;
+    const int64_t work = part_cols(g.n) / 4 * g.m;
+    const int grid = static_cast<int>((work + kReduceThreads - 1) / kReduceThreads);
+    TraceScope trace("moe_linear_reduce", stream);
+    if (bf16) {
+        if (swiglu) gemm_reduce_kernel<Bf16, true><<<grid, kReduceThreads, 0, stream>>>(g);
+        else gemm_reduce_kernel<Bf16, false><<<grid, kReduceThreads, 0, stream>>>(g);
+    } else {
+        if (swiglu) gemm_reduce_kernel<Half, true><<<grid, kReduceThreads, 0, stream>>>(g);
+        else gemm_reduce_kernel<Half, false><<<grid, kReduceThreads, 0, stream>>>(g);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace moe

@@ -6,45 +6,14 @@
 
 #include <hip/hip_runtime.h>
 
-#include <cstdarg>
-#include <cstdio>
-#include <cstring>
-
+#include "moe_host.h"
 #include "moe_launch.h"
 #include "moe_ops.h"
 #include "moe_synth.h"
 
+using namespace moe::host;
+
 namespace {
-
-thread_local char g_last_error[512] = "";
-
-moe_status fail(moe_status st, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    std::vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
-    va_end(ap);
-    return st;
-}
-
-moe_status ok() {
-    g_last_error[0] = '\0';
-    return MOE_OK;
-}
-
-moe_status hip_fail(hipError_t err, const char* what) {
-    return fail(MOE_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-constexpr int64_t kMaxExperts = 256;
-constexpr int64_t kInt32Max = 2147483647;
-// hiddenSize and intermediateSize bound: far above any model's, and small enough that the products of sizes the
-// checks below form stay within 64 bits
-constexpr int64_t kMaxDim = int64_t{1} << 20;
-
-// a * b > limit for a, b >= 0, without forming a product that could overflow
-bool product_exceeds(int64_t a, int64_t b, int64_t limit) { return b != 0 && a > limit / b; }
 
 // Scalar checks shared by the planners and launches.
 moe_status check_routing_sizes(int64_t T, int64_t H, int64_t E, int64_t K) {
@@ -89,8 +58,6 @@ moe_status check_combine_sizes(int64_t T, int64_t H, int64_t K) {
     return ok();
 }
 
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
-
 }  // namespace
 
 extern "C" {
@@ -109,7 +76,7 @@ const char* moe_status_string(moe_status status) {
     return "MOE_ERR_UNKNOWN";
 }
 
-const char* moe_last_error(void) { return g_last_error; }
+const char* moe_last_error(void) { return last_error(); }
 
 const char* moe_version(void) { return "moe_mi355x 0.1.0 (gfx950)"; }
 

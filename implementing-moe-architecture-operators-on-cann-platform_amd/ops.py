@@ -30,6 +30,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", None)
 
 _TORCH_DT = {_lib.DT_FLOAT16: torch.float16, _lib.DT_INT32: torch.int32}
+_FLOAT_DT = {torch.float32: _lib.DT_FLOAT32, torch.float16: _lib.DT_FLOAT16, torch.bfloat16: _lib.DT_BFLOAT16}
+_SCORING = {"softmax": 0, "sigmoid": 1}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
 
 
 def _stream_ptr(stream) -> int:
@@ -260,6 +263,267 @@ def moe_layer_fused(x: torch.Tensor, w_gate: torch.Tensor, expert_weights: torch
                         expert_out.data_ptr(), y.data_ptr(), workspace.data_ptr(), _bytes(workspace), T, H, E, K,
                         inter, _stream_ptr(stream)))
     return y, ids, w, expert_out
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# operators around the routed experts (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _need_float(t, name: str, dtypes, device, dims: int | None = None) -> int:
+    """Checks a floating device tensor of any strides; returns its moe_dtype."""
+    if not isinstance(t, torch.Tensor):
+        raise MoeError(1, f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise MoeError(4, f"{name} must be a device tensor (got {t.device})")
+    if device is not None and t.device != device:
+        raise MoeError(4, f"{name} is on {t.device}, the first tensor on {device}")
+    if t.dtype not in dtypes:
+        raise MoeError(4, f"{name} must be {' or '.join(str(d) for d in dtypes)} (got {t.dtype})")
+    if dims is not None and t.dim() != dims:
+        raise MoeError(2, f"{name} must have {dims} dimensions (got {t.dim()})")
+    return _FLOAT_DT[t.dtype]
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are contiguous."""
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise MoeError(4, f"{name}: the elements of a row must be contiguous (strides {t.stride()})")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _weight_layout(t: torch.Tensor) -> tuple[int, int]:
+    """(stride, transposed) of a 2-D weight that is contiguous along one of its dimensions."""
+    n, h = t.shape
+    if h == 1 or t.stride(1) == 1:
+        return (t.stride(0) if n > 1 else max(t.stride(0), h)), 0
+    if n == 1 or t.stride(0) == 1:
+        return (t.stride(1) if h > 1 else max(t.stride(1), n)), 1
+    raise MoeError(4, f"weight must be contiguous along one dimension (strides {t.stride()})")
+
+
+def _need_shape(t: torch.Tensor, name: str, shape) -> None:
+    if tuple(t.shape) != tuple(shape):
+        raise MoeError(3, f"{name} shape {tuple(t.shape)} != {tuple(shape)}")
+
+
+def _act_code(activation: str) -> int:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise MoeError(4, f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+    return code
+
+
+def _scoring_code(scoring: str) -> int:
+    code = _SCORING.get(scoring)
+    if code is None:
+        raise MoeError(4, f"scoring {scoring!r}: one of {', '.join(_SCORING)}")
+    return code
+
+
+def _need_workspace(workspace, need: int, like, device):
+    if workspace is None:
+        return like.new_empty(max(need, 1), dtype=torch.uint8)
+    if not isinstance(workspace, torch.Tensor) or workspace.device != device or not workspace.is_contiguous():
+        raise MoeError(4, f"workspace must be a contiguous tensor on {device}")
+    return workspace
+
+
+def MoeRoutingGroupTopK(logits: torch.Tensor, bias: torch.Tensor | None = None, topK: int = 2, numGroups: int = 1,
+                        topGroups: int = 1, groupTop: int = 1, scoring: str = "softmax", renormalize: bool = True,
+                        scale: float = 1.0, weightsDtype: torch.dtype = torch.float16, stream=None):
+    """logits[T,E] (fp32, fp16 or bf16), bias[E] fp32 -> (expert_ids[T,K] int32, weights[T,K] fp16 or fp32).
+
+    Scores are the softmax or the sigmoid of the logits. Experts are chosen by score + bias: of numGroups groups of
+    consecutive experts the topGroups best stay, a group's score being its best expert's (groupTop=1) or the sum of its
+    two best (2); of the experts that stay the topK best are chosen, equal ones by lowest index. The weights are the
+    chosen scores, without bias, over their sum (renormalize) and times scale. Experts whose logit is -inf or NaN
+    are not available; picks a row has no expert left for are id -1, weight 0."""
+    lt = _need_float(logits, "logits", (torch.float32, torch.float16, torch.bfloat16), None, 2)
+    T, E = logits.shape
+    if bias is not None:
+        _need_float(bias, "bias", (torch.float32,), logits.device, 1)
+        _need_shape(bias, "bias", (E,))
+        if not bias.is_contiguous():
+            raise MoeError(4, "bias must be contiguous")
+    if weightsDtype not in (torch.float16, torch.float32):
+        raise MoeError(4, f"weightsDtype must be float16 or float32 (got {weightsDtype})")
+    ld = _row_stride(logits, "logits")
+    if type(topK) is not int or topK < 1 or topK > E:
+        raise MoeError(4, f"topK={topK} must be in [1, numExperts={E}]")
+    like = _like(logits)
+    with _on(stream):
+        ids = like.new_empty((T, topK), dtype=torch.int32)
+        w = like.new_empty((T, topK), dtype=weightsDtype)
+    check(_lib.load().moe_routing_group_topk(logits.data_ptr(), ld, lt, _ptr(bias), ids.data_ptr(), w.data_ptr(),
+                                             _FLOAT_DT[weightsDtype], T, E, topK, numGroups, topGroups, groupTop,
+                                             _scoring_code(scoring), int(renormalize), scale, _stream_ptr(stream)))
+    return ids, w
+
+
+def MoeRoutingGroupTopKGrad(grad_weights: torch.Tensor, logits: torch.Tensor, expert_ids: torch.Tensor,
+                            scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+                            stream=None) -> torch.Tensor:
+    """The gradient of MoeRoutingGroupTopK's weights -> the logits', [T,E] contiguous, of the logits' type.
+    expert_ids are the forward's; the choice itself (and with it the bias) has no gradient."""
+    lt = _need_float(logits, "logits", (torch.float32, torch.float16, torch.bfloat16), None, 2)
+    T, E = logits.shape
+    gt = _need_float(grad_weights, "grad_weights", (torch.float32, torch.float16, torch.bfloat16), logits.device, 2)
+    _need(expert_ids, "expert_ids", torch.int32)
+    if expert_ids.device != logits.device:
+        raise MoeError(4, f"expert_ids is on {expert_ids.device}, logits on {logits.device}")
+    if expert_ids.dim() != 2 or expert_ids.shape[0] != T:
+        raise MoeError(3, f"expert_ids shape {tuple(expert_ids.shape)} for {T} rows of logits")
+    _need_shape(grad_weights, "grad_weights", expert_ids.shape)
+    if not grad_weights.is_contiguous():
+        raise MoeError(4, "grad_weights must be contiguous (ND format)")
+    ld = _row_stride(logits, "logits")
+    like = _like(logits)
+    with _on(stream):
+        grad = like.new_empty((T, E))
+    check(_lib.load().moe_routing_group_topk_grad(grad_weights.data_ptr(), gt, logits.data_ptr(), ld, lt,
+                                                  expert_ids.data_ptr(), grad.data_ptr(), T, E, expert_ids.shape[1],
+                                                  _scoring_code(scoring), int(renormalize), scale,
+                                                  _stream_ptr(stream)))
+    return grad
+
+
+def MoeCombineGrad(grad_y: torch.Tensor, expert_out: torch.Tensor, weights: torch.Tensor, stream=None):
+    """grad_y[T,H], expert_out[T,K,H], weights[T,K] fp16 -> (grad_expert_out[T,K,H], grad_weights[T,K]) fp16."""
+    _need(grad_y, "grad_y", torch.float16)
+    _need(expert_out, "expert_out", torch.float16)
+    _need(weights, "weights", torch.float16)
+    if expert_out.dim() != 3:
+        raise MoeError(2, f"expert_out must have 3 dimensions (got {expert_out.dim()})")
+    T, K, H = expert_out.shape
+    _need_shape(grad_y, "grad_y", (T, H))
+    _need_shape(weights, "weights", (T, K))
+    if grad_y.device != expert_out.device or weights.device != expert_out.device:
+        raise MoeError(4, "grad_y, expert_out and weights must be on one device")
+    like = _like(expert_out)
+    with _on(stream):
+        geo = like.new_empty((T, K, H))
+        gw = like.new_empty((T, K))
+    check(_lib.load().moe_combine_grad(grad_y.data_ptr(), expert_out.data_ptr(), weights.data_ptr(), geo.data_ptr(),
+                                       gw.data_ptr(), T, H, K, _stream_ptr(stream)))
+    return geo, gw
+
+
+def linear_workspace_bytes(T: int, N: int, H: int, activation: str = "none") -> int:
+    return int(_lib.load().moe_linear_workspace_bytes(T, N, H, _act_code(activation)))
+
+
+def linear_grad_workspace_bytes(T: int, N: int, H: int, activation: str = "none") -> int:
+    return int(_lib.load().moe_linear_grad_workspace_bytes(T, N, H, _act_code(activation)))
+
+
+def _linear_sizes(x, weight, act: int):
+    T, H = x.shape
+    Z = weight.shape[0]
+    if weight.shape[1] != H:
+        raise MoeError(3, f"hidden size mismatch x[{H}] vs weight[{weight.shape[1]}]")
+    if act == ACTIVATIONS["swiglu"] and Z % 2:
+        raise MoeError(3, f"weight rows ({Z}) of a swiglu must be N gate and N up rows")
+    return T, H, Z // 2 if act == ACTIVATIONS["swiglu"] else Z, Z
+
+
+def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+              residual: torch.Tensor | None = None, activation: str = "none", outDtype: torch.dtype | None = None,
+              returnPre: bool = False, workspace: torch.Tensor | None = None, stream=None):
+    """act(x[T,H] @ weight[N,H]^T + bias[N]) + residual[T,N] -> y[T,N] of outDtype (x's type, or fp32).
+
+    x and weight are fp16 or bf16; x's rows and weight along one of its dimensions must be contiguous (w_gate.t() is a
+    weight). activation: none, relu, gelu, gelu_tanh, silu or swiglu, which takes weight[2N,H] (and bias[2N]), the N gate
+    rows first. residual has y's type. With returnPre -> (y, pre): the sums before the activation, which MoeLinearGrad
+    takes. `workspace` (uint8, >= linear_workspace_bytes) is allocated when not given."""
+    act = _act_code(activation)
+    dt = _need_float(x, "x", (torch.float16, torch.bfloat16), None, 2)
+    _need_float(weight, "weight", (x.dtype,), x.device, 2)
+    T, H, N, Z = _linear_sizes(x, weight, act)
+    out = x.dtype if outDtype is None else outDtype
+    if out not in (x.dtype, torch.float32):
+        raise MoeError(4, f"outDtype must be {x.dtype} or float32 (got {out})")
+    ldx = _row_stride(x, "x")
+    ldw, transposed = _weight_layout(weight)
+    if bias is not None:
+        _need_float(bias, "bias", (x.dtype,), x.device, 1)
+        _need_shape(bias, "bias", (Z,))
+        if not bias.is_contiguous():
+            raise MoeError(4, "bias must be contiguous")
+    if residual is not None:
+        _need_float(residual, "residual", (out,), x.device, 2)
+        _need_shape(residual, "residual", (T, N))
+        if not residual.is_contiguous():
+            raise MoeError(4, "residual must be contiguous (ND format)")
+    lib = _lib.load()
+    like = _like(x)
+    with _on(stream):
+        need = 0 if workspace is not None else int(lib.moe_linear_workspace_bytes(T, N, H, act))
+        workspace = _need_workspace(workspace, need, like, x.device)
+        y = like.new_empty((T, N), dtype=out)
+        pre = like.new_empty((T, Z)) if returnPre else None
+    check(lib.moe_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, _ptr(bias), _ptr(residual),
+                         y.data_ptr(), _ptr(pre), workspace.data_ptr(), _bytes(workspace), T, N, H, act, dt,
+                         _FLOAT_DT[out], _stream_ptr(stream)))
+    return (y, pre) if returnPre else y
+
+
+def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: torch.Tensor | None = None,
+                  activation: str = "none", gradX: bool = True, gradWeight: bool = True, gradBias: bool = False,
+                  workspace: torch.Tensor | None = None, stream=None):
+    """The gradient of MoeLinear's y[T,N] (of x's type) -> (grad_x[T,H], grad_weight[N,H], grad_bias[N]), contiguous, of
+    x's type, None where not asked for. pre is MoeLinear's (needed with an activation). The residual's gradient is
+    grad_y. `workspace` (uint8, >= linear_grad_workspace_bytes) is allocated when not given."""
+    act = _act_code(activation)
+    dt = _need_float(x, "x", (torch.float16, torch.bfloat16), None, 2)
+    _need_float(weight, "weight", (x.dtype,), x.device, 2)
+    _need_float(grad_y, "grad_y", (x.dtype,), x.device, 2)
+    T, H, N, Z = _linear_sizes(x, weight, act)
+    _need_shape(grad_y, "grad_y", (T, N))
+    ldx, ldy = _row_stride(x, "x"), _row_stride(grad_y, "grad_y")
+    ldw, transposed = _weight_layout(weight)
+    if act:
+        if pre is None:
+            raise MoeError(1, f"MoeLinearGrad needs pre with activation {activation!r}")
+        _need_float(pre, "pre", (x.dtype,), x.device, 2)
+        _need_shape(pre, "pre", (T, Z))
+        if not pre.is_contiguous():
+            raise MoeError(4, "pre must be contiguous (ND format)")
+    lib = _lib.load()
+    like = _like(x)
+    with _on(stream):
+        need = 0 if workspace is not None else int(lib.moe_linear_grad_workspace_bytes(T, N, H, act))
+        workspace = _need_workspace(workspace, need, like, x.device)
+        gx = like.new_empty((T, H)) if gradX else None
+        gw = like.new_empty((Z, H)) if gradWeight else None
+        gb = like.new_empty((Z,)) if gradBias else None
+    check(lib.moe_linear_grad(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed,
+                              _ptr(pre) if act else None, _ptr(gx), _ptr(gw), _ptr(gb), workspace.data_ptr(),
+                              _bytes(workspace), T, N, H, act, dt, _stream_ptr(stream)))
+    return gx, gw, gb
+
+
+def moe_layer_shared(x: torch.Tensor, w_gate: torch.Tensor, expert_weights: torch.Tensor,
+                     shared_gate_up: torch.Tensor | None = None, shared_down: torch.Tensor | None = None,
+                     topK: int = 2, bias: torch.Tensor | None = None, numGroups: int = 1, topGroups: int = 1,
+                     groupTop: int = 1, scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+                     stream=None):
+    """A layer with scored and grouped routing and a dense expert that every token passes: fp32 logits x @ w_gate[H,E]
+    (MoeLinear), MoeRoutingGroupTopK, the routed experts (MoeExpertFFNCombine), and, where its weights are given, the
+    dense expert's shared_gate_up[2S,H] (SwiGLU) and shared_down[H,S], whose epilogue adds the routed result.
+    Returns (y, expert_ids, weights, expert_out)."""
+    if (shared_gate_up is None) != (shared_down is None):
+        raise MoeError(1, "shared_gate_up and shared_down are given together")
+    if w_gate.dim() == 2 and expert_weights.dim() == 3 and expert_weights.shape[0] != w_gate.shape[1]:
+        raise MoeError(3, f"w_gate routes to {w_gate.shape[1]} experts, expert_weights holds {expert_weights.shape[0]}")
+    logits = MoeLinear(x, w_gate.t(), outDtype=torch.float32, stream=stream)
+    ids, w = MoeRoutingGroupTopK(logits, bias, topK, numGroups, topGroups, groupTop, scoring, renormalize, scale,
+                                 stream=stream)
+    eo, y = MoeExpertFFNCombine(x, ids, w, expert_weights, stream=stream)
+    if shared_gate_up is not None:
+        hidden = MoeLinear(x, shared_gate_up, activation="swiglu", stream=stream)
+        y = MoeLinear(hidden, shared_down, residual=y, stream=stream)
+    return y, ids, w, eo
 
 
 def synth_normal_f16_(out: torch.Tensor, seed: int, stream_id: int, sigma_a: float, sigma_b: float | None = None,

@@ -57,8 +57,10 @@ typedef enum moe_status {
 } moe_status;
 
 typedef enum moe_dtype {
-    MOE_DT_FLOAT16 = 1, /* ge::DT_FLOAT16 */
-    MOE_DT_INT32 = 3    /* ge::DT_INT32   */
+    MOE_DT_FLOAT32 = 0,  /* ge::DT_FLOAT   */
+    MOE_DT_FLOAT16 = 1,  /* ge::DT_FLOAT16 */
+    MOE_DT_INT32 = 3,    /* ge::DT_INT32   */
+    MOE_DT_BFLOAT16 = 27 /* ge::DT_BF16    */
 } moe_dtype;
 
 /* Human-readable name of a status code. */
@@ -239,6 +241,86 @@ moe_status moe_layer(const uint16_t* x, const uint16_t* w_gate, const uint16_t* 
                      int32_t* expert_ids, uint16_t* weights, uint16_t* expert_out, uint16_t* y, void* workspace,
                      size_t workspace_bytes, int64_t num_tokens, int64_t hidden_size, int64_t num_experts,
                      int64_t top_k, int64_t intermediate_size, void* stream);
+
+/* ======================================================================================================
+ * Operators around the routed experts. The reference has none of them: they are what a layer with scored and
+ * grouped routing, a dense expert beside the routed ones, or a training step of its router needs next to the
+ * three operators above. Tensors, streams, workspaces and errors as there.
+ * ==================================================================================================== */
+
+typedef enum moe_scoring { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 } moe_scoring;
+
+typedef enum moe_activation {
+    MOE_ACT_NONE = 0,
+    MOE_ACT_RELU = 1,
+    MOE_ACT_GELU = 2,      /* z/2 (1 + erf(z / sqrt 2))                              */
+    MOE_ACT_GELU_TANH = 3, /* z/2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3)))        */
+    MOE_ACT_SILU = 4,      /* z / (1 + exp(-z))                                      */
+    MOE_ACT_SWIGLU = 5     /* silu(gate) * up: 2 N weight rows, the N gate rows first */
+} moe_activation;
+
+/* ------------------------------------------------------------------------------------------------------
+ * MoeRoutingGroupTopK: logits[T, E] (float32, float16 or bfloat16, rows logits_stride >= E elements apart),
+ *   bias[E] float32 or NULL -> expert_ids[T, K] int32, weights[T, K] (float16 or float32).
+ *   s = softmax or sigmoid of a row, c = s + bias. The groups are E / groups consecutive experts; a group's score is
+ *   its best c (group_top 1) or the sum of its two best (group_top 2), and only the top_groups best groups stay (equal
+ *   scores: the lower group). expert_ids are the K best c of the experts that stay, in descending order (equal
+ *   c: the lower index). weights = scale * s, divided by the sum of the K chosen s where renormalize is set
+ *   (the ratios hold where the scores themselves would underflow). bias only steers the choice.
+ *   c is compared in float64. An expert whose logit or c is NaN or -infinity is not available; where a row has fewer
+ *   than K available ones the picks left are id -1 and weight 0, which moe_expert_ffn computes as zero rows.
+ *   1 <= K <= top_groups * E / groups, E <= 256.
+ * ---------------------------------------------------------------------------------------------------- */
+moe_status moe_routing_group_topk(const void* logits, int64_t logits_stride, int32_t logits_type, const float* bias,
+                                  int32_t* expert_ids, void* weights, int32_t weights_type, int64_t num_tokens,
+                                  int64_t num_experts, int64_t top_k, int64_t groups, int64_t top_groups,
+                                  int64_t group_top, int32_t scoring, int32_t renormalize, float scale, void* stream);
+
+/* Its gradient: grad_weights[T, K] (float32, float16 or bfloat16), the same logits and the expert_ids it chose ->
+ * grad_logits[T, E] contiguous, of logits_type. The choice itself has no gradient, so bias has none. Ids outside
+ * [0, E) and unavailable experts receive nothing; an id that a row holds twice receives both. Any K in [1, E]. */
+moe_status moe_routing_group_topk_grad(const void* grad_weights, int32_t weights_type, const void* logits,
+                                       int64_t logits_stride, int32_t logits_type, const int32_t* expert_ids,
+                                       void* grad_logits, int64_t num_tokens, int64_t num_experts, int64_t top_k,
+                                       int32_t scoring, int32_t renormalize, float scale, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * MoeCombineGrad: grad_y[T, H], expert_out[T, K, H], weights[T, K] fp16 -> grad_expert_out[T, K, H] =
+ *   weights * grad_y, grad_weights[T, K] = <grad_y, expert_out> (fp32 sums), both fp16. H a multiple of 8.
+ * ---------------------------------------------------------------------------------------------------- */
+moe_status moe_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, const uint16_t* weights,
+                            uint16_t* grad_expert_out, uint16_t* grad_weights, int64_t num_tokens,
+                            int64_t hidden_size, int64_t top_k, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * MoeLinear: x[T, H], weight[N, H] (SwiGLU: [2N, H]) -> y[T, N] = act(x weight^T + bias) + residual, fp32 sums, rounded
+ *   once. x and weight are float16 or bfloat16 (dtype); x rows lie x_stride elements apart. weight's rows lie
+ *   weight_stride apart; with weight_transposed set it is stored [H, N] with weight_stride between the H rows, as
+ *   MoeRoutingTopK's w_gate. bias[N] (SwiGLU: [2N]) of dtype, or NULL; residual[T, N] of out_dtype, or NULL; out_dtype
+ *   is dtype or float32. pre, if not NULL, receives the sums before the activation, [T, N] (SwiGLU: [T, 2N]) of dtype,
+ *   which moe_linear_grad takes. Any sizes from 1; N, H <= 2^20.
+ *   Operands that 16-byte copies can read (16-byte aligned, strides multiples of 8, H a multiple of 8; SwiGLU with a
+ *   transposed weight: N too) run at full speed, others are loaded element by element.
+ *   The workspace (moe_linear_workspace_bytes, may be 0) holds fp32 partial sums of a product split over H; calls in
+ *   flight at the same time need one each. Deterministic; nothing depends on timing.
+ * ---------------------------------------------------------------------------------------------------- */
+size_t moe_linear_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
+moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                      int32_t weight_transposed, const void* bias, const void* residual, void* y, void* pre,
+                      void* workspace, size_t workspace_bytes, int64_t num_tokens, int64_t n, int64_t hidden_size,
+                      int32_t activation, int32_t dtype, int32_t out_dtype, void* stream);
+
+/* MoeLinearGrad: grad_y[T, N] of dtype (rows grad_y_stride apart) and what moe_linear had -> grad_x[T, H],
+ * grad_weight[N, H] (SwiGLU: [2N, H]) and grad_bias, contiguous, of dtype; each may be NULL (not wanted). pre is
+ * moe_linear's (not read without an activation). dz = grad_y * act'(pre) is rounded to dtype for the two products
+ * grad_x = dz weight and grad_weight = dz^T x; grad_bias sums it before that. residual's gradient is grad_y.
+ * With T = 0 grad_weight and grad_bias are zeros. */
+size_t moe_linear_grad_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
+moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
+                           const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
+                           void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                           int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation, int32_t dtype,
+                           void* stream);
 
 #ifdef __cplusplus
 }
