@@ -118,6 +118,8 @@ hipError_t run_product(moe::GemmArgs g, const ProductPlan& plan, void* partial, 
     g.partial = static_cast<float*>(partial);
     g.splits = plan.splits;
     g.split_k = static_cast<int>(plan.split_k);
+    const int64_t tiles = (g.m + 255) / 256 * ((g.n + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256));
+    if (direct && plan.splits == 1 && tiles >= 128) return moe::launch_gemm_tiled(g, p_by_k, q_by_k, bf16, stream);
     hipError_t err = moe::launch_gemm_mid(g, p_by_k, q_by_k, bf16, direct, plan.bm, stream);
     if (err == hipSuccess && plan.splits > 1) err = moe::launch_gemm_reduce(g, bf16, stream);
     return err;

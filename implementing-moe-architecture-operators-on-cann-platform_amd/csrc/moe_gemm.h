@@ -67,13 +67,23 @@ __device__ __forceinline__ float activate(float z, int act) {
     }
 }
 
-// 4 consecutive columns col .. col + 3 of one output row (those below n; `vec`: rows start on whole vectors, so four
-// valid columns are one access), from the sums z (SwiGLU: of the gate) and u (of the up rows).
+__device__ __forceinline__ f32x4 activate4(f32x4 z, int act) {
+    if (act == kActNone) return z;
+    return f32x4{activate(z[0], act), activate(z[1], act), activate(z[2], act), activate(z[3], act)};
+}
+
+// Two fp32 pairs as 16-bit values, each rounded to nearest even
+template <typename T>
+__device__ __forceinline__ uint2 pack4(f32x4 y) {
+    return make_uint2(T::store(y[0]) | (static_cast<uint32_t>(T::store(y[1])) << 16),
+                      T::store(y[2]) | (static_cast<uint32_t>(T::store(y[3])) << 16));
+}
+
+// The epilogue of 4 consecutive columns col .. col + 3 of one output row, the first `valid` of which exist: bias, the sums
+// before the activation stored, activation, residual. z: the sums (SwiGLU: the gate's, u the up rows'). `whole`: all
+// four are there and aligned, so they are one access.
 template <typename T, bool SWIGLU>
-__device__ __forceinline__ void store4(const GemmArgs& g, int64_t row, int col, f32x4 z, f32x4 u, bool vec) {
-    if (col >= g.n) return;
-    const int valid = min(4, g.n - col);
-    const bool whole = vec && valid == 4;
+__device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col, int valid, bool whole, f32x4 z, f32x4 u) {
     if (g.bias) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -85,45 +95,63 @@ __device__ __forceinline__ void store4(const GemmArgs& g, int64_t row, int col, 
     }
     if (g.pre) {
         uint16_t* pz = g.pre + row * (SWIGLU ? 2 * static_cast<int64_t>(g.n) : g.n) + col;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (r < valid) {
+        if (whole && (reinterpret_cast<uintptr_t>(g.pre) & 7) == 0) {
+            *reinterpret_cast<uint2*>(pz) = pack4<T>(z);
+            if (SWIGLU) *reinterpret_cast<uint2*>(pz + g.n) = pack4<T>(u);
+        } else {
+            for (int r = 0; r < valid; ++r) {
                 pz[r] = T::store(z[r]);
                 if (SWIGLU) pz[g.n + r] = T::store(u[r]);
             }
         }
     }
-    float y[4];
+    f32x4 y;
+    if (SWIGLU) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = SWIGLU ? swiglu_f32(z[r], u[r]) : activate(z[r], g.act);
+        for (int r = 0; r < 4; ++r) y[r] = swiglu_f32(z[r], u[r]);
+    } else {
+        y = activate4(z, g.act);
+    }
+    if (!g.residual) return y;
     const int64_t at = row * g.n + col;
     if (g.out_f32) {
-        const float* res = static_cast<const float*>(g.residual);
-        float* out = static_cast<float*>(g.out) + at;
-        if (whole) {
-            f32x4 v = {y[0], y[1], y[2], y[3]};
-            if (res) v += *reinterpret_cast<const f32x4*>(res + at);
-            *reinterpret_cast<f32x4*>(out) = v;
-        } else {
-            for (int r = 0; r < valid; ++r) out[r] = res ? y[r] + res[at + r] : y[r];
-        }
+        const float* res = static_cast<const float*>(g.residual) + at;
+        if (whole) return y + *reinterpret_cast<const f32x4*>(res);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < valid) y[r] += res[r];
     } else {
-        const uint16_t* res = static_cast<const uint16_t*>(g.residual);
-        uint16_t* out = static_cast<uint16_t*>(g.out) + at;
+        const uint16_t* res = static_cast<const uint16_t*>(g.residual) + at;
         if (whole) {
-            if (res) {
-                const uint2 v = *reinterpret_cast<const uint2*>(res + at);
-                y[0] += T::load(static_cast<uint16_t>(v.x));
-                y[1] += T::load(static_cast<uint16_t>(v.x >> 16));
-                y[2] += T::load(static_cast<uint16_t>(v.y));
-                y[3] += T::load(static_cast<uint16_t>(v.y >> 16));
-            }
-            *reinterpret_cast<uint2*>(out) =
-                make_uint2(T::store(y[0]) | (static_cast<uint32_t>(T::store(y[1])) << 16),
-                           T::store(y[2]) | (static_cast<uint32_t>(T::store(y[3])) << 16));
-        } else {
-            for (int r = 0; r < valid; ++r) out[r] = T::store(res ? y[r] + T::load(res[at + r]) : y[r]);
+            const uint2 v = *reinterpret_cast<const uint2*>(res);
+            return f32x4{y[0] + T::load(static_cast<uint16_t>(v.x)), y[1] + T::load(static_cast<uint16_t>(v.x >> 16)),
+                         y[2] + T::load(static_cast<uint16_t>(v.y)), y[3] + T::load(static_cast<uint16_t>(v.y >> 16))};
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < valid) y[r] += T::load(res[r]);
+    }
+    return y;
+}
+
+// The same, written to out; columns from n on are left alone. `vec`: whole vectors are aligned (vector_rows).
+template <typename T, bool SWIGLU>
+__device__ __forceinline__ void store4(const GemmArgs& g, int64_t row, int col, f32x4 z, f32x4 u, bool vec) {
+    if (col >= g.n) return;
+    const int valid = min(4, g.n - col);
+    const bool whole = vec && valid == 4;
+    const f32x4 y = finish4<T, SWIGLU>(g, row, col, valid, whole, z, u);
+    const int64_t at = row * g.n + col;
+    if (g.out_f32) {
+        float* out = static_cast<float*>(g.out) + at;
+        if (whole) *reinterpret_cast<f32x4*>(out) = y;
+        else
+            for (int r = 0; r < valid; ++r) out[r] = y[r];
+    } else {
+        uint16_t* out = static_cast<uint16_t*>(g.out) + at;
+        if (whole) *reinterpret_cast<uint2*>(out) = pack4<T>(y);
+        else
+            for (int r = 0; r < valid; ++r) out[r] = T::store(y[r]);
     }
 }
 
@@ -134,14 +162,64 @@ __host__ __device__ __forceinline__ bool vector_rows(const GemmArgs& g) {
 }
 
 // ds_read_b64_tr_b16: 8 bytes per lane, handed out transposed within each 16-lane group (lane i gets element i % 4 of
-// the 8 bytes addressed by lanes 4 j + i / 4, j = 0 .. 3)
-__device__ __forceinline__ s16x4 lds_read_transposed(const uint16_t* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+// the 8 bytes addressed by lanes 4 j + i / 4, j = 0 .. 3). An operand tile stored by k (64 k x 128 rows, 256 bytes a k) gives
+// a fragment of 16 rows and 32 k as two such reads, 4 k each. These read N fragments for both 32-k steps of a stage,
+// addr[n] being the lane's address at its first k. Inline assembly, with the wait in the same block: at the builtin the
+// compiler waits for every direct-to-LDS copy in flight (256 x 256 tiles, T = 8192: 1195 us with that wait).
+__device__ __forceinline__ void read_transposed(const uint32_t (&addr)[4], s16x8 (&f)[2][4]) {
+    s16x4 v[4][4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %4, %17\n\tds_read_b64_tr_b16 %5, %17 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %8, %18\n\tds_read_b64_tr_b16 %9, %18 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %12, %19\n\tds_read_b64_tr_b16 %13, %19 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %2, %16 offset:8192\n\tds_read_b64_tr_b16 %3, %16 offset:9216\n\t"
+        "ds_read_b64_tr_b16 %6, %17 offset:8192\n\tds_read_b64_tr_b16 %7, %17 offset:9216\n\t"
+        "ds_read_b64_tr_b16 %10, %18 offset:8192\n\tds_read_b64_tr_b16 %11, %18 offset:9216\n\t"
+        "ds_read_b64_tr_b16 %14, %19 offset:8192\n\tds_read_b64_tr_b16 %15, %19 offset:9216\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[0][2]), "=&v"(v[0][3]), "=&v"(v[1][0]), "=&v"(v[1][1]),
+          "=&v"(v[1][2]), "=&v"(v[1][3]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[2][2]), "=&v"(v[2][3]),
+          "=&v"(v[3][0]), "=&v"(v[3][1]), "=&v"(v[3][2]), "=&v"(v[3][3])
+        : "v"(addr[0]), "v"(addr[1]), "v"(addr[2]), "v"(addr[3])
+        : "memory");
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            f[kk][n] = __builtin_shufflevector(v[n][2 * kk], v[n][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ void read_transposed(const uint32_t (&addr)[2], s16x8 (&f)[2][2]) {
+    s16x4 v[2][4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %4, %9\n\tds_read_b64_tr_b16 %5, %9 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:8192\n\tds_read_b64_tr_b16 %3, %8 offset:9216\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:8192\n\tds_read_b64_tr_b16 %7, %9 offset:9216\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[0][2]), "=&v"(v[0][3]), "=&v"(v[1][0]), "=&v"(v[1][1]),
+          "=&v"(v[1][2]), "=&v"(v[1][3])
+        : "v"(addr[0]), "v"(addr[1])
+        : "memory");
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            f[kk][n] = __builtin_shufflevector(v[n][2 * kk], v[n][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// The lane's address in such a tile of the fragment of rows r0 .. r0 + 15 (r0 a multiple of 16) at the first k. The 32-byte
+// pairs of a k stand at pair ^ f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2, which depends on the lane alone here.
+__device__ __forceinline__ uint32_t transposed_address(const uint16_t* tile, int r0, int lane) {
+    const int kg = lane >> 4, j = (lane & 15) >> 2, q = lane & 3, f = (j | ((kg & 1) << 2)) << 1;
+    const uint16_t* p = tile + (kg * 8 + j) * 128 + (((r0 / 8 + (q >> 1)) ^ f) * 8) + (q & 1) * 4;
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)p));
 }
 
 // kernels' launches
 hipError_t launch_gemm_mid(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, bool direct, int bm,
                            hipStream_t stream);
+// 256 x 256 tiles; operands that 16-byte copies can read
+hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);
 
 }  // namespace moe

@@ -44,23 +44,22 @@ __device__ __forceinline__ Granule granule_of(int i, int lane) {
     return Granule{k, ((lane % kPer) ^ (f << 1)) * 8};
 }
 
-// Fragment of 16 operand rows from r0 on and 32 k from 32 kk on: lane (row16, kg) gets 8 k of row r0 + row16.
-template <bool BY_K, int ROWS>
-__device__ __forceinline__ s16x8 read_fragment(const uint16_t* tile, int r0, int kk, int lane) {
-    const int kg = lane >> 4;
-    if (!BY_K) {
-        const int r = r0 + (lane & 15);
-        return *reinterpret_cast<const s16x8*>(tile + r * kBK + (((kk * 4 + kg) ^ ((r >> 1) & 7)) * 8));
-    }
-    s16x4 h[2];
+// Fragments of N blocks of 16 operand rows from r0 on, both 32-k steps: lane (row16, kg) gets 8 k of one row.
+template <bool BY_K, int N>
+__device__ __forceinline__ void read_fragments(const uint16_t* tile, int r0, int lane, s16x8 (&f)[2][N]) {
+    if constexpr (BY_K) {
+        uint32_t addr[N];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int k = kk * 32 + kg * 8 + t * 4 + ((lane & 15) >> 2);
-        const int f = (k & 3) | (((k >> 3) & 1) << 2);
-        const int q = lane & 3;  // 4 rows = 8 bytes: granule r0 / 8 + q / 2, half q & 1
-        h[t] = lds_read_transposed(tile + k * ROWS + (((r0 / 8 + (q >> 1)) ^ (f << 1)) * 8) + (q & 1) * 4);
+        for (int n = 0; n < N; ++n) addr[n] = transposed_address(tile, r0 + n * 16, lane);
+        read_transposed(addr, f);
+    } else {
+        const int row16 = lane & 15, kg = lane >> 4, sw = (row16 >> 1) & 7;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                f[kk][n] = *reinterpret_cast<const s16x8*>(tile + (r0 + n * 16 + row16) * kBK + (((kk * 4 + kg) ^ sw) * 8));
     }
-    return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
 }
 
 // C[m][n] tile of BM x 128 (4 waves), one ring of direct-to-LDS stages, one barrier a stage.
@@ -193,18 +192,15 @@ __global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtil
         copy_stage(s + NS - 1);
         const uint16_t* tp = lds + (s % NS) * kSlot;
         const uint16_t* tq = tp + BM * kBK;
+        s16x8 fp[2][FM], fq[2][FN];
+        read_fragments<PK, FM>(tp, wm * (BM / WM), lane, fp);
+        read_fragments<QK, FN>(tq, wn * (kBN / WN), lane, fq);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            s16x8 fp[FM], fq[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fp[i] = read_fragment<PK, BM>(tp, wm * (BM / WM) + i * 16, kk, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fq[j] = read_fragment<QK, kBN>(tq, wn * (kBN / WN) + j * 16, kk, lane);
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int i = 0; i < FM; ++i) acc[j][i] = T::mfma(fq[j], fp[i], acc[j][i]);
-        }
+                for (int i = 0; i < FM; ++i) acc[j][i] = T::mfma(fq[kk][j], fp[kk][i], acc[j][i]);
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the surplus copies have landed before the workgroup ends
 

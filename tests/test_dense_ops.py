@@ -361,6 +361,85 @@ def test_linear_sizes(ops, dtype, act):
                      pre=n % 4 == 0, transposed=True, seed=n)
 
 
+def random_rows_check(ops, T, N, H, dtype, act, transposed, seed, rows=24, residual=False, out=None):
+    """A product too large for the CPU: every value against fp32 sums on the device, sampled rows against 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    Z = 2 * N if act == "swiglu" else N
+    x = torch.empty((T, H), dtype=dtype, device="cuda").normal_(generator=g)
+    w = torch.empty((H, Z) if transposed else (Z, H), dtype=dtype, device="cuda").normal_(0, H**-0.5, generator=g)
+    w = w.t() if transposed else w
+    b = torch.empty((Z,), dtype=dtype, device="cuda").normal_(generator=g)
+    out = out or dtype
+    r = torch.empty((T, N), dtype=out, device="cuda").normal_(generator=g) if residual else None
+    y, pre = ops.MoeLinear(x, w, b, r, act, out, True)
+    at = torch.randint(0, T, (rows,), generator=gen(seed))
+    at[0], at[1] = 0, T - 1
+    z = x[at.cuda()].double() @ w.double().t() + b.double()
+    zt = (H + 2) * U32 * (x[at.cuda()].double().abs() @ w.double().abs().t() + b.double().abs())
+    check(pre[at.cuda()], z.cpu(), (zt + half_step(z.abs() + zt, dtype)).cpu(), "pre")
+    ref = act_reference(z, act)
+    if act == "swiglu":
+        (gz, uz), (gt, ut) = z.chunk(2, dim=1), zt.chunk(2, dim=1)
+        tol = 1.1 * gt * (uz.abs() + ut) + gz.abs() * ut + FN * ref.abs()
+    else:
+        tol = 1.13 * zt + FN * z.abs()
+    if residual:
+        ref = ref + r[at.cuda()].double()
+        tol = tol + U32 * ref.abs()
+    check(y[at.cuda()], ref.cpu(), (tol + half_step(ref.abs() + tol, out)).cpu(), (T, N, H, act))
+    zf = x.float() @ w.float().t() + b.float()  # all values: two fp32 sums, each within 2 H 2^-24 of |x| |w|
+    # and a rounding; |x| |w| is below 2 sqrt(H) sigma for these distributions, so 2^-8 covers fp16 with room
+    yf = act_reference(zf, act) + (0 if r is None else r.float())
+    err = (y.float() - yf).abs()
+    assert (err <= 2.0**-6 + torch.finfo(dtype).eps * yf.abs()).all(), (T, N, H, act, float(err.max()))
+    return y
+
+
+@gpu
+@pytest.mark.parametrize("T,N,H,act,transposed,out", [
+    (4096, 2048, 64, "none", False, None), (4097, 2056, 72, "gelu", False, None), (2049, 4104, 128, "silu", True, None),
+    (3001, 3000, 200, "relu", False, F32), (8191, 1400, 136, "swiglu", False, None), (4099, 1032, 1000, "swiglu", True, None),
+    (33000, 264, 520, "gelu_tanh", True, F32), (260, 33000, 96, "none", False, None), (2300, 2306, 1544, "none", False, None)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_linear_large_tiles(ops, dtype, T, N, H, act, transposed, out):
+    print(f"[linear large] {T} {N} {H} {act} {transposed} {dtype}", flush=True)
+    random_rows_check(ops, T, N, H, dtype, act, transposed, T + N, residual=N % 16 == 8, out=out)
+
+
+@gpu
+@pytest.mark.parametrize("T,N,H,act,transposed", [
+    (4097, 2056, 2056, "none", False), (2049, 2100, 4104, "silu", True), (8200, 1032, 2048, "swiglu", False),
+    (100, 4100, 4096, "gelu", False)])
+def test_linear_gradient_large_tiles(ops, T, N, H, act, transposed):
+    print(f"[linear grad large] {T} {N} {H} {act} {transposed}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    Z = 2 * N if act == "swiglu" else N
+    new = lambda shape, s: torch.empty(shape, dtype=F16, device="cuda").normal_(0, s, generator=g)  # noqa: E731
+    dy, x, w = new((T, N), 1), new((T, H), 1), new((Z, H), H**-0.5)
+    pre = None if act == "none" else new((T, Z), 1)
+    gx, gw, gb = ops.MoeLinearGrad(dy, x, w.t().contiguous().t() if transposed else w, pre, act, gradBias=True)
+    dz = dy.double()
+    if pre is not None:
+        z = pre.double().requires_grad_(True)
+        dz, = torch.autograd.grad(act_reference(z, act), z, dz)
+    dzt = 2 * half_step(dz, F16) + 2.0**-20 * (0 if pre is None else 1)
+    rows = torch.tensor([0, 1, T // 2, T - 1], device="cuda")
+    cols = torch.tensor([0, Z // 2 - 1, Z // 2, Z - 1], device="cuda")
+    wd, xd = w.double(), x.double()
+    ref = dz[rows] @ wd
+    tol = dzt[rows] @ wd.abs() + Z * U32 * (dz[rows].abs() @ wd.abs())
+    check(gx[rows], ref.cpu(), (tol + half_step(ref.abs() + tol, F16)).cpu(), "grad_x")
+    ref = dz[:, cols].t() @ xd
+    tol = dzt[:, cols].t() @ xd.abs() + T * U32 * (dz[:, cols].abs().t() @ xd.abs())
+    check(gw[cols], ref.cpu(), (tol + half_step(ref.abs() + tol, F16)).cpu(), "grad_weight")
+    for got, ref in ((gx, dz.float() @ w.float()), (gw, dz.t().float() @ x.float())):  # every value, loosely
+        assert ((got.float() - ref).norm() / ref.norm()) < 3 * 2.0**-11
+        assert ((got.float() - ref).abs() <= 2.0**-5 * ref.abs() + 2.0**-4 * ref.square().mean().sqrt()).all()
+    ref = dz.sum(dim=0)
+    tol = (T + 1) * U32 * dz.abs().sum(dim=0) + T * 2.0**-20
+    check(gb, ref.cpu(), (tol + half_step(ref.abs() + tol, F16)).cpu(), "grad_bias")
+
+
 @gpu
 def test_linear_strides_and_alignment(ops):
     """Rows of wider tensors, bases off 16 bytes, rows off 16 bytes, a transposed view: the same values as contiguous."""
