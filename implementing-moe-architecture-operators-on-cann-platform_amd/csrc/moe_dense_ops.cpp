@@ -183,6 +183,8 @@ moe_status moe_routing_group_topk(const void* logits, int64_t logits_stride, int
     r.groups = static_cast<int>(groups);
     r.top_groups = static_cast<int>(top_groups);
     r.group_top = static_cast<int>(group_top);
+    const int size = static_cast<int>(E / groups);
+    r.size_inverse = (65536 + size - 1) / size;
     r.sigmoid = scoring == MOE_SCORE_SIGMOID;
     r.renormalize = renormalize != 0;
     r.scale = scale;

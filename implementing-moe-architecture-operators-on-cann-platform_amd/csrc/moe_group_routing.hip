@@ -5,8 +5,17 @@
 //   groups of E / G consecutive experts, each scored by its best c or the sum of its two best; the best topGroups stay
 //   the K best c among them in descending order, ties to the lowest index; w = scale * s, over the K's sum if asked
 // An expert whose logit or c is NaN or -inf is not available; picks with no expert left are id -1, weight 0.
-// c is compared in float64: fp32 scores that agree to their last bit would be picked in an order that depends on how
-// the exponential was rounded.
+//
+// The choice is the definition's, not fp32's: without a bias experts are compared by their logits, which order the scores
+// exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where two neighbours among a row's picks
+// are nearer than that, they are put in order by their float64 values (some rows in a thousand); where the last pick
+// and the best expert left, or the last group that stays and the first that does not, are, the whole row is chosen again
+// in float64 by the wave.
+//
+// A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers. A
+// pick is the maximum over the lane (max3), over the row (4 DPP steps), the lowest index that has it (4 more) and its
+// removal: ~80 instructions for 4 tokens, which bounds the kernel, not the logits' bytes. Group scores go through LDS,
+// one lane per (token, group).
 #include "moe_device.h"
 #include "moe_launch.h"
 #include "moe_ops.h"
@@ -17,10 +26,11 @@ namespace moe {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kLanes = 16;                     // lanes of one token
-constexpr int kTokens = kThreads / kLanes;     // tokens of a workgroup
+constexpr int kLanes = 16;                   // lanes of one token
+constexpr int kWaveTokens = kWave / kLanes;  // tokens of a workgroup, one wave
 constexpr int kMaxE = 256;
+constexpr int kGone = -2147483647 - 1;         // the key of an expert that is not available or was picked
+constexpr float kLow = -__builtin_huge_valf();
 constexpr double kNone = -__builtin_huge_val();
 
 template <typename L>
@@ -55,15 +65,21 @@ __device__ __forceinline__ void put<B16>(void* p, int64_t i, float v) {
     static_cast<uint16_t*>(p)[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
 }
 
-template <typename V>
-__device__ __forceinline__ V row_max(V v) {
+// 4 consecutive logits, aligned
+template <typename L>
+__device__ __forceinline__ void load4(const void* p, int64_t i, float* v) {
+    if constexpr (std::is_same_v<L, F32>) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+        v[0] = x[0], v[1] = x[1], v[2] = x[2], v[3] = x[3];
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+        const uint16_t b[4] = {static_cast<uint16_t>(x.x), static_cast<uint16_t>(x.x >> 16), static_cast<uint16_t>(x.y),
+                               static_cast<uint16_t>(x.y >> 16)};
 #pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) {
-        const V o = __shfl_xor(v, d, kLanes);
-        v = o > v ? o : v;
+        for (int j = 0; j < 4; ++j) v[j] = logit<L>(b, j);
     }
-    return v;
 }
+
 template <typename V>
 __device__ __forceinline__ V row_sum(V v) {
 #pragma unroll
@@ -71,260 +87,583 @@ __device__ __forceinline__ V row_sum(V v) {
     return v;
 }
 
-// LDS: c [kTokens][E], group scores [kTokens][G] (double), picked scores [kTokens][K] (double), picks [kTokens][K]
-// (int), kept groups [kTokens][G] (int)
-int routing_lds(int E, int G, int K) { return kTokens * (E * 8 + G * 8 + K * 8 + K * 4 + G * 4); }
+// All-reduce over a DPP row of 16 lanes by rotations
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ int row_max_i(int v) {
+    v = max(v, dpp<0x128>(v));
+    v = max(v, dpp<0x124>(v));
+    v = max(v, dpp<0x122>(v));
+    return max(v, dpp<0x121>(v));
+}
+__device__ __forceinline__ int row_min_i(int v) {
+    v = min(v, dpp<0x128>(v));
+    v = min(v, dpp<0x124>(v));
+    v = min(v, dpp<0x122>(v));
+    return min(v, dpp<0x121>(v));
+}
+__device__ __forceinline__ float row_sum_f(float v) {
+    v += __builtin_bit_cast(float, dpp<0x128>(__builtin_bit_cast(int, v)));
+    v += __builtin_bit_cast(float, dpp<0x124>(__builtin_bit_cast(int, v)));
+    v += __builtin_bit_cast(float, dpp<0x122>(__builtin_bit_cast(int, v)));
+    return v + __builtin_bit_cast(float, dpp<0x121>(__builtin_bit_cast(int, v)));
+}
 
-// C: experts of a lane (lane, lane + 16, ...), at most
+// Floats as integers in the same order (-0 as 0); key_value undoes it
+__device__ __forceinline__ int key_of(float v) {
+    const int b = __builtin_bit_cast(int, v + 0.0f);
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float key_value(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
+
+// Two fp32 values of c (or sums of two) that are nearer than this may stand the other way round. With e = 2^-24: exp2 and
+// rcp are within 2 e, the argument's rounding moves e^-l by |l| 1.5 e relative and s (1 - s) |l| < 0.23, so a sigmoid is
+// within 8 e; a softmax score, with a sum of 20 roundings, within 64 e of the row's largest score; adding the bias, or two
+// c, rounds by e |c|. The limit is four such errors.
+__device__ __forceinline__ float gap_limit(bool sigmoid, float s_max, float c) {
+    return (sigmoid ? 32.0f : 256.0f * s_max) * 0x1p-24f + fabsf(c) * 0x1p-21f;
+}
+
+// LDS of the one wave of a workgroup
+struct RoutingLds {
+    int E, G, K;
+    __host__ __device__ int pitch() const { return (E + 3) / 4 * 4 + 4; }
+    __host__ __device__ int picks_at() const { return 8 * kWaveTokens * K; }                 // after the parts (double)
+    __host__ __device__ int scores_at() const { return picks_at() + 4 * kWaveTokens * K; }   // group scores: doubles
+    __host__ __device__ int kept_at() const { return scores_at() + 8 * kWaveTokens * G; }
+    __host__ __device__ int cut_at() const { return kept_at() + 4 * kWaveTokens * G; }
+    // c of the row's experts: floats of 4 tokens, or doubles of one
+    __host__ __device__ int row_at() const { return (cut_at() + 8 * kWaveTokens + 15) / 16 * 16; }
+    __host__ __device__ int bytes() const { return row_at() + 4 * kWaveTokens * pitch(); }
+};
+
+// Expert of lane l's register j: 16-byte (8-byte) pieces of 4 consecutive experts
+template <int C>
+__device__ __forceinline__ int expert_of(int l, int j) {
+    constexpr int V = C < 4 ? C : 4;
+    return j / V * (kLanes * V) + l * V + j % V;
+}
+
+// Lane l's logits of the row that starts at element `at`; -inf past E
+template <typename L, int C, bool VEC>
+__device__ __forceinline__ void load_logits(const void* p, int64_t at, int E, int l, float (&v)[C]) {
+    if constexpr (VEC && C >= 4) {
+#pragma unroll
+        for (int j = 0; j < C; j += 4) {
+            const int e = expert_of<C>(l, j);
+            if (e < E) {  // E % 4 == 0
+                load4<L>(p, at + e, &v[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[j + i] = kLow;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int e = expert_of<C>(l, j);
+            v[j] = e < E ? logit<L>(p, at + e) : kLow;
+        }
+    }
+}
+
+// The choice of one row in float64 by the whole wave: picks [K], -1 where no expert is left
 template <typename L, int C>
-__global__ __launch_bounds__(kThreads) void group_routing_kernel(GroupRouting r, int32_t* __restrict__ ids,
-                                                                 void* __restrict__ weights) {
-    extern __shared__ __align__(16) char shared[];
-    const int E = r.E, G = r.groups, K = r.K, size = E / G;
-    double* cs = reinterpret_cast<double*>(shared);
-    double* gs = cs + kTokens * E;
-    double* ps = gs + kTokens * G;
-    int* pick = reinterpret_cast<int*>(ps + kTokens * K);
-    int* kept = pick + kTokens * K;
-    const int tid = static_cast<int>(threadIdx.x), tok = tid / kLanes, l = tid % kLanes;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + tok;
-    const bool valid = t < r.T;
-
-    double s[C], c[C], lg[C];  // scores, what is compared, logits
-    bool open[C];
+__device__ void choose_exactly(const GroupRouting& r, int64_t t, int* pick, double* gs, int* kept, double* cs) {
+    constexpr int C64 = (C + 3) / 4;
+    const int lane = lane_id(), E = r.E, G = r.groups, size = E / G;
+    double s[C64], c[C64];
+    bool open[C64];
     double top = kNone;
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-        const int e = l + j * kLanes;
-        double v = kNone;
-        if (valid && e < E) v = static_cast<double>(logit<L>(r.logits, t * r.ld + e));
-        open[j] = v > kNone;  // false for NaN too
-        lg[j] = s[j] = v;
-        if (open[j] && v > top) top = v;
+    for (int j = 0; j < C64; ++j) {
+        const int e = lane + j * kWave;
+        s[j] = e < E ? static_cast<double>(logit<L>(r.logits, t * r.ld + e)) : kNone;
+        c[j] = s[j];
+        open[j] = s[j] > kNone;  // false for NaN too
+        if (open[j]) top = fmax(top, s[j]);
     }
     if (r.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < C; ++j) s[j] = open[j] ? 1.0 / (1.0 + exp(-s[j])) : 0.0;
+        for (int j = 0; j < C64; ++j) s[j] = open[j] ? 1.0 / (1.0 + exp(-s[j])) : 0.0;
     } else {
-        top = row_max(top);
+#pragma unroll
+        for (int d = kWave / 2; d > 0; d >>= 1) top = fmax(top, __shfl_xor(top, d, kWave));
         double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
+        for (int j = 0; j < C64; ++j) {
             s[j] = open[j] ? (s[j] == top ? 1.0 : exp(s[j] - top)) : 0.0;
             sum += s[j];
         }
-        sum = row_sum(sum);
 #pragma unroll
-        for (int j = 0; j < C; ++j) s[j] = open[j] ? s[j] / sum : 0.0;
+        for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, kWave);
+#pragma unroll
+        for (int j = 0; j < C64; ++j) s[j] = open[j] ? s[j] / sum : 0.0;
     }
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-        const int e = l + j * kLanes;
-        c[j] = kNone;
-        if (open[j]) {
-            c[j] = r.bias ? s[j] + static_cast<double>(r.bias[e]) : s[j];
-            if (!(c[j] > kNone)) c[j] = kNone;
-        }
+    for (int j = 0; j < C64; ++j) {
+        const int e = lane + j * kWave;
+        if (open[j] && r.bias) c[j] = s[j] + static_cast<double>(r.bias[e]);
+        if (!open[j] || !(c[j] > kNone)) c[j] = kNone;
     }
     if (r.top_groups < G) {
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            const int e = l + j * kLanes;
-            if (e < E) cs[tok * E + e] = c[j];
+        for (int j = 0; j < C64; ++j) {
+            const int e = lane + j * kWave;
+            // two best scores are added; one best is compared, by the logits where there is no bias
+            if (e < E) cs[e] = c[j] > kNone ? (r.group_top == 2 && !r.bias ? s[j] : c[j]) : kNone;
         }
         __syncthreads();
-        for (int i = tid; i < kTokens * G; i += kThreads) {
-            const double* row = cs + (i / G) * E + (i % G) * size;
+        for (int g = lane; g < G; g += kWave) {
             double a = kNone, b = kNone;
-            for (int e = 0; e < size; ++e) {
-                const double v = row[e];
-                if (v > a) {
-                    b = a;
-                    a = v;
-                } else if (v > b) {
-                    b = v;
-                }
+            for (int e = g * size; e < (g + 1) * size; ++e) {
+                b = fmax(b, fmin(a, cs[e]));
+                a = fmax(a, cs[e]);
             }
-            gs[i] = r.group_top == 2 && b > kNone ? a + b : a;
+            gs[g] = r.group_top == 2 && b > kNone ? a + b : a;
         }
         __syncthreads();
-        for (int i = tid; i < kTokens * G; i += kThreads) {
-            const double* row = gs + i / G * G;
-            const int me = i % G;
-            const double v = row[me];
+        for (int g = lane; g < G; g += kWave) {
             int before = 0;
-            for (int o = 0; o < G; ++o) before += row[o] > v || (row[o] == v && o < me);
-            kept[i] = before < r.top_groups;
+            for (int o = 0; o < G; ++o) before += gs[o] > gs[g] || (gs[o] == gs[g] && o < g);
+            kept[g] = before < r.top_groups;
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            const int e = l + j * kLanes;
-            if (e < E && !kept[tok * G + e / size]) c[j] = kNone;
+        for (int j = 0; j < C64; ++j) {
+            const int e = lane + j * kWave;
+            if (e < E && !kept[e / size]) c[j] = kNone;
         }
     }
-    for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < r.K; ++k) {
         double best = kNone;
         int at = kMaxE;
 #pragma unroll
-        for (int j = 0; j < C; ++j)
+        for (int j = 0; j < C64; ++j)
             if (c[j] > best) {  // ascending e: the lowest index of equals stays
                 best = c[j];
-                at = l + j * kLanes;
+                at = lane + j * kWave;
             }
 #pragma unroll
-        for (int d = kLanes / 2; d > 0; d >>= 1) {
-            const double ob = __shfl_xor(best, d, kLanes);
-            const int oa = __shfl_xor(at, d, kLanes);
+        for (int d = kWave / 2; d > 0; d >>= 1) {
+            const double ob = __shfl_xor(best, d, kWave);
+            const int oa = __shfl_xor(at, d, kWave);
             if (ob > best || (ob == best && oa < at)) {
                 best = ob;
                 at = oa;
             }
         }
-        if (at == kMaxE) {
-            if (l == 0) {
-                pick[tok * K + k] = -1;
-                ps[tok * K + k] = r.renormalize ? kNone : 0.0;
-            }
-        } else {
+        if (lane == 0) pick[k] = at == kMaxE ? -1 : at;
 #pragma unroll
-            for (int j = 0; j < C; ++j)
-                if (l + j * kLanes == at) {
-                    pick[tok * K + k] = at;
-                    ps[tok * K + k] = r.renormalize ? lg[j] : s[j];
-                    c[j] = kNone;
-                }
+        for (int j = 0; j < C64; ++j)
+            if (lane + j * kWave == at) c[j] = kNone;
+    }
+}
+
+// C: experts of a lane. VEC: rows allow loads of 4 experts.
+template <typename L, int C, bool VEC>
+__global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, int32_t* __restrict__ ids,
+                                                              void* __restrict__ weights) {
+    extern __shared__ __align__(16) char shared[];
+    const int E = r.E, G = r.groups, K = r.K, size = E / G;
+    const RoutingLds lay{E, G, K};
+    double* parts = reinterpret_cast<double*>(shared);
+    int* pick = reinterpret_cast<int*>(shared + lay.picks_at());
+    float* gs = reinterpret_cast<float*>(shared + lay.scores_at());
+    int* kept = reinterpret_cast<int*>(shared + lay.kept_at());
+    float* cut = reinterpret_cast<float*>(shared + lay.cut_at());  // [token][2]: last score that stays, first that does not
+    float* row = reinterpret_cast<float*>(shared + lay.row_at());
+    const int lane = lane_id(), tok = lane / kLanes, l = lane % kLanes;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaveTokens + tok;
+    const bool valid = t < r.T;
+
+    float v[C];  // logits, -inf where not available
+    if (valid) {
+        load_logits<L, C, VEC>(r.logits, t * r.ld, E, l, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] = kLow;
+    }
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] = v[j] > kLow ? v[j] : kLow;  // NaN too
+    const bool grouped = r.top_groups < G;
+    const bool all_softmax = !r.sigmoid && !r.renormalize;  // weights over the whole row
+    const bool scored = r.bias || (grouped && r.group_top == 2);
+    float top = 0.0f, sum = 1.0f, s_max = 1.0f;
+    if (!r.sigmoid && (scored || all_softmax)) {
+        int m = key_of(v[0]);
+#pragma unroll
+        for (int j = 1; j < C; ++j) m = max(m, key_of(v[j]));
+        top = key_value(row_max_i(m));
+    }
+    int key[C];
+    float s[C];
+    if (scored || all_softmax) {
+        if (r.sigmoid) {
+#pragma unroll
+            for (int j = 0; j < C; ++j)  // 0 for -inf
+                s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v[j] * -1.4426950408889634f));
+        } else {
+            sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const float d = v[j] == top ? 0.0f : v[j] - top;
+                s[j] = v[j] > kLow ? __builtin_amdgcn_exp2f(d * 1.4426950408889634f) : 0.0f;
+                sum += s[j];
+            }
+            sum = row_sum_f(sum);
+            s_max = sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 1.0f;
+#pragma unroll
+            for (int j = 0; j < C; ++j) s[j] *= s_max;
         }
     }
-    __syncthreads();
-    if (!valid) return;
-    // Renormalised, the scores are taken relative to the largest of the picks: their ratios hold where the scores
-    // themselves would underflow.
-    const double* p = ps + tok * K;
-    double ref = kNone, sum = 0.0;
-    auto part = [&](double v) {
-        if (!(v > kNone)) return 0.0;
-        if (r.sigmoid) return exp(fmin(v, 0.0) - ref) / (1.0 + exp(-fabs(v)));
-        return v == ref ? 1.0 : exp(v - ref);
-    };
-    if (r.renormalize) {
-        for (int k = 0; k < K; ++k) ref = fmax(ref, r.sigmoid ? fmin(p[k], 0.0) : p[k]);
-        for (int k = 0; k < K; ++k) sum += part(p[k]);
+    if (r.bias) {
+        float b[C];
+        load_logits<F32, C, VEC>(r.bias, 0, E, l, b);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const float c = s[j] + b[j];
+            key[j] = v[j] > kLow && c > kLow ? key_of(c) : kGone;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) key[j] = v[j] > kLow ? key_of(v[j]) : kGone;
     }
+    bool again = false;  // fp32 does not settle this row's order
+    if (grouped) {
+        const bool by_score = r.group_top == 2 && !r.bias;
+        auto entry = [&](int j) { return key[j] == kGone ? kLow : by_score ? s[j] : key_value(key[j]); };
+        float* out = row + tok * lay.pitch();
+#pragma unroll
+        for (int j = 0; j < C; j += (C < 4 ? 1 : 4)) {  // a row's end may be written past E: the pitch has room
+            const int e = expert_of<C>(l, j);
+            if constexpr (C < 4) {
+                if (e < E) out[e] = entry(j);
+            } else if (e < E) {
+                *reinterpret_cast<f32x4*>(out + e) = f32x4{entry(j), entry(j + 1), entry(j + 2), entry(j + 3)};
+            }
+        }
+        __syncthreads();
+        for (int i = lane; i < kWaveTokens * G; i += kWave) {
+            const int q = i / G, g = i - q * G;
+            const float* c = row + q * lay.pitch() + g * size;
+            float a = kLow, b = kLow;
+            auto take = [&](float x) {
+                b = fmaxf(b, fminf(a, x));
+                a = fmaxf(a, x);
+            };
+            if (size % 4 == 0) {
+#pragma unroll 4
+                for (int n = 0; n < size; n += 4) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(c + n);
+                    take(x[0]), take(x[1]), take(x[2]), take(x[3]);
+                }
+            } else {
+#pragma unroll 4
+                for (int n = 0; n < size; ++n) take(c[n]);
+            }
+            gs[i] = r.group_top == 2 && b > kLow ? a + b : a;
+        }
+        __syncthreads();
+        for (int i = lane; i < kWaveTokens * G; i += kWave) {
+            const int q = i / G, g = i - q * G;
+            const float* o = gs + q * G;
+            const float x = o[g];
+            int before = 0;
+#pragma unroll 8
+            for (int n = 0; n < G; ++n) before += o[n] > x || (o[n] == x && n < g);
+            kept[i] = before < r.top_groups;
+            if (before == r.top_groups - 1) cut[2 * q] = x;
+            if (before == r.top_groups) cut[2 * q + 1] = x;
+        }
+        __syncthreads();
+        if (scored) {
+            const float x = cut[2 * tok], y = cut[2 * tok + 1];
+            again = y > kLow && !(x - y > gap_limit(r.sigmoid, s_max, x));
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int e = expert_of<C>(l, j);
+            if (e < E && !kept[tok * G + ((e * r.size_inverse) >> 16)]) key[j] = kGone;
+        }
+    }
+    // K picks; experts of the lane's registers are expert_of(l, j) = expert_of(0, j) + (C < 4 ? l * C : 4 l)
+    constexpr int kStep = C < 4 ? C : 4;
+    int last = kGone;
+    bool reorder = false;  // two picks are nearer than fp32 tells apart
+    auto best_left = [&]() {
+        int m = key[0];
+#pragma unroll
+        for (int j = 1; j < C; ++j) m = max(m, key[j]);
+        return row_max_i(m);
+    };
+    auto close = [&](int m) {
+        const float x = key_value(last), y = key_value(m);
+        return last != kGone && m != kGone && !(x - y > gap_limit(r.sigmoid, s_max, x));
+    };
+    for (int k = 0; k < K; ++k) {
+        const int m = best_left();
+        int e = 1 << 20;
+#pragma unroll
+        for (int j = C - 1; j >= 0; --j) e = key[j] == m ? expert_of<C>(0, j) : e;
+        e = row_min_i(e + l * kStep);
+        if (r.bias) reorder |= close(m);
+        last = m;
+        if (l == 0) pick[tok * K + k] = m == kGone ? -1 : e;
+        const int mine = e - l * kStep;
+#pragma unroll
+        for (int j = 0; j < C; ++j) key[j] = mine == expert_of<C>(0, j) ? kGone : key[j];
+    }
+    if (r.bias) again |= close(best_left());
+    if (reorder && (K > kLanes || !r.sigmoid)) again = true;
+    __syncthreads();
+    if (__ballot(reorder && !again && valid)) {
+        int e = -1;
+        double c = kNone;
+        if (reorder && !again && valid && l < K) {
+            e = pick[tok * K + l];
+            if (e >= 0) {
+                const double x = static_cast<double>(logit<L>(r.logits, t * r.ld + e));
+                c = 1.0 / (1.0 + exp(-x)) + static_cast<double>(r.bias[e]);
+            }
+            parts[tok * K + l] = c;
+        }
+        __syncthreads();
+        int before = 0;
+        if (e >= 0)
+            for (int k = 0; k < K; ++k) {
+                const double o = parts[tok * K + k];
+                before += o > c || (o == c && pick[tok * K + k] < e);
+            }
+        __syncthreads();
+        if (e >= 0) pick[tok * K + before] = e;
+        __syncthreads();
+    }
+    const uint64_t redo = __ballot(again && valid);
+    if (redo) {
+        for (int q = 0; q < kWaveTokens; ++q) {
+            if (!((redo >> (q * kLanes)) & 1)) continue;
+            choose_exactly<L, C>(r, static_cast<int64_t>(blockIdx.x) * kWaveTokens + q, pick + q * K,
+                                 reinterpret_cast<double*>(shared + lay.scores_at()), kept,
+                                 reinterpret_cast<double*>(row));
+            __syncthreads();
+        }
+    }
+    if (!valid) return;
+    // Weights in float64: K values of a row. Renormalised, the scores are taken relative to the largest of the picks: their
+    // ratios hold where the scores themselves would underflow.
+    const int* my = pick + tok * K;
+    double* part = parts + tok * K;
+    int ref_key = kGone;
+    if (r.renormalize) {
+        for (int k = l; k < K; k += kLanes) {
+            if (my[k] < 0) continue;
+            const float x = logit<L>(r.logits, t * r.ld + my[k]);
+            ref_key = max(ref_key, key_of(r.sigmoid ? fminf(x, 0.0f) : x));
+        }
+        ref_key = row_max_i(ref_key);
+    }
+    const double ref = r.renormalize ? static_cast<double>(key_value(ref_key)) : r.sigmoid ? 0.0 : static_cast<double>(top);
+    double total = 0.0;
     for (int k = l; k < K; k += kLanes) {
-        ids[t * K + k] = pick[tok * K + k];
-        const double q = !r.renormalize ? p[k] : sum > 0.0 ? part(p[k]) / sum : 0.0;
-        const float w = static_cast<float>(q * static_cast<double>(r.scale));
+        double p = 0.0;
+        if (my[k] >= 0) {
+            const double x = static_cast<double>(logit<L>(r.logits, t * r.ld + my[k]));
+            if (r.sigmoid) p = exp(fmin(x, 0.0) - ref) / (1.0 + exp(-fabs(x)));
+            else p = x == ref ? 1.0 : exp(x - ref);
+        }
+        part[k] = p;
+        total += p;
+    }
+    double factor = static_cast<double>(r.scale);
+    if (r.renormalize) {
+        total = row_sum(total);
+        factor = total > 0.0 ? factor / total : 0.0;
+    } else if (!r.sigmoid) {
+        factor = sum > 0.0f ? factor / static_cast<double>(sum) : 0.0;
+    }
+    for (int k = l; k < K; k += kLanes) {  // each lane its own parts
+        ids[t * K + k] = my[k];
+        const float w = static_cast<float>(part[k] * factor);
         if (r.weights_type == MOE_DT_FLOAT32) put<F32>(weights, t * K + k, w);
         else put<F16>(weights, t * K + k, w);
+    }
+}
+
+template <typename L>
+__device__ __forceinline__ void store4_logits(void* p, int64_t i, const float* v) {
+    if constexpr (std::is_same_v<L, F32>) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+        uint16_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put<L>(b, j, v[j]);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
+            make_uint2(b[0] | (static_cast<uint32_t>(b[1]) << 16), b[2] | (static_cast<uint32_t>(b[3]) << 16));
     }
 }
 
 // Gradient of the weights of `ids` to the logits. p = s / sum of the K chosen s, g = scale * grad_w:
 //   renormalised  softmax: dl_k = p_k (g_k - sum g p)          sigmoid: the same times (1 - s_k)
 //   not           sigmoid: dl_k = g_k s_k (1 - s_k)            softmax: dl_e = s_e (g_e [e chosen] - sum g s)
-// 16 lanes have a token. Every expert's lane goes over the K picks itself, so an id that a caller's list holds twice
-// adds up in a fixed order and no lane writes another's element.
-template <typename L, int C>
-__global__ __launch_bounds__(kThreads) void group_routing_grad_kernel(GroupRouting r, const void* __restrict__ grad_w,
-                                                                      const int32_t* __restrict__ ids,
-                                                                      void* __restrict__ grad_logits) {
-    const int E = r.E, K = r.K;
-    const int tid = static_cast<int>(threadIdx.x), tok = tid / kLanes, l = tid % kLanes;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + tok;
-    if (t >= r.T) return;
-    const int32_t* id = ids + t * K;
-    auto g_of = [&](int k) {
-        const float g = r.weights_type == MOE_DT_FLOAT32 ? logit<F32>(grad_w, t * K + k)
-                                                         : r.weights_type == MOE_DT_FLOAT16
-                                                               ? logit<F16>(grad_w, t * K + k)
-                                                               : logit<B16>(grad_w, t * K + k);
-        return g * r.scale;
-    };
-    constexpr float kLow = -__builtin_huge_valf();
+// Bound by its bytes (T E written, and read in the last form; in the others only the picks' logits are read). 16 lanes have
+// a token, a wave four. A lane has every 16th pick; their terms are added into a row of LDS one after another, so an id
+// that a caller's list holds twice adds up in a fixed order, and the row leaves in whole vectors. fp32 throughout.
+template <typename L, int C, bool VEC>
+__global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting r, const void* __restrict__ grad_w,
+                                                                   const int32_t* __restrict__ ids,
+                                                                   void* __restrict__ grad_logits) {
+    extern __shared__ __align__(16) char shared[];
+    const int E = r.E, K = r.K, pitch = (E + 3) / 4 * 4 + 4;
+    const int lane = lane_id(), tok = lane / kLanes, l = lane % kLanes;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaveTokens + tok;
+    const bool valid = t < r.T;
+    float* row = reinterpret_cast<float*>(shared) + tok * pitch;
     const bool softmax_all = !r.sigmoid && !r.renormalize;
-    float lg[C], top = r.sigmoid && !r.renormalize ? 0.0f : kLow, sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-        const int e = l + j * kLanes;
-        lg[j] = e < E ? logit<L>(r.logits, t * r.ld + e) : kLow;
-    }
+
+    struct Pick {
+        int id;  // -1: outside [0, E), or its expert is not available
+        float x, g;
+    };
+    auto load_pick = [&](int k) {
+        Pick p{-1, kLow, 0.0f};
+        if (!valid || k >= K) return p;
+        const int e = ids[t * K + k];
+        if (e < 0 || e >= E) return p;
+        p.x = logit<L>(r.logits, t * r.ld + e);
+        if (!(p.x > kLow)) return p;
+        p.id = e;
+        p.g = r.scale * (r.weights_type == MOE_DT_FLOAT32 ? logit<F32>(grad_w, t * K + k)
+                         : r.weights_type == MOE_DT_FLOAT16 ? logit<F16>(grad_w, t * K + k)
+                                                            : logit<B16>(grad_w, t * K + k));
+        return p;
+    };
+    const Pick first = load_pick(l);
+    auto pick_at = [&](int k) { return k < kLanes ? first : load_pick(k); };
+
     // Scores up to a factor e^-top: of the row's softmax where all of it counts, else, renormalised, relative to the
     // largest of the picks, so that picks far below the row's best keep their ratios.
+    float s[C], top = 0.0f, inv = 1.0f;
     if (softmax_all) {
+        float v[C];
+        if (valid) {
+            load_logits<L, C, VEC>(r.logits, t * r.ld, E, l, v);
+        } else {
 #pragma unroll
-        for (int j = 0; j < C; ++j)
-            if (lg[j] > top) top = lg[j];
-        top = row_max(top);
-    } else if (r.renormalize) {
-        for (int k = 0; k < K; ++k) {
-            const int e = id[k];
-            if (e < 0 || e >= E) continue;
-            const float v = logit<L>(r.logits, t * r.ld + e), x = r.sigmoid ? fminf(v, 0.0f) : v;
-            if (v > kLow && x > top) top = x;
+            for (int j = 0; j < C; ++j) v[j] = kLow;
         }
+        int m = kGone;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            v[j] = v[j] > kLow ? v[j] : kLow;
+            m = max(m, key_of(v[j]));
+        }
+        top = key_value(row_max_i(m));
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const float d = v[j] == top ? 0.0f : v[j] - top;
+            s[j] = v[j] > kLow ? __builtin_amdgcn_exp2f(d * 1.4426950408889634f) : 0.0f;
+            sum += s[j];
+        }
+        sum = row_sum_f(sum);
+        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    } else if (r.renormalize) {
+        int m = kGone;
+        for (int k = l; k < K; k += kLanes) {
+            const Pick p = pick_at(k);
+            if (p.id >= 0) m = max(m, key_of(r.sigmoid ? fminf(p.x, 0.0f) : p.x));
+        }
+        m = row_max_i(m);
+        top = m == kGone ? 0.0f : key_value(m);
     }
     auto score = [&](float v) {
-        if (!(v > kLow)) return 0.0f;
         if (r.sigmoid) return expf(fminf(v, 0.0f) - top) / (1.0f + expf(-fabsf(v)));
-        return v == top ? 1.0f : expf(v - top);
+        return (v == top ? 1.0f : expf(v - top)) * inv;
     };
-    if (softmax_all) {
-#pragma unroll
-        for (int j = 0; j < C; ++j) sum += score(lg[j]);
-        sum = row_sum(sum);
+    float total = 0.0f, dot = 0.0f;  // sums of s and g s over the picks
+    for (int k = l; k < K; k += kLanes) {
+        const Pick p = pick_at(k);
+        if (p.id < 0) continue;
+        const float sk = score(p.x);
+        total += sk;
+        dot += p.g * sk;
     }
-    const float inv = softmax_all ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
-    float total = 0.0f, dot = 0.0f;  // sum s, sum g s over the picks
-    for (int k = 0; k < K; ++k) {
-        const int e = id[k];
-        if (e < 0 || e >= E) continue;
-        const float s = score(logit<L>(r.logits, t * r.ld + e)) * inv;
-        if (s > 0.0f) {
-            total += s;
-            dot += g_of(k) * s;
-        }
-    }
-    const float mean = r.renormalize ? (total > 0.0f ? dot / total : 0.0f) : dot;
+    total = row_sum_f(total);
+    dot = row_sum_f(dot);
     const float norm = r.renormalize ? (total > 0.0f ? 1.0f / total : 0.0f) : 1.0f;
+    const float mean = r.renormalize ? dot * norm : 0.0f;
+
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        const int e = l + j * kLanes;
-        if (e >= E) continue;
+        const int e = expert_of<C>(l, j);
+        if (e < E) row[e] = 0.0f;
+    }
+    __syncthreads();
+    for (int k0 = 0; k0 < K; k0 += kLanes) {
+        const Pick p = pick_at(k0 + l);
         float d = 0.0f;
-        bool hit = false;
-        for (int k = 0; k < K; ++k) {
-            if (id[k] != e) continue;
-            const float g = g_of(k);
-            d += r.renormalize ? g - mean : g;
-            hit = true;
+        if (p.id >= 0) {
+            d = (p.g - mean) * score(p.x) * norm;
+            if (r.sigmoid) d *= expf(fminf(-p.x, 0.0f)) / (1.0f + expf(-fabsf(p.x)));  // 1 - s
         }
-        if (softmax_all) d -= mean;
-        if (softmax_all || hit) {  // without a pick in the row there is nothing the scores are relative to
-            if (r.sigmoid) d *= expf(fminf(-lg[j], 0.0f)) / (1.0f + expf(-fabsf(lg[j])));  // 1 - s
-            const float s = score(lg[j]) * inv;
-            d = s > 0.0f ? d * s * norm : 0.0f;
+        for (int i = 0; i < kLanes && k0 + i < K; ++i) {
+            if (l == i && p.id >= 0) row[p.id] += d;
+            __syncthreads();  // one wave: orders the additions
         }
-        put<L>(grad_logits, t * E + e, d);
+    }
+    if (!valid) return;
+#pragma unroll
+    for (int j = 0; j < C; j += (VEC && C >= 4 ? 4 : 1)) {
+        const int e = expert_of<C>(l, j);
+        if (e >= E) continue;
+        if constexpr (VEC && C >= 4) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + e);
+            float v[4] = {a[0], a[1], a[2], a[3]};
+            if (softmax_all) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] -= s[j + i] * inv * dot;
+            }
+            store4_logits<L>(grad_logits, t * E + e, v);
+        } else {
+            put<L>(grad_logits, t * E + e, softmax_all ? row[e] - s[j] * inv * dot : row[e]);
+        }
     }
 }
 
+// Rows of 4-expert pieces that one load can read
+bool vector_logits(const GroupRouting& r) {
+    const uintptr_t mask = r.logits_type == MOE_DT_FLOAT32 ? 15 : 7;
+    return r.E % 4 == 0 && r.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(r.logits) & mask) == 0 &&
+           (reinterpret_cast<uintptr_t>(r.bias) & 15) == 0;
+}
+
+template <typename L, int C, bool VEC>
+hipError_t run_routing_vec(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream) {
+    TraceScope trace("moe_group_routing", stream);
+    group_routing_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kWaveTokens - 1) / kWaveTokens), kWave,
+                                      RoutingLds{r.E, r.groups, r.K}.bytes(), stream>>>(r, ids, weights);
+    return hipGetLastError();
+}
 template <typename L, int C>
 hipError_t run_routing(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream) {
-    const int lds = routing_lds(r.E, r.groups, r.K);
-    auto fn = &group_routing_kernel<L, C>;
-    const hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(fn), routing_lds(kMaxE, kMaxE, kMaxE));
-    if (err != hipSuccess) return err;
-    TraceScope trace("moe_group_routing", stream);
-    fn<<<static_cast<unsigned>((r.T + kTokens - 1) / kTokens), kThreads, lds, stream>>>(r, ids, weights);
+    return vector_logits(r) ? run_routing_vec<L, C, true>(r, ids, weights, stream)
+                            : run_routing_vec<L, C, false>(r, ids, weights, stream);
+}
+template <typename L, int C, bool VEC>
+hipError_t run_grad_vec(const GroupRouting& r, const void* gw, const int32_t* ids, void* gl, hipStream_t stream) {
+    TraceScope trace("moe_group_routing_grad", stream);
+    const int lds = kWaveTokens * ((r.E + 3) / 4 * 4 + 4) * 4;
+    group_routing_grad_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kWaveTokens - 1) / kWaveTokens), kWave, lds,
+                                           stream>>>(r, gw, ids, gl);
     return hipGetLastError();
 }
 template <typename L, int C>
 hipError_t run_grad(const GroupRouting& r, const void* gw, const int32_t* ids, void* gl, hipStream_t stream) {
-    TraceScope trace("moe_group_routing_grad", stream);
-    group_routing_grad_kernel<L, C>
-        <<<static_cast<unsigned>((r.T + kTokens - 1) / kTokens), kThreads, 0, stream>>>(r, gw, ids, gl);
-    return hipGetLastError();
+    return vector_logits(r) && (reinterpret_cast<uintptr_t>(gl) & 15) == 0 ? run_grad_vec<L, C, true>(r, gw, ids, gl, stream)
+                                                                            : run_grad_vec<L, C, false>(r, gw, ids, gl, stream);
 }
 
 template <typename F>
@@ -333,6 +672,7 @@ hipError_t by_type(const GroupRouting& r, F&& f) {
     auto with = [&](auto type) {
         if (c <= 1) return f(type, std::integral_constant<int, 1>());
         if (c <= 4) return f(type, std::integral_constant<int, 4>());
+        if (c <= 8) return f(type, std::integral_constant<int, 8>());
         return f(type, std::integral_constant<int, 16>());
     };
     if (r.logits_type == MOE_DT_FLOAT32) return with(F32());

@@ -181,6 +181,9 @@ struct GroupRouting {
     bool sigmoid, renormalize;
     float scale;
     int32_t weights_type;  // moe_dtype
+    // e / (E / groups) of an expert e < 256 is e * size_inverse >> 16: size_inverse = ceil(2^16 / size) is off by less than
+    // 1, so the product by less than 2^8, below 2^16 / size
+    int size_inverse;
 };
 hipError_t launch_group_routing(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream);
 // grad_weights (weights_type) and ids [T, K] -> grad_logits [T, E] of logits_type, contiguous
