@@ -7,10 +7,11 @@
 // An expert whose logit or c is NaN or -inf is not available; picks with no expert left are id -1, weight 0.
 //
 // The choice is the definition's, not fp32's: without a bias experts are compared by their logits, which order the scores
-// exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where two neighbours among a row's picks
-// are nearer than that, they are put in order by their float64 values (some rows in a thousand); where the last pick
-// and the best expert left, or the last group that stays and the first that does not, are, the whole row is chosen again
-// in float64 by the wave.
+// exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where the last group that stays and the
+// first that does not are nearer than that, the row's groups are scored again in float64; where two neighbours among
+// its picks are, the picks go on past the K-th until a clear gap and are put in order by their float64 values. That is
+// some rows in a thousand, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
+// never in the instruction cache when it is needed, cost 9 us.
 //
 // A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers. A
 // pick is the maximum over the lane (max3), over the row (4 DPP steps), the lowest index that has it (4 more) and its
@@ -29,6 +30,7 @@ namespace {
 constexpr int kLanes = 16;                   // lanes of one token
 constexpr int kWaveTokens = kWave / kLanes;  // tokens of a workgroup, one wave
 constexpr int kMaxE = 256;
+constexpr int kNoPick = 0xffff;              // a pick with no expert left
 constexpr int kGone = -2147483647 - 1;         // the key of an expert that is not available or was picked
 constexpr float kLow = -__builtin_huge_valf();
 constexpr double kNone = -__builtin_huge_val();
@@ -126,17 +128,18 @@ __device__ __forceinline__ float gap_limit(bool sigmoid, float s_max, float c) {
     return (sigmoid ? 32.0f : 256.0f * s_max) * 0x1p-24f + fabsf(c) * 0x1p-21f;
 }
 
-// LDS of the one wave of a workgroup
+// LDS of the one wave of a workgroup. A row may have E picks.
 struct RoutingLds {
     int E, G, K;
     __host__ __device__ int pitch() const { return (E + 3) / 4 * 4 + 4; }
-    __host__ __device__ int picks_at() const { return 8 * kWaveTokens * K; }                 // after the parts (double)
-    __host__ __device__ int scores_at() const { return picks_at() + 4 * kWaveTokens * K; }   // group scores: doubles
-    __host__ __device__ int kept_at() const { return scores_at() + 8 * kWaveTokens * G; }
+    __host__ __device__ int picks_at() const { return 8 * kWaveTokens * K; }  // after the parts (double): 16 bits each
+    __host__ __device__ int order_at() const { return picks_at() + 2 * kWaveTokens * E; }
+    __host__ __device__ int scores_at() const { return (order_at() + 2 * E + 3) / 4 * 4; }
+    __host__ __device__ int kept_at() const { return scores_at() + 4 * kWaveTokens * G; }
     __host__ __device__ int cut_at() const { return kept_at() + 4 * kWaveTokens * G; }
-    // c of the row's experts: floats of 4 tokens, or doubles of one
+    // c of the rows' experts, fp32; or, once the groups are scored, float64 values of one row and its groups
     __host__ __device__ int row_at() const { return (cut_at() + 8 * kWaveTokens + 15) / 16 * 16; }
-    __host__ __device__ int bytes() const { return row_at() + 4 * kWaveTokens * pitch(); }
+    __host__ __device__ int bytes(bool rows) const { return row_at() + (rows ? 4 * kWaveTokens * pitch() : 0); }
 };
 
 // Expert of lane l's register j: 16-byte (8-byte) pieces of 4 consecutive experts
@@ -169,98 +172,43 @@ __device__ __forceinline__ void load_logits(const void* p, int64_t at, int E, in
     }
 }
 
-// The choice of one row in float64 by the whole wave: picks [K], -1 where no expert is left
-template <typename L, int C>
-__device__ void choose_exactly(const GroupRouting& r, int64_t t, int* pick, double* gs, int* kept, double* cs) {
-    constexpr int C64 = (C + 3) / 4;
-    const int lane = lane_id(), E = r.E, G = r.groups, size = E / G;
-    double s[C64], c[C64];
-    bool open[C64];
-    double top = kNone;
-#pragma unroll
-    for (int j = 0; j < C64; ++j) {
-        const int e = lane + j * kWave;
-        s[j] = e < E ? static_cast<double>(logit<L>(r.logits, t * r.ld + e)) : kNone;
-        c[j] = s[j];
-        open[j] = s[j] > kNone;  // false for NaN too
-        if (open[j]) top = fmax(top, s[j]);
-    }
-    if (r.sigmoid) {
-#pragma unroll
-        for (int j = 0; j < C64; ++j) s[j] = open[j] ? 1.0 / (1.0 + exp(-s[j])) : 0.0;
-    } else {
-#pragma unroll
+// c (what groups are scored by) of all experts of row t in float64, by the whole wave, to cs [E]; -inf where not available
+template <typename L>
+__device__ __forceinline__ void exact_scores(const GroupRouting& r, int64_t t, double* cs) {
+    const int lane = lane_id(), E = r.E;
+    double top = kNone, sum = 1.0;
+    auto at = [&](int e) {
+        const double x = static_cast<double>(logit<L>(r.logits, t * r.ld + e));
+        return x > kNone ? x : kNone;  // NaN too
+    };
+    if (!r.sigmoid) {
+#pragma unroll 1
+        for (int e = lane; e < E; e += kWave) top = fmax(top, at(e));
+#pragma unroll 1
         for (int d = kWave / 2; d > 0; d >>= 1) top = fmax(top, __shfl_xor(top, d, kWave));
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < C64; ++j) {
-            s[j] = open[j] ? (s[j] == top ? 1.0 : exp(s[j] - top)) : 0.0;
-            sum += s[j];
-        }
-#pragma unroll
-        for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, kWave);
-#pragma unroll
-        for (int j = 0; j < C64; ++j) s[j] = open[j] ? s[j] / sum : 0.0;
+        sum = 0.0;
     }
-#pragma unroll
-    for (int j = 0; j < C64; ++j) {
-        const int e = lane + j * kWave;
-        if (open[j] && r.bias) c[j] = s[j] + static_cast<double>(r.bias[e]);
-        if (!open[j] || !(c[j] > kNone)) c[j] = kNone;
+#pragma unroll 1
+    for (int e = lane; e < E; e += kWave) {
+        const double x = at(e);
+        const double p = r.sigmoid ? exp(-x) : x == top ? 1.0 : exp(x - top);
+        const double s = !(x > kNone) ? 0.0 : r.sigmoid ? 1.0 / (1.0 + p) : p;
+        sum += s;
+        cs[e] = x > kNone ? s : kNone;
     }
-    if (r.top_groups < G) {
-#pragma unroll
-        for (int j = 0; j < C64; ++j) {
-            const int e = lane + j * kWave;
-            // two best scores are added; one best is compared, by the logits where there is no bias
-            if (e < E) cs[e] = c[j] > kNone ? (r.group_top == 2 && !r.bias ? s[j] : c[j]) : kNone;
-        }
-        __syncthreads();
-        for (int g = lane; g < G; g += kWave) {
-            double a = kNone, b = kNone;
-            for (int e = g * size; e < (g + 1) * size; ++e) {
-                b = fmax(b, fmin(a, cs[e]));
-                a = fmax(a, cs[e]);
-            }
-            gs[g] = r.group_top == 2 && b > kNone ? a + b : a;
-        }
-        __syncthreads();
-        for (int g = lane; g < G; g += kWave) {
-            int before = 0;
-            for (int o = 0; o < G; ++o) before += gs[o] > gs[g] || (gs[o] == gs[g] && o < g);
-            kept[g] = before < r.top_groups;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < C64; ++j) {
-            const int e = lane + j * kWave;
-            if (e < E && !kept[e / size]) c[j] = kNone;
-        }
+#pragma unroll 1
+    for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, kWave);
+    for (int e = lane; e < E; e += kWave) {  // its own entries
+        double c = cs[e];
+        if (!r.sigmoid) c = c > kNone ? c / sum : kNone;
+        if (r.bias) c += static_cast<double>(r.bias[e]);
+        cs[e] = c > kNone ? c : kNone;
     }
-    for (int k = 0; k < r.K; ++k) {
-        double best = kNone;
-        int at = kMaxE;
-#pragma unroll
-        for (int j = 0; j < C64; ++j)
-            if (c[j] > best) {  // ascending e: the lowest index of equals stays
-                best = c[j];
-                at = lane + j * kWave;
-            }
-#pragma unroll
-        for (int d = kWave / 2; d > 0; d >>= 1) {
-            const double ob = __shfl_xor(best, d, kWave);
-            const int oa = __shfl_xor(at, d, kWave);
-            if (ob > best || (ob == best && oa < at)) {
-                best = ob;
-                at = oa;
-            }
-        }
-        if (lane == 0) pick[k] = at == kMaxE ? -1 : at;
-#pragma unroll
-        for (int j = 0; j < C64; ++j)
-            if (lane + j * kWave == at) c[j] = kNone;
-    }
+    __syncthreads();
 }
+
+// Whether c comes before o in descending order, the lower index first among equals
+__device__ __forceinline__ bool goes_before(double o, int oi, double c, int ci) { return o > c || (o == c && oi < ci); }
 
 // C: experts of a lane. VEC: rows allow loads of 4 experts.
 template <typename L, int C, bool VEC>
@@ -270,11 +218,14 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     const int E = r.E, G = r.groups, K = r.K, size = E / G;
     const RoutingLds lay{E, G, K};
     double* parts = reinterpret_cast<double*>(shared);
-    int* pick = reinterpret_cast<int*>(shared + lay.picks_at());
+    uint16_t* pick = reinterpret_cast<uint16_t*>(shared + lay.picks_at());  // [token][E]
+    uint16_t* order = reinterpret_cast<uint16_t*>(shared + lay.order_at());
     float* gs = reinterpret_cast<float*>(shared + lay.scores_at());
     int* kept = reinterpret_cast<int*>(shared + lay.kept_at());
     float* cut = reinterpret_cast<float*>(shared + lay.cut_at());  // [token][2]: last score that stays, first that does not
     float* row = reinterpret_cast<float*>(shared + lay.row_at());
+    double* cs = reinterpret_cast<double*>(row);
+    double* cgs = cs + E;
     const int lane = lane_id(), tok = lane / kLanes, l = lane % kLanes;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaveTokens + tok;
     const bool valid = t < r.T;
@@ -331,7 +282,6 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
 #pragma unroll
         for (int j = 0; j < C; ++j) key[j] = v[j] > kLow ? key_of(v[j]) : kGone;
     }
-    bool again = false;  // fp32 does not settle this row's order
     if (grouped) {
         const bool by_score = r.group_top == 2 && !r.bias;
         auto entry = [&](int j) { return key[j] == kGone ? kLow : by_score ? s[j] : key_value(key[j]); };
@@ -381,7 +331,29 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         __syncthreads();
         if (scored) {
             const float x = cut[2 * tok], y = cut[2 * tok + 1];
-            again = y > kLow && !(x - y > gap_limit(r.sigmoid, s_max, x));
+            uint64_t open = __ballot(valid && y > kLow && !(x - y > gap_limit(r.sigmoid, s_max, x)));
+#pragma unroll 1
+            for (int q = 0; open && q < kWaveTokens; ++q) {
+                if (!((open >> (q * kLanes)) & 1)) continue;
+                exact_scores<L>(r, static_cast<int64_t>(blockIdx.x) * kWaveTokens + q, cs);
+#pragma unroll 1
+                for (int g = lane; g < G; g += kWave) {
+                    double a = kNone, b = kNone;
+                    for (int e = g * size; e < (g + 1) * size; ++e) {
+                        b = fmax(b, fmin(a, cs[e]));
+                        a = fmax(a, cs[e]);
+                    }
+                    cgs[g] = r.group_top == 2 && b > kNone ? a + b : a;
+                }
+                __syncthreads();
+#pragma unroll 1
+                for (int g = lane; g < G; g += kWave) {
+                    int before = 0;
+                    for (int o = 0; o < G; ++o) before += goes_before(cgs[o], o, cgs[g], g);
+                    kept[q * G + g] = before < r.top_groups;
+                }
+                __syncthreads();
+            }
         }
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -389,77 +361,65 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             if (e < E && !kept[tok * G + ((e * r.size_inverse) >> 16)]) key[j] = kGone;
         }
     }
-    // K picks; experts of the lane's registers are expert_of(l, j) = expert_of(0, j) + (C < 4 ? l * C : 4 l)
     constexpr int kStep = C < 4 ? C : 4;
-    int last = kGone;
-    bool reorder = false;  // two picks are nearer than fp32 tells apart
-    auto best_left = [&]() {
+    int last = kGone, picks = K;  // picks of this row: K, and those that fp32 does not tell from the K-th
+    bool reorder = false;         // two of them are nearer than fp32 tells apart
+#pragma unroll 1
+    for (int k = 0;; ++k) {
         int m = key[0];
 #pragma unroll
         for (int j = 1; j < C; ++j) m = max(m, key[j]);
-        return row_max_i(m);
-    };
-    auto close = [&](int m) {
-        const float x = key_value(last), y = key_value(m);
-        return last != kGone && m != kGone && !(x - y > gap_limit(r.sigmoid, s_max, x));
-    };
-    for (int k = 0; k < K; ++k) {
-        const int m = best_left();
-        int e = 1 << 20;
+        m = row_max_i(m);
+        if (r.bias) {
+            const float x = key_value(last), y = key_value(m);
+            const bool close = last != kGone && m != kGone && !(x - y > gap_limit(r.sigmoid, s_max, x));
+            if (close && k <= picks) {
+                reorder = true;
+                picks = max(picks, k + 1);
+            }
+            last = m;
+        }
+        if (k >= K && !__any(k < picks)) break;
+        int jw = -1;
 #pragma unroll
-        for (int j = C - 1; j >= 0; --j) e = key[j] == m ? expert_of<C>(0, j) : e;
-        e = row_min_i(e + l * kStep);
-        if (r.bias) reorder |= close(m);
-        last = m;
-        if (l == 0) pick[tok * K + k] = m == kGone ? -1 : e;
-        const int mine = e - l * kStep;
+        for (int j = C - 1; j >= 0; --j) jw = key[j] == m ? j : jw;
+        const int e = row_min_i(jw < 0 ? kMaxE : expert_of<C>(l, jw));
+        if (l == 0 && k < picks) pick[tok * E + k] = static_cast<uint16_t>(m == kGone ? kNoPick : e);
+        const int mine = e / kStep % kLanes == l ? e / (kLanes * kStep) * kStep + e % kStep : -1;  // its register
 #pragma unroll
-        for (int j = 0; j < C; ++j) key[j] = mine == expert_of<C>(0, j) ? kGone : key[j];
+        for (int j = 0; j < C; ++j) key[j] = mine == j ? kGone : key[j];
     }
-    if (r.bias) again |= close(best_left());
-    if (reorder && (K > kLanes || !r.sigmoid)) again = true;
     __syncthreads();
-    if (__ballot(reorder && !again && valid)) {
-        int e = -1;
-        double c = kNone;
-        if (reorder && !again && valid && l < K) {
-            e = pick[tok * K + l];
-            if (e >= 0) {
-                const double x = static_cast<double>(logit<L>(r.logits, t * r.ld + e));
-                c = 1.0 / (1.0 + exp(-x)) + static_cast<double>(r.bias[e]);
+    uint64_t redo = __ballot(reorder && valid);
+#pragma unroll 1
+    for (int q = 0; redo && q < kWaveTokens; ++q) {
+        if (!((redo >> (q * kLanes)) & 1)) continue;
+        exact_scores<L>(r, static_cast<int64_t>(blockIdx.x) * kWaveTokens + q, cs);
+        const int n = __shfl(picks, q * kLanes, kWave);
+        uint16_t* of = pick + q * E;
+#pragma unroll 1
+        for (int k = lane; k < n; k += kWave) {
+            const int e = of[k];
+            int before = k;  // empty picks, at the end, stay
+            if (e != kNoPick) {
+                before = 0;
+                for (int o = 0; o < n; ++o) before += of[o] != kNoPick && goes_before(cs[of[o]], of[o], cs[e], e);
             }
-            parts[tok * K + l] = c;
+            order[before] = static_cast<uint16_t>(e);
         }
         __syncthreads();
-        int before = 0;
-        if (e >= 0)
-            for (int k = 0; k < K; ++k) {
-                const double o = parts[tok * K + k];
-                before += o > c || (o == c && pick[tok * K + k] < e);
-            }
+        for (int k = lane; k < K; k += kWave) of[k] = order[k];
         __syncthreads();
-        if (e >= 0) pick[tok * K + before] = e;
-        __syncthreads();
-    }
-    const uint64_t redo = __ballot(again && valid);
-    if (redo) {
-        for (int q = 0; q < kWaveTokens; ++q) {
-            if (!((redo >> (q * kLanes)) & 1)) continue;
-            choose_exactly<L, C>(r, static_cast<int64_t>(blockIdx.x) * kWaveTokens + q, pick + q * K,
-                                 reinterpret_cast<double*>(shared + lay.scores_at()), kept,
-                                 reinterpret_cast<double*>(row));
-            __syncthreads();
-        }
     }
     if (!valid) return;
     // Weights in float64: K values of a row. Renormalised, the scores are taken relative to the largest of the picks: their
     // ratios hold where the scores themselves would underflow.
-    const int* my = pick + tok * K;
+    const uint16_t* my = pick + tok * E;
     double* part = parts + tok * K;
     int ref_key = kGone;
     if (r.renormalize) {
         for (int k = l; k < K; k += kLanes) {
-            if (my[k] < 0) continue;
+            if (my[k] == kNoPick) continue;
             const float x = logit<L>(r.logits, t * r.ld + my[k]);
             ref_key = max(ref_key, key_of(r.sigmoid ? fminf(x, 0.0f) : x));
         }
@@ -469,7 +429,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     double total = 0.0;
     for (int k = l; k < K; k += kLanes) {
         double p = 0.0;
-        if (my[k] >= 0) {
+        if (my[k] != kNoPick) {
             const double x = static_cast<double>(logit<L>(r.logits, t * r.ld + my[k]));
             if (r.sigmoid) p = exp(fmin(x, 0.0) - ref) / (1.0 + exp(-fabs(x)));
             else p = x == ref ? 1.0 : exp(x - ref);
@@ -485,7 +445,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         factor = sum > 0.0f ? factor / static_cast<double>(sum) : 0.0;
     }
     for (int k = l; k < K; k += kLanes) {  // each lane its own parts
-        ids[t * K + k] = my[k];
+        ids[t * K + k] = my[k] == kNoPick ? -1 : my[k];
         const float w = static_cast<float>(part[k] * factor);
         if (r.weights_type == MOE_DT_FLOAT32) put<F32>(weights, t * K + k, w);
         else put<F16>(weights, t * K + k, w);
@@ -644,7 +604,7 @@ template <typename L, int C, bool VEC>
 hipError_t run_routing_vec(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream) {
     TraceScope trace("moe_group_routing", stream);
     group_routing_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kWaveTokens - 1) / kWaveTokens), kWave,
-                                      RoutingLds{r.E, r.groups, r.K}.bytes(), stream>>>(r, ids, weights);
+                                      RoutingLds{r.E, r.groups, r.K}.bytes(r.bias || r.top_groups < r.groups), stream>>>(r, ids, weights);
     return hipGetLastError();
 }
 template <typename L, int C>
