@@ -4,7 +4,7 @@
 //   grad_weights[t, k]       = sum_h grad_y[t, h] * expert_out[t, k, h]
 //
 // The forward is the reference's op_kernel/moe_combine.cpp:80-111; it has no gradient there.
-// Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 4 experts at
+// Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 8 experts at
 // a time, loads their rows, adds to their dot products and writes their gradient rows. A wave has a token to itself, or
 // four waves share it; the dot products are added over the lanes and then over the waves in a fixed order.
 #include "moe_device.h"
@@ -15,9 +15,11 @@ namespace moe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;  // experts in flight per thread
+constexpr int kBatch = 8;  // experts in flight per thread
+// expert_out and its gradient beyond the 256 MB Infinity Cache go past it (non-temporal)
+constexpr int64_t kStreamBytes = int64_t(128) << 20;
 
-template <int WAVES>  // waves of one token: 1 or 4
+template <int WAVES, bool NT>  // waves of one token: 1 or 4
 __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* __restrict__ grad_y,
                                                                 const uint16_t* __restrict__ expert_out,
                                                                 const uint16_t* __restrict__ weights,
@@ -30,7 +32,7 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
     const uint16_t* dy = grad_y + t * H;
     const int first = (WAVES == 1 ? lane : static_cast<int>(threadIdx.x)) * 8;
     for (int k0 = 0; k0 < K; k0 += kBatch) {
-        float dot[kBatch] = {0.f, 0.f, 0.f, 0.f}, w[kBatch];
+        float dot[kBatch] = {}, w[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) w[u] = k0 + u < K ? f16_bits_to_f32(weights[t * K + k0 + u]) : 0.0f;
         for (int c = first; c < H; c += WAVES * kWave * 8) {
@@ -38,7 +40,10 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
             f16x8 o[kBatch];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u)
-                if (k0 + u < K) o[u] = load_f16x8(expert_out + (t * K + k0 + u) * H + c);
+                if (k0 + u < K) {
+                    const uint16_t* at = expert_out + (t * K + k0 + u) * H + c;
+                    o[u] = NT ? load_f16x8_stream(at) : load_f16x8(at);
+                }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 if (k0 + u < K) {
@@ -49,7 +54,9 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
                         dot[u] += g * static_cast<float>(o[u][j]);
                         v[j] = static_cast<f16>(w[u] * g);
                     }
-                    *reinterpret_cast<f16x8*>(grad_eo + (t * K + k0 + u) * H + c) = v;
+                    uint16_t* at = grad_eo + (t * K + k0 + u) * H + c;
+                    if (NT) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(at));
+                    else *reinterpret_cast<f16x8*>(at) = v;
                 }
             }
         }
@@ -58,10 +65,10 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
 #pragma unroll
             for (int d = kWave / 2; d > 0; d >>= 1) dot[u] += __shfl_xor(dot[u], d, kWave);
         if (WAVES == 1) {
-            if (lane < kBatch && k0 + lane < K) {
-                const float v = lane == 0 ? dot[0] : lane == 1 ? dot[1] : lane == 2 ? dot[2] : dot[3];
-                grad_w[t * K + k0 + lane] = f32_to_f16_bits(v);
-            }
+            float v = dot[0];
+#pragma unroll
+            for (int u = 1; u < kBatch; ++u) v = lane == u ? dot[u] : v;
+            if (lane < kBatch && k0 + lane < K) grad_w[t * K + k0 + lane] = f32_to_f16_bits(v);
         } else {
             if (lane == 0) {
 #pragma unroll
@@ -81,13 +88,18 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
 hipError_t launch_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, const uint16_t* weights,
                                uint16_t* grad_eo, uint16_t* grad_w, int64_t T, int H, int K, hipStream_t stream) {
     TraceScope trace("moe_combine_grad", stream);
+    const bool nt = T * K * H * 2 > kStreamBytes;
     // a wave a token once that gives every SIMD two waves
-    if (T >= 2048)
-        combine_grad_kernel<1><<<static_cast<unsigned>((T + 3) / 4), kThreads, 0, stream>>>(
-            grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+    const bool one = T >= 2048;
+    const unsigned grid = static_cast<unsigned>(one ? (T + 3) / 4 : T);
+    if (one && nt)
+        combine_grad_kernel<1, true><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+    else if (one)
+        combine_grad_kernel<1, false><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+    else if (nt)
+        combine_grad_kernel<4, true><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     else
-        combine_grad_kernel<4><<<static_cast<unsigned>(T), kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo,
-                                                                                   grad_w, T, H, K);
+        combine_grad_kernel<4, false><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     return hipGetLastError();
 }
 

@@ -79,71 +79,131 @@ moe_status check_pitch(const char* op, const char* what, int64_t rows, int64_t w
     return ok();
 }
 
-// How one product runs
+// How one product runs: weight streaming, tiles of 32, 64 or 128 x 128 (split over k or not), or 256 x 256 tiles
+enum class Kernel { kStream, kMid, kTiled };
 struct ProductPlan {
-    int bm;
+    Kernel kernel;
+    int bm;  // kMid: rows of a tile
     int splits;
     int64_t split_k;
     size_t partial_bytes;
 };
 
-// The product is split over k while its tiles leave workgroup slots of the GPU empty (two a CU), with at least four
-// stages a piece.
-ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k) {
-    ProductPlan p{};
-    p.bm = p_by_k || m > 32 ? 128 : 32;
-    const int64_t tiles = (m + p.bm - 1) / p.bm * ((n + (swiglu ? 63 : 127)) / (swiglu ? 64 : 128));
-    const int64_t stages = (k + 63) / 64;
-    int64_t splits = tiles > 0 ? 512 / tiles : 1;
-    if (splits > stages / 4) splits = stages / 4;
-    if (splits < 1) splits = 1;
-    const int64_t per = (stages + splits - 1) / splits;
-    p.split_k = per > 0 ? per * 64 : 64;
-    p.splits = per > 0 ? static_cast<int>((stages + per - 1) / per) : 1;
-    p.partial_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * m * moe::part_ld(static_cast<int>(n), swiglu) * 4 : 0;
-    return p;
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Microseconds of a launch by tiles of bm x 128 with `items` workgroups of `stages` 64-k stages: two share a CU. One
+// alone takes 0.45, 0.56 or 0.92 us a stage (32, 64, 128 rows), two together 0.7, 0.86 or 1.45 us.
+double mid_time(int bm, int64_t items, int64_t stages) {
+    const double one = bm == 32 ? 0.45 : bm == 64 ? 0.56 : 0.92, two = bm == 32 ? 0.7 : bm == 64 ? 0.86 : 1.45;
+    const int64_t rest = items % 512;
+    const double tail = rest == 0 ? 0.0 : rest <= 256 ? one : one + (two - one) * (rest / 256.0 - 1.0);
+    return 3.0 + stages * (static_cast<double>(items / 512) * two + tail);
+}
+// The same of 256 x 256 tiles: one workgroup a CU, 0.85 us a stage with few tiles up to 1.7 with one on every CU (the
+// clock falls), 3 us of epilogue a round.
+double tiled_time(int64_t tiles, int64_t stages) {
+    const int64_t rest = tiles % 256;
+    const double tail = rest == 0 ? 0.0 : 3.0 + stages * (0.85 + 0.85 * (rest / 256.0));
+    return 4.0 + static_cast<double>(tiles / 256) * (3.0 + 1.7 * stages) + tail;
+}
+
+// The kernel with the least time by those figures. Against every kernel measured on 63 sizes (T = 512 .. 16384, N = 64 ..
+// 16384, H = 512 .. 7168) the choice was the fastest or within 5 %, but for two SwiGLU sizes with H = 7168 (12 and 29 %).
+// A product by tiles is split over k while that leaves eight stages a piece and at most the 512 workgroups that the GPU
+// holds; the pieces' sums then take another launch.
+// Few rows stream the weights where both operands are read by rows: T = 16, H = 2048, N = 7168 9.1 us (tiles of 32 rows
+// 11.5), T = 64 14.2 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N = 256
+// 12.7 us (9.1 split over k), T = 64, H = 4096, N = 16384 45 us (34).
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct) {
+    ProductPlan best{Kernel::kMid, 128, 1, ceil_div(k > 0 ? k : 1, 64) * 64, 0};
+    const int64_t stages = ceil_div(k > 0 ? k : 1, 64);
+    if (direct && !p_by_k && !q_by_k && m <= 64) {
+        const int64_t tiles = ceil_div(n, swiglu ? 8 : 16);
+        if (m <= 16 || (tiles >= 64 && (m <= 32 || tiles <= 512))) {
+            best.kernel = Kernel::kStream;
+            return best;
+        }
+    }
+    double least = 1e30;
+    for (const int bm : {32, 64, 128}) {
+        if ((bm == 32) != (m <= 32) && bm != 128) continue;
+        if (bm != 128 && p_by_k) continue;
+        if (bm == 128 && !p_by_k && m <= 64) continue;
+        const int64_t tiles = ceil_div(m, bm) * ceil_div(n, swiglu ? 64 : 128);
+        int64_t splits = tiles > 0 ? 512 / tiles : 1;
+        if (splits > stages / 8) splits = stages / 8;
+        if (splits < 1) splits = 1;
+        const int64_t per = ceil_div(stages, splits);
+        splits = ceil_div(stages, per);
+        const size_t partial =
+            splits > 1 ? static_cast<size_t>(splits) * m * moe::part_ld(static_cast<int>(n), swiglu) * 4 : 0;
+        const double t = mid_time(bm, tiles * splits, per) + (splits > 1 ? 2.5 + 2.0 * partial / 6e6 : 0.0);
+        if (t < least) {
+            least = t;
+            best = ProductPlan{Kernel::kMid, bm, static_cast<int>(splits), per * 64, partial};
+        }
+    }
+    const int64_t tiles = ceil_div(m, 256) * ceil_div(n, swiglu ? 128 : 256);
+    if (direct && m > 64 && tiled_time(tiles, stages) < least)
+        best = ProductPlan{Kernel::kTiled, 256, 1, stages * 64, 0};
+    return best;
+}
+
+// The most that a product's partial sums take, whatever its operands' layout and alignment
+size_t most_partial(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k) {
+    size_t most = 0;
+    for (int v = 0; v < 4; ++v) {
+        const size_t b = plan_product(m, n, k, swiglu, p_by_k, p_by_k || (v & 1), (v & 2) != 0).partial_bytes;
+        if (b > most) most = b;
+    }
+    return most;
 }
 
 // Whether an operand allows 16-byte copies: granules on 16 bytes in every row, tile offsets within 32 bits
 bool direct_operand(const void* p, int64_t ld) {
     return aligned16(p) && ld % 8 == 0 && ld <= int64_t{1} << 22;
 }
-
-// p_padded: P's rows are zero from k up to the next multiple of 8
-hipError_t run_product(moe::GemmArgs g, const ProductPlan& plan, void* partial, bool p_by_k, bool q_by_k, bool bf16,
-                       hipStream_t stream, bool p_padded = false) {
-    const bool swiglu = g.act == moe::kActSwiglu;
-    const bool direct = direct_operand(g.p, g.ldp) && direct_operand(g.q, g.ldq) &&
-                        (g.k % 8 == 0 || (q_by_k && (p_by_k || p_padded))) && !(swiglu && q_by_k && g.n % 8 != 0);
+void set_split(moe::GemmArgs& g, const ProductPlan& plan, void* partial) {
     g.partial = static_cast<float*>(partial);
     g.splits = plan.splits;
     g.split_k = static_cast<int>(plan.split_k);
-    const int64_t tiles = (g.m + 255) / 256 * ((g.n + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256));
-    if (direct && plan.splits == 1 && tiles >= 128) return moe::launch_gemm_tiled(g, p_by_k, q_by_k, bf16, stream);
-    hipError_t err = moe::launch_gemm_mid(g, p_by_k, q_by_k, bf16, direct, plan.bm, stream);
-    if (err == hipSuccess && plan.splits > 1) err = moe::launch_gemm_reduce(g, bf16, stream);
-    return err;
+}
+
+// p_padded: P's rows are zero from k up to the next multiple of 8
+bool direct_product(const moe::GemmArgs& g, bool p_by_k, bool q_by_k, bool p_padded) {
+    return direct_operand(g.p, g.ldp) && direct_operand(g.q, g.ldq) &&
+           (g.k % 8 == 0 || (q_by_k && (p_by_k || p_padded))) &&
+           !(g.act == moe::kActSwiglu && q_by_k && g.n % 8 != 0);
+}
+
+hipError_t run_product(moe::GemmArgs g, void* partial, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream,
+                       bool p_padded = false) {
+    const bool direct = direct_product(g, p_by_k, q_by_k, p_padded);
+    const ProductPlan plan = plan_product(g.m, g.n, g.k, g.act == moe::kActSwiglu, p_by_k, q_by_k, direct);
+    set_split(g, plan, partial);
+    if (plan.kernel == Kernel::kStream) return moe::launch_gemm_stream(g, bf16, stream);
+    if (plan.kernel == Kernel::kTiled) return moe::launch_gemm_tiled(g, p_by_k, q_by_k, bf16, stream);
+    const hipError_t err = moe::launch_gemm_mid(g, p_by_k, q_by_k, bf16, direct, plan.bm, stream);
+    return err == hipSuccess && plan.splits > 1 ? moe::launch_gemm_reduce(g, bf16, stream) : err;
 }
 
 size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
-    return plan_product(T, N, H, act == MOE_ACT_SWIGLU, false).partial_bytes;
+    return most_partial(T, N, H, act == MOE_ACT_SWIGLU, false);
 }
 
 // Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | partial sums of a split product
 struct GradWorkspace {
     int64_t Z, ldz;
     size_t sums_at, partial_at, bytes;
-    ProductPlan x, w;
 };
 GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
     GradWorkspace g{};
     g.Z = act == MOE_ACT_SWIGLU ? 2 * N : N;
     g.ldz = round_up(g.Z, 8);
-    g.x = plan_product(T, H, g.ldz, false, false);
-    g.w = plan_product(g.Z, H, T, false, true);
     g.sums_at = round_up(T * g.ldz * 2, 256);
     g.partial_at = g.sums_at + round_up(static_cast<int64_t>(moe::act_grad_row_blocks(T, static_cast<int>(g.Z))) * g.Z * 4, 256);
-    g.bytes = g.partial_at + (g.x.partial_bytes > g.w.partial_bytes ? g.x.partial_bytes : g.w.partial_bytes);
+    const size_t x = most_partial(T, H, g.Z, false, false), w = most_partial(g.Z, H, T, false, true);
+    g.bytes = g.partial_at + round_up(static_cast<int64_t>(x), 256) + w;  // both, for products of one launch
     return g;
 }
 
@@ -267,11 +327,10 @@ moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64
     if (st != MOE_OK) return st;
     if (T == 0) return ok();
     if (!x || !weight || !y) return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
-    const ProductPlan plan = plan_product(T, N, H, activation == MOE_ACT_SWIGLU, false);
-    if (plan.partial_bytes > 0 && (!workspace || workspace_bytes < plan.partial_bytes))
-        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace,
-                    plan.partial_bytes);
-    if (plan.partial_bytes > 0 && !aligned16(workspace))
+    const size_t need = linear_workspace(T, N, H, activation);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace, need);
+    if (need > 0 && !aligned16(workspace))
         return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
     moe::GemmArgs g{};
     g.p = static_cast<const uint16_t*>(x);
@@ -287,8 +346,9 @@ moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64
     g.residual = residual;
     g.act = activation;
     g.out_f32 = out_dtype == MOE_DT_FLOAT32;
-    const hipError_t err = run_product(g, plan, workspace, false, weight_transposed != 0, dtype == MOE_DT_BFLOAT16,
-                                       as_stream(stream));
+    hipError_t err = moe::prepare_linear();
+    if (err != hipSuccess) return hip_fail(err, "MoeLinear kernel attributes");
+    err = run_product(g, workspace, false, weight_transposed != 0, dtype == MOE_DT_BFLOAT16, as_stream(stream));
     if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
     return ok();
 }
@@ -331,41 +391,53 @@ moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void
     const bool need_dz = !as_is && (grad_x || grad_weight) && T > 0;
     const uint16_t* dz = as_is ? static_cast<const uint16_t*>(grad_y) : reinterpret_cast<uint16_t*>(base);
     const int64_t ldz = as_is ? grad_y_stride : ws.ldz;
-    hipError_t err = hipSuccess;
+    hipError_t err = moe::prepare_linear();
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad kernel attributes");
+    float* sums = reinterpret_cast<float*>(base + ws.sums_at);
     if (need_dz || grad_bias)
         err = moe::launch_act_grad(static_cast<const uint16_t*>(grad_y), grad_y_stride,
                                    act ? static_cast<const uint16_t*>(pre) : nullptr,
                                    need_dz ? reinterpret_cast<uint16_t*>(base) : nullptr, ws.ldz,
-                                   reinterpret_cast<float*>(base + ws.sums_at), static_cast<uint16_t*>(grad_bias), T,
-                                   static_cast<int>(N), activation, bf16, s);
+                                   grad_bias ? sums : nullptr, T, static_cast<int>(N), activation, bf16, s);
     if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad activation launch");
+    moe::GradTail tail{};
+    moe::GemmArgs &gx = tail.x, &gw = tail.w;
+    gx.p = gw.p = dz;
+    gx.ldp = gw.ldp = ldz;
+    gx.q = static_cast<const uint16_t*>(weight);
+    gx.ldq = weight_stride;
+    gx.m = gw.k = static_cast<int>(T);
+    gx.n = gw.n = static_cast<int>(H);
+    gx.k = gw.m = static_cast<int>(ws.Z);
+    gx.out = grad_x;
+    gw.q = static_cast<const uint16_t*>(x);
+    gw.ldq = x_stride;
+    gw.out = grad_weight;
+    tail.sums = sums;
+    tail.bias_grad = static_cast<uint16_t*>(grad_bias);
+    tail.Z = static_cast<int>(ws.Z);
+    tail.sum_rows = moe::act_grad_row_blocks(T, tail.Z);
+    const bool want_x = grad_x && T > 0, by_k = weight_transposed == 0;
     void* partial = base + ws.partial_at;
-    if (grad_x && T > 0) {
-        moe::GemmArgs g{};
-        g.p = dz;
-        g.ldp = ldz;
-        g.q = static_cast<const uint16_t*>(weight);
-        g.ldq = weight_stride;
-        g.m = static_cast<int>(T);
-        g.n = static_cast<int>(H);
-        g.k = static_cast<int>(ws.Z);
-        g.out = grad_x;
-        err = run_product(g, ws.x, partial, false, weight_transposed == 0, bf16, s, need_dz);
-        if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad grad_x launch");
+    if (want_x && grad_weight && direct_product(gx, false, by_k, need_dz) && direct_product(gw, true, true, false)) {
+        const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true);
+        const ProductPlan pw = plan_product(gw.m, gw.n, gw.k, false, true, true, true);
+        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid) {
+            set_split(gx, px, partial);
+            set_split(gw, pw, static_cast<char*>(partial) + round_up(static_cast<int64_t>(px.partial_bytes), 256));
+            err = moe::launch_gemm_pair(gx, gw, by_k, bf16, px.bm, s);
+            if (err == hipSuccess) err = moe::launch_grad_tail(tail, bf16, s);
+            if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
+            return ok();
+        }
     }
-    if (grad_weight) {
-        moe::GemmArgs g{};
-        g.p = dz;
-        g.ldp = ldz;
-        g.q = static_cast<const uint16_t*>(x);
-        g.ldq = x_stride;
-        g.m = static_cast<int>(ws.Z);
-        g.n = static_cast<int>(H);
-        g.k = static_cast<int>(T);
-        g.out = grad_weight;
-        err = run_product(g, ws.w, partial, true, true, bf16, s);
-        if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad grad_weight launch");
+    if (want_x) err = run_product(gx, partial, false, by_k, bf16, s, need_dz);
+    if (err == hipSuccess && grad_weight) err = run_product(gw, partial, true, true, bf16, s);
+    if (err == hipSuccess && grad_bias) {
+        gx.splits = gw.splits = 1;
+        err = moe::launch_grad_tail(tail, bf16, s);
     }
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
     return ok();
 }
 

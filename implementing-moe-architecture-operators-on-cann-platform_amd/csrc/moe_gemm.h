@@ -56,17 +56,37 @@ struct GemmArgs {
 __host__ __device__ constexpr int64_t part_cols(int n) { return (static_cast<int64_t>(n) + 3) / 4 * 4; }
 __host__ __device__ constexpr int64_t part_ld(int n, bool swiglu) { return part_cols(n) * (swiglu ? 2 : 1); }
 
-// Activations in fp32. gelu through erfc: 1 + erf(z / sqrt 2) loses every digit for large negative z.
+// 1 / (1 + e^-z) with the hardware exp2 and reciprocal (about 1 ulp each; the exponent's rounding moves it by at most
+// 0.34 * 2^-24)
+__device__ __forceinline__ float sigmoid_fast(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+}
+
+// The normal distribution function 1/2 erfc(-z / sqrt 2) and e = e^(-z^2 / 2), by Abramowitz and Stegun 7.1.26 (absolute
+// error 7.5e-8): a fifth of erfcf's instructions. From the tail's side, so that a large negative z keeps its digits.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float tail = 0.5f * p * e;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+constexpr float kTanhA = 2.0f * 0.79788456080286536f, kTanhB = 0.044715f;  // 1/2 (1 + tanh a) = sigmoid(2 a)
+
+// Activations in fp32
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
-        case kActGelu: return 0.5f * z * erfcf(z * -0.70710678118654752f);
-        case kActGeluTanh: return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
-        case kActSilu: return z / (1.0f + expf(-z));
+        case kActGelu: {
+            float e;
+            return z * normal_cdf(z, e);
+        }
+        case kActGeluTanh: return z * sigmoid_fast(kTanhA * (z + kTanhB * z * z * z));
+        case kActSilu: return z * sigmoid_fast(z);
         default: return z;
     }
 }
-
 __device__ __forceinline__ f32x4 activate4(f32x4 z, int act) {
     if (act == kActNone) return z;
     return f32x4{activate(z[0], act), activate(z[1], act), activate(z[2], act), activate(z[3], act)};
@@ -108,7 +128,7 @@ __device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col
     f32x4 y;
     if (SWIGLU) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = swiglu_f32(z[r], u[r]);
+        for (int r = 0; r < 4; ++r) y[r] = z[r] * sigmoid_fast(z[r]) * u[r];
     } else {
         y = activate4(z, g.act);
     }
@@ -215,9 +235,48 @@ __device__ __forceinline__ uint32_t transposed_address(const uint16_t* tile, int
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)p));
 }
 
-// kernels' launches
+// 16 columns a workgroup of 256 threads; its 16 groups add every 16th row of `part`, then the groups' sums in order
+constexpr int kSumColumns = 16;
+template <typename T>
+__device__ __forceinline__ void column_sums(const float* __restrict__ part, uint16_t* __restrict__ out, int Z, int rows,
+                                            int block) {
+    constexpr int kGroups = 16;
+    __shared__ float sums[kGroups][kSumColumns];
+    const int i = static_cast<int>(threadIdx.x) % kSumColumns, q = static_cast<int>(threadIdx.x) / kSumColumns;
+    const int c = block * kSumColumns + i;
+    float s = 0.0f;
+    if (c < Z) {
+#pragma unroll 4
+        for (int b = q; b < rows; b += kGroups) s += part[static_cast<int64_t>(b) * Z + c];
+    }
+    sums[q][i] = s;
+    __syncthreads();
+    if (q != 0 || c >= Z) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) s += sums[g][i];
+    out[c] = T::store(s);
+}
+
+// What follows the gradients' products: the reduction of those that were split (splits > 1), the bias's column sums
+struct GradTail {
+    GemmArgs x, w;
+    int x_blocks, w_blocks;
+    const float* sums;    // [sum_rows, Z]
+    uint16_t* bias_grad;  // null: not wanted
+    int Z, sum_rows;
+};
+
+// kernels' launches; prepare_*: their LDS limits on the current device, before the first launch of a call
+hipError_t prepare_gemm_mid();
+hipError_t prepare_gemm_stream();
+hipError_t prepare_gemm_tiled();
 hipError_t launch_gemm_mid(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, bool direct, int bm,
                            hipStream_t stream);
+// grad_x (bm rows a tile) and grad_W (both operands by k) together; 16-byte copies
+hipError_t launch_gemm_pair(const GemmArgs& x, const GemmArgs& w, bool q_by_k, bool bf16, int bm, hipStream_t stream);
+hipError_t launch_grad_tail(GradTail t, bool bf16, hipStream_t stream);
+// at most 64 rows, both operands by rows, 16-byte loads
+hipError_t launch_gemm_stream(const GemmArgs& g, bool bf16, hipStream_t stream);
 // 256 x 256 tiles; operands that 16-byte copies can read
 hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);

@@ -27,6 +27,8 @@ class TraceScope {
 // Raises kernel `fn`'s dynamic-LDS limit to `lds_max` bytes on the current device (once per device and kernel;
 // needed above 64 KB). Returns the HIP error of that call, hipSuccess when it was already done.
 hipError_t ensure_lds_limit(const void* fn, int lds_max);
+// The same for all kernels of the dense products: the first call on a device sets them, later ones cost one lookup.
+hipError_t prepare_linear();
 // Workgroups of `fn` (`threads` threads, `lds` bytes of dynamic LDS) the current device holds at once, cached per
 // device, kernel and LDS size; 0 when the device cannot be queried.
 int resident_workgroups(const void* fn, int threads, size_t lds);
@@ -192,11 +194,11 @@ hipError_t launch_group_routing_grad(const GroupRouting& r, const void* grad_wei
 
 // ---- dense products (moe_linear*.hip) ----
 enum Activation { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActSwiglu = 5 };
-// dz = dy * act'(pre) with rows of ldz (zeros past Z); bias_grad (null: not wanted) = column sums through `part`
-// (act_grad_row_blocks(T, Z) * Z floats); dz null: the sums alone
+// dz = dy * act'(pre) with rows of ldz (zeros past Z); part (null: not wanted) gets the column sums of
+// act_grad_row_blocks(T, Z) blocks of rows, Z floats each; dz null: the sums alone
 int act_grad_row_blocks(int64_t T, int Z);
 hipError_t launch_act_grad(const uint16_t* dy, int64_t ldy, const uint16_t* pre, uint16_t* dz, int64_t ldz, float* part,
-                           uint16_t* bias_grad, int64_t T, int N, int act, bool bf16, hipStream_t stream);
+                           int64_t T, int N, int act, bool bf16, hipStream_t stream);
 
 // ---- synthetic inputs / calibration (moe_synth.hip) ----
 hipError_t launch_synth_normal_f16(uint16_t* out, uint64_t n, uint64_t seed, uint64_t stream_id, double sigma_a,

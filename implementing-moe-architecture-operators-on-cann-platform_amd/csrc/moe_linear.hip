@@ -62,12 +62,26 @@ __device__ __forceinline__ void read_fragments(const uint16_t* tile, int r0, int
     }
 }
 
+// 8 consecutive elements (of a row's k, or by k of rows) from an operand of any alignment, zeros past its end
+__device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, bool by_k, int row, int k, int rows, int k1) {
+    typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (row >= rows || k >= k1) return v;
+    const uint16_t* at = p + (by_k ? static_cast<int64_t>(k) * ld + row : static_cast<int64_t>(row) * ld + k);
+    const int valid = by_k ? rows - row : k1 - k;
+    if (valid >= 8) return *reinterpret_cast<const s16x8_any*>(at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < valid) v[e] = static_cast<short>(at[e]);
+    return v;
+}
+
 // C[m][n] tile of BM x 128 (4 waves), one ring of direct-to-LDS stages, one barrier a stage.
 // DIRECT: both operands allow 16-byte copies (bases and row pitches 16-byte aligned, by rows k % 8 == 0). Otherwise the
-// elements are loaded one by one and written to the same layout.
+// granules come through registers (loads of any alignment) and are written to the same layout.
+// block of grid: this product's share of the launch, grid a multiple of the XCDs.
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
-__global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
-    extern __shared__ __align__(16) uint16_t lds[];
+__device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntiles, int block, int grid, uint16_t* lds) {
     constexpr int NS = ring_stages(BM);
     constexpr int WM = BM >= 128 ? 2 : 1, WN = 4 / WM;  // waves along m and n
     constexpr int FM = BM / WM / 16, FN = kBN / WN / 16;  // 16 x 16 blocks of a wave
@@ -78,12 +92,14 @@ __global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtil
     const int wm = wave / WN, wn = wave % WN;
     const int row16 = lane & 15, kg = lane >> 4;
 
-    // Workgroups go round-robin over the XCDs; each XCD takes a contiguous run of the items (n-tile, split, m-tile), m
-    // fastest, so the m-tiles that read the same piece of Q share an L2.
-    const int per_xcd = static_cast<int>(gridDim.x) / kXcds;
-    const int item = (static_cast<int>(blockIdx.x) % kXcds) * per_xcd + static_cast<int>(blockIdx.x) / kXcds;
+    // Workgroups go round-robin over the XCDs; each XCD takes a contiguous run of the items. The tiles that read the same
+    // piece of the larger operand are neighbours in it, so that piece reaches that XCD's L2 once.
+    const int item = block % kXcds * (grid / kXcds) + block / kXcds;
     if (item >= mtiles * ntiles * g.splits) return;
-    const int mt = item % mtiles, sp = item / mtiles % g.splits, nt = item / mtiles / g.splits;
+    const bool n_first = mtiles > ntiles;
+    const int inner = n_first ? ntiles : mtiles, outer = item / inner;
+    const int i0 = item - outer * inner, sp = outer % g.splits, o0 = outer / g.splits;
+    const int mt = n_first ? o0 : i0, nt = n_first ? i0 : o0;
     const int k0 = sp * g.split_k, k1 = min(g.k, k0 + g.split_k);
     const int nst = max(1, (k1 - k0 + kBK - 1) / kBK);
     const int m0 = mt * BM, n0 = nt * (SWIGLU ? kBN / 2 : kBN);
@@ -145,28 +161,14 @@ __global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtil
         } else {
 #pragma unroll
             for (int c = 0; c < PC; ++c) {
-                s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int row = m0 + (PK ? pel[c] + e : prow[c]), k = kc + (PK ? prow[c] : pel[c] + e);
-                    if (row < g.m && k < k1)
-                        v[e] = static_cast<short>(PK ? g.p[static_cast<int64_t>(k) * g.ldp + row]
-                                                     : g.p[static_cast<int64_t>(row) * g.ldp + k]);
-                }
+                const int row = m0 + (PK ? pel[c] : prow[c]), k = kc + (PK ? prow[c] : pel[c]);
+                const s16x8 v = load_granule(g.p, g.ldp, PK, row, k, g.m, k1);
                 *reinterpret_cast<s16x8*>(slot + (wave * PC + c) * 512 + lane * 8) = v;
             }
 #pragma unroll
             for (int c = 0; c < QC; ++c) {
-                s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int tr = QK ? qel[c] + e : qrow[c], col = q_col(tr);
-                    const int k = kc + (QK ? qrow[c] : qel[c] + e);
-                    const int64_t row = col + (q_up(tr) ? g.n : 0);
-                    if (col < g.n && k < k1)
-                        v[e] = static_cast<short>(QK ? g.q[static_cast<int64_t>(k) * g.ldq + row]
-                                                     : g.q[row * g.ldq + k]);
-                }
+                const int tr = QK ? qel[c] : qrow[c], up = q_up(tr) ? g.n : 0;
+                const s16x8 v = load_granule(g.q, g.ldq, QK, q_col(tr) + up, kc + (QK ? qrow[c] : qel[c]), g.n + up, k1);
                 *reinterpret_cast<s16x8*>(slot + BM * kBK + (wave * QC + c) * 512 + lane * 8) = v;
             }
         }
@@ -228,17 +230,52 @@ __global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtil
 }
 
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
+__global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
+    extern __shared__ __align__(16) uint16_t lds[];
+    gemm_mid<T, PK, QK, BM, SWIGLU, DIRECT>(g, mtiles, ntiles, static_cast<int>(blockIdx.x),
+                                            static_cast<int>(gridDim.x), lds);
+}
+
+// Both gradient products in one launch: neither needs the other, and small ones leave the GPU half empty. The first
+// x_blocks workgroups have grad_x.
+template <typename T, bool QK, int BM>
+__global__ __launch_bounds__(kThreads) void gemm_pair_kernel(GemmArgs x, GemmArgs w, int x_blocks) {
+    extern __shared__ __align__(16) uint16_t lds[];
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < x_blocks)
+        gemm_mid<T, false, QK, BM, false, true>(x, (x.m + BM - 1) / BM, (x.n + kBN - 1) / kBN, block, x_blocks, lds);
+    else
+        gemm_mid<T, true, true, 128, false, true>(w, (w.m + 127) / 128, (w.n + kBN - 1) / kBN, block - x_blocks,
+                                                  static_cast<int>(gridDim.x) - x_blocks, lds);
+}
+
+int mid_grid(const GemmArgs& g, int bm, int bn) {
+    const int64_t items = static_cast<int64_t>((g.m + bm - 1) / bm) * ((g.n + bn - 1) / bn) * g.splits;
+    return static_cast<int>((items + kXcds - 1) / kXcds * kXcds);
+}
+
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
 hipError_t run_mid(const GemmArgs& g, hipStream_t stream) {
-    const int bn = SWIGLU ? kBN / 2 : kBN;
-    const int mtiles = (g.m + BM - 1) / BM, ntiles = (g.n + bn - 1) / bn;
-    const int64_t items = static_cast<int64_t>(mtiles) * ntiles * g.splits;
-    const int grid = static_cast<int>((items + kXcds - 1) / kXcds * kXcds);
-    auto fn = &gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT>;
-    const hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(fn), mid_lds_bytes(BM));
-    if (err != hipSuccess) return err;
+    constexpr int kCols = SWIGLU ? kBN / 2 : kBN;
     TraceScope trace("moe_linear_gemm", stream);
-    fn<<<grid, kThreads, mid_lds_bytes(BM), stream>>>(g, mtiles, ntiles);
+    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT><<<mid_grid(g, BM, kCols), kThreads, mid_lds_bytes(BM), stream>>>(
+        g, (g.m + BM - 1) / BM, (g.n + kCols - 1) / kCols);
     return hipGetLastError();
+}
+
+template <typename T, bool QK, int BM>
+hipError_t run_pair(const GemmArgs& x, const GemmArgs& w, hipStream_t stream) {
+    constexpr int kLds = mid_lds_bytes(BM) > mid_lds_bytes(128) ? mid_lds_bytes(BM) : mid_lds_bytes(128);
+    const int x_blocks = mid_grid(x, BM, kBN);
+    TraceScope trace("moe_linear_gemm", stream);
+    gemm_pair_kernel<T, QK, BM><<<x_blocks + mid_grid(w, 128, kBN), kThreads, kLds, stream>>>(x, w, x_blocks);
+    return hipGetLastError();
+}
+template <typename T>
+hipError_t run_pair_any(const GemmArgs& x, const GemmArgs& w, bool q_by_k, int bm, hipStream_t stream) {
+    if (bm == 32) return q_by_k ? run_pair<T, true, 32>(x, w, stream) : run_pair<T, false, 32>(x, w, stream);
+    if (bm == 64) return q_by_k ? run_pair<T, true, 64>(x, w, stream) : run_pair<T, false, 64>(x, w, stream);
+    return q_by_k ? run_pair<T, true, 128>(x, w, stream) : run_pair<T, false, 128>(x, w, stream);
 }
 
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU>
@@ -256,6 +293,12 @@ hipError_t run_mid_any(const GemmArgs& g, bool p_by_k, bool q_by_k, bool direct,
         return swiglu ? run_mid_direct<T, false, false, 128, true>(g, direct, stream)
                       : run_mid_direct<T, false, false, 128, false>(g, direct, stream);
     }
+    if (bm == 64) {
+        if (q_by_k) return swiglu ? run_mid_direct<T, false, true, 64, true>(g, direct, stream)
+                                  : run_mid_direct<T, false, true, 64, false>(g, direct, stream);
+        return swiglu ? run_mid_direct<T, false, false, 64, true>(g, direct, stream)
+                      : run_mid_direct<T, false, false, 64, false>(g, direct, stream);
+    }
     if (q_by_k) return swiglu ? run_mid_direct<T, false, true, 32, true>(g, direct, stream)
                               : run_mid_direct<T, false, true, 32, false>(g, direct, stream);
     return swiglu ? run_mid_direct<T, false, false, 32, true>(g, direct, stream)
@@ -264,10 +307,11 @@ hipError_t run_mid_any(const GemmArgs& g, bool p_by_k, bool q_by_k, bool direct,
 
 // Adds the splits' sums in order and applies the epilogue; a thread has 4 columns of a row.
 constexpr int kReduceThreads = 256;
+int64_t reduce_blocks(const GemmArgs& g) { return (part_cols(g.n) / 4 * g.m + kReduceThreads - 1) / kReduceThreads; }
 template <typename T, bool SWIGLU>
-__global__ __launch_bounds__(kReduceThreads) void gemm_reduce_kernel(GemmArgs g) {
+__device__ __forceinline__ void gemm_reduce(const GemmArgs& g, int block) {
     const int64_t pcols = part_cols(g.n), pld = part_ld(g.n, SWIGLU), per_row = pcols / 4;
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * kReduceThreads + threadIdx.x;
+    const int64_t idx = static_cast<int64_t>(block) * kReduceThreads + threadIdx.x;
     if (idx >= per_row * g.m) return;
     const int64_t row = idx / per_row;
     const int col = static_cast<int>(idx % per_row) * 4;
@@ -281,6 +325,39 @@ __global__ __launch_bounds__(kReduceThreads) void gemm_reduce_kernel(GemmArgs g)
         if (SWIGLU) u += *reinterpret_cast<const f32x4*>(src + s * step + pcols);
     }
     store4<T, SWIGLU>(g, row, col, z, u, vector_rows(g));
+}
+template <typename T, bool SWIGLU>
+__global__ __launch_bounds__(kReduceThreads) void gemm_reduce_kernel(GemmArgs g) {
+    gemm_reduce<T, SWIGLU>(g, static_cast<int>(blockIdx.x));
+}
+
+// What is left of a training step's gradients in one launch: the split products' sums and the bias's column sums
+template <typename T>
+__global__ __launch_bounds__(kReduceThreads) void grad_tail_kernel(GradTail t) {
+    int block = static_cast<int>(blockIdx.x);
+    if (block < t.x_blocks) return gemm_reduce<T, false>(t.x, block);
+    block -= t.x_blocks;
+    if (block < t.w_blocks) return gemm_reduce<T, false>(t.w, block);
+    column_sums<T>(t.sums, t.bias_grad, t.Z, t.sum_rows, block - t.w_blocks);
+}
+
+template <typename T, int BM>
+hipError_t prepare_bm() {
+    const int lds = mid_lds_bytes(BM);
+    for (const void* fn : {reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, false, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, true, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, true, BM, false, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, true, BM, true, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, false, false>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, true, false>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, true, BM, false, false>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, true, BM, true, false>),
+                           reinterpret_cast<const void*>(&gemm_pair_kernel<T, false, BM>),
+                           reinterpret_cast<const void*>(&gemm_pair_kernel<T, true, BM>)}) {
+        const hipError_t err = ensure_lds_limit(fn, lds);
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -304,6 +381,29 @@ hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream) 
         else gemm_reduce_kernel<Half, false><<<grid, kReduceThreads, 0, stream>>>(g);
     }
     return hipGetLastError();
+}
+
+hipError_t launch_gemm_pair(const GemmArgs& x, const GemmArgs& w, bool q_by_k, bool bf16, int bm, hipStream_t stream) {
+    return bf16 ? run_pair_any<Bf16>(x, w, q_by_k, bm, stream) : run_pair_any<Half>(x, w, q_by_k, bm, stream);
+}
+
+hipError_t launch_grad_tail(GradTail t, bool bf16, hipStream_t stream) {
+    t.x_blocks = t.x.splits > 1 ? static_cast<int>(reduce_blocks(t.x)) : 0;
+    t.w_blocks = t.w.splits > 1 ? static_cast<int>(reduce_blocks(t.w)) : 0;
+    const int grid = t.x_blocks + t.w_blocks + (t.bias_grad ? (t.Z + kSumColumns - 1) / kSumColumns : 0);
+    if (grid == 0) return hipSuccess;
+    TraceScope trace("moe_linear_reduce", stream);
+    if (bf16) grad_tail_kernel<Bf16><<<grid, kReduceThreads, 0, stream>>>(t);
+    else grad_tail_kernel<Half><<<grid, kReduceThreads, 0, stream>>>(t);
+    return hipGetLastError();
+}
+
+hipError_t prepare_gemm_mid() {  // 128-row tiles keep within 64 KB
+    hipError_t err = prepare_bm<Half, 32>();
+    if (err == hipSuccess) err = prepare_bm<Half, 64>();
+    if (err == hipSuccess) err = prepare_bm<Bf16, 32>();
+    if (err == hipSuccess) err = prepare_bm<Bf16, 64>();
+    return err;
 }
 
 }  // namespace moe

@@ -6,8 +6,8 @@
 // read it with 16-byte copies whatever the width.
 // Memory bound: dy and z read once, dz written once (SwiGLU: 5 values per output). One workgroup has 64 lanes x 8 columns
 // of a block of rows (the 4 waves take rows in turn), so a wave's access is 1 KB of one row; a SwiGLU lane does the gate
-// and the up column together. Rows off 16 bytes are read element by element. Column sums go through LDS in wave order to
-// one row of `part`; colsum_kernel adds those in a fixed order: no atomics, so the result does not depend on timing.
+// and the up column together. Rows off 16 bytes take loads of any alignment. Column sums go through LDS in wave order to
+// one row of `part`; column_sums adds those in a fixed order: no atomics, so the result does not depend on timing.
 #include "moe_gemm.h"
 
 namespace moe {
@@ -20,15 +20,17 @@ constexpr int kCols = 512;  // columns of a workgroup
 __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
         case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
-        case kActGelu:
-            return 0.5f * erfcf(z * -0.70710678118654752f) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+        case kActGelu: {
+            float e;
+            const float c = normal_cdf(z, e);
+            return c + z * 0.39894228040143268f * e;
+        }
         case kActGeluTanh: {
-            const float a = 0.79788456080286536f, b = 0.044715f;
-            const float t = tanhf(a * (z + b * z * z * z));
-            return 0.5f * (1.0f + t) + 0.5f * z * (1.0f - t * t) * a * (1.0f + 3.0f * b * z * z);
+            const float s = sigmoid_fast(kTanhA * (z + kTanhB * z * z * z));
+            return s * (1.0f + z * (1.0f - s) * kTanhA * (1.0f + 3.0f * kTanhB * z * z));
         }
         case kActSilu: {
-            const float s = 1.0f / (1.0f + expf(-z));
+            const float s = sigmoid_fast(z);
             return s * (1.0f + z * (1.0f - s));
         }
         default: return 1.0f;
@@ -49,31 +51,60 @@ struct ActGradArgs {
 
 // How the columns of a workgroup are read and computed
 enum Mode {
-    kScalar = 0,  // any width and alignment, dz's columns
-    kVector = 1,  // 16-byte loads
-    kPairs = 2    // 16-byte loads, SwiGLU: y's columns, gate and up together
+    kAny = 0,     // any width and alignment, dz's columns
+    kVector = 1,  // aligned 16-byte loads
+    kPairs = 2    // aligned 16-byte loads, SwiGLU: y's columns, gate and up together
 };
 
-// 8 columns of one dz row from column c on: SwiGLU columns below N are the gate's, the others up's
+// 8 values of a row from p on, of which `valid` exist; any alignment
+__device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid) {
+    typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+    if (valid >= 8) return *reinterpret_cast<const s16x8_any*>(p);
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < valid) v[e] = static_cast<short>(p[e]);
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float at(const s16x8& v, int e) {
+    return T::load(static_cast<uint16_t>(v[e]));
+}
+
+// 8 columns of one dz row from column c on, zeros from Z on: SwiGLU columns below N are the gate's, the others up's
 template <typename T>
 __device__ __forceinline__ void dz8(const ActGradArgs& a, int64_t t, int c, float (&v)[8]) {
+    const uint16_t *dy = a.dy + t * a.ldy, *pre = a.pre + t * a.Z;
+    if (a.act == kActSwiglu) {
+        const bool up = c >= a.N;
+        const int n = up ? c - a.N : c, valid = a.N - n;
+        if (valid >= 8 || (up && valid > 0)) {  // all gate or all up
+            const s16x8 d = load8(dy + n, valid), zg = load8(pre + n, valid), zu = load8(pre + a.N + n, valid);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int col = c + e;
-        v[e] = 0.0f;
-        if (col >= a.Z) continue;
-        if (a.act == kActSwiglu) {
-            const bool up = col >= a.N;
-            const int n = up ? col - a.N : col;
-            const float dy = T::load(a.dy[t * a.ldy + n]);
-            const float zg = T::load(a.pre[t * a.Z + n]);
-            const float s = 1.0f / (1.0f + expf(-zg));
-            v[e] = up ? dy * zg * s : dy * T::load(a.pre[t * a.Z + a.N + n]) * s * (1.0f + zg * (1.0f - s));
-        } else {
-            const float dy = T::load(a.dy[t * a.ldy + col]);
-            v[e] = a.pre ? dy * slope(T::load(a.pre[t * a.Z + col]), a.act) : dy;
+            for (int e = 0; e < 8; ++e) {
+                const float g = at<T>(zg, e), s = sigmoid_fast(g);
+                v[e] = e >= valid ? 0.0f : at<T>(d, e) * (up ? g * s : at<T>(zu, e) * s * (1.0f + g * (1.0f - s)));
+            }
+            return;
         }
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {  // the last gate columns and the first up columns
+            const int col = c + e, m = col < a.N ? col : col - a.N;
+            float x = 0.0f;
+            if (col < a.Z) {
+                const float d = T::load(dy[m]), g = T::load(pre[m]), s = sigmoid_fast(g);
+                x = d * (col < a.N ? T::load(pre[a.N + m]) * s * (1.0f + g * (1.0f - s)) : g * s);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i == e) v[i] = x;
+        }
+        return;
     }
+    const s16x8 d = load8(dy + c, a.Z - c), z = a.pre ? load8(pre + c, a.Z - c) : s16x8{};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = a.pre ? at<T>(d, e) * slope(at<T>(z, e), a.act) : at<T>(d, e);
 }
 
 template <typename T>
@@ -98,7 +129,7 @@ __global__ __launch_bounds__(kThreads) void act_grad_kernel(ActGradArgs a) {
 #pragma unroll 2
         for (int64_t t = t0 + wave; t < t1; t += kThreads / kWave) {
             float v[kSums][8];
-            if constexpr (MODE == kScalar) {
+            if constexpr (MODE == kAny) {
                 dz8<T>(a, t, c, v[0]);
             } else {
                 const s16x8 d = *reinterpret_cast<const s16x8*>(a.dy + t * a.ldy + c);
@@ -109,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void act_grad_kernel(ActGradArgs a) {
                 for (int e = 0; e < 8; ++e) {
                     const float dy = T::load(static_cast<uint16_t>(d[e])), zg = T::load(static_cast<uint16_t>(z[e]));
                     if (MODE == kPairs) {
-                        const float s = 1.0f / (1.0f + expf(-zg));
+                        const float s = sigmoid_fast(zg);
                         v[0][e] = dy * T::load(static_cast<uint16_t>(u[e])) * s * (1.0f + zg * (1.0f - s));
                         v[kSums - 1][e] = dy * zg * s;
                     } else {
@@ -143,27 +174,6 @@ __global__ __launch_bounds__(kThreads) void act_grad_kernel(ActGradArgs a) {
     }
 }
 
-// 16 columns a workgroup; its 16 groups of threads add every 16th row of `part`, then the groups' sums in order
-constexpr int kGroups = 16, kColsSum = kThreads / kGroups;
-template <typename T>
-__global__ __launch_bounds__(kThreads) void colsum_kernel(const float* __restrict__ part, uint16_t* __restrict__ out,
-                                                          int Z, int blocks) {
-    __shared__ float sums[kGroups][kColsSum];
-    const int i = static_cast<int>(threadIdx.x) % kColsSum, q = static_cast<int>(threadIdx.x) / kColsSum;
-    const int c = static_cast<int>(blockIdx.x) * kColsSum + i;
-    float s = 0.0f;
-    if (c < Z) {
-#pragma unroll 4
-        for (int b = q; b < blocks; b += kGroups) s += part[static_cast<int64_t>(b) * Z + c];
-    }
-    sums[q][i] = s;
-    __syncthreads();
-    if (q != 0 || c >= Z) return;
-#pragma unroll
-    for (int g = 1; g < kGroups; ++g) s += sums[g][i];
-    out[c] = T::store(s);
-}
-
 template <typename T>
 hipError_t run_act_grad(const ActGradArgs& a, int blocks, hipStream_t stream) {
     const bool aligned = a.N % 8 == 0 && a.ldy % 8 == 0 &&
@@ -174,28 +184,28 @@ hipError_t run_act_grad(const ActGradArgs& a, int blocks, hipStream_t stream) {
     TraceScope trace("moe_linear_act_grad", stream);
     if (pairs) act_grad_kernel<T, kPairs><<<grid, kThreads, 0, stream>>>(a);
     else if (aligned) act_grad_kernel<T, kVector><<<grid, kThreads, 0, stream>>>(a);
-    else act_grad_kernel<T, kScalar><<<grid, kThreads, 0, stream>>>(a);
+    else act_grad_kernel<T, kAny><<<grid, kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int act_grad_row_blocks(int64_t T, int Z) {
-    // about 2048 workgroups over rows and columns, at least 16 rows each (the partial sums stay small beside dz)
+    // about 2048 workgroups over rows and columns, at least 8 rows each (two a wave)
     const int64_t cols = (Z + kCols - 1) / kCols;
     const int64_t want = cols > 2048 ? 1 : 2048 / cols;
-    const int64_t most = (T + 15) / 16;
+    const int64_t most = (T + 7) / 8;
     const int64_t n = want < most ? want : most;
     return static_cast<int>(n < 1 ? 1 : n);
 }
 
 hipError_t launch_act_grad(const uint16_t* dy, int64_t ldy, const uint16_t* pre, uint16_t* dz, int64_t ldz, float* part,
-                           uint16_t* bias_grad, int64_t T, int N, int act, bool bf16, hipStream_t stream) {
+                           int64_t T, int N, int act, bool bf16, hipStream_t stream) {
     ActGradArgs a{};
     a.dy = dy;
     a.pre = pre;
     a.dz = dz;
-    a.part = bias_grad ? part : nullptr;
+    a.part = part;
     a.ldy = ldy;
     a.ldz = ldz;
     a.T = T;
@@ -204,15 +214,7 @@ hipError_t launch_act_grad(const uint16_t* dy, int64_t ldy, const uint16_t* pre,
     a.act = act;
     const int blocks = act_grad_row_blocks(T, a.Z);
     a.rows_per_block = (T + blocks - 1) / blocks;
-    hipError_t err = bf16 ? run_act_grad<Bf16>(a, blocks, stream) : run_act_grad<Half>(a, blocks, stream);
-    if (err != hipSuccess || !bias_grad) return err;
-    {
-        TraceScope trace("moe_linear_bias_grad", stream);
-        const int cgrid = (a.Z + kColsSum - 1) / kColsSum;
-        if (bf16) colsum_kernel<Bf16><<<cgrid, kThreads, 0, stream>>>(part, bias_grad, a.Z, blocks);
-        else colsum_kernel<Half><<<cgrid, kThreads, 0, stream>>>(part, bias_grad, a.Z, blocks);
-    }
-    return hipGetLastError();
+    return bf16 ? run_act_grad<Bf16>(a, blocks, stream) : run_act_grad<Half>(a, blocks, stream);
 }
 
 }  // namespace moe

@@ -318,8 +318,6 @@ template <typename T, bool PK, bool QK, bool SWIGLU>
 hipError_t run_tiled(const GemmArgs& g, hipStream_t stream) {
     auto fn = &gemm_tiled_kernel<T, PK, QK, SWIGLU>;
     const void* p = reinterpret_cast<const void*>(fn);
-    const hipError_t err = ensure_lds_limit(p, kLdsBytes);
-    if (err != hipSuccess) return err;
     const int bn = SWIGLU ? kBN / 2 : kBN;
     const int mtiles = (g.m + kBM - 1) / kBM, ntiles = (g.n + bn - 1) / bn;
     int grid = resident_workgroups(p, kThreads, kLdsBytes) / kXcds * kXcds;
@@ -339,7 +337,25 @@ hipError_t run_tiled_any(const GemmArgs& g, bool p_by_k, bool q_by_k, hipStream_
     return q_by_k ? run_tiled<T, false, true, false>(g, stream) : run_tiled<T, false, false, false>(g, stream);
 }
 
+template <typename T>
+hipError_t prepare() {
+    for (const void* fn : {reinterpret_cast<const void*>(&gemm_tiled_kernel<T, true, true, false>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, true, true>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, false, true>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, true, false>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, false, false>)}) {
+        const hipError_t err = ensure_lds_limit(fn, kLdsBytes);
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
+}
+
 }  // namespace
+
+hipError_t prepare_gemm_tiled() {
+    const hipError_t err = prepare<Half>();
+    return err == hipSuccess ? prepare<Bf16>() : err;
+}
 
 hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream) {
     return bf16 ? run_tiled_any<Bf16>(g, p_by_k, q_by_k, stream) : run_tiled_any<Half>(g, p_by_k, q_by_k, stream);

@@ -6,9 +6,11 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <mutex>
 #include <vector>
 
+#include "moe_gemm.h"
 #include "moe_launch.h"
 
 namespace moe {
@@ -66,6 +68,20 @@ int resident_workgroups(const void* fn, int threads, size_t lds) {
     const int n = cus * (per_cu > 0 ? per_cu : 1);
     g_resident.push_back(Resident{dev, fn, threads, lds, n});
     return n;
+}
+
+hipError_t prepare_linear() {
+    static std::atomic<uint64_t> ready{0};  // devices below 64
+    int dev = 0;
+    hipError_t err = hipGetDevice(&dev);
+    if (err != hipSuccess) return err;
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (ready.load(std::memory_order_acquire) & bit) return hipSuccess;
+    err = prepare_gemm_mid();
+    if (err == hipSuccess) err = prepare_gemm_stream();
+    if (err == hipSuccess) err = prepare_gemm_tiled();
+    if (err == hipSuccess) ready.fetch_or(bit, std::memory_order_release);
+    return err;
 }
 
 }  // namespace moe

@@ -270,40 +270,62 @@ def moe_layer_fused(x: torch.Tensor, w_gate: torch.Tensor, expert_weights: torch
 # ---------------------------------------------------------------------------------------------------------------------
 
 
-def _need_float(t, name: str, dtypes, device, dims: int | None = None) -> int:
-    """Checks a floating device tensor of any strides; returns its moe_dtype."""
+_F16_32 = (torch.float16, torch.float32)
+_HALVES = (torch.float16, torch.bfloat16)
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _here() -> int:
+    """The current device, on whose stream a call is queued: its tensors have to be there."""
+    return torch.cuda.current_device() if _device is None else _device()
+
+
+def _first_float(t, name: str, dtypes, dims: int) -> tuple[int, int]:
+    """Checks a call's first tensor; returns its moe_dtype and the device that all the others have to be on."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _need_float(t, name, dtypes, dims, -1)  # raises
+    dev = t.get_device()
+    code = _need_float(t, name, dtypes, dims, dev)
+    if dev != _here():
+        raise MoeError(4, f"{name} is on cuda:{dev}, the current device is cuda:{_here()}")
+    return code, dev
+
+
+def _need_float(t, name: str, dtypes, dims: int, dev: int) -> int:
+    """Checks a floating tensor of any strides on device `dev`; returns its moe_dtype."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == dims and t.get_device() == dev:
+        return _FLOAT_DT[t.dtype]
     if not isinstance(t, torch.Tensor):
         raise MoeError(1, f"{name} must be a tensor")
     if t.device.type != "cuda":
         raise MoeError(4, f"{name} must be a device tensor (got {t.device})")
-    if device is not None and t.device != device:
-        raise MoeError(4, f"{name} is on {t.device}, the first tensor on {device}")
     if t.dtype not in dtypes:
         raise MoeError(4, f"{name} must be {' or '.join(str(d) for d in dtypes)} (got {t.dtype})")
-    if dims is not None and t.dim() != dims:
+    if t.dim() != dims:
         raise MoeError(2, f"{name} must have {dims} dimensions (got {t.dim()})")
-    return _FLOAT_DT[t.dtype]
+    raise MoeError(4, f"{name} is on {t.device}, the first tensor on cuda:{dev}")
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Elements between the rows of a 2-D tensor whose rows are contiguous."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    st, one = t.stride()
+    if one != 1 and t.shape[1] > 1:
         raise MoeError(4, f"{name}: the elements of a row must be contiguous (strides {t.stride()})")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return st if t.shape[0] > 1 else max(st, t.shape[1])
 
 
 def _weight_layout(t: torch.Tensor) -> tuple[int, int]:
     """(stride, transposed) of a 2-D weight that is contiguous along one of its dimensions."""
-    n, h = t.shape
-    if h == 1 or t.stride(1) == 1:
-        return (t.stride(0) if n > 1 else max(t.stride(0), h)), 0
-    if n == 1 or t.stride(0) == 1:
-        return (t.stride(1) if h > 1 else max(t.stride(1), n)), 1
+    (n, h), (sn, sh) = t.shape, t.stride()
+    if sh == 1 or h == 1:
+        return (sn if n > 1 else max(sn, h)), 0
+    if sn == 1 or n == 1:
+        return (sh if h > 1 else max(sh, n)), 1
     raise MoeError(4, f"weight must be contiguous along one dimension (strides {t.stride()})")
 
 
 def _need_shape(t: torch.Tensor, name: str, shape) -> None:
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise MoeError(3, f"{name} shape {tuple(t.shape)} != {tuple(shape)}")
 
 
@@ -321,12 +343,39 @@ def _scoring_code(scoring: str) -> int:
     return code
 
 
-def _need_workspace(workspace, need: int, like, device):
+def _workspace(workspace, query, args, like, dev):
+    """(address, bytes) of the caller's workspace or of a new one (which the caller keeps until the launch)."""
     if workspace is None:
-        return like.new_empty(max(need, 1), dtype=torch.uint8)
-    if not isinstance(workspace, torch.Tensor) or workspace.device != device or not workspace.is_contiguous():
-        raise MoeError(4, f"workspace must be a contiguous tensor on {device}")
-    return workspace
+        need = int(query(*args))
+        if need == 0:
+            return None, None, 0
+        workspace = like.new_empty(need, dtype=torch.uint8)
+        return workspace, workspace.data_ptr(), need
+    if not isinstance(workspace, torch.Tensor) or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise MoeError(4, f"workspace must be a contiguous tensor on cuda:{dev}")
+    return workspace, workspace.data_ptr(), _bytes(workspace)
+
+
+def _vector(t, name: str, dtype, n: int, dev: int) -> int | None:
+    """The address of an optional contiguous vector."""
+    if t is None:
+        return None
+    _need_float(t, name, (dtype,), 1, dev)
+    _need_shape(t, name, (n,))
+    if not t.is_contiguous():
+        raise MoeError(4, f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _matrix(t, name: str, dtype, shape, dev: int) -> int | None:
+    """The address of an optional contiguous matrix."""
+    if t is None:
+        return None
+    _need_float(t, name, (dtype,), 2, dev)
+    _need_shape(t, name, shape)
+    if not t.is_contiguous():
+        raise MoeError(4, f"{name} must be contiguous (ND format)")
+    return t.data_ptr()
 
 
 def MoeRoutingGroupTopK(logits: torch.Tensor, bias: torch.Tensor | None = None, topK: int = 2, numGroups: int = 1,
@@ -339,14 +388,10 @@ def MoeRoutingGroupTopK(logits: torch.Tensor, bias: torch.Tensor | None = None, 
     two best (2); of the experts that stay the topK best are chosen, equal ones by lowest index. The weights are the
     chosen scores, without bias, over their sum (renormalize) and times scale. Experts whose logit is -inf or NaN
     are not available; picks a row has no expert left for are id -1, weight 0."""
-    lt = _need_float(logits, "logits", (torch.float32, torch.float16, torch.bfloat16), None, 2)
+    lt, dev = _first_float(logits, "logits", _FLOATS, 2)
     T, E = logits.shape
-    if bias is not None:
-        _need_float(bias, "bias", (torch.float32,), logits.device, 1)
-        _need_shape(bias, "bias", (E,))
-        if not bias.is_contiguous():
-            raise MoeError(4, "bias must be contiguous")
-    if weightsDtype not in (torch.float16, torch.float32):
+    bp = _vector(bias, "bias", torch.float32, E, dev)
+    if weightsDtype not in _F16_32:
         raise MoeError(4, f"weightsDtype must be float16 or float32 (got {weightsDtype})")
     ld = _row_stride(logits, "logits")
     if type(topK) is not int or topK < 1 or topK > E:
@@ -355,7 +400,7 @@ def MoeRoutingGroupTopK(logits: torch.Tensor, bias: torch.Tensor | None = None, 
     with _on(stream):
         ids = like.new_empty((T, topK), dtype=torch.int32)
         w = like.new_empty((T, topK), dtype=weightsDtype)
-    check(_lib.load().moe_routing_group_topk(logits.data_ptr(), ld, lt, _ptr(bias), ids.data_ptr(), w.data_ptr(),
+    check(_lib.load().moe_routing_group_topk(logits.data_ptr(), ld, lt, bp, ids.data_ptr(), w.data_ptr(),
                                              _FLOAT_DT[weightsDtype], T, E, topK, numGroups, topGroups, groupTop,
                                              _scoring_code(scoring), int(renormalize), scale, _stream_ptr(stream)))
     return ids, w
@@ -366,15 +411,16 @@ def MoeRoutingGroupTopKGrad(grad_weights: torch.Tensor, logits: torch.Tensor, ex
                             stream=None) -> torch.Tensor:
     """The gradient of MoeRoutingGroupTopK's weights -> the logits', [T,E] contiguous, of the logits' type.
     expert_ids are the forward's; the choice itself (and with it the bias) has no gradient."""
-    lt = _need_float(logits, "logits", (torch.float32, torch.float16, torch.bfloat16), None, 2)
+    lt, dev = _first_float(logits, "logits", _FLOATS, 2)
     T, E = logits.shape
-    gt = _need_float(grad_weights, "grad_weights", (torch.float32, torch.float16, torch.bfloat16), logits.device, 2)
+    gt = _need_float(grad_weights, "grad_weights", _FLOATS, 2, dev)
     _need(expert_ids, "expert_ids", torch.int32)
-    if expert_ids.device != logits.device:
+    if expert_ids.get_device() != dev:
         raise MoeError(4, f"expert_ids is on {expert_ids.device}, logits on {logits.device}")
-    if expert_ids.dim() != 2 or expert_ids.shape[0] != T:
-        raise MoeError(3, f"expert_ids shape {tuple(expert_ids.shape)} for {T} rows of logits")
-    _need_shape(grad_weights, "grad_weights", expert_ids.shape)
+    ks = expert_ids.shape
+    if len(ks) != 2 or ks[0] != T:
+        raise MoeError(3, f"expert_ids shape {tuple(ks)} for {T} rows of logits")
+    _need_shape(grad_weights, "grad_weights", ks)
     if not grad_weights.is_contiguous():
         raise MoeError(4, "grad_weights must be contiguous (ND format)")
     ld = _row_stride(logits, "logits")
@@ -382,7 +428,7 @@ def MoeRoutingGroupTopKGrad(grad_weights: torch.Tensor, logits: torch.Tensor, ex
     with _on(stream):
         grad = like.new_empty((T, E))
     check(_lib.load().moe_routing_group_topk_grad(grad_weights.data_ptr(), gt, logits.data_ptr(), ld, lt,
-                                                  expert_ids.data_ptr(), grad.data_ptr(), T, E, expert_ids.shape[1],
+                                                  expert_ids.data_ptr(), grad.data_ptr(), T, E, ks[1],
                                                   _scoring_code(scoring), int(renormalize), scale,
                                                   _stream_ptr(stream)))
     return grad
@@ -398,8 +444,9 @@ def MoeCombineGrad(grad_y: torch.Tensor, expert_out: torch.Tensor, weights: torc
     T, K, H = expert_out.shape
     _need_shape(grad_y, "grad_y", (T, H))
     _need_shape(weights, "weights", (T, K))
-    if grad_y.device != expert_out.device or weights.device != expert_out.device:
-        raise MoeError(4, "grad_y, expert_out and weights must be on one device")
+    dev = _here()
+    if expert_out.get_device() != dev or grad_y.get_device() != dev or weights.get_device() != dev:
+        raise MoeError(4, f"grad_y, expert_out and weights must be on the current device cuda:{dev}")
     like = _like(expert_out)
     with _on(stream):
         geo = like.new_empty((T, K, H))
@@ -437,34 +484,25 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     rows first. residual has y's type. With returnPre -> (y, pre): the sums before the activation, which MoeLinearGrad
     takes. `workspace` (uint8, >= linear_workspace_bytes) is allocated when not given."""
     act = _act_code(activation)
-    dt = _need_float(x, "x", (torch.float16, torch.bfloat16), None, 2)
-    _need_float(weight, "weight", (x.dtype,), x.device, 2)
+    dt, dev = _first_float(x, "x", _HALVES, 2)
+    dtype = x.dtype
+    _need_float(weight, "weight", (dtype,), 2, dev)
     T, H, N, Z = _linear_sizes(x, weight, act)
-    out = x.dtype if outDtype is None else outDtype
-    if out not in (x.dtype, torch.float32):
-        raise MoeError(4, f"outDtype must be {x.dtype} or float32 (got {out})")
+    out = dtype if outDtype is None else outDtype
+    if out is not dtype and out is not torch.float32:
+        raise MoeError(4, f"outDtype must be {dtype} or float32 (got {out})")
     ldx = _row_stride(x, "x")
     ldw, transposed = _weight_layout(weight)
-    if bias is not None:
-        _need_float(bias, "bias", (x.dtype,), x.device, 1)
-        _need_shape(bias, "bias", (Z,))
-        if not bias.is_contiguous():
-            raise MoeError(4, "bias must be contiguous")
-    if residual is not None:
-        _need_float(residual, "residual", (out,), x.device, 2)
-        _need_shape(residual, "residual", (T, N))
-        if not residual.is_contiguous():
-            raise MoeError(4, "residual must be contiguous (ND format)")
+    bp = _vector(bias, "bias", dtype, Z, dev)
+    rp = _matrix(residual, "residual", out, (T, N), dev)
     lib = _lib.load()
     like = _like(x)
     with _on(stream):
-        need = 0 if workspace is not None else int(lib.moe_linear_workspace_bytes(T, N, H, act))
-        workspace = _need_workspace(workspace, need, like, x.device)
+        workspace, wp, wb = _workspace(workspace, lib.moe_linear_workspace_bytes, (T, N, H, act), like, dev)
         y = like.new_empty((T, N), dtype=out)
         pre = like.new_empty((T, Z)) if returnPre else None
-    check(lib.moe_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, _ptr(bias), _ptr(residual),
-                         y.data_ptr(), _ptr(pre), workspace.data_ptr(), _bytes(workspace), T, N, H, act, dt,
-                         _FLOAT_DT[out], _stream_ptr(stream)))
+    check(lib.moe_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre), wp, wb, T,
+                         N, H, act, dt, _FLOAT_DT[out], _stream_ptr(stream)))
     return (y, pre) if returnPre else y
 
 
@@ -475,31 +513,26 @@ def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, p
     x's type, None where not asked for. pre is MoeLinear's (needed with an activation). The residual's gradient is
     grad_y. `workspace` (uint8, >= linear_grad_workspace_bytes) is allocated when not given."""
     act = _act_code(activation)
-    dt = _need_float(x, "x", (torch.float16, torch.bfloat16), None, 2)
-    _need_float(weight, "weight", (x.dtype,), x.device, 2)
-    _need_float(grad_y, "grad_y", (x.dtype,), x.device, 2)
+    dt, dev = _first_float(x, "x", _HALVES, 2)
+    dtype = x.dtype
+    _need_float(weight, "weight", (dtype,), 2, dev)
+    _need_float(grad_y, "grad_y", (dtype,), 2, dev)
     T, H, N, Z = _linear_sizes(x, weight, act)
     _need_shape(grad_y, "grad_y", (T, N))
     ldx, ldy = _row_stride(x, "x"), _row_stride(grad_y, "grad_y")
     ldw, transposed = _weight_layout(weight)
-    if act:
-        if pre is None:
-            raise MoeError(1, f"MoeLinearGrad needs pre with activation {activation!r}")
-        _need_float(pre, "pre", (x.dtype,), x.device, 2)
-        _need_shape(pre, "pre", (T, Z))
-        if not pre.is_contiguous():
-            raise MoeError(4, "pre must be contiguous (ND format)")
+    if act and pre is None:
+        raise MoeError(1, f"MoeLinearGrad needs pre with activation {activation!r}")
+    pp = _matrix(pre, "pre", dtype, (T, Z), dev) if act else None
     lib = _lib.load()
     like = _like(x)
     with _on(stream):
-        need = 0 if workspace is not None else int(lib.moe_linear_grad_workspace_bytes(T, N, H, act))
-        workspace = _need_workspace(workspace, need, like, x.device)
+        workspace, wp, wb = _workspace(workspace, lib.moe_linear_grad_workspace_bytes, (T, N, H, act), like, dev)
         gx = like.new_empty((T, H)) if gradX else None
         gw = like.new_empty((Z, H)) if gradWeight else None
         gb = like.new_empty((Z,)) if gradBias else None
-    check(lib.moe_linear_grad(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed,
-                              _ptr(pre) if act else None, _ptr(gx), _ptr(gw), _ptr(gb), workspace.data_ptr(),
-                              _bytes(workspace), T, N, H, act, dt, _stream_ptr(stream)))
+    check(lib.moe_linear_grad(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, pp,
+                              _ptr(gx), _ptr(gw), _ptr(gb), wp, wb, T, N, H, act, dt, _stream_ptr(stream)))
     return gx, gw, gb
 
 
