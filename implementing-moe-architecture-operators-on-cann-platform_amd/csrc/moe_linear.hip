@@ -125,38 +125,49 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
         qrow[c] = a.row;
         qel[c] = a.el;
     }
-    // Copies stage s. Offsets are relative to (by rows) the tile's first row, (by k) the stage's first k, with 64-bit
-    // arithmetic in the base alone, so an operand may be larger than 4 GiB.
+    // Byte offsets of this lane's granules, relative to (by rows) the tile's first row, (by k) the stage's first k; past
+    // every buffer where the operand has no such row. 64-bit arithmetic is in the bases alone, so an operand may be
+    // larger than 4 GiB. By rows the k offset of a stage is the instruction's scalar one.
+    uint32_t poff[PC], qoff[QC];
+    if (DIRECT) {
+        const uint32_t ppitch = static_cast<uint32_t>(g.ldp) * 2, qpitch = static_cast<uint32_t>(g.ldq) * 2;
+#pragma unroll
+        for (int c = 0; c < PC; ++c) {
+            const int row = m0 + (PK ? pel[c] : prow[c]);
+            poff[c] = row < g.m ? prow[c] * ppitch + (PK ? row : pel[c]) * 2u : kPastEnd;
+        }
+#pragma unroll
+        for (int c = 0; c < QC; ++c) {
+            const int tr = QK ? qel[c] : qrow[c], col = q_col(tr);
+            const uint32_t off = QK ? qrow[c] * qpitch + (col + (q_up(tr) ? g.n : 0)) * 2u : (col - n0) * qpitch + qel[c] * 2u;
+            qoff[c] = col < g.n ? off : kPastEnd;
+        }
+    }
+    const uint16_t* pbase = g.p + (PK ? 0 : static_cast<int64_t>(m0) * g.ldp);
+    const uint16_t* qbase = g.q + (QK ? 0 : static_cast<int64_t>(n0) * g.ldq);
     auto copy_stage = [&](int s) __attribute__((always_inline)) {
         uint16_t* slot = lds + (s % NS) * kSlot;
         const int kc = k0 + s * kBK;
         if (DIRECT) {
-            const uint32_t ppitch = static_cast<uint32_t>(g.ldp) * 2;
+            const int left = k1 - kc;  // granules from here on are zeros
             const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint16_t*>(g.p + static_cast<int64_t>(PK ? kc : m0) * g.ldp), 0, 0x7fffffff, 0x00020000);
+                const_cast<uint16_t*>(PK ? pbase + static_cast<int64_t>(kc) * g.ldp : pbase), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-            for (int c = 0; c < PC; ++c) {
-                const int row = m0 + (PK ? pel[c] : prow[c]), k = kc + (PK ? prow[c] : pel[c]);
-                const uint32_t off = prow[c] * ppitch + (PK ? row : k) * 2u;
+            for (int c = 0; c < PC; ++c)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     pr, (__attribute__((address_space(3))) void*)(slot + (wave * PC + c) * 512), 16,
-                    static_cast<int>(row < g.m && k < k1 ? off : kPastEnd), 0, 0, 0);
-            }
+                    static_cast<int>((PK ? prow[c] : pel[c]) < left ? poff[c] : kPastEnd), PK ? 0 : kc * 2, 0, 0);
 #pragma unroll
             for (int c = 0; c < QC; ++c) {
                 // by rows a copy instruction covers 8 rows, all gate or all up: the base tells them apart, so that the
                 // offsets stay within the tile
-                const int tr = QK ? qel[c] : qrow[c];
-                const int col = q_col(tr), k = kc + (QK ? qrow[c] : qel[c]);
-                const int64_t first = QK ? kc : n0 + (q_up((wave * QC + c) * 8) ? static_cast<int64_t>(g.n) : 0);
-                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                    const_cast<uint16_t*>(g.q + first * g.ldq), 0, 0x7fffffff, 0x00020000);
-                const uint32_t pitch = static_cast<uint32_t>(g.ldq) * 2;
-                const uint32_t off = QK ? qrow[c] * pitch + (col + (q_up(tr) ? g.n : 0)) * 2u
-                                        : (col - n0) * pitch + k * 2u;
+                const int64_t up = !QK && q_up((wave * QC + c) * 8) ? static_cast<int64_t>(g.n) * g.ldq : 0;
+                const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<uint16_t*>(QK ? qbase + static_cast<int64_t>(kc) * g.ldq : qbase + up), 0, 0x7fffffff,
+                    0x00020000);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    r, (__attribute__((address_space(3))) void*)(slot + BM * kBK + (wave * QC + c) * 512), 16,
-                    static_cast<int>(col < g.n && k < k1 ? off : kPastEnd), 0, 0, 0);
+                    qr, (__attribute__((address_space(3))) void*)(slot + BM * kBK + (wave * QC + c) * 512), 16,
+                    static_cast<int>((QK ? qrow[c] : qel[c]) < left ? qoff[c] : kPastEnd), QK ? 0 : kc * 2, 0, 0);
             }
         } else {
 #pragma unroll
@@ -230,7 +241,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 }
 
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
-__global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
     extern __shared__ __align__(16) uint16_t lds[];
     gemm_mid<T, PK, QK, BM, SWIGLU, DIRECT>(g, mtiles, ntiles, static_cast<int>(blockIdx.x),
                                             static_cast<int>(gridDim.x), lds);
@@ -239,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void gemm_mid_kernel(GemmArgs g, int mtil
 // Both gradient products in one launch: neither needs the other, and small ones leave the GPU half empty. The first
 // x_blocks workgroups have grad_x.
 template <typename T, bool QK, int BM>
-__global__ __launch_bounds__(kThreads) void gemm_pair_kernel(GemmArgs x, GemmArgs w, int x_blocks) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_pair_kernel(GemmArgs x, GemmArgs w, int x_blocks) {
     extern __shared__ __align__(16) uint16_t lds[];
     const int block = static_cast<int>(blockIdx.x);
     if (block < x_blocks)
