@@ -79,7 +79,7 @@ moe_status check_pitch(const char* op, const char* what, int64_t rows, int64_t w
     return ok();
 }
 
-// How one product runs: weight streaming, tiles of 32, 64 or 128 x 128 (split over k or not), or 256 x 256 tiles
+// How one product runs: weight streaming, tiles of 32 to 256 x 128 (split over k or not), or 256 x 256 tiles
 enum class Kernel { kStream, kMid, kTiled };
 struct ProductPlan {
     Kernel kernel;
@@ -91,25 +91,29 @@ struct ProductPlan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Microseconds of a launch by tiles of bm x 128 with `items` workgroups of `stages` 64-k stages: two share a CU. One
-// alone takes 0.45, 0.56 or 0.92 us a stage (32, 64, 128 rows), two together 0.7, 0.86 or 1.45 us.
+// Microseconds of a launch by tiles of bm x 128 with `items` workgroups of `stages` 64-k stages. Up to 128 rows two
+// workgroups share a CU: a stage takes 0.3, 0.38 or 0.78 us (32, 64, 128 rows) alone and 0.65, 0.78 or 1.19 us beside
+// another. At 256 rows a CU has one: 0.87 us with few of them, 1.13 with one on every CU.
 double mid_time(int bm, int64_t items, int64_t stages) {
-    const double one = bm == 32 ? 0.45 : bm == 64 ? 0.56 : 0.92, two = bm == 32 ? 0.7 : bm == 64 ? 0.86 : 1.45;
-    const int64_t rest = items % 512;
-    const double tail = rest == 0 ? 0.0 : rest <= 256 ? one : one + (two - one) * (rest / 256.0 - 1.0);
-    return 3.0 + stages * (static_cast<double>(items / 512) * two + tail);
+    const double one = bm == 32 ? 0.30 : bm == 64 ? 0.38 : bm == 128 ? 0.78 : 0.87;
+    const double two = bm == 32 ? 0.65 : bm == 64 ? 0.78 : bm == 128 ? 1.19 : 1.13;
+    const int64_t slots = bm == 256 ? 256 : 512, rest = items % slots;
+    const double tail = rest == 0 ? 0.0
+                        : bm == 256 ? one + (two - one) * (rest / 256.0)
+                                    : rest <= 256 ? one : one + (two - one) * (rest / 256.0 - 1.0);
+    return 4.3 + stages * (static_cast<double>(items / slots) * two + tail);
 }
-// The same of 256 x 256 tiles: one workgroup a CU, 0.85 us a stage with few tiles up to 1.7 with one on every CU (the
-// clock falls), 3 us of epilogue a round.
+// The same of 256 x 256 tiles: one workgroup a CU, 1.0 us a stage with few tiles up to 1.4 with one on every CU, 3.9 us of
+// epilogue a round.
 double tiled_time(int64_t tiles, int64_t stages) {
     const int64_t rest = tiles % 256;
-    const double tail = rest == 0 ? 0.0 : 3.0 + stages * (0.85 + 0.85 * (rest / 256.0));
-    return 4.0 + static_cast<double>(tiles / 256) * (3.0 + 1.7 * stages) + tail;
+    const double tail = rest == 0 ? 0.0 : 3.9 + stages * (1.01 + 0.4 * (rest / 256.0));
+    return 5.9 + static_cast<double>(tiles / 256) * (3.9 + 1.41 * stages) + tail;
 }
 
-// The kernel with the least time by those figures. Against every kernel measured on 63 sizes (T = 512 .. 16384, N = 64 ..
-// 16384, H = 512 .. 7168) the choice was the fastest or within 5 %, but for two SwiGLU sizes with H = 7168 (12 and 29 %).
-// A product by tiles is split over k while that leaves eight stages a piece and at most the 512 workgroups that the GPU
+// The kernel with the least time by those figures, which are fitted to every kernel's times at 87 sizes (T = 128 ..
+// 16384, N = 64 .. 16384, H = 512 .. 7168): the choice was the fastest there or within 6 %, 0.2 % on average.
+// A product by tiles is split over k while that leaves eight stages a piece and at most the workgroups that the GPU
 // holds; the pieces' sums then take another launch.
 // Few rows stream the weights where both operands are read by rows: T = 16, H = 2048, N = 7168 9.1 us (tiles of 32 rows
 // 11.5), T = 64 14.2 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N = 256
@@ -125,19 +129,18 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by
         }
     }
     double least = 1e30;
-    for (const int bm : {32, 64, 128}) {
-        if ((bm == 32) != (m <= 32) && bm != 128) continue;
-        if (bm != 128 && p_by_k) continue;
-        if (bm == 128 && !p_by_k && m <= 64) continue;
+    for (const int bm : {32, 64, 128, 256}) {
+        if (bm == 32 ? m > 32 : bm == 64 ? m <= 32 : bm == 128 ? !p_by_k && m <= 64 : !direct || m <= 128) continue;
+        if (bm < 128 && p_by_k) continue;
         const int64_t tiles = ceil_div(m, bm) * ceil_div(n, swiglu ? 64 : 128);
-        int64_t splits = tiles > 0 ? 512 / tiles : 1;
+        int64_t splits = tiles > 0 ? (bm == 256 ? 256 : 512) / tiles : 1;
         if (splits > stages / 8) splits = stages / 8;
         if (splits < 1) splits = 1;
         const int64_t per = ceil_div(stages, splits);
         splits = ceil_div(stages, per);
         const size_t partial =
             splits > 1 ? static_cast<size_t>(splits) * m * moe::part_ld(static_cast<int>(n), swiglu) * 4 : 0;
-        const double t = mid_time(bm, tiles * splits, per) + (splits > 1 ? 2.5 + 2.0 * partial / 6e6 : 0.0);
+        const double t = mid_time(bm, tiles * splits, per) + (splits > 1 ? 2.3 + 2.0 * partial / 7e6 : 0.0);
         if (t < least) {
             least = t;
             best = ProductPlan{Kernel::kMid, bm, static_cast<int>(splits), per * 64, partial};
@@ -422,7 +425,7 @@ moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void
     if (want_x && grad_weight && direct_product(gx, false, by_k, need_dz) && direct_product(gw, true, true, false)) {
         const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true);
         const ProductPlan pw = plan_product(gw.m, gw.n, gw.k, false, true, true, true);
-        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid) {
+        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid && px.bm <= 128 && pw.bm <= 128) {
             set_split(gx, px, partial);
             set_split(gw, pw, static_cast<char*>(partial) + round_up(static_cast<int64_t>(px.partial_bytes), 256));
             err = moe::launch_gemm_pair(gx, gw, by_k, bf16, px.bm, s);

@@ -13,12 +13,14 @@ namespace {
 
 constexpr int kBN = 128;      // Q rows of a tile (SwiGLU: 64 gate and the matching 64 up rows)
 constexpr int kBK = 64;       // k of a stage
-constexpr int kThreads = 256; // 4 waves
 constexpr int kXcds = 8;
 constexpr uint32_t kPastEnd = 0x80000000u;  // a buffer offset past every buffer: the load returns zeros
 
-// Stages in the LDS ring: two 64 KB workgroups a CU at 128 rows, two of 72 or 80 KB below
-constexpr int ring_stages(int bm) { return bm >= 128 ? 2 : bm == 64 ? 3 : 4; }
+// Waves of a workgroup: each has 64 x 64 of a tile (narrower below 128 rows)
+constexpr int mid_waves(int bm) { return bm == 256 ? 8 : 4; }
+constexpr int mid_threads(int bm) { return mid_waves(bm) * kWave; }
+// Stages in the LDS ring: one 144 KB workgroup a CU at 256 rows, two of 64 KB at 128, two of 72 or 80 KB below
+constexpr int ring_stages(int bm) { return bm == 128 ? 2 : bm == 32 ? 4 : 3; }
 constexpr int mid_lds_bytes(int bm) { return ring_stages(bm) * (bm + kBN) * kBK * 2; }
 
 // Where the 16 bytes that lane `lane` of copy instruction `i` writes to LDS come from. Direct-to-LDS copies write 64
@@ -31,17 +33,16 @@ struct Granule {
     int row;  // by rows: operand row of the tile; by k: k of the stage
     int el;   // by rows: first k of the stage; by k: first operand row of the tile
 };
+// 256 rows by k are two such tiles of 128 one after the other.
 template <bool BY_K, int ROWS>
 __device__ __forceinline__ Granule granule_of(int i, int lane) {
-    static_assert(!BY_K || ROWS == 128, "the swizzle by k permutes 8 pairs of granules");
+    static_assert(!BY_K || ROWS % 128 == 0, "the swizzle by k permutes 8 pairs of granules");
     if (!BY_K) {
         const int r = i * 8 + lane / 8;
         return Granule{r, ((lane % 8) ^ ((r >> 1) & 7)) * 8};
     }
-    constexpr int kPer = ROWS / 8;  // granules per LDS row
-    const int k = i * (64 / kPer) + lane / kPer;
-    const int f = (k & 3) | (((k >> 3) & 1) << 2);
-    return Granule{k, ((lane % kPer) ^ (f << 1)) * 8};
+    const int k = i % 16 * 4 + lane / 16, f = (k & 3) | (((k >> 3) & 1) << 2);
+    return Granule{k, i / 16 * 128 + ((lane % 16) ^ (f << 1)) * 8};
 }
 
 // Fragments of N blocks of 16 operand rows from r0 on, both 32-k steps: lane (row16, kg) gets 8 k of one row.
@@ -50,7 +51,7 @@ __device__ __forceinline__ void read_fragments(const uint16_t* tile, int r0, int
     if constexpr (BY_K) {
         uint32_t addr[N];
 #pragma unroll
-        for (int n = 0; n < N; ++n) addr[n] = transposed_address(tile, r0 + n * 16, lane);
+        for (int n = 0; n < N; ++n) addr[n] = transposed_address(tile + r0 / 128 * 128 * kBK, r0 % 128 + n * 16, lane);
         read_transposed(addr, f);
     } else {
         const int row16 = lane & 15, kg = lane >> 4, sw = (row16 >> 1) & 7;
@@ -76,16 +77,17 @@ __device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, boo
     return v;
 }
 
-// C[m][n] tile of BM x 128 (4 waves), one ring of direct-to-LDS stages, one barrier a stage.
+// C[m][n] tile of BM x 128, one ring of direct-to-LDS stages, one barrier a stage.
 // DIRECT: both operands allow 16-byte copies (bases and row pitches 16-byte aligned, by rows k % 8 == 0). Otherwise the
 // granules come through registers (loads of any alignment) and are written to the same layout.
 // block of grid: this product's share of the launch, grid a multiple of the XCDs.
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
 __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntiles, int block, int grid, uint16_t* lds) {
     constexpr int NS = ring_stages(BM);
-    constexpr int WM = BM >= 128 ? 2 : 1, WN = 4 / WM;  // waves along m and n
+    constexpr int WAVES = mid_waves(BM);
+    constexpr int WM = BM >= 128 ? BM / 64 : 1, WN = WAVES / WM;  // waves along m and n
     constexpr int FM = BM / WM / 16, FN = kBN / WN / 16;  // 16 x 16 blocks of a wave
-    constexpr int PC = BM / 32, QC = kBN / 32;  // copy instructions per wave and stage
+    constexpr int PC = BM / 8 / WAVES, QC = kBN / 8 / WAVES;  // copy instructions per wave and stage
     constexpr int kSlot = (BM + kBN) * kBK;
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -208,6 +210,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
         s16x8 fp[2][FM], fq[2][FN];
         read_fragments<PK, FM>(tp, wm * (BM / WM), lane, fp);
         read_fragments<QK, FN>(tq, wn * (kBN / WN), lane, fq);
+        __builtin_amdgcn_sched_barrier(0);  // all reads are on their way before the first product
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -241,7 +244,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 }
 
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
+__global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
     extern __shared__ __align__(16) uint16_t lds[];
     gemm_mid<T, PK, QK, BM, SWIGLU, DIRECT>(g, mtiles, ntiles, static_cast<int>(blockIdx.x),
                                             static_cast<int>(gridDim.x), lds);
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 // Both gradient products in one launch: neither needs the other, and small ones leave the GPU half empty. The first
 // x_blocks workgroups have grad_x.
 template <typename T, bool QK, int BM>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_pair_kernel(GemmArgs x, GemmArgs w, int x_blocks) {
+__global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_pair_kernel(GemmArgs x, GemmArgs w, int x_blocks) {
     extern __shared__ __align__(16) uint16_t lds[];
     const int block = static_cast<int>(blockIdx.x);
     if (block < x_blocks)
@@ -269,7 +272,7 @@ template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
 hipError_t run_mid(const GemmArgs& g, hipStream_t stream) {
     constexpr int kCols = SWIGLU ? kBN / 2 : kBN;
     TraceScope trace("moe_linear_gemm", stream);
-    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT><<<mid_grid(g, BM, kCols), kThreads, mid_lds_bytes(BM), stream>>>(
+    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT><<<mid_grid(g, BM, kCols), mid_threads(BM), mid_lds_bytes(BM), stream>>>(
         g, (g.m + BM - 1) / BM, (g.n + kCols - 1) / kCols);
     return hipGetLastError();
 }
@@ -279,7 +282,7 @@ hipError_t run_pair(const GemmArgs& x, const GemmArgs& w, hipStream_t stream) {
     constexpr int kLds = mid_lds_bytes(BM) > mid_lds_bytes(128) ? mid_lds_bytes(BM) : mid_lds_bytes(128);
     const int x_blocks = mid_grid(x, BM, kBN);
     TraceScope trace("moe_linear_gemm", stream);
-    gemm_pair_kernel<T, QK, BM><<<x_blocks + mid_grid(w, 128, kBN), kThreads, kLds, stream>>>(x, w, x_blocks);
+    gemm_pair_kernel<T, QK, BM><<<x_blocks + mid_grid(w, 128, kBN), mid_threads(BM), kLds, stream>>>(x, w, x_blocks);
     return hipGetLastError();
 }
 template <typename T>
@@ -297,7 +300,14 @@ hipError_t run_mid_direct(const GemmArgs& g, bool direct, hipStream_t stream) {
 template <typename T>
 hipError_t run_mid_any(const GemmArgs& g, bool p_by_k, bool q_by_k, bool direct, int bm, hipStream_t stream) {
     const bool swiglu = g.act == kActSwiglu;
-    if (p_by_k) return run_mid_direct<T, true, true, 128, false>(g, direct, stream);
+    if (p_by_k) return bm == 256 ? run_mid<T, true, true, 256, false, true>(g, stream)
+                                 : run_mid_direct<T, true, true, 128, false>(g, direct, stream);
+    if (bm == 256) {  // direct operands only
+        if (q_by_k) return swiglu ? run_mid<T, false, true, 256, true, true>(g, stream)
+                                  : run_mid<T, false, true, 256, false, true>(g, stream);
+        return swiglu ? run_mid<T, false, false, 256, true, true>(g, stream)
+                      : run_mid<T, false, false, 256, false, true>(g, stream);
+    }
     if (bm == 128) {
         if (q_by_k) return swiglu ? run_mid_direct<T, false, true, 128, true>(g, direct, stream)
                                   : run_mid_direct<T, false, true, 128, false>(g, direct, stream);
@@ -350,6 +360,19 @@ __global__ __launch_bounds__(kReduceThreads) void grad_tail_kernel(GradTail t) {
     block -= t.x_blocks;
     if (block < t.w_blocks) return gemm_reduce<T, false>(t.w, block);
     column_sums<T>(t.sums, t.bias_grad, t.Z, t.sum_rows, block - t.w_blocks);
+}
+
+template <typename T>
+hipError_t prepare_256() {
+    for (const void* fn : {reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, 256, false, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, 256, true, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, true, 256, false, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, true, 256, true, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, true, true, 256, false, true>)}) {
+        const hipError_t err = ensure_lds_limit(fn, mid_lds_bytes(256));
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 template <typename T, int BM>
@@ -410,7 +433,9 @@ hipError_t launch_grad_tail(GradTail t, bool bf16, hipStream_t stream) {
 }
 
 hipError_t prepare_gemm_mid() {  // 128-row tiles keep within 64 KB
-    hipError_t err = prepare_bm<Half, 32>();
+    hipError_t err = prepare_256<Half>();
+    if (err == hipSuccess) err = prepare_256<Bf16>();
+    if (err == hipSuccess) err = prepare_bm<Half, 32>();
     if (err == hipSuccess) err = prepare_bm<Half, 64>();
     if (err == hipSuccess) err = prepare_bm<Bf16, 32>();
     if (err == hipSuccess) err = prepare_bm<Bf16, 64>();
