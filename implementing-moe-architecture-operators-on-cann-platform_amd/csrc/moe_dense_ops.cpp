@@ -176,7 +176,7 @@ void set_split(moe::GemmArgs& g, const ProductPlan& plan, void* partial) {
 bool direct_product(const moe::GemmArgs& g, bool p_by_k, bool q_by_k, bool p_padded) {
     return direct_operand(g.p, g.ldp) && direct_operand(g.q, g.ldq) &&
            (g.k % 8 == 0 || (q_by_k && (p_by_k || p_padded))) &&
-           !(g.act == moe::kActSwiglu && q_by_k && g.n % 8 != 0);
+           !(g.act == moe::kActSwiglu && q_by_k && g.up % 8 != 0);
 }
 
 hipError_t run_product(moe::GemmArgs g, void* partial, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream,
@@ -190,22 +190,56 @@ hipError_t run_product(moe::GemmArgs g, void* partial, bool p_by_k, bool q_by_k,
     return err == hipSuccess && plan.splits > 1 ? moe::launch_gemm_reduce(g, bf16, stream) : err;
 }
 
-size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
-    return most_partial(T, N, H, act == MOE_ACT_SWIGLU, false);
+// Room for x and the weight with padded rows (moe_linear_repack.hip), where the sizes alone make them necessary: x and a
+// weight [Z, H] where H is no multiple of 8, a transposed weight [H, Z] where Z (a SwiGLU's N) is none.
+struct RepackRoom {
+    size_t x, w;
+};
+RepackRoom repack_room(int64_t T, int64_t N, int64_t H, bool swiglu) {
+    const int64_t h8 = round_up(H, 8), n8 = round_up(N, 8), halves = swiglu ? 2 : 1;
+    RepackRoom r{};
+    if (H % 8 != 0) r.x = round_up(T * h8 * 2, 256);
+    const int64_t rows = H % 8 != 0 ? halves * N * h8 * 2 : 0, cols = N % 8 != 0 ? H * halves * n8 * 2 : 0;
+    r.w = round_up(rows > cols ? rows : cols, 256);
+    return r;
+}
+moe::Repack repack(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t dst_ld) {
+    moe::Repack r{};
+    r.src = static_cast<const uint16_t*>(src);
+    r.dst = static_cast<uint16_t*>(dst);
+    r.src_ld = ld;
+    r.dst_ld = dst_ld;
+    r.rows = rows;
+    r.cols = static_cast<int>(cols);
+    r.dst_cols = static_cast<int>(round_up(cols, 8));
+    return r;
 }
 
-// Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | partial sums of a split product
+size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
+    const bool swiglu = act == MOE_ACT_SWIGLU;
+    const RepackRoom room = repack_room(T, N, H, swiglu);
+    const size_t padded = H % 8 != 0 ? most_partial(T, N, round_up(H, 8), swiglu, false) : 0;
+    const size_t partial = most_partial(T, N, H, swiglu, false);
+    return room.x + room.w + (partial > padded ? partial : padded);
+}
+
+// Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | x and the weight with padded rows,
+// where needed | partial sums of split products
 struct GradWorkspace {
     int64_t Z, ldz;
-    size_t sums_at, partial_at, bytes;
+    size_t sums_at, x_at, w_at, partial_at, bytes;
 };
 GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
     GradWorkspace g{};
     g.Z = act == MOE_ACT_SWIGLU ? 2 * N : N;
     g.ldz = round_up(g.Z, 8);
     g.sums_at = round_up(T * g.ldz * 2, 256);
-    g.partial_at = g.sums_at + round_up(static_cast<int64_t>(moe::act_grad_row_blocks(T, static_cast<int>(g.Z))) * g.Z * 4, 256);
-    const size_t x = most_partial(T, H, g.Z, false, false), w = most_partial(g.Z, H, T, false, true);
+    g.x_at = g.sums_at + round_up(static_cast<int64_t>(moe::act_grad_row_blocks(T, static_cast<int>(g.Z))) * g.Z * 4, 256);
+    const RepackRoom room = repack_room(T, g.Z, H, false);
+    g.w_at = g.x_at + room.x;
+    g.partial_at = g.w_at + room.w;
+    const size_t x0 = most_partial(T, H, g.Z, false, false), x8 = most_partial(T, H, g.ldz, false, false);
+    const size_t x = x0 > x8 ? x0 : x8, w = most_partial(g.Z, H, T, false, true);
     g.bytes = g.partial_at + round_up(static_cast<int64_t>(x), 256) + w;  // both, for products of one launch
     return g;
 }
@@ -349,9 +383,38 @@ moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64
     g.residual = residual;
     g.act = activation;
     g.out_f32 = out_dtype == MOE_DT_FLOAT32;
+    g.up = g.n;
     hipError_t err = moe::prepare_linear();
     if (err != hipSuccess) return hip_fail(err, "MoeLinear kernel attributes");
-    err = run_product(g, workspace, false, weight_transposed != 0, dtype == MOE_DT_BFLOAT16, as_stream(stream));
+    // rows off 16 bytes by their length: padded copies first
+    const bool swiglu = activation == MOE_ACT_SWIGLU, transposed = weight_transposed != 0;
+    const RepackRoom room = repack_room(T, N, H, swiglu);
+    char* base = static_cast<char*>(workspace);
+    moe::RepackArgs pack{};
+    const int64_t h8 = round_up(H, 8), n8 = round_up(N, 8);
+    bool padded = false;
+    if (H % 8 != 0) {
+        pack.m[0] = repack(x, x_stride, T, H, base, h8);
+        g.p = pack.m[0].dst;
+        g.ldp = h8;
+        padded = true;
+    }
+    if (!transposed && H % 8 != 0) {
+        pack.m[1] = repack(weight, weight_stride, Z, H, base + room.x, h8);
+        g.q = pack.m[1].dst;
+        g.ldq = h8;
+        g.k = static_cast<int>(h8);  // zeros in both
+    } else if (transposed && N % 8 != 0) {
+        g.q = reinterpret_cast<uint16_t*>(base + room.x);
+        g.ldq = swiglu ? 2 * n8 : n8;
+        g.up = static_cast<int>(n8);
+        pack.m[1] = repack(weight, weight_stride, H, N, base + room.x, g.ldq);
+        if (swiglu)
+            pack.m[2] = repack(static_cast<const uint16_t*>(weight) + N, weight_stride, H, N, pack.m[1].dst + n8, g.ldq);
+    }
+    err = moe::launch_repack(pack, as_stream(stream));
+    if (err == hipSuccess)
+        err = run_product(g, base + room.x + room.w, false, transposed, dtype == MOE_DT_BFLOAT16, as_stream(stream), padded);
     if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
     return ok();
 }
@@ -421,6 +484,21 @@ moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void
     tail.Z = static_cast<int>(ws.Z);
     tail.sum_rows = moe::act_grad_row_blocks(T, tail.Z);
     const bool want_x = grad_x && T > 0, by_k = weight_transposed == 0;
+    moe::RepackArgs pack{};
+    if (grad_weight && T > 0 && H % 8 != 0 && !direct_operand(x, x_stride)) {
+        pack.m[0] = repack(x, x_stride, T, H, base + ws.x_at, round_up(H, 8));
+        gw.q = pack.m[0].dst;
+        gw.ldq = round_up(H, 8);
+    }
+    if (want_x && (by_k ? H % 8 != 0 && !direct_operand(weight, weight_stride) : ws.Z % 8 != 0)) {
+        const int64_t cols = by_k ? H : ws.Z;
+        pack.m[1] = repack(weight, weight_stride, by_k ? ws.Z : H, cols, base + ws.w_at, round_up(cols, 8));
+        gx.q = pack.m[1].dst;
+        gx.ldq = round_up(cols, 8);
+        if (!by_k && need_dz) gx.k = static_cast<int>(ws.ldz);  // zeros in both
+    }
+    err = moe::launch_repack(pack, s);
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
     void* partial = base + ws.partial_at;
     if (want_x && grad_weight && direct_product(gx, false, by_k, need_dz) && direct_product(gw, true, true, false)) {
         const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true);

@@ -41,6 +41,7 @@ struct GemmArgs {
     const uint16_t* q;
     int64_t ldp, ldq;
     int m, n, k;          // n: output columns; with SwiGLU Q has 2 n rows, the n gate rows first
+    int up;               // Q row of the first up row: n, or past a repacked operand's padding
     void* out;            // [m, n], contiguous
     uint16_t* pre;        // [m, n or 2 n] sums before the activation, rounded to the operands' type; may be null
     const uint16_t* bias; // [n or 2 n] or null
@@ -256,6 +257,30 @@ __device__ __forceinline__ void column_sums(const float* __restrict__ part, uint
     for (int g = 1; g < kGroups; ++g) s += sums[g][i];
     out[c] = T::store(s);
 }
+
+// 8 values of a row from p on, of which `valid` exist (zeros past them); any alignment
+__device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid) {
+    typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+    if (valid >= 8) return *reinterpret_cast<const s16x8_any*>(p);
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < valid) v[e] = static_cast<short>(p[e]);
+    return v;
+}
+
+// Copies of matrices with rows padded with zeros to dst_cols, a multiple of 8 (moe_linear_repack.hip)
+struct Repack {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t src_ld, dst_ld, rows;
+    int cols, dst_cols;
+};
+constexpr int kRepackMost = 3;
+struct RepackArgs {
+    Repack m[kRepackMost];
+};
+hipError_t launch_repack(const RepackArgs& a, hipStream_t stream);
 
 // What follows the gradients' products: the reduction of those that were split (splits > 1), the bias's column sums
 struct GradTail {

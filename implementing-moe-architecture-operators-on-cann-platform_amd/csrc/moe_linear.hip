@@ -65,16 +65,8 @@ __device__ __forceinline__ void read_fragments(const uint16_t* tile, int r0, int
 
 // 8 consecutive elements (of a row's k, or by k of rows) from an operand of any alignment, zeros past its end
 __device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, bool by_k, int row, int k, int rows, int k1) {
-    typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
-    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (row >= rows || k >= k1) return v;
-    const uint16_t* at = p + (by_k ? static_cast<int64_t>(k) * ld + row : static_cast<int64_t>(row) * ld + k);
-    const int valid = by_k ? rows - row : k1 - k;
-    if (valid >= 8) return *reinterpret_cast<const s16x8_any*>(at);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < valid) v[e] = static_cast<short>(at[e]);
-    return v;
+    const int valid = row >= rows || k >= k1 ? 0 : by_k ? rows - row : k1 - k;
+    return load8(p + (by_k ? static_cast<int64_t>(k) * ld + row : static_cast<int64_t>(row) * ld + k), valid);
 }
 
 // C[m][n] tile of BM x 128, one ring of direct-to-LDS stages, one barrier a stage.
@@ -141,7 +133,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 #pragma unroll
         for (int c = 0; c < QC; ++c) {
             const int tr = QK ? qel[c] : qrow[c], col = q_col(tr);
-            const uint32_t off = QK ? qrow[c] * qpitch + (col + (q_up(tr) ? g.n : 0)) * 2u : (col - n0) * qpitch + qel[c] * 2u;
+            const uint32_t off = QK ? qrow[c] * qpitch + (col + (q_up(tr) ? g.up : 0)) * 2u : (col - n0) * qpitch + qel[c] * 2u;
             qoff[c] = col < g.n ? off : kPastEnd;
         }
     }
@@ -163,7 +155,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
             for (int c = 0; c < QC; ++c) {
                 // by rows a copy instruction covers 8 rows, all gate or all up: the base tells them apart, so that the
                 // offsets stay within the tile
-                const int64_t up = !QK && q_up((wave * QC + c) * 8) ? static_cast<int64_t>(g.n) * g.ldq : 0;
+                const int64_t up = !QK && q_up((wave * QC + c) * 8) ? static_cast<int64_t>(g.up) * g.ldq : 0;
                 const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
                     const_cast<uint16_t*>(QK ? qbase + static_cast<int64_t>(kc) * g.ldq : qbase + up), 0, 0x7fffffff,
                     0x00020000);
@@ -180,7 +172,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
             }
 #pragma unroll
             for (int c = 0; c < QC; ++c) {
-                const int tr = QK ? qel[c] : qrow[c], up = q_up(tr) ? g.n : 0;
+                const int tr = QK ? qel[c] : qrow[c], up = q_up(tr) ? g.up : 0;
                 const s16x8 v = load_granule(g.q, g.ldq, QK, q_col(tr) + up, kc + (QK ? qrow[c] : qel[c]), g.n + up, k1);
                 *reinterpret_cast<s16x8*>(slot + BM * kBK + (wave * QC + c) * 512 + lane * 8) = v;
             }

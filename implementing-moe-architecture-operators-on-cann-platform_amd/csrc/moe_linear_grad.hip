@@ -56,17 +56,6 @@ enum Mode {
     kPairs = 2    // aligned 16-byte loads, SwiGLU: y's columns, gate and up together
 };
 
-// 8 values of a row from p on, of which `valid` exist; any alignment
-__device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid) {
-    typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
-    if (valid >= 8) return *reinterpret_cast<const s16x8_any*>(p);
-    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < valid) v[e] = static_cast<short>(p[e]);
-    return v;
-}
-
 template <typename T>
 __device__ __forceinline__ float at(const s16x8& v, int e) {
     return T::load(static_cast<uint16_t>(v[e]));

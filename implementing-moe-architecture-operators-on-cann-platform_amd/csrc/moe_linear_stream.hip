@@ -64,7 +64,7 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
             const int k = k0 + ((gran ^ (4 * i)) * 8);
             const int col = n0 + (SWIGLU ? r8 : 8 * i + r8);
             // SwiGLU: instruction 0 the gate rows, 1 the up rows
-            const int64_t first = n0 + (SWIGLU && i == 1 ? static_cast<int64_t>(g.n) : 0);
+            const int64_t first = n0 + (SWIGLU && i == 1 ? static_cast<int64_t>(g.up) : 0);
             const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<uint16_t*>(live ? g.q + first * g.ldq : g.q), 0, 0x7fffffff, 0x00020000);
             const uint32_t off = static_cast<uint32_t>(col - n0) * qpitch + static_cast<uint32_t>(k) * 2;

@@ -106,14 +106,14 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
                 // SwiGLU: half 0 the gate rows, half 1 the up rows of the same columns. Else wave column wn has columns
                 // wn * 64 + h * 32 + [0, 32) of half h.
                 const int col = SWIGLU ? qr : (qr >> 5) * 64 + h * 32 + (qr & 31);
-                const uint32_t up = SWIGLU && QK && h ? static_cast<uint32_t>(g.n) : 0u;
+                const uint32_t up = SWIGLU && QK && h ? static_cast<uint32_t>(g.up) : 0u;
                 const uint32_t qo = QK ? qk * qp + (t.n0 + col + up) * 2u : col * qp + qk * 2u;
                 c.qo[h][j] = t.n0 + col < g.n ? qo : kPastEnd;
             }
         }
         c.pb = g.p + (PK ? 0 : static_cast<int64_t>(t.m0) * g.ldp);
         c.qb[0] = g.q + (QK ? 0 : static_cast<int64_t>(t.n0) * g.ldq);
-        c.qb[1] = c.qb[0] + (SWIGLU && !QK ? static_cast<int64_t>(g.n) * g.ldq : 0);
+        c.qb[1] = c.qb[0] + (SWIGLU && !QK ? static_cast<int64_t>(g.up) * g.ldq : 0);
     };
     // One half tile of stage kc into ring slot q % 2. By rows the k offset is the instruction's scalar one, by k it moves
     // the base, so an operand may be larger than 4 GiB. Granules from k on read zeros.

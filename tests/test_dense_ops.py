@@ -504,6 +504,21 @@ def test_linear_split_over_k_is_deterministic_and_takes_its_workspace(ops):
     assert e.value.status == 5
 
 
+@gpu
+@pytest.mark.parametrize("T,N,H,act,transposed", [
+    (3, 40, 333, "none", False), (70, 41, 64, "swiglu", True), (70, 41, 65, "swiglu", True), (300, 130, 2049, "silu", False),
+    (300, 130, 2049, "silu", True), (1, 7, 4099, "swiglu", False)])
+def test_odd_sizes_keep_within_their_workspace(ops, T, N, H, act, transposed):
+    need = ops.linear_workspace_bytes(T, N, H, act)
+    ws = torch.full((need + 256,), 0x5a, dtype=torch.uint8, device="cuda")
+    linear_check(ops, T, N, H, F16, act, bias=True, transposed=transposed, workspace=ws[:need])
+    assert (ws[need:] == 0x5a).all()
+    need = ops.linear_grad_workspace_bytes(T, N, H, act)
+    ws = torch.full((need + 256,), 0x5a, dtype=torch.uint8, device="cuda")
+    grad_check(ops, T, N, H, BF16, act, transposed=transposed, workspace=ws[:need])
+    assert (ws[need:] == 0x5a).all()
+
+
 def grad_check(ops, T, N, H, dtype, act, transposed=False, seed=0, dy=None, x=None, w=None, workspace=None):
     Z = 2 * N if act == "swiglu" else N
     dy = normal((T, N), dtype, seed) if dy is None else dy
