@@ -282,13 +282,12 @@ def _here() -> int:
 
 def _first_float(t, name: str, dtypes, dims: int) -> tuple[int, int]:
     """Checks a call's first tensor; returns its moe_dtype and the device that all the others have to be on."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        _need_float(t, name, dtypes, dims, -1)  # raises
-    dev = t.get_device()
-    code = _need_float(t, name, dtypes, dims, dev)
-    if dev != _here():
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == dims:
+        dev = t.get_device()
+        if dev == _here():
+            return _FLOAT_DT[t.dtype], dev
         raise MoeError(4, f"{name} is on cuda:{dev}, the current device is cuda:{_here()}")
-    return code, dev
+    return _need_float(t, name, dtypes, dims, -1), -1  # raises
 
 
 def _need_float(t, name: str, dtypes, dims: int, dev: int) -> int:
@@ -336,6 +335,21 @@ def _act_code(activation: str) -> int:
     return code
 
 
+def _empty(like: torch.Tensor, stream, shape, dtype: torch.dtype) -> torch.Tensor:
+    """A new tensor that belongs to the stream the kernels run on (_on, without a context for the current one)."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _queue(stream, dev: int) -> int:
+    """The raw stream a call on device `dev`, the current one, runs on."""
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(dev)
+    return _stream_ptr(stream)
+
+
 def _scoring_code(scoring: str) -> int:
     code = _SCORING.get(scoring)
     if code is None:
@@ -343,13 +357,13 @@ def _scoring_code(scoring: str) -> int:
     return code
 
 
-def _workspace(workspace, query, args, like, dev):
+def _workspace(workspace, query, args, like, dev, stream):
     """(address, bytes) of the caller's workspace or of a new one (which the caller keeps until the launch)."""
     if workspace is None:
         need = int(query(*args))
         if need == 0:
             return None, None, 0
-        workspace = like.new_empty(need, dtype=torch.uint8)
+        workspace = _empty(like, stream, need, torch.uint8)
         return workspace, workspace.data_ptr(), need
     if not isinstance(workspace, torch.Tensor) or workspace.get_device() != dev or not workspace.is_contiguous():
         raise MoeError(4, f"workspace must be a contiguous tensor on cuda:{dev}")
@@ -360,9 +374,10 @@ def _vector(t, name: str, dtype, n: int, dev: int) -> int | None:
     """The address of an optional contiguous vector."""
     if t is None:
         return None
-    _need_float(t, name, (dtype,), 1, dev)
-    _need_shape(t, name, (n,))
-    if not t.is_contiguous():
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n,) and t.is_contiguous()
+            and t.get_device() == dev):
+        _need_float(t, name, (dtype,), 1, dev)
+        _need_shape(t, name, (n,))
         raise MoeError(4, f"{name} must be contiguous")
     return t.data_ptr()
 
@@ -371,9 +386,10 @@ def _matrix(t, name: str, dtype, shape, dev: int) -> int | None:
     """The address of an optional contiguous matrix."""
     if t is None:
         return None
-    _need_float(t, name, (dtype,), 2, dev)
-    _need_shape(t, name, shape)
-    if not t.is_contiguous():
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+            and t.get_device() == dev):
+        _need_float(t, name, (dtype,), 2, dev)
+        _need_shape(t, name, shape)
         raise MoeError(4, f"{name} must be contiguous (ND format)")
     return t.data_ptr()
 
@@ -397,12 +413,11 @@ def MoeRoutingGroupTopK(logits: torch.Tensor, bias: torch.Tensor | None = None, 
     if type(topK) is not int or topK < 1 or topK > E:
         raise MoeError(4, f"topK={topK} must be in [1, numExperts={E}]")
     like = _like(logits)
-    with _on(stream):
-        ids = like.new_empty((T, topK), dtype=torch.int32)
-        w = like.new_empty((T, topK), dtype=weightsDtype)
+    ids = _empty(like, stream, (T, topK), torch.int32)
+    w = _empty(like, stream, (T, topK), weightsDtype)
     check(_lib.load().moe_routing_group_topk(logits.data_ptr(), ld, lt, bp, ids.data_ptr(), w.data_ptr(),
                                              _FLOAT_DT[weightsDtype], T, E, topK, numGroups, topGroups, groupTop,
-                                             _scoring_code(scoring), int(renormalize), scale, _stream_ptr(stream)))
+                                             _scoring_code(scoring), int(renormalize), scale, _queue(stream, dev)))
     return ids, w
 
 
@@ -424,13 +439,10 @@ def MoeRoutingGroupTopKGrad(grad_weights: torch.Tensor, logits: torch.Tensor, ex
     if not grad_weights.is_contiguous():
         raise MoeError(4, "grad_weights must be contiguous (ND format)")
     ld = _row_stride(logits, "logits")
-    like = _like(logits)
-    with _on(stream):
-        grad = like.new_empty((T, E))
+    grad = _empty(_like(logits), stream, (T, E), logits.dtype)
     check(_lib.load().moe_routing_group_topk_grad(grad_weights.data_ptr(), gt, logits.data_ptr(), ld, lt,
                                                   expert_ids.data_ptr(), grad.data_ptr(), T, E, ks[1],
-                                                  _scoring_code(scoring), int(renormalize), scale,
-                                                  _stream_ptr(stream)))
+                                                  _scoring_code(scoring), int(renormalize), scale, _queue(stream, dev)))
     return grad
 
 
@@ -439,20 +451,20 @@ def MoeCombineGrad(grad_y: torch.Tensor, expert_out: torch.Tensor, weights: torc
     _need(grad_y, "grad_y", torch.float16)
     _need(expert_out, "expert_out", torch.float16)
     _need(weights, "weights", torch.float16)
-    if expert_out.dim() != 3:
-        raise MoeError(2, f"expert_out must have 3 dimensions (got {expert_out.dim()})")
-    T, K, H = expert_out.shape
+    es = expert_out.shape
+    if len(es) != 3:
+        raise MoeError(2, f"expert_out must have 3 dimensions (got {len(es)})")
+    T, K, H = es
     _need_shape(grad_y, "grad_y", (T, H))
     _need_shape(weights, "weights", (T, K))
     dev = _here()
     if expert_out.get_device() != dev or grad_y.get_device() != dev or weights.get_device() != dev:
         raise MoeError(4, f"grad_y, expert_out and weights must be on the current device cuda:{dev}")
     like = _like(expert_out)
-    with _on(stream):
-        geo = like.new_empty((T, K, H))
-        gw = like.new_empty((T, K))
+    geo = _empty(like, stream, (T, K, H), torch.float16)
+    gw = _empty(like, stream, (T, K), torch.float16)
     check(_lib.load().moe_combine_grad(grad_y.data_ptr(), expert_out.data_ptr(), weights.data_ptr(), geo.data_ptr(),
-                                       gw.data_ptr(), T, H, K, _stream_ptr(stream)))
+                                       gw.data_ptr(), T, H, K, _queue(stream, dev)))
     return geo, gw
 
 
@@ -497,12 +509,11 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     rp = _matrix(residual, "residual", out, (T, N), dev)
     lib = _lib.load()
     like = _like(x)
-    with _on(stream):
-        workspace, wp, wb = _workspace(workspace, lib.moe_linear_workspace_bytes, (T, N, H, act), like, dev)
-        y = like.new_empty((T, N), dtype=out)
-        pre = like.new_empty((T, Z)) if returnPre else None
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_workspace_bytes, (T, N, H, act), like, dev, stream)
+    y = _empty(like, stream, (T, N), out)
+    pre = _empty(like, stream, (T, Z), dtype) if returnPre else None
     check(lib.moe_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre), wp, wb, T,
-                         N, H, act, dt, _FLOAT_DT[out], _stream_ptr(stream)))
+                         N, H, act, dt, _FLOAT_DT[out], _queue(stream, dev)))
     return (y, pre) if returnPre else y
 
 
@@ -526,13 +537,12 @@ def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, p
     pp = _matrix(pre, "pre", dtype, (T, Z), dev) if act else None
     lib = _lib.load()
     like = _like(x)
-    with _on(stream):
-        workspace, wp, wb = _workspace(workspace, lib.moe_linear_grad_workspace_bytes, (T, N, H, act), like, dev)
-        gx = like.new_empty((T, H)) if gradX else None
-        gw = like.new_empty((Z, H)) if gradWeight else None
-        gb = like.new_empty((Z,)) if gradBias else None
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_grad_workspace_bytes, (T, N, H, act), like, dev, stream)
+    gx = _empty(like, stream, (T, H), dtype) if gradX else None
+    gw = _empty(like, stream, (Z, H), dtype) if gradWeight else None
+    gb = _empty(like, stream, (Z,), dtype) if gradBias else None
     check(lib.moe_linear_grad(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, pp,
-                              _ptr(gx), _ptr(gw), _ptr(gb), wp, wb, T, N, H, act, dt, _stream_ptr(stream)))
+                              _ptr(gx), _ptr(gw), _ptr(gb), wp, wb, T, N, H, act, dt, _queue(stream, dev)))
     return gx, gw, gb
 
 
