@@ -10,13 +10,16 @@
 // exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where the last group that stays and the
 // first that does not are nearer than that, the row's groups are scored again in float64; where two neighbours among
 // its picks are, the picks go on past the K-th until a clear gap and are put in order by their float64 values. That is
-// some rows in a thousand, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
+// some rows in a hundred, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
 // never in the instruction cache when it is needed, cost 9 us.
 //
 // A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers. A
-// pick is the maximum over the lane (max3), over the row (4 DPP steps), the lowest index that has it (4 more) and its
-// removal: ~80 instructions for 4 tokens, which bounds the kernel, not the logits' bytes. Group scores go through LDS,
-// one lane per (token, group).
+// pick is the maximum over the lane (max3) and over the row (4 DPP steps), and its removal: 16 compares and 16 selects.
+// Where the key's low 8 bits can hold the expert, the maximum names the pick: ~50 instructions for 4 tokens. fp32 logits
+// without a bias need all of their bits: the lowest index that has the maximum is searched, ~95 instructions. Group scores
+// go through LDS, one lane per (token, group). Vector instructions bound the kernel (T = 16384, E = 256, K = 8, fp32
+// logits: 10.3 us without bias and groups, 17 us with a bias and 4 of 8 groups by their two best, of which a copy of the
+// logits is 4 us; the search in place of the key's bits 21 us), at T = 1 the call on the host (8.4 us).
 #include "moe_device.h"
 #include "moe_launch.h"
 #include "moe_ops.h"
@@ -355,48 +358,90 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
                 __syncthreads();
             }
         }
+        const int* mine = kept + tok * G;
+        if (C >= 4 && size % 4 == 0) {  // a piece's experts are of one group
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            const int e = expert_of<C>(l, j);
-            if (e < E && !kept[tok * G + ((e * r.size_inverse) >> 16)]) key[j] = kGone;
+            for (int j = 0; j < C; j += 4) {
+                const int e = expert_of<C>(l, j);
+                if (e >= E || mine[(e * r.size_inverse) >> 16]) continue;
+#pragma unroll
+                for (int i = j; i < min(j + 4, C); ++i) key[i] = kGone;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const int e = expert_of<C>(l, j);
+                if (e < E && !mine[(e * r.size_inverse) >> 16]) key[j] = kGone;
+            }
         }
     }
-    constexpr int kStep = C < 4 ? C : 4;
-    int last = kGone, picks = K;  // picks of this row: K, and those that fp32 does not tell from the K-th
-    bool reorder = false;         // two of them are nearer than fp32 tells apart
+    int picks = K;         // of this row: K, and those that are not told from the K-th
+    bool reorder = false;  // two of them are nearer than their keys tell apart
+    if (r.bias || !std::is_same_v<L, F32>) {
+        // Keys with 255 - e in their low 8 bits: the maximum is the pick, and the lowest index wins. Half logits leave
+        // those bits free; c loses them, up to 2^-15 of it, which counts as an error like fp32's own.
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            key[j] = key[j] == kGone ? kGone : (key[j] & ~(kMaxE - 1)) | (kMaxE - 1 - expert_of<C>(l, j));
+        int last = kGone;
 #pragma unroll 1
-    for (int k = 0;; ++k) {
-        int m = key[0];
+        for (int k = 0;; ++k) {
+            int m = key[0];
 #pragma unroll
-        for (int j = 1; j < C; ++j) m = max(m, key[j]);
-        m = row_max_i(m);
-        if (r.bias) {
-            const float x = key_value(last), y = key_value(m);
-            const bool close = last != kGone && m != kGone && !(x - y > gap_limit(r.sigmoid, s_max, x));
-            if (close && k <= picks) {
-                reorder = true;
-                picks = max(picks, k + 1);
+            for (int j = 1; j < C; ++j) m = max(m, key[j]);
+            m = row_max_i(m);
+            if (r.bias) {
+                const float x = key_value(last & ~(kMaxE - 1)), y = key_value(m & ~(kMaxE - 1));
+                const bool clear = x - y > gap_limit(r.sigmoid, s_max, x) + fabsf(y) * 0x1p-15f;
+                if (!clear && last != kGone && m != kGone && k <= picks) {
+                    reorder = true;
+                    picks = max(picks, k + 1);
+                }
+                last = m;
             }
-            last = m;
+            if (k >= K && !__any(k < picks)) break;
+            if (l == 0 && k < picks)
+                pick[tok * E + k] = static_cast<uint16_t>(m == kGone ? kNoPick : kMaxE - 1 - (m & (kMaxE - 1)));
+#pragma unroll
+            for (int j = 0; j < C; ++j) key[j] = key[j] == m ? kGone : key[j];
         }
-        if (k >= K && !__any(k < picks)) break;
-        int jw = -1;
+    } else {
+        constexpr int kStep = C < 4 ? C : 4;
+#pragma unroll 1
+        for (int k = 0; k < K; ++k) {
+            int m = key[0];
 #pragma unroll
-        for (int j = C - 1; j >= 0; --j) jw = key[j] == m ? j : jw;
-        const int e = row_min_i(jw < 0 ? kMaxE : expert_of<C>(l, jw));
-        if (l == 0 && k < picks) pick[tok * E + k] = static_cast<uint16_t>(m == kGone ? kNoPick : e);
-        const int mine = e / kStep % kLanes == l ? e / (kLanes * kStep) * kStep + e % kStep : -1;  // its register
+            for (int j = 1; j < C; ++j) m = max(m, key[j]);
+            m = row_max_i(m);
+            int jw = -1;
 #pragma unroll
-        for (int j = 0; j < C; ++j) key[j] = mine == j ? kGone : key[j];
+            for (int j = C - 1; j >= 0; --j) jw = key[j] == m ? j : jw;
+            const int e = row_min_i(jw < 0 ? kMaxE : expert_of<C>(l, jw));
+            if (l == 0) pick[tok * E + k] = static_cast<uint16_t>(m == kGone ? kNoPick : e);
+            const int mine = e / kStep % kLanes == l ? e / (kLanes * kStep) * kStep + e % kStep : -1;  // its register
+#pragma unroll
+            for (int j = 0; j < C; ++j) key[j] = mine == j ? kGone : key[j];
+        }
     }
     __syncthreads();
     uint64_t redo = __ballot(reorder && valid);
 #pragma unroll 1
     for (int q = 0; redo && q < kWaveTokens; ++q) {
         if (!((redo >> (q * kLanes)) & 1)) continue;
-        exact_scores<L>(r, static_cast<int64_t>(blockIdx.x) * kWaveTokens + q, cs);
+        const int64_t tq = static_cast<int64_t>(blockIdx.x) * kWaveTokens + q;
         const int n = __shfl(picks, q * kLanes, kWave);
         uint16_t* of = pick + q * E;
+        if (r.sigmoid) {  // the picks' alone
+            for (int k = lane; k < n; k += kWave) {
+                const int e = of[k];
+                if (e == kNoPick) continue;
+                const double x = static_cast<double>(logit<L>(r.logits, tq * r.ld + e));
+                cs[e] = 1.0 / (1.0 + exp(-x)) + static_cast<double>(r.bias[e]);
+            }
+            __syncthreads();
+        } else {
+            exact_scores<L>(r, tq, cs);
+        }
 #pragma unroll 1
         for (int k = lane; k < n; k += kWave) {
             const int e = of[k];
@@ -417,10 +462,12 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     const uint16_t* my = pick + tok * E;
     double* part = parts + tok * K;
     int ref_key = kGone;
+    const float first = l < K && my[l] != kNoPick ? logit<L>(r.logits, t * r.ld + my[l]) : 0.0f;
+    auto chosen = [&](int k) { return k < kLanes ? first : logit<L>(r.logits, t * r.ld + my[k]); };
     if (r.renormalize) {
         for (int k = l; k < K; k += kLanes) {
             if (my[k] == kNoPick) continue;
-            const float x = logit<L>(r.logits, t * r.ld + my[k]);
+            const float x = chosen(k);
             ref_key = max(ref_key, key_of(r.sigmoid ? fminf(x, 0.0f) : x));
         }
         ref_key = row_max_i(ref_key);
@@ -430,7 +477,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     for (int k = l; k < K; k += kLanes) {
         double p = 0.0;
         if (my[k] != kNoPick) {
-            const double x = static_cast<double>(logit<L>(r.logits, t * r.ld + my[k]));
+            const double x = static_cast<double>(chosen(k));
             if (r.sigmoid) p = exp(fmin(x, 0.0) - ref) / (1.0 + exp(-fabs(x)));
             else p = x == ref ? 1.0 : exp(x - ref);
         }
