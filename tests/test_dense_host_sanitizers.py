@@ -7,12 +7,20 @@ from __future__ import annotations
 import concurrent.futures
 import os
 import pathlib
+import shutil
 import subprocess
 
 import pytest
 
 from conftest import ROOT
-from test_host_sanitizers import PKG, SAN, _hipcc
+
+PKG = ROOT / "implementing-moe-architecture-operators-on-cann-platform_amd"
+SAN = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined", "-Xarch_host",
+       "-fno-omit-frame-pointer"]
+
+
+def _hipcc() -> str | None:
+    return shutil.which("hipcc") or ("/opt/rocm/bin/hipcc" if os.path.exists("/opt/rocm/bin/hipcc") else None)
 
 
 @pytest.mark.skipif(_hipcc() is None, reason="hipcc is not installed")
