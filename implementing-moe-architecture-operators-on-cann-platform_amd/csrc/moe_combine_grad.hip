@@ -7,6 +7,7 @@
 // Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 8 experts at
 // a time, loads their rows, adds to their dot products and writes their gradient rows. A wave has a token to itself, or
 // four waves share it; the dot products are added over the lanes and then over the waves in a fixed order.
+// T = 16384, H = 2048, K = 6: 872 MB in 144 us, 6.07 TB/s (a copy of 1 GB: 5.0). T = 128, K = 2: 8 us, the call itself.
 #include "moe_device.h"
 #include "moe_launch.h"
 
@@ -16,7 +17,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 8;  // experts in flight per thread
-// expert_out and its gradient beyond the 256 MB Infinity Cache go past it (non-temporal)
+// expert_out and its gradient together beyond the 256 MB Infinity Cache go past it (non-temporal): T = 16384, K = 6 144 us,
+// through the cache 171 us
 constexpr int64_t kStreamBytes = int64_t(128) << 20;
 
 template <int WAVES, bool NT>  // waves of one token: 1 or 4

@@ -115,9 +115,9 @@ double tiled_time(int64_t tiles, int64_t stages) {
 // 16384, N = 64 .. 16384, H = 512 .. 7168): the choice was the fastest there or within 6 %, 0.2 % on average.
 // A product by tiles is split over k while that leaves eight stages a piece and at most the workgroups that the GPU
 // holds; the pieces' sums then take another launch.
-// Few rows stream the weights where both operands are read by rows: T = 16, H = 2048, N = 7168 9.1 us (tiles of 32 rows
-// 11.5), T = 64 14.2 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N = 256
-// 12.7 us (9.1 split over k), T = 64, H = 4096, N = 16384 45 us (34).
+// Few rows stream the weights where both operands are read by rows: T = 16, H = 2048, N = 7168 8.2 us (tiles of 32 rows
+// 11.5), T = 64 11.6 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N = 256
+// 12.4 us (8.3 split over k), T = 64, H = 4096, N = 16384 35 us (33).
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct) {
     ProductPlan best{Kernel::kMid, 128, 1, ceil_div(k > 0 ? k : 1, 64) * 64, 0};
     const int64_t stages = ceil_div(k > 0 ? k : 1, 64);

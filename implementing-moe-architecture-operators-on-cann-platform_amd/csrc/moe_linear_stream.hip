@@ -1,10 +1,12 @@
 // moe_linear_stream.hip -- the dense product of few rows (serving's single tokens and small batches): weight streaming.
 //
-// C[m][n] = sum_k P[m][k] Q[n][k], both operands by rows, m <= 32. The weights are read once and bound it: at T = 1 the
-// gate and up rows of a dense expert are 59 MB for 59 MFLOP.
-//   work      a tile is 16 weight rows (SwiGLU: 8 gate and the matching 8 up rows) over the whole k, and its workgroup's
-//             waves share k: wave w takes the 64-k pieces w, w + W, ... Their sums meet in LDS, added in wave order, and
-//             go through the epilogue: one launch, no partial sums in memory.
+// C[m][n] = sum_k P[m][k] Q[n][k], both operands by rows, m <= 64. The weights are read once and bound it: at T = 1 the
+// gate and up rows of a dense expert (H = 7168, N = 2048) are 59 MB for 59 MFLOP, 10.7 us (5.5 TB/s). From 16 rows on x,
+// which every tile reads again from L2, costs as much as the weights: T = 64, H = 2048, N = 7168 11.6 us, 29 MB of weights
+// and 58 MB of x through the CUs' copy paths.
+//   work      a tile is 16 or 32 weight rows (SwiGLU: half gate, half the matching up rows) over the whole k, and its
+//             workgroup's waves share k: wave w takes the 64-k pieces w, w + W, ... Their sums meet in LDS, added in wave
+//             order, and go through the epilogue: one launch, no partial sums in memory.
 //   copies    each wave has its own LDS ring and fills it straight from global memory, 8 rows x 128 bytes an instruction;
 //             nobody else reads it, so the main loop has no barrier. Loaded into registers in fragment order (16 rows x
 //             64 bytes an instruction) the same work ran at 4.2 TB/s.
@@ -24,21 +26,22 @@ constexpr int kBlock = 16 * kBK;            // halfs of 16 rows of a piece
 constexpr uint32_t kPastEnd = 0x80000000u;  // a buffer offset past every buffer: the load returns zeros
 constexpr int kNonTemporal = 2;             // cache policy of the weights: read once
 
-// MB: blocks of 16 rows of P; DEPTH: pieces of a wave's ring
-template <int MB, int WAVES, int DEPTH>
+// QB, MB: blocks of 16 rows of Q and P; DEPTH: pieces of a wave's ring
+template <int QB, int MB, int WAVES, int DEPTH>
 struct StreamLds {
-    static constexpr int kPieceHalfs = (1 + MB) * kBlock;
+    static constexpr int kPieceHalfs = (QB + MB) * kBlock;
     static constexpr int kRings = WAVES * DEPTH * kPieceHalfs * 2;
-    static constexpr int kSums = WAVES * MB * 16 * 17 * 4;
+    static constexpr int kPassBlocks = MB < 2 ? MB : 2;  // blocks of P rows whose sums meet at a time
+    static constexpr int kSums = WAVES * kPassBlocks * 16 * QB * 16 * 4;
     static constexpr int kBytes = kRings + kSums;
 };
 
-template <typename T, int MB, int WAVES, int DEPTH, bool SWIGLU>
+template <typename T, int QB, int MB, int WAVES, int DEPTH, bool SWIGLU>
 __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, int tiles) {
-    using Lds = StreamLds<MB, WAVES, DEPTH>;
-    constexpr int kCopies = 2 * (1 + MB);
+    using Lds = StreamLds<QB, MB, WAVES, DEPTH>;
+    constexpr int kCopies = 2 * (QB + MB), kCols = QB * (SWIGLU ? 8 : 16);
     extern __shared__ __align__(16) uint16_t lds[];
-    float(*sums)[MB * 16][17] = reinterpret_cast<float(*)[MB * 16][17]>(lds + Lds::kRings / 2);  // [wave][P row][Q row]
+    float* sums = reinterpret_cast<float*>(lds + Lds::kRings / 2);  // [wave][P row of the pass][Q row]
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int row16 = lane & 15, kg = lane >> 4;
@@ -58,26 +61,26 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
         uint16_t* slot = ring + cslot * Lds::kPieceHalfs;
         const int k0 = (wave + cpiece * WAVES) * kBK;
         const bool live = ctile < tiles && mine > 0;
-        const int n0 = ctile * (SWIGLU ? 8 : 16);
+        const int n0 = ctile * kCols;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int k = k0 + ((gran ^ (4 * i)) * 8);
-            const int col = n0 + (SWIGLU ? r8 : 8 * i + r8);
-            // SwiGLU: instruction 0 the gate rows, 1 the up rows
-            const int64_t first = n0 + (SWIGLU && i == 1 ? static_cast<int64_t>(g.up) : 0);
+        for (int i = 0; i < 2 * QB; ++i) {
+            const int k = k0 + ((gran ^ (4 * (i & 1))) * 8);
+            const int row = 8 * (SWIGLU ? i % QB : i) + r8;
+            // SwiGLU: the first QB instructions the gate rows, the others the up rows
+            const int64_t first = n0 + (SWIGLU && i >= QB ? static_cast<int64_t>(g.up) : 0);
             const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<uint16_t*>(live ? g.q + first * g.ldq : g.q), 0, 0x7fffffff, 0x00020000);
-            const uint32_t off = static_cast<uint32_t>(col - n0) * qpitch + static_cast<uint32_t>(k) * 2;
+            const uint32_t off = static_cast<uint32_t>(row) * qpitch + static_cast<uint32_t>(k) * 2;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 qr, (__attribute__((address_space(3))) void*)(slot + i * 512), 16,
-                static_cast<int>(live && col < g.n && k < g.k ? off : kPastEnd), 0, 0, kNonTemporal);
+                static_cast<int>(live && n0 + row < g.n && k < g.k ? off : kPastEnd), 0, 0, kNonTemporal);
         }
 #pragma unroll
         for (int i = 0; i < 2 * MB; ++i) {
             const int row = 8 * i + r8, k = k0 + ((gran ^ (4 * (i & 1))) * 8);
             const uint32_t off = static_cast<uint32_t>(row) * ppitch + static_cast<uint32_t>(k) * 2;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                pr, (__attribute__((address_space(3))) void*)(slot + kBlock + i * 512), 16,
+                pr, (__attribute__((address_space(3))) void*)(slot + QB * kBlock + i * 512), 16,
                 static_cast<int>(live && row < g.m && k < g.k ? off : kPastEnd), 0, 0, 0);
         }
         cslot = cslot + 1 == DEPTH ? 0 : cslot + 1;
@@ -93,9 +96,11 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
     const int sw = (row16 >> 1) & 7;
     int slot = 0;
     for (int tile = static_cast<int>(blockIdx.x); tile < tiles; tile += static_cast<int>(gridDim.x)) {
-        f32x4 acc[MB];
+        f32x4 acc[QB][MB];
 #pragma unroll
-        for (int b = 0; b < MB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int i = 0; i < mine; ++i) {
             // the piece has landed and the slot of the one before it, whose reads are in registers, may be filled again
             __builtin_amdgcn_sched_barrier(0);
@@ -106,97 +111,128 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const int at = row16 * kBK + (((kk * 4 + kg) ^ sw) * 8);
-                const s16x8 a = *reinterpret_cast<const s16x8*>(s + at);
+                s16x8 a[QB];
 #pragma unroll
-                for (int b = 0; b < MB; ++b)
-                    acc[b] = T::mfma(a, *reinterpret_cast<const s16x8*>(s + (1 + b) * kBlock + at), acc[b]);
+                for (int q = 0; q < QB; ++q) a[q] = *reinterpret_cast<const s16x8*>(s + q * kBlock + at);
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    const s16x8 x = *reinterpret_cast<const s16x8*>(s + (QB + b) * kBlock + at);
+#pragma unroll
+                    for (int q = 0; q < QB; ++q) acc[q][b] = T::mfma(a[q], x, acc[q][b]);
+                }
             }
             slot = slot + 1 == DEPTH ? 0 : slot + 1;
         }
-        // acc[b]: D[Q row 4 kg + r][P row row16 of block b]
+        // acc[q][b]: D[Q row 4 kg + r of block q][P row row16 of block b]. Granule G (4 Q rows) of P row r stands at G ^ r.
+        constexpr int kGranules = 4 * QB, kRows = 16 * Lds::kPassBlocks;
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
+        for (int b0 = 0; b0 < MB; b0 += Lds::kPassBlocks) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sums[wave][b * 16 + row16][kg * 4 + r] = acc[b][r];
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0); the copies in flight go on
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-        // a thread has 4 columns of one row
-        constexpr int kQuads = SWIGLU ? 2 : 4;
-        for (int i = tid; i < MB * 16 * kQuads; i += WAVES * kWave) {
-            const int row = i / kQuads, c = i % kQuads * 4;
-            if (row >= g.m) continue;
-            f32x4 z = {0.f, 0.f, 0.f, 0.f}, u = z;
+            for (int b = 0; b < Lds::kPassBlocks; ++b)
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w)
+                for (int q = 0; q < QB; ++q)
+                    *reinterpret_cast<f32x4*>(sums + ((wave * kRows + b * 16 + row16) * kGranules +
+                                                      ((q * 4 + kg) ^ (row16 % kGranules))) * 4) = acc[q][b0 + b];
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0); the copies in flight go on
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            // a thread has 4 columns of one row
+            constexpr int kQuads = kCols / 4;
+            for (int i = tid; i < kRows * kQuads; i += WAVES * kWave) {
+                const int r = i / kQuads, c = i % kQuads, row = b0 * 16 + r;
+                if (row >= g.m) continue;
+                f32x4 z = {0.f, 0.f, 0.f, 0.f}, u = z;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    z[r] += sums[w][row][c + r];
-                    if (SWIGLU) u[r] += sums[w][row][8 + c + r];
+                for (int w = 0; w < WAVES; ++w) {
+                    const float* at = sums + (w * kRows + r) * kGranules * 4;
+                    z += *reinterpret_cast<const f32x4*>(at + (c ^ (r % kGranules)) * 4);
+                    if (SWIGLU) u += *reinterpret_cast<const f32x4*>(at + ((kQuads + c) ^ (r % kGranules)) * 4);
                 }
-            store4<T, SWIGLU>(g, row, tile * (SWIGLU ? 8 : 16) + c, z, u, vec);
+                store4<T, SWIGLU>(g, row, tile * kCols + c * 4, z, u, vec);
+            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            __builtin_amdgcn_s_barrier();  // read before the next sums are written
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
         }
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-        __builtin_amdgcn_s_barrier();  // read before the next tile's sums are written
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the surplus copies have landed before the workgroup ends
 }
 
-template <typename T, int MB, int WAVES, int DEPTH, bool SWIGLU>
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// Rows of P up to 16, 32 and 64: waves and depths whose rings fill a CU's LDS
+template <typename F>
+hipError_t by_rows(int m, int qb, F&& f) {
+    if (qb == 2) {
+        if (m <= 16) return f(Int<2>(), Int<1>(), Int<6>(), Int<3>());
+        return m <= 32 ? f(Int<2>(), Int<2>(), Int<4>(), Int<4>()) : f(Int<2>(), Int<4>(), Int<4>(), Int<3>());
+    }
+    if (m <= 16) return f(Int<1>(), Int<1>(), Int<8>(), Int<3>());
+    return m <= 32 ? f(Int<1>(), Int<2>(), Int<4>(), Int<4>()) : f(Int<1>(), Int<4>(), Int<4>(), Int<3>());
+}
+
+// Blocks of 16 weight rows in a tile. Two halve what a tile reads of x, for 1.45 times the time of a tile of one, so they
+// pay where they save rounds of the GPU: T = 64, H = 2048, N = 7168 (2 rounds -> 1) 14.5 -> 11.6 us, H = 18432 100 -> 71.5;
+// H = 4096, N = 4096 (1 round either way) 13.7 -> 16.6. Up to 16 rows x costs little, and tiles of one keep more
+// copies in flight over several rounds: T = 1, N = 16384, H = 4096 (4 rounds -> 2) 23.3 -> 26.5 us; into a single round
+// two are as fast or faster there too (T = 16, N = 7168 9.1 -> 8.2 us).
+int tile_blocks(int m, int64_t rows) {
+    constexpr int64_t kCus = 256;
+    const int64_t one = ((rows + 15) / 16 + kCus - 1) / kCus, two = ((rows + 31) / 32 + kCus - 1) / kCus;
+    if (m <= 16) return one == 2 && two == 1 ? 2 : 1;
+    return 3 * two < 2 * one ? 2 : 1;
+}
+
+template <typename T, int QB, int MB, int WAVES, int DEPTH, bool SWIGLU>
 hipError_t run_stream(const GemmArgs& g, hipStream_t stream) {
-    auto fn = &gemm_stream_kernel<T, MB, WAVES, DEPTH, SWIGLU>;
+    auto fn = &gemm_stream_kernel<T, QB, MB, WAVES, DEPTH, SWIGLU>;
     const void* p = reinterpret_cast<const void*>(fn);
-    constexpr int kLds = StreamLds<MB, WAVES, DEPTH>::kBytes;
-    const int tiles = (g.n + (SWIGLU ? 7 : 15)) / (SWIGLU ? 8 : 16);
+    constexpr int kLds = StreamLds<QB, MB, WAVES, DEPTH>::kBytes, kCols = QB * (SWIGLU ? 8 : 16);
+    static_assert(kLds <= 160 * 1024);
+    const int tiles = (g.n + kCols - 1) / kCols;
     const int resident = resident_workgroups(p, WAVES * kWave, kLds);
     TraceScope trace("moe_linear_stream", stream);
     fn<<<resident > 0 && resident < tiles ? resident : tiles, WAVES * kWave, kLds, stream>>>(g, tiles);
     return hipGetLastError();
 }
 
-template <typename T, int MB, int WAVES, int DEPTH>
-hipError_t run_stream_act(const GemmArgs& g, hipStream_t stream) {
-    return g.act == kActSwiglu ? run_stream<T, MB, WAVES, DEPTH, true>(g, stream)
-                               : run_stream<T, MB, WAVES, DEPTH, false>(g, stream);
-}
-
-// rows of P up to 16, 32 and 64
-template <typename F>
-hipError_t by_rows(int m, F&& f) {
-    if (m <= 16) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>(), std::integral_constant<int, 3>());
-    if (m <= 32) return f(std::integral_constant<int, 2>(), std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
-    return f(std::integral_constant<int, 4>(), std::integral_constant<int, 4>(), std::integral_constant<int, 3>());
-}
-
 template <typename T>
-hipError_t prepare(int m) {
-    return by_rows(m, [](auto mb, auto waves, auto depth) {
-        constexpr int M = decltype(mb)::value, W = decltype(waves)::value, D = decltype(depth)::value;
-        hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, M, W, D, true>),
-                                          StreamLds<M, W, D>::kBytes);
+hipError_t prepare(int m, int qb) {
+    return by_rows(m, qb, [](auto q, auto mb, auto waves, auto depth) {
+        constexpr int Q = decltype(q)::value, M = decltype(mb)::value, W = decltype(waves)::value,
+                      D = decltype(depth)::value;
+        hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, true>),
+                                          StreamLds<Q, M, W, D>::kBytes);
         if (err == hipSuccess)
-            err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, M, W, D, false>),
-                                   StreamLds<M, W, D>::kBytes);
+            err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, false>),
+                                   StreamLds<Q, M, W, D>::kBytes);
         return err;
     });
 }
 
 template <typename T>
 hipError_t run_stream_any(const GemmArgs& g, hipStream_t stream) {
-    return by_rows(g.m, [&](auto mb, auto waves, auto depth) {
-        return run_stream_act<T, decltype(mb)::value, decltype(waves)::value, decltype(depth)::value>(g, stream);
+    const int64_t rows = g.act == kActSwiglu ? 2 * static_cast<int64_t>(g.n) : g.n;
+    return by_rows(g.m, tile_blocks(g.m, rows), [&](auto q, auto mb, auto waves, auto depth) {
+        constexpr int Q = decltype(q)::value, M = decltype(mb)::value, W = decltype(waves)::value,
+                      D = decltype(depth)::value;
+        return g.act == kActSwiglu ? run_stream<T, Q, M, W, D, true>(g, stream)
+                                   : run_stream<T, Q, M, W, D, false>(g, stream);
     });
 }
 
 }  // namespace
 
 hipError_t prepare_gemm_stream() {
-    for (const int m : {16, 32, 64}) {
-        hipError_t err = prepare<Half>(m);
-        if (err == hipSuccess) err = prepare<Bf16>(m);
-        if (err != hipSuccess) return err;
-    }
+    for (const int m : {16, 32, 64})
+        for (const int qb : {1, 2}) {
+            hipError_t err = prepare<Half>(m, qb);
+            if (err == hipSuccess) err = prepare<Bf16>(m, qb);
+            if (err != hipSuccess) return err;
+        }
     return hipSuccess;
 }
 

@@ -267,7 +267,7 @@ typedef enum moe_activation {
  *   scores: the lower group). expert_ids are the K best c of the experts that stay, in descending order (equal
  *   c: the lower index). weights = scale * s, divided by the sum of the K chosen s where renormalize is set
  *   (the ratios hold where the scores themselves would underflow). bias only steers the choice.
- *   c is compared in float64. An expert whose logit or c is NaN or -infinity is not available; where a row has fewer
+ *   c is compared beyond fp32: without a bias by the logits, which order the scores, with one in float64. An expert whose logit or c is NaN or -infinity is not available; where a row has fewer
  *   than K available ones the picks left are id -1 and weight 0, which moe_expert_ffn computes as zero rows.
  *   1 <= K <= top_groups * E / groups, E <= 256.
  * ---------------------------------------------------------------------------------------------------- */
@@ -299,10 +299,12 @@ moe_status moe_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, 
  *   MoeRoutingTopK's w_gate. bias[N] (SwiGLU: [2N]) of dtype, or NULL; residual[T, N] of out_dtype, or NULL; out_dtype
  *   is dtype or float32. pre, if not NULL, receives the sums before the activation, [T, N] (SwiGLU: [T, 2N]) of dtype,
  *   which moe_linear_grad takes. Any sizes from 1; N, H <= 2^20.
- *   Operands that 16-byte copies can read (16-byte aligned, strides multiples of 8, H a multiple of 8; SwiGLU with a
- *   transposed weight: N too) run at full speed, others are loaded element by element.
- *   The workspace (moe_linear_workspace_bytes, may be 0) holds fp32 partial sums of a product split over H; calls in
- *   flight at the same time need one each. Deterministic; nothing depends on timing.
+ *   Any strides and alignment. 16-byte aligned operands whose strides are multiples of 8 run at full speed. Where H (of a
+ *   transposed weight N) is no multiple of 8, x and the weight are first copied with padded rows; other operands that
+ *   16-byte copies cannot read go through registers, at a fraction of the speed. residual may be y itself.
+ *   The workspace (moe_linear_workspace_bytes, 0 where none is needed; 16-byte aligned) holds fp32 partial sums of a product
+ *   split over H and those copies; calls in flight at the same time, captured graphs among them, need one each.
+ *   Deterministic: the order of every sum depends on the sizes, strides and alignment alone.
  * ---------------------------------------------------------------------------------------------------- */
 size_t moe_linear_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
 moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
@@ -314,7 +316,8 @@ moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64
  * grad_weight[N, H] (SwiGLU: [2N, H]) and grad_bias, contiguous, of dtype; each may be NULL (not wanted). pre is
  * moe_linear's (not read without an activation). dz = grad_y * act'(pre) is rounded to dtype for the two products
  * grad_x = dz weight and grad_weight = dz^T x; grad_bias sums it before that. residual's gradient is grad_y.
- * With T = 0 grad_weight and grad_bias are zeros. */
+ * With T = 0 grad_weight and grad_bias are zeros. The workspace holds dz, column sums, copies with padded rows and partial
+ * sums: always needed, by the same rules. */
 size_t moe_linear_grad_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
 moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
                            const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,

@@ -169,6 +169,27 @@ def test_combine_gradient_and_router_replayed_on_changed_inputs(ops):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("T,N,H,act", [(1, 8190, 72, "none"), (16, 4100, 520, "none"), (17, 8184, 264, "none"),
+                                       (33, 16384, 64, "none"), (64, 4100, 2040, "none"), (64, 16381, 1032, "none"),
+                                       (5, 2310, 136, "swiglu"), (23, 4091, 200, "swiglu"), (64, 2816, 712, "swiglu")])
+def test_weight_streaming_by_tiles_of_32_rows(ops, T, N, H, act):
+    """Few rows against weights of more than one round of 16-row tiles: sums exact, so those of `pre` are equal too."""
+    halves = 2 if act == "swiglu" else 1
+    x, w, bias = ones((T, H), 1), ones((halves * N, H), 2), ones((halves * N,), 3)
+    res = ones((T, N), 4)
+    y, pre = ops.MoeLinear(x, w, bias, res, act, returnPre=True)
+    z = x.float() @ w.float().t() + bias.float()
+    assert torch.equal(pre, z.to(F16))
+    if act == "none":
+        assert torch.equal(y, (z + res.float()).to(F16))
+    else:  # the sigmoid within 8 fp32 roundings, its products and the sum one each, then the result's
+        g, u = z.double().chunk(2, dim=1)
+        p = g / (1.0 + torch.exp(-g)) * u
+        ref = p + res.double()
+        tol = 16 * U32 * (p.abs() + ref.abs())
+        assert ((y.double() - ref).abs() <= tol + (ref.abs() + tol) * 2.0**-11 + 2.0**-25).all()
+
+
 @pytest.mark.parametrize("seed", range(24))
 def test_random_sizes_without_activation(ops, seed):
     """Any size, layout, alignment and row stride: whole numbers, compared for equality, so a term lost, repeated or read
