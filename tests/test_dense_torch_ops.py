@@ -105,3 +105,42 @@ def test_opcheck_and_compile(ops):
     compiled = torch.compile(lambda a, b: tops.linear(a, b, activation="swiglu"), backend="aot_eager", fullgraph=True)
     with torch.no_grad():
         assert torch.equal(compiled(x, w), tops.linear(x, w, activation="swiglu"))
+
+
+@pytest.mark.gpu
+def test_captured_training_step_replays_on_changed_inputs(ops):
+    """Forward and backward of a router, its experts' combine and a dense expert in one graph, against eager steps on
+    leaves of their own."""
+    shapes = dict(logits=((40, 16), F32), eo=((40, 3, 64), F16), x=((40, 64), F16), gu=((96, 64), F16), down=((64, 48), F16),
+                  dy=((40, 64), F16))
+
+    def fresh(seed):
+        return {k: leaf(s, seed + n, 0.25, d).detach() for n, (k, (s, d)) in enumerate(shapes.items())}
+
+    def step(v):
+        leaves = [v[k].requires_grad_(True) for k in ("logits", "eo", "x", "gu", "down")]
+        ids, w = op.MoeRoutingGroupTopK(leaves[0], None, 3, 4, 2, 2, "softmax")
+        y = tops.linear(tops.linear(leaves[2], leaves[3], activation="swiglu"), leaves[4],
+                        residual=op.MoeCombine(leaves[1], ids, w, 3))
+        return (y.detach(),) + torch.autograd.grad(y, leaves, v["dy"])
+
+    static = fresh(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for seed in range(100, 130, 10):
+        now = fresh(seed)
+        with torch.no_grad():
+            for k, t in static.items():
+                t.copy_(now[k])
+        graph.replay()
+        eager = step(now)
+        torch.cuda.synchronize()
+        for a, b in zip(eager, out):
+            assert torch.equal(a, b)
