@@ -7,7 +7,7 @@
 // Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 8 experts at
 // a time, loads their rows, adds to their dot products and writes their gradient rows. A wave has a token to itself, or
 // four waves share it; the dot products are added over the lanes and then over the waves in a fixed order.
-// T = 16384, H = 2048, K = 6: 872 MB in 144 us, 6.07 TB/s (a copy of 1 GB: 5.0). T = 128, K = 2: 8 us, the call itself.
+// T = 16384, H = 2048, K = 6: 872 MB in 144 us, 6.07 TB/s (a copy of 1 GB: 5.0). T = 128, K = 2: 4 us, of a call of 7.
 #include "moe_device.h"
 #include "moe_launch.h"
 

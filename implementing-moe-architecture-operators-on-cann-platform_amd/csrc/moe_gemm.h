@@ -258,11 +258,20 @@ __device__ __forceinline__ void column_sums(const float* __restrict__ part, uint
     out[c] = T::store(s);
 }
 
-// 8 values of a row from p on, of which `valid` exist (zeros past them); any alignment
-__device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid) {
+// 8 values of a row from p on, of which `valid` exist (zeros past them); any alignment. `before`: values of the row that
+// stand before p. A row's end is the 8 values that end there, moved down: one load, where single ones wait for each other.
+__device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid, int before) {
     typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
     if (valid >= 8) return *reinterpret_cast<const s16x8_any*>(p);
     s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (valid <= 0) return v;
+    if (before + valid >= 8) {
+        const u64x2 x = __builtin_bit_cast(u64x2, *reinterpret_cast<const s16x8_any*>(p + valid - 8));
+        const int bits = 16 * (8 - valid), b = bits & 63;  // 16 .. 112
+        const uint64_t high = x[1] >> b;
+        return __builtin_bit_cast(s16x8, bits >= 64 ? u64x2{high, 0} : u64x2{x[0] >> b | x[1] << (64 - b), high});
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (e < valid) v[e] = static_cast<short>(p[e]);

@@ -19,7 +19,7 @@
 // without a bias need all of their bits: the lowest index that has the maximum is searched, ~95 instructions. Group scores
 // go through LDS, one lane per (token, group). Vector instructions bound the kernel (T = 16384, E = 256, K = 8, fp32
 // logits: 10.3 us without bias and groups, 17 us with a bias and 4 of 8 groups by their two best, of which a copy of the
-// logits is 4 us; the search in place of the key's bits 21 us), at T = 1 the call on the host (8.4 us).
+// logits is 4 us; the search in place of the key's bits 21 us). At T = 1 the one wave's chain takes 7 us.
 #include "moe_device.h"
 #include "moe_launch.h"
 #include "moe_ops.h"

@@ -72,7 +72,8 @@ __device__ __forceinline__ void read_fragments(const uint16_t* tile, int r0, int
 // 8 consecutive elements (of a row's k, or by k of rows) from an operand of any alignment, zeros past its end
 __device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, bool by_k, int row, int k, int rows, int k1) {
     const int valid = row >= rows || k >= k1 ? 0 : by_k ? rows - row : k1 - k;
-    return load8(p + (by_k ? static_cast<int64_t>(k) * ld + row : static_cast<int64_t>(row) * ld + k), valid);
+    return load8(p + (by_k ? static_cast<int64_t>(k) * ld + row : static_cast<int64_t>(row) * ld + k), valid,
+                 by_k ? row : k);
 }
 
 // C[m][n] tile of BM x 128, one ring of direct-to-LDS stages, one barrier a stage.

@@ -69,7 +69,7 @@ __device__ __forceinline__ void dz8(const ActGradArgs& a, int64_t t, int c, floa
         const bool up = c >= a.N;
         const int n = up ? c - a.N : c, valid = a.N - n;
         if (valid >= 8 || (up && valid > 0)) {  // all gate or all up
-            const s16x8 d = load8(dy + n, valid), zg = load8(pre + n, valid), zu = load8(pre + a.N + n, valid);
+            const s16x8 d = load8(dy + n, valid, n), zg = load8(pre + n, valid, n), zu = load8(pre + a.N + n, valid, n);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float g = at<T>(zg, e), s = sigmoid_fast(g);
@@ -91,7 +91,7 @@ __device__ __forceinline__ void dz8(const ActGradArgs& a, int64_t t, int c, floa
         }
         return;
     }
-    const s16x8 d = load8(dy + c, a.Z - c), z = a.pre ? load8(pre + c, a.Z - c) : s16x8{};
+    const s16x8 d = load8(dy + c, a.Z - c, c), z = a.pre ? load8(pre + c, a.Z - c, c) : s16x8{};
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = a.pre ? at<T>(d, e) * slope(at<T>(z, e), a.act) : at<T>(d, e);
 }

@@ -23,7 +23,7 @@ __global__ __launch_bounds__(kThreads) void repack_kernel(RepackArgs a, int64_t 
             if (at >= 0 && at < count) {
                 const int64_t row = at / per;
                 const int col = static_cast<int>(at - row * per) * 8;
-                *reinterpret_cast<s16x8*>(r.dst + row * r.dst_ld + col) = load8(r.src + row * r.src_ld + col, r.cols - col);
+                *reinterpret_cast<s16x8*>(r.dst + row * r.dst_ld + col) = load8(r.src + row * r.src_ld + col, r.cols - col, col);
             }
             first += count;
         }

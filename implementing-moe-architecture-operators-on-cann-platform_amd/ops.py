@@ -24,10 +24,12 @@ import torch
 from . import _lib
 from ._lib import MoeError, check, dims
 
-# The current stream without the Stream object that torch.cuda.current_stream() makes on each call; both are private to
-# torch, so a torch without them takes the public function.
+# The current stream without the Stream object that torch.cuda.current_stream() makes on each call, and the allocation on
+# the current device that torch's compiled code uses (0.75 us a tensor, new_empty 1.5): private to torch, so a torch
+# without them takes the public functions.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", None)
+_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 _TORCH_DT = {_lib.DT_FLOAT16: torch.float16, _lib.DT_INT32: torch.int32}
 _FLOAT_DT = {torch.float32: _lib.DT_FLOAT32, torch.float16: _lib.DT_FLOAT16, torch.bfloat16: _lib.DT_BFLOAT16}
@@ -335,10 +337,15 @@ def _act_code(activation: str) -> int:
     return code
 
 
-def _empty(like: torch.Tensor, stream, shape, dtype: torch.dtype) -> torch.Tensor:
-    """A new tensor that belongs to the stream the kernels run on (_on, without a context for the current one)."""
+def _empty(like: torch.Tensor, stream, shape: tuple, dtype: torch.dtype) -> torch.Tensor:
+    """A new contiguous tensor that belongs to the stream the kernels run on."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        if _empty_strided is None:
+            return like.new_empty(shape, dtype=dtype)
+        dims = len(shape)
+        if dims == 2:
+            return _empty_strided(shape, (shape[1], 1), dtype)
+        return _empty_strided(shape, (1,) if dims == 1 else (shape[1] * shape[2], shape[2], 1), dtype)
     with torch.cuda.stream(stream):
         return like.new_empty(shape, dtype=dtype)
 
@@ -363,7 +370,7 @@ def _workspace(workspace, query, args, like, dev, stream):
         need = int(query(*args))
         if need == 0:
             return None, None, 0
-        workspace = _empty(like, stream, need, torch.uint8)
+        workspace = _empty(like, stream, (need,), torch.uint8)
         return workspace, workspace.data_ptr(), need
     if not isinstance(workspace, torch.Tensor) or workspace.get_device() != dev or not workspace.is_contiguous():
         raise MoeError(4, f"workspace must be a contiguous tensor on cuda:{dev}")
