@@ -13,13 +13,13 @@
 // some rows in a hundred, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
 // never in the instruction cache when it is needed, cost 9 us.
 //
-// A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers. A
-// pick is the maximum over the lane (max3) and over the row (4 DPP steps), and its removal: 16 compares and 16 selects.
+// A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers; few
+// tokens of many experts have a wave each. A pick is the maximum over the lane (max3) and over the row (4 DPP steps), and its removal: 16 compares and 16 selects.
 // Where the key's low 8 bits can hold the expert, the maximum names the pick: ~50 instructions for 4 tokens. fp32 logits
 // without a bias need all of their bits: the lowest index that has the maximum is searched, ~95 instructions. Group scores
 // go through LDS, one lane per (token, group). Vector instructions bound the kernel (T = 16384, E = 256, K = 8, fp32
 // logits: 10.3 us without bias and groups, 17 us with a bias and 4 of 8 groups by their two best, of which a copy of the
-// logits is 4 us; the search in place of the key's bits 21 us). At T = 1 the one wave's chain takes 7 us.
+// logits is 4 us; the search in place of the key's bits 21 us). At T = 1 the one wave's chain takes 5.8 us.
 #include "moe_device.h"
 #include "moe_launch.h"
 #include "moe_ops.h"
@@ -30,8 +30,8 @@ namespace moe {
 
 namespace {
 
-constexpr int kLanes = 16;                   // lanes of one token
-constexpr int kWaveTokens = kWave / kLanes;  // tokens of a workgroup, one wave
+constexpr int kRow = 16;  // lanes of a DPP row
+constexpr int kRowTokens = kWave / kRow;  // tokens of a wave with a DPP row each
 constexpr int kMaxE = 256;
 constexpr int kNoPick = 0xffff;              // a pick with no expert left
 constexpr int kGone = -2147483647 - 1;         // the key of an expert that is not available or was picked
@@ -85,35 +85,44 @@ __device__ __forceinline__ void load4(const void* p, int64_t i, float* v) {
     }
 }
 
-template <typename V>
-__device__ __forceinline__ V row_sum(V v) {
-#pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kLanes);
-    return v;
-}
-
-// All-reduce over a DPP row of 16 lanes by rotations
+// All-reduce over the LANES lanes of a token: a DPP row of 16 by rotations; of a whole wave the rows' four results after that
 template <int CTRL>
 __device__ __forceinline__ int dpp(int v) {
     return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
 }
+__device__ __forceinline__ int row_of(int v, int row) { return __builtin_amdgcn_readlane(v, row * kRow); }
+template <int LANES>
 __device__ __forceinline__ int row_max_i(int v) {
     v = max(v, dpp<0x128>(v));
     v = max(v, dpp<0x124>(v));
     v = max(v, dpp<0x122>(v));
-    return max(v, dpp<0x121>(v));
+    v = max(v, dpp<0x121>(v));
+    return LANES == kRow ? v : max(max(row_of(v, 0), row_of(v, 1)), max(row_of(v, 2), row_of(v, 3)));
 }
+template <int LANES>
 __device__ __forceinline__ int row_min_i(int v) {
     v = min(v, dpp<0x128>(v));
     v = min(v, dpp<0x124>(v));
     v = min(v, dpp<0x122>(v));
-    return min(v, dpp<0x121>(v));
+    v = min(v, dpp<0x121>(v));
+    return LANES == kRow ? v : min(min(row_of(v, 0), row_of(v, 1)), min(row_of(v, 2), row_of(v, 3)));
 }
+template <int LANES>
+__device__ __forceinline__ double row_sum(double v) {
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, LANES);
+    return v;
+}
+template <int LANES>
 __device__ __forceinline__ float row_sum_f(float v) {
-    v += __builtin_bit_cast(float, dpp<0x128>(__builtin_bit_cast(int, v)));
-    v += __builtin_bit_cast(float, dpp<0x124>(__builtin_bit_cast(int, v)));
-    v += __builtin_bit_cast(float, dpp<0x122>(__builtin_bit_cast(int, v)));
-    return v + __builtin_bit_cast(float, dpp<0x121>(__builtin_bit_cast(int, v)));
+    auto turned = [](float x, auto ctrl) { return __builtin_bit_cast(float, dpp<decltype(ctrl)::value>(__builtin_bit_cast(int, x))); };
+    v += turned(v, std::integral_constant<int, 0x128>());
+    v += turned(v, std::integral_constant<int, 0x124>());
+    v += turned(v, std::integral_constant<int, 0x122>());
+    v += turned(v, std::integral_constant<int, 0x121>());
+    if (LANES == kRow) return v;
+    auto row = [&](int i) { return __builtin_bit_cast(float, row_of(__builtin_bit_cast(int, v), i)); };
+    return (row(0) + row(1)) + (row(2) + row(3));
 }
 
 // Floats as integers in the same order (-0 as 0); key_value undoes it
@@ -132,33 +141,37 @@ __device__ __forceinline__ float gap_limit(bool sigmoid, float s_max, float c) {
 }
 
 // LDS of the one wave of a workgroup. A row may have E picks.
+template <int TOKENS>
 struct RoutingLds {
     int E, G, K;
     __host__ __device__ int pitch() const { return (E + 3) / 4 * 4 + 4; }
-    __host__ __device__ int picks_at() const { return 8 * kWaveTokens * K; }  // after the parts (double): 16 bits each
-    __host__ __device__ int order_at() const { return picks_at() + 2 * kWaveTokens * E; }
+    __host__ __device__ int picks_at() const { return 8 * TOKENS * K; }  // after the parts (double): 16 bits each
+    __host__ __device__ int order_at() const { return picks_at() + 2 * TOKENS * E; }
     __host__ __device__ int scores_at() const { return (order_at() + 2 * E + 3) / 4 * 4; }
-    __host__ __device__ int kept_at() const { return scores_at() + 4 * kWaveTokens * G; }
-    __host__ __device__ int cut_at() const { return kept_at() + 4 * kWaveTokens * G; }
+    __host__ __device__ int kept_at() const { return scores_at() + 4 * TOKENS * G; }
+    __host__ __device__ int cut_at() const { return kept_at() + 4 * TOKENS * G; }
     // c of the rows' experts, fp32; or, once the groups are scored, float64 values of one row and its groups
-    __host__ __device__ int row_at() const { return (cut_at() + 8 * kWaveTokens + 15) / 16 * 16; }
-    __host__ __device__ int bytes(bool rows) const { return row_at() + (rows ? 4 * kWaveTokens * pitch() : 0); }
+    __host__ __device__ int row_at() const { return (cut_at() + 8 * TOKENS + 15) / 16 * 16; }
+    __host__ __device__ int bytes(bool rows) const {
+        const int scores = 4 * TOKENS * pitch(), exact = 8 * (E + G);
+        return row_at() + (rows ? (scores > exact ? scores : exact) : 0);
+    }
 };
 
 // Expert of lane l's register j: 16-byte (8-byte) pieces of 4 consecutive experts
-template <int C>
+template <int LANES, int C>
 __device__ __forceinline__ int expert_of(int l, int j) {
     constexpr int V = C < 4 ? C : 4;
-    return j / V * (kLanes * V) + l * V + j % V;
+    return j / V * (LANES * V) + l * V + j % V;
 }
 
 // Lane l's logits of the row that starts at element `at`; -inf past E
-template <typename L, int C, bool VEC>
+template <typename L, int LANES, int C, bool VEC>
 __device__ __forceinline__ void load_logits(const void* p, int64_t at, int E, int l, float (&v)[C]) {
     if constexpr (VEC && C >= 4) {
 #pragma unroll
         for (int j = 0; j < C; j += 4) {
-            const int e = expert_of<C>(l, j);
+            const int e = expert_of<LANES, C>(l, j);
             if (e < E) {  // E % 4 == 0
                 load4<L>(p, at + e, &v[j]);
             } else {
@@ -169,7 +182,7 @@ __device__ __forceinline__ void load_logits(const void* p, int64_t at, int E, in
     } else {
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const int e = expert_of<C>(l, j);
+            const int e = expert_of<LANES, C>(l, j);
             v[j] = e < E ? logit<L>(p, at + e) : kLow;
         }
     }
@@ -213,13 +226,14 @@ __device__ __forceinline__ void exact_scores(const GroupRouting& r, int64_t t, d
 // Whether c comes before o in descending order, the lower index first among equals
 __device__ __forceinline__ bool goes_before(double o, int oi, double c, int ci) { return o > c || (o == c && oi < ci); }
 
-// C: experts of a lane. VEC: rows allow loads of 4 experts.
-template <typename L, int C, bool VEC>
+// LANES: lanes of a token. C: experts of a lane. VEC: rows allow loads of 4 experts.
+template <typename L, int LANES, int C, bool VEC>
 __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, int32_t* __restrict__ ids,
                                                               void* __restrict__ weights) {
+    constexpr int kTokens = kWave / LANES;
     extern __shared__ __align__(16) char shared[];
     const int E = r.E, G = r.groups, K = r.K, size = E / G;
-    const RoutingLds lay{E, G, K};
+    const RoutingLds<kTokens> lay{E, G, K};
     double* parts = reinterpret_cast<double*>(shared);
     uint16_t* pick = reinterpret_cast<uint16_t*>(shared + lay.picks_at());  // [token][E]
     uint16_t* order = reinterpret_cast<uint16_t*>(shared + lay.order_at());
@@ -229,13 +243,13 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     float* row = reinterpret_cast<float*>(shared + lay.row_at());
     double* cs = reinterpret_cast<double*>(row);
     double* cgs = cs + E;
-    const int lane = lane_id(), tok = lane / kLanes, l = lane % kLanes;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaveTokens + tok;
+    const int lane = lane_id(), tok = lane / LANES, l = lane % LANES;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + tok;
     const bool valid = t < r.T;
 
     float v[C];  // logits, -inf where not available
     if (valid) {
-        load_logits<L, C, VEC>(r.logits, t * r.ld, E, l, v);
+        load_logits<L, LANES, C, VEC>(r.logits, t * r.ld, E, l, v);
     } else {
 #pragma unroll
         for (int j = 0; j < C; ++j) v[j] = kLow;
@@ -245,12 +259,13 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     const bool grouped = r.top_groups < G;
     const bool all_softmax = !r.sigmoid && !r.renormalize;  // weights over the whole row
     const bool scored = r.bias || (grouped && r.group_top == 2);
-    float top = 0.0f, sum = 1.0f, s_max = 1.0f;
+    float top = 0.0f, s_max = 1.0f;
+    double whole = 1.0;  // sum of the row's e^(l - top)
     if (!r.sigmoid && (scored || all_softmax)) {
         int m = key_of(v[0]);
 #pragma unroll
         for (int j = 1; j < C; ++j) m = max(m, key_of(v[j]));
-        top = key_value(row_max_i(m));
+        top = key_value(row_max_i<LANES>(m));
     }
     int key[C];
     float s[C];
@@ -260,14 +275,20 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             for (int j = 0; j < C; ++j)  // 0 for -inf
                 s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v[j] * -1.4426950408889634f));
         } else {
-            sum = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 const float d = v[j] == top ? 0.0f : v[j] - top;
                 s[j] = v[j] > kLow ? __builtin_amdgcn_exp2f(d * 1.4426950408889634f) : 0.0f;
                 sum += s[j];
             }
-            sum = row_sum_f(sum);
+            if (all_softmax) {  // in float64, so that a row's weights do not depend on how it is spread over lanes
+                whole = 0.0;
+#pragma unroll
+                for (int j = 0; j < C; ++j) whole += static_cast<double>(s[j]);
+                whole = row_sum<LANES>(whole);
+            }
+            sum = row_sum_f<LANES>(sum);
             s_max = sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 1.0f;
 #pragma unroll
             for (int j = 0; j < C; ++j) s[j] *= s_max;
@@ -275,7 +296,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     }
     if (r.bias) {
         float b[C];
-        load_logits<F32, C, VEC>(r.bias, 0, E, l, b);
+        load_logits<F32, LANES, C, VEC>(r.bias, 0, E, l, b);
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const float c = s[j] + b[j];
@@ -291,7 +312,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         float* out = row + tok * lay.pitch();
 #pragma unroll
         for (int j = 0; j < C; j += (C < 4 ? 1 : 4)) {  // a row's end may be written past E: the pitch has room
-            const int e = expert_of<C>(l, j);
+            const int e = expert_of<LANES, C>(l, j);
             if constexpr (C < 4) {
                 if (e < E) out[e] = entry(j);
             } else if (e < E) {
@@ -299,7 +320,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             }
         }
         __syncthreads();
-        for (int i = lane; i < kWaveTokens * G; i += kWave) {
+        for (int i = lane; i < kTokens * G; i += kWave) {
             const int q = i / G, g = i - q * G;
             const float* c = row + q * lay.pitch() + g * size;
             float a = kLow, b = kLow;
@@ -320,7 +341,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             gs[i] = r.group_top == 2 && b > kLow ? a + b : a;
         }
         __syncthreads();
-        for (int i = lane; i < kWaveTokens * G; i += kWave) {
+        for (int i = lane; i < kTokens * G; i += kWave) {
             const int q = i / G, g = i - q * G;
             const float* o = gs + q * G;
             const float x = o[g];
@@ -336,9 +357,9 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             const float x = cut[2 * tok], y = cut[2 * tok + 1];
             uint64_t open = __ballot(valid && y > kLow && !(x - y > gap_limit(r.sigmoid, s_max, x)));
 #pragma unroll 1
-            for (int q = 0; open && q < kWaveTokens; ++q) {
-                if (!((open >> (q * kLanes)) & 1)) continue;
-                exact_scores<L>(r, static_cast<int64_t>(blockIdx.x) * kWaveTokens + q, cs);
+            for (int q = 0; open && q < kTokens; ++q) {
+                if (!((open >> (q * LANES)) & 1)) continue;
+                exact_scores<L>(r, static_cast<int64_t>(blockIdx.x) * kTokens + q, cs);
 #pragma unroll 1
                 for (int g = lane; g < G; g += kWave) {
                     double a = kNone, b = kNone;
@@ -362,7 +383,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         if (C >= 4 && size % 4 == 0) {  // a piece's experts are of one group
 #pragma unroll
             for (int j = 0; j < C; j += 4) {
-                const int e = expert_of<C>(l, j);
+                const int e = expert_of<LANES, C>(l, j);
                 if (e >= E || mine[(e * r.size_inverse) >> 16]) continue;
 #pragma unroll
                 for (int i = j; i < min(j + 4, C); ++i) key[i] = kGone;
@@ -370,7 +391,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         } else {
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                const int e = expert_of<C>(l, j);
+                const int e = expert_of<LANES, C>(l, j);
                 if (e < E && !mine[(e * r.size_inverse) >> 16]) key[j] = kGone;
             }
         }
@@ -382,14 +403,14 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         // those bits free; c loses them, up to 2^-15 of it, which counts as an error like fp32's own.
 #pragma unroll
         for (int j = 0; j < C; ++j)
-            key[j] = key[j] == kGone ? kGone : (key[j] & ~(kMaxE - 1)) | (kMaxE - 1 - expert_of<C>(l, j));
+            key[j] = key[j] == kGone ? kGone : (key[j] & ~(kMaxE - 1)) | (kMaxE - 1 - expert_of<LANES, C>(l, j));
         int last = kGone;
 #pragma unroll 1
         for (int k = 0;; ++k) {
             int m = key[0];
 #pragma unroll
             for (int j = 1; j < C; ++j) m = max(m, key[j]);
-            m = row_max_i(m);
+            m = row_max_i<LANES>(m);
             if (r.bias) {
                 const float x = key_value(last & ~(kMaxE - 1)), y = key_value(m & ~(kMaxE - 1));
                 const bool clear = x - y > gap_limit(r.sigmoid, s_max, x) + fabsf(y) * 0x1p-15f;
@@ -412,13 +433,13 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             int m = key[0];
 #pragma unroll
             for (int j = 1; j < C; ++j) m = max(m, key[j]);
-            m = row_max_i(m);
+            m = row_max_i<LANES>(m);
             int jw = -1;
 #pragma unroll
             for (int j = C - 1; j >= 0; --j) jw = key[j] == m ? j : jw;
-            const int e = row_min_i(jw < 0 ? kMaxE : expert_of<C>(l, jw));
+            const int e = row_min_i<LANES>(jw < 0 ? kMaxE : expert_of<LANES, C>(l, jw));
             if (l == 0) pick[tok * E + k] = static_cast<uint16_t>(m == kGone ? kNoPick : e);
-            const int mine = e / kStep % kLanes == l ? e / (kLanes * kStep) * kStep + e % kStep : -1;  // its register
+            const int mine = e / kStep % LANES == l ? e / (LANES * kStep) * kStep + e % kStep : -1;  // its register
 #pragma unroll
             for (int j = 0; j < C; ++j) key[j] = mine == j ? kGone : key[j];
         }
@@ -426,10 +447,10 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     __syncthreads();
     uint64_t redo = __ballot(reorder && valid);
 #pragma unroll 1
-    for (int q = 0; redo && q < kWaveTokens; ++q) {
-        if (!((redo >> (q * kLanes)) & 1)) continue;
-        const int64_t tq = static_cast<int64_t>(blockIdx.x) * kWaveTokens + q;
-        const int n = __shfl(picks, q * kLanes, kWave);
+    for (int q = 0; redo && q < kTokens; ++q) {
+        if (!((redo >> (q * LANES)) & 1)) continue;
+        const int64_t tq = static_cast<int64_t>(blockIdx.x) * kTokens + q;
+        const int n = __shfl(picks, q * LANES, kWave);
         uint16_t* of = pick + q * E;
         if (r.sigmoid) {  // the picks' alone
             for (int k = lane; k < n; k += kWave) {
@@ -463,18 +484,18 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     double* part = parts + tok * K;
     int ref_key = kGone;
     const float first = l < K && my[l] != kNoPick ? logit<L>(r.logits, t * r.ld + my[l]) : 0.0f;
-    auto chosen = [&](int k) { return k < kLanes ? first : logit<L>(r.logits, t * r.ld + my[k]); };
+    auto chosen = [&](int k) { return k < LANES ? first : logit<L>(r.logits, t * r.ld + my[k]); };
     if (r.renormalize) {
-        for (int k = l; k < K; k += kLanes) {
+        for (int k = l; k < K; k += LANES) {
             if (my[k] == kNoPick) continue;
             const float x = chosen(k);
             ref_key = max(ref_key, key_of(r.sigmoid ? fminf(x, 0.0f) : x));
         }
-        ref_key = row_max_i(ref_key);
+        ref_key = row_max_i<LANES>(ref_key);
     }
     const double ref = r.renormalize ? static_cast<double>(key_value(ref_key)) : r.sigmoid ? 0.0 : static_cast<double>(top);
     double total = 0.0;
-    for (int k = l; k < K; k += kLanes) {
+    for (int k = l; k < K; k += LANES) {
         double p = 0.0;
         if (my[k] != kNoPick) {
             const double x = static_cast<double>(chosen(k));
@@ -486,12 +507,12 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     }
     double factor = static_cast<double>(r.scale);
     if (r.renormalize) {
-        total = row_sum(total);
+        total = row_sum<LANES>(total);
         factor = total > 0.0 ? factor / total : 0.0;
     } else if (!r.sigmoid) {
-        factor = sum > 0.0f ? factor / static_cast<double>(sum) : 0.0;
+        factor = whole > 0.0 ? factor / whole : 0.0;
     }
-    for (int k = l; k < K; k += kLanes) {  // each lane its own parts
+    for (int k = l; k < K; k += LANES) {  // each lane its own parts
         ids[t * K + k] = my[k] == kNoPick ? -1 : my[k];
         const float w = static_cast<float>(part[k] * factor);
         if (r.weights_type == MOE_DT_FLOAT32) put<F32>(weights, t * K + k, w);
@@ -524,8 +545,8 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
                                                                    void* __restrict__ grad_logits) {
     extern __shared__ __align__(16) char shared[];
     const int E = r.E, K = r.K, pitch = (E + 3) / 4 * 4 + 4;
-    const int lane = lane_id(), tok = lane / kLanes, l = lane % kLanes;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaveTokens + tok;
+    const int lane = lane_id(), tok = lane / kRow, l = lane % kRow;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kRowTokens + tok;
     const bool valid = t < r.T;
     float* row = reinterpret_cast<float*>(shared) + tok * pitch;
     const bool softmax_all = !r.sigmoid && !r.renormalize;
@@ -548,7 +569,7 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         return p;
     };
     const Pick first = load_pick(l);
-    auto pick_at = [&](int k) { return k < kLanes ? first : load_pick(k); };
+    auto pick_at = [&](int k) { return k < kRow ? first : load_pick(k); };
 
     // Scores up to a factor e^-top: of the row's softmax where all of it counts, else, renormalised, relative to the
     // largest of the picks, so that picks far below the row's best keep their ratios.
@@ -556,7 +577,7 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
     if (softmax_all) {
         float v[C];
         if (valid) {
-            load_logits<L, C, VEC>(r.logits, t * r.ld, E, l, v);
+            load_logits<L, kRow, C, VEC>(r.logits, t * r.ld, E, l, v);
         } else {
 #pragma unroll
             for (int j = 0; j < C; ++j) v[j] = kLow;
@@ -567,7 +588,7 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
             v[j] = v[j] > kLow ? v[j] : kLow;
             m = max(m, key_of(v[j]));
         }
-        top = key_value(row_max_i(m));
+        top = key_value(row_max_i<kRow>(m));
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -575,15 +596,15 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
             s[j] = v[j] > kLow ? __builtin_amdgcn_exp2f(d * 1.4426950408889634f) : 0.0f;
             sum += s[j];
         }
-        sum = row_sum_f(sum);
+        sum = row_sum_f<kRow>(sum);
         inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     } else if (r.renormalize) {
         int m = kGone;
-        for (int k = l; k < K; k += kLanes) {
+        for (int k = l; k < K; k += kRow) {
             const Pick p = pick_at(k);
             if (p.id >= 0) m = max(m, key_of(r.sigmoid ? fminf(p.x, 0.0f) : p.x));
         }
-        m = row_max_i(m);
+        m = row_max_i<kRow>(m);
         top = m == kGone ? 0.0f : key_value(m);
     }
     auto score = [&](float v) {
@@ -591,32 +612,32 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         return (v == top ? 1.0f : expf(v - top)) * inv;
     };
     float total = 0.0f, dot = 0.0f;  // sums of s and g s over the picks
-    for (int k = l; k < K; k += kLanes) {
+    for (int k = l; k < K; k += kRow) {
         const Pick p = pick_at(k);
         if (p.id < 0) continue;
         const float sk = score(p.x);
         total += sk;
         dot += p.g * sk;
     }
-    total = row_sum_f(total);
-    dot = row_sum_f(dot);
+    total = row_sum_f<kRow>(total);
+    dot = row_sum_f<kRow>(dot);
     const float norm = r.renormalize ? (total > 0.0f ? 1.0f / total : 0.0f) : 1.0f;
     const float mean = r.renormalize ? dot * norm : 0.0f;
 
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        const int e = expert_of<C>(l, j);
+        const int e = expert_of<kRow, C>(l, j);
         if (e < E) row[e] = 0.0f;
     }
     __syncthreads();
-    for (int k0 = 0; k0 < K; k0 += kLanes) {
+    for (int k0 = 0; k0 < K; k0 += kRow) {
         const Pick p = pick_at(k0 + l);
         float d = 0.0f;
         if (p.id >= 0) {
             d = (p.g - mean) * score(p.x) * norm;
             if (r.sigmoid) d *= expf(fminf(-p.x, 0.0f)) / (1.0f + expf(-fabsf(p.x)));  // 1 - s
         }
-        for (int i = 0; i < kLanes && k0 + i < K; ++i) {
+        for (int i = 0; i < kRow && k0 + i < K; ++i) {
             if (l == i && p.id >= 0) row[p.id] += d;
             __syncthreads();  // one wave: orders the additions
         }
@@ -624,7 +645,7 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
     if (!valid) return;
 #pragma unroll
     for (int j = 0; j < C; j += (VEC && C >= 4 ? 4 : 1)) {
-        const int e = expert_of<C>(l, j);
+        const int e = expert_of<kRow, C>(l, j);
         if (e >= E) continue;
         if constexpr (VEC && C >= 4) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(row + e);
@@ -640,6 +661,11 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
     }
 }
 
+// Up to two rows a SIMD a token of more than 64 experts has a wave, whose chain is shorter: E = 256 with bias and groups,
+// T = 1 5.8 us (a DPP row 7.2), T = 2048 8.8 (10.5), T = 4096 10.8 (11.6), there without a bias 9.4 (7.9). At 64 experts
+// both take 4.9 us at T = 1 and the DPP row less from there on.
+constexpr int64_t kWaveRows = 2048;
+
 // Rows of 4-expert pieces that one load can read
 bool vector_logits(const GroupRouting& r) {
     const uintptr_t mask = r.logits_type == MOE_DT_FLOAT32 ? 15 : 7;
@@ -647,23 +673,30 @@ bool vector_logits(const GroupRouting& r) {
            (reinterpret_cast<uintptr_t>(r.bias) & 15) == 0;
 }
 
-template <typename L, int C, bool VEC>
+template <typename L, int LANES, int C, bool VEC>
 hipError_t run_routing_vec(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream) {
+    constexpr int kTokens = kWave / LANES;
     TraceScope trace("moe_group_routing", stream);
-    group_routing_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kWaveTokens - 1) / kWaveTokens), kWave,
-                                      RoutingLds{r.E, r.groups, r.K}.bytes(r.bias || r.top_groups < r.groups), stream>>>(r, ids, weights);
+    group_routing_kernel<L, LANES, C, VEC>
+        <<<static_cast<unsigned>((r.T + kTokens - 1) / kTokens), kWave,
+           RoutingLds<kTokens>{r.E, r.groups, r.K}.bytes(r.bias || r.top_groups < r.groups), stream>>>(r, ids, weights);
     return hipGetLastError();
+}
+template <typename L, int LANES, int C>
+hipError_t run_routing_lanes(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream) {
+    return vector_logits(r) ? run_routing_vec<L, LANES, C, true>(r, ids, weights, stream)
+                            : run_routing_vec<L, LANES, C, false>(r, ids, weights, stream);
 }
 template <typename L, int C>
 hipError_t run_routing(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream) {
-    return vector_logits(r) ? run_routing_vec<L, C, true>(r, ids, weights, stream)
-                            : run_routing_vec<L, C, false>(r, ids, weights, stream);
+    if (C > 4 && r.T <= kWaveRows) return run_routing_lanes<L, kWave, 4>(r, ids, weights, stream);
+    return run_routing_lanes<L, kRow, C>(r, ids, weights, stream);
 }
 template <typename L, int C, bool VEC>
 hipError_t run_grad_vec(const GroupRouting& r, const void* gw, const int32_t* ids, void* gl, hipStream_t stream) {
     TraceScope trace("moe_group_routing_grad", stream);
-    const int lds = kWaveTokens * ((r.E + 3) / 4 * 4 + 4) * 4;
-    group_routing_grad_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kWaveTokens - 1) / kWaveTokens), kWave, lds,
+    const int lds = kRowTokens * ((r.E + 3) / 4 * 4 + 4) * 4;
+    group_routing_grad_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kRowTokens - 1) / kRowTokens), kWave, lds,
                                            stream>>>(r, gw, ids, gl);
     return hipGetLastError();
 }
@@ -675,7 +708,7 @@ hipError_t run_grad(const GroupRouting& r, const void* gw, const int32_t* ids, v
 
 template <typename F>
 hipError_t by_type(const GroupRouting& r, F&& f) {
-    const int c = (r.E + kLanes - 1) / kLanes;
+    const int c = (r.E + kRow - 1) / kRow;
     auto with = [&](auto type) {
         if (c <= 1) return f(type, std::integral_constant<int, 1>());
         if (c <= 4) return f(type, std::integral_constant<int, 4>());

@@ -58,6 +58,28 @@ def test_routing_and_its_gradient_past_32_bits(ops):
         assert torch.equal(grad[at], ops.MoeRoutingGroupTopKGrad(gw[at].clone(), part, pids, "sigmoid"))
 
 
+@pytest.mark.parametrize("E,G,TG,GT", [(65, 13, 5, 2), (100, 1, 1, 1), (256, 8, 4, 2), (256, 128, 9, 2)])
+@pytest.mark.parametrize("scoring,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+def test_routing_of_many_rows_is_that_of_few(ops, E, G, TG, GT, scoring, renorm):
+    """A row's choice and weights do not depend on how many rows the call has, which decides how many lanes a row gets."""
+    T = 2500
+    g = torch.Generator(device="cuda").manual_seed(E + G)
+    logits = torch.randn((T, E), generator=g, device="cuda")
+    logits[torch.rand((T, E), generator=g, device="cuda") < 0.2] = float("-inf")
+    logits[7] = float("-inf")
+    logits[8] = torch.finfo(F32).min
+    logits[9:40] = (logits[9:40] * 4).round() / 4  # ties
+    logits[40, 1] = float("nan")
+    bias = ((torch.rand((E,), generator=g, device="cuda") - 0.5) * 0.2 * 64).round() / 64
+    for dtype, b in ((F32, None), (F32, bias), (F16, None), (BF16, bias)):
+        x = logits.to(dtype)
+        ids, w = ops.MoeRoutingGroupTopK(x, b, 8, G, TG, GT, scoring, renorm, 2.0, F32)
+        for t in range(0, T, 500):
+            at = slice(t, t + 500)
+            pids, pw = ops.MoeRoutingGroupTopK(x[at], b, 8, G, TG, GT, scoring, renorm, 2.0, F32)
+            assert torch.equal(ids[at], pids) and torch.equal(w[at], pw)
+
+
 def test_combine_gradient_past_32_bits(ops):
     T, H, K = 140001, 2048, 8  # 2.3e9 elements
     eo, dy = ones((T, K, H), 4), ones((T, H), 5)
