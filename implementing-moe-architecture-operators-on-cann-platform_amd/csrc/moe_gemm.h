@@ -182,6 +182,52 @@ __host__ __device__ __forceinline__ bool vector_rows(const GemmArgs& g) {
     return g.n % 4 == 0 && ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.residual)) & mask) == 0;
 }
 
+// Whether store_block may write 8 columns of the 16-bit result at once
+__device__ __forceinline__ bool whole_lines(const GemmArgs& g, bool vec) {
+    return vec && !g.out_f32 && g.n % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+}
+
+// 16 rows of a wave's sums on their way to memory. They pass through a piece of LDS that is the wave's own, 16 rows x NB
+// blocks of 16 columns of fp32 (SwiGLU: the first half gate, the second up), so that a lane has 8 columns of one row and
+// what the epilogue reads and writes is whole lines. Granule G (16 bytes) of row r stands at G ^ r.
+template <int NB>
+__device__ __forceinline__ void put_block(float* stg, int row16, int kg, int j, f32x4 v) {
+    *reinterpret_cast<f32x4*>(stg + (row16 * NB * 4 + ((j * 4 + kg) ^ (row16 % (NB * 4)))) * 4) = v;
+}
+template <typename T, bool SWIGLU, int NB>
+__device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg, int lane, int row0, int col0, bool vec,
+                                            bool lines) {
+    constexpr int kGranules = NB * 4, kPer = (SWIGLU ? NB / 2 : NB) * 2;  // lanes of a row
+    auto get = [&](int r, int gr) __attribute__((always_inline)) {
+        return *reinterpret_cast<const f32x4*>(stg + (r * kGranules + (gr ^ (r % kGranules))) * 4);
+    };
+    // the reads take what other lanes of this wave just wrote (LDS operations of one wave run in order)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 1
+    for (int at = lane; at < 16 * kPer; at += kWave) {
+        const int r = at / kPer, c = at % kPer, row = row0 + r, col = col0 + c * 8;
+        f32x4 z[2], u[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            z[e] = get(r, 2 * c + e);
+            u[e] = SWIGLU ? get(r, kGranules / 2 + 2 * c + e) : z[e];
+        }
+        if (row >= g.m || col >= g.n) continue;
+        if (lines) {
+            const uint2 a = pack4<T>(finish4<T, SWIGLU>(g, row, col, 4, true, z[0], u[0]));
+            const uint2 b = pack4<T>(finish4<T, SWIGLU>(g, row, col + 4, 4, true, z[1], u[1]));
+            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.n + col) =
+                u32x4{a.x, a.y, b.x, b.y};
+        } else {
+            store4<T, SWIGLU>(g, row, col, z[0], u[0], vec);
+            store4<T, SWIGLU>(g, row, col + 4, z[1], u[1], vec);
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // read before the next block's writes
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // ds_read_b64_tr_b16: 8 bytes per lane, handed out transposed within each 16-lane group (lane i gets element i % 4 of
 // the 8 bytes addressed by lanes 4 j + i / 4, j = 0 .. 3). An operand tile stored by k (64 k x 128 rows, 256 bytes a k) gives
 // a fragment of 16 rows and 32 k as two such reads, 4 k each. These read N fragments for both 32-k steps of a stage,

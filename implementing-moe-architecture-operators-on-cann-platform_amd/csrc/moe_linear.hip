@@ -29,6 +29,13 @@ constexpr int mid_threads(int bm) { return mid_waves(bm) * kWave; }
 constexpr int ring_stages(int bm) { return bm == 128 ? 2 : bm == 32 ? 4 : 3; }
 constexpr int mid_lds_bytes(int bm) { return ring_stages(bm) * (bm + kBN) * kBK * 2; }
 
+__device__ __forceinline__ void ring_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // Where the 16 bytes that lane `lane` of copy instruction `i` writes to LDS come from. Direct-to-LDS copies write 64
 // consecutive 16-byte granules, so the layout's swizzle is in which granule each lane fetches.
 //   by rows: an LDS row is one operand row, 64 k = 8 granules; granule g of row r stands at g ^ ((r >> 1) & 7), so the
@@ -99,7 +106,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
     if (item >= mtiles * ntiles * g.splits) return;
     const bool n_first = mtiles > ntiles;
     const int inner = n_first ? ntiles : mtiles, outer = item / inner;
-    const int i0 = item - outer * inner, sp = outer % g.splits, o0 = outer / g.splits;
+    const int outers = n_first ? mtiles : ntiles;
+    const int i0 = item - outer * inner, sp = outer / outers, o0 = outer - sp * outers;
     const int mt = n_first ? o0 : i0, nt = n_first ? i0 : o0;
     const int k0 = sp * g.split_k, k1 = min(g.k, k0 + g.split_k);
     const int nst = max(1, (k1 - k0 + kBK - 1) / kBK);
@@ -199,10 +207,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
         // so have everyone's, and the slot of stage s - 1 may be filled again
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * (PC + QC)) & 0xf0ffu);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-        __builtin_amdgcn_sched_barrier(0);
+        ring_barrier();
         copy_stage(s + NS - 1);
         const uint16_t* tp = lds + (s % NS) * kSlot;
         const uint16_t* tq = tp + BM * kBK;
@@ -217,28 +222,45 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 #pragma unroll
                 for (int i = 0; i < FM; ++i) acc[j][i] = T::mfma(fq[kk][j], fp[kk][i], acc[j][i]);
     }
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the surplus copies have landed before the workgroup ends
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & 0xf0ffu);  // the surplus copies have landed
 
     // acc[j][i]: D[Q row 4 kg + r of block j][P row row16 of block i], 4 consecutive columns of one row
     constexpr int FO = SWIGLU ? FN / 2 : FN;
-    const bool vec = vector_rows(g);
-    const int64_t pld = part_ld(g.n, SWIGLU), pcols = part_cols(g.n);
+    const int r0 = m0 + wm * (BM / WM), c0 = n0 + wn * (FO * 16);
+    if (g.splits > 1) {
+        const int64_t pld = part_ld(g.n, SWIGLU), pcols = part_cols(g.n);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int row = m0 + wm * (BM / WM) + i * 16 + row16;
-        if (row >= g.m) continue;
+        for (int i = 0; i < FM; ++i) {
+            const int row = r0 + i * 16 + row16;
+            if (row >= g.m) continue;
 #pragma unroll
-        for (int j = 0; j < FO; ++j) {
-            const int col = n0 + wn * (FO * 16) + j * 16 + kg * 4;
-            if (g.splits > 1) {
+            for (int j = 0; j < FO; ++j) {
+                const int col = c0 + j * 16 + kg * 4;
                 if (col >= g.n) continue;
                 float* dst = g.partial + (static_cast<int64_t>(sp) * g.m + row) * pld + col;
                 *reinterpret_cast<f32x4*>(dst) = acc[j][i];
                 if (SWIGLU) *reinterpret_cast<f32x4*>(dst + pcols) = acc[j + FO][i];
-            } else {
-                store4<T, SWIGLU>(g, row, col, acc[j][i], SWIGLU ? acc[j + FO][i] : acc[j][i], vec);
             }
         }
+        return;
+    }
+    ring_barrier();  // everyone's reads and copies are over: the ring's room is the epilogue's
+    const bool vec = vector_rows(g), lines = whole_lines(g, vec);
+    float* stg = reinterpret_cast<float*>(lds) + wave * (FN * 256);
+    auto put = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) put_block<FN>(stg, row16, kg, j, acc[j][i]);
+    };
+#pragma unroll 1
+    for (int i = 0; i < FM; ++i) {  // one copy of the epilogue's code
+        switch (i) {
+            case 0: put(0); break;
+            case 1: put(1); break;
+            case 2: put(FM > 2 ? 2 : 0); break;
+            default: put(FM > 3 ? 3 : 0); break;
+        }
+        store_block<T, SWIGLU, FN>(g, stg, lane, r0 + i * 16, c0, vec, lines);
     }
 }
 

@@ -213,26 +213,16 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         tick_c(acc[1], first);
     };
 
-    // acc[a][b][i][j]: rows a * 128 + wm * 64 + i * 16 + row16, columns of Q half b, 4 consecutive ones from 4 kg on. A
-    // block of 16 rows passes through the wave's own 4 KB of LDS as fp32 (64 columns; SwiGLU: 32 of gate, 32 of up), so
-    // that a lane has 8 columns of one row and everything the epilogue reads and writes is whole lines. The 8 blocks
-    // share one copy of the epilogue's code: unrolled, its activations are too long for the accumulators to stay in
-    // registers. Granule G (16 bytes) of row r stands at G ^ r.
+    // acc[a][b][i][j]: rows a * 128 + wm * 64 + i * 16 + row16, columns of Q half b, 4 consecutive ones from 4 kg on. The 8
+    // blocks of 16 rows share one copy of the epilogue's code: unrolled, its activations are too long for the accumulators
+    // to stay in registers.
     auto epilogue = [&](const Acc (&acc)[2], const Tile& t) __attribute__((always_inline)) {
         const int ln = lane_fresh(), row16 = ln & 15, kg = ln >> 4;
-        const bool vec = vector_rows(g);
-        const bool lines = vec && !g.out_f32 && g.n % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-        constexpr int kCols = SWIGLU ? 32 : 64;  // columns of a wave
-        constexpr int kPer = kCols / 8;          // lanes per row
+        const bool vec = vector_rows(g), lines = whole_lines(g, vec);
         float* stg = reinterpret_cast<float*>(lds + 2 * kStageHalfs) + wave * (kEpiBytes / 4);
         auto put = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<f32x4*>(stg + row16 * 64 + (((j * 4 + kg) ^ row16) << 2)) =
-                    acc[i >> 2][j >> 1][i & 3][j & 1];
-        };
-        auto get = [&](int r, int gr) __attribute__((always_inline)) {
-            return *reinterpret_cast<const f32x4*>(stg + r * 64 + ((gr ^ r) << 2));
+            for (int j = 0; j < 4; ++j) put_block<4>(stg, row16, kg, j, acc[i >> 2][j >> 1][i & 3][j & 1]);
         };
 #pragma unroll 1
         for (int i = 0; i < 8; ++i) {
@@ -246,32 +236,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
                 case 6: put(6); break;
                 default: put(7); break;
             }
-            // the reads take what other lanes of this wave just wrote (LDS operations of one wave run in order)
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 1
-            for (int h = 0; h < 16 * kPer / kWave; ++h) {
-                const int r = h * (kWave / kPer) + ln / kPer, c = ln % kPer;
-                const int row = t.m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16 + r, col = t.n0 + wn * kCols + c * 8;
-                f32x4 z[2], u[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    z[e] = get(r, 2 * c + e);
-                    u[e] = SWIGLU ? get(r, 8 + 2 * c + e) : z[e];
-                }
-                if (row >= g.m || col >= g.n) continue;
-                if (lines) {
-                    const uint2 a = pack4<T>(finish4<T, SWIGLU>(g, row, col, 4, true, z[0], u[0]));
-                    const uint2 b = pack4<T>(finish4<T, SWIGLU>(g, row, col + 4, 4, true, z[1], u[1]));
-                    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.n + col) =
-                        u32x4{a.x, a.y, b.x, b.y};
-                } else {
-                    store4<T, SWIGLU>(g, row, col, z[0], u[0], vec);
-                    store4<T, SWIGLU>(g, row, col + 4, z[1], u[1], vec);
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // read before the next block's writes
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            store_block<T, SWIGLU, 4>(g, stg, ln, t.m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16,
+                                      t.n0 + wn * (SWIGLU ? 32 : 64), vec, lines);
         }
     };
 
