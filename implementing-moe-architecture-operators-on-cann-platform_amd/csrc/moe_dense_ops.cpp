@@ -81,45 +81,66 @@ moe_status check_pitch(const char* op, const char* what, int64_t rows, int64_t w
 
 // How one product runs: weight streaming, tiles of 32 to 256 x 128 (split over k or not), or 256 x 256 tiles
 enum class Kernel { kStream, kMid, kTiled };
+constexpr double kLaunchSaved = 6.0;  // us of a second launch's start and of the CUs its first round leaves idle
+
 struct ProductPlan {
     Kernel kernel;
     int bm;  // kMid: rows of a tile
     int splits;
     int64_t split_k;
     size_t partial_bytes;
+    double us;  // expected, of kMid and kTiled
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Microseconds of a launch by tiles of bm x 128 with `items` workgroups of `stages` 64-k stages. Up to 128 rows two
-// workgroups share a CU: a stage takes 0.3, 0.38 or 0.78 us (32, 64, 128 rows) alone and 0.65, 0.78 or 1.19 us beside
-// another. At 256 rows a CU has one: 0.87 us with few of them, 1.13 with one on every CU.
-double mid_time(int bm, int64_t items, int64_t stages) {
-    const double one = bm == 32 ? 0.30 : bm == 64 ? 0.38 : bm == 128 ? 0.78 : 0.87;
-    const double two = bm == 32 ? 0.65 : bm == 64 ? 0.78 : bm == 128 ? 1.19 : 1.13;
+// workgroups share a CU: a stage takes `one` alone and `two` beside another. At 256 rows a CU has one: `one` with few of them,
+// `two` with one on every CU. A launch takes `launch` besides, and each further round of the GPU `round` for its first
+// copies and its epilogue. Where P is read by k too, both operands go through transposing reads.
+double mid_time(int bm, int64_t items, int64_t stages, bool p_by_k) {
+    struct Cost {
+        double one, two, launch, round;
+    };
+    const Cost c = p_by_k      ? (bm == 128 ? Cost{0.70, 0.93, 5.6, 8.8} : Cost{0.89, 0.96, 7.1, 8.4})
+                   : bm == 32  ? Cost{0.30, 0.55, 5.5, 3.0}
+                   : bm == 64  ? Cost{0.37, 0.65, 5.5, 3.5}
+                   : bm == 128 ? Cost{0.56, 0.92, 7.2, 6.0}
+                               : Cost{0.75, 0.93, 9.1, 5.6};
     const int64_t slots = bm == 256 ? 256 : 512, rest = items % slots;
     const double tail = rest == 0 ? 0.0
-                        : bm == 256 ? one + (two - one) * (rest / 256.0)
-                                    : rest <= 256 ? one : one + (two - one) * (rest / 256.0 - 1.0);
-    return 4.3 + stages * (static_cast<double>(items / slots) * two + tail);
+                        : bm == 256 ? c.one + (c.two - c.one) * (rest / 256.0)
+                                    : rest <= 256 ? c.one : c.one + (c.two - c.one) * (rest / 256.0 - 1.0);
+    return c.launch + c.round * static_cast<double>(ceil_div(items, slots) - 1) +
+           stages * (static_cast<double>(items / slots) * c.two + tail);
 }
-// The same of 256 x 256 tiles: one workgroup a CU, 1.0 us a stage with few tiles up to 1.4 with one on every CU, 3.9 us of
-// epilogue a round.
-double tiled_time(int64_t tiles, int64_t stages) {
-    const int64_t rest = tiles % 256;
-    const double tail = rest == 0 ? 0.0 : 3.9 + stages * (1.01 + 0.4 * (rest / 256.0));
-    return 5.9 + static_cast<double>(tiles / 256) * (3.9 + 1.41 * stages) + tail;
+// The same of 256 x 256 tiles: one workgroup a CU, 1.0 us a stage with few tiles up to 1.46 with one on every CU (the clock
+// falls), 7 to 10 us of first copies and epilogue a round.
+double tiled_time(int64_t tiles, int64_t stages, bool p_by_k) {
+    const double launch = p_by_k ? 7.1 : 5.8, round = p_by_k ? 9.4 : 10.2, stage = p_by_k ? 1.59 : 1.46;
+    const double few_round = p_by_k ? 7.4 : 6.7, few_stage = p_by_k ? 1.2 : 1.01, more = p_by_k ? 0.43 : 0.41;
+    const double f = (tiles % 256) / 256.0;
+    const double tail =
+        tiles % 256 == 0 ? 0.0 : few_round + (round - few_round) * f + stages * (few_stage + more * f * f);
+    return launch + static_cast<double>(tiles / 256) * (round + stage * stages) + tail;
+}
+// Microseconds of adding a split product's pieces in a launch of its own, their writes counted
+double reduce_time(size_t partial, bool p_by_k) {
+    return (p_by_k ? 1.7 : 0.1) + 2.0 * static_cast<double>(partial) / (p_by_k ? 6.2e6 : 5.2e6);
 }
 
-// The kernel with the least time by those figures, which are fitted to every kernel's times at 87 sizes (T = 128 ..
-// 16384, N = 64 .. 16384, H = 512 .. 7168): the choice was the fastest there or within 6 %, 0.2 % on average.
+// The kernel with the least time by those figures, which are fitted to every kernel's times in 306 products (T = 128 ..
+// 16384, N and H = 64 .. 12288, in the forward's two layouts and the weight gradient's): the choice is the fastest of them or
+// 0.3 % slower on average, 16 % at worst (T = 16384, N = 256, H = 7168, where all are within that).
 // A product by tiles is split over k while that leaves eight stages a piece and at most the workgroups that the GPU
 // holds; the pieces' sums then take another launch.
 // Few rows stream the weights where both operands are read by rows: T = 16, H = 2048, N = 7168 8.2 us (tiles of 32 rows
 // 11.5), T = 64 11.6 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N = 256
 // 12.4 us (8.3 split over k), T = 64, H = 4096, N = 16384 35 us (33).
-ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct) {
-    ProductPlan best{Kernel::kMid, 128, 1, ceil_div(k > 0 ? k : 1, 64) * 64, 0};
+// most_rows: the tallest tiles to choose from.
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct,
+                         int most_rows = 256) {
+    ProductPlan best{Kernel::kMid, 128, 1, ceil_div(k > 0 ? k : 1, 64) * 64, 0, 1e30};
     const int64_t stages = ceil_div(k > 0 ? k : 1, 64);
     if (direct && !p_by_k && !q_by_k && m <= 64) {
         const int64_t tiles = ceil_div(n, swiglu ? 8 : 16);
@@ -128,10 +149,9 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by
             return best;
         }
     }
-    double least = 1e30;
     for (const int bm : {32, 64, 128, 256}) {
         if (bm == 32 ? m > 32 : bm == 64 ? m <= 32 : bm == 128 ? !p_by_k && m <= 64 : !direct || m <= 128) continue;
-        if (bm < 128 && p_by_k) continue;
+        if ((bm < 128 && p_by_k) || bm > most_rows) continue;
         const int64_t tiles = ceil_div(m, bm) * ceil_div(n, swiglu ? 64 : 128);
         int64_t splits = tiles > 0 ? (bm == 256 ? 256 : 512) / tiles : 1;
         if (splits > stages / 8) splits = stages / 8;
@@ -140,25 +160,26 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by
         splits = ceil_div(stages, per);
         const size_t partial =
             splits > 1 ? static_cast<size_t>(splits) * m * moe::part_ld(static_cast<int>(n), swiglu) * 4 : 0;
-        const double t = mid_time(bm, tiles * splits, per) + (splits > 1 ? 2.3 + 2.0 * partial / 7e6 : 0.0);
-        if (t < least) {
-            least = t;
-            best = ProductPlan{Kernel::kMid, bm, static_cast<int>(splits), per * 64, partial};
-        }
+        const double t = mid_time(bm, tiles * splits, per, p_by_k) + (splits > 1 ? reduce_time(partial, p_by_k) : 0.0);
+        if (t < best.us) best = ProductPlan{Kernel::kMid, bm, static_cast<int>(splits), per * 64, partial, t};
     }
     const int64_t tiles = ceil_div(m, 256) * ceil_div(n, swiglu ? 128 : 256);
-    if (direct && m > 64 && tiled_time(tiles, stages) < least)
-        best = ProductPlan{Kernel::kTiled, 256, 1, stages * 64, 0};
+    const double t = tiled_time(tiles, stages, p_by_k);
+    if (direct && m > 64 && most_rows >= 256 && t < best.us) best = ProductPlan{Kernel::kTiled, 256, 1, stages * 64, 0, t};
     return best;
 }
 
-// The most that a product's partial sums take, whatever its operands' layout and alignment
-size_t most_partial(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k) {
+// The most that a product's partial sums take, whatever its operands' layout and alignment (Q by k: the plan without
+// streaming, which needs none). pair: also where it shares a launch with another.
+size_t most_partial(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool pair) {
     size_t most = 0;
-    for (int v = 0; v < 4; ++v) {
-        const size_t b = plan_product(m, n, k, swiglu, p_by_k, p_by_k || (v & 1), (v & 2) != 0).partial_bytes;
+    auto take = [&](bool direct, int rows) {
+        const size_t b = plan_product(m, n, k, swiglu, p_by_k, true, direct, rows).partial_bytes;
         if (b > most) most = b;
-    }
+    };
+    take(false, 256);
+    take(true, 256);
+    if (pair) take(true, 128);
     return most;
 }
 
@@ -218,8 +239,8 @@ moe::Repack repack(const void* src, int64_t ld, int64_t rows, int64_t cols, void
 size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
     const bool swiglu = act == MOE_ACT_SWIGLU;
     const RepackRoom room = repack_room(T, N, H, swiglu);
-    const size_t padded = H % 8 != 0 ? most_partial(T, N, round_up(H, 8), swiglu, false) : 0;
-    const size_t partial = most_partial(T, N, H, swiglu, false);
+    const size_t padded = H % 8 != 0 ? most_partial(T, N, round_up(H, 8), swiglu, false, false) : 0;
+    const size_t partial = most_partial(T, N, H, swiglu, false, false);
     return room.x + room.w + (partial > padded ? partial : padded);
 }
 
@@ -238,8 +259,9 @@ GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
     const RepackRoom room = repack_room(T, g.Z, H, false);
     g.w_at = g.x_at + room.x;
     g.partial_at = g.w_at + room.w;
-    const size_t x0 = most_partial(T, H, g.Z, false, false), x8 = most_partial(T, H, g.ldz, false, false);
-    const size_t x = x0 > x8 ? x0 : x8, w = most_partial(g.Z, H, T, false, true);
+    const size_t x0 = most_partial(T, H, g.Z, false, false, true);
+    const size_t x8 = g.ldz != g.Z ? most_partial(T, H, g.ldz, false, false, true) : 0;
+    const size_t x = x0 > x8 ? x0 : x8, w = most_partial(g.Z, H, T, false, true, true);
     g.bytes = g.partial_at + round_up(static_cast<int64_t>(x), 256) + w;  // both, for products of one launch
     return g;
 }
@@ -501,9 +523,12 @@ moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void
     if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
     void* partial = base + ws.partial_at;
     if (want_x && grad_weight && direct_product(gx, false, by_k, need_dz) && direct_product(gw, true, true, false)) {
-        const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true);
-        const ProductPlan pw = plan_product(gw.m, gw.n, gw.k, false, true, true, true);
-        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid && px.bm <= 128 && pw.bm <= 128) {
+        // one launch for both by tiles of at most 128 rows, where that costs less than the launch it saves
+        const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true, 128);
+        const ProductPlan pw = plan_product(gw.m, gw.n, gw.k, false, true, true, true, 128);
+        const double apart = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true).us +
+                             plan_product(gw.m, gw.n, gw.k, false, true, true, true).us;
+        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid && px.us + pw.us < apart + kLaunchSaved) {
             set_split(gx, px, partial);
             set_split(gw, pw, static_cast<char*>(partial) + round_up(static_cast<int64_t>(px.partial_bytes), 256));
             err = moe::launch_gemm_pair(gx, gw, by_k, bf16, px.bm, s);

@@ -192,21 +192,23 @@ __device__ __forceinline__ bool whole_lines(const GemmArgs& g, bool vec) {
 // what the epilogue reads and writes is whole lines. Granule G (16 bytes) of row r stands at G ^ r.
 template <int NB>
 __device__ __forceinline__ void put_block(float* stg, int row16, int kg, int j, f32x4 v) {
-    *reinterpret_cast<f32x4*>(stg + (row16 * NB * 4 + ((j * 4 + kg) ^ (row16 % (NB * 4)))) * 4) = v;
+    *reinterpret_cast<f32x4*>(stg + (row16 * NB * 4 + ((j * 4 + kg) ^ (NB == 4 ? row16 : row16 % (NB * 4)))) * 4) = v;
 }
 template <typename T, bool SWIGLU, int NB>
 __device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg, int lane, int row0, int col0, bool vec,
                                             bool lines) {
     constexpr int kGranules = NB * 4, kPer = (SWIGLU ? NB / 2 : NB) * 2;  // lanes of a row
     auto get = [&](int r, int gr) __attribute__((always_inline)) {
-        return *reinterpret_cast<const f32x4*>(stg + (r * kGranules + (gr ^ (r % kGranules))) * 4);
+        return *reinterpret_cast<const f32x4*>(stg + (r * kGranules + (gr ^ (NB == 4 ? r : r % kGranules))) * 4);
     };
     // the reads take what other lanes of this wave just wrote (LDS operations of one wave run in order)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll 1
-    for (int at = lane; at < 16 * kPer; at += kWave) {
-        const int r = at / kPer, c = at % kPer, row = row0 + r, col = col0 + c * 8;
+    for (int h = 0; h < (16 * kPer + kWave - 1) / kWave; ++h) {
+        const int r = h * (kWave / kPer) + lane / kPer, c = lane % kPer;
+        if (16 * kPer < kWave && r >= 16) continue;
+        const int row = row0 + r, col = col0 + c * 8;
         f32x4 z[2], u[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
