@@ -14,10 +14,10 @@
 // never in the instruction cache when it is needed, cost 9 us.
 //
 // A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers; few
-// tokens of many experts have a wave each. A pick is the maximum over the lane (max3) and over the row (4 DPP steps), and its removal: 16 compares and 16 selects.
-// Where the key's low 8 bits can hold the expert, the maximum names the pick: ~50 instructions for 4 tokens. fp32 logits
-// without a bias need all of their bits: the lowest index that has the maximum is searched, ~95 instructions. Group scores
-// go through LDS, one lane per (token, group). Vector instructions bound the kernel (T = 16384, E = 256, K = 8, fp32
+// tokens of many experts have a wave each. A pick is the maximum over the lane (max3) and over the row (4 DPP steps), and
+// its removal: 16 compares and 16 selects. Where the key's low 8 bits can hold the expert, the maximum names the pick: ~50
+// instructions for 4 tokens. fp32 logits without a bias need all of their bits: the lowest index that has the maximum is
+// searched, ~95 instructions. Group scores go through LDS, one lane per (token, group). Vector instructions bound the kernel (T = 16384, E = 256, K = 8, fp32
 // logits: 10.3 us without bias and groups, 17 us with a bias and 4 of 8 groups by their two best, of which a copy of the
 // logits is 4 us; the search in place of the key's bits 21 us). At T = 1 the one wave's chain takes 5.8 us.
 #include "moe_device.h"

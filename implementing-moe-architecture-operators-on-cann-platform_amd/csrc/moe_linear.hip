@@ -7,10 +7,10 @@
 //   grad_W     P = dz (by k: its T rows are the reduction), Q = x (by k)
 // The tiles here, 32 to 256 rows by 128, are for products that do not fill the GPU with 256 x 256 ones; where even these
 // leave CUs idle the product is split over k and a second launch adds the pieces in order. What bounds them is the copies
-// into LDS: 24 KB a stage and two workgroups a CU, 0.78 us for both (64 rows), is 16 TB/s over the GPU, and 128 and 256
-// rows come to 14 and 11 TB/s. So the taller tile wins until the pieces' sums cost more than its reads save.
-//   T = 4097, H = 7168, N = 256 (130 tiles of 64 rows in 3 pieces): 24.6 + 4.3 us, of which x from HBM alone is 11
-//   both gradients' products at T = 1000, H = 1056, N = 733, one launch of 256 workgroups: 12.2 + 3.4 us
+// into LDS: 24 KB a stage and two workgroups a CU, 0.65 us for both (64 rows), is 19 TB/s over the GPU, and 128 and 256
+// rows come to 18 and 13 TB/s. So the taller tile wins until the pieces' sums cost more than its reads save.
+//   T = 4097, H = 7168, N = 256 (130 tiles of 64 rows in 3 pieces): 25.6 + 4.2 us, of which x from HBM alone is 11
+//   both gradients' products at T = 1000, H = 1056, N = 733, one launch of 256 workgroups: 10.9 + 3.2 us
 #include "moe_gemm.h"
 
 namespace moe {

@@ -9,7 +9,7 @@
 // of an XCD then read 8 + 4 panels a stage, not 32 + 1), and the epilogue of moe_gemm.h.
 //
 // Matrix cores and the clock they leave bound it. T = 16381, H = 2048, N = 2816 SwiGLU bf16: 282-293 us with the epilogue,
-// 1290-1340 TFLOP/s (8192^3 by the library on the same box: 1413); grad_x of a T = 8192 step 148 us, 1277 TFLOP/s. grad_weight
+// 1290-1340 TFLOP/s (8192^3 by the library: 1413); grad_x of a T = 8192 step 148 us, 1277 TFLOP/s. grad_weight
 // there has 176 tiles for 256 CUs and takes 200 us: tiles of 256 x 192 (242 of them) took 170 us where these took 177, and
 // 168 to 199 us where these took 137 to 142 on full rounds, so a product is not bound by the CUs it leaves idle.
 #include "moe_gemm.h"
