@@ -80,6 +80,37 @@ def test_routing_of_many_rows_is_that_of_few(ops, E, G, TG, GT, scoring, renorm)
             assert torch.equal(ids[at], pids) and torch.equal(w[at], pw)
 
 
+@pytest.mark.parametrize("T", [3, 2500])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_equal_scores_go_to_the_lowest_index(ops, T, scoring):
+    """All 256 candidates equal, with a bias: the choice goes on to a clear gap, which is the row's end."""
+    E = 256
+    logits, bias = torch.full((T, E), -1.5, device="cuda"), torch.full((E,), 0.25, device="cuda")
+    logits[1] = torch.finfo(F32).min
+    logits[2, ::2] = float("-inf")
+    want = torch.arange(8, device="cuda", dtype=torch.int32)
+    for G, TG in ((1, 1), (8, 4)):
+        ids, w = ops.MoeRoutingGroupTopK(logits, bias, 8, G, TG, 2, scoring, True, 1.0, F32)
+        assert torch.equal(ids[0], want) and torch.equal(ids[1], want) and torch.equal(ids[2], 2 * want + 1)
+        assert torch.equal(w, torch.full_like(w, 0.125))
+        assert T == 3 or torch.equal(ids[3:], want.expand(T - 3, 8))
+
+
+@pytest.mark.parametrize("T,N,H,act", [(1, 72, 256, 0), (64, 4096, 136, 0), (40, 64, 4096, 0), (300, 200, 1024, 5),
+                                       (2304, 2304, 128, 0)])
+def test_residual_may_be_the_result(ops, T, N, H, act):
+    lib = ops._lib.load()
+    x, w = ones((T, H), 1), ones(((2 if act else 1) * N, H), 2)
+    y = ones((T, N), 3)
+    want = ops.MoeLinear(x, w, residual=y, activation="swiglu" if act else "none")
+    need = ops.linear_workspace_bytes(T, N, H, "swiglu" if act else "none")
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    st = lib.moe_linear(x.data_ptr(), H, w.data_ptr(), H, 0, None, y.data_ptr(), y.data_ptr(), None, ws.data_ptr(), need, T,
+                        N, H, act, 1, 1, torch.cuda.current_stream().cuda_stream)
+    assert st == 0, lib.moe_last_error()
+    assert torch.equal(y, want)
+
+
 def test_combine_gradient_past_32_bits(ops):
     T, H, K = 140001, 2048, 8  # 2.3e9 elements
     eo, dy = ones((T, K, H), 4), ones((T, H), 5)
