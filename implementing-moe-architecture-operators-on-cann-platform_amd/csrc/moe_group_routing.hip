@@ -7,8 +7,8 @@
 // An expert whose logit or c is NaN or -inf is not available; picks with no expert left are id -1, weight 0.
 //
 // The choice is the definition's, not fp32's: without a bias experts are compared by their logits, which order the scores
-// exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where the last group that stays and the
-// first that does not are nearer than that, the row's groups are scored again in float64; where two neighbours among
+// exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where a group that stays and one that
+// does not are nearer than theirs (group_error), the row's groups are scored again in float64; where two neighbours among
 // its picks are, the picks go on past the K-th until a clear gap and are put in order by their float64 values. That is
 // some rows in a hundred, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
 // never in the instruction cache when it is needed, cost 9 us.
@@ -132,12 +132,18 @@ __device__ __forceinline__ int key_of(float v) {
 }
 __device__ __forceinline__ float key_value(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
 
-// Two fp32 values of c (or sums of two) that are nearer than this may stand the other way round. With e = 2^-24: exp2 and
+// Two fp32 values of c that are nearer than this may stand the other way round. With e = 2^-24: exp2 and
 // rcp are within 2 e, the argument's rounding moves e^-l by |l| 1.5 e relative and s (1 - s) |l| < 0.23, so a sigmoid is
-// within 8 e; a softmax score, with a sum of 20 roundings, within 64 e of the row's largest score; adding the bias, or two
-// c, rounds by e |c|. The limit is four such errors.
+// within 8 e; a softmax score, with a sum of 20 roundings, within 64 e of the row's largest score; adding the bias
+// rounds by e |c|. The limit is four such errors.
 __device__ __forceinline__ float gap_limit(bool sigmoid, float s_max, float c) {
     return (sigmoid ? 32.0f : 256.0f * s_max) * 0x1p-24f + fabsf(c) * 0x1p-21f;
+}
+// How far an fp32 group score may be from the definition's. It is the sum of two c, a and b, which may cancel: its error is
+// that of the terms, two scores' and, with the sum's own rounding, at most 2 e (|a| + |b|), not one of the sum's size
+// (biases of +-40 leave sums below 1 that are 4e-6 off). size: |a| + |b|, counted twice.
+__device__ __forceinline__ float group_error(bool sigmoid, float s_max, float size) {
+    return (sigmoid ? 16.0f : 128.0f * s_max) * 0x1p-24f + size * 0x1p-22f;
 }
 
 // LDS of the one wave of a workgroup. A row may have E picks.
@@ -149,9 +155,9 @@ struct RoutingLds {
     __host__ __device__ int order_at() const { return picks_at() + 2 * TOKENS * E; }
     __host__ __device__ int scores_at() const { return (order_at() + 2 * E + 3) / 4 * 4; }
     __host__ __device__ int kept_at() const { return scores_at() + 4 * TOKENS * G; }
-    __host__ __device__ int cut_at() const { return kept_at() + 4 * TOKENS * G; }
+    __host__ __device__ int sizes_at() const { return kept_at() + 4 * TOKENS * G; }
     // c of the rows' experts, fp32; or, once the groups are scored, float64 values of one row and its groups
-    __host__ __device__ int row_at() const { return (cut_at() + 8 * TOKENS + 15) / 16 * 16; }
+    __host__ __device__ int row_at() const { return (sizes_at() + 4 * TOKENS * G + 15) / 16 * 16; }
     __host__ __device__ int bytes(bool rows) const {
         const int scores = 4 * TOKENS * pitch(), exact = 8 * (E + G);
         return row_at() + (rows ? (scores > exact ? scores : exact) : 0);
@@ -239,7 +245,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
     uint16_t* order = reinterpret_cast<uint16_t*>(shared + lay.order_at());
     float* gs = reinterpret_cast<float*>(shared + lay.scores_at());
     int* kept = reinterpret_cast<int*>(shared + lay.kept_at());
-    float* cut = reinterpret_cast<float*>(shared + lay.cut_at());  // [token][2]: last score that stays, first that does not
+    float* sizes = reinterpret_cast<float*>(shared + lay.sizes_at());  // of the groups' terms, for group_error
     float* row = reinterpret_cast<float*>(shared + lay.row_at());
     double* cs = reinterpret_cast<double*>(row);
     double* cgs = cs + E;
@@ -338,7 +344,9 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
 #pragma unroll 4
                 for (int n = 0; n < size; ++n) take(c[n]);
             }
-            gs[i] = r.group_top == 2 && b > kLow ? a + b : a;
+            const bool two = r.group_top == 2 && b > kLow;
+            gs[i] = two ? a + b : a;
+            sizes[i] = a == -kLow ? 0.0f : fabsf(a) + (two ? fabsf(b) : 0.0f);  // an infinite bias decides by itself
         }
         __syncthreads();
         for (int i = lane; i < kTokens * G; i += kWave) {
@@ -349,13 +357,22 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
 #pragma unroll 8
             for (int n = 0; n < G; ++n) before += o[n] > x || (o[n] == x && n < g);
             kept[i] = before < r.top_groups;
-            if (before == r.top_groups - 1) cut[2 * q] = x;
-            if (before == r.top_groups) cut[2 * q + 1] = x;
         }
         __syncthreads();
         if (scored) {
-            const float x = cut[2 * tok], y = cut[2 * tok + 1];
-            uint64_t open = __ballot(valid && y > kLow && !(x - y > gap_limit(r.sigmoid, s_max, x)));
+            // the least that a group that stays may be, the most that one that does not may be; empty groups are exact
+            int least = 2147483647, most = kGone;
+#pragma unroll 1
+            for (int g = l; g < G; g += LANES) {
+                const float x = gs[tok * G + g], err = group_error(r.sigmoid, s_max, sizes[tok * G + g]);
+                if (!(x > kLow)) continue;
+                const float low = x - err;
+                if (!kept[tok * G + g]) most = max(most, key_of(x + err));
+                else least = min(least, key_of(low > kLow ? low : kLow));  // NaN, where x and err are infinite
+            }
+            least = row_min_i<LANES>(least);
+            most = row_max_i<LANES>(most);
+            uint64_t open = __ballot(valid && most != kGone && least <= most);
 #pragma unroll 1
             for (int q = 0; open && q < kTokens; ++q) {
                 if (!((open >> (q * LANES)) & 1)) continue;
