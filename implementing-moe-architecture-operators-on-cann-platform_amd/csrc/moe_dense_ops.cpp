@@ -211,16 +211,21 @@ hipError_t run_product(moe::GemmArgs g, void* partial, bool p_by_k, bool q_by_k,
     return err == hipSuccess && plan.splits > 1 ? moe::launch_gemm_reduce(g, bf16, stream) : err;
 }
 
+// The weight's layout that a workspace is for
+enum class Layout { kRows, kTransposed, kEither };
+Layout layout_of(int32_t weight_transposed) { return weight_transposed ? Layout::kTransposed : Layout::kRows; }
+
 // Room for x and the weight with padded rows (moe_linear_repack.hip), where the sizes alone make them necessary: x and a
 // weight [Z, H] where H is no multiple of 8, a transposed weight [H, Z] where Z (a SwiGLU's N) is none.
 struct RepackRoom {
     size_t x, w;
 };
-RepackRoom repack_room(int64_t T, int64_t N, int64_t H, bool swiglu) {
+RepackRoom repack_room(int64_t T, int64_t N, int64_t H, bool swiglu, Layout layout) {
     const int64_t h8 = round_up(H, 8), n8 = round_up(N, 8), halves = swiglu ? 2 : 1;
     RepackRoom r{};
     if (H % 8 != 0) r.x = round_up(T * h8 * 2, 256);
-    const int64_t rows = H % 8 != 0 ? halves * N * h8 * 2 : 0, cols = N % 8 != 0 ? H * halves * n8 * 2 : 0;
+    const int64_t rows = layout != Layout::kTransposed && H % 8 != 0 ? halves * N * h8 * 2 : 0;
+    const int64_t cols = layout != Layout::kRows && N % 8 != 0 ? H * halves * n8 * 2 : 0;
     r.w = round_up(rows > cols ? rows : cols, 256);
     return r;
 }
@@ -236,9 +241,9 @@ moe::Repack repack(const void* src, int64_t ld, int64_t rows, int64_t cols, void
     return r;
 }
 
-size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
+size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layout layout) {
     const bool swiglu = act == MOE_ACT_SWIGLU;
-    const RepackRoom room = repack_room(T, N, H, swiglu);
+    const RepackRoom room = repack_room(T, N, H, swiglu, layout);
     const size_t padded = H % 8 != 0 ? most_partial(T, N, round_up(H, 8), swiglu, false, false) : 0;
     const size_t partial = most_partial(T, N, H, swiglu, false, false);
     return room.x + room.w + (partial > padded ? partial : padded);
@@ -250,13 +255,13 @@ struct GradWorkspace {
     int64_t Z, ldz;
     size_t sums_at, x_at, w_at, partial_at, bytes;
 };
-GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
+GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layout layout) {
     GradWorkspace g{};
     g.Z = act == MOE_ACT_SWIGLU ? 2 * N : N;
     g.ldz = round_up(g.Z, 8);
     g.sums_at = round_up(T * g.ldz * 2, 256);
     g.x_at = g.sums_at + round_up(static_cast<int64_t>(moe::act_grad_row_blocks(T, static_cast<int>(g.Z))) * g.Z * 4, 256);
-    const RepackRoom room = repack_room(T, g.Z, H, false);
+    const RepackRoom room = repack_room(T, g.Z, H, false, layout);
     g.w_at = g.x_at + room.x;
     g.partial_at = g.w_at + room.w;
     const size_t x0 = most_partial(T, H, g.Z, false, false, true);
@@ -266,6 +271,179 @@ GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act) {
     return g;
 }
 
+// moe_linear; the workspace has to have what `workspace_for` needs
+moe_status linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int32_t weight_transposed,
+                  const void* bias, const void* residual, void* y, void* pre, void* workspace, size_t workspace_bytes,
+                  int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, int32_t out_dtype, void* stream,
+                  Layout workspace_for) {
+    const char* op = "MoeLinear";
+    moe_status st = check_linear(op, T, N, H, activation, dtype);
+    if (st != MOE_OK) return st;
+    if (out_dtype != dtype && out_dtype != MOE_DT_FLOAT32)
+        return fail(MOE_ERR_ARG, "%s: result type %d (the operands' or float32 expected)", op, out_dtype);
+    const int64_t Z = activation == MOE_ACT_SWIGLU ? 2 * N : N;
+    st = check_pitch(op, "x", T, H, x_stride);
+    if (st != MOE_OK) return st;
+    st = weight_transposed ? check_pitch(op, "weight", H, Z, weight_stride) : check_pitch(op, "weight", Z, H, weight_stride);
+    if (st != MOE_OK) return st;
+    if (T == 0) return ok();
+    if (!x || !weight || !y) return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    const size_t need = linear_workspace(T, N, H, activation, workspace_for);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace, need);
+    if (need > 0 && !aligned16(workspace))
+        return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
+    moe::GemmArgs g{};
+    g.p = static_cast<const uint16_t*>(x);
+    g.q = static_cast<const uint16_t*>(weight);
+    g.ldp = x_stride;
+    g.ldq = weight_stride;
+    g.m = static_cast<int>(T);
+    g.n = static_cast<int>(N);
+    g.k = static_cast<int>(H);
+    g.out = y;
+    g.pre = static_cast<uint16_t*>(pre);
+    g.bias = static_cast<const uint16_t*>(bias);
+    g.residual = residual;
+    g.act = activation;
+    g.out_f32 = out_dtype == MOE_DT_FLOAT32;
+    g.up = g.n;
+    hipError_t err = moe::prepare_linear();
+    if (err != hipSuccess) return hip_fail(err, "MoeLinear kernel attributes");
+    // rows off 16 bytes by their length: padded copies first
+    const bool swiglu = activation == MOE_ACT_SWIGLU, transposed = weight_transposed != 0;
+    const RepackRoom room = repack_room(T, N, H, swiglu, layout_of(weight_transposed));
+    char* base = static_cast<char*>(workspace);
+    moe::RepackArgs pack{};
+    const int64_t h8 = round_up(H, 8), n8 = round_up(N, 8);
+    bool padded = false;
+    if (H % 8 != 0) {
+        pack.m[0] = repack(x, x_stride, T, H, base, h8);
+        g.p = pack.m[0].dst;
+        g.ldp = h8;
+        padded = true;
+    }
+    if (!transposed && H % 8 != 0) {
+        pack.m[1] = repack(weight, weight_stride, Z, H, base + room.x, h8);
+        g.q = pack.m[1].dst;
+        g.ldq = h8;
+        g.k = static_cast<int>(h8);  // zeros in both
+    } else if (transposed && N % 8 != 0) {
+        g.q = reinterpret_cast<uint16_t*>(base + room.x);
+        g.ldq = swiglu ? 2 * n8 : n8;
+        g.up = static_cast<int>(n8);
+        pack.m[1] = repack(weight, weight_stride, H, N, base + room.x, g.ldq);
+        if (swiglu)
+            pack.m[2] = repack(static_cast<const uint16_t*>(weight) + N, weight_stride, H, N, pack.m[1].dst + n8, g.ldq);
+    }
+    err = moe::launch_repack(pack, as_stream(stream));
+    if (err == hipSuccess)
+        err = run_product(g, base + room.x + room.w, false, transposed, dtype == MOE_DT_BFLOAT16, as_stream(stream), padded);
+    if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
+    return ok();
+}
+// moe_linear_grad likewise
+moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride, const void* weight,
+                       int64_t weight_stride, int32_t weight_transposed, const void* pre, void* grad_x, void* grad_weight,
+                       void* grad_bias, void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H,
+                       int32_t activation, int32_t dtype, void* stream, Layout workspace_for) {
+    const char* op = "MoeLinearGrad";
+    moe_status st = check_linear(op, T, N, H, activation, dtype);
+    if (st != MOE_OK) return st;
+    const Layout layout = layout_of(weight_transposed);
+    const GradWorkspace ws = grad_workspace(T, N, H, activation, layout);
+    const size_t need = workspace_for == layout ? ws.bytes : grad_workspace(T, N, H, activation, workspace_for).bytes;
+    st = check_pitch(op, "grad_y", T, N, grad_y_stride);
+    if (st != MOE_OK) return st;
+    if (grad_weight) st = check_pitch(op, "x", T, H, x_stride);
+    if (st != MOE_OK) return st;
+    if (grad_x)
+        st = weight_transposed ? check_pitch(op, "weight", H, ws.Z, weight_stride)
+                               : check_pitch(op, "weight", ws.Z, H, weight_stride);
+    if (st != MOE_OK) return st;
+    if (!grad_x && !grad_weight && !grad_bias) return ok();
+    const bool act = activation != MOE_ACT_NONE;
+    if (T > 0 && (!grad_y || (act && !pre) || (grad_weight && !x) || (grad_x && !weight)))
+        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    if (T == 0 && !grad_weight && !grad_bias) return ok();
+    if (!workspace || workspace_bytes < need)
+        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace, need);
+    if (!aligned16(workspace)) return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
+    const hipStream_t s = as_stream(stream);
+    const bool bf16 = dtype == MOE_DT_BFLOAT16;
+    char* base = static_cast<char*>(workspace);
+    // without an activation dz is grad_y itself, where the products can read that in 16-byte copies
+    const bool as_is = !act && N % 8 == 0 && direct_operand(grad_y, grad_y_stride);
+    const bool need_dz = !as_is && (grad_x || grad_weight) && T > 0;
+    const uint16_t* dz = as_is ? static_cast<const uint16_t*>(grad_y) : reinterpret_cast<uint16_t*>(base);
+    const int64_t ldz = as_is ? grad_y_stride : ws.ldz;
+    hipError_t err = moe::prepare_linear();
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad kernel attributes");
+    float* sums = reinterpret_cast<float*>(base + ws.sums_at);
+    if (need_dz || grad_bias)
+        err = moe::launch_act_grad(static_cast<const uint16_t*>(grad_y), grad_y_stride,
+                                   act ? static_cast<const uint16_t*>(pre) : nullptr,
+                                   need_dz ? reinterpret_cast<uint16_t*>(base) : nullptr, ws.ldz,
+                                   grad_bias ? sums : nullptr, T, static_cast<int>(N), activation, bf16, s);
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad activation launch");
+    moe::GradTail tail{};
+    moe::GemmArgs &gx = tail.x, &gw = tail.w;
+    gx.p = gw.p = dz;
+    gx.ldp = gw.ldp = ldz;
+    gx.q = static_cast<const uint16_t*>(weight);
+    gx.ldq = weight_stride;
+    gx.m = gw.k = static_cast<int>(T);
+    gx.n = gw.n = static_cast<int>(H);
+    gx.k = gw.m = static_cast<int>(ws.Z);
+    gx.out = grad_x;
+    gw.q = static_cast<const uint16_t*>(x);
+    gw.ldq = x_stride;
+    gw.out = grad_weight;
+    tail.sums = sums;
+    tail.bias_grad = static_cast<uint16_t*>(grad_bias);
+    tail.Z = static_cast<int>(ws.Z);
+    tail.sum_rows = moe::act_grad_row_blocks(T, tail.Z);
+    const bool want_x = grad_x && T > 0, by_k = weight_transposed == 0;
+    moe::RepackArgs pack{};
+    if (grad_weight && T > 0 && H % 8 != 0 && !direct_operand(x, x_stride)) {
+        pack.m[0] = repack(x, x_stride, T, H, base + ws.x_at, round_up(H, 8));
+        gw.q = pack.m[0].dst;
+        gw.ldq = round_up(H, 8);
+    }
+    if (want_x && (by_k ? H % 8 != 0 && !direct_operand(weight, weight_stride) : ws.Z % 8 != 0)) {
+        const int64_t cols = by_k ? H : ws.Z;
+        pack.m[1] = repack(weight, weight_stride, by_k ? ws.Z : H, cols, base + ws.w_at, round_up(cols, 8));
+        gx.q = pack.m[1].dst;
+        gx.ldq = round_up(cols, 8);
+        if (!by_k && need_dz) gx.k = static_cast<int>(ws.ldz);  // zeros in both
+    }
+    err = moe::launch_repack(pack, s);
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
+    void* partial = base + ws.partial_at;
+    if (want_x && grad_weight && direct_product(gx, false, by_k, need_dz) && direct_product(gw, true, true, false)) {
+        // one launch for both by tiles of at most 128 rows, where that costs less than the launch it saves
+        const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true, 128);
+        const ProductPlan pw = plan_product(gw.m, gw.n, gw.k, false, true, true, true, 128);
+        const double apart = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true).us +
+                             plan_product(gw.m, gw.n, gw.k, false, true, true, true).us;
+        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid && px.us + pw.us < apart + kLaunchSaved) {
+            set_split(gx, px, partial);
+            set_split(gw, pw, static_cast<char*>(partial) + round_up(static_cast<int64_t>(px.partial_bytes), 256));
+            err = moe::launch_gemm_pair(gx, gw, by_k, bf16, px.bm, s);
+            if (err == hipSuccess) err = moe::launch_grad_tail(tail, bf16, s);
+            if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
+            return ok();
+        }
+    }
+    if (want_x) err = run_product(gx, partial, false, by_k, bf16, s, need_dz);
+    if (err == hipSuccess && grad_weight) err = run_product(gw, partial, true, true, bf16, s);
+    if (err == hipSuccess && grad_bias) {
+        gx.splits = gw.splits = 1;
+        err = moe::launch_grad_tail(tail, bf16, s);
+    }
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
+    return ok();
+}
 }  // namespace
 
 extern "C" {
@@ -367,184 +545,57 @@ moe_status moe_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, 
 
 size_t moe_linear_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation) {
     if (check_linear("MoeLinear", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
-    return linear_workspace(T, N, H, activation);
+    return linear_workspace(T, N, H, activation, Layout::kEither);
 }
 
 moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                       int32_t weight_transposed, const void* bias, const void* residual, void* y, void* pre,
                       void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
                       int32_t dtype, int32_t out_dtype, void* stream) {
-    const char* op = "MoeLinear";
-    moe_status st = check_linear(op, T, N, H, activation, dtype);
-    if (st != MOE_OK) return st;
-    if (out_dtype != dtype && out_dtype != MOE_DT_FLOAT32)
-        return fail(MOE_ERR_ARG, "%s: result type %d (the operands' or float32 expected)", op, out_dtype);
-    const int64_t Z = activation == MOE_ACT_SWIGLU ? 2 * N : N;
-    st = check_pitch(op, "x", T, H, x_stride);
-    if (st != MOE_OK) return st;
-    st = weight_transposed ? check_pitch(op, "weight", H, Z, weight_stride) : check_pitch(op, "weight", Z, H, weight_stride);
-    if (st != MOE_OK) return st;
-    if (T == 0) return ok();
-    if (!x || !weight || !y) return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
-    const size_t need = linear_workspace(T, N, H, activation);
-    if (need > 0 && (!workspace || workspace_bytes < need))
-        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace, need);
-    if (need > 0 && !aligned16(workspace))
-        return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
-    moe::GemmArgs g{};
-    g.p = static_cast<const uint16_t*>(x);
-    g.q = static_cast<const uint16_t*>(weight);
-    g.ldp = x_stride;
-    g.ldq = weight_stride;
-    g.m = static_cast<int>(T);
-    g.n = static_cast<int>(N);
-    g.k = static_cast<int>(H);
-    g.out = y;
-    g.pre = static_cast<uint16_t*>(pre);
-    g.bias = static_cast<const uint16_t*>(bias);
-    g.residual = residual;
-    g.act = activation;
-    g.out_f32 = out_dtype == MOE_DT_FLOAT32;
-    g.up = g.n;
-    hipError_t err = moe::prepare_linear();
-    if (err != hipSuccess) return hip_fail(err, "MoeLinear kernel attributes");
-    // rows off 16 bytes by their length: padded copies first
-    const bool swiglu = activation == MOE_ACT_SWIGLU, transposed = weight_transposed != 0;
-    const RepackRoom room = repack_room(T, N, H, swiglu);
-    char* base = static_cast<char*>(workspace);
-    moe::RepackArgs pack{};
-    const int64_t h8 = round_up(H, 8), n8 = round_up(N, 8);
-    bool padded = false;
-    if (H % 8 != 0) {
-        pack.m[0] = repack(x, x_stride, T, H, base, h8);
-        g.p = pack.m[0].dst;
-        g.ldp = h8;
-        padded = true;
-    }
-    if (!transposed && H % 8 != 0) {
-        pack.m[1] = repack(weight, weight_stride, Z, H, base + room.x, h8);
-        g.q = pack.m[1].dst;
-        g.ldq = h8;
-        g.k = static_cast<int>(h8);  // zeros in both
-    } else if (transposed && N % 8 != 0) {
-        g.q = reinterpret_cast<uint16_t*>(base + room.x);
-        g.ldq = swiglu ? 2 * n8 : n8;
-        g.up = static_cast<int>(n8);
-        pack.m[1] = repack(weight, weight_stride, H, N, base + room.x, g.ldq);
-        if (swiglu)
-            pack.m[2] = repack(static_cast<const uint16_t*>(weight) + N, weight_stride, H, N, pack.m[1].dst + n8, g.ldq);
-    }
-    err = moe::launch_repack(pack, as_stream(stream));
-    if (err == hipSuccess)
-        err = run_product(g, base + room.x + room.w, false, transposed, dtype == MOE_DT_BFLOAT16, as_stream(stream), padded);
-    if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
-    return ok();
+    return linear(x, x_stride, weight, weight_stride, weight_transposed, bias, residual, y, pre, workspace, workspace_bytes, T,
+                  N, H, activation, dtype, out_dtype, stream, Layout::kEither);
+}
+
+size_t moe_linear_layout_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation, int32_t weight_transposed) {
+    if (check_linear("MoeLinear", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
+    return linear_workspace(T, N, H, activation, layout_of(weight_transposed));
+}
+
+moe_status moe_linear_layout(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                             int32_t weight_transposed, const void* bias, const void* residual, void* y, void* pre,
+                             void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
+                             int32_t dtype, int32_t out_dtype, void* stream) {
+    return linear(x, x_stride, weight, weight_stride, weight_transposed, bias, residual, y, pre, workspace, workspace_bytes, T,
+                  N, H, activation, dtype, out_dtype, stream, layout_of(weight_transposed));
 }
 
 size_t moe_linear_grad_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation) {
     if (check_linear("MoeLinearGrad", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
-    return grad_workspace(T, N, H, activation).bytes;
+    return grad_workspace(T, N, H, activation, Layout::kEither).bytes;
 }
 
 moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
                            const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                            int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, void* stream) {
-    const char* op = "MoeLinearGrad";
-    moe_status st = check_linear(op, T, N, H, activation, dtype);
-    if (st != MOE_OK) return st;
-    const GradWorkspace ws = grad_workspace(T, N, H, activation);
-    st = check_pitch(op, "grad_y", T, N, grad_y_stride);
-    if (st != MOE_OK) return st;
-    if (grad_weight) st = check_pitch(op, "x", T, H, x_stride);
-    if (st != MOE_OK) return st;
-    if (grad_x)
-        st = weight_transposed ? check_pitch(op, "weight", H, ws.Z, weight_stride)
-                               : check_pitch(op, "weight", ws.Z, H, weight_stride);
-    if (st != MOE_OK) return st;
-    if (!grad_x && !grad_weight && !grad_bias) return ok();
-    const bool act = activation != MOE_ACT_NONE;
-    if (T > 0 && (!grad_y || (act && !pre) || (grad_weight && !x) || (grad_x && !weight)))
-        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
-    if (T == 0 && !grad_weight && !grad_bias) return ok();
-    if (!workspace || workspace_bytes < ws.bytes)
-        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace,
-                    ws.bytes);
-    if (!aligned16(workspace)) return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
-    const hipStream_t s = as_stream(stream);
-    const bool bf16 = dtype == MOE_DT_BFLOAT16;
-    char* base = static_cast<char*>(workspace);
-    // without an activation dz is grad_y itself, where the products can read that in 16-byte copies
-    const bool as_is = !act && N % 8 == 0 && direct_operand(grad_y, grad_y_stride);
-    const bool need_dz = !as_is && (grad_x || grad_weight) && T > 0;
-    const uint16_t* dz = as_is ? static_cast<const uint16_t*>(grad_y) : reinterpret_cast<uint16_t*>(base);
-    const int64_t ldz = as_is ? grad_y_stride : ws.ldz;
-    hipError_t err = moe::prepare_linear();
-    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad kernel attributes");
-    float* sums = reinterpret_cast<float*>(base + ws.sums_at);
-    if (need_dz || grad_bias)
-        err = moe::launch_act_grad(static_cast<const uint16_t*>(grad_y), grad_y_stride,
-                                   act ? static_cast<const uint16_t*>(pre) : nullptr,
-                                   need_dz ? reinterpret_cast<uint16_t*>(base) : nullptr, ws.ldz,
-                                   grad_bias ? sums : nullptr, T, static_cast<int>(N), activation, bf16, s);
-    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad activation launch");
-    moe::GradTail tail{};
-    moe::GemmArgs &gx = tail.x, &gw = tail.w;
-    gx.p = gw.p = dz;
-    gx.ldp = gw.ldp = ldz;
-    gx.q = static_cast<const uint16_t*>(weight);
-    gx.ldq = weight_stride;
-    gx.m = gw.k = static_cast<int>(T);
-    gx.n = gw.n = static_cast<int>(H);
-    gx.k = gw.m = static_cast<int>(ws.Z);
-    gx.out = grad_x;
-    gw.q = static_cast<const uint16_t*>(x);
-    gw.ldq = x_stride;
-    gw.out = grad_weight;
-    tail.sums = sums;
-    tail.bias_grad = static_cast<uint16_t*>(grad_bias);
-    tail.Z = static_cast<int>(ws.Z);
-    tail.sum_rows = moe::act_grad_row_blocks(T, tail.Z);
-    const bool want_x = grad_x && T > 0, by_k = weight_transposed == 0;
-    moe::RepackArgs pack{};
-    if (grad_weight && T > 0 && H % 8 != 0 && !direct_operand(x, x_stride)) {
-        pack.m[0] = repack(x, x_stride, T, H, base + ws.x_at, round_up(H, 8));
-        gw.q = pack.m[0].dst;
-        gw.ldq = round_up(H, 8);
-    }
-    if (want_x && (by_k ? H % 8 != 0 && !direct_operand(weight, weight_stride) : ws.Z % 8 != 0)) {
-        const int64_t cols = by_k ? H : ws.Z;
-        pack.m[1] = repack(weight, weight_stride, by_k ? ws.Z : H, cols, base + ws.w_at, round_up(cols, 8));
-        gx.q = pack.m[1].dst;
-        gx.ldq = round_up(cols, 8);
-        if (!by_k && need_dz) gx.k = static_cast<int>(ws.ldz);  // zeros in both
-    }
-    err = moe::launch_repack(pack, s);
-    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
-    void* partial = base + ws.partial_at;
-    if (want_x && grad_weight && direct_product(gx, false, by_k, need_dz) && direct_product(gw, true, true, false)) {
-        // one launch for both by tiles of at most 128 rows, where that costs less than the launch it saves
-        const ProductPlan px = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true, 128);
-        const ProductPlan pw = plan_product(gw.m, gw.n, gw.k, false, true, true, true, 128);
-        const double apart = plan_product(gx.m, gx.n, gx.k, false, false, by_k, true).us +
-                             plan_product(gw.m, gw.n, gw.k, false, true, true, true).us;
-        if (px.kernel == Kernel::kMid && pw.kernel == Kernel::kMid && px.us + pw.us < apart + kLaunchSaved) {
-            set_split(gx, px, partial);
-            set_split(gw, pw, static_cast<char*>(partial) + round_up(static_cast<int64_t>(px.partial_bytes), 256));
-            err = moe::launch_gemm_pair(gx, gw, by_k, bf16, px.bm, s);
-            if (err == hipSuccess) err = moe::launch_grad_tail(tail, bf16, s);
-            if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
-            return ok();
-        }
-    }
-    if (want_x) err = run_product(gx, partial, false, by_k, bf16, s, need_dz);
-    if (err == hipSuccess && grad_weight) err = run_product(gw, partial, true, true, bf16, s);
-    if (err == hipSuccess && grad_bias) {
-        gx.splits = gw.splits = 1;
-        err = moe::launch_grad_tail(tail, bf16, s);
-    }
-    if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad launch");
-    return ok();
+    return linear_grad(grad_y, grad_y_stride, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x, grad_weight,
+                       grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream, Layout::kEither);
+}
+
+size_t moe_linear_grad_layout_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation,
+                                              int32_t weight_transposed) {
+    if (check_linear("MoeLinearGrad", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
+    return grad_workspace(T, N, H, activation, layout_of(weight_transposed)).bytes;
+}
+
+moe_status moe_linear_grad_layout(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
+                                  const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
+                                  void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                  size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
+                                  int32_t dtype, void* stream) {
+    return linear_grad(grad_y, grad_y_stride, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x, grad_weight,
+                       grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
+                       layout_of(weight_transposed));
 }
 
 }  // extern "C"

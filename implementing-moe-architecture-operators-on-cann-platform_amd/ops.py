@@ -475,12 +475,20 @@ def MoeCombineGrad(grad_y: torch.Tensor, expert_out: torch.Tensor, weights: torc
     return geo, gw
 
 
-def linear_workspace_bytes(T: int, N: int, H: int, activation: str = "none") -> int:
-    return int(_lib.load().moe_linear_workspace_bytes(T, N, H, _act_code(activation)))
+def linear_workspace_bytes(T: int, N: int, H: int, activation: str = "none", transposed: bool | None = None) -> int:
+    """Workspace of MoeLinear: of a weight whose rows are contiguous (False), of one stored [H, N] (True), or of either."""
+    lib, act = _lib.load(), _act_code(activation)
+    if transposed is None:
+        return int(lib.moe_linear_workspace_bytes(T, N, H, act))
+    return int(lib.moe_linear_layout_workspace_bytes(T, N, H, act, int(transposed)))
 
 
-def linear_grad_workspace_bytes(T: int, N: int, H: int, activation: str = "none") -> int:
-    return int(_lib.load().moe_linear_grad_workspace_bytes(T, N, H, _act_code(activation)))
+def linear_grad_workspace_bytes(T: int, N: int, H: int, activation: str = "none", transposed: bool | None = None) -> int:
+    """Workspace of MoeLinearGrad, as linear_workspace_bytes."""
+    lib, act = _lib.load(), _act_code(activation)
+    if transposed is None:
+        return int(lib.moe_linear_grad_workspace_bytes(T, N, H, act))
+    return int(lib.moe_linear_grad_layout_workspace_bytes(T, N, H, act, int(transposed)))
 
 
 def _linear_sizes(x, weight, act: int):
@@ -516,11 +524,11 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     rp = _matrix(residual, "residual", out, (T, N), dev)
     lib = _lib.load()
     like = _like(x)
-    workspace, wp, wb = _workspace(workspace, lib.moe_linear_workspace_bytes, (T, N, H, act), like, dev, stream)
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_layout_workspace_bytes, (T, N, H, act, transposed), like, dev, stream)
     y = _empty(like, stream, (T, N), out)
     pre = _empty(like, stream, (T, Z), dtype) if returnPre else None
-    check(lib.moe_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre), wp, wb, T,
-                         N, H, act, dt, _FLOAT_DT[out], _queue(stream, dev)))
+    check(lib.moe_linear_layout(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre), wp,
+                                wb, T, N, H, act, dt, _FLOAT_DT[out], _queue(stream, dev)))
     return (y, pre) if returnPre else y
 
 
@@ -544,12 +552,12 @@ def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, p
     pp = _matrix(pre, "pre", dtype, (T, Z), dev) if act else None
     lib = _lib.load()
     like = _like(x)
-    workspace, wp, wb = _workspace(workspace, lib.moe_linear_grad_workspace_bytes, (T, N, H, act), like, dev, stream)
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_grad_layout_workspace_bytes, (T, N, H, act, transposed), like, dev, stream)
     gx = _empty(like, stream, (T, H), dtype) if gradX else None
     gw = _empty(like, stream, (Z, H), dtype) if gradWeight else None
     gb = _empty(like, stream, (Z,), dtype) if gradBias else None
-    check(lib.moe_linear_grad(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, pp,
-                              _ptr(gx), _ptr(gw), _ptr(gb), wp, wb, T, N, H, act, dt, _queue(stream, dev)))
+    check(lib.moe_linear_grad_layout(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, pp,
+                                     _ptr(gx), _ptr(gw), _ptr(gb), wp, wb, T, N, H, act, dt, _queue(stream, dev)))
     return gx, gw, gb
 
 
