@@ -94,6 +94,9 @@ SIGNATURES = {
     "moe_linear_grad_layout_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64, _I32, _I32]),
     "moe_linear_grad_layout": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64,
                                       _I64, _I32, _I32, _P]),
+    "moe_linear_grad_f32_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64, _I32, _I32]),
+    "moe_linear_grad_f32": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64,
+                                   _I64, _I32, _I32, _P]),
     "moe_trace_enable": (_I32, [_I32]),
     "moe_trace_collect": (_I32, []),
     "moe_trace_get": (_I32, [_I32, C.POINTER(C.c_char_p), _I64P, C.POINTER(C.c_double)]),

@@ -250,10 +250,10 @@ size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layout lay
 }
 
 // Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | x and the weight with padded rows,
-// where needed | partial sums of split products
+// where needed | partial sums of split products | of an fp32 grad_y, the largest values of dz and its scale's inverse
 struct GradWorkspace {
     int64_t Z, ldz;
-    size_t sums_at, x_at, w_at, partial_at, bytes;
+    size_t sums_at, x_at, w_at, partial_at, bytes, peaks_at, bytes_f32;
 };
 GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layout layout) {
     GradWorkspace g{};
@@ -268,6 +268,8 @@ GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layou
     const size_t x8 = g.ldz != g.Z ? most_partial(T, H, g.ldz, false, false, true) : 0;
     const size_t x = x0 > x8 ? x0 : x8, w = most_partial(g.Z, H, T, false, true, true);
     g.bytes = g.partial_at + round_up(static_cast<int64_t>(x), 256) + w;  // both, for products of one launch
+    g.peaks_at = round_up(static_cast<int64_t>(g.bytes), 256);
+    g.bytes_f32 = g.peaks_at + (moe::kGradPeaks + 1) * sizeof(float);
     return g;
 }
 
@@ -342,8 +344,8 @@ moe_status linear(const void* x, int64_t x_stride, const void* weight, int64_t w
     if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
     return ok();
 }
-// moe_linear_grad likewise
-moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride, const void* weight,
+// moe_linear_grad likewise; grad_y of the operands' type or, with grad_f32, float32
+moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, bool grad_f32, const void* x, int64_t x_stride, const void* weight,
                        int64_t weight_stride, int32_t weight_transposed, const void* pre, void* grad_x, void* grad_weight,
                        void* grad_bias, void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H,
                        int32_t activation, int32_t dtype, void* stream, Layout workspace_for) {
@@ -352,7 +354,9 @@ moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x,
     if (st != MOE_OK) return st;
     const Layout layout = layout_of(weight_transposed);
     const GradWorkspace ws = grad_workspace(T, N, H, activation, layout);
-    const size_t need = workspace_for == layout ? ws.bytes : grad_workspace(T, N, H, activation, workspace_for).bytes;
+    const size_t need = grad_f32                  ? ws.bytes_f32
+                        : workspace_for == layout ? ws.bytes
+                                                  : grad_workspace(T, N, H, activation, workspace_for).bytes;
     st = check_pitch(op, "grad_y", T, N, grad_y_stride);
     if (st != MOE_OK) return st;
     if (grad_weight) st = check_pitch(op, "x", T, H, x_stride);
@@ -373,23 +377,36 @@ moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x,
     const bool bf16 = dtype == MOE_DT_BFLOAT16;
     char* base = static_cast<char*>(workspace);
     // without an activation dz is grad_y itself, where the products can read that in 16-byte copies
-    const bool as_is = !act && N % 8 == 0 && direct_operand(grad_y, grad_y_stride);
+    const bool as_is = !act && !grad_f32 && N % 8 == 0 && direct_operand(grad_y, grad_y_stride);
     const bool need_dz = !as_is && (grad_x || grad_weight) && T > 0;
     const uint16_t* dz = as_is ? static_cast<const uint16_t*>(grad_y) : reinterpret_cast<uint16_t*>(base);
     const int64_t ldz = as_is ? grad_y_stride : ws.ldz;
     hipError_t err = moe::prepare_linear();
     if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad kernel attributes");
     float* sums = reinterpret_cast<float*>(base + ws.sums_at);
-    if (need_dz || grad_bias)
-        err = moe::launch_act_grad(static_cast<const uint16_t*>(grad_y), grad_y_stride,
-                                   act ? static_cast<const uint16_t*>(pre) : nullptr,
-                                   need_dz ? reinterpret_cast<uint16_t*>(base) : nullptr, ws.ldz,
-                                   grad_bias ? sums : nullptr, T, static_cast<int>(N), activation, bf16, s);
+    float* peaks = need_dz && grad_f32 && !bf16 ? reinterpret_cast<float*>(base + ws.peaks_at) : nullptr;
+    if (need_dz || grad_bias) {
+        moe::ActGrad g{};
+        g.dy = grad_y;
+        g.ldy = grad_y_stride;
+        g.pre = act ? static_cast<const uint16_t*>(pre) : nullptr;
+        g.dz = need_dz ? reinterpret_cast<uint16_t*>(base) : nullptr;
+        g.ldz = ws.ldz;
+        g.part = grad_bias ? sums : nullptr;
+        g.peaks = peaks;
+        g.T = T;
+        g.N = static_cast<int>(N);
+        g.act = activation;
+        g.bf16 = bf16;
+        g.dy_f32 = grad_f32;
+        err = moe::launch_act_grad(g, s);
+    }
     if (err != hipSuccess) return hip_fail(err, "MoeLinearGrad activation launch");
     moe::GradTail tail{};
     moe::GemmArgs &gx = tail.x, &gw = tail.w;
     gx.p = gw.p = dz;
     gx.ldp = gw.ldp = ldz;
+    gx.factor = gw.factor = peaks ? peaks + moe::kGradPeaks : nullptr;
     gx.q = static_cast<const uint16_t*>(weight);
     gx.ldq = weight_stride;
     gx.m = gw.k = static_cast<int>(T);
@@ -578,8 +595,9 @@ moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void
                            const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                            int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, void* stream) {
-    return linear_grad(grad_y, grad_y_stride, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x, grad_weight,
-                       grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream, Layout::kEither);
+    return linear_grad(grad_y, grad_y_stride, false, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x,
+                       grad_weight, grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
+                       Layout::kEither);
 }
 
 size_t moe_linear_grad_layout_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation,
@@ -593,8 +611,22 @@ moe_status moe_linear_grad_layout(const void* grad_y, int64_t grad_y_stride, con
                                   void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                                   size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
                                   int32_t dtype, void* stream) {
-    return linear_grad(grad_y, grad_y_stride, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x, grad_weight,
-                       grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
+    return linear_grad(grad_y, grad_y_stride, false, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x,
+                       grad_weight, grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
+                       layout_of(weight_transposed));
+}
+
+size_t moe_linear_grad_f32_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation, int32_t weight_transposed) {
+    if (check_linear("MoeLinearGrad", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
+    return grad_workspace(T, N, H, activation, layout_of(weight_transposed)).bytes_f32;
+}
+
+moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
+                               const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
+                               void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                               int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, void* stream) {
+    return linear_grad(grad_y, grad_y_stride, true, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x,
+                       grad_weight, grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
                        layout_of(weight_transposed));
 }
 

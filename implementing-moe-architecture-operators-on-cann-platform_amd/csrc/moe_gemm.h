@@ -46,6 +46,7 @@ struct GemmArgs {
     uint16_t* pre;        // [m, n or 2 n] sums before the activation, rounded to the operands' type; may be null
     const uint16_t* bias; // [n or 2 n] or null
     const void* residual; // [m, n] of out's type or null
+    const float* factor;  // device: what the sums are multiplied by first (an operand was scaled), or null; not with SwiGLU
     int act;              // moe_activation
     int out_f32;          // out (and residual) fp32, else the operands' type
     float* partial;       // [splits, m, part_ld] fp32 sums of a product split over k
@@ -105,6 +106,7 @@ __device__ __forceinline__ uint2 pack4(f32x4 y) {
 // four are there and aligned, so they are one access.
 template <typename T, bool SWIGLU>
 __device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col, int valid, bool whole, f32x4 z, f32x4 u) {
+    if (!SWIGLU && g.factor) z *= *g.factor;
     if (g.bias) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {

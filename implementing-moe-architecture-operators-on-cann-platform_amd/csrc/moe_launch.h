@@ -195,10 +195,22 @@ hipError_t launch_group_routing_grad(const GroupRouting& r, const void* grad_wei
 // ---- dense products (moe_linear*.hip) ----
 enum Activation { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActSwiglu = 5 };
 // dz = dy * act'(pre) with rows of ldz (zeros past Z); part (null: not wanted) gets the column sums of
-// act_grad_row_blocks(T, Z) blocks of rows, Z floats each; dz null: the sums alone
+// act_grad_row_blocks(T, Z) blocks of rows, Z floats each; dz null: the sums alone. peaks (null: dz is not scaled): room for
+// kGradPeaks + 1 floats; dz is multiplied by a power of two, whose inverse peaks[kGradPeaks] receives.
+constexpr int kGradPeaks = 256;
+struct ActGrad {
+    const void* dy;  // rows ldy elements apart: fp32 where dy_f32 is set, else the operands' type
+    int64_t ldy;
+    const uint16_t* pre;
+    uint16_t* dz;
+    int64_t ldz;
+    float *part, *peaks;
+    int64_t T;
+    int N, act;
+    bool bf16, dy_f32;
+};
 int act_grad_row_blocks(int64_t T, int Z);
-hipError_t launch_act_grad(const uint16_t* dy, int64_t ldy, const uint16_t* pre, uint16_t* dz, int64_t ldz, float* part,
-                           int64_t T, int N, int act, bool bf16, hipStream_t stream);
+hipError_t launch_act_grad(const ActGrad& g, hipStream_t stream);
 
 // ---- synthetic inputs / calibration (moe_synth.hip) ----
 hipError_t launch_synth_normal_f16(uint16_t* out, uint64_t n, uint64_t seed, uint64_t stream_id, double sigma_a,

@@ -484,11 +484,9 @@ def linear_workspace_bytes(T: int, N: int, H: int, activation: str = "none", tra
 
 
 def linear_grad_workspace_bytes(T: int, N: int, H: int, activation: str = "none", transposed: bool | None = None) -> int:
-    """Workspace of MoeLinearGrad, as linear_workspace_bytes."""
-    lib, act = _lib.load(), _act_code(activation)
-    if transposed is None:
-        return int(lib.moe_linear_grad_workspace_bytes(T, N, H, act))
-    return int(lib.moe_linear_grad_layout_workspace_bytes(T, N, H, act, int(transposed)))
+    """Workspace of MoeLinearGrad, as linear_workspace_bytes, for a grad_y of either type."""
+    query, act = _lib.load().moe_linear_grad_f32_workspace_bytes, _act_code(activation)
+    return max(int(query(T, N, H, act, int(t))) for t in ((False, True) if transposed is None else (transposed,)))
 
 
 def _linear_sizes(x, weight, act: int):
@@ -524,7 +522,8 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     rp = _matrix(residual, "residual", out, (T, N), dev)
     lib = _lib.load()
     like = _like(x)
-    workspace, wp, wb = _workspace(workspace, lib.moe_linear_layout_workspace_bytes, (T, N, H, act, transposed), like, dev, stream)
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_layout_workspace_bytes, (T, N, H, act, transposed), like, dev,
+                                   stream)
     y = _empty(like, stream, (T, N), out)
     pre = _empty(like, stream, (T, Z), dtype) if returnPre else None
     check(lib.moe_linear_layout(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre), wp,
@@ -535,14 +534,14 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
 def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: torch.Tensor | None = None,
                   activation: str = "none", gradX: bool = True, gradWeight: bool = True, gradBias: bool = False,
                   workspace: torch.Tensor | None = None, stream=None):
-    """The gradient of MoeLinear's y[T,N] (of x's type) -> (grad_x[T,H], grad_weight[N,H], grad_bias[N]), contiguous, of
-    x's type, None where not asked for. pre is MoeLinear's (needed with an activation). The residual's gradient is
+    """The gradient of MoeLinear's y[T,N] (of x's type or, for an fp32 y, fp32) -> (grad_x[T,H], grad_weight[N,H],
+    grad_bias[N]), contiguous, of x's type, None where not asked for. pre is MoeLinear's (needed with an activation). The residual's gradient is
     grad_y. `workspace` (uint8, >= linear_grad_workspace_bytes) is allocated when not given."""
     act = _act_code(activation)
     dt, dev = _first_float(x, "x", _HALVES, 2)
     dtype = x.dtype
     _need_float(weight, "weight", (dtype,), 2, dev)
-    _need_float(grad_y, "grad_y", (dtype,), 2, dev)
+    wide = _need_float(grad_y, "grad_y", (dtype, torch.float32), 2, dev) == _lib.DT_FLOAT32
     T, H, N, Z = _linear_sizes(x, weight, act)
     _need_shape(grad_y, "grad_y", (T, N))
     ldx, ldy = _row_stride(x, "x"), _row_stride(grad_y, "grad_y")
@@ -552,12 +551,14 @@ def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, p
     pp = _matrix(pre, "pre", dtype, (T, Z), dev) if act else None
     lib = _lib.load()
     like = _like(x)
-    workspace, wp, wb = _workspace(workspace, lib.moe_linear_grad_layout_workspace_bytes, (T, N, H, act, transposed), like, dev, stream)
+    query, call = ((lib.moe_linear_grad_f32_workspace_bytes, lib.moe_linear_grad_f32) if wide else
+                   (lib.moe_linear_grad_layout_workspace_bytes, lib.moe_linear_grad_layout))
+    workspace, wp, wb = _workspace(workspace, query, (T, N, H, act, transposed), like, dev, stream)
     gx = _empty(like, stream, (T, H), dtype) if gradX else None
     gw = _empty(like, stream, (Z, H), dtype) if gradWeight else None
     gb = _empty(like, stream, (Z,), dtype) if gradBias else None
-    check(lib.moe_linear_grad_layout(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, pp,
-                                     _ptr(gx), _ptr(gw), _ptr(gb), wp, wb, T, N, H, act, dt, _queue(stream, dev)))
+    check(call(grad_y.data_ptr(), ldy, x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, pp, _ptr(gx), _ptr(gw),
+               _ptr(gb), wp, wb, T, N, H, act, dt, _queue(stream, dev)))
     return gx, gw, gb
 
 

@@ -215,8 +215,7 @@ def _linear_backward(ctx, grad_y, grad_pre):
     if any(need):
         if pre is not None and pre.numel() == 0 and x.shape[0] > 0:
             raise RuntimeError(f"MoeLinear: the gradient through {ctx.activation!r} needs returnPre=True")
-        dy = grad_y.to(x.dtype).contiguous()  # an fp32 gradient is rounded to the operands' type, as dz is
-        out = getattr(torch.ops, NAMESPACE).MoeLinearGrad(dy, x, weight, pre, ctx.activation, *need)
+        out = getattr(torch.ops, NAMESPACE).MoeLinearGrad(grad_y.contiguous(), x, weight, pre, ctx.activation, *need)
         got = [g if n else None for g, n in zip(out, need)]
     return got[0], got[1], got[2], grad_y if ctx.has[1] else None, None, None, None
 

@@ -324,7 +324,8 @@ moe_status moe_linear_layout(const void* x, int64_t x_stride, const void* weight
 /* MoeLinearGrad: grad_y[T, N] of dtype (rows grad_y_stride apart) and what moe_linear had -> grad_x[T, H],
  * grad_weight[N, H] (SwiGLU: [2N, H]) and grad_bias, contiguous, of dtype; each may be NULL (not wanted). pre is
  * moe_linear's (not read without an activation). dz = grad_y * act'(pre) is rounded to dtype for the two products
- * grad_x = dz weight and grad_weight = dz^T x; grad_bias sums it before that. residual's gradient is grad_y.
+ * grad_x = dz weight and grad_weight = dz^T x (with float16 values above 65504 become infinite, below 2^-25 zero);
+ * grad_bias sums it before that. residual's gradient is grad_y.
  * With T = 0 grad_weight and grad_bias are zeros. The workspace holds dz, column sums, copies with padded rows and partial
  * sums: always needed, by the same rules. */
 size_t moe_linear_grad_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
@@ -342,6 +343,18 @@ moe_status moe_linear_grad_layout(const void* grad_y, int64_t grad_y_stride, con
                                   const void* pre, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                                   size_t workspace_bytes, int64_t num_tokens, int64_t n, int64_t hidden_size,
                                   int32_t activation, int32_t dtype, void* stream);
+
+/* The same for the gradient of a float32 result: grad_y is float32, the gradients of dtype. dz is rounded to dtype for the
+ * products, with float16 after a multiplication by the power of two that takes its largest finite value to [2^14, 2^15),
+ * which the sums are divided by: nothing of grad_y vanishes or overflows but what is 2^-39 of its largest value.
+ * grad_y of any alignment (4 bytes) and row stride. */
+size_t moe_linear_grad_f32_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation,
+                                           int32_t weight_transposed);
+moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
+                               const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
+                               void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                               size_t workspace_bytes, int64_t num_tokens, int64_t n, int64_t hidden_size,
+                               int32_t activation, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }
