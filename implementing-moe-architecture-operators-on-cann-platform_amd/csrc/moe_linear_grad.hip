@@ -22,7 +22,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kCols = 512;  // columns of a workgroup
 
-__device__ __forceinline__ float slope(float z, int act) {
+// pre may hold infinities and values whose powers overflow: a sum that is finite in fp32 rounds to them. From +-128 on every
+// slope below is at its limit in fp32, where the formulas would give 0 * infinity. NaN stays.
+__device__ __forceinline__ float bounded(float z) { return fabsf(z) > 128.0f ? copysignf(128.0f, z) : z; }
+
+__device__ __forceinline__ float slope(float v, int act) {
+    const float z = bounded(v);
     switch (act) {
         case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
         case kActGelu: {
@@ -40,6 +45,12 @@ __device__ __forceinline__ float slope(float z, int act) {
         }
         default: return 1.0f;
     }
+}
+// silu's slope at a SwiGLU's gate g, and silu itself, which grows with g
+__device__ __forceinline__ float silu_slope(float g, float& silu) {
+    const float z = bounded(g), s = sigmoid_fast(z);
+    silu = (g < -128.0f ? z : g) * s;
+    return s * (1.0f + z * (1.0f - s));
 }
 
 struct ActGradArgs {
@@ -110,8 +121,9 @@ __device__ __forceinline__ void dz8(const ActGradArgs& a, int64_t t, int c, floa
             const s16x8 zg = load8(pre + n, valid, n), zu = load8(pre + a.N + n, valid, n);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float g = at<T>(zg, e), s = sigmoid_fast(g);
-                v[e] = e >= valid ? 0.0f : d[e] * (up ? g * s : at<T>(zu, e) * s * (1.0f + g * (1.0f - s)));
+                float silu;
+                const float s = silu_slope(at<T>(zg, e), silu);
+                v[e] = e >= valid ? 0.0f : d[e] * (up ? silu : at<T>(zu, e) * s);
             }
             return;
         }
@@ -120,8 +132,9 @@ __device__ __forceinline__ void dz8(const ActGradArgs& a, int64_t t, int c, floa
             const int col = c + e, m = col < a.N ? col : col - a.N;
             float x = 0.0f;
             if (col < a.Z) {
-                const float g = T::load(pre[m]), s = sigmoid_fast(g);
-                x = dy_value<T>(dy + m) * (col < a.N ? T::load(pre[a.N + m]) * s * (1.0f + g * (1.0f - s)) : g * s);
+                float silu;
+                const float s = silu_slope(T::load(pre[m]), silu);
+                x = dy_value<T>(dy + m) * (col < a.N ? T::load(pre[a.N + m]) * s : silu);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -215,9 +228,10 @@ __global__ __launch_bounds__(kThreads) void act_grad_kernel(ActGradArgs a) {
                 for (int e = 0; e < 8; ++e) {
                     const float dy = T::load(static_cast<uint16_t>(d[e])), zg = T::load(static_cast<uint16_t>(z[e]));
                     if (MODE == kPairs) {
-                        const float s = sigmoid_fast(zg);
-                        v[0][e] = dy * T::load(static_cast<uint16_t>(u[e])) * s * (1.0f + zg * (1.0f - s));
-                        v[kSums - 1][e] = dy * zg * s;
+                        float silu;
+                        const float s = silu_slope(zg, silu);
+                        v[0][e] = dy * T::load(static_cast<uint16_t>(u[e])) * s;
+                        v[kSums - 1][e] = dy * silu;
                     } else {
                         v[0][e] = a.pre ? dy * slope(zg, a.act) : dy;
                     }

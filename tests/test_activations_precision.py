@@ -1,4 +1,5 @@
-"""The activations and their gradients over the whole range of their types: digits in the tail of GELU."""
+"""The activations and their gradients over the whole range of their types: digits in the tail of GELU, limits at
+infinities."""
 from __future__ import annotations
 
 import math
@@ -53,3 +54,30 @@ def test_gelu_slope_keeps_its_digits_in_the_tail(ops):
     tol = half_step(ref, BF16) + ref.abs() * 6 * 2.0**-20 * (1 + 2.0**-8)
     bad = ~((got - ref).abs() <= tol)
     assert not bad.any(), (zd[bad][:4].tolist(), got[bad][:4].tolist(), ref[bad][:4].tolist())
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_slopes_have_their_limits_at_the_ends(ops, act, dtype):
+    """A sum that is finite in fp32 may be infinite in pre: its slope is the limit, 1 or 0. NaN stays NaN (relu's is 0)."""
+    big = torch.finfo(dtype).max
+    z = torch.tensor([math.inf, big, big / 2, 1000.0, -1000.0, -big / 2, -big, -math.inf, math.nan], dtype=dtype)
+    got = slope_of(ops, z, act).flatten()
+    assert got[:4].tolist() == [1.0] * 4 and got[4:8].abs().max() == 0.0, got.tolist()
+    assert act == "relu" or torch.isnan(got[8])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cols", [1, 8])  # the paths of any width and of whole vectors
+def test_swiglu_slopes_have_their_limits_at_the_ends(ops, dtype, cols):
+    big = torch.finfo(dtype).max
+    gate = torch.tensor([math.inf, big, -big, -math.inf], dtype=dtype)
+    up = torch.tensor([2.0, 2.0, 2.0, 2.0], dtype=dtype)
+    pre = torch.cat([gate.reshape(-1, 1).expand(4, cols), up.reshape(-1, 1).expand(4, cols)], dim=1).contiguous().cuda()
+    w = torch.eye(2 * cols, dtype=dtype, device="cuda")
+    x = torch.zeros((4, 2 * cols), dtype=dtype, device="cuda")
+    dy = torch.ones((4, cols), dtype=dtype, device="cuda")
+    _, _, gb = ops.MoeLinearGrad(dy[2:], x[2:], w, pre[2:].contiguous(), "swiglu", gradBias=True)
+    assert gb.abs().max() == 0.0, gb.tolist()  # silu(gate) and its slope are 0
+    _, _, gb = ops.MoeLinearGrad(dy[:1], x[:1], w, pre[:1].contiguous(), "swiglu", gradBias=True)
+    assert (gb[:cols] == 2.0).all() and torch.isinf(gb[cols:]).all(), gb.tolist()
