@@ -125,6 +125,20 @@ __device__ __forceinline__ float row_sum_f(float v) {
     return (row(0) + row(1)) + (row(2) + row(3));
 }
 
+// Over a DPP row, in float64
+__device__ __forceinline__ double row_sum_d(double v) {
+    auto turned = [](double x, auto ctrl) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = dpp<decltype(ctrl)::value>(static_cast<int>(b)), hi = dpp<decltype(ctrl)::value>(static_cast<int>(b >> 32));
+        return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+    };
+    v += turned(v, std::integral_constant<int, 0x128>());
+    v += turned(v, std::integral_constant<int, 0x124>());
+    v += turned(v, std::integral_constant<int, 0x122>());
+    v += turned(v, std::integral_constant<int, 0x121>());
+    return v;
+}
+
 // Floats as integers in the same order (-0 as 0); key_value undoes it
 __device__ __forceinline__ int key_of(float v) {
     const int b = __builtin_bit_cast(int, v + 0.0f);
@@ -550,12 +564,15 @@ __device__ __forceinline__ void store4_logits(void* p, int64_t i, const float* v
     }
 }
 
-// Gradient of the weights of `ids` to the logits. p = s / sum of the K chosen s, g = scale * grad_w:
+// Gradient of the weights of `ids` to the logits. p = s / sum of the K chosen s, g = grad_w, all times scale:
 //   renormalised  softmax: dl_k = p_k (g_k - sum g p)          sigmoid: the same times (1 - s_k)
 //   not           sigmoid: dl_k = g_k s_k (1 - s_k)            softmax: dl_e = s_e (g_e [e chosen] - sum g s)
+// Where one expert has nearly all of a row, g_k nearly is that sum, and the difference is made of the other picks' terms:
+// scores are fp32, relative to the largest, their sums, the mean and the difference float64. The scale comes last, so that
+// g is exact; one renormalised weight is constant, and its gradient 0, since g s / s is g.
 // Bound by its bytes (T E written, and read in the last form; in the others only the picks' logits are read). 16 lanes have
 // a token, a wave four. A lane has every 16th pick; their terms are added into a row of LDS one after another, so an id
-// that a caller's list holds twice adds up in a fixed order, and the row leaves in whole vectors. fp32 throughout.
+// that a caller's list holds twice adds up in a fixed order, and the row leaves in whole vectors.
 template <typename L, int C, bool VEC>
 __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting r, const void* __restrict__ grad_w,
                                                                    const int32_t* __restrict__ ids,
@@ -580,9 +597,9 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         p.x = logit<L>(r.logits, t * r.ld + e);
         if (!(p.x > kLow)) return p;
         p.id = e;
-        p.g = r.scale * (r.weights_type == MOE_DT_FLOAT32 ? logit<F32>(grad_w, t * K + k)
-                         : r.weights_type == MOE_DT_FLOAT16 ? logit<F16>(grad_w, t * K + k)
-                                                            : logit<B16>(grad_w, t * K + k));
+        p.g = r.weights_type == MOE_DT_FLOAT32   ? logit<F32>(grad_w, t * K + k)
+              : r.weights_type == MOE_DT_FLOAT16 ? logit<F16>(grad_w, t * K + k)
+                                                 : logit<B16>(grad_w, t * K + k);
         return p;
     };
     const Pick first = load_pick(l);
@@ -590,7 +607,8 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
 
     // Scores up to a factor e^-top: of the row's softmax where all of it counts, else, renormalised, relative to the
     // largest of the picks, so that picks far below the row's best keep their ratios.
-    float s[C], top = 0.0f, inv = 1.0f;
+    float s[C], top = 0.0f;
+    double inv = 1.0;  // one over the row's sum
     if (softmax_all) {
         float v[C];
         if (valid) {
@@ -606,15 +624,15 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
             m = max(m, key_of(v[j]));
         }
         top = key_value(row_max_i<kRow>(m));
-        float sum = 0.0f;
+        double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const float d = v[j] == top ? 0.0f : v[j] - top;
             s[j] = v[j] > kLow ? __builtin_amdgcn_exp2f(d * 1.4426950408889634f) : 0.0f;
-            sum += s[j];
+            sum += static_cast<double>(s[j]);
         }
-        sum = row_sum_f<kRow>(sum);
-        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        sum = row_sum_d(sum);
+        inv = sum > 0.0 ? 1.0 / sum : 0.0;
     } else if (r.renormalize) {
         int m = kGone;
         for (int k = l; k < K; k += kRow) {
@@ -626,20 +644,22 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
     }
     auto score = [&](float v) {
         if (r.sigmoid) return expf(fminf(v, 0.0f) - top) / (1.0f + expf(-fabsf(v)));
-        return (v == top ? 1.0f : expf(v - top)) * inv;
+        return v == top ? 1.0f : expf(v - top);
     };
-    float total = 0.0f, dot = 0.0f;  // sums of s and g s over the picks
+    double total = 0.0, dot = 0.0;  // sums of s and g s over the picks
     for (int k = l; k < K; k += kRow) {
         const Pick p = pick_at(k);
         if (p.id < 0) continue;
-        const float sk = score(p.x);
+        const double sk = static_cast<double>(score(p.x));
         total += sk;
-        dot += p.g * sk;
+        dot += static_cast<double>(p.g) * sk;
     }
-    total = row_sum_f<kRow>(total);
-    dot = row_sum_f<kRow>(dot);
-    const float norm = r.renormalize ? (total > 0.0f ? 1.0f / total : 0.0f) : 1.0f;
-    const float mean = r.renormalize ? dot * norm : 0.0f;
+    total = row_sum_d(total);
+    dot = row_sum_d(dot);
+    const bool any = total > 0.0;
+    const double norm = !r.renormalize ? 1.0 : any ? 1.0 / total : 0.0;
+    const double mean = softmax_all ? dot * inv : r.renormalize && any ? dot / total : 0.0;
+    const double scale = static_cast<double>(r.scale);
 
 #pragma unroll
     for (int j = 0; j < C; ++j) {
@@ -650,8 +670,10 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
     for (int k0 = 0; k0 < K; k0 += kRow) {
         const Pick p = pick_at(k0 + l);
         float d = 0.0f;
-        if (p.id >= 0) {
-            d = (p.g - mean) * score(p.x) * norm;
+        if (softmax_all) {
+            d = p.g;
+        } else if (p.id >= 0) {
+            d = static_cast<float>(scale * (static_cast<double>(p.g) - mean) * (static_cast<double>(score(p.x)) * norm));
             if (r.sigmoid) d *= expf(fminf(-p.x, 0.0f)) / (1.0f + expf(-fabsf(p.x)));  // 1 - s
         }
         for (int i = 0; i < kRow && k0 + i < K; ++i) {
@@ -660,6 +682,10 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         }
     }
     if (!valid) return;
+    const double all = scale * inv;
+    auto from_all = [&](float g, float sj) {
+        return static_cast<float>((static_cast<double>(g) - mean) * (all * static_cast<double>(sj)));
+    };
 #pragma unroll
     for (int j = 0; j < C; j += (VEC && C >= 4 ? 4 : 1)) {
         const int e = expert_of<kRow, C>(l, j);
@@ -669,11 +695,11 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
             float v[4] = {a[0], a[1], a[2], a[3]};
             if (softmax_all) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] -= s[j + i] * inv * dot;
+                for (int i = 0; i < 4; ++i) v[i] = from_all(v[i], s[j + i]);
             }
             store4_logits<L>(grad_logits, t * E + e, v);
         } else {
-            put<L>(grad_logits, t * E + e, softmax_all ? row[e] - s[j] * inv * dot : row[e]);
+            put<L>(grad_logits, t * E + e, softmax_all ? from_all(row[e], s[j]) : row[e]);
         }
     }
 }

@@ -1,9 +1,10 @@
-"""MoeRoutingGroupTopK where its values cancel: group scores that are small sums of large c."""
+"""MoeRoutingGroupTopK and its gradient where their values cancel: group scores that are small sums of large c, and the
+gradients of rows that one expert dominates."""
 from __future__ import annotations
 
 import pytest
 
-from test_dense_ops import F16, F32, normal, route_reference
+from test_dense_ops import F16, F32, F64, half_step, normal, route_grad_reference, route_reference
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -44,3 +45,53 @@ def test_group_scores_that_cancel(ops, T, E, G, TG, K, scoring, B):
         if G > 4:
             bias[4] = -1e9
         same_choice(ops, logits, bias.reshape(E).contiguous(), K, G, TG, scoring)
+
+
+def dominated(T, E, seed, gap):
+    """Logits N(0, 1), but for one expert of every row, which stands `gap` above the others."""
+    logits = normal((T, E), F32, seed)
+    at = torch.randint(0, E, (T,), generator=torch.Generator().manual_seed(seed + 1))
+    logits[torch.arange(T), at] += gap
+    return logits
+
+
+@pytest.mark.parametrize("scoring,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True)])
+@pytest.mark.parametrize("E,K", [(8, 2), (64, 6), (200, 20), (256, 8)])
+@pytest.mark.parametrize("gap", [0.0, 6.0, 12.0, 20.0])
+def test_gradient_of_dominated_rows(ops, scoring, renorm, E, K, gap):
+    """dl_k = p_k sum_j p_j (g_k - g_j): every term counts, also where p_k is nearly 1 and g_k nearly the mean of g.
+
+    Scores in fp32, relative to the largest: the exponent d = x - top rounds by |d| 2^-24, expf and a product are within
+    4 ulp, so p_k p_j is within 2 (|d| + 16) 2^-24 of itself, |d| <= gap + 10 here; sums are in float64, here and in the
+    reference: each of the mean's up to K + 5 roundings moves the difference by 2^-53 of the largest |g|, times p_k."""
+    T = 70
+    logits = dominated(T, E, 3, gap if scoring == "softmax" else -gap)
+    if scoring == "sigmoid":  # far below zero a sigmoid is e^x
+        logits = -logits.abs() - 5.0
+    ids = logits.topk(K, dim=1)[1].to(torch.int32)
+    gw = normal((T, K), F32, 5)
+    grad = ops.MoeRoutingGroupTopKGrad(gw.cuda(), logits.cuda(), ids.cuda(), scoring, renorm, 2.5)
+    ref = route_grad_reference(gw, logits, ids, scoring, renorm, 2.5)
+    lg, at = logits.double(), ids.long()
+    s = torch.softmax(lg, dim=1) if scoring == "softmax" else torch.sigmoid(lg)
+    g = torch.zeros(T, E, dtype=F64).scatter_(1, at, 2.5 * gw.double())
+    if renorm:
+        chosen = torch.zeros(T, E, dtype=F64).scatter_(1, at, 1.0)
+        p = s * chosen / (s * chosen).sum(dim=1, keepdim=True)
+    else:
+        p = s
+    terms = p * (p.unsqueeze(1) * (g.unsqueeze(2) - g.unsqueeze(1)).abs()).sum(dim=2)
+    sums = 2 * (K + 5) * 2.0**-53 * p * g.abs().amax(dim=1, keepdim=True)
+    tol = terms * (2 * (gap + 10) + 32) * 2.0**-24 + sums + half_step(ref, F32)
+    out = grad.double().cpu()
+    bad = ~((out - ref).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), out[bad][:4].tolist(), ref[bad][:4].tolist(), tol[bad][:4].tolist())
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_gradient_of_a_single_renormalised_weight_is_zero(ops, scoring):
+    """The weight is scale, whatever the logit."""
+    logits, gw = normal((500, 64), F32, 1), normal((500, 1), F32, 2)
+    ids = logits.argmax(dim=1, keepdim=True).to(torch.int32)
+    grad = ops.MoeRoutingGroupTopKGrad(gw.cuda(), logits.cuda(), ids.cuda(), scoring, True, 2.5)
+    assert (grad == 0).all(), float(grad.abs().max())
