@@ -20,6 +20,7 @@ constexpr int kBatch = 8;  // experts in flight per thread
 // expert_out and its gradient together beyond the 256 MB Infinity Cache go past it (non-temporal): T = 16384, K = 6 144 us,
 // through the cache 171 us
 constexpr int64_t kStreamBytes = int64_t(128) << 20;
+constexpr int64_t kMaxBlocks = int64_t(1) << 22;  // of a launch: 2^30 threads, HIP's limit is 2^32
 
 template <int WAVES, bool NT>  // waves of one token: 1 or 4
 __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* __restrict__ grad_y,
@@ -29,58 +30,60 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
                                                                 uint16_t* __restrict__ grad_w, int64_t T, int H, int K) {
     __shared__ float part[4][kBatch];
     const int wave = static_cast<int>(threadIdx.x) / kWave, lane = lane_id();
-    const int64_t t = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : static_cast<int64_t>(blockIdx.x);
-    if (t >= T) return;  // with four waves a token the whole workgroup
-    const uint16_t* dy = grad_y + t * H;
+    constexpr int kTokens = 4 / WAVES;  // of a workgroup at a time; more than kMaxBlocks workgroups' take turns
     const int first = (WAVES == 1 ? lane : static_cast<int>(threadIdx.x)) * 8;
-    for (int k0 = 0; k0 < K; k0 += kBatch) {
-        float dot[kBatch] = {}, w[kBatch];
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + (WAVES == 1 ? wave : 0); t < T;
+         t += static_cast<int64_t>(gridDim.x) * kTokens) {
+        const uint16_t* dy = grad_y + t * H;
+        for (int k0 = 0; k0 < K; k0 += kBatch) {
+            float dot[kBatch] = {}, w[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) w[u] = k0 + u < K ? f16_bits_to_f32(weights[t * K + k0 + u]) : 0.0f;
-        for (int c = first; c < H; c += WAVES * kWave * 8) {
-            const f16x8 d = load_f16x8(dy + c);
-            f16x8 o[kBatch];
+            for (int u = 0; u < kBatch; ++u) w[u] = k0 + u < K ? f16_bits_to_f32(weights[t * K + k0 + u]) : 0.0f;
+            for (int c = first; c < H; c += WAVES * kWave * 8) {
+                const f16x8 d = load_f16x8(dy + c);
+                f16x8 o[kBatch];
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    if (k0 + u < K) {
+                        const uint16_t* at = expert_out + (t * K + k0 + u) * H + c;
+                        o[u] = NT ? load_f16x8_stream(at) : load_f16x8(at);
+                    }
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (k0 + u < K) {
+                        f16x8 v;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float g = static_cast<float>(d[j]);
+                            dot[u] += g * static_cast<float>(o[u][j]);
+                            v[j] = static_cast<f16>(w[u] * g);
+                        }
+                        uint16_t* at = grad_eo + (t * K + k0 + u) * H + c;
+                        if (NT) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(at));
+                        else *reinterpret_cast<f16x8*>(at) = v;
+                    }
+                }
+            }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u)
-                if (k0 + u < K) {
-                    const uint16_t* at = expert_out + (t * K + k0 + u) * H + c;
-                    o[u] = NT ? load_f16x8_stream(at) : load_f16x8(at);
+#pragma unroll
+                for (int d = kWave / 2; d > 0; d >>= 1) dot[u] += __shfl_xor(dot[u], d, kWave);
+            if (WAVES == 1) {
+                float v = dot[0];
+#pragma unroll
+                for (int u = 1; u < kBatch; ++u) v = lane == u ? dot[u] : v;
+                if (lane < kBatch && k0 + lane < K) grad_w[t * K + k0 + lane] = f32_to_f16_bits(v);
+            } else {
+                if (lane == 0) {
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) part[wave][u] = dot[u];
                 }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                if (k0 + u < K) {
-                    f16x8 v;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float g = static_cast<float>(d[j]);
-                        dot[u] += g * static_cast<float>(o[u][j]);
-                        v[j] = static_cast<f16>(w[u] * g);
-                    }
-                    uint16_t* at = grad_eo + (t * K + k0 + u) * H + c;
-                    if (NT) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(at));
-                    else *reinterpret_cast<f16x8*>(at) = v;
-                }
+                __syncthreads();
+                const int u = static_cast<int>(threadIdx.x);
+                if (u < kBatch && k0 + u < K)
+                    grad_w[t * K + k0 + u] = f32_to_f16_bits(part[0][u] + part[1][u] + part[2][u] + part[3][u]);
+                __syncthreads();
             }
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-#pragma unroll
-            for (int d = kWave / 2; d > 0; d >>= 1) dot[u] += __shfl_xor(dot[u], d, kWave);
-        if (WAVES == 1) {
-            float v = dot[0];
-#pragma unroll
-            for (int u = 1; u < kBatch; ++u) v = lane == u ? dot[u] : v;
-            if (lane < kBatch && k0 + lane < K) grad_w[t * K + k0 + lane] = f32_to_f16_bits(v);
-        } else {
-            if (lane == 0) {
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) part[wave][u] = dot[u];
-            }
-            __syncthreads();
-            const int u = static_cast<int>(threadIdx.x);
-            if (u < kBatch && k0 + u < K)
-                grad_w[t * K + k0 + u] = f32_to_f16_bits(part[0][u] + part[1][u] + part[2][u] + part[3][u]);
-            __syncthreads();
         }
     }
 }
@@ -93,7 +96,8 @@ hipError_t launch_combine_grad(const uint16_t* grad_y, const uint16_t* expert_ou
     const bool nt = T * K * H * 2 > kStreamBytes;
     // a wave a token once that gives every SIMD two waves
     const bool one = T >= 2048;
-    const unsigned grid = static_cast<unsigned>(one ? (T + 3) / 4 : T);
+    const int64_t blocks = one ? (T + 3) / 4 : T;
+    const unsigned grid = static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
     if (one && nt)
         combine_grad_kernel<1, true><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     else if (one)

@@ -547,7 +547,7 @@ moe_status moe_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, 
     if (H % 8 != 0) return fail(MOE_ERR_UNSUPPORTED, "%s: hiddenSize=%lld must be a multiple of 8", op, (long long)H);
     if (H > kMaxDim)
         return fail(MOE_ERR_UNSUPPORTED, "%s: hiddenSize=%lld exceeds %lld", op, (long long)H, (long long)kMaxDim);
-    if (product_exceeds(T, K, kInt32Max) || T >= int64_t{1} << 25)
+    if (product_exceeds(T, K, kInt32Max))
         return fail(MOE_ERR_UNSUPPORTED, "%s: T=%lld K=%lld too large", op, (long long)T, (long long)K);
     if (T == 0) return ok();
     if (!grad_y || !expert_out || !weights || !grad_expert_out || !grad_weights)
