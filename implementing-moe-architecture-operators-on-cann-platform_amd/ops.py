@@ -26,10 +26,15 @@ from ._lib import MoeError, check, dims
 
 # The current stream without the Stream object that torch.cuda.current_stream() makes on each call, and the allocation on
 # the current device that torch's compiled code uses (0.75 us a tensor, new_empty 1.5): private to torch, so a torch
-# without them takes the public functions.
+# without them takes the public functions. The allocation passes torch's dispatch modes and its filling of new memory under
+# deterministic algorithms by, so it is used where neither is on.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", None)
 _empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_deterministic = getattr(torch._C, "_get_deterministic_algorithms", None)
+if _modes is None or _deterministic is None:
+    _empty_strided = None
 
 _TORCH_DT = {_lib.DT_FLOAT16: torch.float16, _lib.DT_INT32: torch.int32}
 _FLOAT_DT = {torch.float32: _lib.DT_FLOAT32, torch.float16: _lib.DT_FLOAT16, torch.bfloat16: _lib.DT_BFLOAT16}
@@ -340,7 +345,7 @@ def _act_code(activation: str) -> int:
 def _empty(like: torch.Tensor, stream, shape: tuple, dtype: torch.dtype) -> torch.Tensor:
     """A new contiguous tensor that belongs to the stream the kernels run on."""
     if stream is None:
-        if _empty_strided is None:
+        if _empty_strided is None or _modes() or _deterministic():
             return like.new_empty(shape, dtype=dtype)
         dims = len(shape)
         if dims == 2:
