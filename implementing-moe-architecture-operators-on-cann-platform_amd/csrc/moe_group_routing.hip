@@ -11,7 +11,10 @@
 // does not are nearer than theirs (group_error), the row's groups are scored again in float64; where two neighbours among
 // its picks are, the picks go on past the K-th until a clear gap and are put in order by their float64 values. That is
 // some rows in a hundred, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
-// never in the instruction cache when it is needed, cost 9 us.
+// never in the instruction cache when it is needed, cost 9 us. Where kMore picks more leave no gap (equal scores, biases
+// that leave few bits for the scores), the K best of the row are taken by their float64 values, one maximum of the wave
+// each: calls with 256 equal scores a row take 10.7 us at T = 1 and 43 at T = 16384, where picking and ordering all of them
+// took 157 and 660 (with 8 groups 16.2 and 75, before 62 and 240).
 //
 // A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers; few
 // tokens of many experts have a wave each. A pick is the maximum over the lane (max3) and over the row (4 DPP steps), and
@@ -33,6 +36,7 @@ namespace {
 constexpr int kRow = 16;  // lanes of a DPP row
 constexpr int kRowTokens = kWave / kRow;  // tokens of a wave with a DPP row each
 constexpr int kMaxE = 256;
+constexpr int kMore = 8;                     // picks past the K-th
 constexpr int kNoPick = 0xffff;              // a pick with no expert left
 constexpr int kGone = -2147483647 - 1;         // the key of an expert that is not available or was picked
 constexpr float kLow = -__builtin_huge_valf();
@@ -125,18 +129,33 @@ __device__ __forceinline__ float row_sum_f(float v) {
     return (row(0) + row(1)) + (row(2) + row(3));
 }
 
-// Over a DPP row, in float64
+// A double as the lane that a DPP control names has it; as row `row`'s first lane has it
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = dpp<CTRL>(static_cast<int>(b)), hi = dpp<CTRL>(static_cast<int>(b >> 32));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double row_of_d(double v, int row) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = row_of(static_cast<int>(b), row), hi = row_of(static_cast<int>(b >> 32), row);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Over a DPP row
 __device__ __forceinline__ double row_sum_d(double v) {
-    auto turned = [](double x, auto ctrl) {
-        const uint64_t b = __builtin_bit_cast(uint64_t, x);
-        const uint32_t lo = dpp<decltype(ctrl)::value>(static_cast<int>(b)), hi = dpp<decltype(ctrl)::value>(static_cast<int>(b >> 32));
-        return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-    };
-    v += turned(v, std::integral_constant<int, 0x128>());
-    v += turned(v, std::integral_constant<int, 0x124>());
-    v += turned(v, std::integral_constant<int, 0x122>());
-    v += turned(v, std::integral_constant<int, 0x121>());
+    v += dpp_d<0x128>(v);
+    v += dpp_d<0x124>(v);
+    v += dpp_d<0x122>(v);
+    v += dpp_d<0x121>(v);
     return v;
+}
+// Over the wave
+__device__ __forceinline__ double wave_max_d(double v) {
+    v = fmax(v, dpp_d<0x128>(v));
+    v = fmax(v, dpp_d<0x124>(v));
+    v = fmax(v, dpp_d<0x122>(v));
+    v = fmax(v, dpp_d<0x121>(v));
+    return fmax(fmax(row_of_d(v, 0), row_of_d(v, 1)), fmax(row_of_d(v, 2), row_of_d(v, 3)));
 }
 
 // Floats as integers in the same order (-0 as 0); key_value undoes it
@@ -451,7 +470,7 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
                 }
                 last = m;
             }
-            if (k >= K && !__any(k < picks)) break;
+            if (k >= K && (k == K + kMore || !__any(k < picks))) break;
             if (l == 0 && k < picks)
                 pick[tok * E + k] = static_cast<uint16_t>(m == kGone ? kNoPick : kMaxE - 1 - (m & (kMaxE - 1)));
 #pragma unroll
@@ -476,14 +495,15 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         }
     }
     __syncthreads();
-    uint64_t redo = __ballot(reorder && valid);
+    const uint64_t redo = __ballot(reorder && valid), select = __ballot(picks > K + kMore && valid);
 #pragma unroll 1
     for (int q = 0; redo && q < kTokens; ++q) {
         if (!((redo >> (q * LANES)) & 1)) continue;
         const int64_t tq = static_cast<int64_t>(blockIdx.x) * kTokens + q;
         const int n = __shfl(picks, q * LANES, kWave);
         uint16_t* of = pick + q * E;
-        if (r.sigmoid) {  // the picks' alone
+        const bool whole_row = (select >> (q * LANES)) & 1;
+        if (r.sigmoid && !whole_row) {  // the picks' alone
             for (int k = lane; k < n; k += kWave) {
                 const int e = of[k];
                 if (e == kNoPick) continue;
@@ -493,6 +513,32 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
             __syncthreads();
         } else {
             exact_scores<L>(r, tq, cs);
+        }
+        if (whole_row) {
+            double c[kMaxE / kWave];  // of expert i * 64 + lane
+#pragma unroll
+            for (int i = 0; i < kMaxE / kWave; ++i) {
+                const int e = i * kWave + lane;
+                c[i] = e < E && (!grouped || kept[q * G + ((e * r.size_inverse) >> 16)]) ? cs[e] : kNone;
+            }
+#pragma unroll 1
+            for (int k = 0; k < K; ++k) {
+                double m = c[0];
+#pragma unroll
+                for (int i = 1; i < kMaxE / kWave; ++i) m = fmax(m, c[i]);
+                m = wave_max_d(m);
+                int e = kNoPick;
+#pragma unroll
+                for (int i = kMaxE / kWave - 1; i >= 0; --i) {  // the lowest index last
+                    const uint64_t at = __ballot(c[i] == m);
+                    if (m > kNone && at) e = i * kWave + __builtin_ctzll(at);
+                }
+#pragma unroll
+                for (int i = 0; i < kMaxE / kWave; ++i) c[i] = e == i * kWave + lane ? kNone : c[i];
+                if (lane == 0) of[k] = static_cast<uint16_t>(e);
+            }
+            __syncthreads();
+            continue;
         }
 #pragma unroll 1
         for (int k = lane; k < n; k += kWave) {

@@ -95,3 +95,20 @@ def test_gradient_of_a_single_renormalised_weight_is_zero(ops, scoring):
     ids = logits.argmax(dim=1, keepdim=True).to(torch.int32)
     grad = ops.MoeRoutingGroupTopKGrad(gw.cuda(), logits.cuda(), ids.cuda(), scoring, True, 2.5)
     assert (grad == 0).all(), float(grad.abs().max())
+
+
+@pytest.mark.parametrize("T,E,G,TG,K", [(5, 48, 1, 1, 6), (5, 65, 5, 2, 20), (40, 200, 8, 3, 8), (70, 256, 1, 1, 8),
+                                        (70, 256, 8, 4, 40), (5, 256, 1, 1, 256), (2100, 256, 8, 4, 8), (2100, 64, 1, 1, 2)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_more_scores_than_fp32_tells_apart(ops, T, E, G, TG, K, scoring):
+    """Equal scores, runs of equal ones, and biases beside which the scores keep few bits: the float64 values decide among
+    all of a row's experts, the lowest index among equal ones."""
+    logits = normal((T, E), F32, 23)
+    logits[::3] = (logits[::3] * 2).round() / 2
+    logits[1::7] = 0.0
+    logits[2::11, ::2] = float("-inf")
+    logits[3::13, 1:] = float("-inf")
+    steps = (torch.arange(E) % 5).float() / 4
+    signs = torch.where(torch.arange(E) % 2 == 0, 40.0, -40.0)
+    for bias in (torch.zeros(E), torch.full((E,), 1e4), torch.full((E,), -3e3), steps, signs, 1e5 + signs):
+        same_choice(ops, logits, bias, K, G, TG, scoring)
