@@ -44,3 +44,38 @@ def test_results_are_seen_by_dispatch_modes(ops):
         geo, _ = ops.MoeCombineGrad(x, ones((6, 2, 64), 4), wt[:, :2].contiguous())
     for shape in ((6, 40), (6, 3), (6, 64), (40, 64), (6, 2, 64)):
         assert shape in seen.shapes, (shape, seen.shapes)
+
+
+@pytest.mark.parametrize("T,N,H,transposed", [(4, 72, 8192, True), (4, 72, 8192, False), (130, 72, 8192, False),
+                                              (40, 130, 4100, True)])
+def test_split_sums_are_in_the_workspace_and_in_one_order(ops, T, N, H, transposed):
+    """Where the plan splits k (all but few aligned rows of a weight by rows), the pieces' sums are in the workspace, within
+    it, and every call adds them alike."""
+    w = torch.randn((H, N) if transposed else (N, H), device="cuda", dtype=F16)
+    w, x = w.t() if transposed else w, torch.randn((T, H), device="cuda", dtype=F16)
+    need = ops.linear_workspace_bytes(T, N, H)
+    got = []
+    for _ in range(3):
+        ws = torch.full((need + 256,), 0x7f, dtype=torch.uint8, device="cuda")
+        got.append(ops.MoeLinear(x, w, outDtype=F32, workspace=ws))
+        assert (ws[need:] == 0x7f).all()
+        if transposed or T > 64:
+            assert (ws[:need] != 0x7f).sum() > T * N * 4
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    ref = x.double() @ w.double().t()
+    tol = (H + 1) * 2.0**-24 * (x.double().abs() @ w.double().abs().t())
+    assert ((got[0].double() - ref).abs() <= tol + 2.0**-24 * ref.abs()).all()
+
+
+@pytest.mark.parametrize("T,N,H,transposed", [(4097, 2056, 72, False), (3001, 3000, 200, False), (2049, 4104, 1032, True),
+                                              (8191, 1400, 136, False), (4099, 1032, 1000, True), (260, 33000, 96, False),
+                                              (300, 520, 4096, False), (1000, 733, 1056, True)])
+def test_every_value_of_large_products(ops, T, N, H, transposed):
+    """Operands -1, 0 and 1: sums below 2^24 are whole in fp32 in any order, so a lost or repeated term shows anywhere."""
+    x, w, dy = ones((T, H), 1), ones((H, N) if transposed else (N, H), 2), ones((T, N), 3)
+    w = w.t() if transposed else w
+    assert torch.equal(ops.MoeLinear(x, w, outDtype=F32), x.float() @ w.float().t())
+    gx, gw, gb = ops.MoeLinearGrad(dy, x, w, gradBias=True)
+    assert torch.equal(gx, (dy.float() @ w.float()).to(F16))
+    assert torch.equal(gw, (dy.float().t() @ x.float()).to(F16))
+    assert torch.equal(gb, dy.float().sum(dim=0).to(F16))
