@@ -1,12 +1,13 @@
-// moe_combine_grad.hip -- MoeCombineGrad for gfx950: the gradients of y[t, :] = sum_k weights[t, k] expert_out[t, k, :].
+// moe_combine_grad.hip -- MoeCombineGrad for gfx950: the gradients of y[t, :] = sum_k weights[t, k] *
+// expert_out[t, k, :].
 //
 //   grad_expert_out[t, k, :] = weights[t, k] * grad_y[t, :]
 //   grad_weights[t, k]       = sum_h grad_y[t, h] * expert_out[t, k, h]
 //
 // The forward is the reference's op_kernel/moe_combine.cpp:80-111; it has no gradient there.
-// Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 8 experts at
-// a time, loads their rows, adds to their dot products and writes their gradient rows. A wave has a token to itself, or
-// four waves share it; the dot products are added over the lanes and then over the waves in a fixed order.
+// Pure streaming: T (2 K + 1) H 2 bytes. One pass: a thread holds 8 hidden elements of grad_y and, for up to 8 experts
+// at a time, loads their rows, adds to their dot products and writes their gradient rows. A wave has a token to itself,
+// or four waves share it; the dot products are added over the lanes and then over the waves in a fixed order.
 // T = 16384, H = 2048, K = 6: 872 MB in 144 us, 6.07 TB/s (a copy of 1 GB: 5.0). T = 128, K = 2: 4 us, of a call of 7.
 #include "moe_device.h"
 #include "moe_launch.h"
@@ -17,8 +18,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 8;  // experts in flight per thread
-// expert_out and its gradient together beyond the 256 MB Infinity Cache go past it (non-temporal): T = 16384, K = 6 144 us,
-// through the cache 171 us
+// expert_out and its gradient together beyond the 256 MB Infinity Cache go past it (non-temporal): T = 16384, K = 6 144
+// us, through the cache 171 us
 constexpr int64_t kStreamBytes = int64_t(128) << 20;
 constexpr int64_t kMaxBlocks = int64_t(1) << 22;  // of a launch: 2^30 threads, HIP's limit is 2^32
 
@@ -27,7 +28,8 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(const uint16_t* 
                                                                 const uint16_t* __restrict__ expert_out,
                                                                 const uint16_t* __restrict__ weights,
                                                                 uint16_t* __restrict__ grad_eo,
-                                                                uint16_t* __restrict__ grad_w, int64_t T, int H, int K) {
+                                                                uint16_t* __restrict__ grad_w, int64_t T, int H,
+                                                                int K) {
     __shared__ float part[4][kBatch];
     const int wave = static_cast<int>(threadIdx.x) / kWave, lane = lane_id();
     constexpr int kTokens = 4 / WAVES;  // of a workgroup at a time; more than kMaxBlocks workgroups' take turns
@@ -99,13 +101,17 @@ hipError_t launch_combine_grad(const uint16_t* grad_y, const uint16_t* expert_ou
     const int64_t blocks = one ? (T + 3) / 4 : T;
     const unsigned grid = static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
     if (one && nt)
-        combine_grad_kernel<1, true><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+        combine_grad_kernel<1, true>
+            <<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     else if (one)
-        combine_grad_kernel<1, false><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+        combine_grad_kernel<1, false>
+            <<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     else if (nt)
-        combine_grad_kernel<4, true><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+        combine_grad_kernel<4, true>
+            <<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     else
-        combine_grad_kernel<4, false><<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
+        combine_grad_kernel<4, false>
+            <<<grid, kThreads, 0, stream>>>(grad_y, expert_out, weights, grad_eo, grad_w, T, H, K);
     return hipGetLastError();
 }
 

@@ -95,9 +95,9 @@ struct ProductPlan {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Microseconds of a launch by tiles of bm x 128 with `items` workgroups of `stages` 64-k stages. Up to 128 rows two
-// workgroups share a CU: a stage takes `one` alone and `two` beside another. At 256 rows a CU has one: `one` with few of them,
-// `two` with one on every CU. A launch takes `launch` besides, and each further round of the GPU `round` for its first
-// copies and its epilogue. Where P is read by k too, both operands go through transposing reads.
+// workgroups share a CU: a stage takes `one` alone and `two` beside another. At 256 rows a CU has one: `one` with few
+// of them, `two` with one on every CU. A launch takes `launch` besides, and each further round of the GPU `round` for
+// its first copies and its epilogue. Where P is read by k too, both operands go through transposing reads.
 double mid_time(int bm, int64_t items, int64_t stages, bool p_by_k) {
     struct Cost {
         double one, two, launch, round;
@@ -114,8 +114,8 @@ double mid_time(int bm, int64_t items, int64_t stages, bool p_by_k) {
     return c.launch + c.round * static_cast<double>(ceil_div(items, slots) - 1) +
            stages * (static_cast<double>(items / slots) * c.two + tail);
 }
-// The same of 256 x 256 tiles: one workgroup a CU, 1.0 us a stage with few tiles up to 1.46 with one on every CU (the clock
-// falls), 7 to 10 us of first copies and epilogue a round.
+// The same of 256 x 256 tiles: one workgroup a CU, 1.0 us a stage with few tiles up to 1.46 with one on every CU (the
+// clock falls), 7 to 10 us of first copies and epilogue a round.
 double tiled_time(int64_t tiles, int64_t stages, bool p_by_k) {
     const double launch = p_by_k ? 7.1 : 5.8, round = p_by_k ? 9.4 : 10.2, stage = p_by_k ? 1.59 : 1.46;
     const double few_round = p_by_k ? 7.4 : 6.7, few_stage = p_by_k ? 1.2 : 1.01, more = p_by_k ? 0.43 : 0.41;
@@ -130,13 +130,14 @@ double reduce_time(size_t partial, bool p_by_k) {
 }
 
 // The kernel with the least time by those figures, which are fitted to every kernel's times in 306 products (T = 128 ..
-// 16384, N and H = 64 .. 12288, in the forward's two layouts and the weight gradient's): the choice is the fastest of them or
-// 0.3 % slower on average, 16 % at worst (T = 16384, N = 256, H = 7168, where all are within that).
-// A product by tiles is split over k while that leaves eight stages a piece and at most the workgroups that the GPU
-// holds; the pieces' sums then take another launch.
+// 16384, N and H = 64 .. 12288, in the forward's two layouts and the weight gradient's): of those products the choice
+// is the fastest kernel or 0.3 % slower on average, 16 % at worst (T = 16384, N = 256, H = 7168, where all are within
+// that). A product by tiles is split over k while that leaves eight stages a piece and at most the workgroups that the
+// GPU holds; the pieces' sums then take another launch.
 // Few rows stream the weights where both operands are read by rows: T = 16, H = 2048, N = 7168 8.2 us (tiles of 32 rows
-// 11.5), T = 64 11.6 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N = 256
-// 12.4 us (8.3 split over k), T = 64, H = 4096, N = 16384 35 us (33).
+// 11.5), T = 64 11.6 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N =
+// 256 12.4 us (8.3 split over k), T = 64, H = 4096, N = 16384 35 us (33). Up to 16 rows a call takes 8.3 to 8.9 us from
+// N = 8 to 512 and H = 2048 to 8192, the host's time, where two launches take 10.7.
 // most_rows: the tallest tiles to choose from.
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct,
                          int most_rows = 256) {
@@ -165,7 +166,8 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by
     }
     const int64_t tiles = ceil_div(m, 256) * ceil_div(n, swiglu ? 128 : 256);
     const double t = tiled_time(tiles, stages, p_by_k);
-    if (direct && m > 64 && most_rows >= 256 && t < best.us) best = ProductPlan{Kernel::kTiled, 256, 1, stages * 64, 0, t};
+    if (direct && m > 64 && most_rows >= 256 && t < best.us)
+        best = ProductPlan{Kernel::kTiled, 256, 1, stages * 64, 0, t};
     return best;
 }
 
@@ -215,8 +217,8 @@ hipError_t run_product(moe::GemmArgs g, void* partial, bool p_by_k, bool q_by_k,
 enum class Layout { kRows, kTransposed, kEither };
 Layout layout_of(int32_t weight_transposed) { return weight_transposed ? Layout::kTransposed : Layout::kRows; }
 
-// Room for x and the weight with padded rows (moe_linear_repack.hip), where the sizes alone make them necessary: x and a
-// weight [Z, H] where H is no multiple of 8, a transposed weight [H, Z] where Z (a SwiGLU's N) is none.
+// Room for x and the weight with padded rows (moe_linear_repack.hip), where the sizes alone make them necessary: x and
+// a weight [Z, H] where H is no multiple of 8, a transposed weight [H, Z] where Z (a SwiGLU's N) is none.
 struct RepackRoom {
     size_t x, w;
 };
@@ -249,8 +251,9 @@ size_t linear_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layout lay
     return room.x + room.w + (partial > padded ? partial : padded);
 }
 
-// Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | x and the weight with padded rows,
-// where needed | partial sums of split products | of an fp32 grad_y, the largest values of dz and its scale's inverse
+// Workspace of the gradients: dz [T, Z rounded up to 8] | column sums of row blocks | x and the weight with padded
+// rows, where needed | partial sums of split products | of an fp32 grad_y, the largest values of dz and its scale's
+// inverse
 struct GradWorkspace {
     int64_t Z, ldz;
     size_t sums_at, x_at, w_at, partial_at, bytes, peaks_at, bytes_f32;
@@ -260,7 +263,8 @@ GradWorkspace grad_workspace(int64_t T, int64_t N, int64_t H, int32_t act, Layou
     g.Z = act == MOE_ACT_SWIGLU ? 2 * N : N;
     g.ldz = round_up(g.Z, 8);
     g.sums_at = round_up(T * g.ldz * 2, 256);
-    g.x_at = g.sums_at + round_up(static_cast<int64_t>(moe::act_grad_row_blocks(T, static_cast<int>(g.Z))) * g.Z * 4, 256);
+    const int64_t row_blocks = moe::act_grad_row_blocks(T, static_cast<int>(g.Z));
+    g.x_at = g.sums_at + round_up(row_blocks * g.Z * 4, 256);
     const RepackRoom room = repack_room(T, g.Z, H, false, layout);
     g.w_at = g.x_at + room.x;
     g.partial_at = g.w_at + room.w;
@@ -286,7 +290,8 @@ moe_status linear(const void* x, int64_t x_stride, const void* weight, int64_t w
     const int64_t Z = activation == MOE_ACT_SWIGLU ? 2 * N : N;
     st = check_pitch(op, "x", T, H, x_stride);
     if (st != MOE_OK) return st;
-    st = weight_transposed ? check_pitch(op, "weight", H, Z, weight_stride) : check_pitch(op, "weight", Z, H, weight_stride);
+    st = weight_transposed ? check_pitch(op, "weight", H, Z, weight_stride)
+                           : check_pitch(op, "weight", Z, H, weight_stride);
     if (st != MOE_OK) return st;
     if (T == 0) return ok();
     if (!x || !weight || !y) return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
@@ -336,19 +341,22 @@ moe_status linear(const void* x, int64_t x_stride, const void* weight, int64_t w
         g.up = static_cast<int>(n8);
         pack.m[1] = repack(weight, weight_stride, H, N, base + room.x, g.ldq);
         if (swiglu)
-            pack.m[2] = repack(static_cast<const uint16_t*>(weight) + N, weight_stride, H, N, pack.m[1].dst + n8, g.ldq);
+            pack.m[2] =
+                repack(static_cast<const uint16_t*>(weight) + N, weight_stride, H, N, pack.m[1].dst + n8, g.ldq);
     }
     err = moe::launch_repack(pack, as_stream(stream));
     if (err == hipSuccess)
-        err = run_product(g, base + room.x + room.w, false, transposed, dtype == MOE_DT_BFLOAT16, as_stream(stream), padded);
+        err = run_product(g, base + room.x + room.w, false, transposed, dtype == MOE_DT_BFLOAT16, as_stream(stream),
+                          padded);
     if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
     return ok();
 }
 // moe_linear_grad likewise; grad_y of the operands' type or, with grad_f32, float32
-moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, bool grad_f32, const void* x, int64_t x_stride, const void* weight,
-                       int64_t weight_stride, int32_t weight_transposed, const void* pre, void* grad_x, void* grad_weight,
-                       void* grad_bias, void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H,
-                       int32_t activation, int32_t dtype, void* stream, Layout workspace_for) {
+moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, bool grad_f32, const void* x, int64_t x_stride,
+                       const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
+                       void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                       int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, void* stream,
+                       Layout workspace_for) {
     const char* op = "MoeLinearGrad";
     moe_status st = check_linear(op, T, N, H, activation, dtype);
     if (st != MOE_OK) return st;
@@ -569,21 +577,22 @@ moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64
                       int32_t weight_transposed, const void* bias, const void* residual, void* y, void* pre,
                       void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
                       int32_t dtype, int32_t out_dtype, void* stream) {
-    return linear(x, x_stride, weight, weight_stride, weight_transposed, bias, residual, y, pre, workspace, workspace_bytes, T,
-                  N, H, activation, dtype, out_dtype, stream, Layout::kEither);
+    return linear(x, x_stride, weight, weight_stride, weight_transposed, bias, residual, y, pre, workspace,
+                  workspace_bytes, T, N, H, activation, dtype, out_dtype, stream, Layout::kEither);
 }
 
-size_t moe_linear_layout_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation, int32_t weight_transposed) {
+size_t moe_linear_layout_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation,
+                                         int32_t weight_transposed) {
     if (check_linear("MoeLinear", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
     return linear_workspace(T, N, H, activation, layout_of(weight_transposed));
 }
 
 moe_status moe_linear_layout(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                              int32_t weight_transposed, const void* bias, const void* residual, void* y, void* pre,
-                             void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
-                             int32_t dtype, int32_t out_dtype, void* stream) {
-    return linear(x, x_stride, weight, weight_stride, weight_transposed, bias, residual, y, pre, workspace, workspace_bytes, T,
-                  N, H, activation, dtype, out_dtype, stream, layout_of(weight_transposed));
+                             void* workspace, size_t workspace_bytes, int64_t T, int64_t N, int64_t H,
+                             int32_t activation, int32_t dtype, int32_t out_dtype, void* stream) {
+    return linear(x, x_stride, weight, weight_stride, weight_transposed, bias, residual, y, pre, workspace,
+                  workspace_bytes, T, N, H, activation, dtype, out_dtype, stream, layout_of(weight_transposed));
 }
 
 size_t moe_linear_grad_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation) {
@@ -616,15 +625,17 @@ moe_status moe_linear_grad_layout(const void* grad_y, int64_t grad_y_stride, con
                        layout_of(weight_transposed));
 }
 
-size_t moe_linear_grad_f32_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation, int32_t weight_transposed) {
+size_t moe_linear_grad_f32_workspace_bytes(int64_t T, int64_t N, int64_t H, int32_t activation,
+                                           int32_t weight_transposed) {
     if (check_linear("MoeLinearGrad", T, N, H, activation, MOE_DT_FLOAT16) != MOE_OK) return 0;
     return grad_workspace(T, N, H, activation, layout_of(weight_transposed)).bytes_f32;
 }
 
 moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
                                const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
-                               void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
-                               int64_t T, int64_t N, int64_t H, int32_t activation, int32_t dtype, void* stream) {
+                               void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                               size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int32_t activation,
+                               int32_t dtype, void* stream) {
     return linear_grad(grad_y, grad_y_stride, true, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x,
                        grad_weight, grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
                        layout_of(weight_transposed));

@@ -46,7 +46,7 @@ struct GemmArgs {
     uint16_t* pre;        // [m, n or 2 n] sums before the activation, rounded to the operands' type; may be null
     const uint16_t* bias; // [n or 2 n] or null
     const void* residual; // [m, n] of out's type or null
-    const float* factor;  // device: what the sums are multiplied by first (an operand was scaled), or null; not with SwiGLU
+    const float* factor;  // device: multiplies the sums first (an operand was scaled); null: 1. Not with SwiGLU
     int act;              // moe_activation
     int out_f32;          // out (and residual) fp32, else the operands' type
     float* partial;       // [splits, m, part_ld] fp32 sums of a product split over k
@@ -64,11 +64,11 @@ __device__ __forceinline__ float sigmoid_fast(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
 }
 
-// The normal distribution function Phi(z) = 1/2 erfc(-z / sqrt 2) and e = e^(-z^2 / 2). From the tail's side, so that a large
-// negative z keeps its digits: Phi(-x) = e^(-x^2 / 2) Q(x), where Q(x) = 1/2 erfcx(x / sqrt 2) falls from 1/2 like 1 / x. Q is
-// t P(t) with t = 1 / (1 + 0.35 x) and P of degree 8, fitted here for the least relative error over x = 0 .. 14 (2^-24.9;
-// past that e is 0 in fp32). The exponent is taken in two parts, since its rounding alone would move e by x^2 2^-25. Together
-// within 2^-21 of itself (rounded stepwise on the host over 400000 z).
+// The normal distribution function Phi(z) = 1/2 erfc(-z / sqrt 2) and e = e^(-z^2 / 2). From the tail's side, so that a
+// large negative z keeps its digits: Phi(-x) = e^(-x^2 / 2) Q(x), where Q(x) = 1/2 erfcx(x / sqrt 2) falls from 1/2
+// like 1 / x. Q is t P(t) with t = 1 / (1 + 0.35 x) and P of degree 8, fitted here for the least relative error over x
+// = 0 .. 14 (2^-24.9; past that e is 0 in fp32). The exponent is taken in two parts, since its rounding alone would
+// move e by x^2 2^-25. Together within 2^-21 of itself (rounded stepwise on the host over 400000 z).
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     constexpr float kHalfLog2E = 0.72134752044448170f, kRest = static_cast<float>(0.72134752044448170368 - kHalfLog2E);
     const float x = fminf(fabsf(z), 15.0f);
@@ -116,11 +116,12 @@ __device__ __forceinline__ uint2 pack4(f32x4 y) {
                       T::store(y[2]) | (static_cast<uint32_t>(T::store(y[3])) << 16));
 }
 
-// The epilogue of 4 consecutive columns col .. col + 3 of one output row, the first `valid` of which exist: bias, the sums
-// before the activation stored, activation, residual. z: the sums (SwiGLU: the gate's, u the up rows'). `whole`: all
-// four are there and aligned, so they are one access.
+// The epilogue of 4 consecutive columns col .. col + 3 of one output row, the first `valid` of which exist: bias, the
+// sums before the activation stored, activation, residual. z: the sums (SwiGLU: the gate's, u the up rows'). `whole`:
+// all four are there and aligned, so they are one access.
 template <typename T, bool SWIGLU>
-__device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col, int valid, bool whole, f32x4 z, f32x4 u) {
+__device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col, int valid, bool whole, f32x4 z,
+                                         f32x4 u) {
     if (!SWIGLU && g.factor) z *= *g.factor;
     if (g.bias) {
 #pragma unroll
@@ -204,9 +205,9 @@ __device__ __forceinline__ bool whole_lines(const GemmArgs& g, bool vec) {
     return vec && !g.out_f32 && g.n % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
 }
 
-// 16 rows of a wave's sums on their way to memory. They pass through a piece of LDS that is the wave's own, 16 rows x NB
-// blocks of 16 columns of fp32 (SwiGLU: the first half gate, the second up), so that a lane has 8 columns of one row and
-// what the epilogue reads and writes is whole lines. Granule G (16 bytes) of row r stands at G ^ r.
+// 16 rows of a wave's sums on their way to memory. They pass through a piece of LDS that is the wave's own, 16 rows x
+// NB blocks of 16 columns of fp32 (SwiGLU: the first half gate, the second up), so that a lane has 8 columns of one row
+// and what the epilogue reads and writes is whole lines. Granule G (16 bytes) of row r stands at G ^ r.
 template <int NB>
 __device__ __forceinline__ void put_block(float* stg, int row16, int kg, int j, f32x4 v) {
     *reinterpret_cast<f32x4*>(stg + (row16 * NB * 4 + ((j * 4 + kg) ^ (NB == 4 ? row16 : row16 % (NB * 4)))) * 4) = v;
@@ -248,10 +249,11 @@ __device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg,
 }
 
 // ds_read_b64_tr_b16: 8 bytes per lane, handed out transposed within each 16-lane group (lane i gets element i % 4 of
-// the 8 bytes addressed by lanes 4 j + i / 4, j = 0 .. 3). An operand tile stored by k (64 k x 128 rows, 256 bytes a k) gives
-// a fragment of 16 rows and 32 k as two such reads, 4 k each. These read N fragments for both 32-k steps of a stage,
-// addr[n] being the lane's address at its first k. Inline assembly, with the wait in the same block: at the builtin the
-// compiler waits for every direct-to-LDS copy in flight (256 x 256 tiles, T = 8192: 1195 us with that wait).
+// the 8 bytes addressed by lanes 4 j + i / 4, j = 0 .. 3). An operand tile stored by k (64 k x 128 rows, 256 bytes a k)
+// gives a fragment of 16 rows and 32 k as two such reads, 4 k each. These read N fragments for both 32-k steps of a
+// stage, addr[n] being the lane's address at its first k. Inline assembly, with the wait in the same block: at the
+// builtin the compiler waits for every direct-to-LDS copy in flight (256 x 256 tiles, T = 8192: 1195 us with that
+// wait).
 __device__ __forceinline__ void read_transposed(const uint32_t (&addr)[4], s16x8 (&f)[2][4]) {
     s16x4 v[4][4];
     asm volatile(
@@ -293,8 +295,8 @@ __device__ __forceinline__ void read_transposed(const uint32_t (&addr)[2], s16x8
         for (int n = 0; n < 2; ++n)
             f[kk][n] = __builtin_shufflevector(v[n][2 * kk], v[n][2 * kk + 1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// The lane's address in such a tile of the fragment of rows r0 .. r0 + 15 (r0 a multiple of 16) at the first k. The 32-byte
-// pairs of a k stand at pair ^ f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2, which depends on the lane alone here.
+// The lane's address in such a tile of the fragment of rows r0 .. r0 + 15 (r0 a multiple of 16) at the first k. The
+// 32-byte pairs of a k stand at pair ^ f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2, which depends on the lane alone here.
 __device__ __forceinline__ uint32_t transposed_address(const uint16_t* tile, int r0, int lane) {
     const int kg = lane >> 4, j = (lane & 15) >> 2, q = lane & 3, f = (j | ((kg & 1) << 2)) << 1;
     const uint16_t* p = tile + (kg * 8 + j) * 128 + (((r0 / 8 + (q >> 1)) ^ f) * 8) + (q & 1) * 4;
@@ -323,8 +325,9 @@ __device__ __forceinline__ void column_sums(const float* __restrict__ part, uint
     out[c] = T::store(s);
 }
 
-// 8 values of a row from p on, of which `valid` exist (zeros past them); any alignment. `before`: values of the row that
-// stand before p. A row's end is the 8 values that end there, moved down: one load, where single ones wait for each other.
+// 8 values of a row from p on, of which `valid` exist (zeros past them); any alignment. `before`: values of the row
+// that stand before p. A row's end is the 8 values that end there, moved down: one load, where single ones wait for
+// each other.
 __device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid, int before) {
     typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));
     typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));

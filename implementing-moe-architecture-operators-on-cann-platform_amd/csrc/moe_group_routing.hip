@@ -6,23 +6,24 @@
 //   the K best c among them in descending order, ties to the lowest index; w = scale * s, over the K's sum if asked
 // An expert whose logit or c is NaN or -inf is not available; picks with no expert left are id -1, weight 0.
 //
-// The choice is the definition's, not fp32's: without a bias experts are compared by their logits, which order the scores
-// exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where a group that stays and one that
-// does not are nearer than theirs (group_error), the row's groups are scored again in float64; where two neighbours among
-// its picks are, the picks go on past the K-th until a clear gap and are put in order by their float64 values. That is
-// some rows in a hundred, but a launch waits for its slowest wave: a float64 copy of the whole choice, whose code is
-// never in the instruction cache when it is needed, cost 9 us. Where kMore picks more leave no gap (equal scores, biases
-// that leave few bits for the scores), the K best of the row are taken by their float64 values, one maximum of the wave
-// each: calls with 256 equal scores a row take 10.7 us at T = 1 and 43 at T = 16384, where picking and ordering all of them
-// took 157 and 660 (with 8 groups 16.2 and 75, before 62 and 240).
+// The choice is the definition's, not fp32's: without a bias experts are compared by their logits, which order the
+// scores exactly; with one, c is computed in fp32 with a bound on its error (gap_limit). Where a group that stays and
+// one that does not are nearer than theirs (group_error), the row's groups are scored again in float64; where two
+// neighbours among its picks are, the picks go on past the K-th until a clear gap and are put in order by their float64
+// values. That is some rows in a hundred, but a launch waits for its slowest wave: a float64 copy of the whole choice,
+// whose code is never in the instruction cache when it is needed, cost 9 us. Where kMore picks more leave no gap (equal
+// scores, biases that leave few bits for the scores), the K best of the row are taken by their float64 values, one
+// maximum of the wave each: calls with 256 equal scores a row take 10.7 us at T = 1 and 43 at T = 16384, where picking
+// and ordering all of them took 157 and 660 (with 8 groups 16.2 and 75, before 62 and 240).
 //
-// A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers; few
-// tokens of many experts have a wave each. A pick is the maximum over the lane (max3) and over the row (4 DPP steps), and
-// its removal: 16 compares and 16 selects. Where the key's low 8 bits can hold the expert, the maximum names the pick: ~50
-// instructions for 4 tokens. fp32 logits without a bias need all of their bits: the lowest index that has the maximum is
-// searched, ~95 instructions. Group scores go through LDS, one lane per (token, group). Vector instructions bound the kernel (T = 16384, E = 256, K = 8, fp32
-// logits: 10.3 us without bias and groups, 17 us with a bias and 4 of 8 groups by their two best, of which a copy of the
-// logits is 4 us; the search in place of the key's bits 21 us). At T = 1 the one wave's chain takes 5.8 us.
+// A wave has 4 tokens, 16 lanes (a DPP row) each, up to 16 experts a lane in registers as order-preserving integers;
+// few tokens of many experts have a wave each. A pick is the maximum over the lane (max3) and over the row (4 DPP
+// steps), and its removal: 16 compares and 16 selects. Where the key's low 8 bits can hold the expert, the maximum
+// names the pick: ~50 instructions for 4 tokens. fp32 logits without a bias need all of their bits: the lowest index
+// that has the maximum is searched, ~95 instructions. Group scores go through LDS, one lane per (token, group). Vector
+// instructions bound the kernel (T = 16384, E = 256, K = 8, fp32 logits: 10.3 us without bias and groups, 17 us with a
+// bias and 4 of 8 groups by their two best, of which a copy of the logits is 4 us; the search in place of the key's
+// bits 21 us). At T = 1 the one wave's chain takes 6 us.
 #include "moe_device.h"
 #include "moe_launch.h"
 #include "moe_ops.h"
@@ -89,7 +90,8 @@ __device__ __forceinline__ void load4(const void* p, int64_t i, float* v) {
     }
 }
 
-// All-reduce over the LANES lanes of a token: a DPP row of 16 by rotations; of a whole wave the rows' four results after that
+// All-reduce over the LANES lanes of a token: a DPP row of 16 by rotations; of a whole wave the rows' four results
+// after that
 template <int CTRL>
 __device__ __forceinline__ int dpp(int v) {
     return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
@@ -119,7 +121,9 @@ __device__ __forceinline__ double row_sum(double v) {
 }
 template <int LANES>
 __device__ __forceinline__ float row_sum_f(float v) {
-    auto turned = [](float x, auto ctrl) { return __builtin_bit_cast(float, dpp<decltype(ctrl)::value>(__builtin_bit_cast(int, x))); };
+    auto turned = [](float x, auto ctrl) {
+        return __builtin_bit_cast(float, dpp<decltype(ctrl)::value>(__builtin_bit_cast(int, x)));
+    };
     v += turned(v, std::integral_constant<int, 0x128>());
     v += turned(v, std::integral_constant<int, 0x124>());
     v += turned(v, std::integral_constant<int, 0x122>());
@@ -166,15 +170,15 @@ __device__ __forceinline__ int key_of(float v) {
 __device__ __forceinline__ float key_value(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
 
 // Two fp32 values of c that are nearer than this may stand the other way round. With e = 2^-24: exp2 and
-// rcp are within 2 e, the argument's rounding moves e^-l by |l| 1.5 e relative and s (1 - s) |l| < 0.23, so a sigmoid is
-// within 8 e; a softmax score, with a sum of 20 roundings, within 64 e of the row's largest score; adding the bias
+// rcp are within 2 e, the argument's rounding moves e^-l by |l| 1.5 e relative and s (1 - s) |l| < 0.23, so a sigmoid
+// is within 8 e; a softmax score, with a sum of 20 roundings, within 64 e of the row's largest score; adding the bias
 // rounds by e |c|. The limit is four such errors.
 __device__ __forceinline__ float gap_limit(bool sigmoid, float s_max, float c) {
     return (sigmoid ? 32.0f : 256.0f * s_max) * 0x1p-24f + fabsf(c) * 0x1p-21f;
 }
-// How far an fp32 group score may be from the definition's. It is the sum of two c, a and b, which may cancel: its error is
-// that of the terms, two scores' and, with the sum's own rounding, at most 2 e (|a| + |b|), not one of the sum's size
-// (biases of +-40 leave sums below 1 that are 4e-6 off). size: |a| + |b|, counted twice.
+// How far an fp32 group score may be from the definition's. It is the sum of two c, a and b, which may cancel: its
+// error is that of the terms, two scores' and, with the sum's own rounding, at most 2 e (|a| + |b|), not one of the
+// sum's size (biases of +-40 leave sums below 1 that are 4e-6 off). size: |a| + |b|, counted twice.
 __device__ __forceinline__ float group_error(bool sigmoid, float s_max, float size) {
     return (sigmoid ? 16.0f : 128.0f * s_max) * 0x1p-24f + size * 0x1p-22f;
 }
@@ -227,7 +231,8 @@ __device__ __forceinline__ void load_logits(const void* p, int64_t at, int E, in
     }
 }
 
-// c (what groups are scored by) of all experts of row t in float64, by the whole wave, to cs [E]; -inf where not available
+// c (what groups are scored by) of all experts of row t in float64, by the whole wave, to cs [E]; -inf where not
+// available
 template <typename L>
 __device__ __forceinline__ void exact_scores(const GroupRouting& r, int64_t t, double* cs) {
     const int lane = lane_id(), E = r.E;
@@ -555,8 +560,8 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         __syncthreads();
     }
     if (!valid) return;
-    // Weights in float64: K values of a row. Renormalised, the scores are taken relative to the largest of the picks: their
-    // ratios hold where the scores themselves would underflow.
+    // Weights in float64: K values of a row. Renormalised, the scores are taken relative to the largest of the picks:
+    // their ratios hold where the scores themselves would underflow.
     const uint16_t* my = pick + tok * E;
     double* part = parts + tok * K;
     int ref_key = kGone;
@@ -570,7 +575,9 @@ __global__ __launch_bounds__(kWave) void group_routing_kernel(GroupRouting r, in
         }
         ref_key = row_max_i<LANES>(ref_key);
     }
-    const double ref = r.renormalize ? static_cast<double>(key_value(ref_key)) : r.sigmoid ? 0.0 : static_cast<double>(top);
+    const double ref = r.renormalize ? static_cast<double>(key_value(ref_key))
+                       : r.sigmoid   ? 0.0
+                                     : static_cast<double>(top);
     double total = 0.0;
     for (int k = l; k < K; k += LANES) {
         double p = 0.0;
@@ -613,12 +620,12 @@ __device__ __forceinline__ void store4_logits(void* p, int64_t i, const float* v
 // Gradient of the weights of `ids` to the logits. p = s / sum of the K chosen s, g = grad_w, all times scale:
 //   renormalised  softmax: dl_k = p_k (g_k - sum g p)          sigmoid: the same times (1 - s_k)
 //   not           sigmoid: dl_k = g_k s_k (1 - s_k)            softmax: dl_e = s_e (g_e [e chosen] - sum g s)
-// Where one expert has nearly all of a row, g_k nearly is that sum, and the difference is made of the other picks' terms:
-// scores are fp32, relative to the largest, their sums, the mean and the difference float64. The scale comes last, so that
-// g is exact; one renormalised weight is constant, and its gradient 0, since g s / s is g.
-// Bound by its bytes (T E written, and read in the last form; in the others only the picks' logits are read). 16 lanes have
-// a token, a wave four. A lane has every 16th pick; their terms are added into a row of LDS one after another, so an id
-// that a caller's list holds twice adds up in a fixed order, and the row leaves in whole vectors.
+// Where one expert has nearly all of a row, g_k nearly is that sum, and the difference is made of the other picks'
+// terms: scores are fp32, relative to the largest, their sums, the mean and the difference float64. The scale comes
+// last, so that g is exact; one renormalised weight is constant, and its gradient 0, since g s / s is g.
+// Bound by its bytes (T E written, and read in the last form; in the others only the picks' logits are read). 16 lanes
+// have a token, a wave four. A lane has every 16th pick; their terms are added into a row of LDS one after another, so
+// an id that a caller's list holds twice adds up in a fixed order, and the row leaves in whole vectors.
 template <typename L, int C, bool VEC>
 __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting r, const void* __restrict__ grad_w,
                                                                    const int32_t* __restrict__ ids,
@@ -719,7 +726,8 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         if (softmax_all) {
             d = p.g;
         } else if (p.id >= 0) {
-            d = static_cast<float>(scale * (static_cast<double>(p.g) - mean) * (static_cast<double>(score(p.x)) * norm));
+            const double pk = static_cast<double>(score(p.x)) * norm;
+            d = static_cast<float>(scale * (static_cast<double>(p.g) - mean) * pk);
             if (r.sigmoid) d *= expf(fminf(-p.x, 0.0f)) / (1.0f + expf(-fabsf(p.x)));  // 1 - s
         }
         for (int i = 0; i < kRow && k0 + i < K; ++i) {
@@ -750,9 +758,9 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
     }
 }
 
-// Up to two rows a SIMD a token of more than 64 experts has a wave, whose chain is shorter: E = 256 with bias and groups,
-// T = 1 5.8 us (a DPP row 7.2), T = 2048 8.8 (10.5), T = 4096 10.8 (11.6), there without a bias 9.4 (7.9). At 64 experts
-// both take 4.9 us at T = 1 and the DPP row less from there on.
+// Up to two rows a SIMD a token of more than 64 experts has a wave, whose chain is shorter: E = 256 with bias and
+// groups, T = 1 5.8 us (a DPP row 7.2), T = 2048 8.8 (10.5), T = 4096 10.8 (11.6), there without a bias 9.4 (7.9). At
+// 64 experts both take 4.9 us at T = 1 and the DPP row less from there on.
 constexpr int64_t kWaveRows = 2048;
 
 // Rows of 4-expert pieces that one load can read
@@ -791,8 +799,8 @@ hipError_t run_grad_vec(const GroupRouting& r, const void* gw, const int32_t* id
 }
 template <typename L, int C>
 hipError_t run_grad(const GroupRouting& r, const void* gw, const int32_t* ids, void* gl, hipStream_t stream) {
-    return vector_logits(r) && (reinterpret_cast<uintptr_t>(gl) & 15) == 0 ? run_grad_vec<L, C, true>(r, gw, ids, gl, stream)
-                                                                            : run_grad_vec<L, C, false>(r, gw, ids, gl, stream);
+    const bool vec = vector_logits(r) && (reinterpret_cast<uintptr_t>(gl) & 15) == 0;
+    return vec ? run_grad_vec<L, C, true>(r, gw, ids, gl, stream) : run_grad_vec<L, C, false>(r, gw, ids, gl, stream);
 }
 
 template <typename F>

@@ -183,8 +183,8 @@ struct GroupRouting {
     bool sigmoid, renormalize;
     float scale;
     int32_t weights_type;  // moe_dtype
-    // e / (E / groups) of an expert e < 256 is e * size_inverse >> 16: size_inverse = ceil(2^16 / size) is off by less than
-    // 1, so the product by less than 2^8, below 2^16 / size
+    // e / (E / groups) of an expert e < 256 is e * size_inverse >> 16: size_inverse = ceil(2^16 / size) is off by less
+    // than 1, so the product by less than 2^8, below 2^16 / size
     int size_inverse;
 };
 hipError_t launch_group_routing(const GroupRouting& r, int32_t* ids, void* weights, hipStream_t stream);
@@ -195,8 +195,8 @@ hipError_t launch_group_routing_grad(const GroupRouting& r, const void* grad_wei
 // ---- dense products (moe_linear*.hip) ----
 enum Activation { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActSwiglu = 5 };
 // dz = dy * act'(pre) with rows of ldz (zeros past Z); part (null: not wanted) gets the column sums of
-// act_grad_row_blocks(T, Z) blocks of rows, Z floats each; dz null: the sums alone. peaks (null: dz is not scaled): room for
-// kGradPeaks + 1 floats; dz is multiplied by a power of two, whose inverse peaks[kGradPeaks] receives.
+// act_grad_row_blocks(T, Z) blocks of rows, Z floats each; dz null: the sums alone. peaks (null: dz is not scaled):
+// room for kGradPeaks + 1 floats; dz is multiplied by a power of two, whose inverse peaks[kGradPeaks] receives.
 constexpr int kGradPeaks = 256;
 struct ActGrad {
     const void* dy;  // rows ldy elements apart: fp32 where dy_f32 is set, else the operands' type

@@ -5,10 +5,11 @@
 //   forward    P = x  (by rows), Q = W (by rows, or by k when W is a transposed view)
 //   grad_x     P = dz (by rows), Q = W read the other way round
 //   grad_W     P = dz (by k: its T rows are the reduction), Q = x (by k)
-// The tiles here, 32 to 256 rows by 128, are for products that do not fill the GPU with 256 x 256 ones; where even these
-// leave CUs idle the product is split over k and a second launch adds the pieces in order. What bounds them is the copies
-// into LDS: 24 KB a stage and two workgroups a CU, 0.65 us for both (64 rows), is 19 TB/s over the GPU, and 128 and 256
-// rows come to 18 and 13 TB/s. So the taller tile wins until the pieces' sums cost more than its reads save.
+// The tiles here, 32 to 256 rows by 128, are for products that do not fill the GPU with 256 x 256 ones; where even
+// these leave CUs idle the product is split over k and a second launch adds the pieces in order. What bounds them is
+// the copies into LDS: 24 KB a stage and two workgroups a CU, 0.65 us for both (64 rows), is 19 TB/s over the GPU, and
+// 128 and 256 rows come to 18 and 13 TB/s. So the taller tile wins until the pieces' sums cost more than its reads
+// save.
 //   T = 4097, H = 7168, N = 256 (130 tiles of 64 rows in 3 pieces): 25.6 + 4.2 us, of which x from HBM alone is 11
 //   both gradients' products at T = 1000, H = 1056, N = 733, one launch of 256 workgroups: 10.9 + 3.2 us
 #include "moe_gemm.h"
@@ -72,12 +73,14 @@ __device__ __forceinline__ void read_fragments(const uint16_t* tile, int r0, int
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int n = 0; n < N; ++n)
-                f[kk][n] = *reinterpret_cast<const s16x8*>(tile + (r0 + n * 16 + row16) * kBK + (((kk * 4 + kg) ^ sw) * 8));
+                f[kk][n] = *reinterpret_cast<const s16x8*>(tile + (r0 + n * 16 + row16) * kBK +
+                                                           (((kk * 4 + kg) ^ sw) * 8));
     }
 }
 
 // 8 consecutive elements (of a row's k, or by k of rows) from an operand of any alignment, zeros past its end
-__device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, bool by_k, int row, int k, int rows, int k1) {
+__device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, bool by_k, int row, int k, int rows,
+                                              int k1) {
     const int valid = row >= rows || k >= k1 ? 0 : by_k ? rows - row : k1 - k;
     return load8(p + (by_k ? static_cast<int64_t>(k) * ld + row : static_cast<int64_t>(row) * ld + k), valid,
                  by_k ? row : k);
@@ -88,7 +91,8 @@ __device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, boo
 // granules come through registers (loads of any alignment) and are written to the same layout.
 // block of grid: this product's share of the launch, grid a multiple of the XCDs.
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
-__device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntiles, int block, int grid, uint16_t* lds) {
+__device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntiles, int block, int grid,
+                                         uint16_t* lds) {
     constexpr int NS = ring_stages(BM);
     constexpr int WAVES = mid_waves(BM);
     constexpr int WM = BM >= 128 ? BM / 64 : 1, WN = WAVES / WM;  // waves along m and n
@@ -100,8 +104,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
     const int wm = wave / WN, wn = wave % WN;
     const int row16 = lane & 15, kg = lane >> 4;
 
-    // Workgroups go round-robin over the XCDs; each XCD takes a contiguous run of the items. The tiles that read the same
-    // piece of the larger operand are neighbours in it, so that piece reaches that XCD's L2 once.
+    // Workgroups go round-robin over the XCDs; each XCD takes a contiguous run of the items. The tiles that read the
+    // same piece of the larger operand are neighbours in it, so that piece reaches that XCD's L2 once.
     const int item = block % kXcds * (grid / kXcds) + block / kXcds;
     if (item >= mtiles * ntiles * g.splits) return;
     const bool n_first = mtiles > ntiles;
@@ -134,9 +138,9 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
         qrow[c] = a.row;
         qel[c] = a.el;
     }
-    // Byte offsets of this lane's granules, relative to (by rows) the tile's first row, (by k) the stage's first k; past
-    // every buffer where the operand has no such row. 64-bit arithmetic is in the bases alone, so an operand may be
-    // larger than 4 GiB. By rows the k offset of a stage is the instruction's scalar one.
+    // Byte offsets of this lane's granules, relative to (by rows) the tile's first row, (by k) the stage's first k;
+    // past every buffer where the operand has no such row. 64-bit arithmetic is in the bases alone, so an operand may
+    // be larger than 4 GiB. By rows the k offset of a stage is the instruction's scalar one.
     uint32_t poff[PC], qoff[QC];
     if (DIRECT) {
         const uint32_t ppitch = static_cast<uint32_t>(g.ldp) * 2, qpitch = static_cast<uint32_t>(g.ldq) * 2;
@@ -148,7 +152,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 #pragma unroll
         for (int c = 0; c < QC; ++c) {
             const int tr = QK ? qel[c] : qrow[c], col = q_col(tr);
-            const uint32_t off = QK ? qrow[c] * qpitch + (col + (q_up(tr) ? g.up : 0)) * 2u : (col - n0) * qpitch + qel[c] * 2u;
+            const uint32_t off = QK ? qrow[c] * qpitch + (col + (q_up(tr) ? g.up : 0)) * 2u
+                                    : (col - n0) * qpitch + qel[c] * 2u;
             qoff[c] = col < g.n ? off : kPastEnd;
         }
     }
@@ -160,7 +165,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
         if (DIRECT) {
             const int left = k1 - kc;  // granules from here on are zeros
             const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint16_t*>(PK ? pbase + static_cast<int64_t>(kc) * g.ldp : pbase), 0, 0x7fffffff, 0x00020000);
+                const_cast<uint16_t*>(PK ? pbase + static_cast<int64_t>(kc) * g.ldp : pbase), 0, 0x7fffffff,
+                0x00020000);
 #pragma unroll
             for (int c = 0; c < PC; ++c)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -188,7 +194,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 #pragma unroll
             for (int c = 0; c < QC; ++c) {
                 const int tr = QK ? qel[c] : qrow[c], up = q_up(tr) ? g.up : 0;
-                const s16x8 v = load_granule(g.q, g.ldq, QK, q_col(tr) + up, kc + (QK ? qrow[c] : qel[c]), g.n + up, k1);
+                const s16x8 v =
+                    load_granule(g.q, g.ldq, QK, q_col(tr) + up, kc + (QK ? qrow[c] : qel[c]), g.n + up, k1);
                 *reinterpret_cast<s16x8*>(slot + BM * kBK + (wave * QC + c) * 512 + lane * 8) = v;
             }
         }
@@ -265,7 +272,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 }
 
 template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
-__global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_mid_kernel(GemmArgs g, int mtiles, int ntiles) {
+__global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_mid_kernel(
+    GemmArgs g, int mtiles, int ntiles) {
     extern __shared__ __align__(16) uint16_t lds[];
     gemm_mid<T, PK, QK, BM, SWIGLU, DIRECT>(g, mtiles, ntiles, static_cast<int>(blockIdx.x),
                                             static_cast<int>(gridDim.x), lds);
@@ -274,7 +282,8 @@ __global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu
 // Both gradient products in one launch: neither needs the other, and small ones leave the GPU half empty. The first
 // x_blocks workgroups have grad_x.
 template <typename T, bool QK, int BM>
-__global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_pair_kernel(GemmArgs x, GemmArgs w, int x_blocks) {
+__global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_pair_kernel(
+    GemmArgs x, GemmArgs w, int x_blocks) {
     extern __shared__ __align__(16) uint16_t lds[];
     const int block = static_cast<int>(blockIdx.x);
     if (block < x_blocks)
@@ -293,8 +302,9 @@ template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
 hipError_t run_mid(const GemmArgs& g, hipStream_t stream) {
     constexpr int kCols = SWIGLU ? kBN / 2 : kBN;
     TraceScope trace("moe_linear_gemm", stream);
-    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT><<<mid_grid(g, BM, kCols), mid_threads(BM), mid_lds_bytes(BM), stream>>>(
-        g, (g.m + BM - 1) / BM, (g.n + kCols - 1) / kCols);
+    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT>
+        <<<mid_grid(g, BM, kCols), mid_threads(BM), mid_lds_bytes(BM), stream>>>(g, (g.m + BM - 1) / BM,
+                                                                                (g.n + kCols - 1) / kCols);
     return hipGetLastError();
 }
 

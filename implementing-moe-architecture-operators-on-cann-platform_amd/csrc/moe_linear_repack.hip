@@ -1,8 +1,9 @@
 // moe_linear_repack.hip -- operands whose rows are no multiple of 16 bytes, laid out anew for the dense products.
 //
 // The products copy 16 bytes at a time straight into LDS, so a row of 8 n + r elements cannot be read in place from any
-// row but the first. One pass copies such operands into the workspace with their rows padded with zeros to whole granules;
-// the fast kernels then run as for any other size. The pass moves each byte twice and the launch takes about 3 us.
+// row but the first. One pass copies such operands into the workspace with their rows padded with zeros to whole
+// granules; the fast kernels then run as for any other size. The pass moves each byte twice and the launch takes about
+// 3 us.
 #include "moe_gemm.h"
 
 namespace moe {
@@ -23,7 +24,8 @@ __global__ __launch_bounds__(kThreads) void repack_kernel(RepackArgs a, int64_t 
             if (at >= 0 && at < count) {
                 const int64_t row = at / per;
                 const int col = static_cast<int>(at - row * per) * 8;
-                *reinterpret_cast<s16x8*>(r.dst + row * r.dst_ld + col) = load8(r.src + row * r.src_ld + col, r.cols - col, col);
+                *reinterpret_cast<s16x8*>(r.dst + row * r.dst_ld + col) =
+                    load8(r.src + row * r.src_ld + col, r.cols - col, col);
             }
             first += count;
         }

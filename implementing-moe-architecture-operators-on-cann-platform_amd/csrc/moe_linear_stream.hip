@@ -1,15 +1,16 @@
 // moe_linear_stream.hip -- the dense product of few rows (serving's single tokens and small batches): weight streaming.
 //
 // C[m][n] = sum_k P[m][k] Q[n][k], both operands by rows, m <= 64. The weights are read once and bound it: at T = 1 the
-// gate and up rows of a dense expert (H = 7168, N = 2048) are 59 MB for 59 MFLOP, 10.7 us (5.5 TB/s). From 16 rows on x,
-// which every tile reads again from L2, costs as much as the weights: T = 64, H = 2048, N = 7168 11.6 us, 29 MB of weights
-// and 58 MB of x through the CUs' copy paths.
+// gate and up rows of a dense expert (H = 7168, N = 2048) are 59 MB for 59 MFLOP, 10.7 us (5.5 TB/s). From 16 rows on
+// x, which every tile reads again from L2, adds to it. T = 64, N = 7168 takes 11.3, 19.6 and 32.4 us at H = 2048, 4096
+// and 8192: weights and x come in at 13.8 TB/s together (59 + 117 MB in the last 12.8 us), and 5 us are the launch, the
+// first copies and the sums. T = 16 there: 25.7 us at H = 8192, the weights at 6.2 TB/s in the last 9.4 us.
 //   work      a tile is 16 or 32 weight rows (SwiGLU: half gate, half the matching up rows) over the whole k, and its
-//             workgroup's waves share k: wave w takes the 64-k pieces w, w + W, ... Their sums meet in LDS, added in wave
-//             order, and go through the epilogue: one launch, no partial sums in memory.
-//   copies    each wave has its own LDS ring and fills it straight from global memory, 8 rows x 128 bytes an instruction;
-//             nobody else reads it, so the main loop has no barrier. Loaded into registers in fragment order (16 rows x
-//             64 bytes an instruction) the same work ran at 4.2 TB/s.
+//             workgroup's waves share k: wave w takes the 64-k pieces w, w + W, ... Their sums meet in LDS, added in
+//             wave order, and go through the epilogue: one launch, no partial sums in memory.
+//   copies    each wave has its own LDS ring and fills it straight from global memory, 8 rows x 128 bytes an
+//             instruction; nobody else reads it, so the main loop has no barrier. Loaded into registers in fragment
+//             order (16 rows x 64 bytes an instruction) the same work ran at 4.2 TB/s.
 //   persistent  a workgroup per CU walks its tiles and the rings run on across them, so the next tile's weights are in
 //             flight while the sums of this one are added.
 // Rows past the last and k past the end read zeros without memory traffic.
@@ -123,7 +124,8 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
             }
             slot = slot + 1 == DEPTH ? 0 : slot + 1;
         }
-        // acc[q][b]: D[Q row 4 kg + r of block q][P row row16 of block b]. Granule G (4 Q rows) of P row r stands at G ^ r.
+        // acc[q][b]: D[Q row 4 kg + r of block q][P row row16 of block b]. Granule G (4 Q rows) of P row r stands at G
+        // ^ r.
         constexpr int kGranules = 4 * QB, kRows = 16 * Lds::kPassBlocks;
 #pragma unroll
         for (int b0 = 0; b0 < MB; b0 += Lds::kPassBlocks) {
@@ -174,11 +176,11 @@ hipError_t by_rows(int m, int qb, F&& f) {
     return m <= 32 ? f(Int<1>(), Int<2>(), Int<4>(), Int<4>()) : f(Int<1>(), Int<4>(), Int<4>(), Int<3>());
 }
 
-// Blocks of 16 weight rows in a tile. Two halve what a tile reads of x, for 1.45 times the time of a tile of one, so they
-// pay where they save rounds of the GPU: T = 64, H = 2048, N = 7168 (2 rounds -> 1) 14.5 -> 11.6 us, H = 18432 100 -> 71.5;
-// H = 4096, N = 4096 (1 round either way) 13.7 -> 16.6. Up to 16 rows x costs little, and tiles of one keep more
-// copies in flight over several rounds: T = 1, N = 16384, H = 4096 (4 rounds -> 2) 23.3 -> 26.5 us; into a single round
-// two are as fast or faster there too (T = 16, N = 7168 9.1 -> 8.2 us).
+// Blocks of 16 weight rows in a tile. Two halve what a tile reads of x, for 1.45 times the time of a tile of one, so
+// they pay where they save rounds of the GPU: T = 64, H = 2048, N = 7168 (2 rounds -> 1) 14.5 -> 11.6 us, H = 18432 100
+// -> 71.5; H = 4096, N = 4096 (1 round either way) 13.7 -> 16.6. Up to 16 rows x costs little, and tiles of one keep
+// more copies in flight over several rounds: T = 1, N = 16384, H = 4096 (4 rounds -> 2) 23.3 -> 26.5 us; into a single
+// round two are as fast or faster there too (T = 16, N = 7168 9.1 -> 8.2 us).
 int tile_blocks(int m, int64_t rows) {
     constexpr int64_t kCus = 256;
     const int64_t one = ((rows + 15) / 16 + kCus - 1) / kCus, two = ((rows + 31) / 32 + kCus - 1) / kCus;

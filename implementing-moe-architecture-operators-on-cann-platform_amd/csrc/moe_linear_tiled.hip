@@ -1,17 +1,18 @@
 // moe_linear_tiled.hip -- the dense product on 256 x 256 tiles, for the sizes that the matrix cores bound.
 //
 // C[m][n] = sum_k P[m][k] Q[n][k] as in moe_linear.hip, operands that 16-byte copies can read. The main loop is that of
-// the expert GEMMs (moe_ffn_tiled.hip, where its choices are measured): 8 waves (2 x 4) of 128 x 64, two LDS slots of four
-// 16 KB half tiles (P rows 0-127 and 128-255, two halves of Q rows), a stage of 64 k as two pairs of ticks (LDS reads and
-// copies, then 32 MFMAs), waves 4-7 one tick behind waves 0-3, persistent workgroups whose ring runs on across tiles.
-// New here: either operand may be stored by k (a half tile is then 64 k x 128 rows and its fragments come out of
-// ds_read_b64_tr_b16), k of any length (copies past the end read zeros), tiles in bands of 8 m-tiles (the 32 workgroups
-// of an XCD then read 8 + 4 panels a stage, not 32 + 1), and the epilogue of moe_gemm.h.
+// the expert GEMMs (moe_ffn_tiled.hip, where its choices are measured): 8 waves (2 x 4) of 128 x 64, two LDS slots of
+// four 16 KB half tiles (P rows 0-127 and 128-255, two halves of Q rows), a stage of 64 k as two pairs of ticks (LDS
+// reads and copies, then 32 MFMAs), waves 4-7 one tick behind waves 0-3, persistent workgroups whose ring runs on
+// across tiles. New here: either operand may be stored by k (a half tile is then 64 k x 128 rows and its fragments come
+// out of ds_read_b64_tr_b16), k of any length (copies past the end read zeros), tiles in bands of 8 m-tiles (the 32
+// workgroups of an XCD then read 8 + 4 panels a stage, not 32 + 1), and the epilogue of moe_gemm.h.
 //
-// Matrix cores and the clock they leave bound it. T = 16381, H = 2048, N = 2816 SwiGLU bf16: 282-293 us with the epilogue,
-// 1290-1340 TFLOP/s (8192^3 by the library: 1413); grad_x of a T = 8192 step 148 us, 1277 TFLOP/s. grad_weight
-// there has 176 tiles for 256 CUs and takes 200 us: tiles of 256 x 192 (242 of them) took 170 us where these took 177, and
-// 168 to 199 us where these took 137 to 142 on full rounds, so a product is not bound by the CUs it leaves idle.
+// Matrix cores and the clock they leave bound it. T = 16381, H = 2048, N = 2816 SwiGLU bf16: 282-293 us with the
+// epilogue, 1290-1340 TFLOP/s (8192^3 by the library: 1413); grad_x of a T = 8192 step 148 us, 1277 TFLOP/s.
+// grad_weight there has 176 tiles for 256 CUs and takes 200 us: tiles of 256 x 192 (242 of them) took 170 us where
+// these took 177, and 168 to 199 us where these took 137 to 142 on full rounds, so a product is not bound by the CUs it
+// leaves idle.
 #include "moe_gemm.h"
 
 namespace moe {
@@ -48,8 +49,8 @@ struct Tile {
 };
 
 // Where a tile's copies come from. Per half tile wave w issues instructions 2 w and 2 w + 1, each 64 granules of 16
-// bytes: by rows 8 rows of 8 granules, granule g of row r standing at g ^ ((r >> 1) & 7); by k 4 k of 16 granules (8 rows
-// each), granule g of k standing at g ^ (2 f(k)), f(k) = (k & 3) | (k >> 3 & 1) << 2. Offsets are relative to the
+// bytes: by rows 8 rows of 8 granules, granule g of row r standing at g ^ ((r >> 1) & 7); by k 4 k of 16 granules (8
+// rows each), granule g of k standing at g ^ (2 f(k)), f(k) = (k & 3) | (k >> 3 & 1) << 2. Offsets are relative to the
 // tile's first row (by rows) or the stage's first k (by k).
 struct CopyPlan {
     uint32_t po[2][2], qo[2][2];  // [half][instruction]
@@ -120,12 +121,12 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         c.qb[0] = g.q + (QK ? 0 : static_cast<int64_t>(t.n0) * g.ldq);
         c.qb[1] = c.qb[0] + (SWIGLU && !QK ? static_cast<int64_t>(g.up) * g.ldq : 0);
     };
-    // One half tile of stage kc into ring slot q % 2. By rows the k offset is the instruction's scalar one, by k it moves
-    // the base, so an operand may be larger than 4 GiB. Granules from k on read zeros.
+    // One half tile of stage kc into ring slot q % 2. By rows the k offset is the instruction's scalar one, by k it
+    // moves the base, so an operand may be larger than 4 GiB. Granules from k on read zeros.
     const int pgk[2] = {granule_k(PK, 0, lane), granule_k(PK, 1, lane)};
     const int qgk[2] = {granule_k(QK, 0, lane), granule_k(QK, 1, lane)};
-    auto copy = [&](bool by_k, const uint16_t* base, int64_t ld, const uint32_t (&off)[2], const int (&gk)[2], uint16_t* s,
-                    int kc) __attribute__((always_inline)) {
+    auto copy = [&](bool by_k, const uint16_t* base, int64_t ld, const uint32_t (&off)[2], const int (&gk)[2],
+                    uint16_t* s, int kc) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint16_t*>(by_k ? base + static_cast<int64_t>(kc) * kBK * ld : base), 0, 0x7fffffff, 0x00020000);
         const int left = g.k - kc * kBK;
@@ -213,9 +214,9 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         tick_c(acc[1], first);
     };
 
-    // acc[a][b][i][j]: rows a * 128 + wm * 64 + i * 16 + row16, columns of Q half b, 4 consecutive ones from 4 kg on. The 8
-    // blocks of 16 rows share one copy of the epilogue's code: unrolled, its activations are too long for the accumulators
-    // to stay in registers.
+    // acc[a][b][i][j]: rows a * 128 + wm * 64 + i * 16 + row16, columns of Q half b, 4 consecutive ones from 4 kg on.
+    // The 8 blocks of 16 rows share one copy of the epilogue's code: unrolled, its activations are too long for the
+    // accumulators to stay in registers.
     auto epilogue = [&](const Acc (&acc)[2], const Tile& t) __attribute__((always_inline)) {
         const int ln = lane_fresh(), row16 = ln & 15, kg = ln >> 4;
         const bool vec = vector_rows(g), lines = whole_lines(g, vec);

@@ -24,10 +24,10 @@ import torch
 from . import _lib
 from ._lib import MoeError, check, dims
 
-# The current stream without the Stream object that torch.cuda.current_stream() makes on each call, and the allocation on
-# the current device that torch's compiled code uses (0.75 us a tensor, new_empty 1.5): private to torch, so a torch
-# without them takes the public functions. The allocation passes torch's dispatch modes and its filling of new memory under
-# deterministic algorithms by, so it is used where neither is on.
+# The current stream without the Stream object that torch.cuda.current_stream() makes on each call, and the allocation
+# on the current device that torch's compiled code uses (0.75 us a tensor, new_empty 1.5): private to torch, so a torch
+# without them takes the public functions. The allocation passes torch's dispatch modes and its filling of new memory
+# under deterministic algorithms by, so it is used where neither is on.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", None)
 _empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
@@ -481,14 +481,16 @@ def MoeCombineGrad(grad_y: torch.Tensor, expert_out: torch.Tensor, weights: torc
 
 
 def linear_workspace_bytes(T: int, N: int, H: int, activation: str = "none", transposed: bool | None = None) -> int:
-    """Workspace of MoeLinear: of a weight whose rows are contiguous (False), of one stored [H, N] (True), or of either."""
+    """Workspace of MoeLinear: of a weight whose rows are contiguous (transposed False), of one stored [H, N] (True), or
+    of either (None)."""
     lib, act = _lib.load(), _act_code(activation)
     if transposed is None:
         return int(lib.moe_linear_workspace_bytes(T, N, H, act))
     return int(lib.moe_linear_layout_workspace_bytes(T, N, H, act, int(transposed)))
 
 
-def linear_grad_workspace_bytes(T: int, N: int, H: int, activation: str = "none", transposed: bool | None = None) -> int:
+def linear_grad_workspace_bytes(T: int, N: int, H: int, activation: str = "none",
+                                transposed: bool | None = None) -> int:
     """Workspace of MoeLinearGrad, as linear_workspace_bytes, for a grad_y of either type."""
     query, act = _lib.load().moe_linear_grad_f32_workspace_bytes, _act_code(activation)
     return max(int(query(T, N, H, act, int(t))) for t in ((False, True) if transposed is None else (transposed,)))
@@ -510,9 +512,9 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     """act(x[T,H] @ weight[N,H]^T + bias[N]) + residual[T,N] -> y[T,N] of outDtype (x's type, or fp32).
 
     x and weight are fp16 or bf16; x's rows and weight along one of its dimensions must be contiguous (w_gate.t() is a
-    weight). activation: none, relu, gelu, gelu_tanh, silu or swiglu, which takes weight[2N,H] (and bias[2N]), the N gate
-    rows first. residual has y's type. With returnPre -> (y, pre): the sums before the activation, which MoeLinearGrad
-    takes. `workspace` (uint8, >= linear_workspace_bytes) is allocated when not given."""
+    weight). activation: none, relu, gelu, gelu_tanh, silu or swiglu, which takes weight[2N,H] (and bias[2N]), the N
+    gate rows first. residual has y's type. With returnPre -> (y, pre): the sums before the activation, which
+    MoeLinearGrad takes. `workspace` (uint8, >= linear_workspace_bytes) is allocated when not given."""
     act = _act_code(activation)
     dt, dev = _first_float(x, "x", _HALVES, 2)
     dtype = x.dtype
@@ -527,12 +529,12 @@ def MoeLinear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     rp = _matrix(residual, "residual", out, (T, N), dev)
     lib = _lib.load()
     like = _like(x)
-    workspace, wp, wb = _workspace(workspace, lib.moe_linear_layout_workspace_bytes, (T, N, H, act, transposed), like, dev,
-                                   stream)
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_layout_workspace_bytes, (T, N, H, act, transposed), like,
+                                   dev, stream)
     y = _empty(like, stream, (T, N), out)
     pre = _empty(like, stream, (T, Z), dtype) if returnPre else None
-    check(lib.moe_linear_layout(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre), wp,
-                                wb, T, N, H, act, dt, _FLOAT_DT[out], _queue(stream, dev)))
+    check(lib.moe_linear_layout(x.data_ptr(), ldx, weight.data_ptr(), ldw, transposed, bp, rp, y.data_ptr(), _ptr(pre),
+                                wp, wb, T, N, H, act, dt, _FLOAT_DT[out], _queue(stream, dev)))
     return (y, pre) if returnPre else y
 
 
@@ -540,8 +542,8 @@ def MoeLinearGrad(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, p
                   activation: str = "none", gradX: bool = True, gradWeight: bool = True, gradBias: bool = False,
                   workspace: torch.Tensor | None = None, stream=None):
     """The gradient of MoeLinear's y[T,N] (of x's type or, for an fp32 y, fp32) -> (grad_x[T,H], grad_weight[N,H],
-    grad_bias[N]), contiguous, of x's type, None where not asked for. pre is MoeLinear's (needed with an activation). The residual's gradient is
-    grad_y. `workspace` (uint8, >= linear_grad_workspace_bytes) is allocated when not given."""
+    grad_bias[N]), contiguous, of x's type, None where not asked for. pre is MoeLinear's (needed with an activation).
+    The residual's gradient is grad_y. `workspace` (uint8, >= linear_grad_workspace_bytes) is allocated when not given."""
     act = _act_code(activation)
     dt, dev = _first_float(x, "x", _HALVES, 2)
     dtype = x.dtype

@@ -7,8 +7,8 @@ registered under the reference's names, with its attributes, over the same C ABI
     torch.ops.moe_mi355x.MoeExpertFFN(x, expert_ids, weights, expert_weights, intermediateSize=0) -> expert_out
     torch.ops.moe_mi355x.MoeCombine(expert_out, expert_ids, weights, topK=2) -> y
 
-and the operators around the routed experts, with their gradients (MoeCombine has one too; MoeRoutingTopK and MoeExpertFFN
-have none):
+and the operators around the routed experts, with their gradients (MoeCombine has one too; MoeRoutingTopK and
+MoeExpertFFN have none):
 
     torch.ops.moe_mi355x.MoeRoutingGroupTopK(logits, bias, topK, ...) -> (expert_ids, weights)
     torch.ops.moe_mi355x.MoeLinear(x, weight, bias, residual, activation, outDtype, returnPre) -> (y, pre)

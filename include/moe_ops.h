@@ -267,9 +267,9 @@ typedef enum moe_activation {
  *   scores: the lower group). expert_ids are the K best c of the experts that stay, in descending order (equal
  *   c: the lower index). weights = scale * s, divided by the sum of the K chosen s where renormalize is set
  *   (the ratios hold where the scores themselves would underflow). bias only steers the choice.
- *   c is compared beyond fp32: without a bias by the logits, which order the scores, with one in float64. An expert whose logit or c is NaN or -infinity is not available; where a row has fewer
- *   than K available ones the picks left are id -1 and weight 0, which moe_expert_ffn computes as zero rows.
- *   1 <= K <= top_groups * E / groups, E <= 256.
+ *   c is compared beyond fp32: without a bias by the logits, which order the scores, with one in float64. An expert
+ *   whose logit or c is NaN or -infinity is not available; where a row has fewer than K available ones the picks left
+ *   are id -1 and weight 0, which moe_expert_ffn computes as zero rows. 1 <= K <= top_groups * E / groups, E <= 256.
  * ---------------------------------------------------------------------------------------------------- */
 moe_status moe_routing_group_topk(const void* logits, int64_t logits_stride, int32_t logits_type, const float* bias,
                                   int32_t* expert_ids, void* weights, int32_t weights_type, int64_t num_tokens,
@@ -299,12 +299,12 @@ moe_status moe_combine_grad(const uint16_t* grad_y, const uint16_t* expert_out, 
  *   MoeRoutingTopK's w_gate. bias[N] (SwiGLU: [2N]) of dtype, or NULL; residual[T, N] of out_dtype, or NULL; out_dtype
  *   is dtype or float32. pre, if not NULL, receives the sums before the activation, [T, N] (SwiGLU: [T, 2N]) of dtype,
  *   which moe_linear_grad takes. Any sizes from 1; N, H <= 2^20.
- *   Any strides and alignment. 16-byte aligned operands whose strides are multiples of 8 run at full speed. Where H (of a
- *   transposed weight N) is no multiple of 8, x and the weight are first copied with padded rows; other operands that
+ *   Any strides and alignment. 16-byte aligned operands whose strides are multiples of 8 run at full speed. Where H (of
+ *   a transposed weight N) is no multiple of 8, x and the weight are first copied with padded rows; other operands that
  *   16-byte copies cannot read go through registers, at a fraction of the speed. residual may be y itself.
- *   The workspace (moe_linear_workspace_bytes, either layout's; 0 where none is needed; 16-byte aligned) holds fp32 partial sums of a product
- *   split over H and those copies; calls in flight at the same time, captured graphs among them, need one each.
- *   Deterministic: the order of every sum depends on the sizes, strides and alignment alone.
+ *   The workspace (moe_linear_workspace_bytes, either layout's; 0 where none is needed; 16-byte aligned) holds fp32
+ *   partial sums of a product split over H and those copies; calls in flight at the same time, captured graphs among
+ *   them, need one each. Deterministic: the order of every sum depends on the sizes, strides and alignment alone.
  * ---------------------------------------------------------------------------------------------------- */
 size_t moe_linear_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
 moe_status moe_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
@@ -326,8 +326,8 @@ moe_status moe_linear_layout(const void* x, int64_t x_stride, const void* weight
  * moe_linear's (not read without an activation). dz = grad_y * act'(pre) is rounded to dtype for the two products
  * grad_x = dz weight and grad_weight = dz^T x (with float16 values above 65504 become infinite, below 2^-25 zero);
  * grad_bias sums it before that. residual's gradient is grad_y.
- * With T = 0 grad_weight and grad_bias are zeros. The workspace holds dz, column sums, copies with padded rows and partial
- * sums: always needed, by the same rules. */
+ * With T = 0 grad_weight and grad_bias are zeros. The workspace holds dz, column sums, copies with padded rows and
+ * partial sums: always needed, by the same rules. */
 size_t moe_linear_grad_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation);
 moe_status moe_linear_grad(const void* grad_y, int64_t grad_y_stride, const void* x, int64_t x_stride,
                            const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
@@ -344,9 +344,10 @@ moe_status moe_linear_grad_layout(const void* grad_y, int64_t grad_y_stride, con
                                   size_t workspace_bytes, int64_t num_tokens, int64_t n, int64_t hidden_size,
                                   int32_t activation, int32_t dtype, void* stream);
 
-/* The same for the gradient of a float32 result: grad_y is float32, the gradients of dtype. dz is rounded to dtype for the
- * products, with float16 after a multiplication by the power of two that takes its largest finite value to [2^14, 2^15),
- * which the sums are divided by: nothing of grad_y vanishes or overflows but what is 2^-39 of its largest value.
+/* The same for the gradient of a float32 result: grad_y is float32, the gradients of dtype. dz is rounded to dtype for
+ * the products, with float16 after a multiplication by the power of two that takes its largest finite value to
+ * [2^14, 2^15), which the sums are divided by: dz does not overflow, and what vanishes is below 2^-39 of its largest
+ * value.
  * grad_y of any alignment (4 bytes) and row stride. */
 size_t moe_linear_grad_f32_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int32_t activation,
                                            int32_t weight_transposed);
