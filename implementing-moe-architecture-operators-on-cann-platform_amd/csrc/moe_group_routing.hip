@@ -621,8 +621,9 @@ __device__ __forceinline__ void store4_logits(void* p, int64_t i, const float* v
 //   renormalised  softmax: dl_k = p_k (g_k - sum g p)          sigmoid: the same times (1 - s_k)
 //   not           sigmoid: dl_k = g_k s_k (1 - s_k)            softmax: dl_e = s_e (g_e [e chosen] - sum g s)
 // Where one expert has nearly all of a row, g_k nearly is that sum, and the difference is made of the other picks'
-// terms: scores are fp32, relative to the largest, their sums, the mean and the difference float64. The scale comes
-// last, so that g is exact; one renormalised weight is constant, and its gradient 0, since g s / s is g.
+// terms: scores of the picks, their sums, the mean and the difference are float64 (of the whole row fp32). The scale
+// comes last and the picks' scores have 29 bits, so that g s is exact: one renormalised weight is constant, and its
+// gradient is 0, since g s / s is g.
 // Bound by its bytes (T E written, and read in the last form; in the others only the picks' logits are read). 16 lanes
 // have a token, a wave four. A lane has every 16th pick; their terms are added into a row of LDS one after another, so
 // an id that a caller's list holds twice adds up in a fixed order, and the row leaves in whole vectors.
@@ -695,15 +696,23 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         m = row_max_i<kRow>(m);
         top = m == kGone ? 0.0f : key_value(m);
     }
-    auto score = [&](float v) {
-        if (r.sigmoid) return expf(fminf(v, 0.0f) - top) / (1.0f + expf(-fabsf(v)));
-        return v == top ? 1.0f : expf(v - top);
-    };
+    // A pick's score, and for the sigmoid one less it, in LDS until the sums are known: entry k is lane k % 16's alone
+    double2* scores = reinterpret_cast<double2*>(shared + kRowTokens * pitch * 4) + tok * K;
     double total = 0.0, dot = 0.0;  // sums of s and g s over the picks
+#pragma unroll 1
     for (int k = l; k < K; k += kRow) {
         const Pick p = pick_at(k);
         if (p.id < 0) continue;
-        const double sk = static_cast<double>(score(p.x));
+        const double x = static_cast<double>(p.x), at_top = static_cast<double>(top);
+        const double lead = r.sigmoid ? fmin(x, 0.0) : x;
+        double sk = lead == at_top ? 1.0 : exp(lead - at_top), rest = 0.0;
+        if (r.sigmoid) {
+            const double q = exp(-fabs(x));
+            sk /= 1.0 + q;
+            rest = (x >= 0.0 ? q : 1.0) / (1.0 + q);
+        }
+        sk = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, sk) & ~uint64_t{0xffffff});  // 29 bits
+        scores[k] = make_double2(sk, rest);
         total += sk;
         dot += static_cast<double>(p.g) * sk;
     }
@@ -726,9 +735,9 @@ __global__ __launch_bounds__(kWave) void group_routing_grad_kernel(GroupRouting 
         if (softmax_all) {
             d = p.g;
         } else if (p.id >= 0) {
-            const double pk = static_cast<double>(score(p.x)) * norm;
-            d = static_cast<float>(scale * (static_cast<double>(p.g) - mean) * pk);
-            if (r.sigmoid) d *= expf(fminf(-p.x, 0.0f)) / (1.0f + expf(-fabsf(p.x)));  // 1 - s
+            const double2 sk = scores[k0 + l];
+            const double dw = scale * (static_cast<double>(p.g) - mean) * (sk.x * norm);
+            d = static_cast<float>(r.sigmoid ? dw * sk.y : dw);
         }
         for (int i = 0; i < kRow && k0 + i < K; ++i) {
             if (l == i && p.id >= 0) row[p.id] += d;
@@ -792,7 +801,7 @@ hipError_t run_routing(const GroupRouting& r, int32_t* ids, void* weights, hipSt
 template <typename L, int C, bool VEC>
 hipError_t run_grad_vec(const GroupRouting& r, const void* gw, const int32_t* ids, void* gl, hipStream_t stream) {
     TraceScope trace("moe_group_routing_grad", stream);
-    const int lds = kRowTokens * ((r.E + 3) / 4 * 4 + 4) * 4;
+    const int lds = kRowTokens * (((r.E + 3) / 4 * 4 + 4) * 4 + r.K * 16);
     group_routing_grad_kernel<L, C, VEC><<<static_cast<unsigned>((r.T + kRowTokens - 1) / kRowTokens), kWave, lds,
                                            stream>>>(r, gw, ids, gl);
     return hipGetLastError();
