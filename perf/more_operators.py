@@ -209,7 +209,8 @@ def _plain_quantize(v):
     top = v.abs().amax(dim=1, keepdim=True)
     fine = torch.isfinite(top)
     up = torch.where(top < 2.0**-60, 2.0**64, 1.0)  # so that 127 / top stays finite
-    inverse = torch.where(fine & (top > 0), 127.0 / (top * up), 0.0)
+    # a quotient of tensors: torch takes a number over a tensor as the rounded reciprocal times the number
+    inverse = torch.where(fine & (top > 0), top.new_full((), 127.0) / (top * up), 0.0)
     q = torch.round(torch.where(fine, v * up, 0.0) * inverse).to(torch.int8)
     return q, torch.where(fine, top / 127.0, float("nan")).squeeze(1)
 
