@@ -18,6 +18,7 @@ STATUS_NAMES = {
 }
 DT_FLOAT32 = 0
 DT_FLOAT16 = 1
+DT_INT8 = 2
 DT_INT32 = 3
 DT_BFLOAT16 = 27
 
@@ -97,6 +98,15 @@ SIGNATURES = {
     "moe_linear_grad_f32_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64, _I32, _I32]),
     "moe_linear_grad_f32": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64,
                                    _I64, _I32, _I32, _P]),
+    "moe_add_rms_norm": (_I32, [_P, _I64, _P, _I64, _P, _I32, _P, _P, _P, _P, _I64, _I64, _F32, _I32, _P]),
+    "moe_add_rms_norm_grad_workspace_bytes": (C.c_size_t, [_I64, _I64]),
+    "moe_add_rms_norm_grad": (_I32, [_P, _I64, _P, _I64, _P, _I32, _P, _I64, _P, _P, _P, C.c_size_t, _I64, _I64, _F32,
+                                     _I32, _P]),
+    "moe_quantize": (_I32, [_P, _I64, _P, _P, _I64, _I64, _I32, _P]),
+    "moe_permute_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64]),
+    "moe_permute": (_I32, [_P, _I64, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64, _I64, _I64, _I32, _P]),
+    "moe_unpermute": (_I32, [_P, _I64, _P, _P, _I32, _P, _I64, _I64, _I64, _I32, _P]),
+    "moe_unpermute_grad": (_I32, [_P, _I64, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _I32, _P]),
     "moe_trace_enable": (_I32, [_I32]),
     "moe_trace_collect": (_I32, []),
     "moe_trace_get": (_I32, [_I32, C.POINTER(C.c_char_p), _I64P, C.POINTER(C.c_double)]),

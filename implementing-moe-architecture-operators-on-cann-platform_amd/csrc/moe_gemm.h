@@ -13,6 +13,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // 16-bit element types of the products; storage is uint16_t bits everywhere
 struct Half {
+    using Bits = uint16_t;
     static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                       0, 0);
@@ -21,6 +22,7 @@ struct Half {
     static __device__ __forceinline__ uint16_t store(float v) { return f32_to_f16_bits(v); }
 };
 struct Bf16 {
+    using Bits = uint16_t;
     static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);

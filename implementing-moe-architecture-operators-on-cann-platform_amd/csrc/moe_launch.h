@@ -212,6 +212,62 @@ struct ActGrad {
 int act_grad_row_blocks(int64_t T, int Z);
 hipError_t launch_act_grad(const ActGrad& g, hipStream_t stream);
 
+// ---- norm with 8-bit results, rows in 8 bits, their gradient (moe_norm.hip) ----
+struct NormArgs {
+    const void* x;         // rows ldx elements apart
+    const void* residual;  // rows ldr apart, or null
+    const void* gamma;     // [H] of x's type or, with gamma_f32, fp32
+    const void* grad_y;    // gradient: rows ldy apart; y receives the sum's gradient (null: not wanted)
+    const void* grad_sum;  // gradient: rows lds apart, or null
+    int64_t ldx, ldr, ldy, lds;
+    void* y;       // [rows, H] of x's type, or null
+    void* sum;     // [rows, H] of x's type, or null
+    int8_t* q;     // [rows, H], or null
+    float* scale;  // [rows] where q is given
+    float* part;   // gradient: norm_grad_blocks() rows of H column sums, or null
+    int64_t rows;
+    int H;
+    float eps;
+    bool gamma_f32;
+};
+// type: moe_dtype of x. norm: false quantises x itself into q and scale
+hipError_t launch_norm(const NormArgs& n, int type, bool norm, hipStream_t stream);
+constexpr int kNormGradMost = 16384;  // longest row of the gradient
+int norm_grad_blocks(int64_t rows, int H);
+// grad_gamma (of gamma's type) may be null
+hipError_t launch_norm_grad(const NormArgs& n, int type, void* grad_gamma, hipStream_t stream);
+
+// ---- tokens sorted by expert and back (moe_expert_rows.hip) ----
+struct SortArgs {
+    const int32_t* ids;  // [T, K]
+    const void* x;       // [T, H] rows ldx elements apart
+    const float* scale;  // [T] or null
+    void* rows;          // [T K, H]
+    float* row_scale;    // [T K] where scale is given
+    int32_t* offsets;    // [E + 1]
+    int32_t* position;   // [T, K]
+    int32_t* scratch;    // sort_scratch_bytes()
+    int64_t T, ldx;
+    int H, E, K;
+    int bytes;           // of an element
+};
+size_t sort_scratch_bytes(int64_t T, int E, int K);
+hipError_t launch_sort(const SortArgs& s, hipStream_t stream);
+
+struct UnsortArgs {
+    const void* rows;         // [R, H], contiguous
+    const int32_t* position;  // [T, K]
+    const void* weights;      // [T, K] of weights_type, or null: 1
+    const void* grad_y;       // gradient: [T, H], rows ldy elements apart
+    void* y;                  // [T, H]; gradient: grad_rows [R, H]
+    void* grad_weights;       // gradient: [T, K] of weights_type, null without weights
+    int64_t T, R, ldy;
+    int H, K;
+    int type, weights_type;  // moe_dtype
+};
+hipError_t launch_unsort(const UnsortArgs& u, hipStream_t stream);
+hipError_t launch_unsort_grad(const UnsortArgs& u, hipStream_t stream);
+
 // ---- synthetic inputs / calibration (moe_synth.hip) ----
 hipError_t launch_synth_normal_f16(uint16_t* out, uint64_t n, uint64_t seed, uint64_t stream_id, double sigma_a,
                                    double sigma_b, uint64_t period, uint64_t split, hipStream_t stream);

@@ -1,0 +1,377 @@
+// moe_norm.hip -- MoeAddRmsNorm, MoeAddRmsNormQuant, MoeAddRmsNormGrad and MoeQuantize for gfx950.
+//
+// v = x + residual in fp32, y = v r gamma with r = 1 / sqrt(mean v^2 + eps). The 8-bit form of a row is q = rint(p 127 /
+// max |p|): with p = v gamma the factor r, which a row has in common, cancels, so q needs no sum and is the same
+// whatever the order of the sums; r enters the scale alone, max |p| r / 127. The gradient with u = v r: grad_v = r
+// (grad_y gamma - u mean(grad_y gamma u)) + grad_sum, grad_gamma = the column sums of grad_y u.
+//
+// Memory bounds them: each row is read once into registers by 1, 4 or 16 waves (8 values a lane and step), reduced,
+// and written from there; rows too long for that are read twice. Squares are added in fp64, which neither overflows nor
+// loses a small row, and takes no time that memory does not hide.
+#include "moe_ops.h"
+#include "moe_rows.h"
+
+namespace moe {
+
+namespace {
+
+constexpr int64_t kMaxBlocks = int64_t(1) << 20;  // of a launch
+
+// Sum and largest over the WAVES waves of a row, the same on every lane; `ex`: LDS for the waves' parts
+template <int WAVES>
+struct RowExchange {
+    double a[WAVES], b[WAVES];
+    uint32_t top[WAVES];
+};
+template <int WAVES, bool TWO>
+__device__ __forceinline__ void reduce_row(RowExchange<WAVES>& ex, double& a, double& b, uint32_t& top) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        a += __shfl_xor(a, d, kWave);
+        if (TWO) b += __shfl_xor(b, d, kWave);
+        else top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, kWave)));
+    }
+    if (WAVES == 1) return;
+    const int wave = static_cast<int>(threadIdx.x) / kWave;
+    if (lane_id() == 0) {
+        ex.a[wave] = a;
+        if (TWO) ex.b[wave] = b;
+        else ex.top[wave] = top;
+    }
+    __syncthreads();
+    a = ex.a[0];
+    b = ex.b[0];
+    top = ex.top[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+        a += ex.a[w];
+        if (TWO) b += ex.b[w];
+        else top = max(top, ex.top[w]);
+    }
+    __syncthreads();  // read before the next row's parts
+}
+
+// r of a row as f r', f a power of two that keeps r' and f v in fp32's range for any finite v
+struct RowFactor {
+    float f, r;
+};
+__device__ __forceinline__ RowFactor row_factor(double squares, int H, float eps) {
+    const double m = squares / H + static_cast<double>(eps);
+    RowFactor s;
+    s.f = m > 0x1p100 ? 0x1p-80f : m < 0x1p-100 ? 0x1p100f : 1.0f;
+    s.r = 1.0f / sqrtf(static_cast<float>(m * s.f * s.f));
+    return s;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+// NORM: the norm (its result, its 8-bit form or both), gamma of type G; else the 8-bit form of x itself. CHUNKS steps of V
+// values a lane hold a row; 0: any length, read twice.
+template <typename T, typename G, int WAVES, int CHUNKS, int V, bool NORM>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_kernel(NormArgs n) {
+    using Bits = typename T::Bits;
+    constexpr int kRows = WAVES == 1 ? 4 : 1;  // rows of a workgroup at a time
+    constexpr int kStep = WAVES * kWave * V;
+    constexpr int kSteps = CHUNKS > 0 ? CHUNKS : 1;
+    __shared__ RowExchange<WAVES> ex;
+    const int wave = static_cast<int>(threadIdx.x) / kWave, lead = WAVES == 1 ? lane_id() : static_cast<int>(threadIdx.x);
+    const bool ragged = n.H % V != 0;
+    const typename G::Bits* gamma = static_cast<const typename G::Bits*>(n.gamma);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0); row < n.rows;
+         row += static_cast<int64_t>(gridDim.x) * kRows) {
+        const Bits* x = static_cast<const Bits*>(n.x) + row * n.ldx;
+        const Bits* res = NORM && n.residual ? static_cast<const Bits*>(n.residual) + row * n.ldr : nullptr;
+        float v[kSteps][V];
+        Step<V> at[kSteps];
+        double squares = 0.0, unused = 0.0;
+        uint32_t top = 0;
+        auto load = [&](int col) __attribute__((always_inline)) {  // kSteps steps from col on
+            RawRow<T, V> a[kSteps], b[kSteps];
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) {
+                at[c] = step_at<V>(col + c * kStep, n.H);
+                a[c].load(x + at[c].at);
+            }
+            if (NORM && res) {
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c) b[c].load(res + at[c].at);
+            }
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[c][j] = NORM && res ? a[c].get(j) + b[c].get(j) : a[c].get(j);
+        };
+        auto take = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) {
+                if (NORM) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const double d = (ragged ? j >= at[c].skip : at[c].live) ? v[c][j] : 0.0f;
+                        squares += d * d;
+                    }
+                }
+                if (!NORM || n.q) {
+                    float g[V];
+                    if (NORM) load_row<G, V>(gamma + at[c].at, g);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const uint32_t m = magnitude(NORM ? v[c][j] * g[j] : v[c][j]);
+                        top = max(top, at[c].live ? m : 0u);
+                    }
+                }
+            }
+        };
+        RowFactor s{1.0f, 1.0f};
+        RowQuant quant{};
+        auto finish = [&]() __attribute__((always_inline)) {
+            reduce_row<WAVES, false>(ex, squares, unused, top);
+            if (NORM) s = row_factor(squares, n.H, n.eps);
+            if (!n.q) return;
+            quant = row_quant(top);
+            if (lead != 0) return;
+            const float t = __builtin_bit_cast(float, top), scale = (NORM ? t * s.f * s.r : t) / 127.0f;
+            n.scale[row] = quant.finite ? scale : __builtin_nanf("");
+        };
+        auto put = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) {
+                if (!at[c].live) continue;
+                const int64_t to = row * n.H + at[c].at;
+                if (!NORM) {
+                    store_quant<V>(n.q + to, v[c], quant);
+                    continue;
+                }
+                float g[V], y[V];
+                load_row<G, V>(gamma + at[c].at, g);
+                if (n.sum) store_row<T, V>(static_cast<Bits*>(n.sum) + to, v[c]);
+                if (n.y) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[j] = v[c][j] * s.f * s.r * g[j];
+                    store_row<T, V>(static_cast<Bits*>(n.y) + to, y);
+                }
+                if (n.q) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[j] = v[c][j] * g[j];
+                    store_quant<V>(n.q + to, y, quant);
+                }
+            }
+        };
+        if (CHUNKS > 0) {
+            load(lead * V);
+            take();
+            finish();
+            put();
+        } else {
+            for (int col = lead * V; col < n.H; col += kStep) {
+                load(col);
+                take();
+            }
+            finish();
+            for (int col = lead * V; col < n.H; col += kStep) {
+                load(col);
+                put();
+            }
+        }
+    }
+}
+
+// The gradient. A workgroup walks rows and keeps its share of grad_gamma's column sums in registers; they leave as one
+// row of `part` for each workgroup.
+template <typename T, typename G, int WAVES, int CHUNKS, int V>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_grad_kernel(NormArgs n) {
+    using Bits = typename T::Bits;
+    constexpr int kRows = WAVES == 1 ? 4 : 1;
+    constexpr int kStep = WAVES * kWave * V;
+    __shared__ RowExchange<WAVES> ex;
+    __shared__ float sums[WAVES == 1 ? 4 : 1][WAVES == 1 ? CHUNKS * kStep : 1];
+    const int wave = static_cast<int>(threadIdx.x) / kWave, lead = WAVES == 1 ? lane_id() : static_cast<int>(threadIdx.x);
+    const typename G::Bits* gamma = static_cast<const typename G::Bits*>(n.gamma);
+    Step<V> at[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) at[c] = step_at<V>(lead * V + c * kStep, n.H);
+    float gg[CHUNKS][V] = {};
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0); row < n.rows;
+         row += static_cast<int64_t>(gridDim.x) * kRows) {
+        const Bits* x = static_cast<const Bits*>(n.x) + row * n.ldx;
+        const Bits* gy = static_cast<const Bits*>(n.grad_y) + row * n.ldy;
+        RawRow<T, V> v[CHUNKS], d[CHUNKS];
+        double squares = 0.0, dot = 0.0;
+        uint32_t unused = 0;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            v[c].load(x + at[c].at);
+            d[c].load(gy + at[c].at);
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            float g[V];
+            load_row<G, V>(gamma + at[c].at, g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double a = j >= at[c].skip ? v[c].get(j) : 0.0f;  // of a live step V = skip at least
+                squares += a * a;
+                dot += static_cast<double>(j >= at[c].skip ? d[c].get(j) * g[j] : 0.0f) * a;
+            }
+        }
+        reduce_row<WAVES, true>(ex, squares, dot, unused);
+        const RowFactor s = row_factor(squares, n.H, n.eps);
+        const float r = s.f * s.r;
+        const float mean = static_cast<float>(dot * s.f * s.r / n.H);  // of grad_y gamma u
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            float g[V], gx[V];
+            RawRow<T, V> add;
+            load_row<G, V>(gamma + at[c].at, g);
+            if (n.grad_sum) add.load(static_cast<const Bits*>(n.grad_sum) + row * n.lds + at[c].at);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float u = v[c].get(j) * s.f * s.r, gv = d[c].get(j);
+                gg[c][j] += gv * u;
+                gx[j] = r * (gv * g[j] - u * mean);
+                if (n.grad_sum) gx[j] += add.get(j);
+            }
+            if (n.y && at[c].live) store_row<T, V>(static_cast<Bits*>(n.y) + row * n.H + at[c].at, gx);
+        }
+    }
+    if (!n.part) return;
+    float* out = n.part + static_cast<int64_t>(blockIdx.x) * n.H;
+    if (WAVES == 1) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+            if (at[c].live) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) sums[wave][at[c].at + j] = gg[c][j];
+            }
+        __syncthreads();
+        for (int i = static_cast<int>(threadIdx.x); i < n.H; i += 256)
+            out[i] = sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i];
+    } else {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+            if (at[c].live) store_row<F32, V>(out + at[c].at, gg[c]);
+    }
+}
+
+// grad_gamma: the workgroups' rows added in order, 16 columns a workgroup and 64 groups of rows
+constexpr int kSumThreads = 1024;
+template <typename G>
+__global__ __launch_bounds__(kSumThreads) void gamma_sum_kernel(const float* __restrict__ part,
+                                                                typename G::Bits* __restrict__ out, int H, int rows) {
+    constexpr int kCols = 16, kGroups = kSumThreads / kCols;
+    __shared__ float sums[kGroups][kCols];
+    const int i = static_cast<int>(threadIdx.x) % kCols, q = static_cast<int>(threadIdx.x) / kCols;
+    const int col = static_cast<int>(blockIdx.x) * kCols + i;
+    float s = 0.0f;
+    if (col < H) {
+#pragma unroll 8
+        for (int b = q; b < rows; b += kGroups) s += part[static_cast<int64_t>(b) * H + col];
+    }
+    sums[q][i] = s;
+    __syncthreads();
+    if (q != 0 || col >= H) return;
+    for (int g = 1; g < kGroups; ++g) s += sums[g][i];
+    out[col] = G::store(s);
+}
+
+// Waves of a row and its steps. A row of up to 2048 values has a wave to itself where there are rows enough for every
+// SIMD; else, and where it is longer, 4 or 16 waves share it.
+struct Shape {
+    int waves, chunks;
+};
+int steps(int H, int waves) {
+    const int c = (H + waves * kWave * 8 - 1) / (waves * kWave * 8);
+    return c <= 1 ? 1 : c <= 2 ? 2 : c <= 4 ? 4 : 0;
+}
+Shape norm_shape(int64_t rows, int H) {
+    const bool many = rows >= 2048;
+    if (H <= 512 || (many && H <= 2048)) return Shape{1, steps(H, 1)};
+    if (H <= 2048 || (many && H <= 8192)) return Shape{4, steps(H, 4)};
+    return Shape{16, steps(H, 16)};
+}
+unsigned norm_grid(int64_t rows, int waves) {
+    const int64_t blocks = waves == 1 ? (rows + 3) / 4 : rows;
+    return static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
+}
+
+template <typename T, typename G, int WAVES, int CHUNKS, bool NORM, int V = 8>
+hipError_t run_norm(const NormArgs& n, hipStream_t stream) {
+    norm_kernel<T, G, WAVES, CHUNKS, V, NORM>
+        <<<norm_grid(n.rows, WAVES), WAVES == 1 ? 256 : WAVES * kWave, 0, stream>>>(n);
+    return hipGetLastError();
+}
+template <typename T, typename G, bool NORM>
+hipError_t run_norm_any(const NormArgs& n, hipStream_t stream) {
+    if (n.H < 8) return run_norm<T, G, 1, 1, NORM, 1>(n, stream);
+    const Shape s = norm_shape(n.rows, n.H);
+    if (s.waves == 1) {
+        if (s.chunks == 1) return run_norm<T, G, 1, 1, NORM>(n, stream);
+        return s.chunks == 2 ? run_norm<T, G, 1, 2, NORM>(n, stream) : run_norm<T, G, 1, 4, NORM>(n, stream);
+    }
+    if (s.waves == 4) {
+        if (s.chunks == 1) return run_norm<T, G, 4, 1, NORM>(n, stream);
+        return s.chunks == 2 ? run_norm<T, G, 4, 2, NORM>(n, stream) : run_norm<T, G, 4, 4, NORM>(n, stream);
+    }
+    if (s.chunks == 1) return run_norm<T, G, 16, 1, NORM>(n, stream);
+    if (s.chunks == 2) return run_norm<T, G, 16, 2, NORM>(n, stream);
+    return s.chunks == 4 ? run_norm<T, G, 16, 4, NORM>(n, stream) : run_norm<T, G, 16, 0, NORM>(n, stream);
+}
+
+template <typename T, typename G>
+hipError_t run_norm_grad(const NormArgs& n, int blocks, hipStream_t stream) {
+    if (n.H < 8) norm_grad_kernel<T, G, 1, 1, 1><<<blocks, 256, 0, stream>>>(n);
+    else if (n.H <= 512) norm_grad_kernel<T, G, 1, 1, 8><<<blocks, 256, 0, stream>>>(n);
+    else if (n.H <= 1024) norm_grad_kernel<T, G, 1, 2, 8><<<blocks, 256, 0, stream>>>(n);
+    else if (n.H <= 2048) norm_grad_kernel<T, G, 1, 4, 8><<<blocks, 256, 0, stream>>>(n);
+    else if (n.H <= 4096) norm_grad_kernel<T, G, 4, 2, 8><<<blocks, 256, 0, stream>>>(n);
+    else if (n.H <= 8192) norm_grad_kernel<T, G, 4, 4, 8><<<blocks, 256, 0, stream>>>(n);
+    else norm_grad_kernel<T, G, 16, 2, 8><<<blocks, 1024, 0, stream>>>(n);
+    return hipGetLastError();
+}
+
+// f(row type, gamma type) for the types of a call
+template <typename F>
+hipError_t by_type(int type, bool gamma_f32, F&& f) {
+    if (type == MOE_DT_FLOAT32) return f(F32(), F32());
+    if (type == MOE_DT_FLOAT16) return gamma_f32 ? f(Half(), F32()) : f(Half(), Half());
+    return gamma_f32 ? f(Bf16(), F32()) : f(Bf16(), Bf16());
+}
+
+}  // namespace
+
+hipError_t launch_norm(const NormArgs& n, int type, bool norm, hipStream_t stream) {
+    TraceScope trace(norm ? "moe_norm" : "moe_quantize", stream);
+    if (!norm)
+        return by_type(type, false, [&](auto t, auto) { return run_norm_any<decltype(t), F32, false>(n, stream); });
+    return by_type(type, n.gamma_f32, [&](auto t, auto g) {
+        return run_norm_any<decltype(t), decltype(g), true>(n, stream);
+    });
+}
+
+// Workgroups of the gradient: two on every CU, and no more than have rows
+int norm_grad_blocks(int64_t rows, int H) {
+    const int64_t most = H <= 2048 ? (rows + 3) / 4 : rows;
+    return static_cast<int>(most < 512 ? (most > 0 ? most : 1) : 512);
+}
+
+hipError_t launch_norm_grad(const NormArgs& n, int type, void* grad_gamma, hipStream_t stream) {
+    const int blocks = norm_grad_blocks(n.rows, n.H);
+    hipError_t err;
+    {
+        TraceScope trace("moe_norm_grad", stream);
+        err = by_type(type, n.gamma_f32, [&](auto t, auto g) {
+            return run_norm_grad<decltype(t), decltype(g)>(n, blocks, stream);
+        });
+    }
+    if (err != hipSuccess || !grad_gamma) return err;
+    TraceScope trace("moe_norm_gamma", stream);
+    const int grid = (n.H + 15) / 16;
+    return by_type(type, n.gamma_f32, [&](auto, auto g) {
+        using G = decltype(g);
+        gamma_sum_kernel<G><<<grid, kSumThreads, 0, stream>>>(n.part, static_cast<typename G::Bits*>(grad_gamma), n.H,
+                                                              blocks);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace moe

@@ -38,6 +38,7 @@ if _modes is None or _deterministic is None:
 
 _TORCH_DT = {_lib.DT_FLOAT16: torch.float16, _lib.DT_INT32: torch.int32}
 _FLOAT_DT = {torch.float32: _lib.DT_FLOAT32, torch.float16: _lib.DT_FLOAT16, torch.bfloat16: _lib.DT_BFLOAT16}
+_ROW_DT = {**_FLOAT_DT, torch.int8: _lib.DT_INT8}
 _SCORING = {"softmax": 0, "sigmoid": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
 
@@ -292,7 +293,7 @@ def _first_float(t, name: str, dtypes, dims: int) -> tuple[int, int]:
     if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == dims:
         dev = t.get_device()
         if dev == _here():
-            return _FLOAT_DT[t.dtype], dev
+            return _ROW_DT[t.dtype], dev
         raise MoeError(4, f"{name} is on cuda:{dev}, the current device is cuda:{_here()}")
     return _need_float(t, name, dtypes, dims, -1), -1  # raises
 
@@ -300,7 +301,7 @@ def _first_float(t, name: str, dtypes, dims: int) -> tuple[int, int]:
 def _need_float(t, name: str, dtypes, dims: int, dev: int) -> int:
     """Checks a floating tensor of any strides on device `dev`; returns its moe_dtype."""
     if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == dims and t.get_device() == dev:
-        return _FLOAT_DT[t.dtype]
+        return _ROW_DT[t.dtype]
     if not isinstance(t, torch.Tensor):
         raise MoeError(1, f"{name} must be a tensor")
     if t.device.type != "cuda":
@@ -590,6 +591,203 @@ def moe_layer_shared(x: torch.Tensor, w_gate: torch.Tensor, expert_weights: torc
         hidden = MoeLinear(x, shared_gate_up, activation="swiglu", stream=stream)
         y = MoeLinear(hidden, shared_down, residual=y, stream=stream)
     return y, ids, w, eo
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# quantised and permuted expert layers (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _gamma(gamma, dtype, H: int, dev: int) -> int:
+    """Checks a norm's gamma, of the rows' type or fp32; returns its moe_dtype."""
+    gt = _need_float(gamma, "gamma", (dtype, torch.float32), 1, dev)
+    _need_shape(gamma, "gamma", (H,))
+    if not gamma.is_contiguous():
+        raise MoeError(4, "gamma must be contiguous")
+    return gt
+
+
+def _rows_like(t, name: str, dtype, shape, dev: int) -> tuple[int | None, int]:
+    """(address, row stride) of an optional matrix of any row stride."""
+    if t is None:
+        return None, 0
+    _need_float(t, name, (dtype,), 2, dev)
+    _need_shape(t, name, shape)
+    return t.data_ptr(), _row_stride(t, name)
+
+
+def _ids(t, name: str, T: int | None, dev: int) -> tuple[int, int]:
+    """Checks contiguous int32 ids or positions [T, K]; returns their shape."""
+    _need(t, name, torch.int32)
+    if t.dim() != 2:
+        raise MoeError(2, f"{name} must have 2 dimensions (got {t.dim()})")
+    if t.get_device() != dev:
+        raise MoeError(4, f"{name} is on {t.device}, the first tensor on cuda:{dev}")
+    if T is not None and t.shape[0] != T:
+        raise MoeError(3, f"{name} shape {tuple(t.shape)} for {T} tokens")
+    return t.shape[0], t.shape[1]
+
+
+def _add_rms_norm(x, gamma, residual, eps, want_y: bool, want_q: bool, stream):
+    dt, dev = _first_float(x, "x", _FLOATS, 2)
+    T, H = x.shape
+    gt = _gamma(gamma, x.dtype, H, dev)
+    rp, ldr = _rows_like(residual, "residual", x.dtype, (T, H), dev)
+    ldx = _row_stride(x, "x")
+    like = _like(x)
+    q = _empty(like, stream, (T, H), torch.int8) if want_q else None
+    scale = _empty(like, stream, (T,), torch.float32) if want_q else None
+    y = _empty(like, stream, (T, H), x.dtype) if want_y else None
+    total = None if residual is None else _empty(like, stream, (T, H), x.dtype)
+    check(_lib.load().moe_add_rms_norm(x.data_ptr(), ldx, rp, ldr, gamma.data_ptr(), gt, _ptr(y), _ptr(total), _ptr(q),
+                                       _ptr(scale), T, H, eps, dt, _queue(stream, dev)))
+    return q, scale, y, total
+
+
+def MoeAddRmsNorm(x: torch.Tensor, gamma: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                  stream=None):
+    """v = x[T,H] + residual[T,H] -> (y, v), y = v * gamma[H] / sqrt(mean(v^2) + eps), both of x's type (fp32, fp16 or
+    bf16); the sum, which the next layer adds to, is None without a residual. v is summed and normalised in fp32 and
+    rounded only where it is returned. gamma is of x's type or fp32; rows may be any stride apart."""
+    return _add_rms_norm(x, gamma, residual, eps, True, False, stream)[2:]
+
+
+def MoeAddRmsNormQuant(x: torch.Tensor, gamma: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                       returnNorm: bool = False, stream=None):
+    """MoeAddRmsNorm's y in 8 bits -> (q[T,H] int8, scale[T] fp32, y, v): q * scale is y, scale = max|y| / 127 of a row.
+    y itself (for a router) with returnNorm, else None; v is None without a residual. q is rint(p * (127 / max|p|)) with
+    p = v * gamma, the same bits whatever the launch; a row of zeros has scale 0, one that holds an infinity or a NaN has
+    q 0 and scale NaN."""
+    return _add_rms_norm(x, gamma, residual, eps, returnNorm, True, stream)
+
+
+def add_rms_norm_grad_workspace_bytes(T: int, H: int) -> int:
+    return int(_lib.load().moe_add_rms_norm_grad_workspace_bytes(T, H))
+
+
+def MoeAddRmsNormGrad(grad_y: torch.Tensor, v: torch.Tensor, gamma: torch.Tensor, grad_v: torch.Tensor | None = None,
+                      eps: float = 1e-6, gradX: bool = True, gradGamma: bool = True,
+                      workspace: torch.Tensor | None = None, stream=None):
+    """The gradients of MoeAddRmsNorm -> (grad_x[T,H], grad_gamma[H]), None where not asked for. v is the sum it returned
+    (x itself without a residual), grad_v the gradient that reaches the sum by another way. grad_x is the residual's
+    gradient too. H <= 16384. `workspace` (uint8, >= add_rms_norm_grad_workspace_bytes) is allocated when not given."""
+    dt, dev = _first_float(v, "v", _FLOATS, 2)
+    T, H = v.shape
+    gt = _gamma(gamma, v.dtype, H, dev)
+    yp, ldy = _rows_like(grad_y, "grad_y", v.dtype, (T, H), dev)
+    if yp is None:
+        raise MoeError(1, "grad_y must be a tensor")
+    vp, ldv = _rows_like(grad_v, "grad_v", v.dtype, (T, H), dev)
+    ld = _row_stride(v, "v")
+    lib = _lib.load()
+    like = _like(v)
+    wp, wb = None, 0
+    if gradGamma:
+        workspace, wp, wb = _workspace(workspace, lib.moe_add_rms_norm_grad_workspace_bytes, (T, H), like, dev, stream)
+    gx = _empty(like, stream, (T, H), v.dtype) if gradX else None
+    gg = _empty(like, stream, (H,), gamma.dtype) if gradGamma else None
+    check(lib.moe_add_rms_norm_grad(yp, ldy, v.data_ptr(), ld, gamma.data_ptr(), gt, vp, ldv, _ptr(gx), _ptr(gg), wp, wb,
+                                    T, H, eps, dt, _queue(stream, dev)))
+    return gx, gg
+
+
+def MoeQuantize(x: torch.Tensor, stream=None):
+    """Rows in 8 bits: x[R,H] (fp32, fp16 or bf16) -> (q[R,H] int8, scale[R] fp32), q * scale being x and scale = max|x| /
+    127 of a row. Contiguous experts' weights [E,N,H] -> (q[E,N,H], scale[E,N]): a weight row's scale is its output
+    channel's. q is rint(x * (127 / max|x|)); rows of zeros have scale 0, rows with an infinity or a NaN q 0 and scale NaN."""
+    if isinstance(x, torch.Tensor) and x.dim() == 3:
+        if not x.is_contiguous():
+            raise MoeError(4, "x must be contiguous (ND format)")
+        q, scale = MoeQuantize(x.view(-1, x.shape[2]), stream)
+        return q.view(x.shape), scale.view(x.shape[:2])
+    dt, dev = _first_float(x, "x", _FLOATS, 2)
+    R, H = x.shape
+    ldx = _row_stride(x, "x")
+    like = _like(x)
+    q = _empty(like, stream, (R, H), torch.int8)
+    scale = _empty(like, stream, (R,), torch.float32)
+    check(_lib.load().moe_quantize(x.data_ptr(), ldx, q.data_ptr(), scale.data_ptr(), R, H, dt, _queue(stream, dev)))
+    return q, scale
+
+
+def permute_workspace_bytes(T: int, E: int, K: int) -> int:
+    return int(_lib.load().moe_permute_workspace_bytes(T, E, K))
+
+
+def MoePermute(x: torch.Tensor, expert_ids: torch.Tensor, numExperts: int, xScale: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None, stream=None):
+    """x[T,H] (fp32, fp16, bf16 or int8), expert_ids[T,K] int32 -> (rows[T*K,H], offsets[E+1] int32, position[T,K] int32,
+    row_scale): the rows of all picks sorted by expert, one expert's in the order of their slots. Expert e has rows
+    [offsets[e], offsets[e+1]). Picks whose id is outside [0, E) come last, with rows of zeros. position is a pick's row,
+    -1 - row of a pick of no expert. xScale[T] fp32 (8-bit rows' scales) is sorted alike, else row_scale is None.
+    The gradient of rows is MoeUnpermute(grad_rows, position). `workspace` (uint8, >= permute_workspace_bytes) is
+    allocated when not given."""
+    dt, dev = _first_float(x, "x", (*_FLOATS, torch.int8), 2)
+    T, H = x.shape
+    _, K = _ids(expert_ids, "expert_ids", T, dev)
+    sp = _vector(xScale, "xScale", torch.float32, T, dev)
+    if type(numExperts) is not int or numExperts < 1:
+        raise MoeError(4, f"numExperts={numExperts} must be positive")
+    ldx = _row_stride(x, "x")
+    lib = _lib.load()
+    like = _like(x)
+    workspace, wp, wb = _workspace(workspace, lib.moe_permute_workspace_bytes, (T, numExperts, K), like, dev, stream)
+    rows = _empty(like, stream, (T * K, H), x.dtype)
+    offsets = _empty(like, stream, (numExperts + 1,), torch.int32)
+    position = _empty(like, stream, (T, K), torch.int32)
+    row_scale = None if xScale is None else _empty(like, stream, (T * K,), torch.float32)
+    check(lib.moe_permute(x.data_ptr(), ldx, sp, expert_ids.data_ptr(), rows.data_ptr(), _ptr(row_scale),
+                          offsets.data_ptr(), position.data_ptr(), wp, wb, T, H, numExperts, K, dt, _queue(stream, dev)))
+    return rows, offsets, position, row_scale
+
+
+def _row_weights(weights, shape, dev: int) -> tuple[int | None, int]:
+    """(address, moe_dtype) of optional contiguous weights [T, K]."""
+    if weights is None:
+        return None, 0
+    wt = _need_float(weights, "weights", _FLOATS, 2, dev)
+    _need_shape(weights, "weights", shape)
+    if not weights.is_contiguous():
+        raise MoeError(4, "weights must be contiguous (ND format)")
+    return weights.data_ptr(), wt
+
+
+def MoeUnpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None = None,
+                 stream=None) -> torch.Tensor:
+    """rows[R,H] (fp32, fp16 or bf16), position[T,K], weights[T,K] (fp32, fp16 or bf16; None: 1) -> y[T,H] of rows' type,
+    y[t] = sum over k of weights[t,k] * rows[position[t,k]] in fp32, ascending k. Positions outside [0, R) (a pick of no
+    expert is negative) add nothing."""
+    dt, dev = _first_float(rows, "rows", _FLOATS, 2)
+    if not rows.is_contiguous():
+        raise MoeError(4, "rows must be contiguous (ND format)")
+    R, H = rows.shape
+    T, K = _ids(position, "position", None, dev)
+    wp, wt = _row_weights(weights, (T, K), dev)
+    y = _empty(_like(rows), stream, (T, H), rows.dtype)
+    check(_lib.load().moe_unpermute(rows.data_ptr(), R, position.data_ptr(), wp, wt, y.data_ptr(), T, H, K, dt,
+                                    _queue(stream, dev)))
+    return y
+
+
+def MoeUnpermuteGrad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: torch.Tensor,
+                     weights: torch.Tensor | None = None, stream=None):
+    """The gradients of MoeUnpermute's y[T,H] -> (grad_rows[T*K,H] of grad_y's type, grad_weights[T,K] of weights' type).
+    position is MoePermute's, so every row has one pick; the rows of picks of no expert get zeros. Without weights rows
+    may be None and grad_weights is None."""
+    dt, dev = _first_float(grad_y, "grad_y", _FLOATS, 2)
+    T, H = grad_y.shape
+    _, K = _ids(position, "position", T, dev)
+    wp, wt = _row_weights(weights, (T, K), dev)
+    rp = _matrix(rows, "rows", grad_y.dtype, (T * K, H), dev)
+    if wp is not None and rows is None:
+        raise MoeError(1, "MoeUnpermuteGrad needs rows with weights")
+    ldy = _row_stride(grad_y, "grad_y")
+    like = _like(grad_y)
+    grad_rows = _empty(like, stream, (T * K, H), grad_y.dtype)
+    grad_w = None if wp is None else _empty(like, stream, (T, K), weights.dtype)
+    check(_lib.load().moe_unpermute_grad(grad_y.data_ptr(), ldy, rp, position.data_ptr(), wp, wt, grad_rows.data_ptr(),
+                                         _ptr(grad_w), T, H, K, dt, _queue(stream, dev)))
+    return grad_rows, grad_w
 
 
 def synth_normal_f16_(out: torch.Tensor, seed: int, stream_id: int, sigma_a: float, sigma_b: float | None = None,

@@ -59,6 +59,7 @@ typedef enum moe_status {
 typedef enum moe_dtype {
     MOE_DT_FLOAT32 = 0,  /* ge::DT_FLOAT   */
     MOE_DT_FLOAT16 = 1,  /* ge::DT_FLOAT16 */
+    MOE_DT_INT8 = 2,     /* ge::DT_INT8    */
     MOE_DT_INT32 = 3,    /* ge::DT_INT32   */
     MOE_DT_BFLOAT16 = 27 /* ge::DT_BF16    */
 } moe_dtype;
@@ -356,6 +357,70 @@ moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const
                                void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                                size_t workspace_bytes, int64_t num_tokens, int64_t n, int64_t hidden_size,
                                int32_t activation, int32_t dtype, void* stream);
+
+/* ======================================================================================================
+ * Quantised and permuted expert layers: the norm in front of a layer, rows in 8 bits with a scale each, tokens
+ * sorted by expert and back. The reference has none of them (its FFN gathers rows inside its kernel,
+ * op_kernel/moe_expert_ffn.cpp:182-195). Tensors of any alignment and, where a stride is given, any row stride;
+ * results are contiguous and do not overlap the inputs. Streams, workspaces and errors as above.
+ * ==================================================================================================== */
+
+/* ------------------------------------------------------------------------------------------------------
+ * MoeAddRmsNorm: v = x[T, H] + residual (NULL: x), summed in float32 -> y = v * gamma / sqrt(mean(v^2) + eps) of
+ *   dtype, sum = v of dtype, and y in 8 bits: q[T, H] and scale[T], q = rint(p * (127 / max|p|)) with p = v * gamma
+ *   of a row (the norm's factor, which the row has in common, cancels; quotient and products rounded to float32, ties
+ *   to even) and scale = max|y| / 127, so that q * scale is y. A row of zeros has scale 0; one where p holds an infinity
+ *   or a NaN has scale NaN and q 0. y, sum and the pair q, scale may each be NULL. q is the same bits whatever the
+ *   launch. dtype is float32, float16 or bfloat16, gamma_type that or float32; eps > 0, H <= 2^20.
+ * ---------------------------------------------------------------------------------------------------- */
+moe_status moe_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                            const void* gamma, int32_t gamma_type, void* y, void* sum, int8_t* q, float* scale,
+                            int64_t num_tokens, int64_t hidden_size, float eps, int32_t dtype, void* stream);
+
+/* Its gradient: grad_y, the sum and gamma, and grad_sum[T, H] that reaches the sum by another way (NULL: none) ->
+ * grad_x[T, H], x's and the residual's, and grad_gamma[H] of gamma_type; either may be NULL. H <= 16384. The workspace
+ * (always needed with grad_gamma; any alignment of 4) holds column sums of blocks of rows, added in order. With T = 0
+ * grad_gamma is zeros. */
+size_t moe_add_rms_norm_grad_workspace_bytes(int64_t num_tokens, int64_t hidden_size);
+moe_status moe_add_rms_norm_grad(const void* grad_y, int64_t grad_y_stride, const void* sum, int64_t sum_stride,
+                                 const void* gamma, int32_t gamma_type, const void* grad_sum, int64_t grad_sum_stride,
+                                 void* grad_x, void* grad_gamma, void* workspace, size_t workspace_bytes,
+                                 int64_t num_tokens, int64_t hidden_size, float eps, int32_t dtype, void* stream);
+
+/* MoeQuantize: x[rows, H] float32, float16 or bfloat16 -> q and scale[rows] as above with p = x: a token's row, or a
+ * weight's row, whose scale is then its output channel's. H <= 2^20. */
+moe_status moe_quantize(const void* x, int64_t x_stride, int8_t* q, float* scale, int64_t rows, int64_t hidden_size,
+                        int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * MoePermute: x[T, H] (float32, float16, bfloat16 or int8), expert_ids[T, K] -> rows[T K, H], the rows of the T K picks
+ *   sorted by expert, of one expert in the order of their slots t K + k: the rows of expert e are [offsets[e],
+ *   offsets[e + 1]), offsets[E + 1]. Picks whose id is outside [0, E) stand behind them, in slot order, with rows of
+ *   zeros. position[T, K] is the place of each pick's row, of a pick of no expert -1 - place. x_scale[T] (int8 rows'
+ *   scales; NULL: none) is sorted alike into row_scale[T K], 0 for picks of no expert. 1 <= K <= E <= 256, T K < 2^31.
+ *   The workspace (0 up to 4096 picks; any alignment of 4) holds ranks and counts. The gradient of rows is
+ *   moe_unpermute without weights.
+ * ---------------------------------------------------------------------------------------------------- */
+size_t moe_permute_workspace_bytes(int64_t num_tokens, int64_t num_experts, int64_t top_k);
+moe_status moe_permute(const void* x, int64_t x_stride, const float* x_scale, const int32_t* expert_ids, void* rows,
+                       float* row_scale, int32_t* offsets, int32_t* position, void* workspace, size_t workspace_bytes,
+                       int64_t num_tokens, int64_t hidden_size, int64_t num_experts, int64_t top_k, int32_t dtype,
+                       void* stream);
+
+/* MoeUnpermute: rows[num_rows, H] (float32, float16 or bfloat16), position[T, K], weights[T, K] (float32, float16 or
+ * bfloat16; NULL: 1) -> y[T, H] of dtype, y[t] = sum over k of weights[t, k] * rows[position[t, k]], float32 sums in
+ * ascending k. Positions outside [0, num_rows) add nothing and neither their weight nor a row is read. */
+moe_status moe_unpermute(const void* rows, int64_t num_rows, const int32_t* position, const void* weights,
+                         int32_t weights_type, void* y, int64_t num_tokens, int64_t hidden_size, int64_t top_k,
+                         int32_t dtype, void* stream);
+
+/* Its gradient: grad_y[T, H], and what moe_unpermute had, num_rows = T K -> grad_rows[T K, H] = weights * grad_y at
+ * each pick's place, zeros at the place of a pick of no expert, and grad_weights[T, K] of weights_type = <grad_y, row>
+ * (float32 sums), 0 for a pick of no expert. Without weights rows and grad_weights are NULL. position is moe_permute's,
+ * where every row has one pick: a row that no position names is left as it was, and one that two name is either's. */
+moe_status moe_unpermute_grad(const void* grad_y, int64_t grad_y_stride, const void* rows, const int32_t* position,
+                              const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights,
+                              int64_t num_tokens, int64_t hidden_size, int64_t top_k, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }
