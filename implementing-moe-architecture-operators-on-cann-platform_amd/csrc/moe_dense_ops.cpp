@@ -351,6 +351,41 @@ moe_status linear(const void* x, int64_t x_stride, const void* weight, int64_t w
     if (err != hipSuccess) return hip_fail(err, "MoeLinear launch");
     return ok();
 }
+// 8-bit products. In their plans k counts pairs of integers, as the kernels do (moe_gemm.h).
+constexpr int64_t kMaxInt8K = 131071;  // 2^14 k < 2^31: no sum leaves 32 bits, -128 included
+
+moe_status check_linear_int8(int64_t T, int64_t N, int64_t H, int64_t E, int32_t act) {
+    const char* op = "MoeLinearInt8";
+    moe_status st = check_linear(op, T, N, H, act, MOE_DT_FLOAT16);
+    if (st != MOE_OK) return st;
+    if (H > kMaxInt8K)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: H=%lld exceeds %lld, where 32-bit sums end", op, (long long)H,
+                    (long long)kMaxInt8K);
+    if (E < 0) return fail(MOE_ERR_ARG, "%s: numExperts=%lld", op, (long long)E);
+    if (E > kMaxExperts)
+        return fail(MOE_ERR_UNSUPPORTED, "%s: numExperts=%lld exceeds %lld", op, (long long)E, (long long)kMaxExperts);
+    if (E > 0 && (T / 16 + E) * (N / 8 + 1) > kInt32Max)  // items of 16 rows x 8 columns, the smallest
+        return fail(MOE_ERR_UNSUPPORTED, "%s: T=%lld N=%lld too large", op, (long long)T, (long long)N);
+    return ok();
+}
+
+size_t linear_int8_workspace(int64_t T, int64_t N, int64_t H, int64_t E, int32_t act) {
+    if (E > 0) return 0;
+    size_t most = 0;
+    for (const bool direct : {false, true}) {
+        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, act == MOE_ACT_SWIGLU, false, false, direct);
+        if (plan.partial_bytes > most) most = plan.partial_bytes;
+    }
+    return most;
+}
+
+// Rows of a tile of the experts' products, by their rows on average
+int group_rows(int64_t T, int64_t E, bool direct) {
+    const int64_t mean = T / E;
+    if (!direct) return mean <= 64 ? 64 : 128;
+    return mean <= 8 ? 16 : mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 256 ? 128 : 256;
+}
+
 // moe_linear_grad likewise; grad_y of the operands' type or, with grad_f32, float32
 moe_status linear_grad(const void* grad_y, int64_t grad_y_stride, bool grad_f32, const void* x, int64_t x_stride,
                        const void* weight, int64_t weight_stride, int32_t weight_transposed, const void* pre,
@@ -639,6 +674,83 @@ moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const
     return linear_grad(grad_y, grad_y_stride, true, x, x_stride, weight, weight_stride, weight_transposed, pre, grad_x,
                        grad_weight, grad_bias, workspace, workspace_bytes, T, N, H, activation, dtype, stream,
                        layout_of(weight_transposed));
+}
+
+size_t moe_linear_int8_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t E, int32_t activation) {
+    if (check_linear_int8(T, N, H, E, activation) != MOE_OK) return 0;
+    return linear_int8_workspace(T, N, H, E, activation);
+}
+
+moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* weight,
+                           int64_t weight_stride, int64_t expert_stride, const float* weight_scale,
+                           const int32_t* offsets, const void* bias, const void* residual, void* y, void* workspace,
+                           size_t workspace_bytes, int64_t T, int64_t N, int64_t H, int64_t E, int32_t activation,
+                           int32_t out_dtype, void* stream) {
+    const char* op = "MoeLinearInt8";
+    moe_status st = check_linear_int8(T, N, H, E, activation);
+    if (st != MOE_OK) return st;
+    if (out_dtype != MOE_DT_FLOAT32 && !is_half(out_dtype))
+        return fail(MOE_ERR_ARG, "%s: result type %d (float32, float16 or bfloat16 expected)", op, out_dtype);
+    const bool swiglu = activation == MOE_ACT_SWIGLU;
+    const int64_t Z = swiglu ? 2 * N : N;
+    st = check_pitch(op, "x", T, H, x_stride);
+    if (st == MOE_OK) st = check_pitch(op, "weight", Z, H, weight_stride);
+    if (st != MOE_OK) return st;
+    if (E > 1 && (expert_stride < (Z - 1) * weight_stride + H || expert_stride > int64_t{1} << 50))
+        return fail(MOE_ERR_ARG, "%s: experts' weights %lld elements apart", op, (long long)expert_stride);
+    if (T == 0) return ok();
+    if (!x || !x_scale || !weight || !weight_scale || !y || (E > 0 && !offsets))
+        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    const size_t need = linear_int8_workspace(T, N, H, E, activation);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace, need);
+    if (need > 0 && !aligned16(workspace))
+        return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
+    const int64_t pitch = T > 1 ? x_stride : 0, weight_pitch = Z > 1 ? weight_stride : 0;
+    const int64_t step = E > 1 ? expert_stride : 0;
+    const bool direct = H % 16 == 0 && aligned16(x) && aligned16(weight) && pitch % 16 == 0 && weight_pitch % 16 == 0 &&
+                        step % 16 == 0 && pitch <= int64_t{1} << 23 && weight_pitch <= int64_t{1} << 23;
+    const int unit = direct ? 2 : 1;  // bytes that strides and k count
+    moe::GemmArgs g{};
+    g.p = reinterpret_cast<const uint16_t*>(x);
+    g.q = reinterpret_cast<const uint16_t*>(weight);
+    g.ldp = pitch / unit;
+    g.ldq = weight_pitch / unit;
+    g.m = static_cast<int>(T);
+    g.n = g.up = static_cast<int>(N);
+    g.k = static_cast<int>(H / unit);
+    g.out = y;
+    g.bias = static_cast<const uint16_t*>(bias);
+    g.residual = residual;
+    g.act = activation;
+    g.out_f32 = out_dtype == MOE_DT_FLOAT32;
+    g.splits = 1;
+    g.split_k = g.k;
+    g.row_scale = x_scale;
+    g.col_scale = weight_scale;
+    g.experts = static_cast<int>(E);
+    g.q_expert = step;
+    g.offsets = offsets;
+    const bool bf16 = out_dtype == MOE_DT_BFLOAT16;
+    const hipStream_t s = as_stream(stream);
+    hipError_t err = moe::prepare_linear_int8();
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearInt8 kernel attributes");
+    if (E > 0) {
+        const int rows = group_rows(T, E, direct);
+        if (rows == 256) err = moe::launch_int8_tiled(g, bf16, s);
+        else if (direct && rows <= 64) err = moe::launch_int8_stream(g, bf16, rows, s);
+        else err = moe::launch_int8_mid(g, bf16, direct, rows, s);
+    } else {
+        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, swiglu, false, false, direct);
+        set_split(g, plan, workspace);
+        g.split_k = static_cast<int>(plan.split_k * 2 / unit);
+        if (plan.kernel == Kernel::kStream) err = moe::launch_int8_stream(g, bf16, 0, s);
+        else if (plan.kernel == Kernel::kTiled) err = moe::launch_int8_tiled(g, bf16, s);
+        else err = moe::launch_int8_mid(g, bf16, direct, plan.bm, s);
+        if (err == hipSuccess && plan.splits > 1) err = moe::launch_int8_reduce(g, bf16, s);
+    }
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearInt8 launch");
+    return ok();
 }
 
 }  // extern "C"

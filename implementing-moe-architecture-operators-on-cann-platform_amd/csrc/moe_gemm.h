@@ -11,9 +11,14 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
 // 16-bit element types of the products; storage is uint16_t bits everywhere
 struct Half {
     using Bits = uint16_t;
+    static constexpr bool kInt8 = false;
+    static __device__ __forceinline__ f32x4 add(f32x4 a, f32x4 b) { return a + b; }
     static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                       0, 0);
@@ -23,6 +28,8 @@ struct Half {
 };
 struct Bf16 {
     using Bits = uint16_t;
+    static constexpr bool kInt8 = false;
+    static __device__ __forceinline__ f32x4 add(f32x4 a, f32x4 b) { return a + b; }
     static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -34,6 +41,26 @@ struct Bf16 {
     static __device__ __forceinline__ uint16_t store(float v) {
         return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
     }
+};
+
+// 8-bit integers with results of type O. A pair of them stands where the 16-bit types have one value, so the kernels move
+// the same bytes: k, the strides and the stages count pairs (of operands that 16-byte copies cannot read, bytes). The
+// fp32 registers of the sums hold int32 bits up to the epilogue, which applies the scales; k is short enough that no sum
+// leaves 32 bits.
+template <typename O>
+struct Int8 {
+    using Bits = uint16_t;
+    static constexpr bool kInt8 = true;
+    static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+        return __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                         __builtin_bit_cast(i32x4, c), 0, 0, 0));
+    }
+    static __device__ __forceinline__ f32x4 add(f32x4 a, f32x4 b) {
+        return __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, a) + __builtin_bit_cast(i32x4, b));
+    }
+    static __device__ __forceinline__ float load(uint16_t b) { return O::load(b); }
+    static __device__ __forceinline__ uint16_t store(float v) { return O::store(v); }
 };
 
 // A product C[m][n] = sum_k P[m][k] Q[n][k]. An operand is stored by rows (its k contiguous, rows `ld` elements apart)
@@ -54,7 +81,117 @@ struct GemmArgs {
     float* partial;       // [splits, m, part_ld] fp32 sums of a product split over k
     int splits;           // 1: the whole k in one workgroup, through the epilogue
     int split_k;          // k of one split, a multiple of the kernels' stage
+    const float* row_scale;  // 8-bit operands: [m], and [n or 2 n] of the columns; bias then is of out's type
+    const float* col_scale;
+    // Products of experts: P rows [offsets[e], offsets[e + 1]), of the first from 0 on, by Q + e q_expert (bytes), with
+    // the columns' scales and bias from e (n or 2 n) on; rows from offsets[experts] on are zeros. 0: one product
+    int experts;
+    int64_t q_expert;
+    const int32_t* offsets;
 };
+
+// An item of the experts' products: items are the tiles of bm rows x ntiles of one expert after another
+struct GroupItem {
+    int expert, row0, row1;  // of the expert
+    int first;               // its first item
+};
+__device__ __forceinline__ int group_offset(const GemmArgs& g, int e) {
+    return e == 0 ? 0 : min(max(g.offsets[e], 0), g.m);
+}
+__device__ __forceinline__ const uint16_t* group_q(const GemmArgs& g, int e) {
+    return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(g.q) + e * g.q_expert);
+}
+// The experts' items in a wave's registers: lane l has experts l, l + 64, ... Offsets are taken within [0, m] and
+// ascending, whatever they say.
+constexpr int kGroupParts = 4;  // of 64 experts
+struct GroupTable {
+    int row0[kGroupParts], row1[kGroupParts], end[kGroupParts];  // rows, and the items up to the expert's last
+    int total;
+};
+__device__ __forceinline__ int group_items(int row0, int row1, int bm, int ntiles) {
+    return (row1 - row0 + bm - 1) / bm * ntiles;
+}
+__device__ __forceinline__ GroupTable group_table(const GemmArgs& g, int bm, int ntiles) {
+    const int lane = lane_id();
+    GroupTable t;
+    t.total = 0;
+#pragma unroll
+    for (int s = 0; s < kGroupParts; ++s) {
+        const int e = s * kWave + lane;
+        t.row0[s] = t.row1[s] = 0;
+        if (e < g.experts) {
+            t.row0[s] = group_offset(g, e);
+            t.row1[s] = max(t.row0[s], group_offset(g, e + 1));
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kGroupParts; ++s) {
+        int end = group_items(t.row0[s], t.row1[s], bm, ntiles);
+        if (s * kWave < g.experts) {
+#pragma unroll
+            for (int d = 1; d < kWave; d <<= 1) {
+                const int v = __shfl_up(end, d, kWave);
+                if (lane >= d) end += v;
+            }
+        }
+        t.end[s] = t.total + end;
+        t.total = __builtin_amdgcn_readlane(t.end[s], kWave - 1);
+    }
+    return t;
+}
+// The item `at`, below t.total: its expert is the first whose items end past it
+__device__ __forceinline__ GroupItem group_find(const GroupTable& t, int bm, int ntiles, int at) {
+    GroupItem item{};
+    bool found = false;
+#pragma unroll
+    for (int s = 0; s < kGroupParts; ++s) {
+        const uint64_t past = __ballot(t.end[s] > at);
+        if (found || past == 0) continue;
+        const int l = __builtin_ctzll(past);
+        item.expert = s * kWave + l;
+        item.row0 = __builtin_amdgcn_readlane(t.row0[s], l);
+        item.row1 = __builtin_amdgcn_readlane(t.row1[s], l);
+        item.first = __builtin_amdgcn_readlane(t.end[s], l) - group_items(item.row0, item.row1, bm, ntiles);
+        found = true;
+    }
+    return item;
+}
+// The same for an item at or behind `item`, from one expert to the next: scalar loads, which leave the copies in flight
+// alone, and no vector registers
+__device__ __forceinline__ void group_advance(const GemmArgs& g, int bm, int ntiles, int at, GroupItem& item) {
+    typedef const __attribute__((address_space(4))) int32_t* Constant;
+    const Constant offsets = reinterpret_cast<Constant>(reinterpret_cast<uintptr_t>(g.offsets));
+    int items = group_items(item.row0, item.row1, bm, ntiles);
+    while (at >= item.first + items) {
+        item.first += items;
+        ++item.expert;
+        const int o0 = offsets[item.expert], o1 = offsets[item.expert + 1];
+        item.row0 = item.expert == 0 ? 0 : min(max(o0, 0), g.m);
+        item.row1 = max(item.row0, min(max(o1, 0), g.m));
+        items = group_items(item.row0, item.row1, bm, ntiles);
+    }
+}
+// The rows behind the last expert's, over all workgroups
+__device__ __forceinline__ void group_zero_rows(const GemmArgs& g, int block, int blocks) {
+    const int64_t from = static_cast<int64_t>(group_offset(g, g.experts)) * g.n, to = static_cast<int64_t>(g.m) * g.n;
+    for (int64_t i = from + static_cast<int64_t>(block) * blockDim.x + threadIdx.x; i < to;
+         i += static_cast<int64_t>(blocks) * blockDim.x) {
+        if (g.out_f32) static_cast<float*>(g.out)[i] = 0.0f;
+        else static_cast<uint16_t*>(g.out)[i] = 0;
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the kernels count their copies from here on
+}
+// The product of one expert alone: P and the result keep the rows' numbers
+template <bool SWIGLU>
+__device__ __forceinline__ GemmArgs group_args(const GemmArgs& g, const GroupItem& item) {
+    GemmArgs e = g;
+    const int64_t cols = static_cast<int64_t>(item.expert) * (SWIGLU ? 2 * static_cast<int64_t>(g.n) : g.n);
+    e.q = group_q(g, item.expert);
+    e.m = item.row1;
+    e.col_scale += cols;
+    if (g.bias) e.bias += g.out_f32 ? 2 * cols : cols;
+    return e;
+}
 
 // Row pitch of the partial sums: columns (SwiGLU: gate and up apart) rounded up to whole 16-byte stores
 __host__ __device__ constexpr int64_t part_cols(int n) { return (static_cast<int64_t>(n) + 3) / 4 * 4; }
@@ -124,8 +261,36 @@ __device__ __forceinline__ uint2 pack4(f32x4 y) {
 template <typename T, bool SWIGLU>
 __device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col, int valid, bool whole, f32x4 z,
                                          f32x4 u) {
+    if constexpr (T::kInt8) {  // int32 sums: times the row's scale, times the columns'
+        const float rs = g.row_scale[row];
+        auto scaled = [&](f32x4 bits, const float* cs) __attribute__((always_inline)) {
+            const i32x4 v = __builtin_bit_cast(i32x4, bits);
+            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+            if (valid == 4) {
+                c = *reinterpret_cast<const f32x4_any*>(cs);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 3; ++r)
+                    if (r < valid) c[r] = cs[r];
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c[r] *= static_cast<float>(v[r]) * rs;
+            return c;
+        };
+        z = scaled(z, g.col_scale + col);
+        if (SWIGLU) u = scaled(u, g.col_scale + g.n + col);
+    }
     if (!SWIGLU && g.factor) z *= *g.factor;
-    if (g.bias) {
+    if (T::kInt8 && g.bias && g.out_f32) {
+        const float* bias = reinterpret_cast<const float*>(g.bias);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (r < valid) {
+                z[r] += bias[col + r];
+                if (SWIGLU) u[r] += bias[g.n + col + r];
+            }
+        }
+    } else if (g.bias) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (r < valid) {
@@ -348,6 +513,24 @@ __device__ __forceinline__ s16x8 load8(const uint16_t* p, int valid, int before)
     return v;
 }
 
+// 16 bytes of a row from p on, of which `valid` exist (zeros past them); any alignment
+__device__ __forceinline__ s16x8 load16(const uint8_t* p, int valid, int before) {
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    typedef uint64_t u64x2_any __attribute__((ext_vector_type(2), aligned(1)));
+    u64x2 x = {0, 0};
+    if (valid >= 16) {
+        x = *reinterpret_cast<const u64x2_any*>(p);
+    } else if (valid > 0 && before + valid >= 16) {  // the 16 that end at the row's end, moved down
+        x = *reinterpret_cast<const u64x2_any*>(p + valid - 16);
+        const int bits = 8 * (16 - valid), b = bits & 63;  // 8 .. 120
+        const uint64_t high = x[1] >> b;
+        x = bits >= 64 ? u64x2{high, 0} : u64x2{x[0] >> b | x[1] << (64 - b), high};
+    } else {
+        for (int e = 0; e < valid; ++e) x[e / 8] |= static_cast<uint64_t>(p[e]) << (e % 8 * 8);
+    }
+    return __builtin_bit_cast(s16x8, x);
+}
+
 // Copies of matrices with rows padded with zeros to dst_cols, a multiple of 8 (moe_linear_repack.hip)
 struct Repack {
     const uint16_t* src;
@@ -384,5 +567,15 @@ hipError_t launch_gemm_stream(const GemmArgs& g, bool bf16, hipStream_t stream);
 // 256 x 256 tiles; operands that 16-byte copies can read
 hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);
+
+// The same of 8-bit operands, both by rows; bf16: the results. With experts bm rows a tile (mid: 64 or 128, stream: 16, 32
+// or 64) and no split
+hipError_t prepare_int8_mid();
+hipError_t prepare_int8_stream();
+hipError_t prepare_int8_tiled();
+hipError_t launch_int8_mid(const GemmArgs& g, bool bf16, bool direct, int bm, hipStream_t stream);
+hipError_t launch_int8_stream(const GemmArgs& g, bool bf16, int bm, hipStream_t stream);
+hipError_t launch_int8_tiled(const GemmArgs& g, bool bf16, hipStream_t stream);
+hipError_t launch_int8_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);
 
 }  // namespace moe

@@ -29,6 +29,7 @@ class TraceScope {
 hipError_t ensure_lds_limit(const void* fn, int lds_max);
 // The same for all kernels of the dense products: the first call on a device sets them, later ones cost one lookup.
 hipError_t prepare_linear();
+hipError_t prepare_linear_int8();
 // Workgroups of `fn` (`threads` threads, `lds` bytes of dynamic LDS) the current device holds at once, cached per
 // device, kernel and LDS size; 0 when the device cannot be queried.
 int resident_workgroups(const void* fn, int threads, size_t lds);

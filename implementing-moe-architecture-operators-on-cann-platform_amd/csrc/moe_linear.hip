@@ -90,8 +90,8 @@ __device__ __forceinline__ s16x8 load_granule(const uint16_t* p, int64_t ld, boo
 // DIRECT: both operands allow 16-byte copies (bases and row pitches 16-byte aligned, by rows k % 8 == 0). Otherwise the
 // granules come through registers (loads of any alignment) and are written to the same layout.
 // block of grid: this product's share of the launch, grid a multiple of the XCDs.
-template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
-__device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntiles, int block, int grid,
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT, bool GROUPED = false>
+__device__ __forceinline__ void gemm_mid(const GemmArgs& all, int mtiles, int ntiles, int block, int grid,
                                          uint16_t* lds) {
     constexpr int NS = ring_stages(BM);
     constexpr int WAVES = mid_waves(BM);
@@ -106,16 +106,27 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
 
     // Workgroups go round-robin over the XCDs; each XCD takes a contiguous run of the items. The tiles that read the
     // same piece of the larger operand are neighbours in it, so that piece reaches that XCD's L2 once.
-    const int item = block % kXcds * (grid / kXcds) + block / kXcds;
+    int item = block % kXcds * (grid / kXcds) + block / kXcds;
+    GroupItem group{};
+    if (GROUPED) {  // of the expert whose item this is, the m-tiles that read the same weights as neighbours
+        group_zero_rows(all, block, grid);
+        const GroupTable table = group_table(all, BM, ntiles);
+        if (item >= table.total) return;
+        group = group_find(table, BM, ntiles, item);
+        item -= group.first;
+        mtiles = (group.row1 - group.row0 + BM - 1) / BM;
+    }
+    const GemmArgs g = GROUPED ? group_args<SWIGLU>(all, group) : all;
     if (item >= mtiles * ntiles * g.splits) return;
-    const bool n_first = mtiles > ntiles;
+    const bool n_first = !GROUPED && mtiles > ntiles;
     const int inner = n_first ? ntiles : mtiles, outer = item / inner;
     const int outers = n_first ? mtiles : ntiles;
     const int i0 = item - outer * inner, sp = outer / outers, o0 = outer - sp * outers;
     const int mt = n_first ? o0 : i0, nt = n_first ? i0 : o0;
     const int k0 = sp * g.split_k, k1 = min(g.k, k0 + g.split_k);
-    const int nst = max(1, (k1 - k0 + kBK - 1) / kBK);
-    const int m0 = mt * BM, n0 = nt * (SWIGLU ? kBN / 2 : kBN);
+    constexpr int kStageK = T::kInt8 && !DIRECT ? 2 * kBK : kBK;  // in what k counts: bytes, or 16 bits
+    const int nst = max(1, (k1 - k0 + kStageK - 1) / kStageK);
+    const int m0 = group.row0 + mt * BM, n0 = nt * (SWIGLU ? kBN / 2 : kBN);
 
     // Q row of tile row r. SwiGLU: a wave's rows are half gate, half up, of the same output columns.
     auto q_col = [&](int r) {
@@ -161,8 +172,25 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
     const uint16_t* qbase = g.q + (QK ? 0 : static_cast<int64_t>(n0) * g.ldq);
     auto copy_stage = [&](int s) __attribute__((always_inline)) {
         uint16_t* slot = lds + (s % NS) * kSlot;
-        const int kc = k0 + s * kBK;
-        if (DIRECT) {
+        const int kc = k0 + s * kStageK;
+        if constexpr (T::kInt8 && !DIRECT) {  // by rows, bytes
+            static_assert(!PK && !QK, "8-bit operands are by rows");
+            auto load = [&](const uint16_t* base, int64_t ld, int row, int rows, int el) __attribute__((always_inline)) {
+                const int k = kc + el * 2;
+                return load16(reinterpret_cast<const uint8_t*>(base) + static_cast<int64_t>(row) * ld + k,
+                              row < rows ? k1 - k : 0, k);
+            };
+#pragma unroll
+            for (int c = 0; c < PC; ++c)
+                *reinterpret_cast<s16x8*>(slot + (wave * PC + c) * 512 + lane * 8) =
+                    load(g.p, g.ldp, m0 + prow[c], g.m, pel[c]);
+#pragma unroll
+            for (int c = 0; c < QC; ++c) {
+                const int up = q_up(qrow[c]) ? g.up : 0;
+                *reinterpret_cast<s16x8*>(slot + BM * kBK + (wave * QC + c) * 512 + lane * 8) =
+                    load(g.q, g.ldq, q_col(qrow[c]) + up, g.n + up, qel[c]);
+            }
+        } else if (DIRECT) {
             const int left = k1 - kc;  // granules from here on are zeros
             const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<uint16_t*>(PK ? pbase + static_cast<int64_t>(kc) * g.ldp : pbase), 0, 0x7fffffff,
@@ -271,12 +299,12 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& g, int mtiles, int ntil
     }
 }
 
-template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT, bool GROUPED = false>
 __global__ __launch_bounds__(mid_threads(BM)) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_mid_kernel(
     GemmArgs g, int mtiles, int ntiles) {
     extern __shared__ __align__(16) uint16_t lds[];
-    gemm_mid<T, PK, QK, BM, SWIGLU, DIRECT>(g, mtiles, ntiles, static_cast<int>(blockIdx.x),
-                                            static_cast<int>(gridDim.x), lds);
+    gemm_mid<T, PK, QK, BM, SWIGLU, DIRECT, GROUPED>(g, mtiles, ntiles, static_cast<int>(blockIdx.x),
+                                                     static_cast<int>(gridDim.x), lds);
 }
 
 // Both gradient products in one launch: neither needs the other, and small ones leave the GPU half empty. The first
@@ -298,13 +326,15 @@ int mid_grid(const GemmArgs& g, int bm, int bn) {
     return static_cast<int>((items + kXcds - 1) / kXcds * kXcds);
 }
 
-template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT>
+template <typename T, bool PK, bool QK, int BM, bool SWIGLU, bool DIRECT, bool GROUPED = false>
 hipError_t run_mid(const GemmArgs& g, hipStream_t stream) {
     constexpr int kCols = SWIGLU ? kBN / 2 : kBN;
-    TraceScope trace("moe_linear_gemm", stream);
-    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT>
-        <<<mid_grid(g, BM, kCols), mid_threads(BM), mid_lds_bytes(BM), stream>>>(g, (g.m + BM - 1) / BM,
-                                                                                (g.n + kCols - 1) / kCols);
+    const int ntiles = (g.n + kCols - 1) / kCols;
+    const int mtiles = GROUPED ? g.m / BM + min(g.experts, g.m) : (g.m + BM - 1) / BM;  // experts': at most
+    const int grid = GROUPED ? (mtiles * ntiles + kXcds - 1) / kXcds * kXcds : mid_grid(g, BM, kCols);
+    TraceScope trace(T::kInt8 ? "moe_linear_int8" : "moe_linear_gemm", stream);
+    gemm_mid_kernel<T, PK, QK, BM, SWIGLU, DIRECT, GROUPED>
+        <<<grid, mid_threads(BM), mid_lds_bytes(BM), stream>>>(g, mtiles, ntiles);
     return hipGetLastError();
 }
 
@@ -357,6 +387,24 @@ hipError_t run_mid_any(const GemmArgs& g, bool p_by_k, bool q_by_k, bool direct,
                   : run_mid_direct<T, false, false, 32, false>(g, direct, stream);
 }
 
+template <typename T, int BM, bool GROUPED>
+hipError_t run_int8(const GemmArgs& g, bool direct, hipStream_t stream) {
+    if (g.act == kActSwiglu)
+        return direct ? run_mid<T, false, false, BM, true, true, GROUPED>(g, stream)
+                      : run_mid<T, false, false, BM, true, false, GROUPED>(g, stream);
+    return direct ? run_mid<T, false, false, BM, false, true, GROUPED>(g, stream)
+                  : run_mid<T, false, false, BM, false, false, GROUPED>(g, stream);
+}
+template <typename T>
+hipError_t run_int8_any(const GemmArgs& g, bool direct, int bm, hipStream_t stream) {
+    if (g.experts) return bm == 64 ? run_int8<T, 64, true>(g, direct, stream) : run_int8<T, 128, true>(g, direct, stream);
+    if (bm == 256)  // direct operands only
+        return g.act == kActSwiglu ? run_mid<T, false, false, 256, true, true>(g, stream)
+                                   : run_mid<T, false, false, 256, false, true>(g, stream);
+    if (bm == 128) return run_int8<T, 128, false>(g, direct, stream);
+    return bm == 64 ? run_int8<T, 64, false>(g, direct, stream) : run_int8<T, 32, false>(g, direct, stream);
+}
+
 // Adds the splits' sums in order and applies the epilogue; a thread has 4 columns of a row.
 constexpr int kReduceThreads = 256;
 int64_t reduce_blocks(const GemmArgs& g) { return (part_cols(g.n) / 4 * g.m + kReduceThreads - 1) / kReduceThreads; }
@@ -373,8 +421,8 @@ __device__ __forceinline__ void gemm_reduce(const GemmArgs& g, int block) {
     if (SWIGLU) u = *reinterpret_cast<const f32x4*>(src + pcols);
 #pragma unroll 4
     for (int s = 1; s < g.splits; ++s) {
-        z += *reinterpret_cast<const f32x4*>(src + s * step);
-        if (SWIGLU) u += *reinterpret_cast<const f32x4*>(src + s * step + pcols);
+        z = T::add(z, *reinterpret_cast<const f32x4*>(src + s * step));
+        if (SWIGLU) u = T::add(u, *reinterpret_cast<const f32x4*>(src + s * step + pcols));
     }
     store4<T, SWIGLU>(g, row, col, z, u, vector_rows(g));
 }
@@ -425,12 +473,53 @@ hipError_t prepare_bm() {
     return hipSuccess;
 }
 
+template <typename T, int BM, bool GROUPED>
+hipError_t prepare_int8_bm() {
+    for (const void* fn :
+         {reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, false, true, GROUPED>),
+          reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, true, true, GROUPED>),
+          reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, false, false, GROUPED>),
+          reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, BM, true, false, GROUPED>)}) {
+        const hipError_t err = ensure_lds_limit(fn, mid_lds_bytes(BM));
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
+}
+template <typename T>
+hipError_t prepare_int8() {
+    hipError_t err = prepare_int8_bm<T, 32, false>();
+    if (err == hipSuccess) err = prepare_int8_bm<T, 64, false>();
+    if (err == hipSuccess) err = prepare_int8_bm<T, 64, true>();
+    for (const void* fn : {reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, 256, false, true>),
+                           reinterpret_cast<const void*>(&gemm_mid_kernel<T, false, false, 256, true, true>)})
+        if (err == hipSuccess) err = ensure_lds_limit(fn, mid_lds_bytes(256));
+    return err;
+}
+
 }  // namespace
 
 hipError_t launch_gemm_mid(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, bool direct, int bm,
                            hipStream_t stream) {
     return bf16 ? run_mid_any<Bf16>(g, p_by_k, q_by_k, direct, bm, stream)
                 : run_mid_any<Half>(g, p_by_k, q_by_k, direct, bm, stream);
+}
+
+hipError_t launch_int8_mid(const GemmArgs& g, bool bf16, bool direct, int bm, hipStream_t stream) {
+    return bf16 ? run_int8_any<Int8<Bf16>>(g, direct, bm, stream) : run_int8_any<Int8<Half>>(g, direct, bm, stream);
+}
+
+hipError_t launch_int8_reduce(const GemmArgs& g, bool bf16, hipStream_t stream) {
+    const bool swiglu = g.act == kActSwiglu;
+    const int grid = static_cast<int>(reduce_blocks(g));
+    TraceScope trace("moe_linear_int8_reduce", stream);
+    if (bf16) {
+        if (swiglu) gemm_reduce_kernel<Int8<Bf16>, true><<<grid, kReduceThreads, 0, stream>>>(g);
+        else gemm_reduce_kernel<Int8<Bf16>, false><<<grid, kReduceThreads, 0, stream>>>(g);
+    } else {
+        if (swiglu) gemm_reduce_kernel<Int8<Half>, true><<<grid, kReduceThreads, 0, stream>>>(g);
+        else gemm_reduce_kernel<Int8<Half>, false><<<grid, kReduceThreads, 0, stream>>>(g);
+    }
+    return hipGetLastError();
 }
 
 hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream) {
@@ -461,6 +550,11 @@ hipError_t launch_grad_tail(GradTail t, bool bf16, hipStream_t stream) {
     if (bf16) grad_tail_kernel<Bf16><<<grid, kReduceThreads, 0, stream>>>(t);
     else grad_tail_kernel<Half><<<grid, kReduceThreads, 0, stream>>>(t);
     return hipGetLastError();
+}
+
+hipError_t prepare_int8_mid() {  // 128-row tiles keep within 64 KB
+    const hipError_t err = prepare_int8<Int8<Half>>();
+    return err == hipSuccess ? prepare_int8<Int8<Bf16>>() : err;
 }
 
 hipError_t prepare_gemm_mid() {  // 128-row tiles keep within 64 KB

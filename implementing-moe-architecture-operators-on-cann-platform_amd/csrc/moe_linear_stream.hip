@@ -37,7 +37,7 @@ struct StreamLds {
     static constexpr int kBytes = kRings + kSums;
 };
 
-template <typename T, int QB, int MB, int WAVES, int DEPTH, bool SWIGLU>
+template <typename T, int QB, int MB, int WAVES, int DEPTH, bool SWIGLU, bool GROUPED = false>
 __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, int tiles) {
     using Lds = StreamLds<QB, MB, WAVES, DEPTH>;
     constexpr int kCopies = 2 * (QB + MB), kCols = QB * (SWIGLU ? 8 : 16);
@@ -54,15 +54,39 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
     const __amdgpu_buffer_rsrc_t pr =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.p), 0, 0x7fffffff, 0x00020000);
 
+    // Experts: `tiles` is an expert's, and an item one of them for 16 MB of the expert's rows; items of the same weights
+    // are neighbours.
+    const int ntiles = tiles;
+    GroupItem cgroup{};
+    GroupTable table;
+    if (GROUPED) {
+        table = group_table(g, 16 * MB, ntiles);
+        tiles = table.total;
+        group_zero_rows(g, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    }
+    struct Place {
+        int row0, nt;  // first P row, tile of Q rows
+    };
+    auto place_of = [&](int tile, GroupItem& item) __attribute__((always_inline)) {
+        if (!GROUPED) return Place{0, tile};
+        item = group_find(table, 16 * MB, ntiles, tile);
+        const int passes = (item.row1 - item.row0 + 16 * MB - 1) / (16 * MB);
+        const int in = tile - item.first, nt = in / passes;
+        return Place{item.row0 + (in - nt * passes) * 16 * MB, nt};
+    };
+
     const int stages = (g.k + kBK - 1) / kBK;
     const int mine = stages > wave ? (stages - wave + WAVES - 1) / WAVES : 0;  // pieces of this wave per tile
     // the wave's pieces of all its tiles in a row: where the next copy is
     int ctile = static_cast<int>(blockIdx.x), cpiece = 0, cslot = 0;
+    Place cplace{0, ctile};
+    if (GROUPED && ctile < tiles) cplace = place_of(ctile, cgroup);
     auto copy_next = [&]() __attribute__((always_inline)) {
         uint16_t* slot = ring + cslot * Lds::kPieceHalfs;
         const int k0 = (wave + cpiece * WAVES) * kBK;
         const bool live = ctile < tiles && mine > 0;
-        const int n0 = ctile * kCols;
+        const int n0 = (GROUPED ? cplace.nt : ctile) * kCols;
+        const uint16_t* qe = GROUPED ? group_q(g, cgroup.expert) : g.q;
 #pragma unroll
         for (int i = 0; i < 2 * QB; ++i) {
             const int k = k0 + ((gran ^ (4 * (i & 1))) * 8);
@@ -70,24 +94,30 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
             // SwiGLU: the first QB instructions the gate rows, the others the up rows
             const int64_t first = n0 + (SWIGLU && i >= QB ? static_cast<int64_t>(g.up) : 0);
             const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<uint16_t*>(live ? g.q + first * g.ldq : g.q), 0, 0x7fffffff, 0x00020000);
+                const_cast<uint16_t*>(live ? qe + first * g.ldq : g.q), 0, 0x7fffffff, 0x00020000);
             const uint32_t off = static_cast<uint32_t>(row) * qpitch + static_cast<uint32_t>(k) * 2;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 qr, (__attribute__((address_space(3))) void*)(slot + i * 512), 16,
                 static_cast<int>(live && n0 + row < g.n && k < g.k ? off : kPastEnd), 0, 0, kNonTemporal);
         }
+        const __amdgpu_buffer_rsrc_t pe =
+            GROUPED ? __builtin_amdgcn_make_buffer_rsrc(
+                          const_cast<uint16_t*>(g.p + static_cast<int64_t>(cplace.row0) * g.ldp), 0, 0x7fffffff, 0x00020000)
+                    : pr;
+        const int rows = GROUPED ? cgroup.row1 - cplace.row0 : g.m;
 #pragma unroll
         for (int i = 0; i < 2 * MB; ++i) {
             const int row = 8 * i + r8, k = k0 + ((gran ^ (4 * (i & 1))) * 8);
             const uint32_t off = static_cast<uint32_t>(row) * ppitch + static_cast<uint32_t>(k) * 2;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                pr, (__attribute__((address_space(3))) void*)(slot + QB * kBlock + i * 512), 16,
-                static_cast<int>(live && row < g.m && k < g.k ? off : kPastEnd), 0, 0, 0);
+                pe, (__attribute__((address_space(3))) void*)(slot + QB * kBlock + i * 512), 16,
+                static_cast<int>(live && row < rows && k < g.k ? off : kPastEnd), 0, 0, 0);
         }
         cslot = cslot + 1 == DEPTH ? 0 : cslot + 1;
         if (++cpiece >= mine) {
             cpiece = 0;
             ctile += static_cast<int>(gridDim.x);
+            if (GROUPED && ctile < tiles) cplace = place_of(ctile, cgroup);
         }
     };
 #pragma unroll
@@ -96,7 +126,10 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
     const bool vec = vector_rows(g);
     const int sw = (row16 >> 1) & 7;
     int slot = 0;
+    GroupItem group{};
     for (int tile = static_cast<int>(blockIdx.x); tile < tiles; tile += static_cast<int>(gridDim.x)) {
+        const Place place = place_of(tile, group);
+        const GemmArgs ge = GROUPED ? group_args<SWIGLU>(g, group) : g;
         f32x4 acc[QB][MB];
 #pragma unroll
         for (int q = 0; q < QB; ++q)
@@ -142,16 +175,16 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
             // a thread has 4 columns of one row
             constexpr int kQuads = kCols / 4;
             for (int i = tid; i < kRows * kQuads; i += WAVES * kWave) {
-                const int r = i / kQuads, c = i % kQuads, row = b0 * 16 + r;
-                if (row >= g.m) continue;
+                const int r = i / kQuads, c = i % kQuads, row = place.row0 + b0 * 16 + r;
+                if (row >= ge.m) continue;
                 f32x4 z = {0.f, 0.f, 0.f, 0.f}, u = z;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
                     const float* at = sums + (w * kRows + r) * kGranules * 4;
-                    z += *reinterpret_cast<const f32x4*>(at + (c ^ (r % kGranules)) * 4);
-                    if (SWIGLU) u += *reinterpret_cast<const f32x4*>(at + ((kQuads + c) ^ (r % kGranules)) * 4);
+                    z = T::add(z, *reinterpret_cast<const f32x4*>(at + (c ^ (r % kGranules)) * 4));
+                    if (SWIGLU) u = T::add(u, *reinterpret_cast<const f32x4*>(at + ((kQuads + c) ^ (r % kGranules)) * 4));
                 }
-                store4<T, SWIGLU>(g, row, tile * kCols + c * 4, z, u, vec);
+                store4<T, SWIGLU>(ge, row, place.nt * kCols + c * 4, z, u, vec);
             }
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -188,43 +221,46 @@ int tile_blocks(int m, int64_t rows) {
     return 3 * two < 2 * one ? 2 : 1;
 }
 
-template <typename T, int QB, int MB, int WAVES, int DEPTH, bool SWIGLU>
+template <typename T, int QB, int MB, int WAVES, int DEPTH, bool SWIGLU, bool GROUPED = false>
 hipError_t run_stream(const GemmArgs& g, hipStream_t stream) {
-    auto fn = &gemm_stream_kernel<T, QB, MB, WAVES, DEPTH, SWIGLU>;
+    auto fn = &gemm_stream_kernel<T, QB, MB, WAVES, DEPTH, SWIGLU, GROUPED>;
     const void* p = reinterpret_cast<const void*>(fn);
     constexpr int kLds = StreamLds<QB, MB, WAVES, DEPTH>::kBytes, kCols = QB * (SWIGLU ? 8 : 16);
     static_assert(kLds <= 160 * 1024);
     const int tiles = (g.n + kCols - 1) / kCols;
     const int resident = resident_workgroups(p, WAVES * kWave, kLds);
-    TraceScope trace("moe_linear_stream", stream);
-    fn<<<resident > 0 && resident < tiles ? resident : tiles, WAVES * kWave, kLds, stream>>>(g, tiles);
+    const int64_t most = GROUPED ? static_cast<int64_t>(g.m / (16 * MB) + min(g.experts, g.m)) * tiles : tiles;
+    const int grid = static_cast<int>(resident > 0 && resident < most ? resident : most);
+    TraceScope trace(T::kInt8 ? "moe_linear_int8_stream" : "moe_linear_stream", stream);
+    fn<<<grid, WAVES * kWave, kLds, stream>>>(g, tiles);
     return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool GROUPED = false>
 hipError_t prepare(int m, int qb) {
     return by_rows(m, qb, [](auto q, auto mb, auto waves, auto depth) {
         constexpr int Q = decltype(q)::value, M = decltype(mb)::value, W = decltype(waves)::value,
                       D = decltype(depth)::value;
-        hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, true>),
+        hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, true, GROUPED>),
                                           StreamLds<Q, M, W, D>::kBytes);
         if (err == hipSuccess)
-            err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, false>),
+            err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, false, GROUPED>),
                                    StreamLds<Q, M, W, D>::kBytes);
         return err;
     });
 }
 
-template <typename T>
-hipError_t run_stream_any(const GemmArgs& g, hipStream_t stream) {
-    const int64_t rows = g.act == kActSwiglu ? 2 * static_cast<int64_t>(g.n) : g.n;
-    return by_rows(g.m, tile_blocks(g.m, rows), [&](auto q, auto mb, auto waves, auto depth) {
+template <typename T, bool GROUPED = false>
+hipError_t run_stream_any(const GemmArgs& g, int m, int qb, hipStream_t stream) {
+    return by_rows(m, qb, [&](auto q, auto mb, auto waves, auto depth) {
         constexpr int Q = decltype(q)::value, M = decltype(mb)::value, W = decltype(waves)::value,
                       D = decltype(depth)::value;
-        return g.act == kActSwiglu ? run_stream<T, Q, M, W, D, true>(g, stream)
-                                   : run_stream<T, Q, M, W, D, false>(g, stream);
+        return g.act == kActSwiglu ? run_stream<T, Q, M, W, D, true, GROUPED>(g, stream)
+                                   : run_stream<T, Q, M, W, D, false, GROUPED>(g, stream);
     });
 }
+
+int64_t weight_rows(const GemmArgs& g) { return g.act == kActSwiglu ? 2 * static_cast<int64_t>(g.n) : g.n; }
 
 }  // namespace
 
@@ -239,7 +275,28 @@ hipError_t prepare_gemm_stream() {
 }
 
 hipError_t launch_gemm_stream(const GemmArgs& g, bool bf16, hipStream_t stream) {
-    return bf16 ? run_stream_any<Bf16>(g, stream) : run_stream_any<Half>(g, stream);
+    const int qb = tile_blocks(g.m, weight_rows(g));
+    return bf16 ? run_stream_any<Bf16>(g, g.m, qb, stream) : run_stream_any<Half>(g, g.m, qb, stream);
+}
+
+hipError_t prepare_int8_stream() {
+    for (const int m : {16, 32, 64})
+        for (const int qb : {1, 2}) {
+            hipError_t err = prepare<Int8<Half>>(m, qb);
+            if (err == hipSuccess) err = prepare<Int8<Bf16>>(m, qb);
+            if (err == hipSuccess && qb == 2) err = prepare<Int8<Half>, true>(m, qb);
+            if (err == hipSuccess && qb == 2) err = prepare<Int8<Bf16>, true>(m, qb);
+            if (err != hipSuccess) return err;
+        }
+    return hipSuccess;
+}
+
+hipError_t launch_int8_stream(const GemmArgs& g, bool bf16, int bm, hipStream_t stream) {
+    if (g.experts)
+        return bf16 ? run_stream_any<Int8<Bf16>, true>(g, bm, 2, stream)
+                    : run_stream_any<Int8<Half>, true>(g, bm, 2, stream);
+    const int qb = tile_blocks(g.m, weight_rows(g));
+    return bf16 ? run_stream_any<Int8<Bf16>>(g, g.m, qb, stream) : run_stream_any<Int8<Half>>(g, g.m, qb, stream);
 }
 
 }  // namespace moe

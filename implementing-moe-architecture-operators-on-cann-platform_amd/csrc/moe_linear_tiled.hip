@@ -44,8 +44,14 @@ __device__ __forceinline__ int lane_fresh() {
     return v;
 }
 
+template <bool GROUPED>
 struct Tile {
     int m0, n0;
+};
+template <>
+struct Tile<true> {  // of an expert's product
+    int m0, n0;
+    GroupItem group;
 };
 
 // Where a tile's copies come from. Per half tile wave w issues instructions 2 w and 2 w + 1, each 64 granules of 16
@@ -58,7 +64,7 @@ struct CopyPlan {
     const uint16_t* qb[2];
 };
 
-template <typename T, bool PK, bool QK, bool SWIGLU>
+template <typename T, bool PK, bool QK, bool SWIGLU, bool GROUPED = false>
 __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mtiles, int ntiles) {
     extern __shared__ __align__(16) uint16_t lds[];
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
@@ -68,21 +74,37 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
     const int nst = max(2, (g.k + kBK - 1) / kBK);  // the ring runs two stages ahead; a second one past k is zeros
 
     // XCD x has the tiles [x per_xcd, (x + 1) per_xcd), dealt round-robin to its workgroups
-    const int total = mtiles * ntiles;
+    using Tile = Tile<GROUPED>;
+    int total = mtiles * ntiles;
+    Tile cur;
+    if constexpr (GROUPED) {
+        const GroupTable table = group_table(g, kBM, ntiles);
+        total = table.total;
+        const int first = static_cast<int>(blockIdx.x) % kXcds * ((total + kXcds - 1) / kXcds) +
+                          static_cast<int>(blockIdx.x) / kXcds;
+        cur.group = group_find(table, kBM, ntiles, first);
+        group_zero_rows(g, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    }
     const int nloc = static_cast<int>(gridDim.x) / kXcds;
     const int x = static_cast<int>(blockIdx.x) % kXcds, li = static_cast<int>(blockIdx.x) / kXcds;
     const int per_xcd = (total + kXcds - 1) / kXcds;
     auto tile_at = [&](int i, Tile& t) __attribute__((always_inline)) -> bool {
-        const int loc = li + i * nloc, at = x * per_xcd + loc;
+        const int loc = li + i * nloc;
+        int at = x * per_xcd + loc, mt = mtiles, row0 = 0;
         if (loc >= per_xcd || at >= total) return false;
+        if constexpr (GROUPED) {
+            group_advance(g, kBM, ntiles, at, t.group);
+            at -= t.group.first;
+            mt = (t.group.row1 - t.group.row0 + kBM - 1) / kBM;
+            row0 = t.group.row0;
+        }
         const int band = at / (kBand * ntiles), r = at - band * kBand * ntiles;
-        const int rows = min(kBand, mtiles - band * kBand);
+        const int rows = min(kBand, mt - band * kBand);
         const int nt = r / rows;
-        t.m0 = __builtin_amdgcn_readfirstlane((band * kBand + r - nt * rows) * kBM);
+        t.m0 = __builtin_amdgcn_readfirstlane(row0 + (band * kBand + r - nt * rows) * kBM);
         t.n0 = __builtin_amdgcn_readfirstlane(nt * (SWIGLU ? kBN / 2 : kBN));
         return true;
     };
-    Tile cur;
     if (!tile_at(0, cur)) return;
 
     // k of the stage that this lane's granule of instruction j holds (by rows: its first of 8)
@@ -100,6 +122,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
     auto make_plan = [&](const Tile& t, CopyPlan& c) __attribute__((always_inline)) {
         const int ln = lane_fresh();
         const uint32_t pp = static_cast<uint32_t>(g.ldp) * 2, qp = static_cast<uint32_t>(g.ldq) * 2;
+        int row_end = g.m;
+        if constexpr (GROUPED) row_end = t.group.row1;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int pk = granule_k(PK, j, ln), pr = granule_row(PK, j, ln);
@@ -108,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
             for (int h = 0; h < 2; ++h) {
                 const int row = h * 128 + pr;
                 const uint32_t po = PK ? pk * pp + (t.m0 + row) * 2u : row * pp + pk * 2u;
-                c.po[h][j] = t.m0 + row < g.m ? po : kPastEnd;
+                c.po[h][j] = t.m0 + row < row_end ? po : kPastEnd;
                 // SwiGLU: half 0 the gate rows, half 1 the up rows of the same columns. Else wave column wn has columns
                 // wn * 64 + h * 32 + [0, 32) of half h.
                 const int col = SWIGLU ? qr : (qr >> 5) * 64 + h * 32 + (qr & 31);
@@ -118,7 +142,9 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
             }
         }
         c.pb = g.p + (PK ? 0 : static_cast<int64_t>(t.m0) * g.ldp);
-        c.qb[0] = g.q + (QK ? 0 : static_cast<int64_t>(t.n0) * g.ldq);
+        const uint16_t* q = g.q;
+        if constexpr (GROUPED) q = group_q(g, t.group.expert);
+        c.qb[0] = q + (QK ? 0 : static_cast<int64_t>(t.n0) * g.ldq);
         c.qb[1] = c.qb[0] + (SWIGLU && !QK ? static_cast<int64_t>(g.up) * g.ldq : 0);
     };
     // One half tile of stage kc into ring slot q % 2. By rows the k offset is the instruction's scalar one, by k it
@@ -218,6 +244,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
     // The 8 blocks of 16 rows share one copy of the epilogue's code: unrolled, its activations are too long for the
     // accumulators to stay in registers.
     auto epilogue = [&](const Acc (&acc)[2], const Tile& t) __attribute__((always_inline)) {
+        GemmArgs ge = g;
+        if constexpr (GROUPED) ge = group_args<SWIGLU>(g, t.group);
         const int ln = lane_fresh(), row16 = ln & 15, kg = ln >> 4;
         const bool vec = vector_rows(g), lines = whole_lines(g, vec);
         float* stg = reinterpret_cast<float*>(lds + 2 * kStageHalfs) + wave * (kEpiBytes / 4);
@@ -237,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
                 case 6: put(6); break;
                 default: put(7); break;
             }
-            store_block<T, SWIGLU, 4>(g, stg, ln, t.m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16,
+            store_block<T, SWIGLU, 4>(ge, stg, ln, t.m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16,
                                       t.n0 + wn * (SWIGLU ? 32 : 64), vec, lines);
         }
     };
@@ -286,17 +314,18 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the surplus copies have landed before the workgroup ends
 }
 
-template <typename T, bool PK, bool QK, bool SWIGLU>
+template <typename T, bool PK, bool QK, bool SWIGLU, bool GROUPED = false>
 hipError_t run_tiled(const GemmArgs& g, hipStream_t stream) {
-    auto fn = &gemm_tiled_kernel<T, PK, QK, SWIGLU>;
+    auto fn = &gemm_tiled_kernel<T, PK, QK, SWIGLU, GROUPED>;
     const void* p = reinterpret_cast<const void*>(fn);
     const int bn = SWIGLU ? kBN / 2 : kBN;
-    const int mtiles = (g.m + kBM - 1) / kBM, ntiles = (g.n + bn - 1) / bn;
+    const int mtiles = GROUPED ? g.m / kBM + min(g.experts, g.m) : (g.m + kBM - 1) / kBM;  // experts': at most
+    const int ntiles = (g.n + bn - 1) / bn;
     int grid = resident_workgroups(p, kThreads, kLdsBytes) / kXcds * kXcds;
     const int most = (mtiles * ntiles + kXcds - 1) / kXcds * kXcds;
     if (grid < kXcds) grid = kXcds;
     if (grid > most) grid = most;
-    TraceScope trace("moe_linear_gemm_tiled", stream);
+    TraceScope trace(T::kInt8 ? "moe_linear_int8_tiled" : "moe_linear_gemm_tiled", stream);
     fn<<<grid, kThreads, kLdsBytes, stream>>>(g, mtiles, ntiles);
     return hipGetLastError();
 }
@@ -307,6 +336,27 @@ hipError_t run_tiled_any(const GemmArgs& g, bool p_by_k, bool q_by_k, hipStream_
     if (g.act == kActSwiglu)
         return q_by_k ? run_tiled<T, false, true, true>(g, stream) : run_tiled<T, false, false, true>(g, stream);
     return q_by_k ? run_tiled<T, false, true, false>(g, stream) : run_tiled<T, false, false, false>(g, stream);
+}
+
+template <typename T>
+hipError_t run_int8(const GemmArgs& g, hipStream_t stream) {
+    const bool swiglu = g.act == kActSwiglu;
+    if (g.experts)
+        return swiglu ? run_tiled<T, false, false, true, true>(g, stream)
+                      : run_tiled<T, false, false, false, true>(g, stream);
+    return swiglu ? run_tiled<T, false, false, true>(g, stream) : run_tiled<T, false, false, false>(g, stream);
+}
+
+template <typename T>
+hipError_t prepare_int8() {
+    for (const void* fn : {reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, false, true, true>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, false, false, true>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, false, true>),
+                           reinterpret_cast<const void*>(&gemm_tiled_kernel<T, false, false, false>)}) {
+        const hipError_t err = ensure_lds_limit(fn, kLdsBytes);
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 template <typename T>
@@ -331,6 +381,15 @@ hipError_t prepare_gemm_tiled() {
 
 hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream) {
     return bf16 ? run_tiled_any<Bf16>(g, p_by_k, q_by_k, stream) : run_tiled_any<Half>(g, p_by_k, q_by_k, stream);
+}
+
+hipError_t prepare_int8_tiled() {
+    const hipError_t err = prepare_int8<Int8<Half>>();
+    return err == hipSuccess ? prepare_int8<Int8<Bf16>>() : err;
+}
+
+hipError_t launch_int8_tiled(const GemmArgs& g, bool bf16, hipStream_t stream) {
+    return bf16 ? run_int8<Int8<Bf16>>(g, stream) : run_int8<Int8<Half>>(g, stream);
 }
 
 }  // namespace moe

@@ -70,18 +70,37 @@ int resident_workgroups(const void* fn, int threads, size_t lds) {
     return n;
 }
 
-hipError_t prepare_linear() {
-    static std::atomic<uint64_t> ready{0};  // devices below 64
+namespace {
+// Runs `set` once on each device (below 64), as `ready` tells
+template <typename F>
+hipError_t once_per_device(std::atomic<uint64_t>& ready, F&& set) {
     int dev = 0;
     hipError_t err = hipGetDevice(&dev);
     if (err != hipSuccess) return err;
     const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
     if (ready.load(std::memory_order_acquire) & bit) return hipSuccess;
-    err = prepare_gemm_mid();
-    if (err == hipSuccess) err = prepare_gemm_stream();
-    if (err == hipSuccess) err = prepare_gemm_tiled();
+    err = set();
     if (err == hipSuccess) ready.fetch_or(bit, std::memory_order_release);
     return err;
+}
+}  // namespace
+
+hipError_t prepare_linear() {
+    static std::atomic<uint64_t> ready{0};
+    return once_per_device(ready, [] {
+        hipError_t err = prepare_gemm_mid();
+        if (err == hipSuccess) err = prepare_gemm_stream();
+        return err == hipSuccess ? prepare_gemm_tiled() : err;
+    });
+}
+
+hipError_t prepare_linear_int8() {
+    static std::atomic<uint64_t> ready{0};
+    return once_per_device(ready, [] {
+        hipError_t err = prepare_int8_mid();
+        if (err == hipSuccess) err = prepare_int8_stream();
+        return err == hipSuccess ? prepare_int8_tiled() : err;
+    });
 }
 
 }  // namespace moe

@@ -38,7 +38,7 @@ if _modes is None or _deterministic is None:
 
 _TORCH_DT = {_lib.DT_FLOAT16: torch.float16, _lib.DT_INT32: torch.int32}
 _FLOAT_DT = {torch.float32: _lib.DT_FLOAT32, torch.float16: _lib.DT_FLOAT16, torch.bfloat16: _lib.DT_BFLOAT16}
-_ROW_DT = {**_FLOAT_DT, torch.int8: _lib.DT_INT8}
+_ROW_DT = {**_FLOAT_DT, torch.int8: _lib.DT_INT8, torch.int32: _lib.DT_INT32}
 _SCORING = {"softmax": 0, "sigmoid": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
 
@@ -281,6 +281,7 @@ def moe_layer_fused(x: torch.Tensor, w_gate: torch.Tensor, expert_weights: torch
 _F16_32 = (torch.float16, torch.float32)
 _HALVES = (torch.float16, torch.bfloat16)
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_INT8 = (torch.int8,)
 
 
 def _here() -> int:
@@ -788,6 +789,72 @@ def MoeUnpermuteGrad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: 
     check(_lib.load().moe_unpermute_grad(grad_y.data_ptr(), ldy, rp, position.data_ptr(), wp, wt, grad_rows.data_ptr(),
                                          _ptr(grad_w), T, H, K, dt, _queue(stream, dev)))
     return grad_rows, grad_w
+
+
+def linear_int8_workspace_bytes(T: int, N: int, H: int, activation: str = "none", numExperts: int = 0) -> int:
+    return int(_lib.load().moe_linear_int8_workspace_bytes(T, N, H, numExperts, _act_code(activation)))
+
+
+def _contiguous(t, name: str, dtype, shape, dev: int) -> int | None:
+    """The address of an optional contiguous tensor."""
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+            and t.get_device() == dev):
+        _need_float(t, name, (dtype,), len(shape), dev)
+        _need_shape(t, name, shape)
+        raise MoeError(4, f"{name} must be contiguous (ND format)")
+    return t.data_ptr()
+
+
+def MoeLinearInt8(x: torch.Tensor, xScale: torch.Tensor, weight: torch.Tensor, weightScale: torch.Tensor,
+                  offsets: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                  residual: torch.Tensor | None = None, activation: str = "none",
+                  outDtype: torch.dtype = torch.float16, workspace: torch.Tensor | None = None,
+                  stream=None) -> torch.Tensor:
+    """act((x[T,H] @ weight[N,H]^T) * xScale[T] * weightScale[N] + bias[N]) + residual[T,N] -> y[T,N] of outDtype (fp16,
+    bf16 or fp32), x and weight int8, scales fp32, bias and residual of outDtype; int32 sums, rounded once.
+
+    With offsets[E+1] int32, weight[E,N,H], weightScale[E,N] and bias[E,N] are E experts': rows [offsets[e], offsets[e+1])
+    of x by the matrix of expert e (MoePermute's rows and offsets); rows from offsets[E] on become zeros. activation as
+    MoeLinear's (swiglu: 2N weight rows, the N gate rows first). H <= 131071. Rows of x and of weight may be any stride
+    apart; multiples of 16 (H too) run at full speed. `workspace` (uint8, >= linear_int8_workspace_bytes) is allocated
+    when not given."""
+    act = _act_code(activation)
+    _, dev = _first_float(x, "x", _INT8, 2)
+    _need_float(weight, "weight", _INT8, 2 if offsets is None else 3, dev)
+    if outDtype not in _FLOATS:
+        raise MoeError(4, f"outDtype must be float32, float16 or bfloat16 (got {outDtype})")
+    T, H = x.shape
+    if offsets is None:
+        E, lead, step, rows = 0, (), 0, weight
+    else:
+        E = weight.shape[0]
+        if E < 1:
+            raise MoeError(3, "weight holds no experts")
+        lead, step, rows = (E,), weight.stride(0), weight[0]
+    Z = rows.shape[0]
+    if rows.shape[1] != H:
+        raise MoeError(3, f"hidden size mismatch x[{H}] vs weight[{rows.shape[1]}]")
+    swiglu = act == ACTIVATIONS["swiglu"]
+    if swiglu and Z % 2:
+        raise MoeError(3, f"weight rows ({Z}) of a swiglu must be N gate and N up rows")
+    N = Z // 2 if swiglu else Z
+    sx = _contiguous(xScale, "xScale", torch.float32, (T,), dev)
+    sw = _contiguous(weightScale, "weightScale", torch.float32, (*lead, Z), dev)
+    if sx is None or sw is None:
+        raise MoeError(1, "xScale and weightScale must be tensors")
+    op = _contiguous(offsets, "offsets", torch.int32, (E + 1,), dev)
+    bp = _contiguous(bias, "bias", outDtype, (*lead, Z), dev)
+    rp = _contiguous(residual, "residual", outDtype, (T, N), dev)
+    ldx, ldw = _row_stride(x, "x"), _row_stride(rows, "weight")
+    lib = _lib.load()
+    like = _like(x)
+    workspace, wp, wb = _workspace(workspace, lib.moe_linear_int8_workspace_bytes, (T, N, H, E, act), like, dev, stream)
+    y = _empty(like, stream, (T, N), outDtype)
+    check(lib.moe_linear_int8(x.data_ptr(), ldx, sx, weight.data_ptr(), ldw, step, sw, op, bp, rp, y.data_ptr(), wp, wb, T,
+                              N, H, E, act, _FLOAT_DT[outDtype], _queue(stream, dev)))
+    return y
 
 
 def synth_normal_f16_(out: torch.Tensor, seed: int, stream_id: int, sigma_a: float, sigma_b: float | None = None,

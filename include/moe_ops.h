@@ -422,6 +422,28 @@ moe_status moe_unpermute_grad(const void* grad_y, int64_t grad_y_stride, const v
                               const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights,
                               int64_t num_tokens, int64_t hidden_size, int64_t top_k, int32_t dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------
+ * MoeLinearInt8: x[T, H] int8 with x_scale[T], weight[N, H] int8 (SwiGLU: [2N, H], N gate rows first) with
+ *   weight_scale[N] (SwiGLU: [2N]) -> y[T, N] = act((x weight^T) * x_scale * weight_scale + bias) + residual of out_dtype
+ *   (float32, float16 or bfloat16), int32 sums, rounded once. bias[N] (SwiGLU: [2N]) and residual[T, N] of out_dtype, or
+ *   NULL; residual may be y itself. x rows lie x_stride, weight rows weight_stride elements apart.
+ *   num_experts > 0: weight[E, N, H] (expert_stride elements apart), weight_scale[E, N] and bias[E, N] of E matrices, and
+ *   the rows [offsets[e], offsets[e + 1]) of x by the matrix of expert e, offsets[E + 1] ascending from 0 as moe_permute
+ *   writes them; rows from offsets[E] on are written as zeros, residual and all. Values that do not ascend or lie outside
+ *   [0, T] are taken into it: nothing outside the tensors is read or written. num_experts 0: offsets is not read.
+ *   Any strides and alignment; operands on 16 bytes with H and the strides multiples of 16 run at full speed, others go
+ *   through registers at a fraction of it. H <= 131071, where 32-bit sums end; N <= 2^20, E <= 256.
+ *   The workspace (0 where none is needed, always with experts; 16-byte aligned) holds partial sums of a product split
+ *   over H; calls in flight at the same time need one each. The sums are exact, so y does not depend on the launch.
+ * ---------------------------------------------------------------------------------------------------- */
+size_t moe_linear_int8_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int64_t num_experts,
+                                       int32_t activation);
+moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* weight,
+                           int64_t weight_stride, int64_t expert_stride, const float* weight_scale,
+                           const int32_t* offsets, const void* bias, const void* residual, void* y, void* workspace,
+                           size_t workspace_bytes, int64_t num_tokens, int64_t n, int64_t hidden_size,
+                           int64_t num_experts, int32_t activation, int32_t out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
