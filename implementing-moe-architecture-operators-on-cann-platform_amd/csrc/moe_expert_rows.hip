@@ -15,43 +15,45 @@ namespace moe {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / kWave;
-constexpr int kBuckets = 257;  // 256 experts and the picks of none
-constexpr int kPasses = 4;     // slots of a lane in one ranking
-constexpr int kChunkSlots = kThreads * kPasses;
-constexpr int64_t kStreamBytes = int64_t(128) << 20;  // results beyond this go past the caches
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kCopyThreads = 256;
+constexpr int kBuckets = 257;            // 256 experts and the picks of none
+constexpr int kSingleSlots = 8 * kSortThreads;
+constexpr int64_t kStreamBytes = int64_t(128) << 20;  // beyond this rows go past the caches
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;      // of a launch
 
-// Ranks the slots [s0, s0 + count) by bucket, count <= kChunkSlots: wave w has R consecutive ones from w R on, 64 at a
-// time. Lanes of the same bucket find each other with ballots over the bucket's bits, so a slot's place among the wave's
-// earlier ones is a popcount, and a count for each (wave, bucket) in LDS carries it on. counts[w][b]: the wave's slots,
-// then (scanned) those of the waves before; total[b]: the chunk's.
+// Ranks `count` slots, at most 64 PASSES a wave, by bucket: wave w has R consecutive ones from w R on, 64 at a time. Lanes
+// of the same bucket find each other with ballots over the bucket's bits, so a slot's place among the wave's earlier ones
+// is a popcount, and a count for each (wave, bucket) in LDS carries it on. counts[w][b]: in the end the slots of b in the
+// waves before w; total[b]: all of them.
+template <int PASSES>
 struct Ranking {
-    int bucket[kPasses], rank[kPasses];
-    int R, first;
+    int bucket[PASSES], rank[PASSES];  // bucket -1: no slot
+    int first, R;
 };
-__device__ __forceinline__ void rank_chunk(const int32_t* ids, int64_t s0, int count, int E, int* counts, int* total,
-                                           Ranking& k) {
+template <int PASSES>
+__device__ __forceinline__ void rank_slots_of(const int32_t* ids, int count, int E, int* counts, int* total,
+                                              Ranking<PASSES>& k) {
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    k.R = (count + kThreads - 1) / kThreads * kWave;
+    k.R = (count + kSortThreads - 1) / kSortThreads * kWave;
     k.first = wave * k.R;
     const int end = min(count, k.first + k.R);
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
+    for (int i = 0; i < PASSES; ++i) {
         const int s = k.first + i * kWave + lane;
-        const int e = s < end && i * kWave < k.R ? ids[s0 + s] : -1;
-        k.bucket[i] = s < end && i * kWave < k.R ? (e >= 0 && e < E ? e : E) : -1;
+        const int e = s < end ? ids[s] : -1;
+        k.bucket[i] = s >= end ? -1 : e >= 0 && e < E ? e : E;
     }
     const int B = E + 1;
-    for (int i = tid; i < kWaves * B; i += kThreads) counts[i] = 0;
+    for (int i = tid; i < kSortWaves * B; i += kSortThreads) counts[i] = 0;
     __syncthreads();
     const int bits = 32 - __builtin_clz(E);  // of the largest bucket, E
     const uint64_t below = (uint64_t{1} << lane) - 1;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
+    for (int i = 0; i < PASSES; ++i) {
         k.rank[i] = 0;
-        if (i * kWave >= k.R || k.first + i * kWave >= end) continue;  // uniform
+        if (k.first + i * kWave >= end) continue;  // uniform
         const bool valid = k.bucket[i] >= 0;
         uint64_t same = __ballot(valid);
         for (int b = 0; b < bits; ++b) {
@@ -67,10 +69,10 @@ __device__ __forceinline__ void rank_chunk(const int32_t* ids, int64_t s0, int c
         }
     }
     __syncthreads();
-    for (int b = tid; b < B; b += kThreads) {
+    for (int b = tid; b < B; b += kSortThreads) {
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < kSortWaves; ++w) {
             const int c = counts[w * B + b];
             counts[w * B + b] = sum;
             sum += c;
@@ -80,51 +82,55 @@ __device__ __forceinline__ void rank_chunk(const int32_t* ids, int64_t s0, int c
     __syncthreads();
 }
 
-// Exclusive sums over the buckets, by the first 5 waves; `part`: LDS of 8 ints. Every thread calls it; it ends with a
-// barrier.
-__device__ __forceinline__ void scan_buckets(const int* total, int B, int* start, int* part) {
+// start[b]: the experts' exclusive sums, and of the picks of none all experts'. By the first 256 threads; every thread
+// calls it, and it ends with a barrier.
+__device__ __forceinline__ void scan_buckets(const int* total, int E, int* start) {
+    __shared__ int part[4];
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id(), wave = tid / kWave;
-    const int v = tid < B ? total[tid] : 0;
+    const int v = tid < E ? total[tid] : 0;
     int incl = v;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
         const int o = __shfl_up(incl, d, kWave);
         if (lane >= d) incl += o;
     }
-    if (wave < 8 && lane == kWave - 1) part[wave] = incl;
+    if (wave < 4 && lane == kWave - 1) part[wave] = incl;
     __syncthreads();
-    if (tid < B) {
-        int carry = 0;
-        for (int w = 0; w < wave; ++w) carry += part[w];
-        start[tid] = carry + incl - v;
+    if (tid < E) {
+        for (int w = 0; w < wave; ++w) incl += part[w];
+        start[tid] = incl - v;
+        if (tid == E - 1) start[E] = incl;
     }
     __syncthreads();
 }
 
-// Slots of a chunk, whole tokens, and chunks
+// Whole tokens of a chunk, whose picks one workgroup ranks, and chunks: 1024 picks each, 4096 from 2^18 of them on
 struct Chunks {
-    int64_t tokens, count;
+    int tokens, slots;
+    int64_t count;
 };
 __host__ __device__ __forceinline__ Chunks chunks_of(int64_t T, int K) {
-    const int64_t tokens = kChunkSlots / K;  // K <= E <= 256
-    return Chunks{tokens, (T + tokens - 1) / tokens};
+    const int slots = T * K < int64_t(1) << 18 ? kSortThreads : 4 * kSortThreads;
+    const int tokens = slots / K;  // K <= 256
+    return Chunks{tokens, slots, (T + tokens - 1) / tokens};
 }
 
-// One chunk a workgroup: ranks[s] within the chunk, and the chunk's counts
-__global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
-    __shared__ int counts[kWaves * kBuckets], total[kBuckets];
+// One chunk a workgroup: each slot's rank within the chunk, and the chunk's counts
+template <int PASSES>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
+    __shared__ int counts[kSortWaves * kBuckets], total[kBuckets];
     const Chunks c = chunks_of(a.T, a.K);
     const int64_t s0 = static_cast<int64_t>(blockIdx.x) * c.tokens * a.K;
-    const int count = static_cast<int>(min(c.tokens * a.K, a.T * a.K - s0));
-    Ranking k;
-    rank_chunk(a.ids, s0, count, a.E, counts, total, k);
+    const int count = static_cast<int>(min(static_cast<int64_t>(c.tokens) * a.K, a.T * a.K - s0));
+    Ranking<PASSES> k;
+    rank_slots_of<PASSES>(a.ids + s0, count, a.E, counts, total, k);
     const int B = a.E + 1, lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave;
     int32_t* ranks = a.scratch + c.count * B;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i)
+    for (int i = 0; i < PASSES; ++i)
         if (k.bucket[i] >= 0)
             ranks[s0 + k.first + i * kWave + lane] = counts[wave * B + k.bucket[i]] + k.rank[i];
-    for (int b = static_cast<int>(threadIdx.x); b < B; b += kThreads)
+    for (int b = static_cast<int>(threadIdx.x); b < B; b += kSortThreads)
         a.scratch[static_cast<int64_t>(blockIdx.x) * B + b] = total[b];
 }
 
@@ -162,81 +168,101 @@ __device__ __forceinline__ void copy_row(const char* src, char* rows, int64_t ro
     }
 }
 
-// The places of a chunk's picks and the copies of its tokens. SINGLE: every workgroup ranks all slots (one chunk) for
-// itself, one launch; else the ranks and counts come from sort_count_kernel. Workgroup b of `per` for a chunk copies the
-// chunk's tokens [b tokens / per, (b + 1) tokens / per).
-template <bool SINGLE, bool NT>
-__global__ __launch_bounds__(kThreads) void sort_copy_kernel(SortArgs a, int per) {
-    __shared__ int counts[kWaves * kBuckets], total[kBuckets], start[kBuckets], part[8];
-    __shared__ int place[SINGLE ? kChunkSlots : 1];
+// A token's picks, 16 at a time: their places written down and its row copied there by the wave. place(k): of pick k.
+template <bool NT, typename F>
+__device__ __forceinline__ void copy_token(const SortArgs& a, int64_t t, F&& place) {
+    const int64_t row_bytes = static_cast<int64_t>(a.H) * a.bytes;
+    const char* src = static_cast<const char*>(a.x) + t * a.ldx * a.bytes;
+    for (int k0 = 0; k0 < a.K; k0 += 16) {
+        const int n = min(16, a.K - k0), lane = lane_id();
+        const int mine = lane < n ? place(k0 + lane) : 0;
+        if (lane < n) {
+            a.position[t * a.K + k0 + lane] = mine;
+            if (a.scale) a.row_scale[mine >= 0 ? mine : ~mine] = mine >= 0 ? a.scale[t] : 0.0f;
+        }
+        int p[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) p[k] = __builtin_amdgcn_readlane(mine, k);
+        copy_row<NT>(src, static_cast<char*>(a.rows), row_bytes, p, n);
+    }
+}
+
+// Few picks, one launch: every workgroup ranks all of them for itself and copies its share of the tokens
+template <int PASSES>
+__global__ __launch_bounds__(kSortThreads) void sort_single_kernel(SortArgs a) {
+    __shared__ int counts[kSortWaves * kBuckets], total[kBuckets], start[kBuckets];
+    __shared__ int places[PASSES * kSortThreads];
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int B = a.E + 1, S = static_cast<int>(a.T) * a.K;
+    Ranking<PASSES> k;
+    rank_slots_of<PASSES>(a.ids, S, a.E, counts, total, k);
+    scan_buckets(total, a.E, start);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+        if (k.bucket[i] >= 0) {
+            const int p = start[k.bucket[i]] + counts[wave * B + k.bucket[i]] + k.rank[i];
+            places[k.first + i * kWave + lane] = k.bucket[i] < a.E ? p : ~p;
+        }
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int b = tid; b < B; b += kSortThreads) a.offsets[b] = start[b];
+    for (int64_t t = static_cast<int64_t>(wave) * gridDim.x + blockIdx.x; t < a.T;
+         t += static_cast<int64_t>(kSortWaves) * gridDim.x)
+        copy_token<false>(a, t, [&](int k) { return places[t * a.K + k]; });
+}
+
+// The copies from sort_count_kernel's ranks and counts. Workgroup b of `per` for a chunk adds the counts of all chunks and
+// of those before its own, and copies the chunk's tokens [b tokens / per, (b + 1) tokens / per).
+template <bool NT>
+__global__ __launch_bounds__(kCopyThreads) void sort_copy_kernel(SortArgs a, int per) {
+    constexpr int kWaves = kCopyThreads / kWave;
+    __shared__ int total[kBuckets], before[kBuckets], start[kBuckets];
+    __shared__ int part[2][kCopyThreads];
+    const int tid = static_cast<int>(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int B = a.E + 1;
     const Chunks c = chunks_of(a.T, a.K);
     const int64_t chunk = static_cast<int64_t>(blockIdx.x) / per;
     const int piece = static_cast<int>(blockIdx.x) % per;
-    const int64_t t0 = chunk * c.tokens, tokens = min(c.tokens, a.T - t0);
+    const int64_t t0 = chunk * c.tokens, tokens = min(static_cast<int64_t>(c.tokens), a.T - t0);
     const int64_t first = t0 + tokens * piece / per, last = t0 + tokens * (piece + 1) / per;
     const int32_t* ranks = a.scratch + c.count * B;
-    if (SINGLE) {
-        Ranking k;
-        rank_chunk(a.ids, 0, static_cast<int>(a.T * a.K), a.E, counts, total, k);
-        scan_buckets(total, B, start, part);
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i)
-            if (k.bucket[i] >= 0) {
-                const int p = start[k.bucket[i]] + counts[wave * B + k.bucket[i]] + k.rank[i];
-                place[k.first + i * kWave + lane] = k.bucket[i] < a.E ? p : ~p;
-            }
-        __syncthreads();
-    } else {
-        // column sums of the counts over all chunks (total) and over those before this one (kept in counts)
-        for (int b = tid; b < B; b += kThreads) {
-            int sum = 0, before = 0;
+    // `lanes` threads for each of as many buckets as that leaves, every lanes-th chunk each; their sums meet in LDS
+    const int width = min(B, kCopyThreads), lanes = kCopyThreads / width, own = tid % width, j = tid / width;
+    for (int b0 = 0; b0 < B; b0 += width) {
+        const int b = b0 + own;
+        int sum = 0, pre = 0;
+        if (b < B && j < lanes) {
 #pragma unroll 8
-            for (int64_t i = 0; i < c.count; ++i) {
+            for (int64_t i = j; i < c.count; i += lanes) {
                 const int v = a.scratch[i * B + b];
-                before += i < chunk ? v : 0;
+                pre += i < chunk ? v : 0;
                 sum += v;
             }
+        }
+        part[0][tid] = sum;
+        part[1][tid] = pre;
+        __syncthreads();
+        if (j == 0 && b < B) {
+            for (int l = 1; l < lanes; ++l) {
+                sum += part[0][tid + l * width];
+                pre += part[1][tid + l * width];
+            }
             total[b] = sum;
-            counts[b] = before;
+            before[b] = pre;
         }
         __syncthreads();
-        scan_buckets(total, B, start, part);
     }
+    scan_buckets(total, a.E, start);
     if (blockIdx.x == 0)
-        for (int b = tid; b < B; b += kThreads) a.offsets[b] = start[b];
-    const int64_t row_bytes = static_cast<int64_t>(a.H) * a.bytes;
-    for (int64_t t = first + wave; t < last; t += kWaves) {
-        const char* src = static_cast<const char*>(a.x) + t * a.ldx * a.bytes;
-        const float scale = a.scale ? a.scale[t] : 0.0f;
-        for (int k0 = 0; k0 < a.K; k0 += 16) {
-            const int n = min(16, a.K - k0);
-            int p[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                if (k >= n) continue;
-                const int64_t s = t * a.K + k0 + k;
-                if (SINGLE) {
-                    p[k] = place[s];
-                } else {
-                    const int e = a.ids[s], b = e >= 0 && e < a.E ? e : a.E;
-                    const int at = start[b] + counts[b] + ranks[s];
-                    p[k] = b < a.E ? at : ~at;
-                }
-            }
-            if (lane == 0) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    if (k >= n) continue;
-                    a.position[t * a.K + k0 + k] = p[k];
-                    if (a.scale) a.row_scale[p[k] >= 0 ? p[k] : ~p[k]] = p[k] >= 0 ? scale : 0.0f;
-                }
-            }
-            copy_row<NT>(src, static_cast<char*>(a.rows), row_bytes, p, n);
-        }
-    }
+        for (int b = tid; b < B; b += kCopyThreads) a.offsets[b] = start[b];
+    for (int64_t t = first + wave; t < last; t += kWaves)
+        copy_token<NT>(a, t, [&](int k) {
+            const int64_t s = t * a.K + k;
+            const int e = a.ids[s], b = e >= 0 && e < a.E ? e : a.E;
+            const int p = start[b] + before[b] + ranks[s];
+            return b < a.E ? p : ~p;
+        });
 }
 
 __device__ __forceinline__ float load_weight(const void* w, int64_t at, int type) {
@@ -251,65 +277,85 @@ __device__ __forceinline__ void store_weight(void* w, int64_t at, int type, floa
 
 constexpr int kUnsortThreads = 256;
 
-// A thread has V values of a token; up to 8 rows are loaded before they are added, in ascending k
-template <typename T, int V>
+// A wave has STEPS steps of V values a lane of a token; up to 8 rows are loaded before they are added, in ascending k.
+// The picks' places and weights are read once, a pick a lane.
+template <typename T, int V, int STEPS, bool NT>
 __global__ __launch_bounds__(kUnsortThreads) void unsort_kernel(UnsortArgs a) {
     using Bits = typename T::Bits;
-    constexpr int kBatch = 8;
-    const int steps = (a.H + V - 1) / V;
-    const int64_t work = a.T * steps;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kUnsortThreads + threadIdx.x; i < work;
-         i += static_cast<int64_t>(gridDim.x) * kUnsortThreads) {
-        const int64_t t = i / steps;
-        const int col = step_at<V>(static_cast<int>(i - t * steps) * V, a.H).at;
-        float y[V] = {};
+    constexpr int kBatch = 8, kSpan = STEPS * kWave * V, kWaves = kUnsortThreads / kWave;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int spans = (a.H + kSpan - 1) / kSpan;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kWaves + wave; i < a.T * spans;
+         i += static_cast<int64_t>(gridDim.x) * kWaves) {
+        const int64_t t = i / spans;
+        Step<V> at[STEPS];
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c)
+            at[c] = step_at<V>(static_cast<int>(i - t * spans) * kSpan + (c * kWave + lane) * V, a.H);
+        float y[STEPS][V] = {};
         for (int k0 = 0; k0 < a.K; k0 += kBatch) {
-            RawRow<T, V> v[kBatch];
-            float w[kBatch];
-            bool live[kBatch];
+            int p = -1;
+            float w = 0.0f;
+            if (lane < kBatch && k0 + lane < a.K) {
+                p = a.position[t * a.K + k0 + lane];
+                if (p >= a.R) p = -1;
+                if (p >= 0) w = a.weights ? load_weight(a.weights, t * a.K + k0 + lane, a.weights_type) : 1.0f;
+            }
+            RawRow<T, V> v[kBatch][STEPS];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                const int p = k0 + u < a.K ? a.position[t * a.K + k0 + u] : -1;
-                live[u] = p >= 0 && p < a.R;
-                if (!live[u]) continue;
-                v[u].load(static_cast<const Bits*>(a.rows) + static_cast<int64_t>(p) * a.H + col);
-                w[u] = a.weights ? load_weight(a.weights, t * a.K + k0 + u, a.weights_type) : 1.0f;
+                const int row = __builtin_amdgcn_readlane(p, u);
+                if (row < 0) continue;
+                const Bits* src = static_cast<const Bits*>(a.rows) + static_cast<int64_t>(row) * a.H;
+#pragma unroll
+                for (int c = 0; c < STEPS; ++c) v[u][c].template load<NT>(src + at[c].at);
             }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                if (!live[u]) continue;
+                if (__builtin_amdgcn_readlane(p, u) < 0) continue;
+                const float weight = of_lane(w, u);
 #pragma unroll
-                for (int j = 0; j < V; ++j) y[j] += w[u] * v[u].get(j);
+                for (int c = 0; c < STEPS; ++c)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[c][j] += weight * v[u][c].get(j);
             }
         }
-        store_row<T, V>(static_cast<Bits*>(a.y) + t * a.H + col, y);
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c)
+            if (at[c].live) store_row<T, V>(static_cast<Bits*>(a.y) + t * a.H + at[c].at, y[c]);
     }
 }
 
-// One or four waves a token; the dot products are added over the lanes and then over the waves in a fixed order
+// 1, 2 or 4 waves a token, 8 of its rows at a time; the picks' places and weights are read once, a pick a lane. The dot
+// products are added over the lanes and then over the waves in a fixed order.
 template <typename T, int WAVES, int V, bool NT>
 __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs a) {
     using Bits = typename T::Bits;
-    constexpr int kBatch = 8, kTokens = 4 / WAVES;
-    __shared__ float part[4][kBatch];
-    const int tid = static_cast<int>(threadIdx.x), wave = tid / kWave, lane = lane_id();
-    const int first = (WAVES == 1 ? lane : tid) * V;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + (WAVES == 1 ? wave : 0); t < a.T;
-         t += static_cast<int64_t>(gridDim.x) * kTokens) {
+    constexpr int kBatch = 8, kTokens = kUnsortThreads / (WAVES * kWave);
+    __shared__ float part[kUnsortThreads / kWave][kBatch];
+    const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), team = wave / WAVES;
+    const int first = tid % (WAVES * kWave) * V;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTokens; base < a.T;
+         base += static_cast<int64_t>(gridDim.x) * kTokens) {
+        const bool token = base + team < a.T;
+        const int64_t t = token ? base + team : a.T - 1;
         const Bits* gy = static_cast<const Bits*>(a.grad_y) + t * a.ldy;
         for (int k0 = 0; k0 < a.K; k0 += kBatch) {
-            float dot[kBatch] = {}, w[kBatch];
-            int row[kBatch];  // -1: none, nothing is read or written
-            bool live[kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int64_t at = t * a.K + k0 + u;
-                const int p = k0 + u < a.K ? a.position[at] : 0;
-                row[u] = p >= 0 ? p : ~p;
-                if (k0 + u >= a.K || row[u] >= a.R) row[u] = -1;
-                live[u] = p >= 0 && row[u] >= 0;
-                w[u] = !live[u] ? 0.0f : a.weights ? load_weight(a.weights, at, a.weights_type) : 1.0f;
+            // of pick k0 + lane: its row (past the rows: none, nothing is read or written), whether an expert has it
+            int row = -1;
+            bool live = false;
+            float w = 0.0f;
+            if (token && lane < kBatch && k0 + lane < a.K) {
+                const int64_t at = t * a.K + k0 + lane;
+                const int p = a.position[at];
+                row = p >= 0 ? p : ~p;
+                if (row >= a.R) row = -1;
+                live = p >= 0 && row >= 0;
+                if (live) w = a.weights ? load_weight(a.weights, at, a.weights_type) : 1.0f;
             }
+            const uint64_t lives = __ballot(live);
+            float dot[kBatch] = {};
             for (int c = first; c < a.H; c += WAVES * kWave * V) {
                 const Step<V> s = step_at<V>(c, a.H);
                 RawRow<T, V> d, v[kBatch];
@@ -317,114 +363,134 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
                 if (a.weights) {
 #pragma unroll
                     for (int u = 0; u < kBatch; ++u)
-                        if (live[u])
-                            v[u].load(static_cast<const Bits*>(a.rows) + static_cast<int64_t>(row[u]) * a.H + s.at);
+                        if (lives >> u & 1)
+                            v[u].template load<NT>(static_cast<const Bits*>(a.rows) +
+                                                   static_cast<int64_t>(__builtin_amdgcn_readlane(row, u)) * a.H + s.at);
                 }
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
-                    if (row[u] < 0) continue;
+                    const int to = __builtin_amdgcn_readlane(row, u);
+                    if (to < 0) continue;
+                    const bool on = lives >> u & 1;
+                    const float weight = of_lane(w, u);
                     float g[V];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) g[j] = live[u] ? w[u] * d.get(j) : 0.0f;
-                    if (a.weights && live[u]) {
+                    for (int j = 0; j < V; ++j) g[j] = on ? weight * d.get(j) : 0.0f;
+                    if (a.weights && on) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) dot[u] += j >= s.skip ? d.get(j) * v[u].get(j) : 0.0f;
                     }
-                    store_row<T, V, NT>(static_cast<Bits*>(a.y) + static_cast<int64_t>(row[u]) * a.H + s.at, g);
+                    store_row<T, V, NT>(static_cast<Bits*>(a.y) + static_cast<int64_t>(to) * a.H + s.at, g);
                 }
             }
             if (!a.weights) continue;
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u)
+            for (int u = 0; u < kBatch; ++u) dot[u] = wave_sum(dot[u]);
+            float v = dot[0];
 #pragma unroll
-                for (int s = kWave / 2; s > 0; s >>= 1) dot[u] += __shfl_xor(dot[u], s, kWave);
-            if (WAVES == 1) {
-                float v = dot[0];
+            for (int u = 1; u < kBatch; ++u) v = lane == u ? dot[u] : v;
+            if (WAVES > 1) {
+                if (lane < kBatch) part[wave][lane] = v;
+                __syncthreads();
+                if (lane < kBatch) {
+                    v = part[team * WAVES][lane];
 #pragma unroll
-                for (int u = 1; u < kBatch; ++u) v = lane == u ? dot[u] : v;
-                if (lane < kBatch && k0 + lane < a.K) store_weight(a.grad_weights, t * a.K + k0 + lane, a.weights_type, v);
-            } else {
-                if (lane == 0) {
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) part[wave][u] = dot[u];
+                    for (int x = 1; x < WAVES; ++x) v += part[team * WAVES + x][lane];
                 }
                 __syncthreads();
-                if (tid < kBatch && k0 + tid < a.K)
-                    store_weight(a.grad_weights, t * a.K + k0 + tid, a.weights_type,
-                                 part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]);
-                __syncthreads();
             }
+            if (token && wave % WAVES == 0 && lane < kBatch && k0 + lane < a.K)
+                store_weight(a.grad_weights, t * a.K + k0 + lane, a.weights_type, v);
         }
     }
 }
 
+template <typename T, int V, int STEPS, bool NT>
+void run_unsort(const UnsortArgs& u, hipStream_t stream) {
+    constexpr int kWaves = kUnsortThreads / kWave;
+    const int64_t spans = (u.H + STEPS * kWave * V - 1) / (STEPS * kWave * V), blocks = (u.T * spans + kWaves - 1) / kWaves;
+    unsort_kernel<T, V, STEPS, NT>
+        <<<static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks), kUnsortThreads, 0, stream>>>(u);
+}
 template <typename T>
-void run_unsort(const UnsortArgs& u, unsigned grid, hipStream_t stream) {
-    if (u.H < 8) unsort_kernel<T, 1><<<grid, kUnsortThreads, 0, stream>>>(u);
-    else unsort_kernel<T, 8><<<grid, kUnsortThreads, 0, stream>>>(u);
+void run_unsort_any(const UnsortArgs& u, hipStream_t stream) {
+    const bool nt = u.R * u.H * static_cast<int64_t>(sizeof(typename T::Bits)) > kStreamBytes;
+    const bool two = u.T >= 2048 && u.H > 512;
+    if (u.H < 8) run_unsort<T, 1, 1, false>(u, stream);
+    else if (two) nt ? run_unsort<T, 8, 2, true>(u, stream) : run_unsort<T, 8, 2, false>(u, stream);
+    else nt ? run_unsort<T, 8, 1, true>(u, stream) : run_unsort<T, 8, 1, false>(u, stream);
 }
 
+template <typename T, int WAVES, int V>
+void run_unsort_grad(const UnsortArgs& u, hipStream_t stream) {
+    constexpr int kTokens = kUnsortThreads / (WAVES * kWave);
+    const int64_t blocks = (u.T + kTokens - 1) / kTokens;
+    const unsigned grid = static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
+    if (u.R * u.H * static_cast<int64_t>(sizeof(typename T::Bits)) > kStreamBytes)
+        unsort_grad_kernel<T, WAVES, V, true><<<grid, kUnsortThreads, 0, stream>>>(u);
+    else
+        unsort_grad_kernel<T, WAVES, V, false><<<grid, kUnsortThreads, 0, stream>>>(u);
+}
+// A wave a token once that gives every SIMD two of them, or where it has a token's row in one step
 template <typename T>
-void run_unsort_grad(const UnsortArgs& u, unsigned grid, bool one, bool nt, hipStream_t stream) {
-    if (u.H < 8) unsort_grad_kernel<T, 1, 1, false><<<grid, kUnsortThreads, 0, stream>>>(u);
-    else if (one && nt) unsort_grad_kernel<T, 1, 8, true><<<grid, kUnsortThreads, 0, stream>>>(u);
-    else if (one) unsort_grad_kernel<T, 1, 8, false><<<grid, kUnsortThreads, 0, stream>>>(u);
-    else if (nt) unsort_grad_kernel<T, 4, 8, true><<<grid, kUnsortThreads, 0, stream>>>(u);
-    else unsort_grad_kernel<T, 4, 8, false><<<grid, kUnsortThreads, 0, stream>>>(u);
+void run_unsort_grad_any(const UnsortArgs& u, hipStream_t stream) {
+    if (u.H < 8) run_unsort_grad<T, 1, 1>(u, stream);
+    else if (u.T >= 2048 || u.H <= 512) run_unsort_grad<T, 1, 8>(u, stream);
+    else if (u.H <= 1024) run_unsort_grad<T, 2, 8>(u, stream);
+    else run_unsort_grad<T, 4, 8>(u, stream);
 }
 
 }  // namespace
 
 // chunks' counts [chunks][E + 1], ranks [T K]
 size_t sort_scratch_bytes(int64_t T, int E, int K) {
-    if (T * K <= kChunkSlots) return 0;
+    if (T * K <= kSingleSlots) return 0;
     return static_cast<size_t>(chunks_of(T, K).count * (E + 1) + T * K) * sizeof(int32_t);
 }
 
 hipError_t launch_sort(const SortArgs& s, hipStream_t stream) {
-    const bool nt = s.T * s.K * s.H * s.bytes > kStreamBytes;
-    if (s.T * s.K <= kChunkSlots) {
+    const int64_t S = s.T * s.K;
+    if (S <= kSingleSlots) {
         TraceScope trace("moe_sort_rows", stream);
-        const int64_t most = (s.T + kWaves - 1) / kWaves;  // workgroups that have tokens
-        const int per = static_cast<int>(most < 1 ? 1 : most < 256 ? most : 256);
-        if (nt) sort_copy_kernel<true, true><<<per, kThreads, 0, stream>>>(s, per);
-        else sort_copy_kernel<true, false><<<per, kThreads, 0, stream>>>(s, per);
+        const int grid = static_cast<int>(s.T < 1 ? 1 : s.T < 256 ? s.T : 256);
+        if (S <= kSortThreads) sort_single_kernel<1><<<grid, kSortThreads, 0, stream>>>(s);
+        else sort_single_kernel<kSingleSlots / kSortThreads><<<grid, kSortThreads, 0, stream>>>(s);
         return hipGetLastError();
     }
     const Chunks c = chunks_of(s.T, s.K);
     {
         TraceScope trace("moe_sort_count", stream);
-        sort_count_kernel<<<static_cast<unsigned>(c.count), kThreads, 0, stream>>>(s);
+        if (c.slots == kSortThreads)
+            sort_count_kernel<1><<<static_cast<unsigned>(c.count), kSortThreads, 0, stream>>>(s);
+        else
+            sort_count_kernel<4><<<static_cast<unsigned>(c.count), kSortThreads, 0, stream>>>(s);
     }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     TraceScope trace("moe_sort_rows", stream);
-    const int per = static_cast<int>(c.count < 512 ? (512 + c.count - 1) / c.count : 1);
+    // a token a wave, but no more than 2048 workgroups where a chunk has one
+    constexpr int kWaves = kCopyThreads / kWave;
+    const int64_t most = c.count < 2048 ? 2048 / c.count : 1, want = (c.tokens + kWaves - 1) / kWaves;
+    const int per = static_cast<int>(want < most ? want : most);
     const unsigned grid = static_cast<unsigned>(c.count * per);
-    if (nt) sort_copy_kernel<false, true><<<grid, kThreads, 0, stream>>>(s, per);
-    else sort_copy_kernel<false, false><<<grid, kThreads, 0, stream>>>(s, per);
+    if (S * s.H * s.bytes > kStreamBytes) sort_copy_kernel<true><<<grid, kCopyThreads, 0, stream>>>(s, per);
+    else sort_copy_kernel<false><<<grid, kCopyThreads, 0, stream>>>(s, per);
     return hipGetLastError();
 }
 
 hipError_t launch_unsort(const UnsortArgs& u, hipStream_t stream) {
     TraceScope trace("moe_unsort_rows", stream);
-    const int64_t steps = u.H < 8 ? u.H : (u.H + 7) / 8, blocks = (u.T * steps + kUnsortThreads - 1) / kUnsortThreads;
-    const unsigned grid = static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
-    if (u.type == MOE_DT_FLOAT32) run_unsort<F32>(u, grid, stream);
-    else if (u.type == MOE_DT_FLOAT16) run_unsort<Half>(u, grid, stream);
-    else run_unsort<Bf16>(u, grid, stream);
+    if (u.type == MOE_DT_FLOAT32) run_unsort_any<F32>(u, stream);
+    else if (u.type == MOE_DT_FLOAT16) run_unsort_any<Half>(u, stream);
+    else run_unsort_any<Bf16>(u, stream);
     return hipGetLastError();
 }
 
 hipError_t launch_unsort_grad(const UnsortArgs& u, hipStream_t stream) {
     TraceScope trace("moe_unsort_grad", stream);
-    const bool one = u.T >= 2048 || u.H < 8;  // a wave a token once that gives every SIMD two waves
-    const bool nt = u.R * u.H * (u.type == MOE_DT_FLOAT32 ? 4 : 2) > kStreamBytes;
-    const int64_t blocks = one ? (u.T + 3) / 4 : u.T;
-    const unsigned grid = static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
-    if (u.type == MOE_DT_FLOAT32) run_unsort_grad<F32>(u, grid, one, nt, stream);
-    else if (u.type == MOE_DT_FLOAT16) run_unsort_grad<Half>(u, grid, one, nt, stream);
-    else run_unsort_grad<Bf16>(u, grid, one, nt, stream);
+    if (u.type == MOE_DT_FLOAT32) run_unsort_grad_any<F32>(u, stream);
+    else if (u.type == MOE_DT_FLOAT16) run_unsort_grad_any<Half>(u, stream);
+    else run_unsort_grad_any<Bf16>(u, stream);
     return hipGetLastError();
 }
 

@@ -17,7 +17,7 @@ namespace {
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;  // of a launch
 
-// Sum and largest over the WAVES waves of a row, the same on every lane; `ex`: LDS for the waves' parts
+// Sum and largest (TWO: two sums) over the WAVES waves of a row, the same on every lane; `ex`: LDS for the waves' parts
 template <int WAVES>
 struct RowExchange {
     double a[WAVES], b[WAVES];
@@ -25,14 +25,11 @@ struct RowExchange {
 };
 template <int WAVES, bool TWO>
 __device__ __forceinline__ void reduce_row(RowExchange<WAVES>& ex, double& a, double& b, uint32_t& top) {
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) {
-        a += __shfl_xor(a, d, kWave);
-        if (TWO) b += __shfl_xor(b, d, kWave);
-        else top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, kWave)));
-    }
+    a = wave_sum(a);
+    if (TWO) b = wave_sum(b);
+    else top = wave_max(top);
     if (WAVES == 1) return;
-    const int wave = static_cast<int>(threadIdx.x) / kWave;
+    const int wave = static_cast<int>(threadIdx.x) / kWave % WAVES;
     if (lane_id() == 0) {
         ex.a[wave] = a;
         if (TWO) ex.b[wave] = b;
@@ -176,118 +173,140 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_kernel(
     }
 }
 
-// The gradient. A workgroup walks rows and keeps its share of grad_gamma's column sums in registers; they leave as one
-// row of `part` for each workgroup.
-template <typename T, typename G, int WAVES, int CHUNKS, int V>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_grad_kernel(NormArgs n) {
+// The gradient. A workgroup walks rows, at least 4 waves' worth at a time, and keeps its share of grad_gamma's column sums
+// in registers; they leave as one row of `part` for each workgroup.
+constexpr int grad_threads(int waves) { return waves <= 4 ? 256 : waves * kWave; }
+template <typename T, typename G, int WAVES, int STEPS, int V>
+__global__ __launch_bounds__(grad_threads(WAVES)) void norm_grad_kernel(NormArgs n) {
     using Bits = typename T::Bits;
-    constexpr int kRows = WAVES == 1 ? 4 : 1;
+    constexpr int kRows = grad_threads(WAVES) / (WAVES * kWave);
     constexpr int kStep = WAVES * kWave * V;
-    __shared__ RowExchange<WAVES> ex;
-    __shared__ float sums[WAVES == 1 ? 4 : 1][WAVES == 1 ? CHUNKS * kStep : 1];
-    const int wave = static_cast<int>(threadIdx.x) / kWave, lead = WAVES == 1 ? lane_id() : static_cast<int>(threadIdx.x);
+    __shared__ RowExchange<WAVES> ex[kRows];
+    __shared__ float sums[kRows > 1 ? kRows - 1 : 1][kRows > 1 ? STEPS * kStep : 1];
+    const int team = static_cast<int>(threadIdx.x) / (WAVES * kWave), lead = static_cast<int>(threadIdx.x) % (WAVES * kWave);
     const typename G::Bits* gamma = static_cast<const typename G::Bits*>(n.gamma);
-    Step<V> at[CHUNKS];
+    Step<V> at[STEPS];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) at[c] = step_at<V>(lead * V + c * kStep, n.H);
-    float gg[CHUNKS][V] = {};
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0); row < n.rows;
-         row += static_cast<int64_t>(gridDim.x) * kRows) {
+    for (int c = 0; c < STEPS; ++c) at[c] = step_at<V>(lead * V + c * kStep, n.H);
+    float gg[STEPS][V] = {};
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < n.rows;
+         base += static_cast<int64_t>(gridDim.x) * kRows) {
+        const bool live = base + team < n.rows;  // past the last row: that row again, for nothing
+        const int64_t row = live ? base + team : n.rows - 1;
         const Bits* x = static_cast<const Bits*>(n.x) + row * n.ldx;
         const Bits* gy = static_cast<const Bits*>(n.grad_y) + row * n.ldy;
-        RawRow<T, V> v[CHUNKS], d[CHUNKS];
+        RawRow<T, V> v[STEPS], d[STEPS], add[STEPS];
         double squares = 0.0, dot = 0.0;
         uint32_t unused = 0;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
+        for (int c = 0; c < STEPS; ++c) {
             v[c].load(x + at[c].at);
             d[c].load(gy + at[c].at);
         }
+        if (n.grad_sum) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
+            for (int c = 0; c < STEPS; ++c)
+                add[c].load(static_cast<const Bits*>(n.grad_sum) + row * n.lds + at[c].at);
+        }
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
             float g[V];
             load_row<G, V>(gamma + at[c].at, g);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const double a = j >= at[c].skip ? v[c].get(j) : 0.0f;  // of a live step V = skip at least
+                const bool counts = j >= at[c].skip;  // past the row all are to be skipped
+                const double a = counts ? v[c].get(j) : 0.0f;
                 squares += a * a;
-                dot += static_cast<double>(j >= at[c].skip ? d[c].get(j) * g[j] : 0.0f) * a;
+                dot += static_cast<double>(counts ? d[c].get(j) * g[j] : 0.0f) * a;
             }
         }
-        reduce_row<WAVES, true>(ex, squares, dot, unused);
+        reduce_row<WAVES, true>(ex[team], squares, dot, unused);
+        if (!live) continue;
         const RowFactor s = row_factor(squares, n.H, n.eps);
         const float r = s.f * s.r;
         const float mean = static_cast<float>(dot * s.f * s.r / n.H);  // of grad_y gamma u
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
+        for (int c = 0; c < STEPS; ++c) {
             float g[V], gx[V];
-            RawRow<T, V> add;
             load_row<G, V>(gamma + at[c].at, g);
-            if (n.grad_sum) add.load(static_cast<const Bits*>(n.grad_sum) + row * n.lds + at[c].at);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float u = v[c].get(j) * s.f * s.r, gv = d[c].get(j);
                 gg[c][j] += gv * u;
                 gx[j] = r * (gv * g[j] - u * mean);
-                if (n.grad_sum) gx[j] += add.get(j);
+                if (n.grad_sum) gx[j] += add[c].get(j);
             }
             if (n.y && at[c].live) store_row<T, V>(static_cast<Bits*>(n.y) + row * n.H + at[c].at, gx);
         }
     }
     if (!n.part) return;
-    float* out = n.part + static_cast<int64_t>(blockIdx.x) * n.H;
-    if (WAVES == 1) {
+    if (kRows > 1) {  // the teams' sums, added in order
+        if (team > 0) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-            if (at[c].live) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) sums[wave][at[c].at + j] = gg[c][j];
-            }
+            for (int c = 0; c < STEPS; ++c)
+                if (at[c].live) store_row<F32, V>(&sums[team - 1][at[c].at], gg[c]);
+        }
         __syncthreads();
-        for (int i = static_cast<int>(threadIdx.x); i < n.H; i += 256)
-            out[i] = sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i];
-    } else {
+        if (team > 0) return;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-            if (at[c].live) store_row<F32, V>(out + at[c].at, gg[c]);
+        for (int t = 0; t + 1 < kRows; ++t)
+#pragma unroll
+            for (int c = 0; c < STEPS; ++c) {
+                float other[V];
+                load_row<F32, V>(&sums[t][at[c].at], other);
+#pragma unroll
+                for (int j = 0; j < V; ++j) gg[c][j] += other[j];
+            }
     }
+    float* out = n.part + static_cast<int64_t>(blockIdx.x) * n.H;
+#pragma unroll
+    for (int c = 0; c < STEPS; ++c)
+        if (at[c].live) store_row<F32, V>(out + at[c].at, gg[c]);
 }
 
-// grad_gamma: the workgroups' rows added in order, 16 columns a workgroup and 64 groups of rows
+// grad_gamma: the workgroups' rows, 16 columns a workgroup; 64 groups add every 64th row, 8 of them 8 groups' sums, and
+// one those
 constexpr int kSumThreads = 1024;
 template <typename G>
 __global__ __launch_bounds__(kSumThreads) void gamma_sum_kernel(const float* __restrict__ part,
                                                                 typename G::Bits* __restrict__ out, int H, int rows) {
-    constexpr int kCols = 16, kGroups = kSumThreads / kCols;
-    __shared__ float sums[kGroups][kCols];
+    constexpr int kCols = 16, kGroups = kSumThreads / kCols, kFirst = 8;
+    __shared__ float sums[kGroups][kCols], eighths[kFirst][kCols];
     const int i = static_cast<int>(threadIdx.x) % kCols, q = static_cast<int>(threadIdx.x) / kCols;
     const int col = static_cast<int>(blockIdx.x) * kCols + i;
     float s = 0.0f;
     if (col < H) {
-#pragma unroll 8
+#pragma unroll 16
         for (int b = q; b < rows; b += kGroups) s += part[static_cast<int64_t>(b) * H + col];
     }
     sums[q][i] = s;
     __syncthreads();
+    if (q < kFirst) {
+        s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kGroups / kFirst; ++g) s += sums[q + g * kFirst][i];
+        eighths[q][i] = s;
+    }
+    __syncthreads();
     if (q != 0 || col >= H) return;
-    for (int g = 1; g < kGroups; ++g) s += sums[g][i];
+    s = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kFirst; ++g) s += eighths[g][i];
     out[col] = G::store(s);
 }
 
-// Waves of a row and its steps. A row of up to 2048 values has a wave to itself where there are rows enough for every
-// SIMD; else, and where it is longer, 4 or 16 waves share it.
+// Waves of a row, and the steps that hold it (0: none do). Where there are rows enough for every SIMD a row has two steps
+// in flight for as few waves as that takes; few rows are spread over as many waves as have one step each.
+//   x + residual with y and its 8-bit form, bf16, us with 1, 2, 4 waves: T = 16384, H = 512 18 / 22 / 34; H = 1024 32 / 31
+//   / 42; H = 2048 74 (four steps) / 58 / 59; T = 98304, H = 1408 328 / 244 / 260
 struct Shape {
-    int waves, chunks;
+    int waves, steps;
 };
-int steps(int H, int waves) {
-    const int c = (H + waves * kWave * 8 - 1) / (waves * kWave * 8);
-    return c <= 1 ? 1 : c <= 2 ? 2 : c <= 4 ? 4 : 0;
-}
 Shape norm_shape(int64_t rows, int H) {
-    const bool many = rows >= 2048;
-    if (H <= 512 || (many && H <= 2048)) return Shape{1, steps(H, 1)};
-    if (H <= 2048 || (many && H <= 8192)) return Shape{4, steps(H, 4)};
-    return Shape{16, steps(H, 16)};
+    const int reach = rows >= 2048 ? 1024 : 512;  // values that a wave holds
+    for (int waves = 1; waves <= 16; waves *= 2)
+        if (H <= waves * reach) return Shape{waves, (H + waves * 512 - 1) / (waves * 512)};
+    return Shape{16, H <= 16384 ? 2 : H <= 32768 ? 4 : 0};
 }
 unsigned norm_grid(int64_t rows, int waves) {
     const int64_t blocks = waves == 1 ? (rows + 3) / 4 : rows;
@@ -304,29 +323,36 @@ template <typename T, typename G, bool NORM>
 hipError_t run_norm_any(const NormArgs& n, hipStream_t stream) {
     if (n.H < 8) return run_norm<T, G, 1, 1, NORM, 1>(n, stream);
     const Shape s = norm_shape(n.rows, n.H);
-    if (s.waves == 1) {
-        if (s.chunks == 1) return run_norm<T, G, 1, 1, NORM>(n, stream);
-        return s.chunks == 2 ? run_norm<T, G, 1, 2, NORM>(n, stream) : run_norm<T, G, 1, 4, NORM>(n, stream);
+    switch (s.waves * 8 + s.steps) {
+        case 1 * 8 + 1: return run_norm<T, G, 1, 1, NORM>(n, stream);
+        case 1 * 8 + 2: return run_norm<T, G, 1, 2, NORM>(n, stream);
+        case 2 * 8 + 1: return run_norm<T, G, 2, 1, NORM>(n, stream);
+        case 2 * 8 + 2: return run_norm<T, G, 2, 2, NORM>(n, stream);
+        case 4 * 8 + 1: return run_norm<T, G, 4, 1, NORM>(n, stream);
+        case 4 * 8 + 2: return run_norm<T, G, 4, 2, NORM>(n, stream);
+        case 8 * 8 + 1: return run_norm<T, G, 8, 1, NORM>(n, stream);
+        case 8 * 8 + 2: return run_norm<T, G, 8, 2, NORM>(n, stream);
+        case 16 * 8 + 1: return run_norm<T, G, 16, 1, NORM>(n, stream);
+        case 16 * 8 + 2: return run_norm<T, G, 16, 2, NORM>(n, stream);
+        case 16 * 8 + 4: return run_norm<T, G, 16, 4, NORM>(n, stream);
+        default: return run_norm<T, G, 16, 0, NORM>(n, stream);
     }
-    if (s.waves == 4) {
-        if (s.chunks == 1) return run_norm<T, G, 4, 1, NORM>(n, stream);
-        return s.chunks == 2 ? run_norm<T, G, 4, 2, NORM>(n, stream) : run_norm<T, G, 4, 4, NORM>(n, stream);
-    }
-    if (s.chunks == 1) return run_norm<T, G, 16, 1, NORM>(n, stream);
-    if (s.chunks == 2) return run_norm<T, G, 16, 2, NORM>(n, stream);
-    return s.chunks == 4 ? run_norm<T, G, 16, 4, NORM>(n, stream) : run_norm<T, G, 16, 0, NORM>(n, stream);
 }
 
-template <typename T, typename G>
+template <typename T, typename G, int WAVES, int STEPS, int V = 8>
 hipError_t run_norm_grad(const NormArgs& n, int blocks, hipStream_t stream) {
-    if (n.H < 8) norm_grad_kernel<T, G, 1, 1, 1><<<blocks, 256, 0, stream>>>(n);
-    else if (n.H <= 512) norm_grad_kernel<T, G, 1, 1, 8><<<blocks, 256, 0, stream>>>(n);
-    else if (n.H <= 1024) norm_grad_kernel<T, G, 1, 2, 8><<<blocks, 256, 0, stream>>>(n);
-    else if (n.H <= 2048) norm_grad_kernel<T, G, 1, 4, 8><<<blocks, 256, 0, stream>>>(n);
-    else if (n.H <= 4096) norm_grad_kernel<T, G, 4, 2, 8><<<blocks, 256, 0, stream>>>(n);
-    else if (n.H <= 8192) norm_grad_kernel<T, G, 4, 4, 8><<<blocks, 256, 0, stream>>>(n);
-    else norm_grad_kernel<T, G, 16, 2, 8><<<blocks, 1024, 0, stream>>>(n);
+    norm_grad_kernel<T, G, WAVES, STEPS, V><<<blocks, grad_threads(WAVES), 0, stream>>>(n);
     return hipGetLastError();
+}
+template <typename T, typename G>
+hipError_t run_norm_grad_any(const NormArgs& n, int blocks, hipStream_t stream) {
+    if (n.H < 8) return run_norm_grad<T, G, 1, 1, 1>(n, blocks, stream);
+    if (n.H <= 512) return run_norm_grad<T, G, 1, 1>(n, blocks, stream);
+    if (n.H <= 1024) return run_norm_grad<T, G, 1, 2>(n, blocks, stream);
+    if (n.H <= 2048) return run_norm_grad<T, G, 2, 2>(n, blocks, stream);
+    if (n.H <= 4096) return run_norm_grad<T, G, 4, 2>(n, blocks, stream);
+    if (n.H <= 8192) return run_norm_grad<T, G, 8, 2>(n, blocks, stream);
+    return run_norm_grad<T, G, 16, 2>(n, blocks, stream);
 }
 
 // f(row type, gamma type) for the types of a call
@@ -348,10 +374,12 @@ hipError_t launch_norm(const NormArgs& n, int type, bool norm, hipStream_t strea
     });
 }
 
-// Workgroups of the gradient: two on every CU, and no more than have rows
+// Workgroups of the gradient, 16 waves on every CU at most. T = 8192, H = 2048, us of both launches: 2 waves a row and 1024
+// workgroups 31.5, 512 34.0; 1 wave (four steps) 33.1 with 512; 4 waves (one step) 33.5 with 1024
 int norm_grad_blocks(int64_t rows, int H) {
-    const int64_t most = H <= 2048 ? (rows + 3) / 4 : rows;
-    return static_cast<int>(most < 512 ? (most > 0 ? most : 1) : 512);
+    const int64_t most = H <= 2048 ? 1024 : H <= 8192 ? 512 : 256;
+    const int64_t blocks = H <= 1024 ? (rows + 3) / 4 : H <= 2048 ? (rows + 1) / 2 : rows;
+    return static_cast<int>(blocks < 1 ? 1 : blocks < most ? blocks : most);
 }
 
 hipError_t launch_norm_grad(const NormArgs& n, int type, void* grad_gamma, hipStream_t stream) {
@@ -360,7 +388,7 @@ hipError_t launch_norm_grad(const NormArgs& n, int type, void* grad_gamma, hipSt
     {
         TraceScope trace("moe_norm_grad", stream);
         err = by_type(type, n.gamma_f32, [&](auto t, auto g) {
-            return run_norm_grad<decltype(t), decltype(g)>(n, blocks, stream);
+            return run_norm_grad_any<decltype(t), decltype(g)>(n, blocks, stream);
         });
     }
     if (err != hipSuccess || !grad_gamma) return err;

@@ -37,10 +37,13 @@ template <typename T, int V>
 struct RawRow {
     static constexpr int kVectors = V * sizeof(typename T::Bits) / 16;
     u32x4 v[kVectors];
+    template <bool NT = false>  // past the caches
     __device__ __forceinline__ void load(const typename T::Bits* p) {
 #pragma unroll
-        for (int i = 0; i < kVectors; ++i)
-            v[i] = *reinterpret_cast<const u32x4_any*>(p + i * (16 / sizeof(typename T::Bits)));
+        for (int i = 0; i < kVectors; ++i) {
+            const u32x4_any* at = reinterpret_cast<const u32x4_any*>(p + i * (16 / sizeof(typename T::Bits)));
+            v[i] = NT ? __builtin_nontemporal_load(at) : *at;
+        }
     }
     __device__ __forceinline__ float get(int j) const {
         if constexpr (sizeof(typename T::Bits) == 4) {
@@ -54,6 +57,7 @@ struct RawRow {
 template <typename T>
 struct RawRow<T, 1> {
     typename T::Bits v;
+    template <bool NT = false>
     __device__ __forceinline__ void load(const typename T::Bits* p) { v = *p; }
     __device__ __forceinline__ float get(int) const { return T::load(v); }
 };
@@ -85,6 +89,48 @@ __device__ __forceinline__ void store_row(typename T::Bits* p, const float (&v)[
         for (int h = 0; h < 2; ++h)
             store16<NT>(p + 4 * h, __builtin_bit_cast(u32x4, f32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]}));
     }
+}
+
+// All-reduce over a whole wave, every lane active: the lanes of a DPP row of 16 by rotations, then the four rows' results
+template <int CTRL>
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ float turned(float v) {
+    return __builtin_bit_cast(float, turned<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double turned(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t hi = turned<CTRL>(static_cast<uint32_t>(b >> 32)), lo = turned<CTRL>(static_cast<uint32_t>(b));
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ float of_lane(float v, int lane) {
+    return __builtin_bit_cast(float, of_lane(__builtin_bit_cast(uint32_t, v), lane));
+}
+__device__ __forceinline__ double of_lane(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t hi = of_lane(static_cast<uint32_t>(b >> 32), lane), lo = of_lane(static_cast<uint32_t>(b), lane);
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+template <typename V>
+__device__ __forceinline__ V wave_sum(V v) {
+    v += turned<0x128>(v);
+    v += turned<0x124>(v);
+    v += turned<0x122>(v);
+    v += turned<0x121>(v);
+    return (of_lane(v, 0) + of_lane(v, 16)) + (of_lane(v, 32) + of_lane(v, 48));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, turned<0x128>(v));
+    v = max(v, turned<0x124>(v));
+    v = max(v, turned<0x122>(v));
+    v = max(v, turned<0x121>(v));
+    return max(max(of_lane(v, 0), of_lane(v, 16)), max(of_lane(v, 32), of_lane(v, 48)));
 }
 
 // Rows as 8-bit integers: q = rint(p * (127 / top)), top the row's largest magnitude; the quotient and the products are

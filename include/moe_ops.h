@@ -398,7 +398,7 @@ moe_status moe_quantize(const void* x, int64_t x_stride, int8_t* q, float* scale
  *   offsets[e + 1]), offsets[E + 1]. Picks whose id is outside [0, E) stand behind them, in slot order, with rows of
  *   zeros. position[T, K] is the place of each pick's row, of a pick of no expert -1 - place. x_scale[T] (int8 rows'
  *   scales; NULL: none) is sorted alike into row_scale[T K], 0 for picks of no expert. 1 <= K <= E <= 256, T K < 2^31.
- *   The workspace (0 up to 4096 picks; any alignment of 4) holds ranks and counts. The gradient of rows is
+ *   The workspace (0 up to 8192 picks; any alignment of 4) holds ranks and counts. The gradient of rows is
  *   moe_unpermute without weights.
  * ---------------------------------------------------------------------------------------------------- */
 size_t moe_permute_workspace_bytes(int64_t num_tokens, int64_t num_experts, int64_t top_k);

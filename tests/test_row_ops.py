@@ -200,7 +200,8 @@ def permute_reference(ids, E):
 
 SORTS = [  # T, H, E, K: one workgroup's slots and several chunks of them, whole tokens a chunk, the most experts and picks
     (1, 1, 1, 1), (1, 8, 256, 256), (3, 7, 5, 2), (128, 64, 16, 2), (1000, 17, 64, 4), (511, 40, 256, 8), (1366, 5, 3, 3),
-    (4097, 9, 2, 1), (1400, 33, 7, 3), (2050, 24, 64, 6), (40, 12, 255, 130), (3000, 16, 256, 8), (20000, 3, 17, 1)]
+    (4097, 9, 2, 1), (1400, 33, 7, 3), (2050, 24, 64, 6), (40, 12, 255, 130), (3000, 16, 256, 8), (20000, 3, 17, 1),
+    (1024, 10, 5, 1), (1025, 10, 5, 1), (1024, 9, 64, 8), (1025, 9, 64, 8), (33, 9, 256, 256), (40000, 8, 33, 7)]
 
 
 @gpu
@@ -297,7 +298,7 @@ def test_no_tokens(ops):
 @gpu
 def test_row_operators_captured_with_changed_inputs(ops):
     """A norm, sort and way back with their gradients in one graph, replayed on changed inputs among eager calls."""
-    T, H, E, K = 1500, 264, 16, 4  # two chunks of slots: with a workspace
+    T, H, E, K = 2500, 264, 16, 4  # several chunks of slots: with a workspace
     x, res, gamma = normal((T, H), F16, 1).cuda(), normal((T, H), F16, 2).cuda(), normal((H,), F32, 3).cuda()
     ids = torch.randint(-1, E, (T, K), generator=gen(4), dtype=torch.int32).cuda()
     w, gy = normal((T, K), F32, 5).cuda(), normal((T, H), F16, 6).cuda()
@@ -421,8 +422,8 @@ NAN = float("nan")
     (permute_call, [(dict(T=-1), ARG), (dict(K=0), ARG), (dict(K=9), ARG), (dict(E=257), UNSUPPORTED), (dict(E=0), ARG),
                     (dict(T=1 << 30), UNSUPPORTED), (dict(dtype=3), ARG), (dict(x=None), NULL), (dict(ids=None), NULL),
                     (dict(rows=None), NULL), (dict(offsets=None), NULL), (dict(position=None), NULL), (dict(sx=P), NULL),
-                    (dict(sr=P), NULL), (dict(T=4096, ws=None), WS), (dict(T=4096, wb=16), WS),
-                    (dict(T=4096, ws=P + 1), UNSUPPORTED), (dict(xs=63), ARG)]),
+                    (dict(sr=P), NULL), (dict(T=5000, ws=None), WS), (dict(T=5000, wb=16), WS),
+                    (dict(T=5000, ws=P + 1), UNSUPPORTED), (dict(xs=63), ARG)]),
     (unpermute_call, [(dict(T=-1), ARG), (dict(K=0), ARG), (dict(R=-1), ARG), (dict(R=1 << 31), ARG), (dict(dtype=2), ARG),
                       (dict(wtype=3), ARG), (dict(rows=None), NULL), (dict(position=None), NULL), (dict(y=None), NULL),
                       (dict(T=1 << 30), UNSUPPORTED)]),
@@ -439,8 +440,8 @@ def test_refusals(call, changes):
 
 def test_workspace_queries():
     L = lib.load()
-    assert L.moe_permute_workspace_bytes(512, 64, 8) == 0
-    assert L.moe_permute_workspace_bytes(513, 64, 8) == (2 * 65 + 513 * 8) * 4
+    assert L.moe_permute_workspace_bytes(1024, 64, 8) == 0
+    assert L.moe_permute_workspace_bytes(1025, 64, 8) == (9 * 65 + 1025 * 8) * 4
     assert L.moe_permute_workspace_bytes(-1, 64, 8) == 0 and L.moe_permute_workspace_bytes(1 << 30, 64, 8) == 0
     assert L.moe_add_rms_norm_grad_workspace_bytes(4, 16385) == 0
     assert L.moe_add_rms_norm_grad_workspace_bytes(0, 100) == 400
