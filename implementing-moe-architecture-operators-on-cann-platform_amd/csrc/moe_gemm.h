@@ -5,6 +5,8 @@
 #include "moe_device.h"
 #include "moe_launch.h"
 
+#include <type_traits>
+
 namespace moe {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -255,31 +257,61 @@ __device__ __forceinline__ uint2 pack4(f32x4 y) {
                       T::store(y[2]) | (static_cast<uint32_t>(T::store(y[3])) << 16));
 }
 
+// Sums of 8-bit products: int32 bits times the row's scale, times the columns'
+__device__ __forceinline__ f32x4 scaled4(f32x4 bits, float row_scale, f32x4 col_scale) {
+    const i32x4 v = __builtin_bit_cast(i32x4, bits);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) col_scale[r] *= static_cast<float>(v[r]) * row_scale;
+    return col_scale;
+}
+__device__ __forceinline__ f32x4 load_scales4(const float* p, int valid) {
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+    if (valid >= 4) {
+        c = *reinterpret_cast<const f32x4_any*>(p);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (r < valid) c[r] = p[r];
+    }
+    return c;
+}
+
+// The scales that a wave's epilogue needs, loaded before its blocks: at each block's own time their latency was most of
+// the epilogue (256 x 256 tiles: 12.5 us of 25 at H = 2048). A lane has the same 8 columns in every block (SwiGLU: gate and
+// up), and of each 64 rows the scale of one, which the block's lanes fetch from each other.
+template <bool SWIGLU, int ROWS>
+struct WaveScales {
+    static constexpr int kParts = (ROWS + kWave - 1) / kWave;
+    f32x4 z[2], u[2];
+    float rows[kParts];
+    __device__ __forceinline__ void load(const GemmArgs& g, int lane, int row0, int col) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int valid = g.n - col - 4 * e;
+            z[e] = load_scales4(g.col_scale + col + 4 * e, valid);
+            u[e] = SWIGLU ? load_scales4(g.col_scale + g.n + col + 4 * e, valid) : z[e];
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) rows[p] = g.row_scale[min(row0 + p * kWave + lane, g.m - 1)];
+    }
+    // of row r of the wave's
+    __device__ __forceinline__ float row(int r) const {
+        float v = __shfl(rows[0], r % kWave, kWave);
+        if (kParts > 1) {
+            const float w = __shfl(rows[kParts - 1], r % kWave, kWave);
+            v = r < kWave ? v : w;
+        }
+        return v;
+    }
+};
+struct NoScales {};
+
 // The epilogue of 4 consecutive columns col .. col + 3 of one output row, the first `valid` of which exist: bias, the
 // sums before the activation stored, activation, residual. z: the sums (SwiGLU: the gate's, u the up rows'). `whole`:
 // all four are there and aligned, so they are one access.
 template <typename T, bool SWIGLU>
 __device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col, int valid, bool whole, f32x4 z,
                                          f32x4 u) {
-    if constexpr (T::kInt8) {  // int32 sums: times the row's scale, times the columns'
-        const float rs = g.row_scale[row];
-        auto scaled = [&](f32x4 bits, const float* cs) __attribute__((always_inline)) {
-            const i32x4 v = __builtin_bit_cast(i32x4, bits);
-            f32x4 c = {0.f, 0.f, 0.f, 0.f};
-            if (valid == 4) {
-                c = *reinterpret_cast<const f32x4_any*>(cs);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 3; ++r)
-                    if (r < valid) c[r] = cs[r];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) c[r] *= static_cast<float>(v[r]) * rs;
-            return c;
-        };
-        z = scaled(z, g.col_scale + col);
-        if (SWIGLU) u = scaled(u, g.col_scale + g.n + col);
-    }
     if (!SWIGLU && g.factor) z *= *g.factor;
     if (T::kInt8 && g.bias && g.out_f32) {
         const float* bias = reinterpret_cast<const float*>(g.bias);
@@ -340,12 +372,18 @@ __device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col
     return y;
 }
 
-// The same, written to out; columns from n on are left alone. `vec`: whole vectors are aligned (vector_rows).
-template <typename T, bool SWIGLU>
+// The same, written to out; columns from n on are left alone. `vec`: whole vectors are aligned (vector_rows). SCALED: sums
+// of 8-bit products have their scales.
+template <typename T, bool SWIGLU, bool SCALED = false>
 __device__ __forceinline__ void store4(const GemmArgs& g, int64_t row, int col, f32x4 z, f32x4 u, bool vec) {
     if (col >= g.n) return;
     const int valid = min(4, g.n - col);
     const bool whole = vec && valid == 4;
+    if (T::kInt8 && !SCALED) {
+        const float rs = g.row_scale[row];
+        z = scaled4(z, rs, load_scales4(g.col_scale + col, valid));
+        if (SWIGLU) u = scaled4(u, rs, load_scales4(g.col_scale + g.n + col, valid));
+    }
     const f32x4 y = finish4<T, SWIGLU>(g, row, col, valid, whole, z, u);
     const int64_t at = row * g.n + col;
     if (g.out_f32) {
@@ -367,6 +405,9 @@ __host__ __device__ __forceinline__ bool vector_rows(const GemmArgs& g) {
     return g.n % 4 == 0 && ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.residual)) & mask) == 0;
 }
 
+template <typename T, bool SWIGLU, int ROWS>
+using EpilogueScales = std::conditional_t<T::kInt8, WaveScales<SWIGLU, ROWS>, NoScales>;
+
 // Whether store_block may write 8 columns of the 16-bit result at once
 __device__ __forceinline__ bool whole_lines(const GemmArgs& g, bool vec) {
     return vec && !g.out_f32 && g.n % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
@@ -379,9 +420,10 @@ template <int NB>
 __device__ __forceinline__ void put_block(float* stg, int row16, int kg, int j, f32x4 v) {
     *reinterpret_cast<f32x4*>(stg + (row16 * NB * 4 + ((j * 4 + kg) ^ (NB == 4 ? row16 : row16 % (NB * 4)))) * 4) = v;
 }
-template <typename T, bool SWIGLU, int NB>
+// scales: of 8-bit products (WaveScales), the block being the wave's rows from wave_row on.
+template <typename T, bool SWIGLU, int NB, typename S>
 __device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg, int lane, int row0, int col0, bool vec,
-                                            bool lines) {
+                                            bool lines, const S& scales, int wave_row) {
     constexpr int kGranules = NB * 4, kPer = (SWIGLU ? NB / 2 : NB) * 2;  // lanes of a row
     auto get = [&](int r, int gr) __attribute__((always_inline)) {
         return *reinterpret_cast<const f32x4*>(stg + (r * kGranules + (gr ^ (NB == 4 ? r : r % kGranules))) * 4);
@@ -392,6 +434,8 @@ __device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg,
 #pragma unroll 1
     for (int h = 0; h < (16 * kPer + kWave - 1) / kWave; ++h) {
         const int r = h * (kWave / kPer) + lane / kPer, c = lane % kPer;
+        float rs = 1.0f;
+        if constexpr (T::kInt8) rs = scales.row(wave_row + r % 16);  // every lane gives its rows' before some leave
         if (16 * kPer < kWave && r >= 16) continue;
         const int row = row0 + r, col = col0 + c * 8;
         f32x4 z[2], u[2];
@@ -400,6 +444,13 @@ __device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg,
             z[e] = get(r, 2 * c + e);
             u[e] = SWIGLU ? get(r, kGranules / 2 + 2 * c + e) : z[e];
         }
+        if constexpr (T::kInt8) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                z[e] = scaled4(z[e], rs, scales.z[e]);
+                if (SWIGLU) u[e] = scaled4(u[e], rs, scales.u[e]);
+            }
+        }
         if (row >= g.m || col >= g.n) continue;
         if (lines) {
             const uint2 a = pack4<T>(finish4<T, SWIGLU>(g, row, col, 4, true, z[0], u[0]));
@@ -407,8 +458,8 @@ __device__ __forceinline__ void store_block(const GemmArgs& g, const float* stg,
             *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.n + col) =
                 u32x4{a.x, a.y, b.x, b.y};
         } else {
-            store4<T, SWIGLU>(g, row, col, z[0], u[0], vec);
-            store4<T, SWIGLU>(g, row, col + 4, z[1], u[1], vec);
+            store4<T, SWIGLU, true>(g, row, col, z[0], u[0], vec);
+            store4<T, SWIGLU, true>(g, row, col + 4, z[1], u[1], vec);
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // read before the next block's writes

@@ -283,6 +283,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& all, int mtiles, int nt
     ring_barrier();  // everyone's reads and copies are over: the ring's room is the epilogue's
     const bool vec = vector_rows(g), lines = whole_lines(g, vec);
     float* stg = reinterpret_cast<float*>(lds) + wave * (FN * 256);
+    EpilogueScales<T, SWIGLU, BM / WM> scales;
+    if constexpr (T::kInt8) scales.load(g, lane, r0, c0 + lane % (FO * 2) * 8);
     auto put = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) put_block<FN>(stg, row16, kg, j, acc[j][i]);
@@ -295,7 +297,7 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& all, int mtiles, int nt
             case 2: put(FM > 2 ? 2 : 0); break;
             default: put(FM > 3 ? 3 : 0); break;
         }
-        store_block<T, SWIGLU, FN>(g, stg, lane, r0 + i * 16, c0, vec, lines);
+        store_block<T, SWIGLU, FN>(g, stg, lane, r0 + i * 16, c0, vec, lines, scales, i * 16);
     }
 }
 

@@ -240,6 +240,59 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         tick_c(acc[1], first);
     };
 
+    // The epilogue of 8-bit products without bias and residual, without a branch: scales and SwiGLU while the sums are in
+    // registers (gate and up of a column are in one lane), then 16-bit results through LDS. A lane's 4 columns are 8 bytes;
+    // a block's row has 8 granules of 16 bytes (SwiGLU 4), granule G standing at G ^ (row & 7) (SwiGLU row >> 1 & 3), and
+    // two blocks take turns in the wave's 4 KB. The general epilogue's branches on what each value gets took 11 us of a
+    // tile's 29 (H = 1408), whatever was stored or loaded.
+    auto int8_epilogue = [&](const GemmArgs& ge, const Acc (&acc)[2], char* stg, int ln, int row0, int c0)
+                             __attribute__((always_inline)) {
+        constexpr int kJ = SWIGLU ? 2 : 4, kGran = 2 * kJ, kReads = kGran / 4;
+        const int row16 = ln & 15, kg = ln >> 4;
+        f32x4 cs[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = c0 + (SWIGLU ? j & 1 : j) * 16 + kg * 4;  // SwiGLU: the gate's two blocks, the up rows' two
+            cs[j] = load_scales4(ge.col_scale + col + (SWIGLU && j >= 2 ? ge.n : 0), ge.n - col);
+        }
+        float rs[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rs[i] = ge.row_scale[min(row0 + (i >> 2) * 128 + (i & 3) * 16 + row16, ge.m - 1)];
+        uint16_t* out = static_cast<uint16_t*>(ge.out);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            char* half = stg + (i & 1) * 2048;
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+                f32x4 y;
+                if (SWIGLU) {
+                    const f32x4 z = scaled4(acc[i >> 2][0][i & 3][j], rs[i], cs[j]);
+                    const f32x4 u = scaled4(acc[i >> 2][1][i & 3][j], rs[i], cs[2 + j]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = z[r] * sigmoid_fast(z[r]) * u[r];
+                } else {
+                    y = scaled4(acc[i >> 2][j >> 1][i & 3][j & 1], rs[i], cs[j]);
+                }
+                const int gran = (j * 2 + (kg >> 1)) ^ (SWIGLU ? row16 >> 1 & 3 : row16 & 7);
+                *reinterpret_cast<uint2*>(half + (row16 * kGran + gran) * 16 + (kg & 1) * 8) = pack4<T>(y);
+            }
+            // the reads take what other lanes of this wave just wrote (LDS operations of one wave run in order)
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int h = 0; h < kReads; ++h) {
+                const int r = h * (kWave / kGran) + ln / kGran, c = ln % kGran;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(
+                    half + (r * kGran + (c ^ (SWIGLU ? r >> 1 & 3 : r & 7))) * 16);
+                const int row = row0 + (i >> 2) * 128 + (i & 3) * 16 + r, col = c0 + c * 8;
+                if (row < ge.m && col < ge.n)
+                    *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * ge.n + col) = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // read before the writes of the block after the next
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+    };
+
     // acc[a][b][i][j]: rows a * 128 + wm * 64 + i * 16 + row16, columns of Q half b, 4 consecutive ones from 4 kg on.
     // The 8 blocks of 16 rows share one copy of the epilogue's code: unrolled, its activations are too long for the
     // accumulators to stay in registers.
@@ -249,6 +302,16 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         const int ln = lane_fresh(), row16 = ln & 15, kg = ln >> 4;
         const bool vec = vector_rows(g), lines = whole_lines(g, vec);
         float* stg = reinterpret_cast<float*>(lds + 2 * kStageHalfs) + wave * (kEpiBytes / 4);
+        const int c0 = t.n0 + wn * (SWIGLU ? 32 : 64);
+        // the wave's rows: 64 of each half of the tile
+        EpilogueScales<T, SWIGLU, 64> scales[2];
+        if constexpr (T::kInt8) {
+            if (lines && !ge.bias && !ge.residual && (SWIGLU || ge.act == kActNone))
+                return int8_epilogue(ge, acc, reinterpret_cast<char*>(stg), ln, t.m0 + wm * 64, c0);
+            const int col = c0 + ln % (SWIGLU ? 4 : 8) * 8;
+            scales[0].load(ge, ln, t.m0 + wm * 64, col);
+            scales[1].load(ge, ln, t.m0 + 128 + wm * 64, col);
+        }
         auto put = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) put_block<4>(stg, row16, kg, j, acc[i >> 2][j >> 1][i & 3][j & 1]);
@@ -265,8 +328,13 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
                 case 6: put(6); break;
                 default: put(7); break;
             }
-            store_block<T, SWIGLU, 4>(ge, stg, ln, t.m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16,
-                                      t.n0 + wn * (SWIGLU ? 32 : 64), vec, lines);
+            EpilogueScales<T, SWIGLU, 64> sc;
+            if constexpr (T::kInt8) {
+                sc = scales[0];  // columns alike
+                if (i >= 4) sc.rows[0] = scales[1].rows[0];
+            }
+            store_block<T, SWIGLU, 4>(ge, stg, ln, t.m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16, c0, vec, lines, sc,
+                                      (i & 3) * 16);
         }
     };
 
