@@ -253,7 +253,9 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int col = c0 + (SWIGLU ? j & 1 : j) * 16 + kg * 4;  // SwiGLU: the gate's two blocks, the up rows' two
-            cs[j] = load_scales4(ge.col_scale + col + (SWIGLU && j >= 2 ? ge.n : 0), ge.n - col);
+            // whole vectors, n being a multiple of 8; past the columns any
+            const float* at = ge.col_scale + min(col, ge.n - 4) + (SWIGLU && j >= 2 ? ge.n : 0);
+            cs[j] = *reinterpret_cast<const f32x4_any*>(at);
         }
         float rs[8];
 #pragma unroll
