@@ -115,10 +115,10 @@ double mid_time(int bm, int64_t items, int64_t stages, bool p_by_k) {
            stages * (static_cast<double>(items / slots) * c.two + tail);
 }
 // The same of 256 x 256 tiles: one workgroup a CU, 1.0 us a stage with few tiles up to 1.46 with one on every CU (the
-// clock falls), 7 to 10 us of first copies and epilogue a round.
-double tiled_time(int64_t tiles, int64_t stages, bool p_by_k) {
-    const double launch = p_by_k ? 7.1 : 5.8, round = p_by_k ? 9.4 : 10.2, stage = p_by_k ? 1.59 : 1.46;
-    const double few_round = p_by_k ? 7.4 : 6.7, few_stage = p_by_k ? 1.2 : 1.01, more = p_by_k ? 0.43 : 0.41;
+// clock falls), 7 to 10 us of first copies and epilogue a round, of 8-bit products 4 to 5.
+double tiled_time(int64_t tiles, int64_t stages, bool p_by_k, bool int8) {
+    const double launch = p_by_k ? 7.1 : 5.8, round = p_by_k ? 9.4 : int8 ? 4.5 : 10.2, stage = p_by_k ? 1.59 : 1.46;
+    const double few_round = p_by_k ? 7.4 : int8 ? 4.0 : 6.7, few_stage = p_by_k ? 1.2 : 1.01, more = p_by_k ? 0.43 : 0.41;
     const double f = (tiles % 256) / 256.0;
     const double tail =
         tiles % 256 == 0 ? 0.0 : few_round + (round - few_round) * f + stages * (few_stage + more * f * f);
@@ -138,14 +138,17 @@ double reduce_time(size_t partial, bool p_by_k) {
 // 11.5), T = 64 11.6 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N =
 // 256 12.4 us (8.3 split over k), T = 64, H = 4096, N = 16384 35 us (33). Up to 16 rows a call takes 8.3 to 8.9 us from
 // N = 8 to 512 and H = 2048 to 8192, the host's time, where two launches take 10.7.
+// 8-bit products (k in pairs) take the same times but for the epilogue of their 256 x 256 tiles, and above 16 rows stream
+// up to 512 tiles: H = 4096, N = 14336 SwiGLU (1792 tiles) at T = 32 30 us, tiles of 32 rows 24. Of 90 products (T = 1 ..
+// 16384) the choice is the fastest kernel or 1 to 2 % slower on average.
 // most_rows: the tallest tiles to choose from.
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct,
-                         int most_rows = 256) {
+                         int most_rows = 256, bool int8 = false) {
     ProductPlan best{Kernel::kMid, 128, 1, ceil_div(k > 0 ? k : 1, 64) * 64, 0, 1e30};
     const int64_t stages = ceil_div(k > 0 ? k : 1, 64);
     if (direct && !p_by_k && !q_by_k && m <= 64) {
         const int64_t tiles = ceil_div(n, swiglu ? 8 : 16);
-        if (m <= 16 || (tiles >= 64 && (m <= 32 || tiles <= 512))) {
+        if (m <= 16 || (tiles >= 64 && ((m <= 32 && !int8) || tiles <= 512))) {
             best.kernel = Kernel::kStream;
             return best;
         }
@@ -165,7 +168,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by
         if (t < best.us) best = ProductPlan{Kernel::kMid, bm, static_cast<int>(splits), per * 64, partial, t};
     }
     const int64_t tiles = ceil_div(m, 256) * ceil_div(n, swiglu ? 128 : 256);
-    const double t = tiled_time(tiles, stages, p_by_k);
+    const double t = tiled_time(tiles, stages, p_by_k, int8);
     if (direct && m > 64 && most_rows >= 256 && t < best.us)
         best = ProductPlan{Kernel::kTiled, 256, 1, stages * 64, 0, t};
     return best;
@@ -373,17 +376,21 @@ size_t linear_int8_workspace(int64_t T, int64_t N, int64_t H, int64_t E, int32_t
     if (E > 0) return 0;
     size_t most = 0;
     for (const bool direct : {false, true}) {
-        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, act == MOE_ACT_SWIGLU, false, false, direct);
+        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, act == MOE_ACT_SWIGLU, false, false, direct, 256, true);
         if (plan.partial_bytes > most) most = plan.partial_bytes;
     }
     return most;
 }
 
-// Rows of a tile of the experts' products, by their rows on average
+// Rows of a tile of the experts' products, by their rows on average; 16 streams the weights. us at means of 8, 12, 24 and
+// 32 rows, of which some experts have three times as many (E = 64, H = 2048, N = 1408 SwiGLU): streaming 68, 80, 121,
+// 155; 64 rows 76, 77, 84, 93; 128 rows 76, 89, 91, 93; 256 rows 93, 92, 94, 94, and 99 at 64 rows, where 128 take 116.
+// E = 8, H = 4096, N = 14336 152, 185, 300, 358 / 165, 164, 190, 207 / 178, 179, 178, 203 / 200, 199, 201, 208.
+// Operands that come through registers have tiles of 64 and 128 rows.
 int group_rows(int64_t T, int64_t E, bool direct) {
     const int64_t mean = T / E;
     if (!direct) return mean <= 64 ? 64 : 128;
-    return mean <= 8 ? 16 : mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 256 ? 128 : 256;
+    return mean <= 10 ? 16 : mean < 32 ? 64 : 256;
 }
 
 // moe_linear_grad likewise; grad_y of the operands' type or, with grad_f32, float32
@@ -738,13 +745,13 @@ moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_sca
     if (E > 0) {
         const int rows = group_rows(T, E, direct);
         if (rows == 256) err = moe::launch_int8_tiled(g, bf16, s);
-        else if (direct && rows <= 64) err = moe::launch_int8_stream(g, bf16, rows, s);
+        else if (rows == 16) err = moe::launch_int8_stream(g, bf16, s);
         else err = moe::launch_int8_mid(g, bf16, direct, rows, s);
     } else {
-        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, swiglu, false, false, direct);
+        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, swiglu, false, false, direct, 256, true);
         set_split(g, plan, workspace);
         g.split_k = static_cast<int>(plan.split_k * 2 / unit);
-        if (plan.kernel == Kernel::kStream) err = moe::launch_int8_stream(g, bf16, 0, s);
+        if (plan.kernel == Kernel::kStream) err = moe::launch_int8_stream(g, bf16, s);
         else if (plan.kernel == Kernel::kTiled) err = moe::launch_int8_tiled(g, bf16, s);
         else err = moe::launch_int8_mid(g, bf16, direct, plan.bm, s);
         if (err == hipSuccess && plan.splits > 1) err = moe::launch_int8_reduce(g, bf16, s);

@@ -619,13 +619,13 @@ hipError_t launch_gemm_stream(const GemmArgs& g, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);
 
-// The same of 8-bit operands, both by rows; bf16: the results. With experts bm rows a tile (mid: 64 or 128, stream: 16, 32
-// or 64) and no split
+// The same of 8-bit operands, both by rows; bf16: the results. With experts mid takes 64 or 128 rows a tile, and no product
+// is split
 hipError_t prepare_int8_mid();
 hipError_t prepare_int8_stream();
 hipError_t prepare_int8_tiled();
 hipError_t launch_int8_mid(const GemmArgs& g, bool bf16, bool direct, int bm, hipStream_t stream);
-hipError_t launch_int8_stream(const GemmArgs& g, bool bf16, int bm, hipStream_t stream);
+hipError_t launch_int8_stream(const GemmArgs& g, bool bf16, hipStream_t stream);
 hipError_t launch_int8_tiled(const GemmArgs& g, bool bf16, hipStream_t stream);
 hipError_t launch_int8_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);
 

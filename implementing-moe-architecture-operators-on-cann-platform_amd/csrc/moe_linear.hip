@@ -399,7 +399,10 @@ hipError_t run_int8(const GemmArgs& g, bool direct, hipStream_t stream) {
 }
 template <typename T>
 hipError_t run_int8_any(const GemmArgs& g, bool direct, int bm, hipStream_t stream) {
-    if (g.experts) return bm == 64 ? run_int8<T, 64, true>(g, direct, stream) : run_int8<T, 128, true>(g, direct, stream);
+    if (g.experts && bm == 64) return run_int8<T, 64, true>(g, direct, stream);
+    if (g.experts)  // operands through registers only
+        return g.act == kActSwiglu ? run_mid<T, false, false, 128, true, false, true>(g, stream)
+                                   : run_mid<T, false, false, 128, false, false, true>(g, stream);
     if (bm == 256)  // direct operands only
         return g.act == kActSwiglu ? run_mid<T, false, false, 256, true, true>(g, stream)
                                    : run_mid<T, false, false, 256, false, true>(g, stream);
