@@ -372,14 +372,32 @@ moe_status check_linear_int8(int64_t T, int64_t N, int64_t H, int64_t E, int32_t
     return ok();
 }
 
-size_t linear_int8_workspace(int64_t T, int64_t N, int64_t H, int64_t E, int32_t act) {
-    if (E > 0) return 0;
+// Workspace: x and the weights with rows padded to 16 bytes, where H is no multiple of that and the product has rows enough
+// for it to pay (T = 8000, H = 4001, N = 4000 429 us through registers; T = 200, H = 2001, N = 2000 20 either way) |
+// partial sums of a split product
+struct Int8Workspace {
+    bool padded;
+    size_t w_at, partial_at, bytes;
+};
+Int8Workspace int8_workspace(int64_t T, int64_t N, int64_t H, int64_t E, int32_t act) {
+    const bool swiglu = act == MOE_ACT_SWIGLU;
+    const int64_t h16 = round_up(H, 16), groups = E > 0 ? E : 1;
+    Int8Workspace w{};
+    w.padded = H % 16 != 0 && T >= (E > 0 ? 32 * E : 256);
+    if (w.padded) {
+        w.w_at = round_up(T * h16, 256);
+        w.partial_at = w.w_at + round_up(groups * (swiglu ? 2 : 1) * N * h16, 256);
+    }
+    w.bytes = w.partial_at;
+    if (E > 0) return w;
     size_t most = 0;
     for (const bool direct : {false, true}) {
-        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, act == MOE_ACT_SWIGLU, false, false, direct, 256, true);
+        const int64_t k = (w.padded ? h16 : H + 1) / 2;
+        const ProductPlan plan = plan_product(T, N, k, swiglu, false, false, direct, 256, true);
         if (plan.partial_bytes > most) most = plan.partial_bytes;
     }
-    return most;
+    w.bytes += most;
+    return w;
 }
 
 // Rows of a tile of the experts' products, by their rows on average; 16 streams the weights. us at means of 8, 12, 24 and
@@ -685,7 +703,7 @@ moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const
 
 size_t moe_linear_int8_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t E, int32_t activation) {
     if (check_linear_int8(T, N, H, E, activation) != MOE_OK) return 0;
-    return linear_int8_workspace(T, N, H, E, activation);
+    return int8_workspace(T, N, H, E, activation).bytes;
 }
 
 moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* weight,
@@ -708,14 +726,37 @@ moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_sca
     if (T == 0) return ok();
     if (!x || !x_scale || !weight || !weight_scale || !y || (E > 0 && !offsets))
         return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
-    const size_t need = linear_int8_workspace(T, N, H, E, activation);
+    const Int8Workspace room = int8_workspace(T, N, H, E, activation);
+    const size_t need = room.bytes;
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes at %p, need %zu", op, workspace_bytes, workspace, need);
     if (need > 0 && !aligned16(workspace))
         return fail(MOE_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", op);
-    const int64_t pitch = T > 1 ? x_stride : 0, weight_pitch = Z > 1 ? weight_stride : 0;
-    const int64_t step = E > 1 ? expert_stride : 0;
-    const bool direct = H % 16 == 0 && aligned16(x) && aligned16(weight) && pitch % 16 == 0 && weight_pitch % 16 == 0 &&
+    hipError_t err = moe::prepare_linear_int8();
+    if (err != hipSuccess) return hip_fail(err, "MoeLinearInt8 kernel attributes");
+    const hipStream_t s = as_stream(stream);
+    int64_t pitch = T > 1 ? x_stride : 0, weight_pitch = Z > 1 ? weight_stride : 0, step = E > 1 ? expert_stride : 0, k = H;
+    if (room.padded) {
+        char* base = static_cast<char*>(workspace);
+        moe::Repack8 px{}, pw{};
+        px.src = reinterpret_cast<const uint8_t*>(x);
+        px.dst = reinterpret_cast<uint8_t*>(base);
+        px.src_ld = pitch;
+        px.rows = T;
+        px.cols = pw.cols = static_cast<int>(H);
+        pw.src = reinterpret_cast<const uint8_t*>(weight);
+        pw.dst = reinterpret_cast<uint8_t*>(base + room.w_at);
+        pw.src_ld = weight_pitch;
+        pw.group_ld = step;
+        pw.rows = Z;
+        err = moe::launch_repack8(px, pw, E > 0 ? E : 1, s);
+        if (err != hipSuccess) return hip_fail(err, "MoeLinearInt8 launch");
+        x = reinterpret_cast<const int8_t*>(px.dst);
+        weight = reinterpret_cast<const int8_t*>(pw.dst);
+        k = pitch = weight_pitch = round_up(H, 16);
+        step = Z * k;
+    }
+    const bool direct = k % 16 == 0 && aligned16(x) && aligned16(weight) && pitch % 16 == 0 && weight_pitch % 16 == 0 &&
                         step % 16 == 0 && pitch <= int64_t{1} << 23 && weight_pitch <= int64_t{1} << 23;
     const int unit = direct ? 2 : 1;  // bytes that strides and k count
     moe::GemmArgs g{};
@@ -725,7 +766,7 @@ moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_sca
     g.ldq = weight_pitch / unit;
     g.m = static_cast<int>(T);
     g.n = g.up = static_cast<int>(N);
-    g.k = static_cast<int>(H / unit);
+    g.k = static_cast<int>(k / unit);
     g.out = y;
     g.bias = static_cast<const uint16_t*>(bias);
     g.residual = residual;
@@ -739,17 +780,14 @@ moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_sca
     g.q_expert = step;
     g.offsets = offsets;
     const bool bf16 = out_dtype == MOE_DT_BFLOAT16;
-    const hipStream_t s = as_stream(stream);
-    hipError_t err = moe::prepare_linear_int8();
-    if (err != hipSuccess) return hip_fail(err, "MoeLinearInt8 kernel attributes");
     if (E > 0) {
         const int rows = group_rows(T, E, direct);
         if (rows == 256) err = moe::launch_int8_tiled(g, bf16, s);
         else if (rows == 16) err = moe::launch_int8_stream(g, bf16, s);
         else err = moe::launch_int8_mid(g, bf16, direct, rows, s);
     } else {
-        const ProductPlan plan = plan_product(T, N, (H + 1) / 2, swiglu, false, false, direct, 256, true);
-        set_split(g, plan, workspace);
+        const ProductPlan plan = plan_product(T, N, (k + 1) / 2, swiglu, false, false, direct, 256, true);
+        set_split(g, plan, static_cast<char*>(workspace) + room.partial_at);
         g.split_k = static_cast<int>(plan.split_k * 2 / unit);
         if (plan.kernel == Kernel::kStream) err = moe::launch_int8_stream(g, bf16, s);
         else if (plan.kernel == Kernel::kTiled) err = moe::launch_int8_tiled(g, bf16, s);

@@ -594,6 +594,14 @@ struct RepackArgs {
     Repack m[kRepackMost];
 };
 hipError_t launch_repack(const RepackArgs& a, hipStream_t stream);
+// Of 8-bit rows, padded to whole 16 bytes: `rows` of cols bytes, src_ld apart, and group_ld from one group's to the next's
+struct Repack8 {
+    const uint8_t* src;
+    uint8_t* dst;
+    int64_t src_ld, group_ld, rows;
+    int cols;
+};
+hipError_t launch_repack8(const Repack8& x, const Repack8& w, int64_t groups, hipStream_t stream);
 
 // What follows the gradients' products: the reduction of those that were split (splits > 1), the bias's column sums
 struct GradTail {

@@ -32,7 +32,29 @@ __global__ __launch_bounds__(kThreads) void repack_kernel(RepackArgs a, int64_t 
     }
 }
 
+// The same of 8-bit rows: x, and every expert's weight rows (`groups` of them, group_ld apart; x is one)
+__global__ __launch_bounds__(kThreads) void repack8_kernel(Repack8 x, Repack8 w, int per, int64_t granules) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads, of_x = x.rows * per;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < granules; i += step) {
+        const bool second = i >= of_x;
+        const Repack8& r = second ? w : x;
+        const int64_t at = second ? i - of_x : i, row = at / per, group = row / r.rows;
+        const int col = static_cast<int>(at - row * per) * 16;
+        *reinterpret_cast<s16x8*>(r.dst + row * per * 16 + col) =
+            load16(r.src + group * r.group_ld + (row - group * r.rows) * r.src_ld + col, x.cols - col, col);
+    }
+}
+
 }  // namespace
+
+hipError_t launch_repack8(const Repack8& x, const Repack8& w, int64_t groups, hipStream_t stream) {
+    const int per = (x.cols + 15) / 16;
+    const int64_t granules = (x.rows + w.rows * groups) * per, blocks = (granules + kThreads - 1) / kThreads;
+    TraceScope trace("moe_linear_int8_repack", stream);
+    repack8_kernel<<<static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20), kThreads, 0, stream>>>(x, w, per,
+                                                                                                      granules);
+    return hipGetLastError();
+}
 
 hipError_t launch_repack(const RepackArgs& a, hipStream_t stream) {
     int64_t granules = 0;
