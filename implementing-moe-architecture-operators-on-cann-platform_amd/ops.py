@@ -857,6 +857,31 @@ def MoeLinearInt8(x: torch.Tensor, xScale: torch.Tensor, weight: torch.Tensor, w
     return y
 
 
+def moe_layer_int8(x: torch.Tensor, gamma: torch.Tensor, w_gate: torch.Tensor, gate_up: torch.Tensor,
+                   gate_up_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor,
+                   residual: torch.Tensor | None = None, topK: int = 2, bias: torch.Tensor | None = None,
+                   numGroups: int = 1, topGroups: int = 1, groupTop: int = 1, scoring: str = "softmax",
+                   renormalize: bool = True, scale: float = 1.0, eps: float = 1e-6, stream=None):
+    """A layer of 8-bit experts behind its norm, x fp16 or bf16: the norm of x + residual for the router as it is and for
+    the experts in 8 bits (MoeAddRmsNormQuant), fp32 logits by w_gate[H,E] (MoeLinear), MoeRoutingGroupTopK, the tokens
+    sorted by expert (MoePermute), the products by gate_up[E,2I,H] with SwiGLU and, in 8 bits again (MoeQuantize), by
+    down[E,H,I] (MoeLinearInt8; MoeQuantize makes such weights and their scales [E,2I] and [E,H]), and the way back
+    (MoeUnpermute). Returns (y, v, expert_ids, weights): y without the sum v = x + residual, which the next layer adds y
+    to; v is None without a residual."""
+    if w_gate.dim() != 2 or gate_up.dim() != 3 or gate_up.shape[0] != w_gate.shape[1]:
+        raise MoeError(3, f"w_gate {tuple(w_gate.shape)} and gate_up {tuple(gate_up.shape)}: [H, E] and [E, 2I, H] expected")
+    q, q_scale, normed, v = MoeAddRmsNormQuant(x, gamma, residual, eps, returnNorm=True, stream=stream)
+    logits = MoeLinear(normed, w_gate.t(), outDtype=torch.float32, stream=stream)
+    ids, w = MoeRoutingGroupTopK(logits, bias, topK, numGroups, topGroups, groupTop, scoring, renormalize, scale,
+                                 torch.float32, stream=stream)
+    rows, offsets, position, row_scale = MoePermute(q, ids, gate_up.shape[0], q_scale, stream=stream)
+    hidden = MoeLinearInt8(rows, row_scale, gate_up, gate_up_scale, offsets, activation="swiglu", outDtype=x.dtype,
+                           stream=stream)
+    hidden, hidden_scale = MoeQuantize(hidden, stream=stream)
+    out = MoeLinearInt8(hidden, hidden_scale, down, down_scale, offsets, outDtype=x.dtype, stream=stream)
+    return MoeUnpermute(out, position, w, stream=stream), v, ids, w
+
+
 def synth_normal_f16_(out: torch.Tensor, seed: int, stream_id: int, sigma_a: float, sigma_b: float | None = None,
                       period: int = 0, split: int = 0, stream=None) -> torch.Tensor:
     """Fill an fp16 device tensor in place with the generator of synth.py (moe_synth_normal_f16)."""

@@ -14,6 +14,16 @@ MoeExpertFFN have none):
     torch.ops.moe_mi355x.MoeLinear(x, weight, bias, residual, activation, outDtype, returnPre) -> (y, pre)
     torch.ops.moe_mi355x.MoeRoutingGroupTopKGrad, MoeLinearGrad, MoeCombineGrad: what their backward calls
 
+and those of quantised and permuted expert layers, with the gradients of the norm and of sorting (8-bit results have none):
+
+    torch.ops.moe_mi355x.MoeAddRmsNorm(x, gamma, residual, eps) -> (y, v)
+    torch.ops.moe_mi355x.MoeAddRmsNormQuant(x, gamma, residual, eps, returnNorm) -> (q, scale, y, v)
+    torch.ops.moe_mi355x.MoeQuantize(x) -> (q, scale)
+    torch.ops.moe_mi355x.MoePermute(x, expert_ids, numExperts, xScale) -> (rows, offsets, position, row_scale)
+    torch.ops.moe_mi355x.MoeUnpermute(rows, position, weights) -> y
+    torch.ops.moe_mi355x.MoeLinearInt8(x, xScale, weight, weightScale, offsets, bias, residual, activation, outDtype) -> y
+    torch.ops.moe_mi355x.MoeAddRmsNormGrad, MoeUnpermuteGrad: what their backward calls
+
 The device implementation is registered for GPU tensors only: a CPU tensor finds no kernel (there is no CPU
 fallback). The fake (meta) implementations state the InferShape / InferDataType rules of
 op_host/moe_ops.cpp:181-226, 364-398, 495-525 so that tracers can propagate shapes without running anything;
@@ -230,3 +240,189 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     keep = activation != "none" and torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, weight, bias))
     return getattr(torch.ops, NAMESPACE).MoeLinear(x, weight, bias, residual, activation, outDtype, keep)[0]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# quantised and permuted expert layers; an output that a call does not have is empty
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _or_empty(t: torch.Tensor | None, like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    return like.new_empty(0, dtype=dtype) if t is None else t
+
+
+def _norm_shape(x, gamma, residual):
+    if x.dim() != 2 or gamma.shape != x.shape[1:] or (residual is not None and residual.shape != x.shape):
+        raise RuntimeError("MoeAddRmsNorm: x and residual must be [T, H] and gamma [H]")
+    return x.shape
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeAddRmsNorm", mutates_args=(), device_types="cuda")
+def moe_add_rms_norm(x: torch.Tensor, gamma: torch.Tensor, residual: torch.Tensor | None = None,
+                     eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """-> (y, v = x + residual); v is empty without a residual."""
+    y, v = ops.MoeAddRmsNorm(x, gamma, residual, eps)
+    return y, _or_empty(v, x)
+
+
+@moe_add_rms_norm.register_fake
+def _(x, gamma, residual=None, eps=1e-6):
+    shape = _norm_shape(x, gamma, residual)
+    return x.new_empty(shape), x.new_empty(0 if residual is None else shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeAddRmsNormGrad", mutates_args=(), device_types="cuda")
+def moe_add_rms_norm_grad(grad_y: torch.Tensor, v: torch.Tensor, gamma: torch.Tensor,
+                          grad_v: torch.Tensor | None = None, eps: float = 1e-6, gradX: bool = True,
+                          gradGamma: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """-> (grad_x, grad_gamma), empty where not asked for."""
+    gx, gg = ops.MoeAddRmsNormGrad(grad_y, v, gamma, grad_v, eps, gradX, gradGamma)
+    return _or_empty(gx, v), _or_empty(gg, gamma)
+
+
+@moe_add_rms_norm_grad.register_fake
+def _(grad_y, v, gamma, grad_v=None, eps=1e-6, gradX=True, gradGamma=True):
+    return v.new_empty(v.shape if gradX else 0), gamma.new_empty(gamma.shape if gradGamma else 0)
+
+
+def _norm_setup(ctx, inputs, output):
+    x, gamma, residual, ctx.eps = inputs
+    ctx.summed = residual is not None
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(output[1] if ctx.summed else x, gamma)
+
+
+def _norm_backward(ctx, grad_y, grad_v):
+    v, gamma = ctx.saved_tensors
+    grad_v = grad_v if ctx.summed else None
+    want = [ctx.needs_input_grad[0] or (ctx.summed and ctx.needs_input_grad[2]), ctx.needs_input_grad[1]]
+    gx = gg = None
+    if grad_y is None:
+        gx = grad_v
+    elif any(want):
+        op = getattr(torch.ops, NAMESPACE).MoeAddRmsNormGrad
+        got = op(grad_y.contiguous(), v, gamma, None if grad_v is None else grad_v.contiguous(), ctx.eps, *want)
+        gx, gg = (g if w else None for g, w in zip(got, want))
+    return gx, gg, gx if ctx.summed else None, None
+
+
+moe_add_rms_norm.register_autograd(_norm_backward, setup_context=_norm_setup)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeAddRmsNormQuant", mutates_args=(), device_types="cuda")
+def moe_add_rms_norm_quant(
+        x: torch.Tensor, gamma: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+        returnNorm: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    q, scale, y, v = ops.MoeAddRmsNormQuant(x, gamma, residual, eps, returnNorm)
+    return q, scale, _or_empty(y, x), _or_empty(v, x)
+
+
+@moe_add_rms_norm_quant.register_fake
+def _(x, gamma, residual=None, eps=1e-6, returnNorm=False):
+    shape = _norm_shape(x, gamma, residual)
+    return (x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[0], dtype=torch.float32),
+            x.new_empty(shape if returnNorm else 0), x.new_empty(0 if residual is None else shape))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeQuantize", mutates_args=(), device_types="cuda")
+def moe_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.MoeQuantize(x)
+
+
+@moe_quantize.register_fake
+def _(x):
+    if x.dim() not in (2, 3):
+        raise RuntimeError("MoeQuantize: x must be [R, H] or [E, N, H]")
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoePermute", mutates_args=(), device_types="cuda")
+def moe_permute(x: torch.Tensor, expert_ids: torch.Tensor, numExperts: int, xScale: torch.Tensor | None = None
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    rows, offsets, position, row_scale = ops.MoePermute(x, expert_ids, numExperts, xScale)
+    return rows, offsets, position, _or_empty(row_scale, x, torch.float32)
+
+
+@moe_permute.register_fake
+def _(x, expert_ids, numExperts, xScale=None):
+    if x.dim() != 2 or expert_ids.dim() != 2 or expert_ids.shape[0] != x.shape[0]:
+        raise RuntimeError("MoePermute: x must be [T, H] and expert_ids [T, K]")
+    picks = expert_ids.shape[0] * expert_ids.shape[1]
+    return (x.new_empty((picks, x.shape[1])), expert_ids.new_empty(numExperts + 1),
+            expert_ids.new_empty(expert_ids.shape), x.new_empty(0 if xScale is None else picks, dtype=torch.float32))
+
+
+def _permute_setup(ctx, inputs, output):
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(output[2])
+
+
+def _permute_backward(ctx, grad_rows, *_):
+    if grad_rows is None:
+        return (None,) * 4
+    return getattr(torch.ops, NAMESPACE).MoeUnpermute(grad_rows.contiguous(), ctx.saved_tensors[0], None), None, None, None
+
+
+moe_permute.register_autograd(_permute_backward, setup_context=_permute_setup)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeUnpermute", mutates_args=(), device_types="cuda")
+def moe_unpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
+    return ops.MoeUnpermute(rows, position, weights)
+
+
+@moe_unpermute.register_fake
+def _(rows, position, weights=None):
+    if rows.dim() != 2 or position.dim() != 2 or (weights is not None and weights.shape != position.shape):
+        raise RuntimeError("MoeUnpermute: rows must be [R, H], position and weights [T, K]")
+    return rows.new_empty((position.shape[0], rows.shape[1]))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeUnpermuteGrad", mutates_args=(), device_types="cuda")
+def moe_unpermute_grad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: torch.Tensor,
+                       weights: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """-> (grad_rows, grad_weights), the latter empty without weights."""
+    grad_rows, grad_w = ops.MoeUnpermuteGrad(grad_y, rows, position, weights)
+    return grad_rows, _or_empty(grad_w, grad_y)
+
+
+@moe_unpermute_grad.register_fake
+def _(grad_y, rows, position, weights=None):
+    return (grad_y.new_empty((position.shape[0] * position.shape[1], grad_y.shape[1])),
+            grad_y.new_empty(0) if weights is None else weights.new_empty(weights.shape))
+
+
+def _unpermute_setup(ctx, inputs, output):
+    rows, position, weights = inputs
+    ctx.picks = position.shape[0] * position.shape[1]
+    ctx.save_for_backward(rows if weights is not None else None, position, weights)
+    ctx.num_rows = rows.shape[0]
+
+
+def _unpermute_backward(ctx, grad_y):
+    rows, position, weights = ctx.saved_tensors
+    if ctx.num_rows != ctx.picks:
+        raise RuntimeError("MoeUnpermute has a gradient where rows are MoePermute's, one for each pick")
+    grad_rows, grad_w = getattr(torch.ops, NAMESPACE).MoeUnpermuteGrad(grad_y.contiguous(), rows, position, weights)
+    return grad_rows, None, None if weights is None else grad_w
+
+
+moe_unpermute.register_autograd(_unpermute_backward, setup_context=_unpermute_setup)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::MoeLinearInt8", mutates_args=(), device_types="cuda")
+def moe_linear_int8(x: torch.Tensor, xScale: torch.Tensor, weight: torch.Tensor, weightScale: torch.Tensor,
+                    offsets: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                    residual: torch.Tensor | None = None, activation: str = "none",
+                    outDtype: torch.dtype = torch.float16) -> torch.Tensor:
+    return ops.MoeLinearInt8(x, xScale, weight, weightScale, offsets, bias, residual, activation, outDtype)
+
+
+@moe_linear_int8.register_fake
+def _(x, xScale, weight, weightScale, offsets=None, bias=None, residual=None, activation="none",
+      outDtype=torch.float16):
+    dims = 2 if offsets is None else 3
+    if x.dim() != 2 or weight.dim() != dims or x.shape[1] != weight.shape[-1]:
+        raise RuntimeError("MoeLinearInt8: x must be [T, H] and weight [N, H], with offsets [E, N, H]")
+    n = weight.shape[-2]
+    return x.new_empty((x.shape[0], n // 2 if activation == "swiglu" else n), dtype=outDtype)

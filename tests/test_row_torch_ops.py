@@ -1,0 +1,243 @@
+"""Quantised and permuted expert layers through torch: shapes on fake tensors here; gradients, opcheck, compilation and the
+whole layer on the GPU."""
+from __future__ import annotations
+
+import importlib
+
+import pytest
+
+from conftest import PKG_NAME
+from test_dense_ops import BF16, F16, F32, F64, gen, gpu, normal
+
+torch = pytest.importorskip("torch")
+tops = importlib.import_module(PKG_NAME + ".torch_ops")
+op = torch.ops.moe_mi355x
+
+
+def meta(*shape, dtype=F16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def test_meta_shapes():
+    x, g, ids = meta(7, 64), meta(64), meta(7, 3, dtype=torch.int32)
+    y, v = op.MoeAddRmsNorm(x, g, x)
+    assert y.shape == v.shape == (7, 64) and op.MoeAddRmsNorm(x, g)[1].numel() == 0
+    q, s, y, v = op.MoeAddRmsNormQuant(x, g, None, 1e-6, True)
+    assert (q.dtype, s.dtype, s.shape, y.shape, v.numel()) == (torch.int8, F32, (7,), (7, 64), 0)
+    gx, gg = op.MoeAddRmsNormGrad(x, x, g, None, 1e-6, True, False)
+    assert gx.shape == (7, 64) and gg.numel() == 0
+    q, s = op.MoeQuantize(meta(4, 10, 64))
+    assert q.shape == (4, 10, 64) and s.shape == (4, 10)
+    rows, off, pos, rs = op.MoePermute(q[0], meta(10, 2, dtype=torch.int32), 5, s[0])
+    assert (rows.shape, rows.dtype, off.shape, pos.shape, rs.shape) == ((20, 64), torch.int8, (6,), (10, 2), (20,))
+    y = op.MoeUnpermute(meta(21, 64), ids, meta(7, 3))
+    assert y.shape == (7, 64)
+    gr, gw = op.MoeUnpermuteGrad(y, meta(21, 64), ids, meta(7, 3, dtype=F32))
+    assert (gr.shape, gr.dtype, gw.shape, gw.dtype) == ((21, 64), F16, (7, 3), F32)
+    y = op.MoeLinearInt8(rows, rs, meta(5, 24, 64, dtype=torch.int8), meta(5, 24, dtype=F32), off, activation="swiglu")
+    assert (y.shape, y.dtype) == ((20, 12), F16)
+    for call in (lambda: op.MoeAddRmsNorm(x, meta(63)), lambda: op.MoePermute(x, meta(6, 2, dtype=torch.int32), 4),
+                 lambda: op.MoeLinearInt8(rows, rs, meta(24, 63, dtype=torch.int8), s), lambda: op.MoeQuantize(g),
+                 lambda: op.MoeUnpermute(x, ids, meta(7, 2))):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_cpu_tensors_have_no_kernel():
+    with pytest.raises(NotImplementedError):
+        op.MoeQuantize(torch.zeros(4, 64))
+    with pytest.raises(NotImplementedError):
+        op.MoeAddRmsNorm(torch.zeros(4, 64), torch.ones(64))
+
+
+def leaf(t):
+    return t.cuda().requires_grad_(True)
+
+
+def inputs(T=45, H=96, E=8, K=3, dtype=F32):
+    ids = torch.stack([torch.randperm(E, generator=gen(t))[:K] for t in range(T)]).to(torch.int32)
+    ids[5, 1] = -1
+    return (normal((T, H), dtype, 1), normal((T, H), dtype, 2), 1 + 0.2 * normal((H,), F32, 3), ids,
+            torch.rand((T, K), generator=gen(4)))
+
+
+def sorted_layer(x, res, gamma, ids, w, E):
+    """A norm, the tokens by expert, something that differs by expert, and back; the sum goes on beside it."""
+    y, v = op.MoeAddRmsNorm(x, gamma, res, 1e-5)
+    rows, offsets, position, _ = op.MoePermute(y, ids, E)
+    return op.MoeUnpermute(rows * rows, position, w) + v
+
+
+@gpu
+def test_gradients_through_torch(ops):
+    """Against torch's differentiation of the definition in 64 bits. fp32 throughout: each value passes at most about 40
+    roundings (norm 8, square 1, sum 4, their gradients twice that), and those of grad_gamma T sums more."""
+    x, res, gamma, ids, w = inputs()
+    args = [leaf(t) for t in (x, res, gamma, w)]
+    dy = normal(x.shape, F32, 9)
+    out = sorted_layer(args[0], args[1], args[2], ids.cuda(), args[3], 8)
+    got = torch.autograd.grad(out, args, dy.cuda())
+    a, b, g, k = (t.double().requires_grad_(True) for t in (x, res, gamma, w))
+    v = a + b
+    n = v / torch.sqrt(v.square().mean(dim=1, keepdim=True) + 1e-5) * g
+    ref = n * n * (k * (ids >= 0)).sum(dim=1, keepdim=True) + v
+    want = torch.autograd.grad(ref, (a, b, g, k), dy.double())
+    scale = [float(t.abs().max()) for t in want]
+    assert (out.double().cpu() - ref).abs().max() <= 40 * 2.0**-24 * float(ref.detach().abs().max())
+    for u, r, s, n in zip(got, want, scale, (1, 1, 45, 96)):
+        assert (u.double().cpu() - r).abs().max() <= (60 + n) * 2.0**-24 * s * 4
+    assert torch.equal(got[0], got[1])
+
+
+@gpu
+def test_parts_that_need_no_gradient(ops):
+    x, res, gamma, ids, w = inputs()
+    X, R, G = leaf(x), leaf(res), leaf(gamma)
+    y, v = op.MoeAddRmsNorm(X, G, R)
+    gx, gr = torch.autograd.grad(v.sum(), (X, R), retain_graph=True)  # the sum alone
+    assert torch.equal(gx, torch.ones_like(gx)) and torch.equal(gr, gx)
+    gx, = torch.autograd.grad(y.sum() + v.sum(), X, retain_graph=True)
+    gy, = torch.autograd.grad(y.sum(), X)
+    assert torch.allclose(gx - 1, gy, atol=1e-5)  # 1 + gy rounded to fp32: within 2^-24 of at most 16
+    y, _ = op.MoeAddRmsNorm(x.cuda(), G)
+    assert torch.autograd.grad(y.sum(), G)[0].shape == G.shape
+    rows, _, position, _ = op.MoePermute(leaf(x), ids.cuda(), 8)
+    g, = torch.autograd.grad(op.MoeUnpermute(rows, position).sum(), rows)
+    live = (ids >= 0).sum()
+    assert g[:live].eq(1).all() and g[live:].eq(0).all()
+    with pytest.raises(RuntimeError, match="one for each pick"):
+        more = leaf(torch.zeros(200, 96))
+        torch.autograd.grad(op.MoeUnpermute(more, position).sum(), more)
+
+
+@gpu
+def test_opcheck(ops):
+    x, res, gamma, ids, w = (t.cuda() for t in inputs(dtype=F16))
+    # with results of whole numbers torch's own test of the traced gradient adds their sums to those of floats, and fails
+    utils = ("test_schema", "test_faketensor", "test_autograd_registration")
+
+    def check(fn, args, utils=utils):
+        torch.library.opcheck(fn, args, test_utils=utils)
+
+    for args in ((leaf(x), leaf(gamma), leaf(res), 1e-5), (leaf(x), leaf(gamma))):
+        check(op.MoeAddRmsNorm, args, utils + ("test_aot_dispatch_dynamic",))
+    check(op.MoeAddRmsNormQuant, (x, gamma, res, 1e-5, True))
+    check(op.MoeQuantize, (x,))
+    check(op.MoePermute, (leaf(x), ids, 8))
+    q, s = op.MoeQuantize(x)
+    check(op.MoePermute, (q, ids, 8, s))
+    rows, off, pos, rs = op.MoePermute(q, ids, 8, s)
+    check(op.MoeUnpermute, (leaf(rows.half()), pos, leaf(w)), utils + ("test_aot_dispatch_dynamic",))
+    wq, ws = op.MoeQuantize(normal((8, 40, 96), F16, 5).cuda())
+    check(op.MoeLinearInt8, (rows, rs, wq, ws, off, None, None, "swiglu", BF16))
+
+
+def layer_inputs(T, H, E, I, dtype):
+    gate_up = normal((E, 2 * I, H), dtype, 5, H**-0.5)
+    down = normal((E, H, I), dtype, 6, I**-0.5)
+    return (normal((T, H), dtype, 1), normal((T, H), dtype, 2), 1 + 0.2 * normal((H,), F32, 3),
+            normal((H, E), dtype, 4, 2 * H**-0.5), gate_up, down)
+
+
+@gpu
+@pytest.mark.parametrize("T,H,E,I,K,dtype", [(1, 256, 8, 128, 2, F16), (45, 96, 16, 80, 3, BF16), (700, 512, 8, 384, 2, BF16),
+                                             (2500, 256, 64, 144, 6, F16)])
+def test_int8_layer_is_its_parts_and_near_the_definition(ops, T, H, E, I, K, dtype):
+    x, res, gamma, w_gate, gate_up, down = (t.cuda() for t in layer_inputs(T, H, E, I, dtype))
+    (gq, gs), (dq, ds) = ops.MoeQuantize(gate_up), ops.MoeQuantize(down)
+    y, v, ids, w = ops.moe_layer_int8(x, gamma, w_gate, gq, gs, dq, ds, res, K, scoring="sigmoid", eps=1e-5)
+    q, qs, n, v2 = ops.MoeAddRmsNormQuant(x, gamma, res, 1e-5, True)
+    rows, off, pos, rs = ops.MoePermute(q, ids, E, qs)
+    hidden = ops.MoeLinearInt8(rows, rs, gq, gs, off, activation="swiglu", outDtype=dtype)
+    hq, hs = ops.MoeQuantize(hidden)
+    part = ops.MoeLinearInt8(hq, hs, dq, ds, off, outDtype=dtype)
+    assert torch.equal(y, ops.MoeUnpermute(part, pos, w)) and torch.equal(v, v2)
+    # the layer that its 8-bit weights and inputs stand for, in 64 bits, from the ids and weights chosen
+    W1, W2 = gq.double() * gs.double()[:, :, None], dq.double() * ds.double()[:, :, None]
+    a, h8 = q.double() * qs.double()[:, None], torch.zeros((T, K, H), dtype=F64, device="cuda")
+    for e in range(E):
+        t, k = (ids == e).nonzero(as_tuple=True)
+        if len(t):
+            g, u = (a[t] @ W1[e].t()).chunk(2, dim=1)
+            h = g * torch.sigmoid(g) * u
+            step = h.abs().amax(dim=1, keepdim=True) / 127
+            # rounded to dtype before it is quantised: a quantised value may be one step off near a border
+            h8[t, k] = torch.round(h / step) * step @ W2[e].t()
+    ref = (h8 * w.double()[:, :, None]).sum(dim=1)
+    # a step of hidden (1/127 of its row's largest value, some 3.5 of its rms) off by half in the rare value, the rounding of
+    # hidden to dtype moving a share of 127 eps of them over a border: sqrt(127 eps) / 127 * 3.5 of the result, its own
+    # rounding and that of the products' results eps / 2 each; compared by their root mean squares, twice that
+    eps = torch.finfo(dtype).eps
+    off_by = float((y.double() - ref).norm() / ref.norm())
+    assert off_by <= 2 * ((min(1.0, 127 * eps)) ** 0.5 / 127 * 3.5 + 2 * eps), off_by
+
+
+@gpu
+def test_int8_layer_captured_and_compiled(ops):
+    x, res, gamma, w_gate, gate_up, down = (t.cuda() for t in layer_inputs(200, 128, 8, 96, F16))
+    (gq, gs), (dq, ds) = ops.MoeQuantize(gate_up), ops.MoeQuantize(down)
+
+    def step():
+        return ops.moe_layer_int8(x, gamma, w_gate, gq, gs, dq, ds, res, 2)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in range(3):
+        x.copy_(normal(x.shape, F16, 50 + n))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), n
+        torch.cuda.synchronize()
+
+    def through_torch(x):
+        q, s, y, v = op.MoeAddRmsNormQuant(x, gamma, res, 1e-6, True)
+        ids, w = op.MoeRoutingGroupTopK(op.MoeLinear(y, w_gate.t(), outDtype=F32)[0], topK=2, weightsDtype=F32)
+        rows, off, pos, rs = op.MoePermute(q, ids, 8, s)
+        h, hs = op.MoeQuantize(op.MoeLinearInt8(rows, rs, gq, gs, off, activation="swiglu"))
+        return op.MoeUnpermute(op.MoeLinearInt8(h, hs, dq, ds, off), pos, w), v
+
+    want = step()
+    for fn in (through_torch, torch.compile(through_torch, fullgraph=True)):
+        assert all(torch.equal(a, b) for a, b in zip(fn(x), want[:2]))
+
+
+@gpu
+def test_training_step_in_a_graph(ops):
+    """Forward and backward as a whole, captured after warm-up steps whose results are dropped."""
+    x, res, gamma, ids, w = inputs(T=64)
+    ids = ids.cuda()
+    leaves = [leaf(t) for t in (x, res, gamma, w)]
+
+    def step():
+        grads = torch.autograd.grad(sorted_layer(leaves[0], leaves[1], leaves[2], ids, leaves[3], 8).square().sum(), leaves)
+        return [g.clone() for g in grads]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(normal(x.shape, F32, 70 + n))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [g.clone() for g in got]
+        assert all(torch.equal(a, b) for a, b in zip(kept, step())), n
+
+
+@gpu
+def test_layer_refusals(ops):
+    x, res, gamma, w_gate, gate_up, down = (t.cuda() for t in layer_inputs(4, 64, 4, 32, F16))
+    (gq, gs), (dq, ds) = ops.MoeQuantize(gate_up), ops.MoeQuantize(down)
+    with pytest.raises(ops.MoeError):
+        ops.moe_layer_int8(x, gamma, w_gate, gq[:3], gs, dq, ds, res)
+    with pytest.raises(ops.MoeError):
+        ops.moe_layer_int8(x, gamma, w_gate, gq, gs[:3], dq, ds, res)
