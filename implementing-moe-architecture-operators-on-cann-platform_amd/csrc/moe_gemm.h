@@ -164,7 +164,7 @@ __device__ __forceinline__ void group_advance(const GemmArgs& g, int bm, int nti
     typedef const __attribute__((address_space(4))) int32_t* Constant;
     const Constant offsets = reinterpret_cast<Constant>(reinterpret_cast<uintptr_t>(g.offsets));
     int items = group_items(item.row0, item.row1, bm, ntiles);
-    while (at >= item.first + items) {
+    while (at >= item.first + items && item.expert + 1 < g.experts) {
         item.first += items;
         ++item.expert;
         const int o0 = offsets[item.expert], o1 = offsets[item.expert + 1];

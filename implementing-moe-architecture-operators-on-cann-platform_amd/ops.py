@@ -599,21 +599,34 @@ def moe_layer_shared(x: torch.Tensor, w_gate: torch.Tensor, expert_weights: torc
 # ---------------------------------------------------------------------------------------------------------------------
 
 
+def _new(shape: tuple, dtype: torch.dtype) -> torch.Tensor:
+    """A new contiguous tensor of one or two dimensions on the current device, where _empty may use private functions."""
+    return _empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype)
+
+
+def _allocator(like: torch.Tensor, stream):
+    """_empty for several results of a call, which looks at torch's modes once: (shape, dtype) -> tensor."""
+    if stream is None and _empty_strided is not None and not _modes() and not _deterministic():
+        return _new
+    return lambda shape, dtype: _empty(like, stream, shape, dtype)
+
+
 def _gamma(gamma, dtype, H: int, dev: int) -> int:
     """Checks a norm's gamma, of the rows' type or fp32; returns its moe_dtype."""
-    gt = _need_float(gamma, "gamma", (dtype, torch.float32), 1, dev)
-    _need_shape(gamma, "gamma", (H,))
-    if not gamma.is_contiguous():
-        raise MoeError(4, "gamma must be contiguous")
-    return gt
+    gt = getattr(gamma, "dtype", None)
+    if gt is not dtype and gt is not torch.float32:
+        _need_float(gamma, "gamma", (dtype, torch.float32), 1, dev)  # raises
+    _vector(gamma, "gamma", gt, H, dev)
+    return _FLOAT_DT[gt]
 
 
 def _rows_like(t, name: str, dtype, shape, dev: int) -> tuple[int | None, int]:
     """(address, row stride) of an optional matrix of any row stride."""
     if t is None:
         return None, 0
-    _need_float(t, name, (dtype,), 2, dev)
-    _need_shape(t, name, shape)
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev):
+        _need_float(t, name, (dtype,), 2, dev)
+        _need_shape(t, name, shape)
     return t.data_ptr(), _row_stride(t, name)
 
 
@@ -636,10 +649,11 @@ def _add_rms_norm(x, gamma, residual, eps, want_y: bool, want_q: bool, stream):
     rp, ldr = _rows_like(residual, "residual", x.dtype, (T, H), dev)
     ldx = _row_stride(x, "x")
     like = _like(x)
-    q = _empty(like, stream, (T, H), torch.int8) if want_q else None
-    scale = _empty(like, stream, (T,), torch.float32) if want_q else None
-    y = _empty(like, stream, (T, H), x.dtype) if want_y else None
-    total = None if residual is None else _empty(like, stream, (T, H), x.dtype)
+    new = _allocator(like, stream)
+    q = new((T, H), torch.int8) if want_q else None
+    scale = new((T,), torch.float32) if want_q else None
+    y = new((T, H), x.dtype) if want_y else None
+    total = None if residual is None else new((T, H), x.dtype)
     check(_lib.load().moe_add_rms_norm(x.data_ptr(), ldx, rp, ldr, gamma.data_ptr(), gt, _ptr(y), _ptr(total), _ptr(q),
                                        _ptr(scale), T, H, eps, dt, _queue(stream, dev)))
     return q, scale, y, total
@@ -685,8 +699,9 @@ def MoeAddRmsNormGrad(grad_y: torch.Tensor, v: torch.Tensor, gamma: torch.Tensor
     wp, wb = None, 0
     if gradGamma:
         workspace, wp, wb = _workspace(workspace, lib.moe_add_rms_norm_grad_workspace_bytes, (T, H), like, dev, stream)
-    gx = _empty(like, stream, (T, H), v.dtype) if gradX else None
-    gg = _empty(like, stream, (H,), gamma.dtype) if gradGamma else None
+    new = _allocator(like, stream)
+    gx = new((T, H), v.dtype) if gradX else None
+    gg = new((H,), gamma.dtype) if gradGamma else None
     check(lib.moe_add_rms_norm_grad(yp, ldy, v.data_ptr(), ld, gamma.data_ptr(), gt, vp, ldv, _ptr(gx), _ptr(gg), wp, wb,
                                     T, H, eps, dt, _queue(stream, dev)))
     return gx, gg
@@ -699,14 +714,15 @@ def MoeQuantize(x: torch.Tensor, stream=None):
     if isinstance(x, torch.Tensor) and x.dim() == 3:
         if not x.is_contiguous():
             raise MoeError(4, "x must be contiguous (ND format)")
-        q, scale = MoeQuantize(x.view(-1, x.shape[2]), stream)
+        q, scale = MoeQuantize(x.view(x.shape[0] * x.shape[1], x.shape[2]), stream)
         return q.view(x.shape), scale.view(x.shape[:2])
     dt, dev = _first_float(x, "x", _FLOATS, 2)
     R, H = x.shape
     ldx = _row_stride(x, "x")
     like = _like(x)
-    q = _empty(like, stream, (R, H), torch.int8)
-    scale = _empty(like, stream, (R,), torch.float32)
+    new = _allocator(like, stream)
+    q = new((R, H), torch.int8)
+    scale = new((R,), torch.float32)
     check(_lib.load().moe_quantize(x.data_ptr(), ldx, q.data_ptr(), scale.data_ptr(), R, H, dt, _queue(stream, dev)))
     return q, scale
 
@@ -733,10 +749,11 @@ def MoePermute(x: torch.Tensor, expert_ids: torch.Tensor, numExperts: int, xScal
     lib = _lib.load()
     like = _like(x)
     workspace, wp, wb = _workspace(workspace, lib.moe_permute_workspace_bytes, (T, numExperts, K), like, dev, stream)
-    rows = _empty(like, stream, (T * K, H), x.dtype)
-    offsets = _empty(like, stream, (numExperts + 1,), torch.int32)
-    position = _empty(like, stream, (T, K), torch.int32)
-    row_scale = None if xScale is None else _empty(like, stream, (T * K,), torch.float32)
+    new = _allocator(like, stream)
+    rows = new((T * K, H), x.dtype)
+    offsets = new((numExperts + 1,), torch.int32)
+    position = new((T, K), torch.int32)
+    row_scale = None if xScale is None else new((T * K,), torch.float32)
     check(lib.moe_permute(x.data_ptr(), ldx, sp, expert_ids.data_ptr(), rows.data_ptr(), _ptr(row_scale),
                           offsets.data_ptr(), position.data_ptr(), wp, wb, T, H, numExperts, K, dt, _queue(stream, dev)))
     return rows, offsets, position, row_scale
@@ -784,8 +801,9 @@ def MoeUnpermuteGrad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: 
         raise MoeError(1, "MoeUnpermuteGrad needs rows with weights")
     ldy = _row_stride(grad_y, "grad_y")
     like = _like(grad_y)
-    grad_rows = _empty(like, stream, (T * K, H), grad_y.dtype)
-    grad_w = None if wp is None else _empty(like, stream, (T, K), weights.dtype)
+    new = _allocator(like, stream)
+    grad_rows = new((T * K, H), grad_y.dtype)
+    grad_w = None if wp is None else new((T, K), weights.dtype)
     check(_lib.load().moe_unpermute_grad(grad_y.data_ptr(), ldy, rp, position.data_ptr(), wp, wt, grad_rows.data_ptr(),
                                          _ptr(grad_w), T, H, K, dt, _queue(stream, dev)))
     return grad_rows, grad_w
