@@ -402,8 +402,8 @@ Int8Workspace int8_workspace(int64_t T, int64_t N, int64_t H, int64_t E, int32_t
 
 // Rows of a tile of the experts' products, by their rows on average; 16 streams the weights. us at means of 8, 12, 24 and
 // 32 rows, of which some experts have three times as many (E = 64, H = 2048, N = 1408 SwiGLU): streaming 68, 80, 121,
-// 155; 64 rows 76, 77, 84, 93; 128 rows 76, 89, 91, 93; 256 rows 93, 92, 94, 94, and 99 at 64 rows, where 128 take 116.
-// E = 8, H = 4096, N = 14336 152, 185, 300, 358 / 165, 164, 190, 207 / 178, 179, 178, 203 / 200, 199, 201, 208.
+// 155; 64 rows 76, 77, 84, 93; 128 rows 76, 89, 91, 93; 256 rows 93, 92, 94, 84, and 90 at 64 rows, where 128 take 116.
+// E = 8, H = 4096, N = 14336 152, 185, 300, 358 / 165, 164, 190, 207 / 178, 179, 178, 203 / 200, 199, 201, 190.
 // Operands that come through registers have tiles of 64 and 128 rows.
 int group_rows(int64_t T, int64_t E, bool direct) {
     const int64_t mean = T / E;
