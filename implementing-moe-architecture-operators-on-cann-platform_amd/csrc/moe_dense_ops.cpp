@@ -118,7 +118,8 @@ double mid_time(int bm, int64_t items, int64_t stages, bool p_by_k) {
 // clock falls), 7 to 10 us of first copies and epilogue a round, of 8-bit products 4 to 5.
 double tiled_time(int64_t tiles, int64_t stages, bool p_by_k, bool int8) {
     const double launch = p_by_k ? 7.1 : 5.8, round = p_by_k ? 9.4 : int8 ? 4.5 : 10.2, stage = p_by_k ? 1.59 : 1.46;
-    const double few_round = p_by_k ? 7.4 : int8 ? 4.0 : 6.7, few_stage = p_by_k ? 1.2 : 1.01, more = p_by_k ? 0.43 : 0.41;
+    const double few_round = p_by_k ? 7.4 : int8 ? 4.0 : 6.7, few_stage = p_by_k ? 1.2 : 1.01;
+    const double more = p_by_k ? 0.43 : 0.41;
     const double f = (tiles % 256) / 256.0;
     const double tail =
         tiles % 256 == 0 ? 0.0 : few_round + (round - few_round) * f + stages * (few_stage + more * f * f);
@@ -138,9 +139,9 @@ double reduce_time(size_t partial, bool p_by_k) {
 // 11.5), T = 64 11.6 (16.0). Above 16 rows that holds between 64 and 512 tiles of 16 weight rows: T = 32, H = 7168, N =
 // 256 12.4 us (8.3 split over k), T = 64, H = 4096, N = 16384 35 us (33). Up to 16 rows a call takes 8.3 to 8.9 us from
 // N = 8 to 512 and H = 2048 to 8192, the host's time, where two launches take 10.7.
-// 8-bit products (k in pairs) take the same times but for the epilogue of their 256 x 256 tiles, and above 16 rows stream
-// up to 512 tiles: H = 4096, N = 14336 SwiGLU (1792 tiles) at T = 32 30 us, tiles of 32 rows 24. Of 90 products (T = 1 ..
-// 16384) the choice is the fastest kernel or 1 to 2 % slower on average.
+// 8-bit products (k in pairs) take the same times but for the epilogue of their 256 x 256 tiles, and above 16 rows
+// stream up to 512 tiles: H = 4096, N = 14336 SwiGLU (1792 tiles) at T = 32 30 us, tiles of 32 rows 24. Of 90 products
+// (T = 1 .. 16384) the choice is the fastest kernel or 1 to 2 % slower on average.
 // most_rows: the tallest tiles to choose from.
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, bool swiglu, bool p_by_k, bool q_by_k, bool direct,
                          int most_rows = 256, bool int8 = false) {
@@ -372,9 +373,9 @@ moe_status check_linear_int8(int64_t T, int64_t N, int64_t H, int64_t E, int32_t
     return ok();
 }
 
-// Workspace: x and the weights with rows padded to 16 bytes, where H is no multiple of that and the product has rows enough
-// for it to pay (T = 8000, H = 4001, N = 4000 429 us through registers; T = 200, H = 2001, N = 2000 20 either way) |
-// partial sums of a split product
+// Workspace: x and the weights with rows padded to 16 bytes, where H is no multiple of that and the product has rows
+// enough for it to pay (T = 8000, H = 4001, N = 4000 429 us through registers; T = 200, H = 2001, N = 2000 20 either
+// way) | partial sums of a split product
 struct Int8Workspace {
     bool padded;
     size_t w_at, partial_at, bytes;
@@ -400,10 +401,10 @@ Int8Workspace int8_workspace(int64_t T, int64_t N, int64_t H, int64_t E, int32_t
     return w;
 }
 
-// Rows of a tile of the experts' products, by their rows on average; 16 streams the weights. us at means of 8, 12, 24 and
-// 32 rows, of which some experts have three times as many (E = 64, H = 2048, N = 1408 SwiGLU): streaming 68, 80, 121,
-// 155; 64 rows 76, 77, 84, 93; 128 rows 76, 89, 91, 93; 256 rows 93, 92, 94, 84, and 90 at 64 rows, where 128 take 116.
-// E = 8, H = 4096, N = 14336 152, 185, 300, 358 / 165, 164, 190, 207 / 178, 179, 178, 203 / 200, 199, 201, 190.
+// Rows of a tile of the experts' products, by their rows on average; 16 streams the weights. us at means of 8, 12, 24
+// and 32 rows, of which some experts have three times as many (E = 64, H = 2048, N = 1408 SwiGLU): streaming 68, 80,
+// 121, 155; 64 rows 76, 77, 84, 93; 128 rows 76, 89, 91, 93; 256 rows 93, 92, 94, 84, and 90 at 64 rows, where 128 take
+// 116. E = 8, H = 4096, N = 14336 152, 185, 300, 358 / 165, 164, 190, 207 / 178, 179, 178, 203 / 200, 199, 201, 190.
 // Operands that come through registers have tiles of 64 and 128 rows.
 int group_rows(int64_t T, int64_t E, bool direct) {
     const int64_t mean = T / E;
@@ -735,7 +736,8 @@ moe_status moe_linear_int8(const int8_t* x, int64_t x_stride, const float* x_sca
     hipError_t err = moe::prepare_linear_int8();
     if (err != hipSuccess) return hip_fail(err, "MoeLinearInt8 kernel attributes");
     const hipStream_t s = as_stream(stream);
-    int64_t pitch = T > 1 ? x_stride : 0, weight_pitch = Z > 1 ? weight_stride : 0, step = E > 1 ? expert_stride : 0, k = H;
+    int64_t pitch = T > 1 ? x_stride : 0, weight_pitch = Z > 1 ? weight_stride : 0;
+    int64_t step = E > 1 ? expert_stride : 0, k = H;
     if (room.padded) {
         char* base = static_cast<char*>(workspace);
         moe::Repack8 px{}, pw{};

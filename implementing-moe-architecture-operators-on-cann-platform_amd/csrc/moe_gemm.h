@@ -45,10 +45,10 @@ struct Bf16 {
     }
 };
 
-// 8-bit integers with results of type O. A pair of them stands where the 16-bit types have one value, so the kernels move
-// the same bytes: k, the strides and the stages count pairs (of operands that 16-byte copies cannot read, bytes). The
-// fp32 registers of the sums hold int32 bits up to the epilogue, which applies the scales; k is short enough that no sum
-// leaves 32 bits.
+// 8-bit integers with results of type O. A pair of them stands where the 16-bit types have one value, so the kernels
+// move the same bytes: k, the strides and the stages count pairs (of operands that 16-byte copies cannot read, bytes).
+// The fp32 registers of the sums hold int32 bits up to the epilogue, which applies the scales; k is short enough that
+// no sum leaves 32 bits.
 template <typename O>
 struct Int8 {
     using Bits = uint16_t;
@@ -277,8 +277,8 @@ __device__ __forceinline__ f32x4 load_scales4(const float* p, int valid) {
 }
 
 // The scales that a wave's epilogue needs, loaded before its blocks: at each block's own time their latency was most of
-// the epilogue (256 x 256 tiles: 12.5 us of 25 at H = 2048). A lane has the same 8 columns in every block (SwiGLU: gate and
-// up), and of each 64 rows the scale of one, which the block's lanes fetch from each other.
+// the epilogue (256 x 256 tiles: 12.5 us of 25 at H = 2048). A lane has the same 8 columns in every block (SwiGLU: gate
+// and up), and of each 64 rows the scale of one, which the block's lanes fetch from each other.
 template <bool SWIGLU, int ROWS>
 struct WaveScales {
     static constexpr int kParts = (ROWS + kWave - 1) / kWave;
@@ -372,8 +372,8 @@ __device__ __forceinline__ f32x4 finish4(const GemmArgs& g, int64_t row, int col
     return y;
 }
 
-// The same, written to out; columns from n on are left alone. `vec`: whole vectors are aligned (vector_rows). SCALED: sums
-// of 8-bit products have their scales.
+// The same, written to out; columns from n on are left alone. `vec`: whole vectors are aligned (vector_rows). SCALED:
+// sums of 8-bit products have their scales.
 template <typename T, bool SWIGLU, bool SCALED = false>
 __device__ __forceinline__ void store4(const GemmArgs& g, int64_t row, int col, f32x4 z, f32x4 u, bool vec) {
     if (col >= g.n) return;
@@ -594,7 +594,8 @@ struct RepackArgs {
     Repack m[kRepackMost];
 };
 hipError_t launch_repack(const RepackArgs& a, hipStream_t stream);
-// Of 8-bit rows, padded to whole 16 bytes: `rows` of cols bytes, src_ld apart, and group_ld from one group's to the next's
+// Of 8-bit rows, padded to whole 16 bytes: `rows` of cols bytes, src_ld apart, and group_ld from one group's to the
+// next's
 struct Repack8 {
     const uint8_t* src;
     uint8_t* dst;
@@ -627,8 +628,8 @@ hipError_t launch_gemm_stream(const GemmArgs& g, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_tiled(const GemmArgs& g, bool p_by_k, bool q_by_k, bool bf16, hipStream_t stream);
 hipError_t launch_gemm_reduce(const GemmArgs& g, bool bf16, hipStream_t stream);
 
-// The same of 8-bit operands, both by rows; bf16: the results. With experts mid takes 64 or 128 rows a tile, and no product
-// is split
+// The same of 8-bit operands, both by rows; bf16: the results. With experts mid takes 64 or 128 rows a tile, and no
+// product is split
 hipError_t prepare_int8_mid();
 hipError_t prepare_int8_stream();
 hipError_t prepare_int8_tiled();

@@ -1,5 +1,5 @@
-// moe_linear_mid.h -- the dense product on tiles of 32 to 256 rows by 128, and the sum of a product's pieces: kernels and
-// their launches for the types that moe_linear.hip and moe_linear_int8.hip give them.
+// moe_linear_mid.h -- the dense product on tiles of 32 to 256 rows by 128, and the sum of a product's pieces: kernels
+// and their launches for the types that moe_linear.hip and moe_linear_int8.hip give them.
 #pragma once
 
 #include "moe_gemm.h"
@@ -165,7 +165,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& all, int mtiles, int nt
         const int kc = k0 + s * kStageK;
         if constexpr (T::kInt8 && !DIRECT) {  // by rows, bytes
             static_assert(!PK && !QK, "8-bit operands are by rows");
-            auto load = [&](const uint16_t* base, int64_t ld, int row, int rows, int el) __attribute__((always_inline)) {
+            auto load = [&](const uint16_t* base, int64_t ld, int row, int rows, int el)
+                            __attribute__((always_inline)) {
                 const int k = kc + el * 2;
                 return load16(reinterpret_cast<const uint8_t*>(base) + static_cast<int64_t>(row) * ld + k,
                               row < rows ? k1 - k : 0, k);
@@ -318,7 +319,9 @@ hipError_t run_mid(const GemmArgs& g, hipStream_t stream) {
 
 // Adds the splits' sums in order and applies the epilogue; a thread has 4 columns of a row.
 constexpr int kReduceThreads = 256;
-inline int64_t reduce_blocks(const GemmArgs& g) { return (part_cols(g.n) / 4 * g.m + kReduceThreads - 1) / kReduceThreads; }
+inline int64_t reduce_blocks(const GemmArgs& g) {
+    return (part_cols(g.n) / 4 * g.m + kReduceThreads - 1) / kReduceThreads;
+}
 template <typename T, bool SWIGLU>
 __device__ __forceinline__ void gemm_reduce(const GemmArgs& g, int block) {
     const int64_t pcols = part_cols(g.n), pld = part_ld(g.n, SWIGLU), per_row = pcols / 4;

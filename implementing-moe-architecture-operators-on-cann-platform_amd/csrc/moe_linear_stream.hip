@@ -14,6 +14,9 @@
 //   persistent  a workgroup per CU walks its tiles and the rings run on across them, so the next tile's weights are in
 //             flight while the sums of this one are added.
 // Rows past the last and k past the end read zeros without memory traffic.
+// 8-bit integers (MoeLinearInt8) take half the bytes: T = 1, H = 7168, N = 2048 SwiGLU, 29 MB, 7.4 us. The products of
+// experts with few rows each (GROUPED) are items of 16 rows of an expert by 64 of its weight rows; a workgroup has the
+// experts' items in registers, as loads of the offsets between the copies would wait for those.
 #include "moe_gemm.h"
 
 #include <type_traits>
@@ -54,8 +57,8 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
     const __amdgpu_buffer_rsrc_t pr =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.p), 0, 0x7fffffff, 0x00020000);
 
-    // Experts: `tiles` is an expert's, and an item one of them for 16 MB of the expert's rows; items of the same weights
-    // are neighbours.
+    // Experts: `tiles` is an expert's, and an item one of them for 16 MB of the expert's rows; items of the same
+    // weights are neighbours.
     const int ntiles = tiles;
     GroupItem cgroup{};
     GroupTable table;
@@ -100,10 +103,9 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
                 qr, (__attribute__((address_space(3))) void*)(slot + i * 512), 16,
                 static_cast<int>(live && n0 + row < g.n && k < g.k ? off : kPastEnd), 0, 0, kNonTemporal);
         }
+        const uint16_t* px = g.p + static_cast<int64_t>(cplace.row0) * g.ldp;
         const __amdgpu_buffer_rsrc_t pe =
-            GROUPED ? __builtin_amdgcn_make_buffer_rsrc(
-                          const_cast<uint16_t*>(g.p + static_cast<int64_t>(cplace.row0) * g.ldp), 0, 0x7fffffff, 0x00020000)
-                    : pr;
+            GROUPED ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(px), 0, 0x7fffffff, 0x00020000) : pr;
         const int rows = GROUPED ? cgroup.row1 - cplace.row0 : g.m;
 #pragma unroll
         for (int i = 0; i < 2 * MB; ++i) {
@@ -182,7 +184,8 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
                 for (int w = 0; w < WAVES; ++w) {
                     const float* at = sums + (w * kRows + r) * kGranules * 4;
                     z = T::add(z, *reinterpret_cast<const f32x4*>(at + (c ^ (r % kGranules)) * 4));
-                    if (SWIGLU) u = T::add(u, *reinterpret_cast<const f32x4*>(at + ((kQuads + c) ^ (r % kGranules)) * 4));
+                    const float* ups = at + ((kQuads + c) ^ (r % kGranules)) * 4;
+                    if (SWIGLU) u = T::add(u, *reinterpret_cast<const f32x4*>(ups));
                 }
                 store4<T, SWIGLU>(ge, row, place.nt * kCols + c * 4, z, u, vec);
             }
@@ -198,8 +201,8 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-// Rows of P up to 16, 32 and 64: waves and depths whose rings fill a CU's LDS. Four blocks of weight rows: 8-bit products
-// of up to 16 rows
+// Rows of P up to 16, 32 and 64: waves and depths whose rings fill a CU's LDS. Four blocks of weight rows: 8-bit
+// products of up to 16 rows
 constexpr int kWideBlocks = 4;
 template <typename F>
 hipError_t by_rows(int m, int qb, F&& f) {
@@ -244,11 +247,12 @@ hipError_t prepare(int m, int qb) {
     return by_rows(m, qb, [](auto q, auto mb, auto waves, auto depth) {
         constexpr int Q = decltype(q)::value, M = decltype(mb)::value, W = decltype(waves)::value,
                       D = decltype(depth)::value;
-        hipError_t err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, true, GROUPED>),
-                                          StreamLds<Q, M, W, D>::kBytes);
+        constexpr int kBytes = StreamLds<Q, M, W, D>::kBytes;
+        hipError_t err = ensure_lds_limit(
+            reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, true, GROUPED>), kBytes);
         if (err == hipSuccess)
-            err = ensure_lds_limit(reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, false, GROUPED>),
-                                   StreamLds<Q, M, W, D>::kBytes);
+            err = ensure_lds_limit(
+                reinterpret_cast<const void*>(&gemm_stream_kernel<T, Q, M, W, D, false, GROUPED>), kBytes);
         return err;
     });
 }
@@ -296,14 +300,14 @@ hipError_t prepare_int8_stream() {
     return err;
 }
 
-// Experts' products go by 64 weight rows for 16 rows of P. E = 64, H = 2048, N = 1408 SwiGLU, 4 rows an expert on average:
-// 63 us, 5.6 TB/s of weights (32 weight rows a tile 72, 16 100; tiles for 32 rows of P 80, for 64 107).
+// Experts' products go by 64 weight rows for 16 rows of P. E = 64, H = 2048, N = 1408 SwiGLU, 4 rows an expert on
+// average: 63 us, 5.6 TB/s of weights (32 weight rows a tile 72, 16 100; tiles for 32 rows of P 80, for 64 107).
 hipError_t launch_int8_stream(const GemmArgs& g, bool bf16, hipStream_t stream) {
     if (g.experts)
         return bf16 ? run_stream_any<Int8<Bf16>, true>(g, 16, kWideBlocks, stream)
                     : run_stream_any<Int8<Half>, true>(g, 16, kWideBlocks, stream);
-    // Up to 16 rows the widest tile that gives every CU one; us of 16, 32 and 64 weight rows at T = 1, H = 4096: N = 8192
-    // 12.7, 11.0, 11.3, N = 16384 19.6, 16.5, 14.9; H = 14336, N = 4096 12.8, 14.7, 24.1
+    // Up to 16 rows the widest tile that gives every CU one; us of 16, 32 and 64 weight rows at T = 1, H = 4096: N =
+    // 8192 12.7, 11.0, 11.3, N = 16384 19.6, 16.5, 14.9; H = 14336, N = 4096 12.8, 14.7, 24.1
     const int64_t rows = weight_rows(g);
     const int qb = g.m > 16 ? tile_blocks(g.m, rows) : rows >= 64 * 256 ? kWideBlocks : rows >= 32 * 256 ? 2 : 1;
     return bf16 ? run_stream_any<Int8<Bf16>>(g, g.m, qb, stream) : run_stream_any<Int8<Half>>(g, g.m, qb, stream);

@@ -13,6 +13,13 @@
 // grad_weight there has 176 tiles for 256 CUs and takes 200 us: tiles of 256 x 192 (242 of them) took 170 us where
 // these took 177, and 168 to 199 us where these took 137 to 142 on full rounds, so a product is not bound by the CUs it
 // leaves idle.
+//
+// 8-bit integers (MoeLinearInt8, both operands by rows) run through the same loop with half the stages, so what a tile
+// takes beside them counts twice: its epilogue has a form without branches (int8_epilogue). T = 16381, H = 2048, N =
+// 2816 SwiGLU 162-172 us, 2200-2330 TOP/s with the epilogue; 8192^3 382 us, 2880 TOP/s (the library's product alone:
+// 2415). The products of experts (GROUPED): a tile's expert comes from the offsets, by scalar loads from the tile
+// before's on. 98304 rows by 64 experts, N = 2048, H = 1408: 302 us, 1880 TOP/s, of which 44 are the stores' and 8 % of
+// the tiles' rows are empty.
 #include "moe_gemm.h"
 
 namespace moe {
@@ -246,11 +253,11 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         tick_c(acc[1], first, upper);
     };
 
-    // The epilogue of 8-bit products without bias and residual, without a branch: scales and SwiGLU while the sums are in
-    // registers (gate and up of a column are in one lane), then 16-bit results through LDS. A lane's 4 columns are 8 bytes;
-    // a block's row has 8 granules of 16 bytes (SwiGLU 4), granule G standing at G ^ (row & 7) (SwiGLU row >> 1 & 3), and
-    // two blocks take turns in the wave's 4 KB. The general epilogue's branches on what each value gets took 11 us of a
-    // tile's 29 (H = 1408), whatever was stored or loaded.
+    // The epilogue of 8-bit products without bias and residual, without a branch: scales and SwiGLU while the sums are
+    // in registers (gate and up of a column are in one lane), then 16-bit results through LDS. A lane's 4 columns are 8
+    // bytes; a block's row has 8 granules of 16 bytes (SwiGLU 4), granule G standing at G ^ (row & 7) (SwiGLU row >> 1
+    // & 3), and two blocks take turns in the wave's 4 KB. The general epilogue's branches on what each value gets took
+    // 11 us of a tile's 29 (H = 1408), whatever was stored or loaded.
     auto int8_epilogue = [&](const GemmArgs& ge, const Acc (&acc)[2], char* stg, int ln, int row0, int c0)
                              __attribute__((always_inline)) {
         constexpr int kJ = SWIGLU ? 2 : 4, kGran = 2 * kJ, kReads = kGran / 4;
@@ -296,7 +303,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
                 if (row < ge.m && col < ge.n)
                     *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * ge.n + col) = v;
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // read before the writes of the block after the next
+            // read before the writes of the block after the next
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
     };
@@ -418,8 +426,8 @@ hipError_t run_tiled_any(const GemmArgs& g, bool p_by_k, bool q_by_k, hipStream_
 template <typename T>
 hipError_t run_int8(const GemmArgs& g, hipStream_t stream) {
     const bool swiglu = g.act == kActSwiglu;
-    // Half tiles left out pay where most experts have them: E = 64, H = 2048, N = 1408 SwiGLU, means of 32, 64 and 128 rows
-    // 93 -> 84, 99 -> 90, 105 -> 100 us; 1536 rows 511 -> 517
+    // Half tiles left out pay where most experts have them: E = 64, H = 2048, N = 1408 SwiGLU, means of 32, 64 and 128
+    // rows 93 -> 84, 99 -> 90, 105 -> 100 us; 1536 rows 511 -> 517
     if (g.experts && g.m < 160 * static_cast<int64_t>(g.experts))
         return swiglu ? run_tiled<T, false, false, true, true, true>(g, stream)
                       : run_tiled<T, false, false, false, true, true>(g, stream);

@@ -1,13 +1,18 @@
 // moe_norm.hip -- MoeAddRmsNorm, MoeAddRmsNormQuant, MoeAddRmsNormGrad and MoeQuantize for gfx950.
 //
-// v = x + residual in fp32, y = v r gamma with r = 1 / sqrt(mean v^2 + eps). The 8-bit form of a row is q = rint(p 127 /
-// max |p|): with p = v gamma the factor r, which a row has in common, cancels, so q needs no sum and is the same
+// v = x + residual in fp32, y = v r gamma with r = 1 / sqrt(mean v^2 + eps). The 8-bit form of a row is q = rint(p 127
+// / max |p|): with p = v gamma the factor r, which a row has in common, cancels, so q needs no sum and is the same
 // whatever the order of the sums; r enters the scale alone, max |p| r / 127. The gradient with u = v r: grad_v = r
 // (grad_y gamma - u mean(grad_y gamma u)) + grad_sum, grad_gamma = the column sums of grad_y u.
 //
-// Memory bounds them: each row is read once into registers by 1, 4 or 16 waves (8 values a lane and step), reduced,
-// and written from there; rows too long for that are read twice. Squares are added in fp64, which neither overflows nor
-// loses a small row, and takes no time that memory does not hide.
+// Memory bounds them: a row is read once into the registers of 1 to 16 waves (8 values a lane and step), reduced, and
+// written from there; rows above 32768 values are read twice. Squares are added in fp64, which neither overflows nor
+// loses a small row, and takes no time that memory does not hide. Reductions go over the lanes by DPP and then over the
+// waves through LDS, in a fixed order.
+//   T = 16381, H = 2048 bf16, x + residual -> sum, y, q  58.6 us, 5.15 TB/s (a copy of 1 GB: 5.13)
+//   98304 rows of 1408 bf16 -> q                         72.3 us, 5.75 TB/s
+//   gradient of T = 8192, H = 2048 fp16 with grad_sum    29.7 us, 4.5 TB/s, and 5.1 for the workgroups' column sums
+//   T = 1, H = 7168                                      4.3 us, a row's latency: of a call of 8.6
 #include "moe_ops.h"
 #include "moe_rows.h"
 
@@ -62,8 +67,8 @@ __device__ __forceinline__ RowFactor row_factor(double squares, int H, float eps
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// NORM: the norm (its result, its 8-bit form or both), gamma of type G; else the 8-bit form of x itself. CHUNKS steps of V
-// values a lane hold a row; 0: any length, read twice.
+// NORM: the norm (its result, its 8-bit form or both), gamma of type G; else the 8-bit form of x itself. CHUNKS steps
+// of V values a lane hold a row; 0: any length, read twice.
 template <typename T, typename G, int WAVES, int CHUNKS, int V, bool NORM>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_kernel(NormArgs n) {
     using Bits = typename T::Bits;
@@ -71,7 +76,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_kernel(
     constexpr int kStep = WAVES * kWave * V;
     constexpr int kSteps = CHUNKS > 0 ? CHUNKS : 1;
     __shared__ RowExchange<WAVES> ex;
-    const int wave = static_cast<int>(threadIdx.x) / kWave, lead = WAVES == 1 ? lane_id() : static_cast<int>(threadIdx.x);
+    const int wave = static_cast<int>(threadIdx.x) / kWave;
+    const int lead = WAVES == 1 ? lane_id() : static_cast<int>(threadIdx.x);
     const bool ragged = n.H % V != 0;
     const typename G::Bits* gamma = static_cast<const typename G::Bits*>(n.gamma);
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0); row < n.rows;
@@ -173,8 +179,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_kernel(
     }
 }
 
-// The gradient. A workgroup walks rows, at least 4 waves' worth at a time, and keeps its share of grad_gamma's column sums
-// in registers; they leave as one row of `part` for each workgroup.
+// The gradient. A workgroup walks rows, at least 4 waves' worth at a time, and keeps its share of grad_gamma's column
+// sums in registers; they leave as one row of `part` for each workgroup.
 constexpr int grad_threads(int waves) { return waves <= 4 ? 256 : waves * kWave; }
 template <typename T, typename G, int WAVES, int STEPS, int V>
 __global__ __launch_bounds__(grad_threads(WAVES)) void norm_grad_kernel(NormArgs n) {
@@ -183,7 +189,8 @@ __global__ __launch_bounds__(grad_threads(WAVES)) void norm_grad_kernel(NormArgs
     constexpr int kStep = WAVES * kWave * V;
     __shared__ RowExchange<WAVES> ex[kRows];
     __shared__ float sums[kRows > 1 ? kRows - 1 : 1][kRows > 1 ? STEPS * kStep : 1];
-    const int team = static_cast<int>(threadIdx.x) / (WAVES * kWave), lead = static_cast<int>(threadIdx.x) % (WAVES * kWave);
+    const int team = static_cast<int>(threadIdx.x) / (WAVES * kWave);
+    const int lead = static_cast<int>(threadIdx.x) % (WAVES * kWave);
     const typename G::Bits* gamma = static_cast<const typename G::Bits*>(n.gamma);
     Step<V> at[STEPS];
 #pragma unroll
@@ -214,7 +221,7 @@ __global__ __launch_bounds__(grad_threads(WAVES)) void norm_grad_kernel(NormArgs
             load_row<G, V>(gamma + at[c].at, g);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const bool counts = j >= at[c].skip;  // past the row all are to be skipped
+                const bool counts = j >= at[c].skip;  // past the row none does
                 const double a = counts ? v[c].get(j) : 0.0f;
                 squares += a * a;
                 dot += static_cast<double>(counts ? d[c].get(j) * g[j] : 0.0f) * a;
@@ -295,10 +302,10 @@ __global__ __launch_bounds__(kSumThreads) void gamma_sum_kernel(const float* __r
     out[col] = G::store(s);
 }
 
-// Waves of a row, and the steps that hold it (0: none do). Where there are rows enough for every SIMD a row has two steps
-// in flight for as few waves as that takes; few rows are spread over as many waves as have one step each.
-//   x + residual with y and its 8-bit form, bf16, us with 1, 2, 4 waves: T = 16384, H = 512 18 / 22 / 34; H = 1024 32 / 31
-//   / 42; H = 2048 74 (four steps) / 58 / 59; T = 98304, H = 1408 328 / 244 / 260
+// Waves of a row, and the steps that hold it (0: none do). Where there are rows enough for every SIMD a row has two
+// steps in flight for as few waves as that takes; few rows are spread over as many waves as have one step each.
+//   x + residual with y and its 8-bit form, bf16, us with 1, 2, 4 waves: T = 16384, H = 512 18 / 22 / 34; H = 1024 32 /
+//   31 / 42; H = 2048 74 (four steps) / 58 / 59; T = 98304, H = 1408 328 / 244 / 260
 struct Shape {
     int waves, steps;
 };
@@ -374,8 +381,8 @@ hipError_t launch_norm(const NormArgs& n, int type, bool norm, hipStream_t strea
     });
 }
 
-// Workgroups of the gradient, 16 waves on every CU at most. T = 8192, H = 2048, us of both launches: 2 waves a row and 1024
-// workgroups 31.5, 512 34.0; 1 wave (four steps) 33.1 with 512; 4 waves (one step) 33.5 with 1024
+// Workgroups of the gradient, 16 waves on every CU at most. T = 8192, H = 2048, us of both launches: 2 waves a row and
+// 1024 workgroups 31.5, 512 34.0; 1 wave (four steps) 33.1 with 512; 4 waves (one step) 33.5 with 1024
 int norm_grad_blocks(int64_t rows, int H) {
     const int64_t most = H <= 2048 ? 1024 : H <= 8192 ? 512 : 256;
     const int64_t blocks = H <= 1024 ? (rows + 3) / 4 : H <= 2048 ? (rows + 1) / 2 : rows;

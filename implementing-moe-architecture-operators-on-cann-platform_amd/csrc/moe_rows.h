@@ -87,11 +87,13 @@ __device__ __forceinline__ void store_row(typename T::Bits* p, const float (&v)[
     } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            store16<NT>(p + 4 * h, __builtin_bit_cast(u32x4, f32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]}));
+            store16<NT>(p + 4 * h,
+                        __builtin_bit_cast(u32x4, f32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]}));
     }
 }
 
-// All-reduce over a whole wave, every lane active: the lanes of a DPP row of 16 by rotations, then the four rows' results
+// All-reduce over a whole wave, every lane active: the lanes of a DPP row of 16 by rotations, then the four rows'
+// results
 template <int CTRL>
 __device__ __forceinline__ uint32_t turned(uint32_t v) {
     return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xf, 0xf, true));

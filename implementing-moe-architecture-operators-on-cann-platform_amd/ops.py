@@ -671,8 +671,8 @@ def MoeAddRmsNormQuant(x: torch.Tensor, gamma: torch.Tensor, residual: torch.Ten
                        returnNorm: bool = False, stream=None):
     """MoeAddRmsNorm's y in 8 bits -> (q[T,H] int8, scale[T] fp32, y, v): q * scale is y, scale = max|y| / 127 of a row.
     y itself (for a router) with returnNorm, else None; v is None without a residual. q is rint(p * (127 / max|p|)) with
-    p = v * gamma, the same bits whatever the launch; a row of zeros has scale 0, one that holds an infinity or a NaN has
-    q 0 and scale NaN."""
+    p = v * gamma, the same bits whatever the launch; a row of zeros has scale 0, one that holds an infinity or a NaN
+    has q 0 and scale NaN."""
     return _add_rms_norm(x, gamma, residual, eps, returnNorm, True, stream)
 
 
@@ -683,9 +683,10 @@ def add_rms_norm_grad_workspace_bytes(T: int, H: int) -> int:
 def MoeAddRmsNormGrad(grad_y: torch.Tensor, v: torch.Tensor, gamma: torch.Tensor, grad_v: torch.Tensor | None = None,
                       eps: float = 1e-6, gradX: bool = True, gradGamma: bool = True,
                       workspace: torch.Tensor | None = None, stream=None):
-    """The gradients of MoeAddRmsNorm -> (grad_x[T,H], grad_gamma[H]), None where not asked for. v is the sum it returned
-    (x itself without a residual), grad_v the gradient that reaches the sum by another way. grad_x is the residual's
-    gradient too. H <= 16384. `workspace` (uint8, >= add_rms_norm_grad_workspace_bytes) is allocated when not given."""
+    """The gradients of MoeAddRmsNorm -> (grad_x[T,H], grad_gamma[H]), None where not asked for. v is the sum it
+    returned (x itself without a residual), grad_v the gradient that reaches the sum by another way. grad_x is the
+    residual's gradient too. H <= 16384. `workspace` (uint8, >= add_rms_norm_grad_workspace_bytes) is allocated when not
+    given."""
     dt, dev = _first_float(v, "v", _FLOATS, 2)
     T, H = v.shape
     gt = _gamma(gamma, v.dtype, H, dev)
@@ -702,15 +703,16 @@ def MoeAddRmsNormGrad(grad_y: torch.Tensor, v: torch.Tensor, gamma: torch.Tensor
     new = _allocator(like, stream)
     gx = new((T, H), v.dtype) if gradX else None
     gg = new((H,), gamma.dtype) if gradGamma else None
-    check(lib.moe_add_rms_norm_grad(yp, ldy, v.data_ptr(), ld, gamma.data_ptr(), gt, vp, ldv, _ptr(gx), _ptr(gg), wp, wb,
-                                    T, H, eps, dt, _queue(stream, dev)))
+    check(lib.moe_add_rms_norm_grad(yp, ldy, v.data_ptr(), ld, gamma.data_ptr(), gt, vp, ldv, _ptr(gx), _ptr(gg), wp,
+                                    wb, T, H, eps, dt, _queue(stream, dev)))
     return gx, gg
 
 
 def MoeQuantize(x: torch.Tensor, stream=None):
-    """Rows in 8 bits: x[R,H] (fp32, fp16 or bf16) -> (q[R,H] int8, scale[R] fp32), q * scale being x and scale = max|x| /
-    127 of a row. Contiguous experts' weights [E,N,H] -> (q[E,N,H], scale[E,N]): a weight row's scale is its output
-    channel's. q is rint(x * (127 / max|x|)); rows of zeros have scale 0, rows with an infinity or a NaN q 0 and scale NaN."""
+    """Rows in 8 bits: x[R,H] (fp32, fp16 or bf16) -> (q[R,H] int8, scale[R] fp32), q * scale being x and scale = max|x|
+    / 127 of a row. Contiguous experts' weights [E,N,H] -> (q[E,N,H], scale[E,N]): a weight row's scale is its output
+    channel's. q is rint(x * (127 / max|x|)); rows of zeros have scale 0, rows with an infinity or a NaN q 0 and scale
+    NaN."""
     if isinstance(x, torch.Tensor) and x.dim() == 3:
         if not x.is_contiguous():
             raise MoeError(4, "x must be contiguous (ND format)")
@@ -733,11 +735,11 @@ def permute_workspace_bytes(T: int, E: int, K: int) -> int:
 
 def MoePermute(x: torch.Tensor, expert_ids: torch.Tensor, numExperts: int, xScale: torch.Tensor | None = None,
                workspace: torch.Tensor | None = None, stream=None):
-    """x[T,H] (fp32, fp16, bf16 or int8), expert_ids[T,K] int32 -> (rows[T*K,H], offsets[E+1] int32, position[T,K] int32,
-    row_scale): the rows of all picks sorted by expert, one expert's in the order of their slots. Expert e has rows
-    [offsets[e], offsets[e+1]). Picks whose id is outside [0, E) come last, with rows of zeros. position is a pick's row,
-    -1 - row of a pick of no expert. xScale[T] fp32 (8-bit rows' scales) is sorted alike, else row_scale is None.
-    The gradient of rows is MoeUnpermute(grad_rows, position). `workspace` (uint8, >= permute_workspace_bytes) is
+    """x[T,H] (fp32, fp16, bf16 or int8), expert_ids[T,K] int32 -> (rows[T*K,H], offsets[E+1] int32, position[T,K]
+    int32, row_scale): the rows of all picks sorted by expert, one expert's in the order of their slots. Expert e has
+    rows [offsets[e], offsets[e+1]). Picks whose id is outside [0, E) come last, with rows of zeros. position is a
+    pick's row, -1 - row of a pick of no expert. xScale[T] fp32 (8-bit rows' scales) is sorted alike, else row_scale is
+    None. The gradient of rows is MoeUnpermute(grad_rows, position). `workspace` (uint8, >= permute_workspace_bytes) is
     allocated when not given."""
     dt, dev = _first_float(x, "x", (*_FLOATS, torch.int8), 2)
     T, H = x.shape
@@ -755,7 +757,8 @@ def MoePermute(x: torch.Tensor, expert_ids: torch.Tensor, numExperts: int, xScal
     position = new((T, K), torch.int32)
     row_scale = None if xScale is None else new((T * K,), torch.float32)
     check(lib.moe_permute(x.data_ptr(), ldx, sp, expert_ids.data_ptr(), rows.data_ptr(), _ptr(row_scale),
-                          offsets.data_ptr(), position.data_ptr(), wp, wb, T, H, numExperts, K, dt, _queue(stream, dev)))
+                          offsets.data_ptr(), position.data_ptr(), wp, wb, T, H, numExperts, K, dt,
+                          _queue(stream, dev)))
     return rows, offsets, position, row_scale
 
 
@@ -772,9 +775,9 @@ def _row_weights(weights, shape, dev: int) -> tuple[int | None, int]:
 
 def MoeUnpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None = None,
                  stream=None) -> torch.Tensor:
-    """rows[R,H] (fp32, fp16 or bf16), position[T,K], weights[T,K] (fp32, fp16 or bf16; None: 1) -> y[T,H] of rows' type,
-    y[t] = sum over k of weights[t,k] * rows[position[t,k]] in fp32, ascending k. Positions outside [0, R) (a pick of no
-    expert is negative) add nothing."""
+    """rows[R,H] (fp32, fp16 or bf16), position[T,K], weights[T,K] (fp32, fp16 or bf16; None: 1) -> y[T,H] of rows'
+    type, y[t] = sum over k of weights[t,k] * rows[position[t,k]] in fp32, ascending k. Positions outside [0, R) (a pick
+    of no expert is negative) add nothing."""
     dt, dev = _first_float(rows, "rows", _FLOATS, 2)
     if not rows.is_contiguous():
         raise MoeError(4, "rows must be contiguous (ND format)")
@@ -789,9 +792,9 @@ def MoeUnpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tens
 
 def MoeUnpermuteGrad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: torch.Tensor,
                      weights: torch.Tensor | None = None, stream=None):
-    """The gradients of MoeUnpermute's y[T,H] -> (grad_rows[T*K,H] of grad_y's type, grad_weights[T,K] of weights' type).
-    position is MoePermute's, so every row has one pick; the rows of picks of no expert get zeros. Without weights rows
-    may be None and grad_weights is None."""
+    """The gradients of MoeUnpermute's y[T,H] -> (grad_rows[T*K,H] of grad_y's type, grad_weights[T,K] of weights'
+    type). position is MoePermute's, so every row has one pick; the rows of picks of no expert get zeros. Without
+    weights rows may be None and grad_weights is None."""
     dt, dev = _first_float(grad_y, "grad_y", _FLOATS, 2)
     T, H = grad_y.shape
     _, K = _ids(position, "position", T, dev)
@@ -833,11 +836,11 @@ def MoeLinearInt8(x: torch.Tensor, xScale: torch.Tensor, weight: torch.Tensor, w
     """act((x[T,H] @ weight[N,H]^T) * xScale[T] * weightScale[N] + bias[N]) + residual[T,N] -> y[T,N] of outDtype (fp16,
     bf16 or fp32), x and weight int8, scales fp32, bias and residual of outDtype; int32 sums, rounded once.
 
-    With offsets[E+1] int32, weight[E,N,H], weightScale[E,N] and bias[E,N] are E experts': rows [offsets[e], offsets[e+1])
-    of x by the matrix of expert e (MoePermute's rows and offsets); rows from offsets[E] on become zeros. activation as
-    MoeLinear's (swiglu: 2N weight rows, the N gate rows first). H <= 131071. Rows of x and of weight may be any stride
-    apart; multiples of 16 (H too) run at full speed. `workspace` (uint8, >= linear_int8_workspace_bytes) is allocated
-    when not given."""
+    With offsets[E+1] int32, weight[E,N,H], weightScale[E,N] and bias[E,N] are E experts': rows [offsets[e],
+    offsets[e+1]) of x by the matrix of expert e (MoePermute's rows and offsets); rows from offsets[E] on become zeros.
+    activation as MoeLinear's (swiglu: 2N weight rows, the N gate rows first). H <= 131071. Rows of x and of weight may
+    be any stride apart; multiples of 16 (H too) run at full speed. `workspace` (uint8, >= linear_int8_workspace_bytes)
+    is allocated when not given."""
     act = _act_code(activation)
     _, dev = _first_float(x, "x", _INT8, 2)
     _need_float(weight, "weight", _INT8, 2 if offsets is None else 3, dev)
@@ -870,8 +873,8 @@ def MoeLinearInt8(x: torch.Tensor, xScale: torch.Tensor, weight: torch.Tensor, w
     like = _like(x)
     workspace, wp, wb = _workspace(workspace, lib.moe_linear_int8_workspace_bytes, (T, N, H, E, act), like, dev, stream)
     y = _empty(like, stream, (T, N), outDtype)
-    check(lib.moe_linear_int8(x.data_ptr(), ldx, sx, weight.data_ptr(), ldw, step, sw, op, bp, rp, y.data_ptr(), wp, wb, T,
-                              N, H, E, act, _FLOAT_DT[outDtype], _queue(stream, dev)))
+    check(lib.moe_linear_int8(x.data_ptr(), ldx, sx, weight.data_ptr(), ldw, step, sw, op, bp, rp, y.data_ptr(), wp, wb,
+                              T, N, H, E, act, _FLOAT_DT[outDtype], _queue(stream, dev)))
     return y
 
 
@@ -880,14 +883,15 @@ def moe_layer_int8(x: torch.Tensor, gamma: torch.Tensor, w_gate: torch.Tensor, g
                    residual: torch.Tensor | None = None, topK: int = 2, bias: torch.Tensor | None = None,
                    numGroups: int = 1, topGroups: int = 1, groupTop: int = 1, scoring: str = "softmax",
                    renormalize: bool = True, scale: float = 1.0, eps: float = 1e-6, stream=None):
-    """A layer of 8-bit experts behind its norm, x fp16 or bf16: the norm of x + residual for the router as it is and for
-    the experts in 8 bits (MoeAddRmsNormQuant), fp32 logits by w_gate[H,E] (MoeLinear), MoeRoutingGroupTopK, the tokens
-    sorted by expert (MoePermute), the products by gate_up[E,2I,H] with SwiGLU and, in 8 bits again (MoeQuantize), by
-    down[E,H,I] (MoeLinearInt8; MoeQuantize makes such weights and their scales [E,2I] and [E,H]), and the way back
-    (MoeUnpermute). Returns (y, v, expert_ids, weights): y without the sum v = x + residual, which the next layer adds y
-    to; v is None without a residual."""
+    """A layer of 8-bit experts behind its norm, x fp16 or bf16: the norm of x + residual for the router as it is and
+    for the experts in 8 bits (MoeAddRmsNormQuant), fp32 logits by w_gate[H,E] (MoeLinear), MoeRoutingGroupTopK, the
+    tokens sorted by expert (MoePermute), the products by gate_up[E,2I,H] with SwiGLU and, in 8 bits again
+    (MoeQuantize), by down[E,H,I] (MoeLinearInt8; MoeQuantize makes such weights and their scales [E,2I] and [E,H]), and
+    the way back (MoeUnpermute). Returns (y, v, expert_ids, weights): y without the sum v = x + residual, which the next
+    layer adds y to; v is None without a residual."""
     if w_gate.dim() != 2 or gate_up.dim() != 3 or gate_up.shape[0] != w_gate.shape[1]:
-        raise MoeError(3, f"w_gate {tuple(w_gate.shape)} and gate_up {tuple(gate_up.shape)}: [H, E] and [E, 2I, H] expected")
+        raise MoeError(3, f"w_gate {tuple(w_gate.shape)} and gate_up {tuple(gate_up.shape)}: "
+                          "[H, E] and [E, 2I, H] expected")
     q, q_scale, normed, v = MoeAddRmsNormQuant(x, gamma, residual, eps, returnNorm=True, stream=stream)
     logits = MoeLinear(normed, w_gate.t(), outDtype=torch.float32, stream=stream)
     ids, w = MoeRoutingGroupTopK(logits, bias, topK, numGroups, topGroups, groupTop, scoring, renormalize, scale,

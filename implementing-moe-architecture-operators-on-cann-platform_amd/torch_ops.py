@@ -14,14 +14,16 @@ MoeExpertFFN have none):
     torch.ops.moe_mi355x.MoeLinear(x, weight, bias, residual, activation, outDtype, returnPre) -> (y, pre)
     torch.ops.moe_mi355x.MoeRoutingGroupTopKGrad, MoeLinearGrad, MoeCombineGrad: what their backward calls
 
-and those of quantised and permuted expert layers, with the gradients of the norm and of sorting (8-bit results have none):
+and those of quantised and permuted expert layers, with the gradients of the norm and of sorting (8-bit results have
+none):
 
     torch.ops.moe_mi355x.MoeAddRmsNorm(x, gamma, residual, eps) -> (y, v)
     torch.ops.moe_mi355x.MoeAddRmsNormQuant(x, gamma, residual, eps, returnNorm) -> (q, scale, y, v)
     torch.ops.moe_mi355x.MoeQuantize(x) -> (q, scale)
     torch.ops.moe_mi355x.MoePermute(x, expert_ids, numExperts, xScale) -> (rows, offsets, position, row_scale)
     torch.ops.moe_mi355x.MoeUnpermute(rows, position, weights) -> y
-    torch.ops.moe_mi355x.MoeLinearInt8(x, xScale, weight, weightScale, offsets, bias, residual, activation, outDtype) -> y
+    torch.ops.moe_mi355x.MoeLinearInt8(x, xScale, weight, weightScale, offsets, bias, residual, activation,
+                                    outDtype) -> y
     torch.ops.moe_mi355x.MoeAddRmsNormGrad, MoeUnpermuteGrad: what their backward calls
 
 The device implementation is registered for GPU tensors only: a CPU tensor finds no kernel (there is no CPU
@@ -360,7 +362,8 @@ def _permute_setup(ctx, inputs, output):
 def _permute_backward(ctx, grad_rows, *_):
     if grad_rows is None:
         return (None,) * 4
-    return getattr(torch.ops, NAMESPACE).MoeUnpermute(grad_rows.contiguous(), ctx.saved_tensors[0], None), None, None, None
+    grad_x = getattr(torch.ops, NAMESPACE).MoeUnpermute(grad_rows.contiguous(), ctx.saved_tensors[0], None)
+    return grad_x, None, None, None
 
 
 moe_permute.register_autograd(_permute_backward, setup_context=_permute_setup)

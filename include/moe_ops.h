@@ -369,9 +369,9 @@ moe_status moe_linear_grad_f32(const float* grad_y, int64_t grad_y_stride, const
  * MoeAddRmsNorm: v = x[T, H] + residual (NULL: x), summed in float32 -> y = v * gamma / sqrt(mean(v^2) + eps) of
  *   dtype, sum = v of dtype, and y in 8 bits: q[T, H] and scale[T], q = rint(p * (127 / max|p|)) with p = v * gamma
  *   of a row (the norm's factor, which the row has in common, cancels; quotient and products rounded to float32, ties
- *   to even) and scale = max|y| / 127, so that q * scale is y. A row of zeros has scale 0; one where p holds an infinity
- *   or a NaN has scale NaN and q 0. y, sum and the pair q, scale may each be NULL. q is the same bits whatever the
- *   launch. dtype is float32, float16 or bfloat16, gamma_type that or float32; eps > 0, H <= 2^20.
+ *   to even) and scale = max|y| / 127, so that q * scale is y. A row of zeros has scale 0; one where p holds an
+ *   infinity or a NaN has scale NaN and q 0. y, sum and the pair q, scale may each be NULL. q is the same bits whatever
+ *   the launch. dtype is float32, float16 or bfloat16, gamma_type that or float32; eps > 0, H <= 2^20.
  * ---------------------------------------------------------------------------------------------------- */
 moe_status moe_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                             const void* gamma, int32_t gamma_type, void* y, void* sum, int8_t* q, float* scale,
@@ -424,18 +424,19 @@ moe_status moe_unpermute_grad(const void* grad_y, int64_t grad_y_stride, const v
 
 /* ------------------------------------------------------------------------------------------------------
  * MoeLinearInt8: x[T, H] int8 with x_scale[T], weight[N, H] int8 (SwiGLU: [2N, H], N gate rows first) with
- *   weight_scale[N] (SwiGLU: [2N]) -> y[T, N] = act((x weight^T) * x_scale * weight_scale + bias) + residual of out_dtype
- *   (float32, float16 or bfloat16), int32 sums, rounded once. bias[N] (SwiGLU: [2N]) and residual[T, N] of out_dtype, or
- *   NULL; residual may be y itself. x rows lie x_stride, weight rows weight_stride elements apart.
- *   num_experts > 0: weight[E, N, H] (expert_stride elements apart), weight_scale[E, N] and bias[E, N] of E matrices, and
- *   the rows [offsets[e], offsets[e + 1]) of x by the matrix of expert e, offsets[E + 1] ascending from 0 as moe_permute
- *   writes them; rows from offsets[E] on are written as zeros, residual and all. Values that do not ascend or lie outside
- *   [0, T] are taken into it: nothing outside the tensors is read or written. num_experts 0: offsets is not read.
- *   Any strides and alignment; operands on 16 bytes with H and the strides multiples of 16 run at full speed. Where H is
- *   none, products of many rows (T >= 256, with experts 32 E) first copy x and all weights with padded rows; other
- *   operands go through registers at a fraction of the speed. H <= 131071, where 32-bit sums end; N <= 2^20, E <= 256.
- *   The workspace (0 where none is needed; 16-byte aligned) holds those copies and partial sums of a product split over
- *   H; calls in flight at the same time need one each. Not monotone in num_tokens. The sums are exact, so y does not depend on the launch.
+ *   weight_scale[N] (SwiGLU: [2N]) -> y[T, N] = act((x weight^T) * x_scale * weight_scale + bias) + residual of
+ *   out_dtype (float32, float16 or bfloat16), int32 sums, rounded once. bias[N] (SwiGLU: [2N]) and residual[T, N] of
+ *   out_dtype, or NULL; residual may be y itself. x rows lie x_stride, weight rows weight_stride elements apart.
+ *   num_experts > 0: weight[E, N, H] (expert_stride elements apart), weight_scale[E, N] and bias[E, N] of E matrices,
+ *   and the rows [offsets[e], offsets[e + 1]) of x by the matrix of expert e, offsets[E + 1] ascending from 0 as
+ *   moe_permute writes them; rows from offsets[E] on are written as zeros, residual and all. Values that do not ascend
+ *   or lie outside [0, T] are taken into it: nothing outside the tensors is read or written. num_experts 0: offsets is
+ *   not read. Any strides and alignment; operands on 16 bytes with H and the strides multiples of 16 run at full speed.
+ *   Where H is none, products of many rows (T >= 256, with experts 32 E) first copy x and all weights with padded rows;
+ *   other operands go through registers at a fraction of the speed. H <= 131071, where 32-bit sums end; N <= 2^20, E <=
+ *   256. The workspace (0 where none is needed; 16-byte aligned) holds those copies and partial sums of a product split
+ *   over H; calls in flight at the same time need one each. Not monotone in num_tokens. The sums are exact, so y does
+ *   not depend on the launch.
  * ---------------------------------------------------------------------------------------------------- */
 size_t moe_linear_int8_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int64_t num_experts,
                                        int32_t activation);

@@ -1,8 +1,8 @@
-// Host-side fuzz driver for the operators on rows and the 8-bit products (include/moe_ops.h), built with AddressSanitizer
-// and UBSan on the host side of libmoe_mi355x.so. It launches no kernel: launch calls get null pointers, no rows or a
-// workspace one byte short, which their checks reject or return from before any launch. Sizes are seeded random and edge
-// cases. It checks statuses and messages, that a workspace holds what a call puts there (column sums, ranks, padded copies)
-// and that no query gives room for sizes its call refuses.
+// Host-side fuzz driver for the operators on rows and the 8-bit products (include/moe_ops.h), built with
+// AddressSanitizer and UBSan on the host side of libmoe_mi355x.so. It launches no kernel: launch calls get null
+// pointers, no rows or a workspace one byte short, which their checks reject or return from before any launch. Sizes
+// are seeded random and edge cases. It checks statuses and messages, that a workspace holds what a call puts there
+// (column sums, ranks, padded copies) and that no query gives room for sizes its call refuses.
 // Usage: host_fuzz_rows ITERATIONS
 #include <cstdint>
 #include <cstdio>

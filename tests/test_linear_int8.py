@@ -1,7 +1,7 @@
 """MoeLinearInt8, one product and those of experts, against 64-bit sums of the same integers.
 
-Tolerances: the int32 sums are exact; their conversion to fp32, the product with the row's scale and that with the column's
-round once each (3 * 2^-24 of the scaled sum), the bias's addition and the residual's once; activations as in
+Tolerances: the int32 sums are exact; their conversion to fp32, the product with the row's scale and that with the
+column's round once each (3 * 2^-24 of the scaled sum), the bias's addition and the residual's once; activations as in
 test_dense_ops (FN and their slopes); the result's rounding is half a step of its type."""
 from __future__ import annotations
 

@@ -1,6 +1,7 @@
-"""The host code of the operators on rows and of the 8-bit products under AddressSanitizer and UBSan: all sources are rebuilt
-with the sanitizers on the host side (-Xarch_host; the device code as usual), and tests/host_fuzz_rows.cpp calls their entry
-points with seeded random and edge-case sizes, never far enough to launch. CPU only: skipped where a GPU is present."""
+"""The host code of the operators on rows and of the 8-bit products under AddressSanitizer and UBSan: all sources are
+rebuilt with the sanitizers on the host side (-Xarch_host; the device code as usual), and tests/host_fuzz_rows.cpp calls
+their entry points with seeded random and edge-case sizes, never far enough to launch. CPU only: skipped where a GPU is
+present."""
 from __future__ import annotations
 
 import concurrent.futures

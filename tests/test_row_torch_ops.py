@@ -1,5 +1,5 @@
-"""Quantised and permuted expert layers through torch: shapes on fake tensors here; gradients, opcheck, compilation and the
-whole layer on the GPU."""
+"""Quantised and permuted expert layers through torch: shapes on fake tensors here; gradients, opcheck, compilation and
+the whole layer on the GPU."""
 from __future__ import annotations
 
 import importlib
