@@ -67,11 +67,13 @@ __device__ __forceinline__ void rank_slots_of(const int32_t* ids, int count, int
             same &= bit ? m : ~m;
         }
         const int before = __popcll(same & below);
-        if (valid) {
-            k.rank[i] = counts[wave * B + k.bucket[i]] + before;
-            // the bucket's first lane advances the count; every lane's read above is issued first
-            if (before == 0) counts[wave * B + k.bucket[i]] += __popcll(same);
-        }
+        int* const count_of = counts + wave * B + (valid ? k.bucket[i] : 0);
+        const int had = *count_of;
+        k.rank[i] = had + before;
+        // the bucket's first lane advances the count, when every lane has read it and before any reads it again
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (valid && before == 0) *count_of = had + __popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     __syncthreads();
     for (int b = tid; b < B; b += kSortThreads) {

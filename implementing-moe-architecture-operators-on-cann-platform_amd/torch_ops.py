@@ -371,6 +371,7 @@ moe_permute.register_autograd(_permute_backward, setup_context=_permute_setup)
 
 @torch.library.custom_op(f"{NAMESPACE}::MoeUnpermute", mutates_args=(), device_types="cuda")
 def moe_unpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """Any positions; its gradient is that of MoePermute's, where each row has one pick."""
     return ops.MoeUnpermute(rows, position, weights)
 
 
