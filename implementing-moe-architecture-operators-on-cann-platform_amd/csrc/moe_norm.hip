@@ -11,7 +11,7 @@
 // waves through LDS, in a fixed order.
 //   T = 16381, H = 2048 bf16, x + residual -> sum, y, q  58.6 us, 5.15 TB/s (a copy of 1 GB: 5.13)
 //   98304 rows of 1408 bf16 -> q                         72.3 us, 5.75 TB/s
-//   gradient of T = 8192, H = 2048 fp16 with grad_sum    29.7 us, 4.5 TB/s, and 5.1 for the workgroups' column sums
+//   gradient of T = 8192, H = 2048 fp16 with grad_sum    29.7 us, 4.5 TB/s, and 4.4 for the workgroups' column sums
 //   T = 1, H = 7168                                      4.3 us, a row's latency: of a call of 8.6
 #include "moe_ops.h"
 #include "moe_rows.h"
@@ -179,9 +179,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void norm_kernel(
     }
 }
 
-// The gradient. A workgroup walks rows, at least 4 waves' worth at a time, and keeps its share of grad_gamma's column
-// sums in registers; they leave as one row of `part` for each workgroup.
-constexpr int grad_threads(int waves) { return waves <= 4 ? 256 : waves * kWave; }
+// The gradient. A workgroup walks rows, at least 8 waves' worth at a time, and keeps its share of grad_gamma's column
+// sums in registers; they leave as one row of `part` for each workgroup. us of both launches with 4, 8 and 16 waves a
+// workgroup: T = 8192, H = 2048 30.8, 30.4, 33.7; T = 16384, H = 512 19.4, 17.6, 19.3; T = 4096, H = 4096 30.7, 29.8,
+// 32.7 (fewer rows of `part`, but more waves wait for each other)
+constexpr int kGradWaves = 8;
+constexpr int grad_waves(int H) {  // of a row, two steps each
+    return H <= 1024 ? 1 : H <= 2048 ? 2 : H <= 4096 ? 4 : H <= 8192 ? 8 : 16;
+}
+constexpr int grad_threads(int waves) { return (waves < kGradWaves ? kGradWaves : waves) * kWave; }
 template <typename T, typename G, int WAVES, int STEPS, int V>
 __global__ __launch_bounds__(grad_threads(WAVES)) void norm_grad_kernel(NormArgs n) {
     using Bits = typename T::Bits;
@@ -271,13 +277,13 @@ __global__ __launch_bounds__(grad_threads(WAVES)) void norm_grad_kernel(NormArgs
         if (at[c].live) store_row<F32, V>(out + at[c].at, gg[c]);
 }
 
-// grad_gamma: the workgroups' rows, 16 columns a workgroup; 64 groups add every 64th row, 8 of them 8 groups' sums, and
-// one those
-constexpr int kSumThreads = 1024;
+// grad_gamma: the workgroups' rows, 32 columns a workgroup (whole lines; 16 columns took 1 to 2 us more); 32 groups add
+// every 32nd row, 8 of them 4 groups' sums, and one those
+constexpr int kSumThreads = 1024, kSumCols = 32;
 template <typename G>
 __global__ __launch_bounds__(kSumThreads) void gamma_sum_kernel(const float* __restrict__ part,
                                                                 typename G::Bits* __restrict__ out, int H, int rows) {
-    constexpr int kCols = 16, kGroups = kSumThreads / kCols, kFirst = 8;
+    constexpr int kCols = kSumCols, kGroups = kSumThreads / kCols, kFirst = 8;
     __shared__ float sums[kGroups][kCols], eighths[kFirst][kCols];
     const int i = static_cast<int>(threadIdx.x) % kCols, q = static_cast<int>(threadIdx.x) / kCols;
     const int col = static_cast<int>(blockIdx.x) * kCols + i;
@@ -355,11 +361,13 @@ template <typename T, typename G>
 hipError_t run_norm_grad_any(const NormArgs& n, int blocks, hipStream_t stream) {
     if (n.H < 8) return run_norm_grad<T, G, 1, 1, 1>(n, blocks, stream);
     if (n.H <= 512) return run_norm_grad<T, G, 1, 1>(n, blocks, stream);
-    if (n.H <= 1024) return run_norm_grad<T, G, 1, 2>(n, blocks, stream);
-    if (n.H <= 2048) return run_norm_grad<T, G, 2, 2>(n, blocks, stream);
-    if (n.H <= 4096) return run_norm_grad<T, G, 4, 2>(n, blocks, stream);
-    if (n.H <= 8192) return run_norm_grad<T, G, 8, 2>(n, blocks, stream);
-    return run_norm_grad<T, G, 16, 2>(n, blocks, stream);
+    switch (grad_waves(n.H)) {
+        case 1: return run_norm_grad<T, G, 1, 2>(n, blocks, stream);
+        case 2: return run_norm_grad<T, G, 2, 2>(n, blocks, stream);
+        case 4: return run_norm_grad<T, G, 4, 2>(n, blocks, stream);
+        case 8: return run_norm_grad<T, G, 8, 2>(n, blocks, stream);
+        default: return run_norm_grad<T, G, 16, 2>(n, blocks, stream);
+    }
 }
 
 // f(row type, gamma type) for the types of a call
@@ -381,11 +389,13 @@ hipError_t launch_norm(const NormArgs& n, int type, bool norm, hipStream_t strea
     });
 }
 
-// Workgroups of the gradient, 16 waves on every CU at most. T = 8192, H = 2048, us of both launches: 2 waves a row and
-// 1024 workgroups 31.5, 512 34.0; 1 wave (four steps) 33.1 with 512; 4 waves (one step) 33.5 with 1024
+// Workgroups of the gradient, 16 waves on every CU at most. T = 8192, H = 2048, us of both launches with workgroups of 4
+// waves: 2 waves a row and 1024 workgroups 31.5, 512 34.0; 1 wave (four steps) 33.1 with 512; 4 waves (one step) 33.5
+// with 1024
 int norm_grad_blocks(int64_t rows, int H) {
-    const int64_t most = H <= 2048 ? 1024 : H <= 8192 ? 512 : 256;
-    const int64_t blocks = H <= 1024 ? (rows + 3) / 4 : H <= 2048 ? (rows + 1) / 2 : rows;
+    const int waves = grad_waves(H);
+    const int64_t each = waves < kGradWaves ? kGradWaves / waves : 1, most = waves <= kGradWaves ? 512 : 256;
+    const int64_t blocks = (rows + each - 1) / each;
     return static_cast<int>(blocks < 1 ? 1 : blocks < most ? blocks : most);
 }
 
@@ -400,7 +410,7 @@ hipError_t launch_norm_grad(const NormArgs& n, int type, void* grad_gamma, hipSt
     }
     if (err != hipSuccess || !grad_gamma) return err;
     TraceScope trace("moe_norm_gamma", stream);
-    const int grid = (n.H + 15) / 16;
+    const int grid = (n.H + kSumCols - 1) / kSumCols;
     return by_type(type, n.gamma_f32, [&](auto, auto g) {
         using G = decltype(g);
         gamma_sum_kernel<G><<<grid, kSumThreads, 0, stream>>>(n.part, static_cast<typename G::Bits*>(grad_gamma), n.H,
