@@ -241,3 +241,20 @@ def test_layer_refusals(ops):
         ops.moe_layer_int8(x, gamma, w_gate, gq[:3], gs, dq, ds, res)
     with pytest.raises(ops.MoeError):
         ops.moe_layer_int8(x, gamma, w_gate, gq, gs[:3], dq, ds, res)
+
+
+@gpu
+@pytest.mark.parametrize("T,H,E,I,K", [(0, 64, 4, 32, 2), (1, 64, 1, 16, 1), (7, 100, 4, 33, 2), (300, 257, 8, 129, 3)])
+def test_layer_of_odd_sizes_on_another_stream(ops, T, H, E, I, K):
+    """Rows on odd addresses; a layer without a residual is the one with a residual of zeros."""
+    x, _, gamma, w_gate, gate_up, down = (t.cuda() for t in layer_inputs(T, H, E, I, BF16))
+    wide = torch.empty((T, H + 8), dtype=BF16, device="cuda")
+    wide[:, 3:H + 3] = x
+    (gq, gs), (dq, ds) = ops.MoeQuantize(gate_up), ops.MoeQuantize(down)
+    y, v, ids, w = ops.moe_layer_int8(x, gamma, w_gate, gq, gs, dq, ds, None, K)
+    assert v is None and y.shape == (T, H) and ids.shape == w.shape == (T, K) and y.isfinite().all()
+    zeros, side = torch.zeros_like(x), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    other = ops.moe_layer_int8(wide[:, 3:H + 3], gamma, w_gate, gq, gs, dq, ds, zeros, K, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(y, other[0]) and torch.equal(other[1], x) and torch.equal(ids, other[2])
