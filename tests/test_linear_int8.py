@@ -198,6 +198,24 @@ def test_one_expert_is_the_product_alone(ops):
 
 
 @gpu
+@pytest.mark.parametrize("act", ("none", "swiglu"))
+@pytest.mark.parametrize("out", (F16, BF16, F32))
+def test_results_do_not_depend_on_the_launch(ops, act, out):
+    """Rows of a large product without bias and residual, from tiles of 256 rows, and the same rows alone: streamed, from
+    smaller tiles, split over H, and as an expert's."""
+    T, N, H = 9000, 2048, 2048
+    o = on_gpu(operands(T, 2 * N if act == "swiglu" else N, H, 0, out, 8, False, False, N))
+    full = call(ops, o, None, act, out)
+    for rows in (1, 20, 64, 100, 300, 1500):
+        some = dict(o, x=o["x"][:rows], xs=o["xs"][:rows])
+        assert torch.equal(call(ops, some, None, act, out), full[:rows]), rows
+        for E in (1, 8):  # of 8 experts the third has all rows
+            offsets = torch.tensor([0] * (1 + E // 4) + [rows] * (E - E // 4), dtype=torch.int32).cuda()
+            many = dict(some, w=o["w"][None].expand(E, -1, -1).contiguous(), ws=o["ws"][None].expand(E, -1).contiguous())
+            assert torch.equal(call(ops, many, offsets, act, out), full[:rows]), (rows, E)
+
+
+@gpu
 @pytest.mark.parametrize("T,E", [(30, 4), (200, 4), (1200, 4)])
 def test_offsets_that_lie_stay_within_the_tensors(ops, T, E):
     """Offsets that fall, pass the end or are negative: guards before and after the result keep their values."""
