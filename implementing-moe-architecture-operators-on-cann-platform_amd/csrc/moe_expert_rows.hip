@@ -343,7 +343,7 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
     __shared__ float part[kUnsortThreads / kWave][kBatch];
     const int tid = static_cast<int>(threadIdx.x), lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), team = wave / WAVES;
-    const int first = tid % (WAVES * kWave) * V;
+    const int first = wave % WAVES * kWave * V;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTokens; base < a.T;
          base += static_cast<int64_t>(gridDim.x) * kTokens) {
         const bool token = base + team < a.T;
@@ -364,8 +364,9 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
             }
             const uint64_t lives = __ballot(live);
             float dot[kBatch] = {};
+            // a wave's lanes go through this together, since readlane is for active ones
             for (int c = first; c < a.H; c += WAVES * kWave * V) {
-                const Step<V> s = step_at<V>(c, a.H);
+                const Step<V> s = step_repeating<V>(c + lane * V, a.H);
                 RawRow<T, V> d, v[kBatch];
                 d.load(gy + s.at);
                 if (a.weights) {

@@ -31,6 +31,12 @@ __device__ __forceinline__ Step<V> step_at(int col, int H) {
     const int at = min(col, H - V);
     return Step<V>{live ? at : 0, live ? col - at : V, live};
 }
+// The same for lanes that all read and write: those past the row repeat its last values
+template <int V>
+__device__ __forceinline__ Step<V> step_repeating(int col, int H) {
+    const int at = min(col, H - V);
+    return Step<V>{at, min(col - at, V), true};
+}
 
 // V values as they are stored
 template <typename T, int V>

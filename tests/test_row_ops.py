@@ -372,6 +372,63 @@ def test_offsets_past_32_bits(ops):
     assert torch.equal(back[-4:], torch.where(at[:, None] >= 0, x[-4:], 0)) and torch.equal(back[2], rows[position[2, 0].item()])
 
 
+@gpu
+@pytest.mark.parametrize("T,H,K,dtype", [(6000, 2049, 6, F16), (9000, 1003, 8, BF16), (3001, 2051, 6, F32)])
+def test_unpermute_gradient_of_rows_past_the_caches(ops, T, H, K, dtype):
+    """Rows of more than 128 MB, which are read and written past the caches, with picks of no expert."""
+    E = 16
+    ids = torch.randint(-1, E, (T, K), generator=gen(1), dtype=torch.int32).cuda()
+    gy, w = normal((T, H), dtype, 2).cuda(), normal((T, K), F32, 3).cuda()
+    _, _, position, _ = ops.MoePermute(gy, ids, E)
+    g = torch.Generator("cuda").manual_seed(4)
+    rows = torch.randn((T * K, H), generator=g, device="cuda", dtype=F32).to(dtype)
+    grad_rows, grad_w = ops.MoeUnpermuteGrad(gy, rows, position, w)
+    only, none = ops.MoeUnpermuteGrad(gy, None, position)
+    assert none is None
+    live, at = position >= 0, torch.where(position >= 0, position, -1 - position).long()
+    assert torch.equal(at.flatten().sort()[0], torch.arange(T * K, device="cuda"))  # every row is compared
+    for k in range(K):
+        on, d = live[:, k, None], gy.double()
+        assert torch.equal(only[at[:, k]], torch.where(on, gy, 0)), k
+        want = torch.where(on, w[:, k, None].double() * d, 0.0)
+        off = (grad_rows[at[:, k]].double() - want).abs()
+        assert (off <= half_step(want, dtype) * (1 + U32) + want.abs() * U32).all(), k
+        products = torch.where(on, rows[at[:, k]].double() * d, 0.0)
+        off = (grad_w[:, k].double() - products.sum(dim=1)).abs()
+        assert (off <= products.abs().sum(dim=1) * (H + 2) * U32).all(), k
+
+
+@gpu
+def test_gradients_past_32_bits(ops):
+    """Rows whose elements lie past 2^31, in both gradients: the last tokens'."""
+    T, H = 70000, 32768
+    gy = torch.empty((T, H), dtype=F16, device="cuda")
+    gy[-4:] = normal((4, H), F16, 1).cuda()
+    rows = torch.empty_like(gy)
+    ids = (torch.arange(T, dtype=torch.int32) * 7 % 3 - 1).view(T, 1).cuda()
+    position = ops.MoePermute(gy[:, :8].contiguous(), ids, 2)[2]
+    at, on = position[-4:, 0].long(), position[-4:] >= 0
+    at = torch.where(at >= 0, at, -1 - at)
+    rows[at] = normal((4, H), F16, 2).cuda()
+    w = normal((T, 1), F32, 3).cuda()
+    grad_rows, grad_w = ops.MoeUnpermuteGrad(gy, rows, position, w)
+    want = torch.where(on, w[-4:].double() * gy[-4:].double(), 0.0)
+    assert ((grad_rows[at].double() - want).abs() <= half_step(want, F16) * (1 + U32) + want.abs() * U32).all()
+    products = torch.where(on, rows[at].double() * gy[-4:].double(), 0.0)
+    assert ((grad_w[-4:, 0].double() - products.sum(dim=1)).abs() <= products.abs().sum(dim=1) * (H + 2) * U32).all()
+    del gy, rows, grad_rows
+    T, H = 140000, 16384
+    v, grad_y = torch.ones((T, H), dtype=F16, device="cuda"), torch.zeros((T, H), dtype=F16, device="cuda")
+    v[-4:], grad_y[-4:] = normal((4, H), F16, 4).cuda(), normal((4, H), F16, 5).cuda()
+    gamma = normal((H,), F32, 6).cuda()
+    gx, gg = ops.MoeAddRmsNormGrad(grad_y, v, gamma, grad_y, EPS)
+    tail, dtail = v[-4:].contiguous(), grad_y[-4:].contiguous()
+    assert torch.equal(gx[-4:], ops.MoeAddRmsNormGrad(dtail, tail, gamma, dtail, EPS)[0])
+    assert (gx[:8] == 0).all()
+    terms = dtail.double() * norm_reference(tail, gamma, None)[1] * tail.double()  # the other rows add zeros
+    assert ((gg.double() - terms.sum(dim=0)).abs() <= terms.abs().sum(dim=0) * (4 + 8) * U32).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # refusals, on the CPU: every check runs before anything is launched
 # ---------------------------------------------------------------------------------------------------------------------
