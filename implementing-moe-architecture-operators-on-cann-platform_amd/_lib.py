@@ -107,6 +107,8 @@ SIGNATURES = {
     "moe_permute": (_I32, [_P, _I64, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64, _I64, _I64, _I32, _P]),
     "moe_unpermute": (_I32, [_P, _I64, _P, _P, _I32, _P, _I64, _I64, _I64, _I32, _P]),
     "moe_unpermute_grad": (_I32, [_P, _I64, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _I32, _P]),
+    "moe_unpermute_grad_any_workspace_bytes": (C.c_size_t, [_I64, _I64]),
+    "moe_unpermute_grad_any": (_I32, [_P, _I64, _P, _P, _P, _I32, _P, _P, _P, C.c_size_t, _I64, _I64, _I64, _I32, _P]),
     "moe_linear_int8_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64, _I64, _I32]),
     "moe_linear_int8": (_I32, [_P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, C.c_size_t, _I64, _I64, _I64, _I64,
                                _I32, _I32, _P]),

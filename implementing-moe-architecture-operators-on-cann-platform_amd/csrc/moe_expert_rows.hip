@@ -6,6 +6,8 @@
 //   back       y[t] = sum_k weights[t, k] rows[position[t, k]], fp32 sums in ascending k
 //   gradients  of rows: weights[t, k] grad_y[t] at position[t, k] (zeros for a pick of no expert); of weights[t, k]:
 //              <grad_y[t], rows[position[t, k]]>; the gradient of MoePermute is the way back without weights
+//   any        positions: a row has the sum over the picks that name it, in ascending order, so every row's picks are
+//              found first (lists by atomic exchange, whose order decides nothing)
 // Memory bounds all three: a token's row is read once and its K copies are written, or the other way round; a wave
 // works on one token, so its picks' places and weights are read once and stand in scalar registers. No atomics: a
 // pick's place is offsets[expert] + the expert's picks in earlier chunks + its rank in its chunk.
@@ -334,9 +336,92 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_kernel(UnsortArgs a) {
     }
 }
 
+// Lists of the picks that name a row: heads[row], then links[pick]; -1 ends one
+__global__ __launch_bounds__(kUnsortThreads) void unsort_heads_kernel(UnsortArgs a) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kUnsortThreads + threadIdx.x; i < a.R;
+         i += static_cast<int64_t>(gridDim.x) * kUnsortThreads)
+        a.heads[i] = -1;
+}
+__global__ __launch_bounds__(kUnsortThreads) void unsort_links_kernel(UnsortArgs a) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kUnsortThreads + threadIdx.x; i < a.T * a.K;
+         i += static_cast<int64_t>(gridDim.x) * kUnsortThreads) {
+        const int p = a.position[i];
+        if (p >= 0 && p < a.R) a.links[i] = atomicExch(a.heads + p, static_cast<int>(i));
+    }
+}
+
+// The gradient's rows that not exactly one pick names: zeros, or the picks' sum in ascending order. A wave looks at 8
+// rows. It takes up to 64 picks from a row's list and ranks them; for a row of more, which at most every 64th can be, it
+// reads all positions again.
+template <typename T, int V>
+__global__ __launch_bounds__(kUnsortThreads) void unsort_rest_kernel(UnsortArgs a) {
+    using Bits = typename T::Bits;
+    constexpr int kRows = 8, kBatch = 8, kWaves = kUnsortThreads / kWave;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int64_t picks = a.T * a.K;
+    for (int64_t base = (static_cast<int64_t>(blockIdx.x) * kWaves + wave) * kRows; base < a.R;
+         base += static_cast<int64_t>(gridDim.x) * kWaves * kRows) {
+        int head = -1;
+        bool open = false;
+        if (lane < kRows && base + lane < a.R) {
+            head = a.heads[base + lane];
+            open = head < 0 || a.links[head] >= 0;
+        }
+        for (uint64_t left = __ballot(open); left != 0; left &= left - 1) {
+            const int64_t row = base + __builtin_ctzll(left);
+            int pick = __builtin_amdgcn_readlane(head, __builtin_ctzll(left)), mine = 0, n = 0;
+            for (; pick >= 0 && n < kWave; ++n) {
+                mine = lane == n ? pick : mine;
+                pick = __builtin_amdgcn_readfirstlane(a.links[pick]);
+            }
+            const bool more = pick >= 0;
+            int rank = 0;  // of this lane's pick; lanes without one take the places behind
+            for (int i = 0; i < n; ++i) rank += __builtin_amdgcn_readlane(mine, i) < mine;
+            mine = __builtin_amdgcn_ds_permute((lane < n ? rank : lane) * 4, mine);
+            for (int c = 0; c < a.H; c += kWave * V) {
+                const Step<V> s = step_repeating<V>(c + lane * V, a.H);
+                float y[V] = {};
+                // adds the picks of `bits` from the lowest on, 8 loads at a time
+                auto add = [&](uint64_t bits, auto&& pick_of) __attribute__((always_inline)) {
+                    while (bits != 0) {
+                        int64_t at[kBatch];
+                        float w[kBatch];
+                        RawRow<T, V> d[kBatch];
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) {
+                            at[u] = bits != 0 ? pick_of(__builtin_ctzll(bits)) : -1;
+                            bits &= bits - 1;
+                            if (at[u] < 0) continue;
+                            d[u].load(static_cast<const Bits*>(a.grad_y) + at[u] / a.K * a.ldy + s.at);
+                            w[u] = a.weights ? load_weight(a.weights, at[u], a.weights_type) : 1.0f;
+                        }
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) {
+                            if (at[u] < 0) continue;
+#pragma unroll
+                            for (int j = 0; j < V; ++j) y[j] += w[u] * d[u].get(j);
+                        }
+                    }
+                };
+                if (more) {
+                    for (int64_t from = 0; from < picks; from += kWave) {
+                        const int p = from + lane < picks ? a.position[from + lane] : -1;
+                        add(__ballot(p == row), [&](int bit) { return from + bit; });
+                    }
+                } else if (n > 0) {
+                    add(~uint64_t{0} >> (kWave - n),
+                        [&](int bit) { return static_cast<int64_t>(__builtin_amdgcn_readlane(mine, bit)); });
+                }
+                store_row<T, V>(static_cast<Bits*>(a.y) + row * a.H + s.at, y);
+            }
+        }
+    }
+}
+
 // 1, 2 or 4 waves a token, 8 of its rows at a time; the picks' places and weights are read once, a pick a lane. The dot
-// products are added over the lanes and then over the waves in a fixed order.
-template <typename T, int WAVES, int V, bool NT>
+// products are added over the lanes and then over the waves in a fixed order. ANY: positions that are not MoePermute's;
+// the rows that not exactly one pick names are unsort_rest_kernel's.
+template <typename T, int WAVES, int V, bool NT, bool ANY>
 __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs a) {
     using Bits = typename T::Bits;
     constexpr int kBatch = 8, kTokens = kUnsortThreads / (WAVES * kWave);
@@ -352,7 +437,7 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
         for (int k0 = 0; k0 < a.K; k0 += kBatch) {
             // of pick k0 + lane: its row (past the rows: none, nothing is read or written), whether an expert has it
             int row = -1;
-            bool live = false;
+            bool live = false, sole = true;
             float w = 0.0f;
             if (token && lane < kBatch && k0 + lane < a.K) {
                 const int64_t at = t * a.K + k0 + lane;
@@ -360,9 +445,10 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
                 row = p >= 0 ? p : ~p;
                 if (row >= a.R) row = -1;
                 live = p >= 0 && row >= 0;
+                if (ANY) sole = live && a.heads[row] == at && a.links[at] < 0;
                 if (live) w = a.weights ? load_weight(a.weights, at, a.weights_type) : 1.0f;
             }
-            const uint64_t lives = __ballot(live);
+            const uint64_t lives = __ballot(live), soles = __ballot(sole);
             float dot[kBatch] = {};
             // a wave's lanes go through this together, since readlane is for active ones
             for (int c = first; c < a.H; c += WAVES * kWave * V) {
@@ -380,8 +466,8 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
                     const int to = __builtin_amdgcn_readlane(row, u);
-                    if (to < 0) continue;
                     const bool on = lives >> u & 1;
+                    if (ANY ? !on : to < 0) continue;
                     const float weight = of_lane(w, u);
                     float g[V];
 #pragma unroll
@@ -390,7 +476,8 @@ __global__ __launch_bounds__(kUnsortThreads) void unsort_grad_kernel(UnsortArgs 
 #pragma unroll
                         for (int j = 0; j < V; ++j) dot[u] += j >= s.skip ? d.get(j) * v[u].get(j) : 0.0f;
                     }
-                    store_row<T, V, NT>(static_cast<Bits*>(a.y) + static_cast<int64_t>(to) * a.H + s.at, g);
+                    if (!ANY || soles >> u & 1)
+                        store_row<T, V, NT>(static_cast<Bits*>(a.y) + static_cast<int64_t>(to) * a.H + s.at, g);
                 }
             }
             if (!a.weights) continue;
@@ -437,10 +524,18 @@ void run_unsort_grad(const UnsortArgs& u, hipStream_t stream) {
     constexpr int kTokens = kUnsortThreads / (WAVES * kWave);
     const int64_t blocks = (u.T + kTokens - 1) / kTokens;
     const unsigned grid = static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
-    if (u.R * u.H * static_cast<int64_t>(sizeof(typename T::Bits)) > kStreamBytes)
-        unsort_grad_kernel<T, WAVES, V, true><<<grid, kUnsortThreads, 0, stream>>>(u);
-    else
-        unsort_grad_kernel<T, WAVES, V, false><<<grid, kUnsortThreads, 0, stream>>>(u);
+    const bool nt = u.R * u.H * static_cast<int64_t>(sizeof(typename T::Bits)) > kStreamBytes;
+    if (u.heads) {
+        if (nt) unsort_grad_kernel<T, WAVES, V, true, true><<<grid, kUnsortThreads, 0, stream>>>(u);
+        else unsort_grad_kernel<T, WAVES, V, false, true><<<grid, kUnsortThreads, 0, stream>>>(u);
+    } else {
+        if (nt) unsort_grad_kernel<T, WAVES, V, true, false><<<grid, kUnsortThreads, 0, stream>>>(u);
+        else unsort_grad_kernel<T, WAVES, V, false, false><<<grid, kUnsortThreads, 0, stream>>>(u);
+    }
+}
+unsigned threads_grid(int64_t items, int each) {
+    const int64_t blocks = (items + each - 1) / each;
+    return static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
 }
 // A wave a token once that gives every SIMD two of them, or where it has a token's row in one step
 template <typename T>
@@ -449,6 +544,10 @@ void run_unsort_grad_any(const UnsortArgs& u, hipStream_t stream) {
     else if (u.T >= 2048 || u.H <= 512) run_unsort_grad<T, 1, 8>(u, stream);
     else if (u.H <= 1024) run_unsort_grad<T, 2, 8>(u, stream);
     else run_unsort_grad<T, 4, 8>(u, stream);
+    if (!u.heads) return;
+    const unsigned grid = threads_grid(u.R, kUnsortThreads / kWave * 8);
+    if (u.H < 8) unsort_rest_kernel<T, 1><<<grid, kUnsortThreads, 0, stream>>>(u);
+    else unsort_rest_kernel<T, 8><<<grid, kUnsortThreads, 0, stream>>>(u);
 }
 
 }  // namespace
@@ -499,6 +598,10 @@ hipError_t launch_unsort(const UnsortArgs& u, hipStream_t stream) {
 
 hipError_t launch_unsort_grad(const UnsortArgs& u, hipStream_t stream) {
     TraceScope trace("moe_unsort_grad", stream);
+    if (u.heads) {
+        unsort_heads_kernel<<<threads_grid(u.R, kUnsortThreads), kUnsortThreads, 0, stream>>>(u);
+        unsort_links_kernel<<<threads_grid(u.T * u.K, kUnsortThreads), kUnsortThreads, 0, stream>>>(u);
+    }
     if (u.type == MOE_DT_FLOAT32) run_unsort_grad_any<F32>(u, stream);
     else if (u.type == MOE_DT_FLOAT16) run_unsort_grad_any<Half>(u, stream);
     else run_unsort_grad_any<Bf16>(u, stream);

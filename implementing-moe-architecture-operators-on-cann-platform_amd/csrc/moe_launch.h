@@ -262,6 +262,8 @@ struct UnsortArgs {
     const void* grad_y;       // gradient: [T, H], rows ldy elements apart
     void* y;                  // [T, H]; gradient: grad_rows [R, H]
     void* grad_weights;       // gradient: [T, K] of weights_type, null without weights
+    int32_t* heads;           // gradient of any positions: [R] and [T, K], each row's list of picks; null: MoePermute's
+    int32_t* links;
     int64_t T, R, ldy;
     int H, K;
     int type, weights_type;  // moe_dtype

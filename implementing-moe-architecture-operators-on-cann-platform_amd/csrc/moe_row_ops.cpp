@@ -70,6 +70,45 @@ moe_status check_permute(const char* op, int64_t T, int64_t E, int64_t K) {
     return check_picks(op, T, K);
 }
 
+// moe_unpermute_grad and, with `any`, moe_unpermute_grad_any
+moe_status unpermute_grad(const void* grad_y, int64_t grad_y_stride, const void* rows, const int32_t* position,
+                          const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights, bool any,
+                          void* workspace, size_t workspace_bytes, int64_t T, int64_t H, int64_t K, int32_t dtype,
+                          void* stream) {
+    const char* op = "MoeUnpermuteGrad";
+    moe_status st = check_rows(op, T, H, dtype);
+    if (st == MOE_OK) st = check_picks(op, T, K);
+    if (st == MOE_OK) st = check_stride(op, "grad_y", T, H, grad_y_stride);
+    if (st != MOE_OK) return st;
+    if (weights && !is_float(weights_type)) return fail(MOE_ERR_ARG, "%s: weights type %d", op, weights_type);
+    if (T == 0) return ok();
+    if (!grad_y || !position || !grad_rows || (weights && (!rows || !grad_weights)))
+        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
+    if (any) st = check_words(op, workspace, workspace_bytes, static_cast<size_t>(T) * K * 2 * sizeof(int32_t));
+    if (st != MOE_OK) return st;
+    moe::UnsortArgs u{};
+    u.rows = rows;
+    u.R = T * K;
+    u.position = position;
+    u.weights = weights;
+    u.weights_type = weights_type;
+    u.grad_y = grad_y;
+    u.ldy = grad_y_stride;
+    u.y = grad_rows;
+    u.grad_weights = grad_weights;
+    if (any) {
+        u.heads = static_cast<int32_t*>(workspace);
+        u.links = u.heads + T * K;
+    }
+    u.T = T;
+    u.H = static_cast<int>(H);
+    u.K = static_cast<int>(K);
+    u.type = dtype;
+    const hipError_t err = moe::launch_unsort_grad(u, as_stream(stream));
+    if (err != hipSuccess) return hip_fail(err, "MoeUnpermuteGrad launch");
+    return ok();
+}
+
 }  // namespace
 
 extern "C" {
@@ -234,32 +273,22 @@ moe_status moe_unpermute(const void* rows, int64_t num_rows, const int32_t* posi
 moe_status moe_unpermute_grad(const void* grad_y, int64_t grad_y_stride, const void* rows, const int32_t* position,
                               const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights,
                               int64_t T, int64_t H, int64_t K, int32_t dtype, void* stream) {
-    const char* op = "MoeUnpermuteGrad";
-    moe_status st = check_rows(op, T, H, dtype);
-    if (st == MOE_OK) st = check_picks(op, T, K);
-    if (st == MOE_OK) st = check_stride(op, "grad_y", T, H, grad_y_stride);
-    if (st != MOE_OK) return st;
-    if (weights && !is_float(weights_type)) return fail(MOE_ERR_ARG, "%s: weights type %d", op, weights_type);
-    if (T == 0) return ok();
-    if (!grad_y || !position || !grad_rows || (weights && (!rows || !grad_weights)))
-        return fail(MOE_ERR_NULL, "%s: null tensor pointer", op);
-    moe::UnsortArgs u{};
-    u.rows = rows;
-    u.R = T * K;
-    u.position = position;
-    u.weights = weights;
-    u.weights_type = weights_type;
-    u.grad_y = grad_y;
-    u.ldy = grad_y_stride;
-    u.y = grad_rows;
-    u.grad_weights = grad_weights;
-    u.T = T;
-    u.H = static_cast<int>(H);
-    u.K = static_cast<int>(K);
-    u.type = dtype;
-    const hipError_t err = moe::launch_unsort_grad(u, as_stream(stream));
-    if (err != hipSuccess) return hip_fail(err, "MoeUnpermuteGrad launch");
-    return ok();
+    return unpermute_grad(grad_y, grad_y_stride, rows, position, weights, weights_type, grad_rows, grad_weights, false,
+                          nullptr, 0, T, H, K, dtype, stream);
+}
+
+size_t moe_unpermute_grad_any_workspace_bytes(int64_t T, int64_t K) {
+    if (check_rows("MoeUnpermuteGrad", T, 1, MOE_DT_FLOAT32) != MOE_OK || check_picks("MoeUnpermuteGrad", T, K) != MOE_OK)
+        return 0;
+    return static_cast<size_t>(T) * K * 2 * sizeof(int32_t);
+}
+
+moe_status moe_unpermute_grad_any(const void* grad_y, int64_t grad_y_stride, const void* rows, const int32_t* position,
+                                  const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights,
+                                  void* workspace, size_t workspace_bytes, int64_t T, int64_t H, int64_t K,
+                                  int32_t dtype, void* stream) {
+    return unpermute_grad(grad_y, grad_y_stride, rows, position, weights, weights_type, grad_rows, grad_weights, true,
+                          workspace, workspace_bytes, T, H, K, dtype, stream);
 }
 
 }  // extern "C"

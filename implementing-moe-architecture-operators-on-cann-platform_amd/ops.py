@@ -790,11 +790,20 @@ def MoeUnpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tens
     return y
 
 
+def unpermute_grad_any_workspace_bytes(T: int, K: int) -> int:
+    return int(_lib.load().moe_unpermute_grad_any_workspace_bytes(T, K))
+
+
 def MoeUnpermuteGrad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: torch.Tensor,
-                     weights: torch.Tensor | None = None, stream=None):
+                     weights: torch.Tensor | None = None, stream=None, anyPosition: bool = False,
+                     workspace: torch.Tensor | None = None):
     """The gradients of MoeUnpermute's y[T,H] -> (grad_rows[T*K,H] of grad_y's type, grad_weights[T,K] of weights'
     type). position is MoePermute's, so every row has one pick; the rows of picks of no expert get zeros. Without
-    weights rows may be None and grad_weights is None."""
+    weights rows may be None and grad_weights is None.
+
+    With anyPosition position is whatever MoeUnpermute takes: positions outside [0, T*K) have no row and weight gradient
+    0, a row that none names gets zeros and one that several name their sum (fp32, in ascending slot). `workspace`
+    (uint8, >= unpermute_grad_any_workspace_bytes) is allocated when not given; otherwise it is not used."""
     dt, dev = _first_float(grad_y, "grad_y", _FLOATS, 2)
     T, H = grad_y.shape
     _, K = _ids(position, "position", T, dev)
@@ -807,8 +816,12 @@ def MoeUnpermuteGrad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: 
     new = _allocator(like, stream)
     grad_rows = new((T * K, H), grad_y.dtype)
     grad_w = None if wp is None else new((T, K), weights.dtype)
-    check(_lib.load().moe_unpermute_grad(grad_y.data_ptr(), ldy, rp, position.data_ptr(), wp, wt, grad_rows.data_ptr(),
-                                         _ptr(grad_w), T, H, K, dt, _queue(stream, dev)))
+    lib, args = _lib.load(), (grad_y.data_ptr(), ldy, rp, position.data_ptr(), wp, wt, grad_rows.data_ptr(), _ptr(grad_w))
+    if anyPosition:
+        workspace, ap, ab = _workspace(workspace, lib.moe_unpermute_grad_any_workspace_bytes, (T, K), like, dev, stream)
+        check(lib.moe_unpermute_grad_any(*args, ap, ab, T, H, K, dt, _queue(stream, dev)))
+    else:
+        check(lib.moe_unpermute_grad(*args, T, H, K, dt, _queue(stream, dev)))
     return grad_rows, grad_w
 
 

@@ -371,7 +371,7 @@ moe_permute.register_autograd(_permute_backward, setup_context=_permute_setup)
 
 @torch.library.custom_op(f"{NAMESPACE}::MoeUnpermute", mutates_args=(), device_types="cuda")
 def moe_unpermute(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
-    """Any positions; its gradient is that of MoePermute's, where each row has one pick."""
+    """Any positions; it has a gradient where there are as many rows as picks (MoePermute's), whatever they name."""
     return ops.MoeUnpermute(rows, position, weights)
 
 
@@ -384,14 +384,15 @@ def _(rows, position, weights=None):
 
 @torch.library.custom_op(f"{NAMESPACE}::MoeUnpermuteGrad", mutates_args=(), device_types="cuda")
 def moe_unpermute_grad(grad_y: torch.Tensor, rows: torch.Tensor | None, position: torch.Tensor,
-                       weights: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                       weights: torch.Tensor | None = None,
+                       anyPosition: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """-> (grad_rows, grad_weights), the latter empty without weights."""
-    grad_rows, grad_w = ops.MoeUnpermuteGrad(grad_y, rows, position, weights)
+    grad_rows, grad_w = ops.MoeUnpermuteGrad(grad_y, rows, position, weights, anyPosition=anyPosition)
     return grad_rows, _or_empty(grad_w, grad_y)
 
 
 @moe_unpermute_grad.register_fake
-def _(grad_y, rows, position, weights=None):
+def _(grad_y, rows, position, weights=None, anyPosition=False):
     return (grad_y.new_empty((position.shape[0] * position.shape[1], grad_y.shape[1])),
             grad_y.new_empty(0) if weights is None else weights.new_empty(weights.shape))
 
@@ -407,7 +408,8 @@ def _unpermute_backward(ctx, grad_y):
     rows, position, weights = ctx.saved_tensors
     if ctx.num_rows != ctx.picks:
         raise RuntimeError("MoeUnpermute has a gradient where rows are MoePermute's, one for each pick")
-    grad_rows, grad_w = getattr(torch.ops, NAMESPACE).MoeUnpermuteGrad(grad_y.contiguous(), rows, position, weights)
+    op = getattr(torch.ops, NAMESPACE).MoeUnpermuteGrad
+    grad_rows, grad_w = op(grad_y.contiguous(), rows, position, weights, True)  # the forward takes any positions
     return grad_rows, None, None if weights is None else grad_w
 
 

@@ -422,6 +422,15 @@ moe_status moe_unpermute_grad(const void* grad_y, int64_t grad_y_stride, const v
                               const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights,
                               int64_t num_tokens, int64_t hidden_size, int64_t top_k, int32_t dtype, void* stream);
 
+/* The same for any positions, num_rows = T K: those outside [0, T K) have no row and weight gradient 0, a row that no
+ * position names gets zeros, and one that several name the sum over them (float32, in ascending t K + k). The workspace
+ * (any alignment of 4; calls in flight at the same time need one each) holds the picks of each row. */
+size_t moe_unpermute_grad_any_workspace_bytes(int64_t num_tokens, int64_t top_k);
+moe_status moe_unpermute_grad_any(const void* grad_y, int64_t grad_y_stride, const void* rows, const int32_t* position,
+                                  const void* weights, int32_t weights_type, void* grad_rows, void* grad_weights,
+                                  void* workspace, size_t workspace_bytes, int64_t num_tokens, int64_t hidden_size,
+                                  int64_t top_k, int32_t dtype, void* stream);
+
 /* ------------------------------------------------------------------------------------------------------
  * MoeLinearInt8: x[T, H] int8 with x_scale[T], weight[N, H] int8 (SwiGLU: [2N, H], N gate rows first) with
  *   weight_scale[N] (SwiGLU: [2N]) -> y[T, N] = act((x weight^T) * x_scale * weight_scale + bias) + residual of

@@ -7,7 +7,7 @@ import importlib
 import pytest
 
 from conftest import PKG_NAME
-from test_dense_ops import BF16, F16, F32, F64, gen, gpu, normal
+from test_dense_ops import BF16, F16, F32, F64, U32, check, gen, gpu, half_step, normal
 
 torch = pytest.importorskip("torch")
 tops = importlib.import_module(PKG_NAME + ".torch_ops")
@@ -108,6 +108,110 @@ def test_parts_that_need_no_gradient(ops):
     with pytest.raises(RuntimeError, match="one for each pick"):
         more = leaf(torch.zeros(200, 96))
         torch.autograd.grad(op.MoeUnpermute(more, position).sum(), more)
+
+
+def any_positions(T, K, kind):
+    """Positions that MoeUnpermute takes and MoePermute does not give."""
+    position = torch.randperm(T * K, generator=gen(T)).to(torch.int32).view(T, K)
+    u = torch.rand((T, K), generator=gen(K))
+    if kind == "masked":  # no expert's without a place, and past the rows
+        position[u < 0.2], position[u > 0.9], position[u > 0.95] = -1, T * K, 2**31 - 1
+        position[0] = -2**31
+    elif kind == "shared":
+        position = torch.where(u < 0.5, position // 3, position)
+    elif kind == "one row":
+        position[:] = T * K - 1
+    else:
+        position //= kind
+    return position
+
+
+@gpu
+@pytest.mark.parametrize("T,H,K,dtype", [(1, 1, 1, F32), (40, 7, 3, BF16), (33, 9, 8, F16), (300, 1056, 4, BF16),
+                                         (2049, 264, 3, F32), (130, 2051, 6, F16), (5000, 72, 2, F32)])
+@pytest.mark.parametrize("kind", ["masked", "shared", 2, 63, 64, 65, "one row"])
+def test_way_back_has_the_gradient_of_any_positions(ops, T, H, K, dtype, kind):
+    """Rows that no pick, one or many name, against 64-bit sums: a row's is of at most T K products in fp32."""
+    position = any_positions(T, K, kind)
+    rows, dy = normal((T * K, H), dtype, 1), normal((T, H), dtype, 2)
+    on = (position >= 0) & (position < T * K)
+    at = torch.where(on, position, 0).long()
+    for wdt in (None, F32, F16):
+        w = None if wdt is None else normal((T, K), wdt, 3)
+        args = [leaf(t) for t in (rows, w) if t is not None]
+        y = op.MoeUnpermute(args[0], position.cuda(), *args[1:])
+        got = torch.autograd.grad(y, args, dy.cuda())
+        terms = on[:, :, None] * (1.0 if w is None else w.double()[:, :, None]) * dy.double()[:, None]
+        want = torch.zeros((T * K, H), dtype=F64).index_add_(0, at.flatten(), terms.flatten(0, 1))
+        size = torch.zeros((T * K, H), dtype=F64).index_add_(0, at.flatten(), terms.abs().flatten(0, 1))
+        many = torch.bincount(at[on], minlength=T * K)[:, None]
+        check(got[0], want, half_step(want, dtype) * (1 + U32) + size * (many + 1) * U32, "rows")
+        if w is not None:
+            products = on[:, :, None] * rows.double()[at] * dy.double()[:, None]
+            ref = products.sum(dim=2)
+            check(got[1], ref, half_step(ref, wdt) * (1 + U32) + products.abs().sum(dim=2) * (H + 1) * U32, "weights")
+        y = op.MoeUnpermute(args[0], position.cuda(), *args[1:])
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, args, dy.cuda()), got))
+
+
+@gpu
+@pytest.mark.parametrize("T,H,E,K,dtype", [(45, 96, 8, 3, F32), (2100, 1031, 16, 4, BF16), (1, 5, 2, 2, F16)])
+def test_gradient_of_any_positions_is_that_of_sorted_ones(ops, T, H, E, K, dtype):
+    ids = torch.randint(-1, E, (T, K), generator=gen(1), dtype=torch.int32).cuda()
+    dy, w = normal((T, H), dtype, 2).cuda(), normal((T, K), F32, 3).cuda()
+    rows, _, position, _ = ops.MoePermute(normal((T, H), dtype, 4).cuda(), ids, E)
+    need = ops.unpermute_grad_any_workspace_bytes(T, K)
+    assert need == 8 * T * K
+    room = torch.full((need + 64,), 0x7f, dtype=torch.uint8, device="cuda")
+    for a, b in zip(ops.MoeUnpermuteGrad(dy, rows, position, w),
+                    ops.MoeUnpermuteGrad(dy, rows, position, w, anyPosition=True, workspace=room)):
+        assert torch.equal(a, b)
+    assert (room[need:] == 0x7f).all()
+    assert torch.equal(ops.MoeUnpermuteGrad(dy, None, position)[0],
+                       ops.MoeUnpermuteGrad(dy, None, position, anyPosition=True)[0])
+    with pytest.raises(ops.MoeError):
+        ops.MoeUnpermuteGrad(dy, rows, position, w, anyPosition=True, workspace=room[:need - 4])
+
+
+@gpu
+def test_gradient_of_any_positions_captured_with_changed_ones(ops):
+    """On another stream, with rows of an odd length and gradients any stride apart; every replay against an eager call."""
+    T, H, K = 700, 333, 4
+    dy, rows = normal((T, H + 5), F16, 1).cuda()[:, 2:2 + H], normal((T * K, H), F16, 2).cuda()
+    position, w = any_positions(T, K, "masked").cuda(), normal((T, K), F32, 3).cuda()
+
+    def step(stream=None):
+        return ops.MoeUnpermuteGrad(dy, rows, position, w, stream, True)
+
+    want, side = step(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = step(side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for kind in ("shared", 65, "masked", "one row"):
+        position.copy_(any_positions(T, K, kind))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), kind
+        torch.cuda.synchronize()
+
+
+def test_gradient_of_any_positions_refuses_like_the_other():
+    L, P = tops.ops._lib.load(), 1 << 20
+
+    def call(T=4, H=64, K=2, dtype=1, gy=P, rows=P, position=P, w=P, wtype=0, gr=P, gw=P, ys=64, ws=P, wb=1 << 30):
+        return L.moe_unpermute_grad_any(gy, ys, rows, position, w, wtype, gr, gw, ws, wb, T, H, K, dtype, None)
+
+    assert call(T=0, gy=None, gr=None, ws=None) == 0
+    for change, status in ((dict(T=-1), 4), (dict(K=0), 4), (dict(dtype=2), 4), (dict(wtype=2), 4), (dict(gy=None), 1),
+                           (dict(rows=None), 1), (dict(position=None), 1), (dict(gr=None), 1), (dict(gw=None), 1),
+                           (dict(ys=63), 4), (dict(T=1 << 30), 6), (dict(ws=None), 5), (dict(wb=63), 5),
+                           (dict(ws=P + 2), 6)):
+        assert call(**change) == status, (change, L.moe_last_error())
+    assert L.moe_unpermute_grad_any_workspace_bytes(4, 2) == 64
+    assert L.moe_unpermute_grad_any_workspace_bytes(-1, 2) == L.moe_unpermute_grad_any_workspace_bytes(1 << 30, 2) == 0
 
 
 @gpu
