@@ -356,14 +356,18 @@ def _(x, expert_ids, numExperts, xScale=None):
 
 def _permute_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
+    ctx.scaled = inputs[3] is not None
     ctx.save_for_backward(output[2])
 
 
-def _permute_backward(ctx, grad_rows, *_):
-    if grad_rows is None:
-        return (None,) * 4
-    grad_x = getattr(torch.ops, NAMESPACE).MoeUnpermute(grad_rows.contiguous(), ctx.saved_tensors[0], None)
-    return grad_x, None, None, None
+def _permute_backward(ctx, grad_rows, grad_offsets, grad_position, grad_scale):
+    back, (position,) = getattr(torch.ops, NAMESPACE).MoeUnpermute, ctx.saved_tensors
+    grad_x = grad_xs = None
+    if grad_rows is not None and ctx.needs_input_grad[0]:
+        grad_x = back(grad_rows.contiguous(), position, None)
+    if ctx.scaled and grad_scale is not None and ctx.needs_input_grad[3]:  # scales go the way of their rows
+        grad_xs = back(grad_scale.contiguous()[:, None], position, None)[:, 0]
+    return grad_x, None, None, grad_xs
 
 
 moe_permute.register_autograd(_permute_backward, setup_context=_permute_setup)

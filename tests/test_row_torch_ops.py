@@ -110,6 +110,31 @@ def test_parts_that_need_no_gradient(ops):
         torch.autograd.grad(op.MoeUnpermute(more, position).sum(), more)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.int8, F16, F32])
+def test_scales_sorted_with_their_rows_have_a_gradient(ops, dtype):
+    """Of a loss that takes row_scale: the sum over a token's picks, those of no expert left out (K - 1 fp32 additions)."""
+    T, H, E, K = 45, 24, 8, 3
+    ids = torch.randint(-1, E, (T, K), generator=gen(1), dtype=torch.int32)
+    x = torch.randint(-127, 128, (T, H), generator=gen(2)).to(dtype)
+    scale, d = leaf(torch.rand(T, generator=gen(3))), normal((T * K,), F32, 4)
+    X = x.cuda() if dtype == torch.int8 else leaf(x)
+    rows, _, position, row_scale = op.MoePermute(X, ids.cuda(), E, scale)
+    at = torch.where(ids >= 0, position.cpu(), 0).long()
+    terms = d.double()[at] * (ids >= 0)
+    got, = torch.autograd.grad(row_scale, scale, d.cuda(), retain_graph=True)
+    check(got, terms.sum(dim=1), terms.abs().sum(dim=1) * K * U32)
+    if dtype == torch.int8:
+        return
+    dr = normal((T * K, H), dtype, 5)
+    both = torch.autograd.grad((rows, row_scale), (X, scale), (dr.cuda(), d.cuda()), retain_graph=True)
+    assert torch.equal(both[1], got)
+    alone, = torch.autograd.grad(rows, X, dr.cuda(), retain_graph=True)
+    assert torch.equal(both[0], alone)
+    assert torch.autograd.grad(row_scale, X, d.cuda(), allow_unused=True, retain_graph=True)[0] is None
+    assert torch.autograd.grad(rows, scale, dr.cuda(), allow_unused=True)[0] is None
+
+
 def any_positions(T, K, kind):
     """Positions that MoeUnpermute takes and MoePermute does not give."""
     position = torch.randperm(T * K, generator=gen(T)).to(torch.int32).view(T, K)
