@@ -102,34 +102,47 @@ struct GroupItem {
     int expert, row0, row1;  // of the expert
     int first;               // its first item
 };
-__device__ __forceinline__ int group_offset(const GemmArgs& g, int e) {
-    return e == 0 ? 0 : min(max(g.offsets[e], 0), g.m);
-}
 __device__ __forceinline__ const uint16_t* group_q(const GemmArgs& g, int e) {
     return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(g.q) + e * g.q_expert);
 }
-// The experts' items in a wave's registers: lane l has experts l, l + 64, ... Offsets are taken within [0, m] and
-// ascending, whatever they say.
+// The experts' items in a wave's registers: lane l has experts l, l + 64, ... An expert's rows end at its offset within
+// [0, m], or where the last one's did if that is further, and begin there: whatever the offsets say, every row below
+// `rows` is one expert's and the items are as many as the grids are made for.
 constexpr int kGroupParts = 4;  // of 64 experts
 struct GroupTable {
     int row0[kGroupParts], row1[kGroupParts], end[kGroupParts];  // rows, and the items up to the expert's last
-    int total;
+    int total, rows;
 };
 __device__ __forceinline__ int group_items(int row0, int row1, int bm, int ntiles) {
     return (row1 - row0 + bm - 1) / bm * ntiles;
 }
+// v of the lane before, `first` in lane 0 (every lane active)
+__device__ __forceinline__ int lane_before(int v, int first) {
+    return __builtin_amdgcn_update_dpp(first, v, 0x138, 0xf, 0xf, false);
+}
 __device__ __forceinline__ GroupTable group_table(const GemmArgs& g, int bm, int ntiles) {
     const int lane = lane_id();
     GroupTable t;
-    t.total = 0;
+    t.total = t.rows = 0;
 #pragma unroll
     for (int s = 0; s < kGroupParts; ++s) {
-        const int e = s * kWave + lane;
-        t.row0[s] = t.row1[s] = 0;
-        if (e < g.experts) {
-            t.row0[s] = group_offset(g, e);
-            t.row1[s] = max(t.row0[s], group_offset(g, e + 1));
+        const int e = min(s * kWave + lane, g.experts - 1);  // lanes past the experts: without rows behind the last
+        t.row1[s] = s * kWave < g.experts ? min(max(g.offsets[e + 1], 0), g.m) : 0;
+    }
+#pragma unroll
+    for (int s = 0; s < kGroupParts; ++s) {
+        int row0 = t.rows, row1 = max(t.row1[s], t.rows);
+        if (s * kWave < g.experts) {
+            row0 = lane_before(row1, t.rows);
+            if (__ballot(row1 < row0) != 0) {  // they fall: the largest so far
+#pragma unroll
+                for (int d = 1; d < kWave; d <<= 1) row1 = max(row1, __shfl_up(row1, d, kWave));
+                row0 = lane_before(row1, t.rows);
+            }
+            t.rows = __builtin_amdgcn_readlane(row1, kWave - 1);
         }
+        t.row0[s] = row0;
+        t.row1[s] = row1;
     }
 #pragma unroll
     for (int s = 0; s < kGroupParts; ++s) {
@@ -172,15 +185,14 @@ __device__ __forceinline__ void group_advance(const GemmArgs& g, int bm, int nti
     while (at >= item.first + items && item.expert + 1 < g.experts) {
         item.first += items;
         ++item.expert;
-        const int o0 = offsets[item.expert], o1 = offsets[item.expert + 1];
-        item.row0 = item.expert == 0 ? 0 : min(max(o0, 0), g.m);
-        item.row1 = max(item.row0, min(max(o1, 0), g.m));
+        item.row0 = item.row1;
+        item.row1 = max(item.row0, min(offsets[item.expert + 1], g.m));
         items = group_items(item.row0, item.row1, bm, ntiles);
     }
 }
 // The rows behind the last expert's, over all workgroups
-__device__ __forceinline__ void group_zero_rows(const GemmArgs& g, int block, int blocks) {
-    const int64_t from = static_cast<int64_t>(group_offset(g, g.experts)) * g.n, to = static_cast<int64_t>(g.m) * g.n;
+__device__ __forceinline__ void group_zero_rows(const GemmArgs& g, int rows, int block, int blocks) {
+    const int64_t from = static_cast<int64_t>(rows) * g.n, to = static_cast<int64_t>(g.m) * g.n;
     for (int64_t i = from + static_cast<int64_t>(block) * blockDim.x + threadIdx.x; i < to;
          i += static_cast<int64_t>(blocks) * blockDim.x) {
         if (g.out_f32) static_cast<float*>(g.out)[i] = 0.0f;

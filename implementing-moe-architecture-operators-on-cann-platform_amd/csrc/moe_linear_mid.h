@@ -99,8 +99,8 @@ __device__ __forceinline__ void gemm_mid(const GemmArgs& all, int mtiles, int nt
     int item = block % kXcds * (grid / kXcds) + block / kXcds;
     GroupItem group{};
     if (GROUPED) {  // of the expert whose item this is, the m-tiles that read the same weights as neighbours
-        group_zero_rows(all, block, grid);
         const GroupTable table = group_table(all, BM, ntiles);
+        group_zero_rows(all, table.rows, block, grid);
         if (item >= table.total) return;
         group = group_find(table, BM, ntiles, item);
         item -= group.first;

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(WAVES * kWave) void gemm_stream_kernel(GemmArgs g, 
     if (GROUPED) {
         table = group_table(g, 16 * MB, ntiles);
         tiles = table.total;
-        group_zero_rows(g, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+        group_zero_rows(g, table.rows, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
     }
     struct Place {
         int row0, nt;  // first P row, tile of Q rows

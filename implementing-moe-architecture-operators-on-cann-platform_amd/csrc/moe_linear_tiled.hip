@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tiled_kernel(GemmArgs g, int mt
         const int first = static_cast<int>(blockIdx.x) % kXcds * ((total + kXcds - 1) / kXcds) +
                           static_cast<int>(blockIdx.x) / kXcds;
         cur.group = group_find(table, kBM, ntiles, first);
-        group_zero_rows(g, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+        group_zero_rows(g, table.rows, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
     }
     const int nloc = static_cast<int>(gridDim.x) / kXcds;
     const int x = static_cast<int>(blockIdx.x) % kXcds, li = static_cast<int>(blockIdx.x) / kXcds;

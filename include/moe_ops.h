@@ -439,13 +439,13 @@ moe_status moe_unpermute_grad_any(const void* grad_y, int64_t grad_y_stride, con
  *   num_experts > 0: weight[E, N, H] (expert_stride elements apart), weight_scale[E, N] and bias[E, N] of E matrices,
  *   and the rows [offsets[e], offsets[e + 1]) of x by the matrix of expert e, offsets[E + 1] ascending from 0 as
  *   moe_permute writes them; rows from offsets[E] on are written as zeros, residual and all. Values that do not ascend
- *   or lie outside [0, T] are taken into it: nothing outside the tensors is read or written. num_experts 0: offsets is
- *   not read. Any strides and alignment; operands on 16 bytes with H and the strides multiples of 16 run at full speed.
- *   Where H is none, products of many rows (T >= 256, with experts 32 E) first copy x and all weights with padded rows;
- *   other operands go through registers at a fraction of the speed. H <= 131071, where 32-bit sums end; N <= 2^20, E <=
- *   256. The workspace (0 where none is needed; 16-byte aligned) holds those copies and partial sums of a product split
- *   over H; calls in flight at the same time need one each. Not monotone in num_tokens. The sums are exact, so y does
- *   not depend on the launch.
+ *   or lie outside [0, T] are taken as the largest so far within it, so that every row is one expert's or zeros.
+ *   num_experts 0: offsets is not read. Any strides and alignment; operands on 16 bytes with H and the strides
+ *   multiples of 16 run at full speed. Where H is none, products of many rows (T >= 256, with experts 32 E) first copy
+ *   x and all weights with padded rows; other operands go through registers at a fraction of the speed. H <= 131071,
+ *   where 32-bit sums end; N <= 2^20, E <= 256. The workspace (0 where none is needed; 16-byte aligned) holds those
+ *   copies and partial sums of a product split over H; calls in flight at the same time need one each. Not monotone in
+ *   num_tokens. The sums are exact, so y does not depend on the launch.
  * ---------------------------------------------------------------------------------------------------- */
 size_t moe_linear_int8_workspace_bytes(int64_t num_tokens, int64_t n, int64_t hidden_size, int64_t num_experts,
                                        int32_t activation);

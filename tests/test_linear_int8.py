@@ -235,6 +235,35 @@ def test_offsets_that_lie_stay_within_the_tensors(ops, T, E):
 
 
 @gpu
+@pytest.mark.parametrize("T,E,at", [(30, 4, 0), (50, 70, 0), (200, 9, 0), (600, 130, 0), (640, 9, 0), (200, 9, 1), (1200, 9, 1),
+                                    (1500, 9, 0), (5000, 9, 0), (2000, 256, 0)])
+def test_offsets_that_lie_give_every_row_one_expert(ops, T, E, at):
+    """Streams and every height of tiles: an expert ends at its offset within [0, T] or where the last one did if that is
+    further, and begins there, so each row is as with the offsets of which that is true. at: odd addresses."""
+    N, H = 72, 64
+    o = on_gpu(operands(T, N, H, E, F32, 1, True, True, N))
+    frame = torch.zeros(T * H + 16, dtype=torch.int8, device="cuda")
+    x = frame[at:at + T * H].view(T, H)
+    x.copy_(o["x"])
+    u = torch.randint(-T, 2 * T, (E + 1,), generator=gen(E))
+    lies = {"there and back": [0] + [T * (e % 2 == 0) for e in range(E)], "falling": [T - e for e in range(E + 1)],
+            "the last below": [0] + [T // 2] * (E - 1) + [T // 3], "far": [2**31 - 1] + [-2**31, T // 2] * E, "any": u.tolist()}
+    for name, values in lies.items():
+        offsets = torch.tensor(values[:E + 1], dtype=torch.int32)
+        honest = offsets.long().clamp(0, T)
+        honest[0] = 0
+        honest = honest.cummax(0)[0].to(torch.int32)
+        y = torch.full((T, N), float("nan"), device="cuda")
+        off = offsets.cuda()
+        st = lib.load().moe_linear_int8(x.data_ptr(), H, o["xs"].data_ptr(), o["w"].data_ptr(), H, N * H, o["ws"].data_ptr(),
+                                        off.data_ptr(), o["bias"].data_ptr(), o["residual"].data_ptr(), y.data_ptr(), None, 0,
+                                        T, N, H, E, 0, 0, torch.cuda.current_stream().cuda_stream)
+        assert st == 0 and torch.equal(y, call(ops, dict(o, x=x), honest.cuda(), "none", F32)), name
+        ref, tol = reference_experts(o, honest, "none", N)
+        check(y, ref.cpu(), (tol + half_step(ref.abs() + tol, F32)).cpu(), name)
+
+
+@gpu
 def test_residual_that_is_the_result(ops):
     T, N, H = 70, 136, 256
     o = on_gpu(operands(T, N, H, 0, F16, 2, True, True, N))
