@@ -223,11 +223,14 @@ __global__ __launch_bounds__(kSingleThreads) void permute_single_kernel(const in
             same &= bit ? m : ~m;
         }
         const int before = __popcll(same & below);
-        if (valid) {
-            r[it] = wcnt[wave * E + e[it]] + before;
-            // the lane of each expert's first slot advances the count; every lane's read above is issued first
-            if (before == 0) wcnt[wave * E + e[it]] += __popcll(same);
-        }
+        int* const count = wcnt + wave * E + (valid ? e[it] : 0);
+        const int had = *count;
+        if (valid) r[it] = had + before;
+        // the lane of each expert's first slot advances the count, when every lane has read it and before any reads it
+        // again
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (valid && before == 0) *count = had + __popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     __syncthreads();
     if (wave == 0) {  // totals and their exclusive sums, 64 experts at a time
