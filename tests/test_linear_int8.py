@@ -134,6 +134,28 @@ def test_experts(ops, T, N, H, E, act):
 
 
 @gpu
+@pytest.mark.parametrize("T,N,H,act,out", [(8192, 2816, 2048, "swiglu", BF16), (8192, 2816, 2048, "swiglu", F16),
+                                           (16381, 1032, 1040, "none", F16), (9001, 2056, 528, "none", BF16),
+                                           (5000, 4104, 272, "swiglu", F16)])
+def test_large_tiles_without_bias_and_residual(ops, T, N, H, act, out):
+    """16-bit results that need scales alone, which tiles of 256 rows write by a way of their own; every value."""
+    run_case(ops, T, N, H, act, out, bias=False, residual=False, seed=T)
+
+
+@gpu
+@pytest.mark.parametrize("act", ("none", "swiglu"))
+@pytest.mark.parametrize("out", (F16, BF16))
+@pytest.mark.parametrize("T,N,H,E", [(300, 264, 96, 9), (2300, 1408, 272, 64), (1300, 520, 1040, 9), (5100, 72, 64, 33),
+                                     (1500, 264, 96, 9), (6000, 1032, 528, 4), (40000, 136, 80, 200)])
+def test_experts_without_bias_and_residual(ops, T, N, H, E, act, out):
+    """The same of experts: 33 to 159 rows each on average, where half tiles without rows are left out, and more."""
+    for dropped in (0, T // 7):
+        offsets = cuts(T, E, T + dropped, dropped)
+        _, y = run_case(ops, T, N, H, act, out, bias=False, residual=False, offsets=offsets, seed=E)
+        assert (y[int(offsets[-1]):] == 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("T,E", [(40, 5), (400, 9), (1200, 8), (4000, 6)])
 def test_experts_with_all_or_no_rows(ops, T, E):
     for filled in (0, E // 2, E - 1):
