@@ -16,10 +16,10 @@
 //
 // 8-bit integers (MoeLinearInt8, both operands by rows) run through the same loop with half the stages, so what a tile
 // takes beside them counts twice: its epilogue has a form without branches (int8_epilogue). T = 16381, H = 2048, N =
-// 2816 SwiGLU 162-172 us, 2200-2330 TOP/s with the epilogue; 8192^3 382 us, 2880 TOP/s (the library's product alone:
+// 2816 SwiGLU 162-179 us, 2110-2330 TOP/s with the epilogue; 8192^3 382 us, 2880 TOP/s (the library's product alone:
 // 2415). The products of experts (GROUPED): a tile's expert comes from the offsets, by scalar loads from the tile
-// before's on. 98304 rows by 64 experts, N = 2048, H = 1408: 302 us, 1880 TOP/s, of which 44 are the stores' and 8 % of
-// the tiles' rows are empty.
+// before's on. 98304 rows by 64 experts, N = 2048, H = 1408: 288-317 us, 1790-1970 TOP/s, of which 44 us are the
+// stores' and 8 % of the tiles' rows are empty.
 #include "moe_gemm.h"
 
 namespace moe {

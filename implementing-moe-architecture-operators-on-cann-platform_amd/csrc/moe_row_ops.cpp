@@ -278,8 +278,8 @@ moe_status moe_unpermute_grad(const void* grad_y, int64_t grad_y_stride, const v
 }
 
 size_t moe_unpermute_grad_any_workspace_bytes(int64_t T, int64_t K) {
-    if (check_rows("MoeUnpermuteGrad", T, 1, MOE_DT_FLOAT32) != MOE_OK || check_picks("MoeUnpermuteGrad", T, K) != MOE_OK)
-        return 0;
+    const char* op = "MoeUnpermuteGrad";
+    if (check_rows(op, T, 1, MOE_DT_FLOAT32) != MOE_OK || check_picks(op, T, K) != MOE_OK) return 0;
     return static_cast<size_t>(T) * K * 2 * sizeof(int32_t);
 }
 
