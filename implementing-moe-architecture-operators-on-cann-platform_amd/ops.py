@@ -739,8 +739,8 @@ def MoePermute(x: torch.Tensor, expert_ids: torch.Tensor, numExperts: int, xScal
     int32, row_scale): the rows of all picks sorted by expert, one expert's in the order of their slots. Expert e has
     rows [offsets[e], offsets[e+1]). Picks whose id is outside [0, E) come last, with rows of zeros. position is a
     pick's row, -1 - row of a pick of no expert. xScale[T] fp32 (8-bit rows' scales) is sorted alike, else row_scale is
-    None. The gradient of rows is MoeUnpermute(grad_rows, position). `workspace` (uint8, >= permute_workspace_bytes) is
-    allocated when not given."""
+    None. The gradient of rows is MoeUnpermute(grad_rows, position), of row_scale the same of its gradient as a column.
+    `workspace` (uint8, >= permute_workspace_bytes) is allocated when not given."""
     dt, dev = _first_float(x, "x", (*_FLOATS, torch.int8), 2)
     T, H = x.shape
     _, K = _ids(expert_ids, "expert_ids", T, dev)
